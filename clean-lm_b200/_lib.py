@@ -100,6 +100,12 @@ class CdlMxProduct(ctypes.Structure):
 CDL_MXFP8, CDL_NVFP4 = 0, 1
 CDL_MX_ROWWISE, CDL_MX_COLWISE = 0, 1
 
+
+class CdlHeadLossDesc(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("grad_scale", ctypes.c_float),
+                ("accumulate_dw", ctypes.c_int32), ("chunk_rows", ctypes.c_int64)]
+
+
 _BLOCK_PARAMS = ("norm1", "wqkv", "wo", "norm2", "wup", "wgate", "wdown")
 
 
@@ -129,6 +135,7 @@ _T = ctypes.POINTER(CdlTensor)
 _MX = ctypes.POINTER(CdlMxTensor)
 _MO = ctypes.POINTER(CdlMatmulOptions)
 _NO = ctypes.POINTER(CdlNormOptions)
+_HL = ctypes.POINTER(CdlHeadLossDesc)
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 
@@ -194,6 +201,10 @@ SIGNATURES = {
     "cdl_b200_swiglu_fwd": ([_T, _T, _T, _vp], ctypes.c_int32),
     "cdl_b200_swiglu_bwd": ([_T, _T, _T, _T, _T, _vp], ctypes.c_int32),
     "cdl_b200_cross_entropy": ([_T, _T, _T, ctypes.c_float, _vp], ctypes.c_int32),
+    "cdl_b200_distillation": ([_HL, _T, _T, _T, _T, _T, _T, _T, _vp], ctypes.c_int32),
+    "cdl_b200_linear_loss_scratch_bytes": ([_HL, _T, _T, ctypes.c_int64, _T, _T, ctypes.POINTER(_sz)], ctypes.c_int32),
+    "cdl_b200_linear_cross_entropy": ([_HL, _T, _T, _T, _T, _T, _T, _T, _T, _vp, _sz, _vp], ctypes.c_int32),
+    "cdl_b200_linear_distillation": ([_HL, _T, _T, _T, _T, _T, _T, _T, _T, _T, _vp, _sz, _vp], ctypes.c_int32),
     "cdl_b200_embedding_bwd": ([_T, _T, _T, _vp], ctypes.c_int32),
     "cdl_b200_sum": ([_vp, ctypes.c_int64, _vp, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _vp,
                       _sz, _vp], ctypes.c_int32),

@@ -1,0 +1,651 @@
+// Losses of a language-model head: softmax cross entropy and distillation from a teacher's top entries, from the logits or
+// from the hidden states and the head's weights without the logits in memory.
+//
+// Every loss here holds q = softmax(z / tau) of a row of logits against a distribution p that is zero but for a few
+// entries (one for a target, K for a teacher), so that the gradient of the logits is
+//     G_j = s tau (q_j - p_j),      s = grad_scale * d_loss[row]
+// (cross entropy: tau = 1, p = 1 at the target).  With t_j = z_j log2(e) / tau, M = max t, S = sum 2^(t_j - M):
+//     q_j = 2^(t_j - M) / S,   log q_j = ln 2 ((t_j - M) - log2 S),   lse = ln 2 (M + log2 S).
+// All statistics are f32.
+#include "host.h"
+#include "ops.h"
+#include "ptx.cuh"
+
+#include <math.h>
+
+namespace cdl {
+namespace head {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int MAX_ENTRIES = 1024;  // of a teacher, per row: they are kept in shared memory
+constexpr int ROW_THREADS = 512;
+
+// The distributions p of all rows: targets (one entry of probability 1), or a teacher's ids and logits.
+struct Entries {
+  const int* ids;       // targets, or ids [rows, K]
+  const void* teacher;  // logits [rows, K]
+  long long ids_ld, teacher_ld;
+  int K, kind;  // kind: what the teacher's logits are
+};
+enum EntryKind { TARGETS, TEACHER_BF16, TEACHER_F32 };
+
+__device__ __forceinline__ float teacher_logit(const Entries& e, long long row, int k) {
+  return e.kind == TEACHER_F32 ? static_cast<const float*>(e.teacher)[row * e.teacher_ld + k]
+                               : __bfloat162float(static_cast<const __nv_bfloat16*>(e.teacher)[row * e.teacher_ld + k]);
+}
+
+// What every row has besides its logits.
+struct RowTerms {
+  const float* d_loss;  // nullptr: 1
+  long long d_loss_stride;
+  float* loss;
+  float* lse;  // nullptr: not wanted
+  float grad_scale, tau;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// (M, S) of two parts of a row.  A part without finite logits has M = -inf and S = 0 (or NaN, which stays).
+__device__ __forceinline__ void join(float& m, float& s, float om, float os) {
+  const float nm = fmaxf(m, om);
+  const float base = nm == -INFINITY ? 0.f : nm;
+  s = s * ex2(m - base) + os * ex2(om - base);
+  m = nm;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// A row's entries in shared memory.
+struct RowEntries {
+  int id[MAX_ENTRIES];    // -1: does not count
+  float p[MAX_ENTRIES];
+  float at[MAX_ENTRIES];  // t of the row at the entry's id
+  float part[32];         // of a reduction over the CTA
+};
+
+__device__ __forceinline__ float cta_reduce(float v, bool max, float* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v = max ? warp_max(v) : warp_sum(v);
+  __syncthreads();  // (the last reduction's readers are through)
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  v = lane < warps ? part[lane] : (max ? -INFINITY : 0.f);
+  return max ? warp_max(v) : warp_sum(v);
+}
+
+// Loads the entries of a row by the whole CTA: ids, and p = softmax(teacher / tau) over those that count (id in [0, vocab),
+// logit above -inf).  Returns whether there are any, and sum p log p.
+__device__ __forceinline__ bool load_entries(RowEntries& e, const Entries& src, long long row, int vocab, float tau, float& p_log_p) {
+  p_log_p = 0.f;
+  if (src.kind == TARGETS) {
+    const int id = src.ids[row];
+    const bool counts = id >= 0 && id < vocab;
+    if (threadIdx.x == 0) {
+      e.id[0] = counts ? id : -1;
+      e.p[0] = counts ? 1.f : 0.f;
+    }
+    __syncthreads();
+    return counts;
+  }
+  const int* ids = src.ids + row * src.ids_ld;
+  const float c = LOG2E / tau;
+  float m = -INFINITY;
+  for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+    const int id = ids[k];
+    float y = -INFINITY;
+    if (id >= 0 && id < vocab)  // (padding may hold anything)
+      y = c * teacher_logit(src, row, k);
+    e.id[k] = y == -INFINITY ? -1 : id;
+    e.p[k] = y;
+    m = fmaxf(m, y != y ? INFINITY : y);  // a NaN makes the row NaN
+  }
+  m = cta_reduce(m, true, e.part);
+  if (m == -INFINITY) {
+    for (int k = threadIdx.x; k < src.K; k += blockDim.x) e.p[k] = 0.f;
+    __syncthreads();
+    return false;
+  }
+  float s = 0.f, sy = 0.f;
+  for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+    const float y = e.p[k] - m, x = e.id[k] < 0 ? 0.f : ex2(y);
+    e.p[k] = x;
+    s += x;
+    if (x != 0.f) sy += x * y;
+  }
+  s = cta_reduce(s, false, e.part);
+  sy = cta_reduce(sy, false, e.part);
+  for (int k = threadIdx.x; k < src.K; k += blockDim.x) e.p[k] /= s;
+  p_log_p = LN2 * (sy / s - log2f(s));
+  __syncthreads();
+  return true;
+}
+
+// One CTA per row: the row is read twice (the second time from the L2), any alignment.
+template <typename TIN, typename TOUT>
+__global__ void __launch_bounds__(ROW_THREADS)
+    loss_row_kernel(const TIN* z, long long ld_z, TOUT* g, long long ld_g, int vocab, const Entries src, const RowTerms terms) {
+  __shared__ RowEntries e;
+  const long long row = blockIdx.x;
+  const TIN* x = z + row * ld_z;
+  const float c = LOG2E / terms.tau;
+  float p_log_p;
+  const bool counts = load_entries(e, src, row, vocab, terms.tau, p_log_p);
+  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) e.at[k] = e.id[k] < 0 ? 0.f : c * to_f32(x[e.id[k]]);
+  float m = -INFINITY, s = 0.f;
+  bool bad = false;
+  for (int j = threadIdx.x; j < vocab; j += ROW_THREADS) {
+    const float t = c * to_f32(x[j]);
+    bad = bad || t != t;
+    if (t > m) {
+      s = s * ex2(m - t) + 1.f;
+      m = t;
+    } else if (t != -INFINITY) {
+      s += ex2(t - m);
+    }
+  }
+  const float top = cta_reduce(m, true, e.part);
+  const float base = top == -INFINITY ? 0.f : top;
+  s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(m - base)), false, e.part);
+  const float log2_s = log2f(s);
+  // sum_k p_k (log p_k - log q_k)
+  float cross = 0.f;
+  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
+    if (e.id[k] >= 0 && e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
+  cross = cta_reduce(cross, false, e.part);
+  if (threadIdx.x == 0) {
+    terms.loss[row] = counts ? terms.tau * terms.tau * (p_log_p - LN2 * cross) : 0.f;
+    if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+  }
+  if (g == nullptr) return;
+  TOUT* y = g + row * ld_g;
+  const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
+  const float over_s = scale / s;
+  __syncthreads();
+  for (int j = threadIdx.x; j < vocab; j += ROW_THREADS)
+    y[j] = from_f32<TOUT>(counts ? ex2(fmaf(to_f32(x[j]), c, -base)) * over_s : 0.f);
+  __syncthreads();
+  // The entries, each id once: the sum of its entries' probabilities, in their order.
+  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) {
+    const int id = e.id[k];
+    if (id < 0) continue;
+    bool first = true;
+    for (int i = 0; i < k; ++i) first = first && e.id[i] != id;
+    if (!first) continue;
+    float p = e.p[k];
+    for (int i = k + 1; i < src.K; ++i) p += e.id[i] == id ? e.p[i] : 0.f;
+    y[id] = from_f32<TOUT>(scale * (ex2(e.at[k] - base) / s - p));
+  }
+}
+
+// dst[r, c] = src[r, c] for any strides of the source, or 0 where keep[r] says that row r does not count; the threads run
+// along dst's columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    copy_kernel(const T* src, long long s_row, long long s_col, T* dst, long long ld, long long rows, int cols,
+                const float* keep) {
+  const long long per_row = (cols + 255) / 256;
+  for (long long b = blockIdx.x; b < rows * per_row; b += gridDim.x) {
+    const long long r = b / per_row;
+    const int c = static_cast<int>(b - r * per_row) * 256 + threadIdx.x;
+    if (c >= cols) continue;
+    dst[r * ld + c] = keep != nullptr && keep[r] == 0.f ? from_f32<T>(0.f) : src[r * s_row + c * s_col];
+  }
+}
+
+// out[r, c] = sum[r, c] (+ out[r, c]): the end of a gradient that is summed in f32 scratch; sum = nullptr: zeros.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    finish_kernel(const float* sum, long long ld, T* out, long long o_row, long long o_col, long long rows, int cols, int add) {
+  const long long per_row = (cols + 255) / 256;
+  for (long long b = blockIdx.x; b < rows * per_row; b += gridDim.x) {
+    const long long r = b / per_row;
+    const int c = static_cast<int>(b - r * per_row) * 256 + threadIdx.x;
+    if (c >= cols) continue;
+    float v = sum != nullptr ? sum[r * ld + c] : 0.f;
+    T* o = out + r * o_row + c * o_col;
+    if (add) v += to_f32(*o);
+    *o = from_f32<T>(v);
+  }
+}
+
+// 1 for a row that counts, 0 for one without a target or entries.
+__global__ void __launch_bounds__(256) keep_kernel(const Entries src, long long rows, int vocab, float* keep) {
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  bool any = false;
+  for (int k = threadIdx.x & 31; k < src.K; k += 32) {
+    const int id = src.ids[row * src.ids_ld + k];
+    if (id < 0 || id >= vocab) continue;
+    any = any || src.kind == TARGETS || teacher_logit(src, row, k) != -INFINITY;
+  }
+  any = __any_sync(0xffffffffu, any);
+  if ((threadIdx.x & 31) == 0) keep[row] = any ? 1.f : 0.f;
+}
+
+static Entries from_row(Entries e, long long row) {
+  e.ids += row * e.ids_ld;
+  if (e.kind != TARGETS) e.teacher = static_cast<const char*>(e.teacher) + row * e.teacher_ld * (e.kind == TEACHER_F32 ? 4 : 2);
+  return e;
+}
+static RowTerms from_row(RowTerms t, long long row) {
+  if (t.d_loss) t.d_loss += row * t.d_loss_stride;
+  t.loss += row;
+  if (t.lse) t.lse += row;
+  return t;
+}
+
+static int32_t launch_rows(const void* z, int32_t z_type, long long ld_z, void* g, int32_t g_type, long long ld_g, long long rows,
+                           int vocab, const Entries& e, const RowTerms& t, cudaStream_t stream) {
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (dtype_size(z_type) + (g ? dtype_size(g_type) : 0)), stream);
+  const unsigned grid = static_cast<unsigned>(rows);
+  using bf = __nv_bfloat16;
+  if (z_type == CDL_BF16)
+    loss_row_kernel<bf, bf><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const bf*>(z), ld_z, static_cast<bf*>(g), ld_g, vocab, e, t);
+  else if (g_type == CDL_BF16)
+    loss_row_kernel<float, bf><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const float*>(z), ld_z, static_cast<bf*>(g), ld_g, vocab, e, t);
+  else
+    loss_row_kernel<float, float><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const float*>(z), ld_z, static_cast<float*>(g), ld_g, vocab, e, t);
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+static unsigned copy_grid(long long rows, long long cols) {
+  const long long blocks = rows * ((cols + 255) / 256), most = 32LL * sm_count();
+  return static_cast<unsigned>(blocks < most ? blocks : most);
+}
+
+// dst [rows, cols] (ld) = src, of which the threads' direction is dimension 1.
+static int32_t copy(const cdl_tensor& src, void* dst, long long ld, const float* keep, cudaStream_t stream) {
+  const long long rows = src.shape[0], cols = src.shape[1];
+  if (src.dtype == CDL_BF16)
+    copy_kernel<__nv_bfloat16><<<copy_grid(rows, cols), 256, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(src.ptr), src.stride[0], src.stride[1], static_cast<__nv_bfloat16*>(dst), ld, rows,
+        static_cast<int>(cols), keep);
+  else
+    copy_kernel<float><<<copy_grid(rows, cols), 256, 0, stream>>>(static_cast<const float*>(src.ptr), src.stride[0], src.stride[1],
+                                                                static_cast<float*>(dst), ld, rows, static_cast<int>(cols), keep);
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+static int32_t finish(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
+  const long long rows = out.shape[0], cols = out.shape[1];
+  if (out.dtype == CDL_BF16)
+    finish_kernel<__nv_bfloat16><<<copy_grid(rows, cols), 256, 0, stream>>>(
+        sum, ld, static_cast<__nv_bfloat16*>(out.ptr), out.stride[0], out.stride[1], rows, static_cast<int>(cols), add);
+  else
+    finish_kernel<float><<<copy_grid(rows, cols), 256, 0, stream>>>(sum, ld, static_cast<float*>(out.ptr), out.stride[0],
+                                                                  out.stride[1], rows, static_cast<int>(cols), add);
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+// ------------------------------------------------------------------------------------------ checks
+static bool is_float(int32_t t) { return t == CDL_BF16 || t == CDL_F32; }
+
+static int32_t check_desc(const char* op, const cdl_head_loss_desc* d) {
+  if (!d) return fail(CDL_ERR_INVALID, "%s: desc is required", op);
+  if (!(d->temperature > 0.f) || isinf(d->temperature)) return fail(CDL_ERR_INVALID, "%s: temperature must be positive and finite", op);
+  if (d->chunk_rows < 0) return fail(CDL_ERR_INVALID, "%s: chunk_rows must not be negative", op);
+  return CDL_OK;
+}
+
+static int32_t check_row_values(const char* op, const char* name, const cdl_tensor* t, long long rows, int32_t type, bool packed) {
+  if (t->rank != 1 || t->dtype != type || t->shape[0] != rows || (packed && rows > 1 && t->stride[0] != 1))
+    return fail(CDL_ERR_INVALID, "%s: %s must be %s%s [tokens]", op, name, packed ? "packed " : "", dtype_name(type));
+  return CDL_OK;
+}
+
+static int32_t check_terms(const char* op, const cdl_head_loss_desc* desc, long long rows, const cdl_tensor* d_loss,
+                           const cdl_tensor* loss, const cdl_tensor* lse, RowTerms* out) {
+  if (!loss) return fail(CDL_ERR_INVALID, "%s: loss is required", op);
+  CDL_CHECK(check_row_values(op, "loss", loss, rows, CDL_F32, true));
+  if (lse) CDL_CHECK(check_row_values(op, "lse", lse, rows, CDL_F32, true));
+  if (d_loss) CDL_CHECK(check_row_values(op, "d_loss", d_loss, rows, CDL_F32, false));
+  *out = {d_loss ? static_cast<const float*>(d_loss->ptr) : nullptr, d_loss ? (long long)d_loss->stride[0] : 0,
+          static_cast<float*>(loss->ptr), lse ? static_cast<float*>(lse->ptr) : nullptr, desc->grad_scale, desc->temperature};
+  return CDL_OK;
+}
+
+static int32_t check_targets(const char* op, long long rows, const cdl_tensor* targets, Entries* out) {
+  if (!targets) return fail(CDL_ERR_INVALID, "%s: targets are required", op);
+  CDL_CHECK(check_row_values(op, "targets", targets, rows, CDL_I32, true));
+  *out = {static_cast<const int*>(targets->ptr), nullptr, 1, 0, 1, TARGETS};
+  return CDL_OK;
+}
+
+static int32_t check_teacher(const char* op, long long rows, const cdl_tensor* ids, const cdl_tensor* teacher, Entries* out) {
+  if (!ids || !teacher) return fail(CDL_ERR_INVALID, "%s: teacher_ids and teacher_logits are required", op);
+  const long long K = ids->rank == 2 ? ids->shape[1] : -1;
+  if (ids->rank != 2 || ids->dtype != CDL_I32 || ids->shape[0] != rows || (K > 1 && ids->stride[1] != 1))
+    return fail(CDL_ERR_INVALID, "%s: teacher_ids must be i32 [tokens, entries] with contiguous rows", op);
+  if (teacher->rank != 2 || !is_float(teacher->dtype) || teacher->shape[0] != rows || teacher->shape[1] != K ||
+      (K > 1 && teacher->stride[1] != 1))
+    return fail(CDL_ERR_INVALID, "%s: teacher_logits must be bf16 or f32 [tokens, entries] like teacher_ids, with contiguous rows", op);
+  if (K > MAX_ENTRIES) return fail(CDL_ERR_UNSUPPORTED, "%s: at most %d entries per token (got %lld)", op, MAX_ENTRIES, K);
+  *out = {static_cast<const int*>(ids->ptr), teacher->ptr, ids->stride[0], teacher->stride[0], static_cast<int>(K),
+          teacher->dtype == CDL_F32 ? TEACHER_F32 : TEACHER_BF16};
+  return CDL_OK;
+}
+
+// ------------------------------------------------------------------------------------------ from the logits
+static int32_t distillation_execute(const cdl_head_loss_desc* desc, const cdl_tensor* logits, const cdl_tensor* ids,
+                                    const cdl_tensor* teacher, const cdl_tensor* d_loss, const cdl_tensor* loss,
+                                    const cdl_tensor* lse, const cdl_tensor* d_logits, cudaStream_t stream) {
+  const char* op = "distillation";
+  CDL_CHECK(check_desc(op, desc));
+  if (!logits || logits->rank != 2 || !is_float(logits->dtype))
+    return fail(CDL_ERR_INVALID, "%s: logits must be bf16 or f32 [tokens, vocab]", op);
+  const long long T = logits->shape[0], V = logits->shape[1];
+  if (V > 1 && logits->stride[1] != 1) return fail(CDL_ERR_INVALID, "%s: logits must have contiguous rows", op);
+  if (T > INT32_MAX || V > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  RowTerms terms;
+  Entries e;
+  CDL_CHECK(check_teacher(op, T, ids, teacher, &e));
+  CDL_CHECK(check_terms(op, desc, T, d_loss, loss, lse, &terms));
+  if (d_logits) {
+    if (d_logits->rank != 2 || d_logits->dtype != logits->dtype || d_logits->shape[0] != T || d_logits->shape[1] != V ||
+        (V > 1 && d_logits->stride[1] != 1))
+      return fail(CDL_ERR_INVALID, "%s: d_logits must have the logits' type and shape and contiguous rows", op);
+    if (T > 1 && d_logits->stride[0] < V) return fail(CDL_ERR_INVALID, "%s: rows of d_logits overlap", op);
+    if (d_logits->ptr == logits->ptr && T > 1 && d_logits->stride[0] != logits->stride[0])
+      return fail(CDL_ERR_INVALID, "%s: d_logits must be the logits themselves or lie elsewhere", op);
+  }
+  if (T == 0) return CDL_OK;
+  if (V == 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
+  return launch_rows(logits->ptr, logits->dtype, logits->stride[0], d_logits ? d_logits->ptr : nullptr, logits->dtype,
+                     d_logits ? d_logits->stride[0] : 0, T, static_cast<int>(V), e, terms, stream);
+}
+
+// ------------------------------------------------------------------------------------------ from the hidden states
+static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
+
+// Where a product's operand is read: its own place, or scratch that it is copied to (bf16: rows on the 16-byte grid).
+static bool readable(const cdl_tensor& t) {
+  const long long r = t.shape[0], c = t.shape[1], sr = t.stride[0], sc = t.stride[1];
+  if (t.dtype == CDL_F32) return sc == 1 || c == 1 || sr == 1 || r == 1;
+  if (reinterpret_cast<uintptr_t>(t.ptr) & 15) return false;
+  return ((sc == 1 || c == 1) && (r == 1 || (sr % 8 == 0 && sr >= c))) || ((sr == 1 || r == 1) && (c == 1 || (sc % 8 == 0 && sc >= r)));
+}
+static bool columns_first(const cdl_tensor& t) { return t.stride[0] < t.stride[1]; }  // dimension 0 is the nearer one in memory
+
+struct Linear {
+  const char* op;
+  cdl_tensor x, w, dx, dw;  // dx, dw: ptr = nullptr where not wanted
+  bool has_dx, has_dw;
+  long long T, D, V;
+  // scratch
+  long long chunk;
+  bool copy_x, copy_w, sums;  // sums: dw is summed in f32 scratch and written at the end
+  long long ld_z, ld_g, ld_sum;
+  size_t at_x, at_w, at_z, at_g, at_clean, at_keep, at_sum, at_products, bytes;
+  size_t products_bytes;
+};
+
+// A view of `rows` rows from `row`.
+static cdl_tensor rows_of(const cdl_tensor& t, long long row, long long rows) {
+  cdl_tensor o = t;
+  o.ptr = static_cast<char*>(t.ptr) + row * t.stride[0] * static_cast<long long>(dtype_size(t.dtype));
+  o.shape[0] = rows;
+  return o;
+}
+
+static cdl_tensor strided2(void* p, int32_t dt, long long r, long long c, long long ld) {
+  cdl_tensor t = view2(p, dt, r, c);
+  t.stride[0] = ld;
+  return t;
+}
+
+// Rows that are taken at a time: their logits (and the gradients of those) are what the scratch holds.
+static long long choose_chunk(long long T, long long V, size_t bytes_per_logit) {
+  const long long most = (512LL << 20) / static_cast<long long>(bytes_per_logit * V);
+  long long rows = most < 256 ? 256 : most;
+  if (rows >= T) return T;
+  const long long chunks = (T + rows - 1) / rows;
+  return up((T + chunks - 1) / chunks, 256);
+}
+
+static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc) {
+  const bool grad = p.has_dx || p.has_dw;
+  const int32_t type = p.x.dtype;
+  const size_t es = dtype_size(type);
+  p.copy_x = !readable(p.x) || (type == CDL_BF16 && p.T > 1 && p.x.stride[0] < p.D);  // (chunks of rows start on the grid)
+  p.copy_w = !readable(p.w);
+  p.chunk = desc->chunk_rows > 0 ? (desc->chunk_rows < p.T ? desc->chunk_rows : p.T) : choose_chunk(p.T, p.V, 4);
+  const bool whole = p.chunk >= p.T;
+  const bool dw_rows = p.has_dw && (p.dw.stride[1] == 1 || p.dw.stride[0] == 1);
+  p.sums = p.has_dw && (!dw_rows || (p.dw.dtype == CDL_BF16 && !whole));
+  p.ld_z = up(p.V, 64);
+  p.ld_g = up(p.V, 64);
+  p.ld_sum = p.has_dw ? up(columns_first(p.dw) ? p.D : p.V, 64) : 0;
+  size_t at = 0;
+  auto take = [&](bool want, size_t bytes) {
+    const size_t here = at;
+    if (want) at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const long long x_ld = up(p.D, 8);
+  p.at_x = take(p.copy_x, static_cast<size_t>(p.T) * x_ld * es);
+  const bool wc = columns_first(p.w);
+  p.at_w = take(p.copy_w, static_cast<size_t>(wc ? p.V : p.D) * up(wc ? p.D : p.V, 8) * es);
+  p.at_z = take(true, static_cast<size_t>(p.chunk) * p.ld_z * 4);
+  p.at_g = take(grad && type == CDL_BF16, static_cast<size_t>(p.chunk) * p.ld_g * 2);
+  if (type == CDL_F32) p.at_g = p.at_z;  // in place
+  p.at_clean = take(p.has_dw, static_cast<size_t>(p.chunk) * x_ld * es);
+  p.at_keep = take(p.has_dw, static_cast<size_t>(p.chunk) * 4);
+  p.at_sum = take(p.sums, static_cast<size_t>(columns_first(p.dw) ? p.V : p.D) * p.ld_sum * 4);
+  p.products_bytes = 0;
+  if (type == CDL_F32) {  // (bf16 operands are on the grid by now)
+    auto need = [&](const cdl_tensor& a, const cdl_tensor& b, const cdl_tensor& d) {
+      const size_t n = matmul_general_scratch_bytes(&a, &b, &d);
+      if (n > p.products_bytes) p.products_bytes = n;
+    };
+    alignas(256) static float nowhere[64];
+    const cdl_tensor z = strided2(nowhere, CDL_F32, p.chunk, p.V, p.ld_z);
+    const cdl_tensor x = p.copy_x ? strided2(nowhere, type, p.chunk, p.D, x_ld) : rows_of(p.x, 0, p.chunk);
+    need(x, p.w, z);
+    if (p.has_dx) need(z, transposed(p.w), strided2(nowhere, type, p.chunk, p.D, p.D));
+    if (p.has_dw) {
+      const cdl_tensor clean = strided2(nowhere, type, p.chunk, p.D, x_ld);
+      if (columns_first(p.dw)) need(transposed(z), clean, strided2(nowhere, CDL_F32, p.V, p.D, up(p.D, 4)));
+      else need(transposed(clean), z, strided2(nowhere, CDL_F32, p.D, p.V, p.ld_z));
+    }
+  }
+  p.at_products = take(p.products_bytes != 0, p.products_bytes);
+  p.bytes = at;
+  return CDL_OK;
+}
+
+static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                            const cdl_tensor* dx, const cdl_tensor* dw, Linear* out) {
+  CDL_CHECK(check_desc(op, desc));
+  if (!x || !w || x->rank != 2 || w->rank != 2 || !is_float(x->dtype) || x->dtype != w->dtype)
+    return fail(CDL_ERR_INVALID, "%s: x must be bf16 or f32 [tokens, hidden], w of the same type [hidden, vocab]", op);
+  Linear& p = *out;
+  p = Linear{};
+  p.op = op;
+  p.x = *x;
+  p.w = *w;
+  p.T = x->shape[0];
+  p.D = x->shape[1];
+  p.V = w->shape[1];
+  p.has_dx = dx != nullptr;
+  p.has_dw = dw != nullptr;
+  if (w->shape[0] != p.D)
+    return fail(CDL_ERR_INVALID, "%s: x is [tokens, %lld], w is [%lld, vocab]: the hidden sizes differ", op, p.D, (long long)w->shape[0]);
+  if (p.T > INT32_MAX || p.D > INT32_MAX || p.V > INT32_MAX - 64) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  if (dx) {
+    if (dx->rank != 2 || dx->dtype != x->dtype || dx->shape[0] != p.T || dx->shape[1] != p.D || (p.D > 1 && dx->stride[1] != 1) ||
+        (p.T > 1 && dx->stride[0] < p.D))
+      return fail(CDL_ERR_INVALID, "%s: dx must have x's type and shape and contiguous rows that do not overlap", op);
+    p.dx = *dx;
+  }
+  if (dw) {
+    const long long a = dw->rank == 2 ? dw->stride[0] : 0, b = dw->rank == 2 ? dw->stride[1] : 0;
+    if (dw->rank != 2 || !(dw->dtype == CDL_F32 || dw->dtype == x->dtype) || dw->shape[0] != p.D || dw->shape[1] != p.V)
+      return fail(CDL_ERR_INVALID, "%s: dw must be [hidden, vocab] in f32 or x's type", op);
+    const bool apart = p.D == 0 || p.V == 0 ? true : a <= 0 || b <= 0 ? (p.D <= 1 || a > 0) && (p.V <= 1 || b > 0)
+                                        : a < b ? (p.V <= 1 || b >= (p.D - 1) * a + 1) : (p.D <= 1 || a >= (p.V - 1) * b + 1);
+    if (!apart) return fail(CDL_ERR_INVALID, "%s: elements of dw overlap", op);
+    p.dw = *dw;
+  }
+  if (p.V == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
+  if (p.D == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: hidden is zero", op);
+  return plan_linear(p, desc);
+}
+
+static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& entries, const RowTerms& terms, void* scratch,
+                              size_t scratch_bytes, cudaStream_t stream) {
+  const bool grad = p.has_dx || p.has_dw;
+  if (p.T == 0) {  // no rows: no loss, and a gradient of zeros
+    if (p.has_dw && !desc->accumulate_dw && p.D > 0 && p.V > 0) CDL_CHECK(finish(nullptr, 0, p.dw, 0, stream));
+    return CDL_OK;
+  }
+  if (p.bytes > 0 && (!scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(scratch) & 255)))
+    return fail(CDL_ERR_INVALID, "%s: scratch must hold %zu bytes, 256-byte aligned", p.op, p.bytes);
+  char* base = static_cast<char*>(scratch);
+  const int32_t type = p.x.dtype;
+  const long long x_ld = up(p.D, 8);
+  cdl_tensor x = p.x, w = p.w;
+  if (p.copy_x) {
+    CDL_CHECK(copy(p.x, base + p.at_x, x_ld, nullptr, stream));
+    x = strided2(base + p.at_x, type, p.T, p.D, x_ld);
+  }
+  if (p.copy_w) {
+    if (columns_first(p.w)) {
+      const long long ld = up(p.D, 8);
+      CDL_CHECK(copy(transposed(p.w), base + p.at_w, ld, nullptr, stream));
+      w = transposed(strided2(base + p.at_w, type, p.V, p.D, ld));
+    } else {
+      const long long ld = up(p.V, 8);
+      CDL_CHECK(copy(p.w, base + p.at_w, ld, nullptr, stream));
+      w = strided2(base + p.at_w, type, p.D, p.V, ld);
+    }
+  }
+  const cdl_tensor wt = transposed(w);
+  void* products = p.products_bytes ? base + p.at_products : nullptr;
+  // Sums over the rows in a fixed order: the same gradient every time.
+  cdl_matmul_options fixed = {CDL_GEMM_AUTO, 1};
+  const bool dw_columns = p.has_dw && columns_first(p.dw);
+  cdl_tensor sum = p.dw;
+  if (p.sums)
+    sum = dw_columns ? transposed(strided2(base + p.at_sum, CDL_F32, p.V, p.D, p.ld_sum))
+                     : strided2(base + p.at_sum, CDL_F32, p.D, p.V, p.ld_sum);
+  for (long long row = 0; row < p.T; row += p.chunk) {
+    const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
+    const cdl_tensor xc = rows_of(x, row, n);
+    const cdl_tensor z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_z);
+    const Entries e = from_row(entries, row);
+    CDL_CHECK(matmul_execute(&xc, &w, nullptr, &z, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
+    const cdl_tensor g = strided2(base + p.at_g, type, n, p.V, p.ld_g);
+    CDL_CHECK(launch_rows(z.ptr, CDL_F32, p.ld_z, grad ? g.ptr : nullptr, type, p.ld_g, n, static_cast<int>(p.V), e, from_row(terms, row), stream));
+    if (p.has_dw) {
+      // A row that does not count adds nothing whatever it holds, infinities and NaN too: its gradient's zeros alone
+      // would not do that.  (Copied before dx is written, which may be x itself.)
+      float* keep = reinterpret_cast<float*>(base + p.at_keep);
+      keep_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(e, n, static_cast<int>(p.V), keep);
+      CDL_CUDA(cudaGetLastError());
+      CDL_CHECK(copy(xc, base + p.at_clean, x_ld, keep, stream));
+    }
+    if (p.has_dx) {
+      const cdl_tensor d = rows_of(p.dx, row, n);
+      CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
+    }
+    if (p.has_dw) {
+      const cdl_tensor clean = strided2(base + p.at_clean, type, n, p.D, x_ld);
+      const bool add = row > 0 || (!p.sums && desc->accumulate_dw);
+      const cdl_tensor gt = transposed(g), xt = transposed(clean), sum_t = transposed(sum);
+      const cdl_tensor *a = dw_columns ? &gt : &xt, *b = dw_columns ? &clean : &g, *d = dw_columns ? &sum_t : &sum;
+      CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes));
+    }
+  }
+  if (p.sums) {
+    if (dw_columns) CDL_CHECK(finish(static_cast<float*>(sum.ptr), p.ld_sum, transposed(p.dw), desc->accumulate_dw, stream));
+    else CDL_CHECK(finish(static_cast<float*>(sum.ptr), p.ld_sum, p.dw, desc->accumulate_dw, stream));
+  }
+  return CDL_OK;
+}
+
+}  // namespace head
+}  // namespace cdl
+
+extern "C" {
+
+int32_t cdl_b200_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* logits, const cdl_tensor* teacher_ids,
+                              const cdl_tensor* teacher_logits, const cdl_tensor* d_loss, const cdl_tensor* loss,
+                              const cdl_tensor* lse, const cdl_tensor* d_logits, cdl_stream stream) {
+  return cdl::head::distillation_execute(desc, logits, teacher_ids, teacher_logits, d_loss, loss, lse, d_logits,
+                                         static_cast<cudaStream_t>(stream));
+}
+
+int32_t cdl_b200_linear_loss_scratch_bytes(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                           int64_t entries, const cdl_tensor* dx, const cdl_tensor* dw, size_t* bytes_out) {
+  using namespace cdl;
+  if (!bytes_out) return fail(CDL_ERR_INVALID, "linear_loss_scratch_bytes: bytes_out is required");
+  *bytes_out = 0;
+  if (entries < 0) return fail(CDL_ERR_INVALID, "linear_loss_scratch_bytes: entries must not be negative");
+  head::Linear p;
+  CDL_CHECK(head::check_linear("linear_loss_scratch_bytes", desc, x, w, dx, dw, &p));
+  if (p.T > 0) *bytes_out = p.bytes;
+  return CDL_OK;
+}
+
+int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                      const cdl_tensor* targets, const cdl_tensor* d_loss, const cdl_tensor* loss,
+                                      const cdl_tensor* lse, const cdl_tensor* dx, const cdl_tensor* dw, void* scratch,
+                                      size_t scratch_bytes, cdl_stream stream) {
+  using namespace cdl;
+  const char* op = "linear_cross_entropy";
+  head::Linear p;
+  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, &p));
+  if (desc->temperature != 1.f) return fail(CDL_ERR_UNSUPPORTED, "%s: temperature must be 1", op);
+  head::Entries e;
+  head::RowTerms terms;
+  CDL_CHECK(head::check_targets(op, p.T, targets, &e));
+  CDL_CHECK(head::check_terms(op, desc, p.T, d_loss, loss, lse, &terms));
+  return head::linear_execute(p, desc, e, terms, scratch, scratch_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int32_t cdl_b200_linear_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                     const cdl_tensor* teacher_ids, const cdl_tensor* teacher_logits, const cdl_tensor* d_loss,
+                                     const cdl_tensor* loss, const cdl_tensor* lse, const cdl_tensor* dx, const cdl_tensor* dw,
+                                     void* scratch, size_t scratch_bytes, cdl_stream stream) {
+  using namespace cdl;
+  const char* op = "linear_distillation";
+  head::Linear p;
+  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, &p));
+  head::Entries e;
+  head::RowTerms terms;
+  CDL_CHECK(head::check_teacher(op, p.T, teacher_ids, teacher_logits, &e));
+  CDL_CHECK(head::check_terms(op, desc, p.T, d_loss, loss, lse, &terms));
+  return head::linear_execute(p, desc, e, terms, scratch, scratch_bytes, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

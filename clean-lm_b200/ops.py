@@ -295,3 +295,128 @@ def attention_bwd(q, k, v, out, d_out, lse, opts: AttentionOpts | None = None, s
     check(fn(ctypes.byref(desc), *(ref(a) for a in args), ctypes.c_void_p(scratch.data_ptr()),
              scratch.numel() * scratch.element_size(), current_stream()))
     return dq, dk, dv
+
+
+# --------------------------------------------------------------------------- losses of the head
+@dataclass
+class LinearLossOpts:
+    """Options of `linear_cross_entropy` and `linear_distillation`."""
+
+    temperature: float = 1.0  # of teacher and student (distillation)
+    grad_scale: float = 1.0  # of every gradient, e.g. 1 / tokens of the step
+    d_loss: Optional[torch.Tensor] = None  # f32 [tokens]: gradient of each token's loss, any stride; None is 1
+    grad: bool = True  # False: the loss alone
+    grad_x: bool = True
+    grad_w: bool = True
+    accumulate: bool = False  # add to the `dw` that is passed in place of writing it
+    chunk_rows: int = 0  # tokens whose rows the scratch holds at a time; 0: the library's choice
+
+
+@dataclass
+class LinearLossOutputs:
+    loss: torch.Tensor  # f32 [tokens]
+    lse: torch.Tensor  # f32 [tokens]: logsumexp of the logits over the temperature, natural log
+    dx: Optional[torch.Tensor]
+    dw: Optional[torch.Tensor]
+
+
+def _require_current_device(*tensors):
+    """The kernels run on the current device's current stream: operands of another one are refused."""
+    _require_cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise _lib.CdlError(-1, f"operands must live on the current device (cuda:{here}, got {t.device})")
+
+
+def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
+    if x.dim() != 2 or w.dim() != 2:
+        raise _lib.CdlError(-1, f"{name}: x must be [tokens, hidden] and w [hidden, vocab]")
+    _require_current_device(x, w, *entries, opts.d_loss, dx, dw, scratch)
+    if opts.accumulate and dw is None:
+        raise _lib.CdlError(-1, f"{name}: accumulate needs the dw that is added to")
+    want_x, want_w = opts.grad and (opts.grad_x or dx is not None), opts.grad and (opts.grad_w or dw is not None)
+    tokens = x.shape[0]
+    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=x.device)
+    if not want_x:
+        dx = None
+    elif dx is None:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not want_w:
+        dw = None
+    elif dw is None:  # laid out as w is
+        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w.stride(0) >= w.stride(1) else \
+            torch.empty(w.shape[::-1], dtype=w.dtype, device=w.device).t()
+    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
+    tx, tw, tl, ts, tdl, tdx, tdw = (tensor_bytes(t) for t in (x, w, loss, lse, opts.d_loss, dx, dw))
+    te = [tensor_bytes(t) for t in entries]
+    n = ctypes.c_size_t(0)
+    check(packed_lib.cdl_b200_linear_loss_scratch_bytes(ctypes.byref(desc), tx, tw, entries[0].shape[-1] if len(entries) > 1 else 1,
+                                                        tdx, tdw, ctypes.byref(n)))
+    if scratch is None:
+        scratch = torch.empty(max(n.value, 256), dtype=torch.uint8, device=x.device)
+    fn = packed_lib.cdl_b200_linear_distillation if len(entries) > 1 else packed_lib.cdl_b200_linear_cross_entropy
+    check(fn(ctypes.byref(desc), tx, tw, *te, tdl, tl, ts, tdx, tdw, scratch.data_ptr(),
+             scratch.numel() * scratch.element_size(), current_stream()))
+    return LinearLossOutputs(loss, lse, dx, dw)
+
+
+def linear_loss_scratch_bytes(x, w, opts: LinearLossOpts | None = None, entries: int = 1, dx=None, dw=None) -> int:
+    """The scratch that the call below needs for these operands; dx, dw: the gradients' tensors, None where not wanted."""
+    opts = opts or LinearLossOpts()
+    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
+    n = ctypes.c_size_t(0)
+    check(packed_lib.cdl_b200_linear_loss_scratch_bytes(ctypes.byref(desc), tensor_bytes(x), tensor_bytes(w), entries,
+                                                        tensor_bytes(dx), tensor_bytes(dw), ctypes.byref(n)))
+    return n.value
+
+
+def linear_cross_entropy(x, w, targets, opts: LinearLossOpts | None = None, dx=None, dw=None, scratch=None) -> LinearLossOutputs:
+    """Softmax cross entropy of the logits x w against `targets` (i32 [tokens]; outside [0, vocab): ignored), and its
+    gradients, without the logits in memory.
+
+    x [tokens, hidden], w [hidden, vocab] (a transposed view of a tied embedding table too), bf16 or f32, any strides.
+    dx comes in x's type; dw in w's type and layout, or in the tensor passed, f32 or w's type, which `opts.accumulate`
+    adds to."""
+    return _linear_loss("linear_cross_entropy", x, w, (targets,), opts or LinearLossOpts(), dx, dw, scratch)
+
+
+def linear_distillation(x, w, teacher_ids, teacher_logits, opts: LinearLossOpts | None = None, dx=None, dw=None,
+                        scratch=None) -> LinearLossOutputs:
+    """`distillation` of the logits x w, with the gradients of x and w; operands as for `linear_cross_entropy`."""
+    return _linear_loss("linear_distillation", x, w, (teacher_ids, teacher_logits), opts or LinearLossOpts(), dx, dw, scratch)
+
+
+@dataclass
+class DistillationOpts:
+    temperature: float = 1.0  # of teacher and student
+    grad_scale: float = 1.0
+    d_loss: Optional[torch.Tensor] = None  # f32 [tokens], any stride; None is 1
+    grad: bool = True  # False: the loss alone
+
+
+@dataclass
+class DistillationOutputs:
+    loss: torch.Tensor  # f32 [tokens]
+    lse: torch.Tensor  # f32 [tokens]: logsumexp of the logits over the temperature, natural log
+    d_logits: Optional[torch.Tensor]
+
+
+def distillation(logits, teacher_ids, teacher_logits, opts: DistillationOpts | None = None,
+                 d_logits=None) -> DistillationOutputs:
+    """temperature^2 KL(p || softmax(logits / temperature)) of every row against a teacher's top entries: p is the
+    softmax of teacher_logits / temperature over the row's entries, teacher_ids (i32) their ids (outside [0, vocab): padding).
+    With the gradient of the logits in `d_logits`, which may be the logits themselves."""
+    opts = opts or DistillationOpts()
+    if logits.dim() != 2:
+        raise _lib.CdlError(-1, "distillation: logits must be [tokens, vocab]")
+    _require_current_device(logits, teacher_ids, teacher_logits, opts.d_loss, d_logits)
+    loss, lse = torch.empty(2, logits.shape[0], dtype=torch.float32, device=logits.device)
+    if not opts.grad:
+        d_logits = None
+    elif d_logits is None:
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 0, 0)
+    check(packed_lib.cdl_b200_distillation(ctypes.byref(desc), *(tensor_bytes(t) for t in (
+        logits, teacher_ids, teacher_logits, opts.d_loss, loss, lse, d_logits)), current_stream()))
+    return DistillationOutputs(loss, lse, d_logits)

@@ -491,6 +491,59 @@ typedef struct {
 int32_t cdl_b200_adamw(float* master, void* replica_bf16, float* grad, float* m, float* v, int64_t n,
                        const float* grad_sumsq, const cdl_adamw_params* hp, cdl_stream stream);
 
+/* ---- Losses of the head against a target or a teacher, with and without the logits in memory -----------
+ * Softmax cross entropy straight from the hidden states and the head's weights, and distillation from a teacher's
+ * top entries, which trains on a few of the teacher's logits per token in place of a target.  (The reference's training
+ * step has the cross entropy of stored logits alone, crates/sky-1/src/training/model/mod.rs:262-271.)
+ *
+ * With z the logits [tokens, vocab] of a row, q = softmax(z / temperature), lse = log sum_j exp(z_j / temperature)
+ * and s = grad_scale * d_loss[row]:
+ *   cross entropy  loss = lse - z[target]                                d z_j = s (q_j - [j = target])
+ *   distillation   p = softmax(teacher_logits / temperature) over the row's entries
+ *                  loss = temperature^2 sum_k p_k (log p_k - log q[id_k])
+ *                  d z_j = s temperature (q_j - sum over k with id_k = j of p_k)
+ * A target or a teacher's id outside [0, vocab) does not count, nor does an entry whose logit is -inf; what else the row
+ * holds there may be anything.  A row in which nothing counts has loss 0 and adds nothing to any gradient, whatever x,
+ * d_loss and the row's logits hold.  An id may occur more than once in a row: its entries' probabilities add up.  Logits
+ * of -inf (masked vocabulary) have probability 0; a NaN or +inf among a row's logits, or -inf in all of them, makes the row's
+ * results NaN (lse: -inf in the last case).  All statistics, and the sums over tokens, are f32; results do not depend on
+ * timing.
+ *
+ * Operands: targets packed i32 [tokens]; teacher_ids i32 and teacher_logits bf16 or f32 [tokens, entries], contiguous
+ * rows, at most 1024 entries; d_loss f32 [tokens] of any stride, 0 too (nullable: 1); loss and lse (nullable) packed f32
+ * [tokens]. */
+typedef struct {
+  float temperature; /* > 0; 1 for the cross entropy */
+  float grad_scale;  /* of every gradient, e.g. 1 / tokens of the step */
+  int32_t accumulate_dw; /* != 0: dw is added to, else written */
+  int64_t chunk_rows;    /* tokens whose rows the scratch holds at a time; 0 = the library's choice */
+} cdl_head_loss_desc;
+
+/* Distillation from logits bf16 or f32 [tokens, vocab] with contiguous rows.  d_logits (nullable: the loss alone) has their
+ * type; it may be the logits themselves. */
+int32_t cdl_b200_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* logits, const cdl_tensor* teacher_ids,
+                              const cdl_tensor* teacher_logits, const cdl_tensor* d_loss, const cdl_tensor* loss,
+                              const cdl_tensor* lse, const cdl_tensor* d_logits, cdl_stream stream);
+/* The losses of z = x . w, x [tokens, hidden] and w [hidden, vocab] both bf16 or both f32, of any strides (w may be the
+ * transposed view of a [vocab, hidden] embedding table; operands whose rows are off the 16-byte grid are copied first).
+ * The logits are not kept: the scratch holds chunk_rows tokens' worth at a time, however many tokens there are.
+ *   dx  (nullable) x's type [tokens, hidden], contiguous rows:  d z . w^T; may be x itself
+ *   dw  (nullable) f32 or x's type [hidden, vocab], any strides:  x^T . d z, added to with accumulate_dw.  Held in f32 over
+ *       all tokens and rounded once.
+ * For bf16 operands d z is rounded to bf16 before both products, as cdl_b200_cross_entropy rounds it: an f32 dw has that
+ * accuracy then.  f32 operands keep it in f32.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that
+ * the call below gives for the same operands (entries: teacher_ids' second dimension, 1 for targets). */
+int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                      const cdl_tensor* targets, const cdl_tensor* d_loss, const cdl_tensor* loss,
+                                      const cdl_tensor* lse, const cdl_tensor* dx, const cdl_tensor* dw, void* scratch,
+                                      size_t scratch_bytes, cdl_stream stream);
+int32_t cdl_b200_linear_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                     const cdl_tensor* teacher_ids, const cdl_tensor* teacher_logits, const cdl_tensor* d_loss,
+                                     const cdl_tensor* loss, const cdl_tensor* lse, const cdl_tensor* dx, const cdl_tensor* dw,
+                                     void* scratch, size_t scratch_bytes, cdl_stream stream);
+int32_t cdl_b200_linear_loss_scratch_bytes(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
+                                           int64_t entries, const cdl_tensor* dx, const cdl_tensor* dw, size_t* bytes_out);
+
 /* ---- sky-1 decoder block ---------------------------------------------------------------
  * One call per direction for the dataflow of DecoderExecutor::train_forward / train_backward
  * (crates/sky-1/src/training/model/decoder.rs:332-520, 523-695): pre-RMSNorm, fused QKV
