@@ -22,6 +22,7 @@
 #include "ops.h"
 #include "ptx.cuh"
 
+#include <cuda_fp16.h>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -504,6 +505,97 @@ __device__ __forceinline__ void add_tile_rows(const Params& p, const CUtensorMap
   }
 }
 
+// One of 32 registers, by a tree of selections.
+__device__ __forceinline__ uint32_t pick32(const uint32_t (&r)[32], int i) {
+  uint32_t a[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a[j] = i & 16 ? r[16 + j] : r[j];
+#pragma unroll
+  for (int n = 8; n > 0; n >>= 1)
+#pragma unroll
+    for (int j = 0; j < n; ++j) a[j] = i & n ? a[n + j] : a[j];
+  return a[0];
+}
+
+// What a thread's row wants of a piece besides its statistics: its ids from `e` to `end`, the next of which is `id`.
+struct Wanted {
+  int e, end, id;
+  __device__ __forceinline__ void load(const Params& p, int row, int col_base) {
+    e = end = 0;
+    id = -1;
+    if (row >= p.M || col_base >= p.N || p.exp.ids == nullptr) return;
+    if (p.exp.first == nullptr) {
+      end = 1;
+    } else {
+      const unsigned short* f = p.exp.first + static_cast<long long>(row) * (p.exp.pieces + 1) + (col_base >> 7);
+      e = f[0];
+      end = f[1];
+    }
+    if (e < end) id = p.exp.ids[row * p.exp.ids_ld + e];
+  }
+};
+
+// The store of a loss's logits for the calling warp, 32 rows and a piece of 128 columns, t = alpha * product in the base-2
+// domain (alpha = log2(e) / temperature).  The logits stay here: what leaves is, per row, M' = max t - 15 and S' = sum 2^(t - M'),
+// t itself at the row's ids, and (with a gradient to come) the exponentials 2^(t - M') in f16.  Those are at most 2^15,
+// so they keep f16's 11 bits down to 2^-29 of the piece's largest: bf16's 8 would round the gradient a second time as
+// coarsely as its own rounding does.  128 accumulators at a time are a thread's registers: one read of the tensor memory.
+__device__ __forceinline__ void store_tile_rows_exp(const Params& p, uint32_t t_row, int row, int col_base, Wanted want) {
+  if (col_base >= p.N) return;  // warp-uniform
+  uint32_t r[4][32];
+  tmem_ld32(t_row, r[0]);
+  tmem_ld32(t_row + 32, r[1]);
+  tmem_ld32(t_row + 64, r[2]);
+  tmem_ld32(t_row + 96, r[3]);
+  tmem_wait_ld(r[0], r[1], r[2], r[3]);
+  if (col_base + 128 > p.N) {  // columns that do not exist
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col_base + c * 32 + j >= p.N) r[c][j] = __float_as_uint(-INFINITY);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    for (;;) {
+      const bool has = want.e < want.end && want.id >= col_base + c * 32 && want.id < col_base + c * 32 + 32;
+      if (!__any_sync(0xffffffffu, has)) break;
+      const uint32_t v = pick32(r[c], want.id & 31);
+      if (has) {
+        p.exp.at[row * p.exp.ids_ld + want.e] = p.alpha * __uint_as_float(v);
+        if (++want.e < want.end) want.id = p.exp.ids[row * p.exp.ids_ld + want.e];
+      }
+    }
+  }
+  if (row >= p.M) return;
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m4[c] = fmaxf(m4[c], __uint_as_float(r[c][j]));
+  const float m = p.alpha * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+  const float base = (m == -INFINITY ? 0.f : m) - 15.f;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  __half* dp = static_cast<__half*>(p.d) + static_cast<long long>(row) * p.ldd + col_base;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float e0, e1;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fmaf(__uint_as_float(r[c][g * 16 + 2 * j]), p.alpha, -base)));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fmaf(__uint_as_float(r[c][g * 16 + 2 * j + 1]), p.alpha, -base)));
+        s[c] += e0 + e1;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(e1), "f"(e0));
+      }
+      if (p.d != nullptr) st_global_v8(dp + c * 32 + g * 16, w);
+    }
+  }
+  p.exp.stats[(col_base >> 7) * p.exp.stats_ld + row] = make_float2(m == -INFINITY ? -INFINITY : base, (s[0] + s[1]) + (s[2] + s[3]));
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
                      const __grid_constant__ CUtensorMap tmap_b, const Params p) {
@@ -671,8 +763,8 @@ constexpr int PAIR_BARRIER_BYTES = 512;
 // One kernel per kind of store.  All of them in one, with the buffers that the plain ones do not need (they take room
 // from the L1, through which C is read), cost those 0.2 to 0.9 us (2048 x 5632 x
 // 256 12.3 instead of 11.9, with a bf16 C 18.8 instead of 18.0).
-enum PairStore { STORE, STORE_ADD, STORE_SWIGLU };  // D in any form, D += by TMA, the SwiGLU forms whose operands TMA brings
-constexpr int pair_staging(int kind) { return kind == STORE ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
+enum PairStore { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP };  // D in any form, D += by TMA, the SwiGLU forms whose operands TMA brings, a loss's exponentials
+constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_EXP ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
 constexpr size_t pair_smem_bytes(int kind) {
   return 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + pair_staging(kind) + PAIR_BARRIER_BYTES;
 }
@@ -923,6 +1015,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int row = tm * PAIR_M + static_cast<int>(rank) * BM + quad * 32 + lane;
       const int col = tn * BN + half * (BN / 2);
       if (KIND == STORE_SWIGLU && row - lane < p.M && col < p.N) feed.load(lane, row - lane, col);  // under the products
+      Wanted want;
+      if (KIND == STORE_EXP) want.load(p, row, col);
       if (!mbar_wait(&bars->acc_full[acc], acc_ph, abort_word, 311)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
@@ -931,6 +1025,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       } else if constexpr (KIND == STORE_SWIGLU) {
         if (p.epi_mode == 1) store_tile_rows_swiglu<false>(p, feed, t_row, row, col, lane, abort_word);
         else store_tile_rows_swiglu<true>(p, feed, t_row, row, col, lane, abort_word);
+      } else if constexpr (KIND == STORE_EXP) {
+        store_tile_rows_exp(p, t_row, row, col, want);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
         else store_tile_rows(p, t_row, b, row, col);
@@ -1117,6 +1213,50 @@ static int32_t check_epi_operand(const char* name, const cdl_tensor* t, long lon
       t->stride[1] != 1 || t->stride[0] % 8 != 0 || (reinterpret_cast<uintptr_t>(t->ptr) & 15) != 0)
     return fail(CDL_ERR_INVALID,
                 "matmul (fused SwiGLU): %s must be bf16 [%lld, %lld] with 16-byte aligned rows", name, M, N);
+  return CDL_OK;
+}
+
+static int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
+}
+
+// Once per device: the kernels' shared memory, and how many CTA pairs the device can hold at once (GPCs with an odd SM
+// count lose one SM).
+static int32_t prepare_kernels(int* clusters) {
+  using namespace gemm;
+  static std::once_flag attr_once[64];
+  static int max_clusters[64] = {};
+  int dev = 0;
+  CDL_CUDA(cudaGetDevice(&dev));
+  cudaError_t attr_err = cudaSuccess;
+  std::call_once(attr_once[dev & 63], [&] {
+    attr_err = cudaFuncSetAttribute(gemm_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(SMEM_BYTES));
+    auto pair = [&](auto kernel, int kind) {
+      if (attr_err == cudaSuccess)
+        attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(pair_smem_bytes(kind)));
+    };
+    pair(gemm_bf16_pair_kernel<STORE>, STORE);
+    pair(gemm_bf16_pair_kernel<STORE_ADD>, STORE_ADD);
+    pair(gemm_bf16_pair_kernel<STORE_SWIGLU>, STORE_SWIGLU);
+    pair(gemm_bf16_pair_kernel<STORE_EXP>, STORE_EXP);
+    int n = 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = pair_smem_bytes(STORE);
+    if (attr_err == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&n, gemm_bf16_pair_kernel<STORE>, &cfg) == cudaSuccess && n > 0)
+      max_clusters[dev & 63] = n;
+    else
+      max_clusters[dev & 63] = sm_count() / 2;
+    (void)cudaGetLastError();
+  });
+  if (attr_err != cudaSuccess)
+    return fail(CDL_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(attr_err));
+  *clusters = max_clusters[dev & 63];
   return CDL_OK;
 }
 
@@ -1388,37 +1528,8 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
     return gemm_cluster_launch(tm_a, tm_b, p, early, stream);
   }
 
-  static std::once_flag attr_once[64];
-  static int max_clusters[64] = {};
-  int dev = 0;
-  CDL_CUDA(cudaGetDevice(&dev));
-  cudaError_t attr_err = cudaSuccess;
-  std::call_once(attr_once[dev & 63], [&] {
-    attr_err = cudaFuncSetAttribute(gemm_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(SMEM_BYTES));
-    auto pair = [&](auto kernel, int kind) {
-      if (attr_err == cudaSuccess)
-        attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(pair_smem_bytes(kind)));
-    };
-    pair(gemm_bf16_pair_kernel<STORE>, STORE);
-    pair(gemm_bf16_pair_kernel<STORE_ADD>, STORE_ADD);
-    pair(gemm_bf16_pair_kernel<STORE_SWIGLU>, STORE_SWIGLU);
-    // How many CTA pairs the device can hold at once (GPCs with an odd SM count lose one SM).
-    int n = 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = pair_smem_bytes(STORE);
-    if (attr_err == cudaSuccess &&
-        cudaOccupancyMaxActiveClusters(&n, gemm_bf16_pair_kernel<STORE>, &cfg) == cudaSuccess && n > 0)
-      max_clusters[dev & 63] = n;
-    else
-      max_clusters[dev & 63] = sm_count() / 2;
-    (void)cudaGetLastError();
-  });
-  if (attr_err != cudaSuccess)
-    return fail(CDL_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(attr_err));
+  int clusters_held = 0;
+  CDL_CHECK(prepare_kernels(&clusters_held));
 
   // K slicing for the accumulate-in-place form (D = C, f32, beta = 1: the weight-gradient GEMM,
   // whose output is small and whose K is long).  Slices add into D with atomics, which removes
@@ -1426,7 +1537,7 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   // unordered f32 sum; the caller's `deterministic` option turns it off.
   if (use_pair && adds_in_place) {
     if (!(opts && opts->deterministic != 0)) {
-      const int best_s = choose_pair_slices(p.num_tiles, p.k_blocks, max_clusters[dev & 63]);
+      const int best_s = choose_pair_slices(p.num_tiles, p.k_blocks, clusters_held);
       if (best_s > 1) {
         p.split_k = best_s;
         p.atomic_out = 1;
@@ -1447,8 +1558,8 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(batch) * M * N * K, stream);
   if (use_pair) {
     const long long units = static_cast<long long>(p.num_tiles) * p.split_k;
-    const int clusters = units < max_clusters[dev & 63] ? static_cast<int>(units) : max_clusters[dev & 63];
-    p.sched_counter = units > clusters ? sched_counter_for(gemm_counter_kind(early), dev, stream) : nullptr;
+    const int clusters = units < clusters_held ? static_cast<int>(units) : clusters_held;
+    p.sched_counter = units > clusters ? sched_counter_for(gemm_counter_kind(early), current_device(), stream) : nullptr;
     auto run = [&](auto kernel, int kind) {
       return launch_pdl(kernel, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(kind), stream, tm_a, tm_b, tm_e0, tm_e1, p);
     };
@@ -1459,6 +1570,58 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
     const int grid = p.num_tiles < sm_count() ? p.num_tiles : sm_count();
     CDL_CUDA(launch_pdl(gemm_bf16_kernel, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, tm_a, tm_b, p));
   }
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+// The logits of a loss (see store_tile_rows_exp): always CTA pairs.  With few rows a pair's second half has none, but the
+// columns of B are what such a product reads, and they are loaded as fast.
+int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
+                           cudaStream_t stream) {
+  using namespace gemm;
+  const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
+  OperandLayout la, lb;
+  CDL_CHECK(analyze_operand("x", a, true, &la));
+  CDL_CHECK(analyze_operand("w", b, false, &lb));
+  CUtensorMap tm_a, tm_b;
+  {
+    const uint64_t da[3] = {static_cast<uint64_t>(la.mn_major ? M : K), static_cast<uint64_t>(la.mn_major ? K : M), 1};
+    const uint64_t db[3] = {static_cast<uint64_t>(lb.mn_major ? N : K), static_cast<uint64_t>(lb.mn_major ? K : N), 1};
+    const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(la.ld) * da[1] * 2};
+    const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(lb.ld) * db[1] * 2};
+    const uint32_t ba[3] = {64, static_cast<uint32_t>(la.mn_major ? 64 : BM), 1};
+    const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : BN / 2), 1};
+    CDL_CHECK(encode_tmap(&tm_a, a->ptr, CDL_BF16, 3, da, sa, ba, true));
+    CDL_CHECK(encode_tmap(&tm_b, b->ptr, CDL_BF16, 3, db, sb, bb, true));
+  }
+  Params p = {};
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.batch = 1;
+  p.num_m_tiles = static_cast<int>((M + PAIR_M - 1) / PAIR_M);
+  p.num_n_tiles = static_cast<int>((N + BN - 1) / BN);
+  const long long tiles = static_cast<long long>(p.num_m_tiles) * p.num_n_tiles;
+  if (tiles > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "matmul: too many tiles");
+  p.num_tiles = static_cast<int>(tiles);
+  p.k_blocks = static_cast<int>((K + BK - 1) / BK);
+  p.raster_w = RASTER_W;
+  p.a_mn = la.mn_major;
+  p.b_mn = lb.mn_major;
+  p.d = d;
+  p.ldd = ldd;
+  p.alpha = scale;
+  p.split_k = 1;
+  p.exp = {out.stats, out.stats_ld, out.ids, out.ids_ld, out.first, out.at, static_cast<int>((N + 127) / 128)};
+  p.status = device_status_ptr();
+  if (!p.status) return fail(CDL_ERR_CUDA, "cannot resolve the device status word");
+  int held = 0;
+  CDL_CHECK(prepare_kernels(&held));
+  const int clusters = tiles < held ? static_cast<int>(tiles) : held;
+  p.sched_counter = tiles > clusters ? sched_counter_for(gemm_counter_kind(0), current_device(), stream) : nullptr;
+  ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(M) * N * K, stream);
+  CDL_CUDA(launch_pdl(gemm_bf16_pair_kernel<STORE_EXP>, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(STORE_EXP), stream, tm_a,
+                      tm_b, tm_a, tm_a, p));
   CDL_CUDA(cudaGetLastError());
   return CDL_OK;
 }

@@ -8,6 +8,17 @@ namespace gemm {
 
 constexpr int RASTER_W = 8;  // N tiles per raster panel (upper bound; see Params::raster_w)
 
+// The store of the losses' logits (pair kernel): see store_tile_rows_exp in gemm.cu.  A piece is 128 columns.
+struct ExpStore {
+  float2* stats;  // [pieces][stats_ld]: (M', S') of every row and piece
+  long long stats_ld;
+  const int* ids;  // the columns whose t is wanted besides: [rows][ids_ld], ascending
+  long long ids_ld;
+  const unsigned short* first;  // [rows][pieces + 1]: a row's first id at or behind a piece's columns; nullptr: one id, not sorted
+  float* at;                    // t at the ids, [rows][ids_ld]
+  int pieces;
+};
+
 struct Params {
   int M, N, K, batch;
   int num_m_tiles, num_n_tiles, num_tiles, k_blocks;
@@ -48,6 +59,7 @@ struct Params {
   // 1 = starts before the kernel ahead of it has finished (see grid_dep_wait); 2 (CTA pairs) = the same, but what the
   // epilogue reads comes from that kernel: the epilogue waits for it.
   int early;
+  ExpStore exp;
 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& b, int& m, int& n) {

@@ -11,6 +11,7 @@
 #include "ops.h"
 #include "ptx.cuh"
 
+#include <cuda_fp16.h>
 #include <math.h>
 
 namespace cdl {
@@ -201,6 +202,162 @@ __global__ void __launch_bounds__(ROW_THREADS)
     float p = e.p[k];
     for (int i = k + 1; i < src.K; ++i) p += e.id[i] == id ? e.p[i] : 0.f;
     y[id] = from_f32<TOUT>(scale * (ex2(e.at[k] - base) / s - p));
+  }
+}
+
+// ------------------------------------------------------------------------------------------ rows behind the fused product
+// (matmul_exp_execute in gemm.cu: per row and piece of 128 columns M' and S', the exponentials 2^(t - M') in f16, t at the
+// entries' ids.)
+
+// What the product and the row kernel read of a row's entries.
+struct Prepared {
+  const int* ids;               // targets, or a teacher's ids in ascending order, those that do not count behind them
+  long long ids_ld;
+  const unsigned short* first;  // [rows][pieces + 1]: the first entry at or behind a piece's columns; nullptr: targets
+  const float* p;               // [rows][K], in the same order; nullptr: targets
+  const float* p_log_p;         // [rows]
+  const float* at;              // [rows][K]
+};
+
+constexpr int PREPARE_THREADS = 128;
+
+// A teacher's entries in the order of their ids (equal ids in their own order), one CTA per row.  An entry's place is the
+// number of those before it: K^2 comparisons of words in shared memory, no barrier between them; a sort of the 64 entries
+// that a row has would take 21 steps with one each.
+__global__ void __launch_bounds__(PREPARE_THREADS)
+    prepare_entries_kernel(const Entries src, int vocab, float tau, int pieces, int* ids, unsigned short* first, float* p, float* p_log_p) {
+  __shared__ RowEntries e;
+  __shared__ int sorted[MAX_ENTRIES];
+  grid_dep_wait();
+  grid_dep_launch();
+  const long long row = blockIdx.x;
+  float plp;
+  load_entries(e, src, row, vocab, tau, plp);
+  if (threadIdx.x == 0) p_log_p[row] = plp;
+  for (int k = threadIdx.x; k < src.K; k += PREPARE_THREADS) sorted[k] = INT32_MAX;
+  __syncthreads();
+  for (int k = threadIdx.x; k < src.K; k += PREPARE_THREADS) {
+    const int id = e.id[k];
+    if (id < 0) continue;
+    int place = 0;
+    for (int i = 0; i < src.K; ++i) place += static_cast<unsigned>(e.id[i]) < static_cast<unsigned>(id) + (i < k);
+    sorted[place] = id;
+    ids[row * src.K + place] = id;
+    p[row * src.K + place] = e.p[k];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i <= pieces; i += PREPARE_THREADS) {
+    const long long col = static_cast<long long>(i) * 128;
+    int lo = 0, hi = src.K;  // the first place whose id is at or behind col
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sorted[mid] < col || (i == pieces && sorted[mid] != INT32_MAX)) lo = mid + 1;
+      else hi = mid;
+    }
+    first[row * (pieces + 1) + i] = static_cast<unsigned short>(lo);
+  }
+}
+
+constexpr int PIECES_PER_CTA = 64;  // at most: 8192 columns
+constexpr int ROWS_PER_CTA = 8;     // a warp's each
+
+// From the pieces' statistics the rows': loss, lse, and (GRAD) the gradient of the logits in bf16 in place of the
+// exponentials, which are only multiplied with 2^(M' - M) s tau / S; the rows of x for the weight gradient's product,
+// zeros where a row does not count.  Grid (rows / 8, pieces / per).
+template <bool GRAD>
+__global__ void __launch_bounds__(256)
+    softmax_rows_kernel(const float2* stats, long long stats_ld, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
+                        int K, const Prepared src, const RowTerms terms, const __nv_bfloat16* x, long long ld_x, __nv_bfloat16* clean,
+                        long long ld_clean, int cols) {
+  __shared__ float factor[ROWS_PER_CTA][PIECES_PER_CTA];
+  __shared__ int s_counts[ROWS_PER_CTA];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.x * ROWS_PER_CTA, row = row0 + warp;
+  const int piece0 = blockIdx.y * per, piece1 = min(pieces, piece0 + per);
+  float base = 0.f, S = 0.f, scale = 0.f, over_s = 0.f;
+  bool counts = false;
+  if (row < rows) {
+    float m = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, stats[i * stats_ld + row].x);
+    m = warp_max(m);
+    base = m == -INFINITY ? 0.f : m;
+    for (int i = lane; i < pieces; i += 32) {
+      const float2 v = stats[i * stats_ld + row];
+      S += v.y * ex2(v.x - base);
+    }
+    S = warp_sum(S);
+    const float log2_s = log2f(S);
+    const int target = src.first == nullptr ? src.ids[row] : -1;
+    const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
+    const int n = src.first == nullptr ? (target >= 0 && target < vocab ? 1 : 0) : first[pieces];
+    counts = n > 0;
+    if (blockIdx.y == 0) {
+      float cross = 0.f;  // sum_k p_k log2 q_k
+      for (int k = lane; k < n; k += 32) {
+        const float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
+        if (p != 0.f) cross += p * ((src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
+      }
+      cross = warp_sum(cross);
+      if (lane == 0) {
+        const float entropy = src.p == nullptr ? 0.f : src.p_log_p[row];
+        terms.loss[row] = counts ? terms.tau * terms.tau * (entropy - LN2 * cross) : 0.f;
+        if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+      }
+    }
+    if (GRAD) {
+      scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
+      over_s = scale / S;
+      for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i * stats_ld + row].x - base) * over_s;
+      if (lane == 0) s_counts[warp] = counts;
+    }
+  }
+  if (!GRAD) return;
+  __syncthreads();
+  const int here = min(ROWS_PER_CTA, rows - row0), vecs = (piece1 - piece0) * 16;  // of 8 columns
+  for (int i = threadIdx.x; i < here * vecs; i += 256) {
+    const int r = i / vecs, v = i - r * vecs;
+    uint4* at = reinterpret_cast<uint4*>(e + (row0 + r) * ld_e + piece0 * 128) + v;
+    const float f = factor[r][v >> 4];
+    uint4 q = *at;
+    uint32_t* w = &q.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      w[j] = pack_bf16x2(h.x * f, h.y * f);
+    }
+    *at = s_counts[r] ? q : make_uint4(0, 0, 0, 0);
+  }
+  if (clean != nullptr && blockIdx.y == 0) {
+    const int per_row = (cols + 7) / 8;
+    for (int i = threadIdx.x; i < here * per_row; i += 256) {
+      const int r = i / per_row, c = (i - r * per_row) * 8;
+      const __nv_bfloat16* from = x + (row0 + r) * ld_x + c;
+      __nv_bfloat16* to = clean + (row0 + r) * ld_clean + c;
+      if (c + 8 <= cols) {
+        *reinterpret_cast<uint4*>(to) = s_counts[r] ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+      } else {
+        for (int j = 0; c + j < cols; ++j) to[j] = s_counts[r] ? from[j] : __float2bfloat16_rn(0.f);
+      }
+    }
+  }
+  __syncthreads();
+  // The entries of these columns, each id once: the sum of its entries' probabilities, in their order.
+  if (!counts) return;
+  int k0 = 0, k1 = 1;
+  if (src.first != nullptr) {
+    const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
+    k0 = first[piece0];
+    k1 = first[piece1];
+  }
+  const int* ids = src.ids + row * src.ids_ld;
+  for (int k = k0 + lane; k < k1; k += 32) {
+    const int id = ids[k];
+    if (src.first == nullptr ? id / 128 < piece0 || id / 128 >= piece1 : k > k0 && ids[k - 1] == id) continue;
+    float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
+    for (int i = k + 1; i < k1 && ids[i] == id; ++i) p += src.p[static_cast<long long>(row) * K + i];
+    e[row * ld_e + id] = __float2bfloat16_rn(scale * (ex2(src.at[static_cast<long long>(row) * K + k] - base) / S - p));
   }
 }
 
@@ -407,6 +564,9 @@ struct Linear {
   long long ld_z, ld_g, ld_sum;
   size_t at_x, at_w, at_z, at_g, at_clean, at_keep, at_sum, at_products, bytes;
   size_t products_bytes;
+  // bf16: the product writes statistics and exponentials (at_g), not logits
+  int pieces, K;
+  size_t at_stats, at_ids, at_first, at_p, at_p_log_p, at_at;
 };
 
 // A view of `rows` rows from `row`.
@@ -423,6 +583,8 @@ static cdl_tensor strided2(void* p, int32_t dt, long long r, long long c, long l
   return t;
 }
 
+constexpr long long TARGET_ENTRIES = -1;
+
 // Rows that are taken at a time: their logits (and the gradients of those) are what the scratch holds.
 static long long choose_chunk(long long T, long long V, size_t bytes_per_logit) {
   const long long most = (512LL << 20) / static_cast<long long>(bytes_per_logit * V);
@@ -432,18 +594,23 @@ static long long choose_chunk(long long T, long long V, size_t bytes_per_logit) 
   return up((T + chunks - 1) / chunks, 256);
 }
 
-static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc) {
+static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long entries) {
   const bool grad = p.has_dx || p.has_dw;
   const int32_t type = p.x.dtype;
   const size_t es = dtype_size(type);
-  p.copy_x = !readable(p.x) || (type == CDL_BF16 && p.T > 1 && p.x.stride[0] < p.D);  // (chunks of rows start on the grid)
+  p.copy_x = !readable(p.x);
+  if (type == CDL_BF16)  // (a chunk of its rows starts on the grid too)
+    p.copy_x = (reinterpret_cast<uintptr_t>(p.x.ptr) & 15) != 0 || (p.D > 1 && p.x.stride[1] != 1) ||
+               (p.T > 1 && (p.x.stride[0] % 8 != 0 || p.x.stride[0] < p.D));
   p.copy_w = !readable(p.w);
-  p.chunk = desc->chunk_rows > 0 ? (desc->chunk_rows < p.T ? desc->chunk_rows : p.T) : choose_chunk(p.T, p.V, 4);
+  p.chunk = desc->chunk_rows > 0 ? (desc->chunk_rows < p.T ? desc->chunk_rows : p.T) : choose_chunk(p.T, p.V, es);
   const bool whole = p.chunk >= p.T;
   const bool dw_rows = p.has_dw && (p.dw.stride[1] == 1 || p.dw.stride[0] == 1);
   p.sums = p.has_dw && (!dw_rows || (p.dw.dtype == CDL_BF16 && !whole));
   p.ld_z = up(p.V, 64);
-  p.ld_g = up(p.V, 64);
+  p.ld_g = up(p.V, 128);
+  p.pieces = static_cast<int>(up(p.V, 128) / 128);
+  p.K = static_cast<int>(entries);
   p.ld_sum = p.has_dw ? up(columns_first(p.dw) ? p.D : p.V, 64) : 0;
   size_t at = 0;
   auto take = [&](bool want, size_t bytes) {
@@ -455,11 +622,19 @@ static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc) {
   p.at_x = take(p.copy_x, static_cast<size_t>(p.T) * x_ld * es);
   const bool wc = columns_first(p.w);
   p.at_w = take(p.copy_w, static_cast<size_t>(wc ? p.V : p.D) * up(wc ? p.D : p.V, 8) * es);
-  p.at_z = take(true, static_cast<size_t>(p.chunk) * p.ld_z * 4);
-  p.at_g = take(grad && type == CDL_BF16, static_cast<size_t>(p.chunk) * p.ld_g * 2);
-  if (type == CDL_F32) p.at_g = p.at_z;  // in place
+  const bool fused = type == CDL_BF16, teacher = entries != TARGET_ENTRIES;
+  const size_t n = static_cast<size_t>(p.chunk);
+  p.at_z = take(!fused, n * p.ld_z * 4);
+  p.at_g = take(fused && grad, n * p.ld_g * 2);
+  if (!fused) p.at_g = p.at_z, p.ld_g = p.ld_z;  // in place
+  p.at_stats = take(fused, n * p.pieces * sizeof(float2));
+  p.at_at = take(fused, n * (teacher ? p.K : 1) * 4);
+  p.at_ids = take(fused && teacher, n * p.K * 4);
+  p.at_p = take(fused && teacher, n * p.K * 4);
+  p.at_p_log_p = take(fused && teacher, n * 4);
+  p.at_first = take(fused && teacher, n * (p.pieces + 1) * 2);
   p.at_clean = take(p.has_dw, static_cast<size_t>(p.chunk) * x_ld * es);
-  p.at_keep = take(p.has_dw, static_cast<size_t>(p.chunk) * 4);
+  p.at_keep = take(!fused && p.has_dw, static_cast<size_t>(p.chunk) * 4);
   p.at_sum = take(p.sums, static_cast<size_t>(columns_first(p.dw) ? p.V : p.D) * p.ld_sum * 4);
   p.products_bytes = 0;
   if (type == CDL_F32) {  // (bf16 operands are on the grid by now)
@@ -484,7 +659,7 @@ static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc) {
 }
 
 static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
-                            const cdl_tensor* dx, const cdl_tensor* dw, Linear* out) {
+                            const cdl_tensor* dx, const cdl_tensor* dw, long long entries, Linear* out) {
   CDL_CHECK(check_desc(op, desc));
   if (!x || !w || x->rank != 2 || w->rank != 2 || !is_float(x->dtype) || x->dtype != w->dtype)
     return fail(CDL_ERR_INVALID, "%s: x must be bf16 or f32 [tokens, hidden], w of the same type [hidden, vocab]", op);
@@ -500,7 +675,7 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
   p.has_dw = dw != nullptr;
   if (w->shape[0] != p.D)
     return fail(CDL_ERR_INVALID, "%s: x is [tokens, %lld], w is [%lld, vocab]: the hidden sizes differ", op, p.D, (long long)w->shape[0]);
-  if (p.T > INT32_MAX || p.D > INT32_MAX || p.V > INT32_MAX - 64) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  if (p.T > INT32_MAX || p.D > INT32_MAX || p.V > 65535LL * 8 * 128) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
   if (dx) {
     if (dx->rank != 2 || dx->dtype != x->dtype || dx->shape[0] != p.T || dx->shape[1] != p.D || (p.D > 1 && dx->stride[1] != 1) ||
         (p.T > 1 && dx->stride[0] < p.D))
@@ -518,7 +693,41 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
   }
   if (p.V == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
   if (p.D == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: hidden is zero", op);
-  return plan_linear(p, desc);
+  return plan_linear(p, desc, entries);
+}
+
+// The statistics, losses and logits' gradients of a chunk of rows of bf16 operands on the 16-byte grid.
+static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor& w, const Entries& e, const RowTerms& t,
+                          const cdl_tensor& clean, char* base, bool grad, cudaStream_t stream) {
+  const int rows = static_cast<int>(x.shape[0]), vocab = static_cast<int>(p.V);
+  const bool teacher = e.kind != TARGETS;
+  float2* stats = reinterpret_cast<float2*>(base + p.at_stats);
+  float* at = reinterpret_cast<float*>(base + p.at_at);
+  int* ids = reinterpret_cast<int*>(base + p.at_ids);
+  float *probs = reinterpret_cast<float*>(base + p.at_p), *p_log_p = reinterpret_cast<float*>(base + p.at_p_log_p);
+  unsigned short* first = reinterpret_cast<unsigned short*>(base + p.at_first);
+  const Prepared src = teacher ? Prepared{ids, e.K, first, probs, p_log_p, at} : Prepared{e.ids, e.ids_ld, nullptr, nullptr, nullptr, at};
+  if (teacher)
+    CDL_CUDA(launch_pdl(prepare_entries_kernel, dim3(rows), dim3(PREPARE_THREADS), 0, stream, e, vocab, t.tau, p.pieces, ids, first, probs, p_log_p));
+  void* out = grad ? base + p.at_g : nullptr;
+  CDL_CHECK(matmul_exp_execute(&x, &w, LOG2E / t.tau, out, p.ld_g, {stats, p.chunk, src.ids, src.ids_ld, src.first, at}, stream));
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (grad ? 4 : 0) + 8.0 * rows * p.pieces, stream);
+  const dim3 block(256);
+  const unsigned row_ctas = (rows + ROWS_PER_CTA - 1) / ROWS_PER_CTA;
+  auto run = [&](auto kernel, unsigned splits, int per) {
+    return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, p.chunk, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
+                      vocab, p.pieces, per, e.K, src, t, static_cast<const __nv_bfloat16*>(x.ptr), static_cast<long long>(x.stride[0]),
+                      p.has_dw ? static_cast<__nv_bfloat16*>(clean.ptr) : nullptr, static_cast<long long>(clean.stride[0]),
+                      static_cast<int>(p.D));
+  };
+  if (!grad) {
+    CDL_CUDA(run(softmax_rows_kernel<false>, 1, p.pieces));
+    return CDL_OK;
+  }
+  int per = PIECES_PER_CTA;  // fewer where that leaves SMs without a CTA
+  while (per > 8 && row_ctas * ((p.pieces + per - 1) / per) < 2u * sm_count()) per /= 2;
+  CDL_CUDA(run(softmax_rows_kernel<true>, (p.pieces + per - 1) / per, per));
+  return CDL_OK;
 }
 
 static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& entries, const RowTerms& terms, void* scratch,
@@ -530,6 +739,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
   }
   if (p.bytes > 0 && (!scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(scratch) & 255)))
     return fail(CDL_ERR_INVALID, "%s: scratch must hold %zu bytes, 256-byte aligned", p.op, p.bytes);
+  const FixedWorkInGraph fixed_work(stream);
   char* base = static_cast<char*>(scratch);
   const int32_t type = p.x.dtype;
   const long long x_ld = up(p.D, 8);
@@ -558,28 +768,35 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
   if (p.sums)
     sum = dw_columns ? transposed(strided2(base + p.at_sum, CDL_F32, p.V, p.D, p.ld_sum))
                      : strided2(base + p.at_sum, CDL_F32, p.D, p.V, p.ld_sum);
+  const bool fused = type == CDL_BF16;
   for (long long row = 0; row < p.T; row += p.chunk) {
     const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
     const cdl_tensor xc = rows_of(x, row, n);
-    const cdl_tensor z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_z);
     const Entries e = from_row(entries, row);
-    CDL_CHECK(matmul_execute(&xc, &w, nullptr, &z, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
+    const RowTerms t = from_row(terms, row);
     const cdl_tensor g = strided2(base + p.at_g, type, n, p.V, p.ld_g);
-    CDL_CHECK(launch_rows(z.ptr, CDL_F32, p.ld_z, grad ? g.ptr : nullptr, type, p.ld_g, n, static_cast<int>(p.V), e, from_row(terms, row), stream));
-    if (p.has_dw) {
-      // A row that does not count adds nothing whatever it holds, infinities and NaN too: its gradient's zeros alone
-      // would not do that.  (Copied before dx is written, which may be x itself.)
-      float* keep = reinterpret_cast<float*>(base + p.at_keep);
-      keep_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(e, n, static_cast<int>(p.V), keep);
-      CDL_CUDA(cudaGetLastError());
-      CDL_CHECK(copy(xc, base + p.at_clean, x_ld, keep, stream));
+    // A row that does not count adds nothing to dw whatever x holds there, infinities and NaN too, which a gradient of zeros
+    // alone would not do: the product takes a copy of x with zeros in such rows (made before dx is written, which may
+    // be x itself).
+    const cdl_tensor clean = strided2(base + p.at_clean, type, n, p.D, x_ld);
+    if (fused) {
+      CDL_CHECK(fused_rows(p, xc, w, e, t, clean, base, grad, stream));
+    } else {
+      const cdl_tensor z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_z);
+      CDL_CHECK(matmul_execute(&xc, &w, nullptr, &z, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
+      CDL_CHECK(launch_rows(z.ptr, CDL_F32, p.ld_z, grad ? g.ptr : nullptr, type, p.ld_g, n, static_cast<int>(p.V), e, t, stream));
+      if (p.has_dw) {
+        float* keep = reinterpret_cast<float*>(base + p.at_keep);
+        keep_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(e, n, static_cast<int>(p.V), keep);
+        CDL_CUDA(cudaGetLastError());
+        CDL_CHECK(copy(xc, clean.ptr, x_ld, keep, stream));
+      }
     }
     if (p.has_dx) {
       const cdl_tensor d = rows_of(p.dx, row, n);
       CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
     }
     if (p.has_dw) {
-      const cdl_tensor clean = strided2(base + p.at_clean, type, n, p.D, x_ld);
       const bool add = row > 0 || (!p.sums && desc->accumulate_dw);
       const cdl_tensor gt = transposed(g), xt = transposed(clean), sum_t = transposed(sum);
       const cdl_tensor *a = dw_columns ? &gt : &xt, *b = dw_columns ? &clean : &g, *d = dw_columns ? &sum_t : &sum;
@@ -610,9 +827,11 @@ int32_t cdl_b200_linear_loss_scratch_bytes(const cdl_head_loss_desc* desc, const
   using namespace cdl;
   if (!bytes_out) return fail(CDL_ERR_INVALID, "linear_loss_scratch_bytes: bytes_out is required");
   *bytes_out = 0;
-  if (entries < 0) return fail(CDL_ERR_INVALID, "linear_loss_scratch_bytes: entries must not be negative");
+  if (entries < 0 || entries > head::MAX_ENTRIES)
+    return fail(CDL_ERR_INVALID, "linear_loss_scratch_bytes: entries must be in 0 .. %d", head::MAX_ENTRIES);
+  if (entries == 0) entries = 1;  // (targets have one)
   head::Linear p;
-  CDL_CHECK(head::check_linear("linear_loss_scratch_bytes", desc, x, w, dx, dw, &p));
+  CDL_CHECK(head::check_linear("linear_loss_scratch_bytes", desc, x, w, dx, dw, entries, &p));
   if (p.T > 0) *bytes_out = p.bytes;
   return CDL_OK;
 }
@@ -624,7 +843,7 @@ int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_
   using namespace cdl;
   const char* op = "linear_cross_entropy";
   head::Linear p;
-  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, &p));
+  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, head::TARGET_ENTRIES, &p));
   if (desc->temperature != 1.f) return fail(CDL_ERR_UNSUPPORTED, "%s: temperature must be 1", op);
   head::Entries e;
   head::RowTerms terms;
@@ -639,8 +858,11 @@ int32_t cdl_b200_linear_distillation(const cdl_head_loss_desc* desc, const cdl_t
                                      void* scratch, size_t scratch_bytes, cdl_stream stream) {
   using namespace cdl;
   const char* op = "linear_distillation";
+  const long long entries = teacher_ids && teacher_ids->rank == 2 ? teacher_ids->shape[1] : 0;
+  if (entries > head::MAX_ENTRIES)
+    return fail(CDL_ERR_UNSUPPORTED, "%s: at most %d entries per token (got %lld)", op, head::MAX_ENTRIES, entries);
   head::Linear p;
-  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, &p));
+  CDL_CHECK(head::check_linear(op, desc, x, w, dx, dw, entries, &p));
   head::Entries e;
   head::RowTerms terms;
   CDL_CHECK(head::check_teacher(op, p.T, teacher_ids, teacher_logits, &e));

@@ -70,7 +70,16 @@ constexpr int SCHED_KINDS = 8;
 constexpr int SCHED_STREAMS = 256;
 __device__ unsigned int g_sched_counters[SCHED_KINDS * SCHED_STREAMS];
 
+static thread_local bool t_fixed_work = false;
+FixedWorkInGraph::FixedWorkInGraph(cudaStream_t stream) : before_(t_fixed_work) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) (void)cudaGetLastError();
+  if (status != cudaStreamCaptureStatusNone) t_fixed_work = true;
+}
+FixedWorkInGraph::~FixedWorkInGraph() { t_fixed_work = before_; }
+
 unsigned int* sched_counter_for(int kind, int dev, cudaStream_t stream) {
+  if (t_fixed_work) return nullptr;
 #if CDL_DYNAMIC_WORK
   static std::mutex mu;
   static unsigned int* base[kMaxDevices] = {};

@@ -97,6 +97,17 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
 
 // Device counter for a kernel that hands out its work at run time (see host.cu); nullptr: none.
 unsigned int* sched_counter_for(int kind, int dev, cudaStream_t stream);
+// While it lives, the calling thread's launches get no counter if `stream` is being captured: graphs captured on one stream may
+// be replayed beside one another on two, where a counter of the stream that captured them would mix up their work.
+class FixedWorkInGraph {
+ public:
+  explicit FixedWorkInGraph(cudaStream_t stream);
+  ~FixedWorkInGraph();
+  FixedWorkInGraph(const FixedWorkInGraph&) = delete;
+  FixedWorkInGraph& operator=(const FixedWorkInGraph&) = delete;
+ private:
+  bool before_;
+};
 // The kind of a GEMM's counter; those that start early (1 to 4) may overlap and have one each.
 inline int gemm_counter_kind(int early) { return (early & 7) > 0 ? 3 + (early & 7) : 0; }
 
