@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <mutex>
+
 namespace cdl {
 namespace head {
 
@@ -21,6 +23,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int MAX_ENTRIES = 1024;  // of a teacher, per row: they are kept in shared memory
 constexpr int ROW_THREADS = 512;
+
+static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
 
 // The distributions p of all rows: targets (one entry of probability 1), or a teacher's ids and logits.
 struct Entries {
@@ -62,14 +66,6 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// (M, S) of two parts of a row.  A part without finite logits has M = -inf and S = 0 (or NaN, which stays).
-__device__ __forceinline__ void join(float& m, float& s, float om, float os) {
-  const float nm = fmaxf(m, om);
-  const float base = nm == -INFINITY ? 0.f : nm;
-  s = s * ex2(m - base) + os * ex2(om - base);
-  m = nm;
-}
-
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -83,12 +79,20 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// A row's entries in shared memory.
+// A row's entries in shared memory, and what a reduction over the CTA uses.
 struct RowEntries {
-  int id[MAX_ENTRIES];    // -1: does not count
-  float p[MAX_ENTRIES];
-  float at[MAX_ENTRIES];  // t of the row at the entry's id
-  float part[32];         // of a reduction over the CTA
+  int* id;    // -1: does not count
+  float* p;   // of the entry
+  float* sum; // of all entries of its id, at the first of them; -1 at the others
+  float* at;  // t of the row at the id
+  __device__ __forceinline__ RowEntries(void* smem, int K)
+      : id(static_cast<int*>(smem)), p(static_cast<float*>(smem) + K), sum(p + K), at(sum + K) {}
+};
+constexpr int ENTRY_BYTES = 16;
+struct RowShared {
+  float part[32];
+  float p_log_p;
+  int counts;
 };
 
 __device__ __forceinline__ float cta_reduce(float v, bool max, float* part) {
@@ -101,24 +105,26 @@ __device__ __forceinline__ float cta_reduce(float v, bool max, float* part) {
   return max ? warp_max(v) : warp_sum(v);
 }
 
-// Loads the entries of a row by the whole CTA: ids, and p = softmax(teacher / tau) over those that count (id in [0, vocab),
-// logit above -inf).  Returns whether there are any, and sum p log p.
-__device__ __forceinline__ bool load_entries(RowEntries& e, const Entries& src, long long row, int vocab, float tau, float& p_log_p) {
-  p_log_p = 0.f;
+// A row's entries by one warp: ids and p = softmax(teacher / tau) over those that count (id in [0, vocab), logit above
+// -inf); sum p log p; whether there are any.
+__device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh, const Entries& src, long long row, int vocab,
+                                             float tau) {
+  const int lane = threadIdx.x & 31;
   if (src.kind == TARGETS) {
     const int id = src.ids[row];
     const bool counts = id >= 0 && id < vocab;
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
       e.id[0] = counts ? id : -1;
       e.p[0] = counts ? 1.f : 0.f;
+      sh.counts = counts;
+      sh.p_log_p = 0.f;
     }
-    __syncthreads();
-    return counts;
+    return;
   }
   const int* ids = src.ids + row * src.ids_ld;
   const float c = LOG2E / tau;
   float m = -INFINITY;
-  for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+  for (int k = lane; k < src.K; k += 32) {
     const int id = ids[k];
     float y = -INFINITY;
     if (id >= 0 && id < vocab)  // (padding may hold anything)
@@ -127,37 +133,55 @@ __device__ __forceinline__ bool load_entries(RowEntries& e, const Entries& src, 
     e.p[k] = y;
     m = fmaxf(m, y != y ? INFINITY : y);  // a NaN makes the row NaN
   }
-  m = cta_reduce(m, true, e.part);
-  if (m == -INFINITY) {
-    for (int k = threadIdx.x; k < src.K; k += blockDim.x) e.p[k] = 0.f;
-    __syncthreads();
-    return false;
-  }
+  m = warp_max(m);
+  const bool counts = m != -INFINITY;
   float s = 0.f, sy = 0.f;
-  for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+  for (int k = lane; k < src.K; k += 32) {
     const float y = e.p[k] - m, x = e.id[k] < 0 ? 0.f : ex2(y);
     e.p[k] = x;
     s += x;
     if (x != 0.f) sy += x * y;
   }
-  s = cta_reduce(s, false, e.part);
-  sy = cta_reduce(sy, false, e.part);
-  for (int k = threadIdx.x; k < src.K; k += blockDim.x) e.p[k] /= s;
-  p_log_p = LN2 * (sy / s - log2f(s));
-  __syncthreads();
-  return true;
+  s = warp_sum(s);
+  sy = warp_sum(sy);
+  for (int k = lane; k < src.K; k += 32) e.p[k] = counts ? e.p[k] / s : 0.f;
+  if (lane == 0) {
+    sh.counts = counts;
+    sh.p_log_p = counts ? LN2 * (sy / s - log2f(s)) : 0.f;
+  }
 }
 
-// One CTA per row: the row is read twice (the second time from the L2), any alignment.
-template <typename TIN, typename TOUT>
+// Each id once: the sum of its entries' probabilities, in their order.  All threads, entries visible.
+__device__ __forceinline__ void merge_entries(const RowEntries& e, int K) {
+  for (int k = threadIdx.x; k < K; k += blockDim.x) {
+    const int id = e.id[k];
+    float sum = 0.f;
+    bool again = id < 0;
+#pragma unroll 8
+    for (int i = 0; i < K; ++i) {
+      const bool same = e.id[i] == id;
+      again = again || (same && i < k);
+      sum += same ? e.p[i] : 0.f;
+    }
+    e.sum[k] = again ? -1.f : sum;
+  }
+}
+
+// One CTA per row: the row is read twice (the second time from the L2), any alignment and length.
+template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS)
-    loss_row_kernel(const TIN* z, long long ld_z, TOUT* g, long long ld_g, int vocab, const Entries src, const RowTerms terms) {
-  __shared__ RowEntries e;
+    loss_row_kernel(const T* z, long long ld_z, T* g, long long ld_g, int vocab, const Entries src, const RowTerms terms) {
+  __shared__ int4 entries[MAX_ENTRIES];
+  __shared__ RowShared sh;
+  const RowEntries e(entries, src.K);
+  grid_dep_wait();
+  grid_dep_launch();
   const long long row = blockIdx.x;
-  const TIN* x = z + row * ld_z;
+  const T* x = z + row * ld_z;
   const float c = LOG2E / terms.tau;
-  float p_log_p;
-  const bool counts = load_entries(e, src, row, vocab, terms.tau, p_log_p);
+  if (threadIdx.x < 32) load_entries(e, sh, src, row, vocab, terms.tau);
+  __syncthreads();
+  merge_entries(e, src.K);
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) e.at[k] = e.id[k] < 0 ? 0.f : c * to_f32(x[e.id[k]]);
   float m = -INFINITY, s = 0.f;
   bool bad = false;
@@ -171,38 +195,230 @@ __global__ void __launch_bounds__(ROW_THREADS)
       s += ex2(t - m);
     }
   }
-  const float top = cta_reduce(m, true, e.part);
+  const float top = cta_reduce(m, true, sh.part);
   const float base = top == -INFINITY ? 0.f : top;
-  s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(m - base)), false, e.part);
+  s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(m - base)), false, sh.part);
   const float log2_s = log2f(s);
-  // sum_k p_k (log p_k - log q_k)
-  float cross = 0.f;
+  float cross = 0.f;  // sum_k p_k log2 q_k
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
-    if (e.id[k] >= 0 && e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
-  cross = cta_reduce(cross, false, e.part);
+    if (e.sum[k] > 0.f || e.sum[k] != e.sum[k]) cross += e.sum[k] * ((e.at[k] - base) - log2_s);
+  cross = cta_reduce(cross, false, sh.part);
+  const bool counts = sh.counts;
   if (threadIdx.x == 0) {
-    terms.loss[row] = counts ? terms.tau * terms.tau * (p_log_p - LN2 * cross) : 0.f;
+    terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
     if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
   }
   if (g == nullptr) return;
-  TOUT* y = g + row * ld_g;
+  T* y = g + row * ld_g;
   const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
   const float over_s = scale / s;
-  __syncthreads();
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS)
-    y[j] = from_f32<TOUT>(counts ? ex2(fmaf(to_f32(x[j]), c, -base)) * over_s : 0.f);
+    y[j] = from_f32<T>(counts ? ex2(fmaf(to_f32(x[j]), c, -base)) * over_s : 0.f);
   __syncthreads();
-  // The entries, each id once: the sum of its entries' probabilities, in their order.
-  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) {
-    const int id = e.id[k];
-    if (id < 0) continue;
-    bool first = true;
-    for (int i = 0; i < k; ++i) first = first && e.id[i] != id;
-    if (!first) continue;
-    float p = e.p[k];
-    for (int i = k + 1; i < src.K; ++i) p += e.id[i] == id ? e.p[i] : 0.f;
-    y[id] = from_f32<TOUT>(scale * (ex2(e.at[k] - base) / s - p));
+  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
+    if (e.sum[k] != -1.f) y[e.id[k]] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - e.sum[k]));
+}
+
+// The same with the row in shared memory, read from and written to HBM once: a cluster of 1 to 8 CTAs per row, whose warps have
+// a slice of it each.  A warp brings its slice by a bulk copy of its own and goes over it in three passes: the maximum;
+// the exponentials, which replace the logits (bf16: as f16 of up to 2^15, see store_tile_rows_exp in gemm.cu; their sum is
+// of the f32 values); and, behind the one barrier at which the slices' (M', S') meet, the gradient.  One exponential per
+// element: a second one would put 4096 clk of special functions per 64 KB on an SM, whose share of the HBM's rate takes 5500.
+// Three CTAs per SM are in different passes and keep the copies going.  The slices depend on the vocabulary alone, not on
+// how many CTAs share a row, so a row's results do not depend on the number of rows.
+struct Share {
+  int warps, vecs, ctas;  // warps of a row, 16-byte vectors of a warp, CTAs of a row
+  size_t smem;            // of a CTA
+};
+constexpr int SHARE_BYTES = 72 * 1024;  // three CTAs per SM
+constexpr int MAX_ROW_WARPS = 8 * ROW_THREADS / 32;
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& q, float (&f)[16 / sizeof(T)]);
+template <>
+__device__ __forceinline__ void unpack<float>(const uint4& q, float (&f)[4]) {
+  f[0] = __uint_as_float(q.x); f[1] = __uint_as_float(q.y); f[2] = __uint_as_float(q.z); f[3] = __uint_as_float(q.w);
+}
+template <>
+__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& q, float (&f)[8]) {
+  f[0] = bf16_lo(q.x); f[1] = bf16_hi(q.x); f[2] = bf16_lo(q.y); f[3] = bf16_hi(q.y);
+  f[4] = bf16_lo(q.z); f[5] = bf16_hi(q.z); f[6] = bf16_lo(q.w); f[7] = bf16_hi(q.w);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS, 3)
+    loss_share_kernel(const T* z, long long ld_z, T* g, long long ld_g, int vocab, int slice, int ctas, const Entries src,
+                      const RowTerms terms, int* status) {
+  constexpr bool HALF = sizeof(T) == 2;
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ RowShared sh;
+  __shared__ float2 s_part[ROW_THREADS / 32];  // (M', S') of the CTA's slices
+  __shared__ uint64_t full[ROW_THREADS / 32];
+  __shared__ int abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const long long row = blockIdx.x / ctas;
+  const int rank = blockIdx.x - static_cast<int>(row) * ctas;
+  const T* x = z + row * ld_z;
+  // The row in 16-byte vectors of memory: its first element is element `lead` of vector 0.
+  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
+  const int all = (lead + vocab + VEC - 1) / VEC, whole0 = lead != 0, whole1 = (lead + vocab) / VEC;
+  const int v0 = min(all, (rank * warps + warp) * slice), v1 = min(all, v0 + slice);  // the warp's
+  uint4* vec = reinterpret_cast<uint4*>(smem) + warp * slice;  // vector v0's place
+  const RowEntries e(smem + static_cast<size_t>(warps) * slice * 16, src.K);
+  if (threadIdx.x == 0) abort_word = 0;
+  if (lane == 0) {
+    mbar_init(&full[warp], 1);
+    fence_mbar_init();
   }
+  grid_dep_wait();
+  grid_dep_launch();
+  const int b0 = max(v0, whole0), b1 = min(v1, whole1);
+  if (lane == 0 && b1 > b0) {
+    mbar_arrive_expect_tx(&full[warp], (b1 - b0) * 16);
+    bulk_load_1d(vec + (b0 - v0), x - lead + static_cast<long long>(b0) * VEC, (b1 - b0) * 16, &full[warp]);
+  }
+  // What the copy does not bring: vectors that the row fills in part, with -inf around its elements.
+  auto partial = [&](int v) {
+    const int at = v * VEC + lane - lead;
+    if (lane < VEC) reinterpret_cast<T*>(vec + (v - v0))[lane] = at >= 0 && at < vocab ? x[at] : from_f32<T>(-INFINITY);
+  };
+  if (v0 == 0 && v1 > 0 && whole0 > 0) partial(0);
+  if (v0 <= whole1 && whole1 < v1 && whole1 >= whole0) partial(whole1);
+  const float c = LOG2E / terms.tau;
+  if (warp == 0) {
+    load_entries(e, sh, src, row, vocab, terms.tau);
+    __syncwarp();
+    for (int k = lane; k < src.K; k += 32) e.at[k] = e.id[k] < 0 ? 0.f : c * to_f32(x[e.id[k]]);
+  }
+  __syncthreads();  // (abort_word; and entries for merge_entries)
+  bool arrived = true;
+  if (b1 > b0) arrived = mbar_wait(&full[warp], 0, &abort_word, 701);
+  __syncwarp();
+  const int n = v1 - v0;
+  float m = -INFINITY;
+  if constexpr (HALF) {
+    __nv_bfloat162 top = __float2bfloat162_rn(-INFINITY);
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) {
+      const uint4 q = vec[i];
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+      top = __hmax2(__hmax2(top, __hmax2(h[0], h[1])), __hmax2(h[2], h[3]));
+    }
+    m = fmaxf(__low2float(top), __high2float(top));
+  } else {
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) {
+      float f[VEC];
+      unpack<T>(vec[i], f);
+      m = fmaxf(m, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
+    }
+  }
+  m = c * warp_max(m);
+  const float own = (m == -INFINITY ? 0.f : m) - (HALF ? 15.f : 0.f);  // M'
+  float s = 0.f;
+#pragma unroll 2
+  for (int i = lane; i < n; i += 32) {
+    float f[VEC];
+    unpack<T>(vec[i], f);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      f[j] = ex2(fmaf(f[j], c, -own));
+      s += f[j];
+    }
+    if (g != nullptr) {
+      uint4 q;
+      uint32_t* w = &q.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
+        else w[j] = __float_as_uint(f[j]);
+      }
+      vec[i] = q;
+    }
+  }
+  s = warp_sum(arrived ? s : NAN);
+  if (lane == 0) s_part[warp] = make_float2(m == -INFINITY ? -INFINITY : own, s);
+  if (ctas > 1) cluster_sync_all();  // (the entries' logits have been read, too: they may be overwritten)
+  else __syncthreads();
+  float2 part[MAX_ROW_WARPS / 32];
+  float base = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < MAX_ROW_WARPS / 32; ++i) {
+    const int w = lane + 32 * i;
+    part[i] = make_float2(-INFINITY, 0.f);
+    if (w < warps * ctas) {
+      if (ctas == 1) part[i] = s_part[w];
+      else
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(part[i].x), "=f"(part[i].y)
+                     : "r"(mapa_shared(smem_u32(&s_part[w % warps]), w / warps)));
+    }
+    base = fmaxf(base, part[i].x);
+  }
+  base = warp_max(base);
+  if (base == -INFINITY) base = 0.f;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_ROW_WARPS / 32; ++i) s += part[i].y * ex2(part[i].x - base);
+  s = warp_sum(s);
+  const float log2_s = log2f(s);
+  const bool counts = sh.counts;
+  if (rank == 0 && warp == warps - 1) {
+    float cross = 0.f;  // sum_k p_k log2 q_k
+    for (int k = lane; k < src.K; k += 32)
+      if (e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
+    cross = warp_sum(cross);
+    if (lane == 0) {
+      terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
+      if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+    }
+  }
+  if (g != nullptr) {
+    T* y = g + row * ld_g;
+    const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
+    const float factor = counts ? ex2(own - base) * (scale / s) : 0.f;
+    const bool in_step = static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
+#pragma unroll 2
+    for (int i = lane; i < n; i += 32) {
+      const uint4 in = vec[i];
+      const uint32_t* w = &in.x;
+      uint4 q;
+      uint32_t* o = &q.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (HALF) {
+          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          o[j] = pack_bf16x2(h.x * factor, h.y * factor);
+        } else {
+          o[j] = __float_as_uint(__uint_as_float(w[j]) * factor);
+        }
+      }
+      if (!counts) q = make_uint4(0, 0, 0, 0);  // (whatever the logits were)
+      const int v = v0 + i;
+      if (in_step && v >= whole0 && v < whole1) {
+        *reinterpret_cast<uint4*>(y - lead + static_cast<long long>(v) * VEC) = q;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int at = v * VEC + j - lead;
+          if (at >= 0 && at < vocab) y[at] = reinterpret_cast<const T*>(&q)[j];
+        }
+      }
+    }
+    merge_entries(e, src.K);
+    __syncthreads();
+    const int first = rank * warps * slice * VEC - lead, last = first + warps * slice * VEC;  // the CTA's elements
+    for (int k = threadIdx.x; k < src.K; k += blockDim.x)
+      if (e.sum[k] != -1.f && e.id[k] >= first && e.id[k] < last)
+        y[e.id[k]] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - e.sum[k]));
+  }
+  if (threadIdx.x == 0 && abort_word != 0) {
+    const unsigned long long t0 = globaltimer_ns();  // a copy that may still be under way lands before its memory is given up
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    atomicExch(status, abort_word);
+  }
+  if (ctas > 1) cluster_sync_all();  // the peers have read (M', S')
 }
 
 // ------------------------------------------------------------------------------------------ rows behind the fused product
@@ -219,135 +435,154 @@ struct Prepared {
   const float* at;              // [rows][K]
 };
 
-constexpr int PREPARE_THREADS = 128;
+constexpr int PREPARE_WARPS = 4;  // a row each
 
-// A teacher's entries in the order of their ids (equal ids in their own order), one CTA per row.  An entry's place is the
-// number of those before it: K^2 comparisons of words in shared memory, no barrier between them; a sort of the 64 entries
-// that a row has would take 21 steps with one each.
-__global__ void __launch_bounds__(PREPARE_THREADS)
-    prepare_entries_kernel(const Entries src, int vocab, float tau, int pieces, int* ids, unsigned short* first, float* p, float* p_log_p) {
-  __shared__ RowEntries e;
-  __shared__ int sorted[MAX_ENTRIES];
+// A teacher's entries in the order of their ids (equal ids in their own order), one warp per row.  An entry's place is the
+// number of those before it: K^2 comparisons of words in shared memory without a step that waits for another.
+__global__ void __launch_bounds__(PREPARE_WARPS * 32)
+    prepare_entries_kernel(const Entries src, long long rows, int vocab, float tau, int pieces, int* ids, unsigned short* first, float* p,
+                           float* p_log_p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ RowShared shared[PREPARE_WARPS];
   grid_dep_wait();
   grid_dep_launch();
-  const long long row = blockIdx.x;
-  float plp;
-  load_entries(e, src, row, vocab, tau, plp);
-  if (threadIdx.x == 0) p_log_p[row] = plp;
-  for (int k = threadIdx.x; k < src.K; k += PREPARE_THREADS) sorted[k] = INT32_MAX;
-  __syncthreads();
-  for (int k = threadIdx.x; k < src.K; k += PREPARE_THREADS) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * PREPARE_WARPS + warp;
+  if (row >= rows) return;
+  const RowEntries e(smem + static_cast<size_t>(warp) * ENTRY_BYTES * src.K, src.K);
+  int* sorted = reinterpret_cast<int*>(e.sum);
+  load_entries(e, shared[warp], src, row, vocab, tau);
+  for (int k = lane; k < src.K; k += 32) sorted[k] = INT32_MAX;
+  __syncwarp();
+  if (lane == 0) p_log_p[row] = shared[warp].p_log_p;
+  int n = 0;
+  for (int k = lane; k < src.K; k += 32) {
     const int id = e.id[k];
     if (id < 0) continue;
+    ++n;
     int place = 0;
-    for (int i = 0; i < src.K; ++i) place += static_cast<unsigned>(e.id[i]) < static_cast<unsigned>(id) + (i < k);
+#pragma unroll 8
+    for (int i = 0; i < src.K; ++i)  // (-1 is the largest unsigned)
+      place += static_cast<unsigned>(e.id[i]) < static_cast<unsigned>(id) || (e.id[i] == id && i < k);
     sorted[place] = id;
     ids[row * src.K + place] = id;
     p[row * src.K + place] = e.p[k];
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i <= pieces; i += PREPARE_THREADS) {
-    const long long col = static_cast<long long>(i) * 128;
-    int lo = 0, hi = src.K;  // the first place whose id is at or behind col
+  n = __reduce_add_sync(0xffffffffu, n);
+  __syncwarp();
+  // Where each piece's ids begin: the number of ids before its columns.
+  unsigned short* f = first + row * (pieces + 1);
+  for (int i = lane; i <= pieces; i += 32) {
+    const unsigned col = i == pieces ? 0x7fffffffu : static_cast<unsigned>(i) * 128u;
+    int lo = 0, hi = n;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (sorted[mid] < col || (i == pieces && sorted[mid] != INT32_MAX)) lo = mid + 1;
+      if (static_cast<unsigned>(sorted[mid]) < col) lo = mid + 1;
       else hi = mid;
     }
-    first[row * (pieces + 1) + i] = static_cast<unsigned short>(lo);
+    f[i] = static_cast<unsigned short>(lo);
   }
 }
 
-constexpr int PIECES_PER_CTA = 64;  // at most: 8192 columns
-constexpr int ROWS_PER_CTA = 8;     // a warp's each
+constexpr int PIECES_PER_WARP = 64;  // at most: 8192 columns
+constexpr int ROWS_PER_CTA = 8;      // a warp's each
 
 // From the pieces' statistics the rows': loss, lse, and (GRAD) the gradient of the logits in bf16 in place of the
 // exponentials, which are only multiplied with 2^(M' - M) s tau / S; the rows of x for the weight gradient's product,
-// zeros where a row does not count.  Grid (rows / 8, pieces / per).
+// zeros where a row does not count.  Grid (rows / 8, pieces / per), a row and `per` pieces per warp; the warps have nothing
+// to wait for in one another.
 template <bool GRAD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     softmax_rows_kernel(const float2* stats, long long stats_ld, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
                         int K, const Prepared src, const RowTerms terms, const __nv_bfloat16* x, long long ld_x, __nv_bfloat16* clean,
                         long long ld_clean, int cols) {
-  __shared__ float factor[ROWS_PER_CTA][PIECES_PER_CTA];
-  __shared__ int s_counts[ROWS_PER_CTA];
+  __shared__ float factor[ROWS_PER_CTA][PIECES_PER_WARP];
   grid_dep_wait();
   grid_dep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.x * ROWS_PER_CTA, row = row0 + warp;
+  const int row = blockIdx.x * ROWS_PER_CTA + warp;
+  if (row >= rows) return;
   const int piece0 = blockIdx.y * per, piece1 = min(pieces, piece0 + per);
-  float base = 0.f, S = 0.f, scale = 0.f, over_s = 0.f;
-  bool counts = false;
-  if (row < rows) {
-    float m = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, stats[i * stats_ld + row].x);
-    m = warp_max(m);
-    base = m == -INFINITY ? 0.f : m;
-    for (int i = lane; i < pieces; i += 32) {
-      const float2 v = stats[i * stats_ld + row];
-      S += v.y * ex2(v.x - base);
+  const int target = src.first == nullptr ? src.ids[row] : -1;
+  const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
+  const int entries = src.first == nullptr ? (target >= 0 && target < vocab ? 1 : 0) : first[pieces];
+  const float d_loss = GRAD && terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f;
+  float m = -INFINITY, S = 0.f;
+  for (int i = lane; i < pieces; i += 256) {  // eight loads under way
+    float2 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = i + 32 * j < pieces ? stats[(i + 32 * j) * stats_ld + row] : make_float2(-INFINITY, 0.f);
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, v[j].x);
+    const float from = top == -INFINITY ? 0.f : top;
+    S *= ex2(m - from);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) S += v[j].y * ex2(v[j].x - from);
+    m = top;
+  }
+  const float top = warp_max(m);
+  const float base = top == -INFINITY ? 0.f : top;
+  S = warp_sum(S * ex2(m - base));
+  const float log2_s = log2f(S);
+  const bool counts = entries > 0;
+  if (blockIdx.y == 0) {
+    float cross = 0.f;  // sum_k p_k log2 q_k
+    for (int k = lane; k < entries; k += 32) {
+      const float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
+      if (p != 0.f) cross += p * ((src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
     }
-    S = warp_sum(S);
-    const float log2_s = log2f(S);
-    const int target = src.first == nullptr ? src.ids[row] : -1;
-    const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
-    const int n = src.first == nullptr ? (target >= 0 && target < vocab ? 1 : 0) : first[pieces];
-    counts = n > 0;
-    if (blockIdx.y == 0) {
-      float cross = 0.f;  // sum_k p_k log2 q_k
-      for (int k = lane; k < n; k += 32) {
-        const float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
-        if (p != 0.f) cross += p * ((src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
-      }
-      cross = warp_sum(cross);
-      if (lane == 0) {
-        const float entropy = src.p == nullptr ? 0.f : src.p_log_p[row];
-        terms.loss[row] = counts ? terms.tau * terms.tau * (entropy - LN2 * cross) : 0.f;
-        if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
-      }
-    }
-    if (GRAD) {
-      scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
-      over_s = scale / S;
-      for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i * stats_ld + row].x - base) * over_s;
-      if (lane == 0) s_counts[warp] = counts;
+    cross = warp_sum(cross);
+    if (lane == 0) {
+      const float entropy = src.p == nullptr ? 0.f : src.p_log_p[row];
+      terms.loss[row] = counts ? terms.tau * terms.tau * (entropy - LN2 * cross) : 0.f;
+      if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
     }
   }
   if (!GRAD) return;
-  __syncthreads();
-  const int here = min(ROWS_PER_CTA, rows - row0), vecs = (piece1 - piece0) * 16;  // of 8 columns
-  for (int i = threadIdx.x; i < here * vecs; i += 256) {
-    const int r = i / vecs, v = i - r * vecs;
-    uint4* at = reinterpret_cast<uint4*>(e + (row0 + r) * ld_e + piece0 * 128) + v;
-    const float f = factor[r][v >> 4];
-    uint4 q = *at;
-    uint32_t* w = &q.x;
+  const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f, over_s = scale / S;
+  for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i * stats_ld + row].x - base) * over_s;
+  __syncwarp();
+  uint4* at = reinterpret_cast<uint4*>(e + row * ld_e + piece0 * 128);
+  const int vecs = (piece1 - piece0) * 16;  // of 8 columns
+  constexpr int DEEP = 4;
+  for (int v = lane; v < vecs; v += 32 * DEEP) {
+    uint4 q[DEEP];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-      w[j] = pack_bf16x2(h.x * f, h.y * f);
+    for (int d = 0; d < DEEP; ++d)
+      if (v + 32 * d < vecs) q[d] = at[v + 32 * d];
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      if (v + 32 * d >= vecs) break;
+      const float f = factor[warp][(v + 32 * d) >> 4];
+      uint32_t* w = &q[d].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        w[j] = pack_bf16x2(h.x * f, h.y * f);
+      }
+      at[v + 32 * d] = counts ? q[d] : make_uint4(0, 0, 0, 0);  // (whatever the logits were)
     }
-    *at = s_counts[r] ? q : make_uint4(0, 0, 0, 0);
   }
-  if (clean != nullptr && blockIdx.y == 0) {
-    const int per_row = (cols + 7) / 8;
-    for (int i = threadIdx.x; i < here * per_row; i += 256) {
-      const int r = i / per_row, c = (i - r * per_row) * 8;
-      const __nv_bfloat16* from = x + (row0 + r) * ld_x + c;
-      __nv_bfloat16* to = clean + (row0 + r) * ld_clean + c;
-      if (c + 8 <= cols) {
-        *reinterpret_cast<uint4*>(to) = s_counts[r] ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+  if (clean != nullptr) {  // the splits share the row of x
+    const int per_row = (cols + 7) / 8, share = (per_row + gridDim.y - 1) / gridDim.y;
+    const int c1 = min(per_row, static_cast<int>(blockIdx.y + 1) * share);
+    for (int i = blockIdx.y * share + lane; i < c1; i += 32) {
+      const __nv_bfloat16* from = x + row * ld_x + i * 8;
+      __nv_bfloat16* to = clean + row * ld_clean + i * 8;
+      if (i * 8 + 8 <= cols) {
+        *reinterpret_cast<uint4*>(to) = counts ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
       } else {
-        for (int j = 0; c + j < cols; ++j) to[j] = s_counts[r] ? from[j] : __float2bfloat16_rn(0.f);
+        for (int j = 0; i * 8 + j < cols; ++j) to[j] = counts ? from[j] : __float2bfloat16_rn(0.f);
       }
     }
   }
-  __syncthreads();
+  __syncwarp();
   // The entries of these columns, each id once: the sum of its entries' probabilities, in their order.
   if (!counts) return;
   int k0 = 0, k1 = 1;
   if (src.first != nullptr) {
-    const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
     k0 = first[piece0];
     k1 = first[piece1];
   }
@@ -376,19 +611,40 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// out[r, c] = sum[r, c] (+ out[r, c]): the end of a gradient that is summed in f32 scratch; sum = nullptr: zeros.
-template <typename T>
+// out[r, c] = sum[r, c] (+ out[r, c]): the end of a gradient that is summed in f32 scratch; sum = nullptr: zeros.  A thread
+// has eight columns of a row, by vectors where out's rows allow them (sum's always do).
+template <typename T, bool VECTORS>
 __global__ void __launch_bounds__(256)
     finish_kernel(const float* sum, long long ld, T* out, long long o_row, long long o_col, long long rows, int cols, int add) {
-  const long long per_row = (cols + 255) / 256;
-  for (long long b = blockIdx.x; b < rows * per_row; b += gridDim.x) {
-    const long long r = b / per_row;
-    const int c = static_cast<int>(b - r * per_row) * 256 + threadIdx.x;
-    if (c >= cols) continue;
-    float v = sum != nullptr ? sum[r * ld + c] : 0.f;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int per_row = (cols + 7) / 8;
+  const long long all = rows * per_row, step = static_cast<long long>(gridDim.x) * 256;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
+    const long long r = i / per_row;
+    const int c = static_cast<int>(i - r * per_row) * 8;
+    float v[8] = {};
+    if (sum != nullptr) {  // (its rows are padded to whole vectors)
+      const float4 lo = *reinterpret_cast<const float4*>(sum + r * ld + c), hi = *reinterpret_cast<const float4*>(sum + r * ld + c + 4);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    }
     T* o = out + r * o_row + c * o_col;
-    if (add) v += to_f32(*o);
-    *o = from_f32<T>(v);
+    if (VECTORS && c + 8 <= cols) {
+      if (add) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += to_f32(o[j]);
+      }
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      } else {
+        *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < cols) o[j * o_col] = from_f32<T>(add ? v[j] + to_f32(o[j * o_col]) : v[j]);
+    }
   }
 }
 
@@ -418,18 +674,67 @@ static RowTerms from_row(RowTerms t, long long row) {
   return t;
 }
 
-static int32_t launch_rows(const void* z, int32_t z_type, long long ld_z, void* g, int32_t g_type, long long ld_g, long long rows,
-                           int vocab, const Entries& e, const RowTerms& t, cudaStream_t stream) {
-  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (dtype_size(z_type) + (g ? dtype_size(g_type) : 0)), stream);
-  const unsigned grid = static_cast<unsigned>(rows);
-  using bf = __nv_bfloat16;
-  if (z_type == CDL_BF16)
-    loss_row_kernel<bf, bf><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const bf*>(z), ld_z, static_cast<bf*>(g), ld_g, vocab, e, t);
-  else if (g_type == CDL_BF16)
-    loss_row_kernel<float, bf><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const float*>(z), ld_z, static_cast<bf*>(g), ld_g, vocab, e, t);
-  else
-    loss_row_kernel<float, float><<<grid, ROW_THREADS, 0, stream>>>(static_cast<const float*>(z), ld_z, static_cast<float*>(g), ld_g, vocab, e, t);
-  CDL_CUDA(cudaGetLastError());
+// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and more, 16 for each of as many CTAs as keep
+// three shares on an SM.  More CTAs share those warps while SMs are without one and a warp's slice stays above 2 KB.
+// warps = 0: rows of over 1.6 MB, which are read twice.
+static Share choose_share(long long rows, int vocab, int size, int K) {
+  const int vec = 16 / size;
+  const long long vecs = up(vocab + vec - 1, vec) / vec, entry = static_cast<long long>(ENTRY_BYTES) * K;
+  Share s = {};
+  s.warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : 16;
+  s.ctas = 1;
+  auto slice = [&] { return up(vecs, s.warps) / s.warps; };
+  auto bytes = [&] { return s.warps / s.ctas * slice() * 16 + entry; };
+  while (s.ctas < 8 && bytes() > SHARE_BYTES) {
+    s.ctas *= 2;
+    s.warps = 16 * s.ctas;
+  }
+  if (bytes() > 200 * 1024) return {};
+  s.vecs = static_cast<int>(slice());
+  while (s.ctas < 8 && rows * s.ctas < sm_count() && s.warps / s.ctas >= 2 && s.vecs >= 128) s.ctas *= 2;
+  s.smem = static_cast<size_t>(bytes());
+  return s;
+}
+
+template <typename T>
+static int32_t launch_rows(const void* z, long long ld_z, void* g, long long ld_g, long long rows, int vocab, const Entries& e,
+                           const RowTerms& t, cudaStream_t stream) {
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * sizeof(T) * (g ? 2 : 1), stream);
+  const Share share = choose_share(rows, vocab, sizeof(T), e.K);
+  if (share.warps == 0 || rows * share.ctas > INT32_MAX) {
+    CDL_CUDA(launch_pdl(loss_row_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(z),
+                        ld_z, static_cast<T*>(g), ld_g, vocab, e, t));
+    return CDL_OK;
+  }
+  static std::once_flag once[64];
+  int dev = 0;
+  CDL_CUDA(cudaGetDevice(&dev));
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    err = cudaFuncSetAttribute(loss_share_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  });
+  if (err != cudaSuccess) return fail(CDL_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(err));
+  int* status = device_status_ptr();
+  if (!status) return fail(CDL_ERR_CUDA, "cannot resolve the device status word");
+  CDL_CUDA(launch_pdl_cluster(loss_share_kernel<T>, dim3(static_cast<unsigned>(rows * share.ctas)), dim3(share.warps / share.ctas * 32),
+                              share.smem, share.ctas, stream, static_cast<const T*>(z), ld_z, static_cast<T*>(g), ld_g, vocab,
+                              share.vecs, share.ctas, e, t, status));
+  return CDL_OK;
+}
+
+static int32_t prepare_entries(const Entries& e, long long rows, int vocab, float tau, int pieces, int* ids, unsigned short* first, float* p,
+                               float* p_log_p, cudaStream_t stream) {
+  static std::once_flag once[64];
+  int dev = 0;
+  CDL_CUDA(cudaGetDevice(&dev));
+  cudaError_t err = cudaSuccess;
+  constexpr size_t row_bytes = static_cast<size_t>(PREPARE_WARPS) * ENTRY_BYTES;
+  std::call_once(once[dev & 63], [&] {
+    err = cudaFuncSetAttribute(prepare_entries_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(row_bytes * MAX_ENTRIES));
+  });
+  if (err != cudaSuccess) return fail(CDL_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(err));
+  CDL_CUDA(launch_pdl(prepare_entries_kernel, dim3(static_cast<unsigned>((rows + PREPARE_WARPS - 1) / PREPARE_WARPS)),
+                      dim3(PREPARE_WARPS * 32), row_bytes * e.K, stream, e, rows, vocab, tau, pieces, ids, first, p, p_log_p));
   return CDL_OK;
 }
 
@@ -452,16 +757,21 @@ static int32_t copy(const cdl_tensor& src, void* dst, long long ld, const float*
   return CDL_OK;
 }
 
-static int32_t finish(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
-  const long long rows = out.shape[0], cols = out.shape[1];
-  if (out.dtype == CDL_BF16)
-    finish_kernel<__nv_bfloat16><<<copy_grid(rows, cols), 256, 0, stream>>>(
-        sum, ld, static_cast<__nv_bfloat16*>(out.ptr), out.stride[0], out.stride[1], rows, static_cast<int>(cols), add);
-  else
-    finish_kernel<float><<<copy_grid(rows, cols), 256, 0, stream>>>(sum, ld, static_cast<float*>(out.ptr), out.stride[0],
-                                                                  out.stride[1], rows, static_cast<int>(cols), add);
-  CDL_CUDA(cudaGetLastError());
+template <typename T>
+static int32_t finish_as(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
+  const long long rows = out.shape[0], cols = out.shape[1], blocks = (rows * ((cols + 7) / 8) + 255) / 256, most = 16LL * sm_count();
+  const bool vectors = out.stride[1] == 1 && (reinterpret_cast<uintptr_t>(out.ptr) & 15) == 0 && (rows == 1 || out.stride[0] % 8 == 0);
+  auto run = [&](auto kernel) {
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, stream, sum, ld,
+                      static_cast<T*>(out.ptr), static_cast<long long>(out.stride[0]), static_cast<long long>(out.stride[1]), rows,
+                      static_cast<int>(cols), add);
+  };
+  CDL_CUDA(vectors ? run(finish_kernel<T, true>) : run(finish_kernel<T, false>));
   return CDL_OK;
+}
+static int32_t finish(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(out.shape[0]) * out.shape[1] * (4 + dtype_size(out.dtype)), stream);
+  return out.dtype == CDL_BF16 ? finish_as<__nv_bfloat16>(sum, ld, out, add, stream) : finish_as<float>(sum, ld, out, add, stream);
 }
 
 // ------------------------------------------------------------------------------------------ checks
@@ -537,12 +847,12 @@ static int32_t distillation_execute(const cdl_head_loss_desc* desc, const cdl_te
   }
   if (T == 0) return CDL_OK;
   if (V == 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
-  return launch_rows(logits->ptr, logits->dtype, logits->stride[0], d_logits ? d_logits->ptr : nullptr, logits->dtype,
-                     d_logits ? d_logits->stride[0] : 0, T, static_cast<int>(V), e, terms, stream);
+  auto rows = logits->dtype == CDL_BF16 ? launch_rows<__nv_bfloat16> : launch_rows<float>;
+  return rows(logits->ptr, logits->stride[0], d_logits ? d_logits->ptr : nullptr, d_logits ? d_logits->stride[0] : 0, T,
+              static_cast<int>(V), e, terms, stream);
 }
 
 // ------------------------------------------------------------------------------------------ from the hidden states
-static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
 
 // Where a product's operand is read: its own place, or scratch that it is copied to (bf16: rows on the 16-byte grid).
 static bool readable(const cdl_tensor& t) {
@@ -708,11 +1018,11 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
   unsigned short* first = reinterpret_cast<unsigned short*>(base + p.at_first);
   const Prepared src = teacher ? Prepared{ids, e.K, first, probs, p_log_p, at} : Prepared{e.ids, e.ids_ld, nullptr, nullptr, nullptr, at};
   if (teacher)
-    CDL_CUDA(launch_pdl(prepare_entries_kernel, dim3(rows), dim3(PREPARE_THREADS), 0, stream, e, vocab, t.tau, p.pieces, ids, first, probs, p_log_p));
+    CDL_CHECK(prepare_entries(e, rows, vocab, t.tau, p.pieces, ids, first, probs, p_log_p, stream));
   void* out = grad ? base + p.at_g : nullptr;
   CDL_CHECK(matmul_exp_execute(&x, &w, LOG2E / t.tau, out, p.ld_g, {stats, p.chunk, src.ids, src.ids_ld, src.first, at}, stream));
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (grad ? 4 : 0) + 8.0 * rows * p.pieces, stream);
-  const dim3 block(256);
+  const dim3 block(ROWS_PER_CTA * 32);
   const unsigned row_ctas = (rows + ROWS_PER_CTA - 1) / ROWS_PER_CTA;
   auto run = [&](auto kernel, unsigned splits, int per) {
     return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, p.chunk, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
@@ -724,7 +1034,7 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
     CDL_CUDA(run(softmax_rows_kernel<false>, 1, p.pieces));
     return CDL_OK;
   }
-  int per = PIECES_PER_CTA;  // fewer where that leaves SMs without a CTA
+  int per = PIECES_PER_WARP;  // fewer where that leaves SMs without a CTA
   while (per > 8 && row_ctas * ((p.pieces + per - 1) / per) < 2u * sm_count()) per /= 2;
   CDL_CUDA(run(softmax_rows_kernel<true>, (p.pieces + per - 1) / per, per));
   return CDL_OK;
@@ -784,7 +1094,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
     } else {
       const cdl_tensor z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_z);
       CDL_CHECK(matmul_execute(&xc, &w, nullptr, &z, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
-      CDL_CHECK(launch_rows(z.ptr, CDL_F32, p.ld_z, grad ? g.ptr : nullptr, type, p.ld_g, n, static_cast<int>(p.V), e, t, stream));
+      CDL_CHECK(launch_rows<float>(z.ptr, p.ld_z, grad ? g.ptr : nullptr, p.ld_g, n, static_cast<int>(p.V), e, t, stream));
       if (p.has_dw) {
         float* keep = reinterpret_cast<float*>(base + p.at_keep);
         keep_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(e, n, static_cast<int>(p.V), keep);
@@ -800,7 +1110,9 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       const bool add = row > 0 || (!p.sums && desc->accumulate_dw);
       const cdl_tensor gt = transposed(g), xt = transposed(clean), sum_t = transposed(sum);
       const cdl_tensor *a = dw_columns ? &gt : &xt, *b = dw_columns ? &clean : &g, *d = dw_columns ? &sum_t : &sum;
-      CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes));
+      // (beside dx's product, whose last wave leaves SMs idle: the two share what they read alone)
+      CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
+                               fused && p.has_dx ? 1 : 0));
     }
   }
   if (p.sums) {

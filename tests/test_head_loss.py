@@ -69,7 +69,10 @@ def _check_distillation(cdl, logits, ids, teacher, tau, d_loss=None, grad_scale=
     _close("loss", o.loss, loss, e_loss)
     p_err = _stat(vocab) + 2.0 ** -22 * (1 + lse.abs() + top)[:, None]
     s = (tau * scale.abs())[:, None]
-    tol = HALF[logits.dtype] * grad.abs() + 2 * p_err * (grad.abs() + 2.0 ** -10 * s) + 2.0 ** -19 * s * _hit(ids, vocab)
+    # bf16: the exponentials stand in f16 in between, half a step of which is 2^-11 of the value, or 2^-40 of the row's
+    # largest: (1 + 2^-11)(1 + 2^-8) - 1 = 2^-8 + 2^-11 + 2^-19.
+    half = HALF[logits.dtype] + (2.0 ** -11 + 2.0 ** -19 if logits.dtype == BF16 else 0.0)
+    tol = half * grad.abs() + 2.0 ** -40 * s + 2 * p_err * (grad.abs() + 2.0 ** -10 * s) + 2.0 ** -19 * s * _hit(ids, vocab)
     _close("d_logits", o.d_logits, grad, tol + 1e-38)
     return o
 
@@ -92,7 +95,9 @@ def _hit(ids, vocab):
 @pytest.mark.parametrize("rows,vocab,k,tau,dtype,pad", [
     (1, 1, 1, 1.0, F32, 0), (3, 7, 3, 2.0, BF16, 1), (1, 1000, 1, 1.0, BF16, 0), (37, 4099, 5, 0.7, BF16, 3), (5, 4099, 64, 3.0, F32, 0),
     (64, 8192, 33, 2.0, BF16, 16), (9, 32768, 64, 2.0, BF16, 0), (6, 32768, 300, 4.0, F32, 8), (4, 50001, 1024, 1.0, BF16, 0),
-    (3, 150000, 20, 1.5, BF16, 0), (3, 150001, 20, 1.5, F32, 2), (17, 129, 129, 1.0, F32, 0), (300, 2048, 16, 1.0, BF16, 0)])
+    (3, 150000, 20, 1.5, BF16, 0), (3, 150001, 20, 1.5, F32, 2), (17, 129, 129, 1.0, F32, 0), (300, 2048, 16, 1.0, BF16, 0),
+    (700, 1003, 3, 1.0, BF16, 0), (200, 36861, 9, 1.0, BF16, 0), (2, 900001, 8, 1.0, BF16, 0), (2, 450001, 8, 2.0, F32, 0),
+    (2, 400000, 1024, 2.0, F32, 4), (160, 2, 2, 1.0, BF16, 0), (160, 9, 4, 1.0, F32, 1)])
 def test_distillation(cdl, gpu_ok, rows, vocab, k, tau, dtype, pad):
     gen = torch.Generator(device="cuda").manual_seed(rows * 7 + vocab)
     _, logits = _logits(gen, rows, vocab, dtype, pad)
