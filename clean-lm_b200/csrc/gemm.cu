@@ -593,7 +593,7 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, uint32_t t_
       if (p.d != nullptr) st_global_v8(dp + c * 32 + g * 16, w);
     }
   }
-  p.exp.stats[(col_base >> 7) * p.exp.stats_ld + row] = make_float2(m == -INFINITY ? -INFINITY : base, (s[0] + s[1]) + (s[2] + s[3]));
+  p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] = make_float2(m == -INFINITY ? -INFINITY : base, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -820,8 +820,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   // operands, 46 MB of f32 output read and written): numbered tile by tile (a wave = three slices
   // of ~25 tiles, which share nothing) 693 MB read + 42 MB written; slice by slice over all tiles
   // 525 + 75 MB (every slice pass brings all of D back).
-  auto unit_range = [&](int unit, int& tile, int& kb0, int& kb1) {
-    int slice;
+  auto unit_range = [&](int unit, int& tile, int& slice, int& kb0, int& kb1) {
     if (p.split_k == 1) {
       tile = unit;
       slice = 0;
@@ -909,8 +908,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         if (unit_u == SCHED_DONE) break;
         const int unit = static_cast<int>(unit_u);
-        int tile, kb0, kb1, b, tm, tn;
-        unit_range(unit, tile, kb0, kb1);
+        int tile, slice, kb0, kb1, b, tm, tn;
+        unit_range(unit, tile, slice, kb0, kb1);
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * PAIR_M + static_cast<int>(rank) * BM;
         const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
@@ -959,8 +958,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t unit_u = bars->unit_ring[slot];
         if (unit_u == SCHED_DONE) break;
         const int unit = static_cast<int>(unit_u);
-        int tile, kb0, kb1;
-        unit_range(unit, tile, kb0, kb1);
+        int tile, slice, kb0, kb1;
+        unit_range(unit, tile, slice, kb0, kb1);
         const int acc = t & 1;
         const uint32_t acc_ph = (t >> 1) & 1;
         if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 211)) break;
@@ -1007,8 +1006,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const uint32_t unit_u = bars->unit_ring[slot];
       if (unit_u == SCHED_DONE) break;
       const int unit = static_cast<int>(unit_u);
-      int tile, kb0, kb1, b, tm, tn;
-      unit_range(unit, tile, kb0, kb1);
+      int tile, slice, kb0, kb1, b, tm, tn;
+      unit_range(unit, tile, slice, kb0, kb1);
       tile_coords(p, tile, b, tm, tn);
       const int acc = t & 1;
       const uint32_t acc_ph = (t >> 1) & 1;
@@ -1029,7 +1028,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         store_tile_rows_exp(p, t_row, row, col, want);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
-        else store_tile_rows(p, t_row, b, row, col);
+        else store_tile_rows(p, t_row, p.planes ? slice : b, row, col);
       }
       tc_fence_before();
       __syncwarp();
@@ -1431,6 +1430,7 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   p.beta = use_c ? beta : 0.0f;
   p.split_k = use_cluster ? cluster_splits : 1;
   p.sched_counter = nullptr;
+  p.planes = 0;
   p.atomic_out = 0;
   p.tma_add = 0;
   p.early = (early & EARLY_PRODUCTS) ? (use_pair ? 2 : 0) : early > 0 ? 1 : 0;
@@ -1574,27 +1574,22 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   return CDL_OK;
 }
 
-// The logits of a loss (see store_tile_rows_exp): always CTA pairs.  With few rows a pair's second half has none, but the
-// columns of B are what such a product reads, and they are loaded as fast.
-int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
-                           cudaStream_t stream) {
+// The pair kernel's operands of a plain product of bf16 tensors on the 16-byte grid.
+static int32_t pair_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Params& p, CUtensorMap* tm_a, CUtensorMap* tm_b) {
   using namespace gemm;
   const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
   OperandLayout la, lb;
-  CDL_CHECK(analyze_operand("x", a, true, &la));
-  CDL_CHECK(analyze_operand("w", b, false, &lb));
-  CUtensorMap tm_a, tm_b;
-  {
-    const uint64_t da[3] = {static_cast<uint64_t>(la.mn_major ? M : K), static_cast<uint64_t>(la.mn_major ? K : M), 1};
-    const uint64_t db[3] = {static_cast<uint64_t>(lb.mn_major ? N : K), static_cast<uint64_t>(lb.mn_major ? K : N), 1};
-    const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(la.ld) * da[1] * 2};
-    const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(lb.ld) * db[1] * 2};
-    const uint32_t ba[3] = {64, static_cast<uint32_t>(la.mn_major ? 64 : BM), 1};
-    const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : BN / 2), 1};
-    CDL_CHECK(encode_tmap(&tm_a, a->ptr, CDL_BF16, 3, da, sa, ba, true));
-    CDL_CHECK(encode_tmap(&tm_b, b->ptr, CDL_BF16, 3, db, sb, bb, true));
-  }
-  Params p = {};
+  CDL_CHECK(analyze_operand("a", a, true, &la));
+  CDL_CHECK(analyze_operand("b", b, false, &lb));
+  const uint64_t da[3] = {static_cast<uint64_t>(la.mn_major ? M : K), static_cast<uint64_t>(la.mn_major ? K : M), 1};
+  const uint64_t db[3] = {static_cast<uint64_t>(lb.mn_major ? N : K), static_cast<uint64_t>(lb.mn_major ? K : N), 1};
+  const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(la.ld) * da[1] * 2};
+  const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(lb.ld) * db[1] * 2};
+  const uint32_t ba[3] = {64, static_cast<uint32_t>(la.mn_major ? 64 : BM), 1};
+  const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : BN / 2), 1};
+  CDL_CHECK(encode_tmap(tm_a, a->ptr, CDL_BF16, 3, da, sa, ba, true));
+  CDL_CHECK(encode_tmap(tm_b, b->ptr, CDL_BF16, 3, db, sb, bb, true));
+  p = {};
   p.M = static_cast<int>(M);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
@@ -1602,28 +1597,76 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
   p.num_m_tiles = static_cast<int>((M + PAIR_M - 1) / PAIR_M);
   p.num_n_tiles = static_cast<int>((N + BN - 1) / BN);
   const long long tiles = static_cast<long long>(p.num_m_tiles) * p.num_n_tiles;
-  if (tiles > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "matmul: too many tiles");
+  if (tiles > INT32_MAX / 64) return fail(CDL_ERR_UNSUPPORTED, "matmul: too many tiles");
   p.num_tiles = static_cast<int>(tiles);
   p.k_blocks = static_cast<int>((K + BK - 1) / BK);
   p.raster_w = RASTER_W;
   p.a_mn = la.mn_major;
   p.b_mn = lb.mn_major;
+  p.alpha = 1.f;
+  p.split_k = 1;
+  p.status = device_status_ptr();
+  return p.status ? CDL_OK : fail(CDL_ERR_CUDA, "cannot resolve the device status word");
+}
+
+template <int KIND>
+static int32_t pair_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtensorMap& tm_b, cudaStream_t stream) {
+  using namespace gemm;
+  int held = 0;
+  CDL_CHECK(prepare_kernels(&held));
+  const int units = p.num_tiles * p.split_k, clusters = units < held ? units : held;
+  p.sched_counter = units > clusters ? sched_counter_for(gemm_counter_kind(0), current_device(), stream) : nullptr;
+  ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(p.M) * p.N * p.K, stream);
+  CDL_CUDA(launch_pdl(gemm_bf16_pair_kernel<KIND>, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(KIND), stream, tm_a, tm_b, tm_a,
+                      tm_a, p));
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+// The logits of a loss (see store_tile_rows_exp): always CTA pairs.  With few rows a pair's second half has none, but the
+// columns of B are what such a product reads, and they are loaded as fast.
+int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
+                           cudaStream_t stream) {
+  gemm::Params p;
+  CUtensorMap tm_a, tm_b;
+  CDL_CHECK(pair_operands(a, b, p, &tm_a, &tm_b));
   p.d = d;
   p.ldd = ldd;
   p.alpha = scale;
-  p.split_k = 1;
-  p.exp = {out.stats, out.stats_ld, out.ids, out.ids_ld, out.first, out.at, static_cast<int>((N + 127) / 128)};
-  p.status = device_status_ptr();
-  if (!p.status) return fail(CDL_ERR_CUDA, "cannot resolve the device status word");
-  int held = 0;
-  CDL_CHECK(prepare_kernels(&held));
-  const int clusters = tiles < held ? static_cast<int>(tiles) : held;
-  p.sched_counter = tiles > clusters ? sched_counter_for(gemm_counter_kind(0), current_device(), stream) : nullptr;
-  ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(M) * N * K, stream);
-  CDL_CUDA(launch_pdl(gemm_bf16_pair_kernel<STORE_EXP>, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(STORE_EXP), stream, tm_a,
-                      tm_b, tm_a, tm_a, p));
-  CDL_CUDA(cudaGetLastError());
-  return CDL_OK;
+  p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
+  return pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
+}
+
+// K slices of a product whose output is small and whose K is long (dx of a head: K is the vocabulary), each stored in f32 in
+// a plane of its own, to be summed in their order.  Estimated in microseconds as in choose_cluster_splits: 0.28 per K
+// block, 4 per unit's store and set-up, a plane's way out and back at 5 TB/s and 3 for the kernel that sums them.
+int matmul_plane_slices(long long M, long long N, long long K) {
+  using namespace gemm;
+  const long long tiles = ((M + PAIR_M - 1) / PAIR_M) * ((N + BN - 1) / BN), k_blocks = (K + BK - 1) / BK, pairs = sm_count() / 2;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= MAX_PLANES && (s == 1 || s * 8 <= k_blocks); ++s) {
+    const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
+    double t = waves * (0.28 * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
+    if (s > 1) t = 1.05 * (t + 3.0 + 8e-6 * static_cast<double>(s) * M * N / 5.0);
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream) {
+  gemm::Params p;
+  CUtensorMap tm_a, tm_b;
+  CDL_CHECK(pair_operands(a, b, p, &tm_a, &tm_b));
+  p.d = planes;
+  p.ldd = ld;
+  p.d_batch = ld * p.M;
+  p.out_f32 = p.d_vec = p.wide = p.planes = 1;  // (rows of whole 32 bytes)
+  p.split_k = slices;
+  return pair_launch<gemm::STORE>(p, tm_a, tm_b, stream);
 }
 
 }  // namespace cdl

@@ -10,8 +10,7 @@ constexpr int RASTER_W = 8;  // N tiles per raster panel (upper bound; see Param
 
 // The store of the losses' logits (pair kernel): see store_tile_rows_exp in gemm.cu.  A piece is 128 columns.
 struct ExpStore {
-  float2* stats;  // [pieces][stats_ld]: (M', S') of every row and piece
-  long long stats_ld;
+  float2* stats;  // [rows][pieces]: (M', S') of every row and piece
   const int* ids;  // the columns whose t is wanted besides: [rows][ids_ld], ascending
   long long ids_ld;
   const unsigned short* first;  // [rows][pieces + 1]: a row's first id at or behind a piece's columns; nullptr: one id, not sorted
@@ -33,6 +32,7 @@ struct Params {
   int split_k;     // K slices per tile (pair kernel: accumulate-in-place form only; cluster kernels: CTAs
                    // per cluster); 1 = none
   int sum_blocks;  // gemm_general.cu: K blocks that one tensor-core accumulator sums up
+  int planes;      // 1 = K slice s is stored at d + s d_batch (pair kernel)
   int atomic_out;  // 1 = add alpha * partial into D with red.global.add (D already holds C)
   int tma_add;     // 1 = the pair kernel adds by TMA reductions (add_chunk)
   // Fused SwiGLU epilogues (bf16 [M, N] operands, 16-byte aligned rows):

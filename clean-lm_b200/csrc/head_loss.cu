@@ -493,7 +493,7 @@ constexpr int ROWS_PER_CTA = 8;      // a warp's each
 // to wait for in one another.
 template <bool GRAD>
 __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
-    softmax_rows_kernel(const float2* stats, long long stats_ld, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
+    softmax_rows_kernel(const float2* stats, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
                         int K, const Prepared src, const RowTerms terms, const __nv_bfloat16* x, long long ld_x, __nv_bfloat16* clean,
                         long long ld_clean, int cols) {
   __shared__ float factor[ROWS_PER_CTA][PIECES_PER_WARP];
@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * ROWS_PER_CTA + warp;
   if (row >= rows) return;
+  stats += static_cast<long long>(row) * pieces;
   const int piece0 = blockIdx.y * per, piece1 = min(pieces, piece0 + per);
   const int target = src.first == nullptr ? src.ids[row] : -1;
   const unsigned short* first = src.first + static_cast<long long>(row) * (pieces + 1);
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     float2 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      v[j] = i + 32 * j < pieces ? stats[(i + 32 * j) * stats_ld + row] : make_float2(-INFINITY, 0.f);
+      v[j] = i + 32 * j < pieces ? stats[i + 32 * j] : make_float2(-INFINITY, 0.f);
     float top = m;
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, v[j].x);
@@ -542,11 +543,11 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
   }
   if (!GRAD) return;
   const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f, over_s = scale / S;
-  for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i * stats_ld + row].x - base) * over_s;
+  for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i].x - base) * over_s;
   __syncwarp();
   uint4* at = reinterpret_cast<uint4*>(e + row * ld_e + piece0 * 128);
   const int vecs = (piece1 - piece0) * 16;  // of 8 columns
-  constexpr int DEEP = 4;
+  constexpr int DEEP = 2;  // (4 and 8: the same to 2 % more)
   for (int v = lane; v < vecs; v += 32 * DEEP) {
     uint4 q[DEEP];
 #pragma unroll
@@ -645,6 +646,32 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < 8; ++j)
         if (c + j < cols) o[j * o_col] = from_f32<T>(add ? v[j] + to_f32(o[j * o_col]) : v[j]);
     }
+  }
+}
+
+// out[r, c] = the planes' sum at r, c, in their order.
+__global__ void __launch_bounds__(256)
+    sum_planes_kernel(const float* planes, long long ld, int slices, __nv_bfloat16* out, long long ld_out, int rows, int cols, int vectors) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int per_row = (cols + 7) / 8;
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, r = i / per_row;
+  if (r >= rows) return;
+  const int c = static_cast<int>(i - r * per_row) * 8;
+  const float* from = planes + r * ld + c;
+  float v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < slices; ++s, from += rows * ld) {
+    const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+    v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w; v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+  }
+  __nv_bfloat16* o = out + r * ld_out + c;
+  if (vectors && c + 8 <= cols) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) o[j] = __float2bfloat16_rn(v[j]);
   }
 }
 
@@ -877,6 +904,8 @@ struct Linear {
   // bf16: the product writes statistics and exponentials (at_g), not logits
   int pieces, K;
   size_t at_stats, at_ids, at_first, at_p, at_p_log_p, at_at;
+  int slices;  // of dx's product, in f32 planes
+  size_t at_planes;
 };
 
 // A view of `rows` rows from `row`.
@@ -943,6 +972,8 @@ static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long 
   p.at_p = take(fused && teacher, n * p.K * 4);
   p.at_p_log_p = take(fused && teacher, n * 4);
   p.at_first = take(fused && teacher, n * (p.pieces + 1) * 2);
+  p.slices = fused && p.has_dx ? matmul_plane_slices(p.chunk, p.D, p.V) : 1;
+  p.at_planes = take(p.slices > 1, static_cast<size_t>(p.slices) * n * x_ld * 4);
   p.at_clean = take(p.has_dw, static_cast<size_t>(p.chunk) * x_ld * es);
   p.at_keep = take(!fused && p.has_dw, static_cast<size_t>(p.chunk) * 4);
   p.at_sum = take(p.sums, static_cast<size_t>(columns_first(p.dw) ? p.V : p.D) * p.ld_sum * 4);
@@ -1020,12 +1051,12 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
   if (teacher)
     CDL_CHECK(prepare_entries(e, rows, vocab, t.tau, p.pieces, ids, first, probs, p_log_p, stream));
   void* out = grad ? base + p.at_g : nullptr;
-  CDL_CHECK(matmul_exp_execute(&x, &w, LOG2E / t.tau, out, p.ld_g, {stats, p.chunk, src.ids, src.ids_ld, src.first, at}, stream));
+  CDL_CHECK(matmul_exp_execute(&x, &w, LOG2E / t.tau, out, p.ld_g, {stats, src.ids, src.ids_ld, src.first, at}, stream));
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (grad ? 4 : 0) + 8.0 * rows * p.pieces, stream);
   const dim3 block(ROWS_PER_CTA * 32);
   const unsigned row_ctas = (rows + ROWS_PER_CTA - 1) / ROWS_PER_CTA;
   auto run = [&](auto kernel, unsigned splits, int per) {
-    return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, p.chunk, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
+    return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
                       vocab, p.pieces, per, e.K, src, t, static_cast<const __nv_bfloat16*>(x.ptr), static_cast<long long>(x.stride[0]),
                       p.has_dw ? static_cast<__nv_bfloat16*>(clean.ptr) : nullptr, static_cast<long long>(clean.stride[0]),
                       static_cast<int>(p.D));
@@ -1102,8 +1133,11 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
         CDL_CHECK(copy(xc, clean.ptr, x_ld, keep, stream));
       }
     }
-    if (p.has_dx) {
-      const cdl_tensor d = rows_of(p.dx, row, n);
+    const cdl_tensor d = p.has_dx ? rows_of(p.dx, row, n) : cdl_tensor{};
+    float* planes = reinterpret_cast<float*>(base + p.at_planes);
+    if (p.slices > 1) {
+      CDL_CHECK(matmul_planes_execute(&g, &wt, planes, x_ld, p.slices, stream));
+    } else if (p.has_dx) {
       CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
     }
     if (p.has_dw) {
@@ -1113,6 +1147,13 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       // (beside dx's product, whose last wave leaves SMs idle: the two share what they read alone)
       CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
                                fused && p.has_dx ? 1 : 0));
+    }
+    if (p.slices > 1) {
+      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 15) == 0 && (n == 1 || d.stride[0] % 8 == 0);
+      ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(n) * p.D * (4 * p.slices + 2), stream);
+      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * (x_ld / 8) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
+                          p.slices, static_cast<__nv_bfloat16*>(d.ptr), static_cast<long long>(d.stride[0]), static_cast<int>(n),
+                          static_cast<int>(p.D), vectors ? 1 : 0));
     }
   }
   if (p.sums) {

@@ -47,8 +47,7 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
 // The logits of a loss, t = scale * (A . B), of which statistics, exponentials and single values are stored (bf16 operands
 // on the 16-byte grid; see store_tile_rows_exp in gemm.cu).
 struct ExpOutputs {
-  float2* stats;  // [pieces of 128 columns][stats_ld]
-  long long stats_ld;
+  float2* stats;  // [rows][pieces of 128 columns]
   const int* ids;  // columns whose t is stored besides, [rows][ids_ld]; nullptr: none
   long long ids_ld;
   const unsigned short* first;  // [rows][pieces + 1], nullptr: one id per row
@@ -57,6 +56,11 @@ struct ExpOutputs {
 // d: f16 [rows, ldd], 32-byte aligned, ldd a multiple of 128 that holds all columns; nullptr: no exponentials.
 int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
                            cudaStream_t stream);
+// A product of bf16 tensors on the 16-byte grid in K slices: slice s is stored at planes + s M ld (f32, 32-byte aligned, ld >= N a
+// multiple of 8).  matmul_plane_slices: how many pay; 1: none do.
+constexpr int MAX_PLANES = 16;
+int matmul_plane_slices(long long M, long long N, long long K);
+int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream);
 // norm_general.cu: any float types, strides and column counts (layer = 0 RmsNorm, 1 LayerNorm).
 int32_t norm_general_execute(int layer, const cdl_tensor* x, const cdl_tensor* scale,
                              const cdl_tensor* bias, float eps, const cdl_tensor* y,
