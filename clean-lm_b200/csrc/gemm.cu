@@ -505,6 +505,42 @@ __device__ __forceinline__ void add_tile_rows(const Params& p, const CUtensorMap
   }
 }
 
+// The epilogue of a bf16 D = alpha * accumulator for the calling warp: rows row0 .. row0 + 31, 128 columns, as two TMA stores
+// of 32 x 64 from its 4 KiB buffer (128-byte swizzle).  A thread's own stores cover 32 bytes of 32 rows per instruction; a
+// product of a short K is bound by them: 2048 x 32768 with K = 64 STORE_BF16_TIMES.
+__device__ __forceinline__ void store_tile_rows_tma(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row,
+                                                    int b, int row0, int col_base, int lane) {
+  if (row0 >= p.M) return;  // warp-uniform; rows past M inside the box are clipped
+#pragma unroll 1
+  for (int ch = 0; ch < 2; ++ch) {
+    const int col0 = col_base + ch * 64;
+    if (col0 >= p.N) break;
+    uint32_t r[2][32];
+    tmem_ld32(t_row + ch * 64, r[0]);
+    tmem_ld32(t_row + ch * 64 + 32, r[1]);
+    tmem_wait_ld(r[0], r[1]);
+    if (lane == 0) tma_store_wait_read<0>();  // the buffer's last store has read it
+    __syncwarp();
+    const uint32_t row = smem_u32(buf) + lane * 128, x = (lane & 7) << 4;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = pack_bf16x2(p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j]),
+                           p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j + 1]));
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((c << 4) ^ x)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(tm_d, buf, col0, row0, b);
+      tma_store_commit();
+    }
+  }
+}
+
 // One of 32 registers, by a tree of selections.
 __device__ __forceinline__ uint32_t pick32(const uint32_t (&r)[32], int i) {
   uint32_t a[16];
@@ -596,6 +632,14 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, uint32_t t_
   p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] = make_float2(m == -INFINITY ? -INFINITY : base, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
+// One kernel per kind of store.  All of them in one, with the buffers that the plain ones do not need (they take room
+// from the L1, through which C is read), cost those 0.2 to 0.9 us (2048 x 5632 x
+// 256 12.3 instead of 11.9, with a bf16 C 18.8 instead of 18.0).
+// D in any form; D += by TMA; the SwiGLU forms whose operands TMA brings; a loss's exponentials; every K slice in a plane of
+// its own; a bf16 D by TMA.
+enum Store { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP, STORE_PLANES, STORE_BF16 };
+
+template <int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
                      const __grid_constant__ CUtensorMap tmap_b, const Params p) {
@@ -632,6 +676,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  // Unit of work: a tile, or (STORE_PLANES) one of its K slices, numbered slice by slice.
+  const int num_units = KIND == STORE_PLANES ? p.num_tiles * p.split_k : p.num_tiles;
+  auto unit_range = [&](int unit, int& tile, int& slice, int& kb0, int& kb1) {
+    if constexpr (KIND == STORE_PLANES) {
+      slice = unit / p.num_tiles;
+      tile = unit - slice * p.num_tiles;
+      kb0 = static_cast<int>(static_cast<long long>(slice) * p.k_blocks / p.split_k);
+      kb1 = static_cast<int>(static_cast<long long>(slice + 1) * p.k_blocks / p.split_k);
+    } else {
+      tile = unit;
+      slice = kb0 = 0;
+      kb1 = p.k_blocks;
+    }
+  };
   // Everything above overlaps the tail of the previous kernel of the stream; operands are read
   // (and outputs written) only from here on.
   grid_dep_wait();
@@ -642,11 +700,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
-        int b, tm, tn;
+      for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x) {
+        int tile, slice, kb0, kb1, b, tm, tn;
+        unit_range(unit, tile, slice, kb0, kb1);
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * BM, n0 = tn * BN;
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait(&bars->empty[s], ph ^ 1, abort_word, 101)) {
@@ -683,13 +742,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t it = 0;
       int t = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x, ++t) {
+      for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x, ++t) {
+        int tile, slice, kb0, kb1;
+        unit_range(unit, tile, slice, kb0, kb1);
         const int acc = t & 1;
         const uint32_t acc_ph = (t >> 1) & 1;
         if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 201)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait(&bars->full[s], ph, abort_word, 202)) {
@@ -703,7 +764,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
             const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
-            umma_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_ss(d_tmem, da, db, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
           }
           umma_commit(&bars->empty[s]);
         }
@@ -715,16 +776,26 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quad = warp & 3;  // TMEM lane quadrant this warp may read
     const int half = (warp - 2) >> 2;  // which 128 of the tile's 256 columns
     int t = 0;
-    for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++t) {
-      int b, tm, tn;
+    for (int unit = blockIdx.x; unit < num_units; unit += gridDim.x, ++t) {
+      int tile, slice, kb0, kb1, b, tm, tn;
+      unit_range(unit, tile, slice, kb0, kb1);
       tile_coords(p, tile, b, tm, tn);
       const int acc = t & 1;
       const uint32_t acc_ph = (t >> 1) & 1;
+      Wanted want;
+      if (KIND == STORE_EXP) want.load(p, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
       if (!mbar_wait(&bars->acc_full[acc], acc_ph, abort_word, 301)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
-      if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
-      else store_tile_rows(p, t_row, b, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
+      const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
+      if constexpr (KIND == STORE_EXP) {
+        store_tile_rows_exp(p, t_row, row, col, want);
+      } else if constexpr (KIND == STORE_PLANES) {
+        store_tile_rows(p, t_row, slice, row, col);
+      } else {
+        if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
+        else store_tile_rows(p, t_row, b, row, col);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
@@ -760,11 +831,7 @@ constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = 2 * A_BYTES;  // A 128 x 64 and half of B 128 x 64
 constexpr int PAIR_M = 2 * BM;
 constexpr int PAIR_BARRIER_BYTES = 512;
-// One kernel per kind of store.  All of them in one, with the buffers that the plain ones do not need (they take room
-// from the L1, through which C is read), cost those 0.2 to 0.9 us (2048 x 5632 x
-// 256 12.3 instead of 11.9, with a bf16 C 18.8 instead of 18.0).
-enum PairStore { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP };  // D in any form, D += by TMA, the SwiGLU forms whose operands TMA brings, a loss's exponentials
-constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_EXP ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
+constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_EXP || kind == STORE_PLANES ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
 constexpr size_t pair_smem_bytes(int kind) {
   return 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + pair_staging(kind) + PAIR_BARRIER_BYTES;
 }
@@ -1026,15 +1093,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         else store_tile_rows_swiglu<true>(p, feed, t_row, row, col, lane, abort_word);
       } else if constexpr (KIND == STORE_EXP) {
         store_tile_rows_exp(p, t_row, row, col, want);
+      } else if constexpr (KIND == STORE_PLANES) {
+        store_tile_rows(p, t_row, slice, row, col);
+      } else if constexpr (KIND == STORE_BF16) {
+        store_tile_rows_tma(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
-        else store_tile_rows(p, t_row, p.planes ? slice : b, row, col);
+        else store_tile_rows(p, t_row, b, row, col);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[acc]), 0));
     }
-    if (KIND == STORE_ADD && lane == 0) tma_store_wait<0>();
+    if ((KIND == STORE_ADD || KIND == STORE_BF16) && lane == 0) tma_store_wait<0>();
   }
 
   // ------------------------------------------------------------ tear-down
@@ -1230,8 +1301,13 @@ static int32_t prepare_kernels(int* clusters) {
   CDL_CUDA(cudaGetDevice(&dev));
   cudaError_t attr_err = cudaSuccess;
   std::call_once(attr_once[dev & 63], [&] {
-    attr_err = cudaFuncSetAttribute(gemm_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(SMEM_BYTES));
+    auto one = [&](auto kernel) {
+      if (attr_err == cudaSuccess)
+        attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM_BYTES));
+    };
+    one(gemm_bf16_kernel<STORE>);
+    one(gemm_bf16_kernel<STORE_EXP>);
+    one(gemm_bf16_kernel<STORE_PLANES>);
     auto pair = [&](auto kernel, int kind) {
       if (attr_err == cudaSuccess)
         attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1241,6 +1317,8 @@ static int32_t prepare_kernels(int* clusters) {
     pair(gemm_bf16_pair_kernel<STORE_ADD>, STORE_ADD);
     pair(gemm_bf16_pair_kernel<STORE_SWIGLU>, STORE_SWIGLU);
     pair(gemm_bf16_pair_kernel<STORE_EXP>, STORE_EXP);
+    pair(gemm_bf16_pair_kernel<STORE_PLANES>, STORE_PLANES);
+    pair(gemm_bf16_pair_kernel<STORE_BF16>, STORE_BF16);
     int n = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
@@ -1430,7 +1508,6 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   p.beta = use_c ? beta : 0.0f;
   p.split_k = use_cluster ? cluster_splits : 1;
   p.sched_counter = nullptr;
-  p.planes = 0;
   p.atomic_out = 0;
   p.tma_add = 0;
   p.early = (early & EARLY_PRODUCTS) ? (use_pair ? 2 : 0) : early > 0 ? 1 : 0;
@@ -1568,14 +1645,15 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
                        : run(gemm_bf16_pair_kernel<STORE>, STORE));
   } else {  // (this one always waits at its start)
     const int grid = p.num_tiles < sm_count() ? p.num_tiles : sm_count();
-    CDL_CUDA(launch_pdl(gemm_bf16_kernel, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, tm_a, tm_b, p));
+    CDL_CUDA(launch_pdl(gemm_bf16_kernel<STORE>, dim3(grid), dim3(THREADS), SMEM_BYTES, stream, tm_a, tm_b, p));
   }
   CDL_CUDA(cudaGetLastError());
   return CDL_OK;
 }
 
-// The pair kernel's operands of a plain product of bf16 tensors on the 16-byte grid.
-static int32_t pair_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Params& p, CUtensorMap* tm_a, CUtensorMap* tm_b) {
+// The wide tiles' operands of a plain product of bf16 tensors on the 16-byte grid; one CTA per tile up to 128 rows, else CTA
+// pairs.
+static int32_t wide_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Params& p, CUtensorMap* tm_a, CUtensorMap* tm_b, bool pair) {
   using namespace gemm;
   const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
   OperandLayout la, lb;
@@ -1586,7 +1664,7 @@ static int32_t pair_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Par
   const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(la.ld) * da[1] * 2};
   const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(lb.ld) * db[1] * 2};
   const uint32_t ba[3] = {64, static_cast<uint32_t>(la.mn_major ? 64 : BM), 1};
-  const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : BN / 2), 1};
+  const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : pair ? BN / 2 : BN), 1};
   CDL_CHECK(encode_tmap(tm_a, a->ptr, CDL_BF16, 3, da, sa, ba, true));
   CDL_CHECK(encode_tmap(tm_b, b->ptr, CDL_BF16, 3, db, sb, bb, true));
   p = {};
@@ -1594,7 +1672,8 @@ static int32_t pair_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Par
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.batch = 1;
-  p.num_m_tiles = static_cast<int>((M + PAIR_M - 1) / PAIR_M);
+  const int tile_m = pair ? PAIR_M : BM;
+  p.num_m_tiles = static_cast<int>((M + tile_m - 1) / tile_m);
   p.num_n_tiles = static_cast<int>((N + BN - 1) / BN);
   const long long tiles = static_cast<long long>(p.num_m_tiles) * p.num_n_tiles;
   if (tiles > INT32_MAX / 64) return fail(CDL_ERR_UNSUPPORTED, "matmul: too many tiles");
@@ -1610,31 +1689,46 @@ static int32_t pair_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Par
 }
 
 template <int KIND>
-static int32_t pair_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtensorMap& tm_b, cudaStream_t stream) {
+static int32_t pair_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap& tm_d, int early,
+                           cudaStream_t stream) {
   using namespace gemm;
   int held = 0;
   CDL_CHECK(prepare_kernels(&held));
   const int units = p.num_tiles * p.split_k, clusters = units < held ? units : held;
-  p.sched_counter = units > clusters ? sched_counter_for(gemm_counter_kind(0), current_device(), stream) : nullptr;
+  p.sched_counter = units > clusters ? sched_counter_for(gemm_counter_kind(early), current_device(), stream) : nullptr;
+  p.early = early > 0 ? 1 : 0;
   ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(p.M) * p.N * p.K, stream);
-  CDL_CUDA(launch_pdl(gemm_bf16_pair_kernel<KIND>, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(KIND), stream, tm_a, tm_b, tm_a,
-                      tm_a, p));
+  CDL_CUDA(launch_pdl(gemm_bf16_pair_kernel<KIND>, dim3(2 * clusters), dim3(THREADS), pair_smem_bytes(KIND), stream, tm_a, tm_b, tm_d,
+                      tm_d, p));
   CDL_CUDA(cudaGetLastError());
   return CDL_OK;
 }
 
-// The logits of a loss (see store_tile_rows_exp): always CTA pairs.  With few rows a pair's second half has none, but the
-// columns of B are what such a product reads, and they are loaded as fast.
+template <int KIND>
+static int32_t one_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtensorMap& tm_b, cudaStream_t stream) {
+  using namespace gemm;
+  int held = 0;
+  CDL_CHECK(prepare_kernels(&held));
+  const int units = p.num_tiles * p.split_k;
+  ProfileScope ps(PROF_GEMM, 2.0 * static_cast<double>(p.M) * p.N * p.K, stream);
+  CDL_CUDA(launch_pdl(gemm_bf16_kernel<KIND>, dim3(units < sm_count() ? units : sm_count()), dim3(THREADS), SMEM_BYTES, stream, tm_a, tm_b, p));
+  CDL_CUDA(cudaGetLastError());
+  return CDL_OK;
+}
+
+// The logits of a loss (see store_tile_rows_exp).  Up to 128 rows one CTA per 256 columns: a pair's second half would have no
+// rows but take as long over its products, which then, not the bytes of B, set the time (64 x 2048 x 32768 EXP_ONE_TIMES).
 int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
                            cudaStream_t stream) {
   gemm::Params p;
   CUtensorMap tm_a, tm_b;
-  CDL_CHECK(pair_operands(a, b, p, &tm_a, &tm_b));
+  const bool pair = a->shape[0] > gemm::BM;
+  CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, pair));
   p.d = d;
   p.ldd = ldd;
   p.alpha = scale;
   p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
-  return pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
+  return pair ? pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
 }
 
 // K slices of a product whose output is small and whose K is long (dx of a head: K is the vocabulary), each stored in f32 in
@@ -1642,11 +1736,13 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
 // block, 4 per unit's store and set-up, a plane's way out and back at 5 TB/s and 3 for the kernel that sums them.
 int matmul_plane_slices(long long M, long long N, long long K) {
   using namespace gemm;
-  const long long tiles = ((M + PAIR_M - 1) / PAIR_M) * ((N + BN - 1) / BN), k_blocks = (K + BK - 1) / BK, pairs = sm_count() / 2;
+  const bool pair = M > BM;
+  const long long tiles = (pair ? (M + PAIR_M - 1) / PAIR_M : 1) * ((N + BN - 1) / BN), k_blocks = (K + BK - 1) / BK;
+  const long long slots = pair ? sm_count() / 2 : sm_count();
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= MAX_PLANES && (s == 1 || s * 8 <= k_blocks); ++s) {
-    const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
+    const double waves = static_cast<double>((tiles * s + slots - 1) / slots);
     double t = waves * (0.28 * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
     if (s > 1) t = 1.05 * (t + 3.0 + 8e-6 * static_cast<double>(s) * M * N / 5.0);
     if (t < least) {
@@ -1660,13 +1756,34 @@ int matmul_plane_slices(long long M, long long N, long long K) {
 int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream) {
   gemm::Params p;
   CUtensorMap tm_a, tm_b;
-  CDL_CHECK(pair_operands(a, b, p, &tm_a, &tm_b));
+  const bool pair = a->shape[0] > gemm::BM;
+  CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, pair));
   p.d = planes;
   p.ldd = ld;
   p.d_batch = ld * p.M;
-  p.out_f32 = p.d_vec = p.wide = p.planes = 1;  // (rows of whole 32 bytes)
+  p.out_f32 = p.d_vec = p.wide = 1;  // (rows of whole 32 bytes)
   p.split_k = slices;
-  return pair_launch<gemm::STORE>(p, tm_a, tm_b, stream);
+  return pair ? pair_launch<gemm::STORE_PLANES>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_PLANES>(p, tm_a, tm_b, stream);
+}
+
+// Whether a plain product is bound by the store of its bf16 D, which TMA makes the shorter: a short K and pairs with several
+// tiles each.
+bool matmul_store_bound(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d) {
+  using namespace gemm;
+  const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
+  return d->dtype == CDL_BF16 && K <= 512 && M > BM && ((M + PAIR_M - 1) / PAIR_M) * ((N + BN - 1) / BN) >= sm_count() &&
+         (reinterpret_cast<uintptr_t>(d->ptr) & 15) == 0 && d->stride[1] == 1 && d->stride[0] % 8 == 0 && d->stride[0] >= N;
+}
+
+int32_t matmul_store_execute(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d, cudaStream_t stream, int early) {
+  gemm::Params p;
+  CUtensorMap tm_a, tm_b, tm_d;
+  CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, true));
+  const uint64_t ld = static_cast<uint64_t>(d->stride[0]) * 2;
+  const uint64_t dims[3] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M), 1}, strides[3] = {0, ld, ld * p.M};
+  const uint32_t box[3] = {64, 32, 1};
+  CDL_CHECK(encode_tmap(&tm_d, d->ptr, CDL_BF16, 3, dims, strides, box, true));
+  return pair_launch<gemm::STORE_BF16>(p, tm_a, tm_b, tm_d, early, stream);
 }
 
 }  // namespace cdl

@@ -32,7 +32,6 @@ struct Params {
   int split_k;     // K slices per tile (pair kernel: accumulate-in-place form only; cluster kernels: CTAs
                    // per cluster); 1 = none
   int sum_blocks;  // gemm_general.cu: K blocks that one tensor-core accumulator sums up
-  int planes;      // 1 = K slice s is stored at d + s d_batch (pair kernel)
   int atomic_out;  // 1 = add alpha * partial into D with red.global.add (D already holds C)
   int tma_add;     // 1 = the pair kernel adds by TMA reductions (add_chunk)
   // Fused SwiGLU epilogues (bf16 [M, N] operands, 16-byte aligned rows):

@@ -654,24 +654,25 @@ __global__ void __launch_bounds__(256)
     sum_planes_kernel(const float* planes, long long ld, int slices, __nv_bfloat16* out, long long ld_out, int rows, int cols, int vectors) {
   grid_dep_wait();
   grid_dep_launch();
-  const int per_row = (cols + 7) / 8;
+  const int per_row = (cols + 3) / 4;
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, r = i / per_row;
   if (r >= rows) return;
-  const int c = static_cast<int>(i - r * per_row) * 8;
+  const int c = static_cast<int>(i - r * per_row) * 4;
   const float* from = planes + r * ld + c;
-  float v[8] = {};
-#pragma unroll 4
-  for (int s = 0; s < slices; ++s, from += rows * ld) {
-    const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
-    v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w; v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < slices; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(from + s * (rows * ld));
+    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
   }
   __nv_bfloat16* o = out + r * ld_out + c;
-  if (vectors && c + 8 <= cols) {
-    *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  if (vectors && c + 4 <= cols) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   } else {
+    const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) o[j] = __float2bfloat16_rn(v[j]);
+    for (int j = 0; j < 4; ++j)
+      if (c + j < cols) o[j] = __float2bfloat16_rn(f[j]);
   }
 }
 
@@ -1145,13 +1146,14 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       const cdl_tensor gt = transposed(g), xt = transposed(clean), sum_t = transposed(sum);
       const cdl_tensor *a = dw_columns ? &gt : &xt, *b = dw_columns ? &clean : &g, *d = dw_columns ? &sum_t : &sum;
       // (beside dx's product, whose last wave leaves SMs idle: the two share what they read alone)
-      CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
+      if (fused && !add && matmul_store_bound(a, b, d)) CDL_CHECK(matmul_store_execute(a, b, d, stream, p.has_dx ? 1 : 0));
+      else CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
                                fused && p.has_dx ? 1 : 0));
     }
     if (p.slices > 1) {
-      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 15) == 0 && (n == 1 || d.stride[0] % 8 == 0);
+      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 7) == 0 && (n == 1 || d.stride[0] % 4 == 0);
       ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(n) * p.D * (4 * p.slices + 2), stream);
-      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * (x_ld / 8) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
+      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * ((p.D + 3) / 4) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
                           p.slices, static_cast<__nv_bfloat16*>(d.ptr), static_cast<long long>(d.stride[0]), static_cast<int>(n),
                           static_cast<int>(p.D), vectors ? 1 : 0));
     }

@@ -58,9 +58,12 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
                            cudaStream_t stream);
 // A product of bf16 tensors on the 16-byte grid in K slices: slice s is stored at planes + s M ld (f32, 32-byte aligned, ld >= N a
 // multiple of 8).  matmul_plane_slices: how many pay; 1: none do.
-constexpr int MAX_PLANES = 16;
+constexpr int MAX_PLANES = 24;
 int matmul_plane_slices(long long M, long long N, long long K);
 int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream);
+// D = A . B of such tensors with a bf16 D whose store sets the time (matmul_store_bound), stored by TMA.
+bool matmul_store_bound(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d);
+int32_t matmul_store_execute(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d, cudaStream_t stream, int early);
 // norm_general.cu: any float types, strides and column counts (layer = 0 RmsNorm, 1 LayerNorm).
 int32_t norm_general_execute(int layer, const cdl_tensor* x, const cdl_tensor* scale,
                              const cdl_tensor* bias, float eps, const cdl_tensor* y,
