@@ -83,12 +83,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 struct RowEntries {
   int* id;    // -1: does not count
   float* p;   // of the entry
-  float* sum; // of all entries of its id, at the first of them; -1 at the others
   float* at;  // t of the row at the id
-  __device__ __forceinline__ RowEntries(void* smem, int K)
-      : id(static_cast<int*>(smem)), p(static_cast<float*>(smem) + K), sum(p + K), at(sum + K) {}
+  __device__ __forceinline__ RowEntries(void* smem, int K) : id(static_cast<int*>(smem)), p(static_cast<float*>(smem) + K), at(p + K) {}
 };
-constexpr int ENTRY_BYTES = 16;
+constexpr int ENTRY_BYTES = 12;
 struct RowShared {
   float part[32];
   float p_log_p;
@@ -106,64 +104,90 @@ __device__ __forceinline__ float cta_reduce(float v, bool max, float* part) {
 }
 
 // A row's entries by one warp: ids and p = softmax(teacher / tau) over those that count (id in [0, vocab), logit above
-// -inf); sum p log p; whether there are any.
+// -inf); sum p log p; whether there are any; and (x != nullptr) t at the ids.  Four entries of a lane are under way at a
+// time: their latency is what this costs.
+template <typename T>
 __device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh, const Entries& src, long long row, int vocab,
-                                             float tau) {
+                                             float tau, const T* x) {
   const int lane = threadIdx.x & 31;
+  const float c = LOG2E / tau;
   if (src.kind == TARGETS) {
     const int id = src.ids[row];
     const bool counts = id >= 0 && id < vocab;
     if (lane == 0) {
       e.id[0] = counts ? id : -1;
       e.p[0] = counts ? 1.f : 0.f;
+      if (x != nullptr) e.at[0] = counts ? c * to_f32(x[id]) : 0.f;
       sh.counts = counts;
       sh.p_log_p = 0.f;
     }
     return;
   }
   const int* ids = src.ids + row * src.ids_ld;
-  const float c = LOG2E / tau;
   float m = -INFINITY;
-  for (int k = lane; k < src.K; k += 32) {
-    const int id = ids[k];
-    float y = -INFINITY;
-    if (id >= 0 && id < vocab)  // (padding may hold anything)
-      y = c * teacher_logit(src, row, k);
-    e.id[k] = y == -INFINITY ? -1 : id;
-    e.p[k] = y;
-    m = fmaxf(m, y != y ? INFINITY : y);  // a NaN makes the row NaN
+  for (int k0 = lane; k0 < src.K; k0 += 128) {
+    int id[4];
+    float y[4], at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + 32 * j;
+      id[j] = k < src.K ? ids[k] : -1;
+      y[j] = k < src.K ? teacher_logit(src, row, k) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (id[j] >= vocab) id[j] = -1;
+      if (id[j] < 0) y[j] = -INFINITY;  // (padding may hold anything)
+      y[j] *= c;
+      if (y[j] == -INFINITY) id[j] = -1;
+      at[j] = x != nullptr && id[j] >= 0 ? to_f32(x[id[j]]) : 0.f;
+      m = fmaxf(m, y[j] != y[j] ? INFINITY : y[j]);  // a NaN makes the row NaN
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + 32 * j;
+      if (k >= src.K) break;
+      e.id[k] = id[j];
+      e.p[k] = y[j];
+      if (x != nullptr) e.at[k] = c * at[j];
+    }
   }
   m = warp_max(m);
   const bool counts = m != -INFINITY;
   float s = 0.f, sy = 0.f;
   for (int k = lane; k < src.K; k += 32) {
-    const float y = e.p[k] - m, x = e.id[k] < 0 ? 0.f : ex2(y);
-    e.p[k] = x;
-    s += x;
-    if (x != 0.f) sy += x * y;
+    const float y = e.p[k] - m, v = e.id[k] < 0 ? 0.f : ex2(y);
+    e.p[k] = v;
+    s += v;
+    if (v != 0.f) sy += v * y;
   }
   s = warp_sum(s);
   sy = warp_sum(sy);
-  for (int k = lane; k < src.K; k += 32) e.p[k] = counts ? e.p[k] / s : 0.f;
+  const float over = 1.f / s;
+  for (int k = lane; k < src.K; k += 32) e.p[k] = counts ? e.p[k] * over : 0.f;
   if (lane == 0) {
     sh.counts = counts;
-    sh.p_log_p = counts ? LN2 * (sy / s - log2f(s)) : 0.f;
+    sh.p_log_p = counts ? LN2 * (sy * over - log2f(s)) : 0.f;
   }
 }
 
-// Each id once: the sum of its entries' probabilities, in their order.  All threads, entries visible.
-__device__ __forceinline__ void merge_entries(const RowEntries& e, int K) {
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const int id = e.id[k];
-    float sum = 0.f;
-    bool again = id < 0;
-#pragma unroll 8
-    for (int i = 0; i < K; ++i) {
-      const bool same = e.id[i] == id;
-      again = again || (same && i < k);
-      sum += same ? e.p[i] : 0.f;
+// Which of a row's ids occur more than once: a hash table of more slots than entries, all -1 at first, in which
+// an entry meets those of its id; a slot that has met one has the sign bit set.  0 <= id < INT32_MAX.
+__device__ __forceinline__ unsigned slot_of(int slots_log2, int id) { return (static_cast<unsigned>(id) * 2654435761u) >> (32 - slots_log2); }
+__device__ __forceinline__ void mark_id(int* table, int slots_log2, int id) {
+  for (unsigned h = slot_of(slots_log2, id);; h = (h + 1) & ((1u << slots_log2) - 1)) {
+    const int was = atomicCAS(&table[h], -1, id);
+    if (was == -1 || was == (id | INT32_MIN)) return;
+    if (was == id) {
+      table[h] = id | INT32_MIN;
+      return;
     }
-    e.sum[k] = again ? -1.f : sum;
+  }
+}
+__device__ __forceinline__ bool is_marked(const int* table, int slots_log2, int id) {  // of an id that is in the table
+  for (unsigned h = slot_of(slots_log2, id);; h = (h + 1) & ((1u << slots_log2) - 1)) {
+    if (table[h] == id) return false;
+    if (table[h] == (id | INT32_MIN)) return true;
   }
 }
 
@@ -171,7 +195,7 @@ __device__ __forceinline__ void merge_entries(const RowEntries& e, int K) {
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS)
     loss_row_kernel(const T* z, long long ld_z, T* g, long long ld_g, int vocab, const Entries src, const RowTerms terms) {
-  __shared__ int4 entries[MAX_ENTRIES];
+  __shared__ int entries[3 * MAX_ENTRIES];
   __shared__ RowShared sh;
   const RowEntries e(entries, src.K);
   grid_dep_wait();
@@ -179,10 +203,8 @@ __global__ void __launch_bounds__(ROW_THREADS)
   const long long row = blockIdx.x;
   const T* x = z + row * ld_z;
   const float c = LOG2E / terms.tau;
-  if (threadIdx.x < 32) load_entries(e, sh, src, row, vocab, terms.tau);
+  if (threadIdx.x < 32) load_entries(e, sh, src, row, vocab, terms.tau, x);
   __syncthreads();
-  merge_entries(e, src.K);
-  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) e.at[k] = e.id[k] < 0 ? 0.f : c * to_f32(x[e.id[k]]);
   float m = -INFINITY, s = 0.f;
   bool bad = false;
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS) {
@@ -201,7 +223,7 @@ __global__ void __launch_bounds__(ROW_THREADS)
   const float log2_s = log2f(s);
   float cross = 0.f;  // sum_k p_k log2 q_k
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
-    if (e.sum[k] > 0.f || e.sum[k] != e.sum[k]) cross += e.sum[k] * ((e.at[k] - base) - log2_s);
+    if (e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
   cross = cta_reduce(cross, false, sh.part);
   const bool counts = sh.counts;
   if (threadIdx.x == 0) {
@@ -215,210 +237,293 @@ __global__ void __launch_bounds__(ROW_THREADS)
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS)
     y[j] = from_f32<T>(counts ? ex2(fmaf(to_f32(x[j]), c, -base)) * over_s : 0.f);
   __syncthreads();
-  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
-    if (e.sum[k] != -1.f) y[e.id[k]] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - e.sum[k]));
+  for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) {
+    const int id = e.id[k];
+    if (id < 0) continue;
+    float p = 0.f;  // each id once: the sum of its entries' probabilities, in their order
+    bool again = false;
+    for (int i = 0; i < src.K; ++i) {
+      if (e.id[i] != id) continue;
+      again = again || i < k;
+      p += e.p[i];
+    }
+    if (!again) y[id] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - p));
+  }
 }
 
-// The same with the row in shared memory, read from and written to HBM once: a cluster of 1 to 8 CTAs per row, whose warps have
-// a slice of it each.  A warp brings its slice by a bulk copy of its own and goes over it in three passes: the maximum;
-// the exponentials, which replace the logits (bf16: as f16 of up to 2^15, see store_tile_rows_exp in gemm.cu; their sum is
-// of the f32 values); and, behind the one barrier at which the slices' (M', S') meet, the gradient.  One exponential per
-// element: a second one would put 4096 clk of special functions per 64 KB on an SM, whose share of the HBM's rate takes 5500.
-// Three CTAs per SM are in different passes and keep the copies going.  The slices depend on the vocabulary alone, not on
-// how many CTAs share a row, so a row's results do not depend on the number of rows.
-struct Share {
-  int warps, vecs, ctas;  // warps of a row, 16-byte vectors of a warp, CTAs of a row
-  size_t smem;            // of a CTA
-};
-constexpr int SHARE_BYTES = 72 * 1024;  // three CTAs per SM
-constexpr int MAX_ROW_WARPS = 8 * ROW_THREADS / 32;
+// The same with a row read from and written to HBM once: a cluster of 1 to 8 CTAs per row, whose warps have a slice of it each, at
+// most 32 x VECS vectors of 16 bytes, which stay in registers: the maximum; the exponentials in place of the logits (bf16: as
+// f16 of up to 2^15, see store_tile_rows_exp in gemm.cu; their sum is of the f32 values); and, behind the one barrier at
+// which the slices' parts of the statistics meet, the gradient.  The row's entries are a thread's each, and their softmax
+// meets at the same barrier: where one warp prepared them all, the others waited for it (8192 x 32768 with 64
+// entries 244 us; PLACEHOLDER).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
+// whose share of the HBM's rate takes 5500.  The slices depend on the vocabulary alone, not on how many CTAs share a row, so
+// a row's results do not depend on the number of rows.
+//
+// A vector that starts before the row or ends behind it is read whole where it holds an element of the row (the same 16
+// bytes of memory); what is not the row's counts as -inf and is never written.
+constexpr int WARPS = 16;              // of a CTA, at most
+constexpr int MAX_ROW_WARPS = 8 * WARPS;
 
+// Elements of a vector outside [lo, hi) become -inf.
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4& q, float (&f)[16 / sizeof(T)]);
-template <>
-__device__ __forceinline__ void unpack<float>(const uint4& q, float (&f)[4]) {
-  f[0] = __uint_as_float(q.x); f[1] = __uint_as_float(q.y); f[2] = __uint_as_float(q.z); f[3] = __uint_as_float(q.w);
-}
-template <>
-__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& q, float (&f)[8]) {
-  f[0] = bf16_lo(q.x); f[1] = bf16_hi(q.x); f[2] = bf16_lo(q.y); f[3] = bf16_hi(q.y);
-  f[4] = bf16_lo(q.z); f[5] = bf16_hi(q.z); f[6] = bf16_lo(q.w); f[7] = bf16_hi(q.w);
+__device__ __forceinline__ void mask_vector(uint4& q, int lo, int hi) {
+  uint32_t* w = &q.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      if (j < lo || j >= hi) w[j] = 0xff800000u;
+    } else {
+      if (2 * j < lo || 2 * j >= hi) w[j] = (w[j] & 0xffff0000u) | 0xff80u;
+      if (2 * j + 1 < lo || 2 * j + 1 >= hi) w[j] = (w[j] & 0xffffu) | 0xff800000u;
+    }
+  }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS, 3)
-    loss_share_kernel(const T* z, long long ld_z, T* g, long long ld_g, int vocab, int slice, int ctas, const Entries src,
-                      const RowTerms terms, int* status) {
+// Two f32 operations as one.
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <typename T, int VECS>
+__global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
+    loss_slices_kernel(const T* z, long long ld_z, T* g, long long ld_g, long long rows, long long ahead, int vocab, int slice, int ctas,
+                       int slots_log2, const Entries src, const RowTerms terms) {
   constexpr bool HALF = sizeof(T) == 2;
   constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ RowShared sh;
-  __shared__ float2 s_part[ROW_THREADS / 32];  // (M', S') of the CTA's slices
-  __shared__ uint64_t full[ROW_THREADS / 32];
-  __shared__ int abort_word;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float2 s_part[WARPS];     // (M', S') of the CTA's slices
+  __shared__ float3 s_entries[WARPS];  // of the entries of a warp's threads: max y, sum 2^(y - max), sum 2^(y - max) (y - max)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const long long row = blockIdx.x / ctas;
   const int rank = blockIdx.x - static_cast<int>(row) * ctas;
   const T* x = z + row * ld_z;
-  // The row in 16-byte vectors of memory: its first element is element `lead` of vector 0.
+  // The row in 16-byte vectors of memory: its first element is element `lead` of vector 0.  Element j of the row is
+  // element j + first of the slice, which has n vectors.
   const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
-  const int all = (lead + vocab + VEC - 1) / VEC, whole0 = lead != 0, whole1 = (lead + vocab) / VEC;
-  const int v0 = min(all, (rank * warps + warp) * slice), v1 = min(all, v0 + slice);  // the warp's
-  uint4* vec = reinterpret_cast<uint4*>(smem) + warp * slice;  // vector v0's place
-  const RowEntries e(smem + static_cast<size_t>(warps) * slice * 16, src.K);
-  if (threadIdx.x == 0) abort_word = 0;
-  if (lane == 0) {
-    mbar_init(&full[warp], 1);
-    fence_mbar_init();
-  }
+  const int v0 = (rank * warps + warp) * slice;
+  const int n = min(max((lead + vocab + VEC - 1) / VEC - v0, 0), slice), first = lead - v0 * VEC;
+  const RowEntries e(smem, src.K);
   grid_dep_wait();
   grid_dep_launch();
-  const int b0 = max(v0, whole0), b1 = min(v1, whole1);
-  if (lane == 0 && b1 > b0) {
-    mbar_arrive_expect_tx(&full[warp], (b1 - b0) * 16);
-    bulk_load_1d(vec + (b0 - v0), x - lead + static_cast<long long>(b0) * VEC, (b1 - b0) * 16, &full[warp]);
+  uint4 q[VECS];
+  const T* from = x - first + lane * VEC;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const uint32_t none = HALF ? 0xff80ff80u : 0xff800000u;  // -inf
+    q[i] = lane + 32 * i < n ? *reinterpret_cast<const uint4*>(from + i * 32 * VEC) : make_uint4(none, none, none, none);
   }
-  // What the copy does not bring: vectors that the row fills in part, with -inf around its elements.
-  auto partial = [&](int v) {
-    const int at = v * VEC + lane - lead;
-    if (lane < VEC) reinterpret_cast<T*>(vec + (v - v0))[lane] = at >= 0 && at < vocab ? x[at] : from_f32<T>(-INFINITY);
-  };
-  if (v0 == 0 && v1 > 0 && whole0 > 0) partial(0);
-  if (v0 <= whole1 && whole1 < v1 && whole1 >= whole0) partial(whole1);
   const float c = LOG2E / terms.tau;
-  if (warp == 0) {
-    load_entries(e, sh, src, row, vocab, terms.tau);
-    __syncwarp();
-    for (int k = lane; k < src.K; k += 32) e.at[k] = e.id[k] < 0 ? 0.f : c * to_f32(x[e.id[k]]);
+  const float d_loss = terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f;
+  // The row of a CTA that will follow this one goes to the L2 meanwhile, so that HBM is read under the arithmetic, too.
+  if (lane == 0 && row + ahead < rows && n > 0) {
+    const T* later = x + ahead * ld_z;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(later) & 15) / static_cast<int>(sizeof(T));
+    const int count = min(max((off + vocab + VEC - 1) / VEC - v0, 0), slice);
+    if (count > 0) bulk_prefetch_l2(later - off + static_cast<long long>(v0) * VEC, count * 16);
   }
-  __syncthreads();  // (abort_word; and entries for merge_entries)
-  bool arrived = true;
-  if (b1 > b0) arrived = mbar_wait(&full[warp], 0, &abort_word, 701);
-  __syncwarp();
-  const int n = v1 - v0;
+  int* table = reinterpret_cast<int*>(smem + static_cast<size_t>(ENTRY_BYTES) * src.K);
+  for (int i = threadIdx.x; i < 1 << slots_log2; i += blockDim.x) table[i] = -1;
+  __syncthreads();
+  float at_first = 0.f;  // t at the thread's first entry: its load may take until the exponentials are done
+  {
+    float m = -INFINITY, s = 0.f, sy = 0.f;
+    for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+      int id = src.ids[row * src.ids_ld + k];
+      float y = src.kind == TARGETS ? 0.f : c * teacher_logit(src, row, k);
+      if (id < 0 || id >= vocab || y == -INFINITY) id = -1, y = -INFINITY;  // (padding may hold anything)
+      else mark_id(table, slots_log2, id);
+      e.id[k] = id;
+      e.p[k] = y;
+      m = fmaxf(m, y != y ? INFINITY : y);  // a NaN makes the row NaN
+      const float at = id < 0 ? 0.f : to_f32(x[id]);
+      if (k == threadIdx.x) at_first = at;
+      else e.at[k] = c * at;
+    }
+    if (warp * 32 < src.K) {
+      m = warp_max(m);
+      for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
+        const float y = e.p[k] - m, v = e.id[k] < 0 ? 0.f : ex2(y);
+        e.p[k] = v;  // over the warp's maximum
+        s += v;
+        if (v != 0.f) sy += v * y;
+      }
+      s = warp_sum(s);
+      sy = warp_sum(sy);
+    }
+    if (lane == 0) s_entries[warp] = make_float3(m, s, sy);
+  }
+  if ((v0 == 0 && lead != 0) || first + vocab < n * VEC) {  // vectors of which the row has a part
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int at = (lane + 32 * i) * VEC;
+      if (at < first || at + VEC > first + vocab) mask_vector<T>(q[i], first - at, first + vocab - at);
+    }
+  }
   float m = -INFINITY;
   if constexpr (HALF) {
     __nv_bfloat162 top = __float2bfloat162_rn(-INFINITY);
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) {
-      const uint4 q = vec[i];
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q[i]);
       top = __hmax2(__hmax2(top, __hmax2(h[0], h[1])), __hmax2(h[2], h[3]));
     }
     m = fmaxf(__low2float(top), __high2float(top));
   } else {
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) {
-      float f[VEC];
-      unpack<T>(vec[i], f);
-      m = fmaxf(m, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
-    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(q[i].x), __uint_as_float(q[i].y)), fmaxf(__uint_as_float(q[i].z), __uint_as_float(q[i].w))));
   }
   m = c * warp_max(m);
   const float own = (m == -INFINITY ? 0.f : m) - (HALF ? 15.f : 0.f);  // M'
-  float s = 0.f;
-#pragma unroll 2
-  for (int i = lane; i < n; i += 32) {
-    float f[VEC];
-    unpack<T>(vec[i], f);
+  const uint64_t c2 = pack_f2(c, c), from2 = pack_f2(-own, -own);
+  uint64_t sum2 = pack_f2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      f[j] = ex2(fmaf(f[j], c, -own));
-      s += f[j];
-    }
-    if (g != nullptr) {
-      uint4 q;
-      uint32_t* w = &q.x;
+  for (int i = 0; i < VECS; ++i) {
+    if (32 * i >= n) break;
+    uint32_t* w = &q[i].x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
-        else w[j] = __float_as_uint(f[j]);
-      }
-      vec[i] = q;
+    for (int j = 0; j < VEC / 2; ++j) {
+      float lo, hi;
+      if constexpr (HALF) lo = bf16_lo(w[j]), hi = bf16_hi(w[j]);
+      else lo = __uint_as_float(w[2 * j]), hi = __uint_as_float(w[2 * j + 1]);
+      unpack_f2(fma_f2(pack_f2(lo, hi), c2, from2), lo, hi);
+      lo = ex2(lo);
+      hi = ex2(hi);
+      sum2 = add_f2(sum2, pack_f2(lo, hi));
+      if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(hi), "f"(lo));
+      else w[2 * j] = __float_as_uint(lo), w[2 * j + 1] = __float_as_uint(hi);
     }
   }
-  s = warp_sum(arrived ? s : NAN);
+  float s, s_hi;
+  unpack_f2(sum2, s, s_hi);
+  s = warp_sum(s + s_hi);
   if (lane == 0) s_part[warp] = make_float2(m == -INFINITY ? -INFINITY : own, s);
+  if (threadIdx.x < src.K) e.at[threadIdx.x] = c * at_first;
   if (ctas > 1) cluster_sync_all();  // (the entries' logits have been read, too: they may be overwritten)
   else __syncthreads();
-  float2 part[MAX_ROW_WARPS / 32];
-  float base = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < MAX_ROW_WARPS / 32; ++i) {
-    const int w = lane + 32 * i;
-    part[i] = make_float2(-INFINITY, 0.f);
-    if (w < warps * ctas) {
-      if (ctas == 1) part[i] = s_part[w];
-      else
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                     : "=f"(part[i].x), "=f"(part[i].y)
-                     : "r"(mapa_shared(smem_u32(&s_part[w % warps]), w / warps)));
-    }
-    base = fmaxf(base, part[i].x);
-  }
+  auto part = [&](int w) {
+    if (ctas == 1) return s_part[w];
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                 : "=f"(v.x), "=f"(v.y)
+                 : "r"(mapa_shared(smem_u32(&s_part[w % warps]), w / warps)));
+    return v;
+  };
+  // Up to 32 warps have a part per lane; more go through twice.
+  const int all_warps = warps * ctas;
+  const float2 mine = lane < all_warps ? part(lane) : make_float2(-INFINITY, 0.f);
+  float base = mine.x;
+  for (int i = lane + 32; i < all_warps; i += 32) base = fmaxf(base, part(i).x);
   base = warp_max(base);
   if (base == -INFINITY) base = 0.f;
-  s = 0.f;
-#pragma unroll
-  for (int i = 0; i < MAX_ROW_WARPS / 32; ++i) s += part[i].y * ex2(part[i].x - base);
+  s = mine.y * ex2(mine.x - base);
+  for (int i = lane + 32; i < all_warps; i += 32) {
+    const float2 v = part(i);
+    s += v.y * ex2(v.x - base);
+  }
   s = warp_sum(s);
-  const float log2_s = log2f(s);
-  const bool counts = sh.counts;
+  if (ctas > 1) cluster_arrive();  // this warp has read its peers' parts
+  // The teacher's softmax: p of an entry is its 2^(y - max of its warp's) times that warp's weight.
+  const float3 ent = lane < warps ? s_entries[lane] : make_float3(-INFINITY, 0.f, 0.f);
+  const float ent_top = warp_max(ent.x);
+  const bool counts = ent_top != -INFINITY;
+  float weight = ex2(ent.x - (counts ? ent_top : 0.f));
+  const float ent_sum = warp_sum(ent.y * weight), over = 1.f / ent_sum;
   if (rank == 0 && warp == warps - 1) {
+    // sum p log2 p = sum p (y - max) - log2 of the sum
+    const float p_log_p = warp_sum(ent.y == 0.f ? 0.f : weight * (ent.z + ent.y * (ent.x - ent_top))) * over - log2f(ent_sum);
+    const float log2_s = log2f(s);
     float cross = 0.f;  // sum_k p_k log2 q_k
-    for (int k = lane; k < src.K; k += 32)
-      if (e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
+    for (int k0 = 0; k0 < src.K; k0 += 32) {
+      const int k = k0 + lane;
+      const float v = __shfl_sync(0xffffffffu, weight, (k0 % blockDim.x) >> 5) * (k < src.K ? e.p[k] : 0.f);
+      if (v != 0.f) cross += v * over * ((e.at[k] - base) - log2_s);
+    }
     cross = warp_sum(cross);
     if (lane == 0) {
-      terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
+      terms.loss[row] = counts ? terms.tau * terms.tau * (LN2 * (p_log_p - cross)) : 0.f;
       if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
     }
   }
+  weight *= over;
   if (g != nullptr) {
     T* y = g + row * ld_g;
-    const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
-    const float factor = counts ? ex2(own - base) * (scale / s) : 0.f;
+    const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f;
+    const float factor = ex2(own - base) * (scale / s);
+    const uint64_t f2 = pack_f2(factor, factor);
     const bool in_step = static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
-#pragma unroll 2
-    for (int i = lane; i < n; i += 32) {
-      const uint4 in = vec[i];
-      const uint32_t* w = &in.x;
-      uint4 q;
-      uint32_t* o = &q.x;
+    const int at0 = lane * VEC - first;  // the row's element at the lane's first vector
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (HALF) {
+    for (int i = 0; i < VECS; ++i) {
+      if (32 * i >= n) break;
+      uint32_t* w = &q[i].x;
+      if constexpr (HALF) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          o[j] = pack_bf16x2(h.x * factor, h.y * factor);
-        } else {
-          o[j] = __float_as_uint(__uint_as_float(w[j]) * factor);
+          float lo, hi;
+          unpack_f2(mul_f2(pack_f2(h.x, h.y), f2), lo, hi);
+          w[j] = pack_bf16x2(lo, hi);
         }
-      }
-      if (!counts) q = make_uint4(0, 0, 0, 0);  // (whatever the logits were)
-      const int v = v0 + i;
-      if (in_step && v >= whole0 && v < whole1) {
-        *reinterpret_cast<uint4*>(y - lead + static_cast<long long>(v) * VEC) = q;
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int at = v * VEC + j - lead;
-          if (at >= 0 && at < vocab) y[at] = reinterpret_cast<const T*>(&q)[j];
-        }
+        for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * factor);
+      }
+      if (!counts) q[i] = make_uint4(0, 0, 0, 0);  // (whatever the logits were)
+      const int at = at0 + i * 32 * VEC;
+      if (lane + 32 * i >= n) continue;
+      if (in_step && at >= 0 && at + VEC <= vocab) {
+        *reinterpret_cast<uint4*>(y + at) = q[i];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at + j >= 0 && at + j < vocab) {
+            if constexpr (HALF) reinterpret_cast<uint16_t*>(y)[at + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+            else reinterpret_cast<uint32_t*>(y)[at + j] = w[j];
+          }
       }
     }
-    merge_entries(e, src.K);
-    __syncthreads();
-    const int first = rank * warps * slice * VEC - lead, last = first + warps * slice * VEC;  // the CTA's elements
-    for (int k = threadIdx.x; k < src.K; k += blockDim.x)
-      if (e.sum[k] != -1.f && e.id[k] >= first && e.id[k] < last)
-        y[e.id[k]] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - e.sum[k]));
+    __syncwarp();
+    // The entries in this slice, each id once: the sum of its entries' probabilities, in their order.
+    for (int k0 = 0; k0 < src.K; k0 += 32) {
+      const int k = k0 + lane, id = k < src.K ? e.id[k] : -1, at = id + first;
+      float p = __shfl_sync(0xffffffffu, weight, (k0 % blockDim.x) >> 5);
+      if (id < 0 || at < 0 || at >= n * VEC) continue;
+      p *= e.p[k];
+      if (is_marked(table, slots_log2, id)) {
+        p = 0.f;
+        bool again = false;
+        for (int i = 0; i < src.K; ++i) {
+          if (e.id[i] != id) continue;
+          again = again || i < k;
+          const float3 of = s_entries[(i % blockDim.x) >> 5];
+          p += ex2(of.x - ent_top) * over * e.p[i];
+        }
+        if (again) continue;
+      }
+      y[id] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - p));
+    }
   }
-  if (threadIdx.x == 0 && abort_word != 0) {
-    const unsigned long long t0 = globaltimer_ns();  // a copy that may still be under way lands before its memory is given up
-    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    atomicExch(status, abort_word);
-  }
-  if (ctas > 1) cluster_sync_all();  // the peers have read (M', S')
+  if (ctas > 1) cluster_wait();  // the peers have read this CTA's parts
 }
 
 // ------------------------------------------------------------------------------------------ rows behind the fused product
@@ -450,8 +555,9 @@ __global__ void __launch_bounds__(PREPARE_WARPS * 32)
   const long long row = static_cast<long long>(blockIdx.x) * PREPARE_WARPS + warp;
   if (row >= rows) return;
   const RowEntries e(smem + static_cast<size_t>(warp) * ENTRY_BYTES * src.K, src.K);
-  int* sorted = reinterpret_cast<int*>(e.sum);
-  load_entries(e, shared[warp], src, row, vocab, tau);
+  int* sorted = reinterpret_cast<int*>(e.at);
+  load_entries<float>(e, shared[warp], src, row, vocab, tau, nullptr);
+  __syncwarp();
   for (int k = lane; k < src.K; k += 32) sorted[k] = INT32_MAX;
   __syncwarp();
   if (lane == 0) p_log_p[row] = shared[warp].p_log_p;
@@ -702,25 +808,26 @@ static RowTerms from_row(RowTerms t, long long row) {
   return t;
 }
 
-// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and more, 16 for each of as many CTAs as keep
-// three shares on an SM.  More CTAs share those warps while SMs are without one and a warp's slice stays above 2 KB.
-// warps = 0: rows of over 1.6 MB, which are read twice.
-static Share choose_share(long long rows, int vocab, int size, int K) {
+// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and 64 KB, 16 for each of up to 8 CTAs up to 512 KB
+// (a lane has 8 vectors of a slice then, 16 up to 1 MB).  More CTAs share those warps while SMs are without one.
+// warps = 0: longer rows, which are read twice.
+struct Share {
+  int warps, slice, ctas, slots_log2;  // warps of a row, vectors of a warp, CTAs of a row, the entries' hash table
+  size_t smem;                         // of a CTA
+};
+static Share choose_share(const void* z, long long ld, long long rows, int vocab, int size, int K) {
   const int vec = 16 / size;
-  const long long vecs = up(vocab + vec - 1, vec) / vec, entry = static_cast<long long>(ENTRY_BYTES) * K;
+  const bool on_grid = (reinterpret_cast<uintptr_t>(z) & 15) == 0 && (rows == 1 || ld * size % 16 == 0);
+  const long long vecs = (static_cast<long long>(vocab) + (on_grid ? 1 : 2) * (vec - 1)) / vec;  // (wherever the row starts in its first)
   Share s = {};
-  s.warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : 16;
-  s.ctas = 1;
-  auto slice = [&] { return up(vecs, s.warps) / s.warps; };
-  auto bytes = [&] { return s.warps / s.ctas * slice() * 16 + entry; };
-  while (s.ctas < 8 && bytes() > SHARE_BYTES) {
-    s.ctas *= 2;
-    s.warps = 16 * s.ctas;
-  }
-  if (bytes() > 200 * 1024) return {};
-  s.vecs = static_cast<int>(slice());
-  while (s.ctas < 8 && rows * s.ctas < sm_count() && s.warps / s.ctas >= 2 && s.vecs >= 128) s.ctas *= 2;
-  s.smem = static_cast<size_t>(bytes());
+  s.ctas = vecs <= 8 * 16 * 256 ? static_cast<int>((vecs + 16 * 256 - 1) / (16 * 256)) : 8;
+  s.warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : WARPS * s.ctas;
+  s.slice = static_cast<int>((vecs + s.warps - 1) / s.warps);
+  if (s.slice > 512) return {};
+  while (2 * s.ctas <= 8 && rows * s.ctas < sm_count() && s.warps / s.ctas >= 2 && s.slice >= 64) s.ctas *= 2;
+  s.slots_log2 = 5;
+  while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (2 K: 8192 x 32768 with 64 random ids 290 us, not PH)
+  s.smem = static_cast<size_t>(ENTRY_BYTES) * K + (4u << s.slots_log2);  // at most 44 KB
   return s;
 }
 
@@ -728,25 +835,18 @@ template <typename T>
 static int32_t launch_rows(const void* z, long long ld_z, void* g, long long ld_g, long long rows, int vocab, const Entries& e,
                            const RowTerms& t, cudaStream_t stream) {
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * sizeof(T) * (g ? 2 : 1), stream);
-  const Share share = choose_share(rows, vocab, sizeof(T), e.K);
+  const Share share = choose_share(z, ld_z, rows, vocab, sizeof(T), e.K);
   if (share.warps == 0 || rows * share.ctas > INT32_MAX) {
     CDL_CUDA(launch_pdl(loss_row_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(z),
                         ld_z, static_cast<T*>(g), ld_g, vocab, e, t));
     return CDL_OK;
   }
-  static std::once_flag once[64];
-  int dev = 0;
-  CDL_CUDA(cudaGetDevice(&dev));
-  cudaError_t err = cudaSuccess;
-  std::call_once(once[dev & 63], [&] {
-    err = cudaFuncSetAttribute(loss_share_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  });
-  if (err != cudaSuccess) return fail(CDL_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(err));
-  int* status = device_status_ptr();
-  if (!status) return fail(CDL_ERR_CUDA, "cannot resolve the device status word");
-  CDL_CUDA(launch_pdl_cluster(loss_share_kernel<T>, dim3(static_cast<unsigned>(rows * share.ctas)), dim3(share.warps / share.ctas * 32),
-                              share.smem, share.ctas, stream, static_cast<const T*>(z), ld_z, static_cast<T*>(g), ld_g, vocab,
-                              share.vecs, share.ctas, e, t, status));
+  auto kernel = share.slice <= 256 ? loss_slices_kernel<T, 8> : loss_slices_kernel<T, 16>;
+  // (rows that run at once, two CTAs of 16 warps or as many threads per SM)
+  const long long ahead = static_cast<long long>(sm_count()) * (share.slice <= 256 ? 1024 : 512) / (share.warps * 32);
+  CDL_CUDA(launch_pdl_cluster(kernel, dim3(static_cast<unsigned>(rows * share.ctas)), dim3(share.warps / share.ctas * 32), share.smem,
+                              share.ctas, stream, static_cast<const T*>(z), ld_z, static_cast<T*>(g), ld_g, rows, ahead, vocab,
+                              share.slice, share.ctas, share.slots_log2, e, t));
   return CDL_OK;
 }
 
@@ -1138,6 +1238,11 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
     float* planes = reinterpret_cast<float*>(base + p.at_planes);
     if (p.slices > 1) {
       CDL_CHECK(matmul_planes_execute(&g, &wt, planes, x_ld, p.slices, stream));
+      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 7) == 0 && (n == 1 || d.stride[0] % 4 == 0);
+      ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(n) * p.D * (4 * p.slices + 2), stream);
+      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * ((p.D + 3) / 4) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
+                          p.slices, static_cast<__nv_bfloat16*>(d.ptr), static_cast<long long>(d.stride[0]), static_cast<int>(n),
+                          static_cast<int>(p.D), vectors ? 1 : 0));
     } else if (p.has_dx) {
       CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
     }
@@ -1149,13 +1254,6 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       if (fused && !add && matmul_store_bound(a, b, d)) CDL_CHECK(matmul_store_execute(a, b, d, stream, p.has_dx ? 1 : 0));
       else CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
                                fused && p.has_dx ? 1 : 0));
-    }
-    if (p.slices > 1) {
-      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 7) == 0 && (n == 1 || d.stride[0] % 4 == 0);
-      ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(n) * p.D * (4 * p.slices + 2), stream);
-      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * ((p.D + 3) / 4) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
-                          p.slices, static_cast<__nv_bfloat16*>(d.ptr), static_cast<long long>(d.stride[0]), static_cast<int>(n),
-                          static_cast<int>(p.D), vectors ? 1 : 0));
     }
   }
   if (p.sums) {
