@@ -128,7 +128,8 @@ if not LIB_PATH.exists():
     )
 
 lib = ctypes.CDLL(str(LIB_PATH))
-# The same library for callers that pass every `const cdl_tensor*` as the bytes of tensor_bytes(): nothing else is taken there.
+# The same library for callers that pass every `const cdl_tensor*` as the bytes of tensor_bytes() and every
+# `const cdl_head_loss_desc*` as those of head_loss_bytes(): nothing else is taken there.
 packed_lib = ctypes.CDLL(str(LIB_PATH))
 
 _T = ctypes.POINTER(CdlTensor)
@@ -237,9 +238,9 @@ SIGNATURES = {
 }
 
 for _name, (_args, _res) in SIGNATURES.items():
-    for _of, _tensor in ((lib, _T), (packed_lib, ctypes.c_char_p)):
+    for _of, _tensor, _desc in ((lib, _T, _HL), (packed_lib, ctypes.c_char_p, ctypes.c_char_p)):
         _fn = getattr(_of, _name)
-        _fn.argtypes = [_tensor if a is _T else a for a in _args]
+        _fn.argtypes = [_tensor if a is _T else _desc if a is _HL else a for a in _args]
         _fn.restype = _res
 
 
@@ -276,6 +277,16 @@ def tensor_bytes(t):
         raise CdlError(-1, f"rank {rank} exceeds 4")
     rest = _UNUSED[rank]
     return _pack_tensor(t.data_ptr(), dt, rank, *shape, *rest, *t.stride(), *rest)
+
+
+def rows_bytes(ptr: int, n: int) -> bytes:
+    """The bytes of a cdl_tensor for n packed f32 values."""
+    return _pack_tensor(ptr, CDL_F32, 1, n, 0, 0, 0, 1, 0, 0, 0)
+
+
+_HEAD_LOSS_BYTES = struct.Struct("ffiq")  # the layout of cdl_head_loss_desc
+assert _HEAD_LOSS_BYTES.size == ctypes.sizeof(CdlHeadLossDesc)
+head_loss_bytes = _HEAD_LOSS_BYTES.pack  # (temperature, grad_scale, accumulate_dw, chunk_rows)
 
 
 def tensor_arg(t):

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(ROW_THREADS)
 // f16 of up to 2^15, see store_tile_rows_exp in gemm.cu; their sum is of the f32 values); and, behind the one barrier at
 // which the slices' parts of the statistics meet, the gradient.  The row's entries are a thread's each, and their softmax
 // meets at the same barrier: where one warp prepared them all, the others waited for it (8192 x 32768 with 64
-// entries 244 us; PLACEHOLDER).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
+// entries 244 us, not 216).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
 // whose share of the HBM's rate takes 5500.  The slices depend on the vocabulary alone, not on how many CTAs share a row, so
 // a row's results do not depend on the number of rows.
 //
@@ -808,9 +808,9 @@ static RowTerms from_row(RowTerms t, long long row) {
   return t;
 }
 
-// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and 64 KB, 16 for each of up to 8 CTAs up to 512 KB
-// (a lane has 8 vectors of a slice then, 16 up to 1 MB).  More CTAs share those warps while SMs are without one.
-// warps = 0: longer rows, which are read twice.
+// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and 64 KB; longer rows in a cluster of up to 8 CTAs,
+// of 8 warps up to 256 KB (1500 x 50000 f32 168 us; with 16 195), else of 16: 512 KB, and 1 MB with 16 vectors a lane.
+// More CTAs share those warps while SMs are without one.  warps = 0: longer rows, which are read twice.
 struct Share {
   int warps, slice, ctas, slots_log2;  // warps of a row, vectors of a warp, CTAs of a row, the entries' hash table
   size_t smem;                         // of a CTA
@@ -820,13 +820,15 @@ static Share choose_share(const void* z, long long ld, long long rows, int vocab
   const bool on_grid = (reinterpret_cast<uintptr_t>(z) & 15) == 0 && (rows == 1 || ld * size % 16 == 0);
   const long long vecs = (static_cast<long long>(vocab) + (on_grid ? 1 : 2) * (vec - 1)) / vec;  // (wherever the row starts in its first)
   Share s = {};
-  s.ctas = vecs <= 8 * 16 * 256 ? static_cast<int>((vecs + 16 * 256 - 1) / (16 * 256)) : 8;
-  s.warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : WARPS * s.ctas;
+  const int warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : vecs <= 16 * 256 || vecs > 8 * 8 * 256 ? 16 : 8;  // of a CTA
+  const long long ctas = (vecs + warps * 256 - 1) / (warps * 256);
+  s.ctas = ctas <= 8 ? static_cast<int>(ctas) : 8;
+  s.warps = warps * s.ctas;
   s.slice = static_cast<int>((vecs + s.warps - 1) / s.warps);
   if (s.slice > 512) return {};
   while (2 * s.ctas <= 8 && rows * s.ctas < sm_count() && s.warps / s.ctas >= 2 && s.slice >= 64) s.ctas *= 2;
   s.slots_log2 = 5;
-  while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (2 K: 8192 x 32768 with 64 random ids 290 us, not PH)
+  while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (with 2 K slots 64 random ids cost 8192 x 32768 290 us, not 228)
   s.smem = static_cast<size_t>(ENTRY_BYTES) * K + (4u << s.slots_log2);  // at most 44 KB
   return s;
 }
@@ -842,7 +844,7 @@ static int32_t launch_rows(const void* z, long long ld_z, void* g, long long ld_
     return CDL_OK;
   }
   auto kernel = share.slice <= 256 ? loss_slices_kernel<T, 8> : loss_slices_kernel<T, 16>;
-  // (rows that run at once, two CTAs of 16 warps or as many threads per SM)
+  // Rows that run at once: two CTAs of 16 warps, or as many threads in more, per SM.
   const long long ahead = static_cast<long long>(sm_count()) * (share.slice <= 256 ? 1024 : 512) / (share.warps * 32);
   CDL_CUDA(launch_pdl_cluster(kernel, dim3(static_cast<unsigned>(rows * share.ctas)), dim3(share.warps / share.ctas * 32), share.smem,
                               share.ctas, stream, static_cast<const T*>(z), ld_z, static_cast<T*>(g), ld_g, rows, ahead, vocab,

@@ -322,22 +322,23 @@ class LinearLossOutputs:
 
 def _require_current_device(*tensors):
     """The kernels run on the current device's current stream: operands of another one are refused."""
-    _require_cuda(*tensors)
-    here = torch.cuda.current_device()
+    here = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
     for t in tensors:
-        if t is not None and t.device.index != here:
-            raise _lib.CdlError(-1, f"operands must live on the current device (cuda:{here}, got {t.device})")
+        if t is not None and (here < 0 or t.get_device() != here):
+            _require_cuda(t)
+            here = torch.cuda.current_device()
+            if t.get_device() != here:
+                raise _lib.CdlError(-1, f"operands must live on the current device (cuda:{here}, got {t.device})")
 
 
 def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
     if x.dim() != 2 or w.dim() != 2:
         raise _lib.CdlError(-1, f"{name}: x must be [tokens, hidden] and w [hidden, vocab]")
-    _require_current_device(x, w, *entries, opts.d_loss, dx, dw, scratch)
+    d_loss = opts.d_loss
+    _require_current_device(x, w, *entries, d_loss, dx, dw, scratch)
     if opts.accumulate and dw is None:
         raise _lib.CdlError(-1, f"{name}: accumulate needs the dw that is added to")
     want_x, want_w = opts.grad and (opts.grad_x or dx is not None), opts.grad and (opts.grad_w or dw is not None)
-    tokens = x.shape[0]
-    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=x.device)
     if not want_x:
         dx = None
     elif dx is None:
@@ -347,27 +348,29 @@ def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
     elif dw is None:  # laid out as w is
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w.stride(0) >= w.stride(1) else \
             torch.empty(w.shape[::-1], dtype=w.dtype, device=w.device).t()
-    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
-    tx, tw, tl, ts, tdl, tdx, tdw = (tensor_bytes(t) for t in (x, w, loss, lse, opts.d_loss, dx, dw))
-    te = [tensor_bytes(t) for t in entries]
-    n = ctypes.c_size_t(0)
-    check(packed_lib.cdl_b200_linear_loss_scratch_bytes(ctypes.byref(desc), tx, tw, entries[0].shape[-1] if len(entries) > 1 else 1,
-                                                        tdx, tdw, ctypes.byref(n)))
+    tokens, distil = x.shape[0], len(entries) > 1
+    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=x.device).unbind()
+    desc = _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
+    tx, tw, tdx, tdw = tensor_bytes(x), tensor_bytes(w), tensor_bytes(dx), tensor_bytes(dw)
     if scratch is None:
+        n = ctypes.c_size_t(0)
+        check(packed_lib.cdl_b200_linear_loss_scratch_bytes(desc, tx, tw, entries[0].shape[-1] if distil else 1, tdx, tdw,
+                                                            ctypes.byref(n)))
         scratch = torch.empty(max(n.value, 256), dtype=torch.uint8, device=x.device)
-    fn = packed_lib.cdl_b200_linear_distillation if len(entries) > 1 else packed_lib.cdl_b200_linear_cross_entropy
-    check(fn(ctypes.byref(desc), tx, tw, *te, tdl, tl, ts, tdx, tdw, scratch.data_ptr(),
-             scratch.numel() * scratch.element_size(), current_stream()))
+    fn = packed_lib.cdl_b200_linear_distillation if distil else packed_lib.cdl_b200_linear_cross_entropy
+    check(fn(desc, tx, tw, *map(tensor_bytes, entries), tensor_bytes(d_loss), _lib.rows_bytes(loss.data_ptr(), tokens),
+             _lib.rows_bytes(lse.data_ptr(), tokens), tdx, tdw, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+             current_stream()))
     return LinearLossOutputs(loss, lse, dx, dw)
 
 
 def linear_loss_scratch_bytes(x, w, opts: LinearLossOpts | None = None, entries: int = 1, dx=None, dw=None) -> int:
     """The scratch that the call below needs for these operands; dx, dw: the gradients' tensors, None where not wanted."""
     opts = opts or LinearLossOpts()
-    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
+    desc = _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
     n = ctypes.c_size_t(0)
-    check(packed_lib.cdl_b200_linear_loss_scratch_bytes(ctypes.byref(desc), tensor_bytes(x), tensor_bytes(w), entries,
-                                                        tensor_bytes(dx), tensor_bytes(dw), ctypes.byref(n)))
+    check(packed_lib.cdl_b200_linear_loss_scratch_bytes(desc, tensor_bytes(x), tensor_bytes(w), entries, tensor_bytes(dx),
+                                                        tensor_bytes(dw), ctypes.byref(n)))
     return n.value
 
 
@@ -410,13 +413,16 @@ def distillation(logits, teacher_ids, teacher_logits, opts: DistillationOpts | N
     opts = opts or DistillationOpts()
     if logits.dim() != 2:
         raise _lib.CdlError(-1, "distillation: logits must be [tokens, vocab]")
-    _require_current_device(logits, teacher_ids, teacher_logits, opts.d_loss, d_logits)
-    loss, lse = torch.empty(2, logits.shape[0], dtype=torch.float32, device=logits.device)
+    d_loss = opts.d_loss
+    _require_current_device(logits, teacher_ids, teacher_logits, d_loss, d_logits)
+    tokens = logits.shape[0]
+    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=logits.device).unbind()
     if not opts.grad:
         d_logits = None
     elif d_logits is None:
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    desc = _lib.CdlHeadLossDesc(opts.temperature, opts.grad_scale, 0, 0)
-    check(packed_lib.cdl_b200_distillation(ctypes.byref(desc), *(tensor_bytes(t) for t in (
-        logits, teacher_ids, teacher_logits, opts.d_loss, loss, lse, d_logits)), current_stream()))
+    check(packed_lib.cdl_b200_distillation(
+        _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 0, 0), tensor_bytes(logits), tensor_bytes(teacher_ids),
+        tensor_bytes(teacher_logits), tensor_bytes(d_loss), _lib.rows_bytes(loss.data_ptr(), tokens),
+        _lib.rows_bytes(lse.data_ptr(), tokens), tensor_bytes(d_logits), current_stream()))
     return DistillationOutputs(loss, lse, d_logits)
