@@ -417,6 +417,11 @@ __device__ __forceinline__ F32x2 fma2(F32x2 a, F32x2 b, F32x2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return d;
 }
+__device__ __forceinline__ F32x2 add2(F32x2 a, F32x2 b) {
+  F32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
 __device__ __forceinline__ F32x2 tanh2(F32x2 a) {
   float lo, hi;
   a.get(lo, hi);
@@ -576,8 +581,12 @@ struct Wanted {
 // t itself at the row's ids, and (with a gradient to come) the exponentials 2^(t - M') in f16.  Those are at most 2^15,
 // so they keep f16's 11 bits down to 2^-29 of the piece's largest: bf16's 8 would round the gradient a second time as
 // coarsely as its own rounding does.  128 accumulators at a time are a thread's registers: one read of the tensor memory.
-__device__ __forceinline__ void store_tile_rows_exp(const Params& p, uint32_t t_row, int row, int col_base, Wanted want) {
-  if (col_base >= p.N) return;  // warp-uniform
+// Up to a K of about 1000 these warps, not the products, set the pace.  Packed arithmetic, and (TMA) the exponentials stored
+// as two boxes of 32 x 64 from the warp's 4 KiB buffer instead of 32 bytes of 32 rows per instruction: EXP_TIMES.
+template <bool TMA>
+__device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row, int row,
+                                                    int col_base, int lane, Wanted want) {
+  if (col_base >= p.N || row - lane >= p.M) return;  // warp-uniform
   uint32_t r[4][32];
   tmem_ld32(t_row, r[0]);
   tmem_ld32(t_row + 32, r[1]);
@@ -603,33 +612,61 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, uint32_t t_
       }
     }
   }
-  if (row >= p.M) return;
   float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int j = 0; j < 32; ++j) m4[c] = fmaxf(m4[c], __uint_as_float(r[c][j]));
+    for (int j = 0; j < 32; j += 2) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1])));
   const float m = p.alpha * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
   const float base = (m == -INFINITY ? 0.f : m) - 15.f;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  const F32x2 scale(p.alpha, p.alpha), from(-base, -base);
+  F32x2 s[2] = {F32x2(0.f, 0.f), F32x2(0.f, 0.f)};
   __half* dp = static_cast<__half*>(p.d) + static_cast<long long>(row) * p.ldd + col_base;
+  const bool store = p.d != nullptr;
+  const uint32_t line = smem_u32(buf) + lane * 128, x = (lane & 7) << 4;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float e0, e1;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fmaf(__uint_as_float(r[c][g * 16 + 2 * j]), p.alpha, -base)));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fmaf(__uint_as_float(r[c][g * 16 + 2 * j + 1]), p.alpha, -base)));
-        s[c] += e0 + e1;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(e1), "f"(e0));
+    for (int j = 0; j < 16; ++j) {
+      const F32x2 t = fma2(F32x2(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), scale, from);
+      float e0, e1;
+      t.get(e0, e1);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+      s[j & 1] = add2(s[j & 1], F32x2(e0, e1));
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(e1), "f"(e0));
+    }
+    if (!store) continue;
+    if constexpr (TMA) {
+      if ((c & 1) == 0) {
+        if (lane == 0) tma_store_wait_read<0>();  // the buffer's last store has read it
+        __syncwarp();
       }
-      if (p.d != nullptr) st_global_v8(dp + c * 32 + g * 16, w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((((c & 1) * 4 + k) << 4) ^ x)), "r"(w[4 * k]),
+                     "r"(w[4 * k + 1]), "r"(w[4 * k + 2]), "r"(w[4 * k + 3])
+                     : "memory");
+      if ((c & 1) == 1) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(tm_d, buf, col_base + (c - 1) * 32, row, 0);
+          tma_store_commit();
+        }
+      }
+    } else if (row < p.M) {
+      st_global_v8(dp + c * 32, reinterpret_cast<const uint32_t(&)[8]>(w[0]));
+      st_global_v8(dp + c * 32 + 16, reinterpret_cast<const uint32_t(&)[8]>(w[8]));
     }
   }
-  p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] = make_float2(m == -INFINITY ? -INFINITY : base, (s[0] + s[1]) + (s[2] + s[3]));
+  if (row >= p.M) return;
+  float a0, a1, b0, b1;
+  s[0].get(a0, a1);
+  s[1].get(b0, b1);
+  p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] =
+      make_float2(m == -INFINITY ? -INFINITY : base, (a0 + a1) + (b0 + b1));
 }
 
 // One kernel per kind of store.  All of them in one, with the buffers that the plain ones do not need (they take room
@@ -789,7 +826,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
       const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
       if constexpr (KIND == STORE_EXP) {
-        store_tile_rows_exp(p, t_row, row, col, want);
+        store_tile_rows_exp<false>(p, nullptr, nullptr, t_row, row, col, lane, want);
       } else if constexpr (KIND == STORE_PLANES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else {
@@ -831,7 +868,7 @@ constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = 2 * A_BYTES;  // A 128 x 64 and half of B 128 x 64
 constexpr int PAIR_M = 2 * BM;
 constexpr int PAIR_BARRIER_BYTES = 512;
-constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_EXP || kind == STORE_PLANES ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
+constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_PLANES ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
 constexpr size_t pair_smem_bytes(int kind) {
   return 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + pair_staging(kind) + PAIR_BARRIER_BYTES;
 }
@@ -1092,7 +1129,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (p.epi_mode == 1) store_tile_rows_swiglu<false>(p, feed, t_row, row, col, lane, abort_word);
         else store_tile_rows_swiglu<true>(p, feed, t_row, row, col, lane, abort_word);
       } else if constexpr (KIND == STORE_EXP) {
-        store_tile_rows_exp(p, t_row, row, col, want);
+        store_tile_rows_exp<true>(p, &tmap_e0, buf, t_row, row, col, lane, want);
       } else if constexpr (KIND == STORE_PLANES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else if constexpr (KIND == STORE_BF16) {
@@ -1105,7 +1142,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[acc]), 0));
     }
-    if ((KIND == STORE_ADD || KIND == STORE_BF16) && lane == 0) tma_store_wait<0>();
+    if ((KIND == STORE_ADD || KIND == STORE_BF16 || KIND == STORE_EXP) && lane == 0) tma_store_wait<0>();
   }
 
   // ------------------------------------------------------------ tear-down
@@ -1728,7 +1765,14 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
   p.ldd = ldd;
   p.alpha = scale;
   p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
-  return pair ? pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
+  CUtensorMap tm_d = tm_a;  // (a valid map where none is used)
+  if (pair && d != nullptr) {
+    const uint64_t ld = static_cast<uint64_t>(ldd) * 2;
+    const uint64_t dims[3] = {static_cast<uint64_t>(ldd), static_cast<uint64_t>(p.M), 1}, strides[3] = {0, ld, ld * p.M};
+    const uint32_t box[3] = {64, 32, 1};
+    CDL_CHECK(encode_tmap(&tm_d, d, CDL_BF16, 3, dims, strides, box, true));  // (16 bits each, moved as they are)
+  }
+  return pair ? pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, tm_d, 0, stream) : one_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
 }
 
 // K slices of a product whose output is small and whose K is long (dx of a head: K is the vocabulary), each stored in f32 in
