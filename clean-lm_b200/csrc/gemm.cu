@@ -512,7 +512,7 @@ __device__ __forceinline__ void add_tile_rows(const Params& p, const CUtensorMap
 
 // The epilogue of a bf16 D = alpha * accumulator for the calling warp: rows row0 .. row0 + 31, 128 columns, as two TMA stores
 // of 32 x 64 from its 4 KiB buffer (128-byte swizzle).  A thread's own stores cover 32 bytes of 32 rows per instruction; a
-// product of a short K is bound by them: 2048 x 32768 with K = 64 STORE_BF16_TIMES.
+// product of a short K is bound by them: 2048 x 32768 with K = 64 45 -> 31 us (134 MB).
 __device__ __forceinline__ void store_tile_rows_tma(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row,
                                                     int b, int row0, int col_base, int lane) {
   if (row0 >= p.M) return;  // warp-uniform; rows past M inside the box are clipped
@@ -582,7 +582,8 @@ struct Wanted {
 // so they keep f16's 11 bits down to 2^-29 of the piece's largest: bf16's 8 would round the gradient a second time as
 // coarsely as its own rounding does.  128 accumulators at a time are a thread's registers: one read of the tensor memory.
 // Up to a K of about 1000 these warps, not the products, set the pace.  Packed arithmetic, and (TMA) the exponentials stored
-// as two boxes of 32 x 64 from the warp's 4 KiB buffer instead of 32 bytes of 32 rows per instruction: EXP_TIMES.
+// as two boxes of 32 x 64 from the warp's 4 KiB buffer instead of 32 bytes of 32 rows per instruction: 8192 x 512
+// x 32768 271 -> 226 us.
 template <bool TMA>
 __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row, int row,
                                                     int col_base, int lane, Wanted want) {
@@ -1754,7 +1755,7 @@ static int32_t one_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtens
 }
 
 // The logits of a loss (see store_tile_rows_exp).  Up to 128 rows one CTA per 256 columns: a pair's second half would have no
-// rows but take as long over its products, which then, not the bytes of B, set the time (64 x 2048 x 32768 EXP_ONE_TIMES).
+// rows but take as long over its products, which then, not the bytes of B, set the time (64 x 2048 x 32768 40 -> 32 us).
 int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
                            cudaStream_t stream) {
   gemm::Params p;
@@ -1763,7 +1764,10 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
   CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, pair));
   p.d = d;
   p.ldd = ldd;
-  p.alpha = scale;
+  // A tensor-core accumulator truncates: the sum of n steps of 16 products lies about 1.6e-8 n below its value (measured in
+  // gemm_general.cu).  Put back, the loss of a trained head is 1.7e-7 off at K = 2048 and 4.3e-7 at 4096 (2-norm, against
+  // f64; f32 products 1.9e-7 and 4.1e-7), without it 7.5e-7 and 2.0e-6.
+  p.alpha = static_cast<float>(scale * (1.0 + 1e-9 * p.K));
   p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
   CUtensorMap tm_d = tm_a;  // (a valid map where none is used)
   if (pair && d != nullptr) {

@@ -441,56 +441,60 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
     s += v.y * ex2(v.x - base);
   }
   s = warp_sum(s);
-  if (ctas > 1) cluster_arrive();  // this warp has read its peers' parts
+  if (ctas > 1) cluster_arrive_relaxed();  // this warp has read its peers' parts
   // The teacher's softmax: p of an entry is its 2^(y - max of its warp's) times that warp's weight.
-  const float3 ent = lane < warps ? s_entries[lane] : make_float3(-INFINITY, 0.f, 0.f);
-  const float ent_top = warp_max(ent.x);
+  const int holders = min(warps, (src.K + 31) / 32);
+  float ent_top = -INFINITY, ent_sum = 0.f;
+  for (int i = 0; i < holders; ++i) ent_top = fmaxf(ent_top, s_entries[i].x);
   const bool counts = ent_top != -INFINITY;
-  float weight = ex2(ent.x - (counts ? ent_top : 0.f));
-  const float ent_sum = warp_sum(ent.y * weight), over = 1.f / ent_sum;
+  for (int i = 0; i < holders; ++i) ent_sum += s_entries[i].y * ex2(s_entries[i].x - ent_top);  // (counts)
+  const float over = 1.f / ent_sum;
+  auto weight_of = [&](int k) { return ex2(s_entries[(k % blockDim.x) >> 5].x - ent_top) * over; };  // (uniform in a warp's 32 entries)
   if (rank == 0 && warp == warps - 1) {
-    // sum p log2 p = sum p (y - max) - log2 of the sum
-    const float p_log_p = warp_sum(ent.y == 0.f ? 0.f : weight * (ent.z + ent.y * (ent.x - ent_top))) * over - log2f(ent_sum);
     const float log2_s = log2f(s);
-    float cross = 0.f;  // sum_k p_k log2 q_k
-    for (int k0 = 0; k0 < src.K; k0 += 32) {
-      const int k = k0 + lane;
-      const float v = __shfl_sync(0xffffffffu, weight, (k0 % blockDim.x) >> 5) * (k < src.K ? e.p[k] : 0.f);
-      if (v != 0.f) cross += v * over * ((e.at[k] - base) - log2_s);
+    // sum_k p_k (log2 p_k - log2 q_k); the first part: sum p (y - max) - log2 of the sum
+    float sum = 0.f;
+    for (int k = lane; k < src.K; k += 32) {
+      const float v = e.p[k];
+      if (v != 0.f) sum -= v * weight_of(k) * ((e.at[k] - base) - log2_s);
     }
-    cross = warp_sum(cross);
+    if (lane < holders && s_entries[lane].y != 0.f) {
+      const float3 v = s_entries[lane];
+      sum += ex2(v.x - ent_top) * over * (v.z + v.y * (v.x - ent_top));
+    }
+    sum = warp_sum(sum) - log2f(ent_sum);
     if (lane == 0) {
-      terms.loss[row] = counts ? terms.tau * terms.tau * (LN2 * (p_log_p - cross)) : 0.f;
+      terms.loss[row] = counts ? terms.tau * terms.tau * LN2 * sum : 0.f;
       if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
     }
   }
-  weight *= over;
   if (g != nullptr) {
     T* y = g + row * ld_g;
     const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f;
     const float factor = ex2(own - base) * (scale / s);
-    const uint64_t f2 = pack_f2(factor, factor);
     const bool in_step = static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
     const int at0 = lane * VEC - first;  // the row's element at the lane's first vector
+    const uint64_t f2 = pack_f2(factor, factor);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       if (32 * i >= n) break;
       uint32_t* w = &q[i].x;
-      if constexpr (HALF) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; j += HALF ? 1 : 2) {
+        float lo, hi;
+        if constexpr (HALF) {
           const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          float lo, hi;
           unpack_f2(mul_f2(pack_f2(h.x, h.y), f2), lo, hi);
           w[j] = pack_bf16x2(lo, hi);
+        } else {
+          unpack_f2(mul_f2(pack_f2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), f2), lo, hi);
+          w[j] = __float_as_uint(lo);
+          w[j + 1] = __float_as_uint(hi);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * factor);
       }
       if (!counts) q[i] = make_uint4(0, 0, 0, 0);  // (whatever the logits were)
-      const int at = at0 + i * 32 * VEC;
       if (lane + 32 * i >= n) continue;
+      const int at = at0 + i * 32 * VEC;
       if (in_step && at >= 0 && at + VEC <= vocab) {
         *reinterpret_cast<uint4*>(y + at) = q[i];
       } else {
@@ -504,19 +508,17 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
     }
     __syncwarp();
     // The entries in this slice, each id once: the sum of its entries' probabilities, in their order.
-    for (int k0 = 0; k0 < src.K; k0 += 32) {
-      const int k = k0 + lane, id = k < src.K ? e.id[k] : -1, at = id + first;
-      float p = __shfl_sync(0xffffffffu, weight, (k0 % blockDim.x) >> 5);
+    for (int k = lane; k < src.K; k += 32) {
+      const int id = e.id[k], at = id + first;
       if (id < 0 || at < 0 || at >= n * VEC) continue;
-      p *= e.p[k];
+      float p = e.p[k] * weight_of(k);
       if (is_marked(table, slots_log2, id)) {
         p = 0.f;
         bool again = false;
         for (int i = 0; i < src.K; ++i) {
           if (e.id[i] != id) continue;
           again = again || i < k;
-          const float3 of = s_entries[(i % blockDim.x) >> 5];
-          p += ex2(of.x - ent_top) * over * e.p[i];
+          p += e.p[i] * weight_of(i);
         }
         if (again) continue;
       }

@@ -228,6 +228,9 @@ class Sky1LMConfig:
     adam_eps: float = 1e-8
     weight_decay: float = 0.1
     max_grad_norm: float = 0.0  # 0 = no clipping
+    # False: the loss and the head's gradients straight from the hidden states (ops.linear_cross_entropy), without the
+    # bf16 [tokens, vocab] buffer; its logits are not rounded to bf16 either.
+    keep_logits: bool = True
 
     def param_count(self) -> int:
         return self.layers * self.block.param_count() + 2 * self.vocab * self.block.hidden + self.block.hidden
@@ -307,13 +310,20 @@ class Sky1LM:
         self.acts = [torch.empty(t, b.hidden, **bf) for _ in range(cfg.layers + 1)]
         self.hf = torch.empty(t, b.hidden, **bf)
         self.r_inv = torch.empty(t, **f32)
-        self.logits = torch.empty(t, cfg.vocab, **bf)
+        self.logits = torch.empty(t, cfg.vocab, **bf) if cfg.keep_logits else None
         self.loss_tok = torch.empty(t, **f32)
         self.loss = torch.zeros(1, **f32)
         self.sumsq = torch.zeros(1, **f32)
         self.dx = [torch.empty(t, b.hidden, **bf) for _ in range(2)]
         self.red_scratch = torch.empty(4096, dtype=torch.uint8, device=self.device)
         self.norm_scratch = torch.empty(ops_norm_bwd_scratch(t, b.hidden), dtype=torch.uint8, device=self.device)
+        if not cfg.keep_logits:
+            from . import ops
+
+            head = self.view("replica", "lm_head"), self.view("grads", "lm_head")
+            self.head_scratch = torch.empty(ops.linear_loss_scratch_bytes(self.hf, head[0], ops.LinearLossOpts(accumulate=True),
+                                                                          dx=self.hf, dw=head[1]),
+                                            dtype=torch.uint8, device=self.device)
         self.step_count = 0
         self.comm = torch.cuda.Stream(device=self.device) if self.world > 1 else None
         self._tokens = None
@@ -343,15 +353,21 @@ class Sky1LM:
             blk.forward(self.acts[i], self.acts[i + 1])
         xl, hf, gam, rinv = ta(self.acts[-1]), ta(self.hf), ta(self.view("replica", "final_norm")), ta(self.r_inv)
         check(lib.cdl_b200_rmsnorm_fwd(L.ref(xl), L.ref(gam), None, c.block.eps, L.ref(hf), L.ref(rinv), st))
-        ops.matmul(self.hf, self.view("replica", "lm_head"), out=self.logits)
-        lg, lt = ta(self.logits), ta(self.loss_tok)
-        check(lib.cdl_b200_cross_entropy(L.ref(lg), L.ref(tgt), L.ref(lt), loss_scale, st))
-        check(lib.cdl_b200_sum(self.loss_tok.data_ptr(), self.loss_tok.numel(), self.loss.data_ptr(),
+        head, g_head = self.view("replica", "lm_head"), self.view("grads", "lm_head")
+        if c.keep_logits:
+            ops.matmul(self.hf, head, out=self.logits)
+            lg, lt = ta(self.logits), ta(self.loss_tok)
+            check(lib.cdl_b200_cross_entropy(L.ref(lg), L.ref(tgt), L.ref(lt), loss_scale, st))
+            loss_tok = self.loss_tok
+        else:  # d_hf in place of hf, and the head's gradient
+            loss_tok = ops.linear_cross_entropy(self.hf, head, targets, ops.LinearLossOpts(grad_scale=loss_scale, accumulate=True),
+                                                dx=self.hf, dw=g_head, scratch=self.head_scratch).loss
+        check(lib.cdl_b200_sum(loss_tok.data_ptr(), loss_tok.numel(), self.loss.data_ptr(),
                                loss_scale, 0, 1, self.red_scratch.data_ptr(), 4096, st))
         # backward
-        g_head = self.view("grads", "lm_head")
-        ops.matmul(self.hf.T, self.logits, ops.MatmulOpts(out=torch.float32, c=g_head, beta=1.0), out=g_head)
-        ops.matmul(self.logits, self.view("replica", "lm_head").T, out=self.hf)  # d_hf, in place of hf
+        if c.keep_logits:
+            ops.matmul(self.hf.T, self.logits, ops.MatmulOpts(out=torch.float32, c=g_head, beta=1.0), out=g_head)
+            ops.matmul(self.logits, head.T, out=self.hf)  # d_hf, in place of hf
         dgam, dxl = ta(self.view("grads", "final_norm")), ta(self.dx[0])
         check(lib.cdl_b200_rmsnorm_bwd(L.ref(xl), L.ref(hf), None, L.ref(gam), L.ref(rinv), L.ref(dxl),
                                        L.ref(dgam), self.norm_scratch.data_ptr(),

@@ -252,7 +252,8 @@ SHAPES = [(1, 64, 1000, 0, BF16, "rows"), (1, 8, 1, 0, BF16, "rows"), (7, 65, 12
           (130, 96, 520, 0, BF16, "strided"), (129, 256, 4096, 0, BF16, "rows"), (513, 128, 2304, 0, BF16, "rows"),
           (65, 515, 770, 0, F32, "rows"), (40, 64, 301, 0, F32, "tied"), (33, 48, 100, 0, F32, "strided"), (70, 64, 300, 0, BF16, "columns"),
           (1, 64, 1000, 5, BF16, "rows"), (257, 256, 4097, 64, BF16, "rows"), (300, 72, 1001, 7, BF16, "tied"), (12, 128, 640, 300, BF16, "rows"),
-          (50, 65, 300, 16, F32, "rows"), (200, 64, 8200, 1, BF16, "tied"), (600, 64, 128, 128, BF16, "rows"), (5, 64, 2000, 1024, BF16, "rows")]
+          (50, 65, 300, 16, F32, "rows"), (200, 64, 8200, 1, BF16, "tied"), (600, 64, 128, 128, BF16, "rows"), (5, 64, 2000, 1024, BF16, "rows"),
+          (100, 512, 3000, 0, BF16, "rows"), (128, 320, 40000, 0, BF16, "rows"), (128, 320, 40001, 9, BF16, "tied"), (700, 256, 30000, 33, BF16, "rows")]
 
 
 @gpu
@@ -495,6 +496,61 @@ def test_calls_from_threads_on_their_own_streams(cdl, gpu_ok):
     assert not errors
     for a, b in zip(got, want):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@gpu
+def test_losses_together_on_one_head(cdl, gpu_ok):
+    """A step that trains a tied head on targets and on a teacher at once: the norm's output through both losses, dw the sum of
+    both in f32, and each of them against the same loss of stored logits."""
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    t, d, v, tau = 300, 256, 2000, 2.0
+    x = cdl.ops.norm_fwd(torch.randn(t, d, generator=gen, device="cuda").to(BF16)).y
+    table = (torch.randn(v, d, generator=gen, device="cuda") * 0.1).to(BF16)
+    w, targets = table.t(), _entries(gen, t, v, 0)[0]
+    ids, teacher = _teacher(gen, t, v, 12, BF16)
+    d_table = torch.zeros(v, d, device="cuda")
+    hard = cdl.ops.linear_cross_entropy(x, w, targets, cdl.ops.LinearLossOpts(grad_scale=0.7, accumulate=True), dw=d_table.t())
+    soft = cdl.ops.linear_distillation(x, w, ids, teacher, cdl.ops.LinearLossOpts(temperature=tau, grad_scale=0.3, accumulate=True),
+                                       dw=d_table.t())
+    one = torch.ones(t, dtype=torch.float64, device="cuda")
+    _, _, _, dx0, dw0 = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets, 0.7 * one))
+    _, _, _, dx1, dw1 = ref.linear(x, w, lambda z: ref.distillation(z, ids, teacher, tau, 0.3 * one))
+    # d z rounded twice (2^-8 each), the result once: at most 3 * 2^-8 of the 2-norm
+    for got, want in ((hard.dx, dx0), (soft.dx, dx1), (d_table.t(), dw0 + dw1)):
+        assert (got.double() - want).norm() <= 3 * 2.0 ** -8 * want.norm()
+    # logits stored in bf16 (|z| < 8 here: 2^-6 off at most): the losses move by twice that over tau, times tau^2
+    logits = cdl.ops.matmul(x, w)
+    assert float(logits.float().abs().max()) < 8
+    stored = cdl.ops.distillation(logits, ids, teacher, cdl.ops.DistillationOpts(temperature=tau, grad_scale=0.3))
+    assert bool(((stored.loss - soft.loss).abs() <= 2 * tau * 2.0 ** -6 + 1e-4).all())
+    assert (cdl.ops.matmul(stored.d_logits, table).double() - dx1).norm() <= 2.0 ** -4 * dx1.norm()
+
+
+@gpu
+def test_language_model_without_stored_logits(cdl, gpu_ok):
+    """Sky1LM with keep_logits=False against the same model with them.  Stored logits are rounded to bf16: |z| < 4 here (N(0, 0.32^2)),
+    so they are 2^-7 off at most, losses twice that, softmax and gradients 2 * 2^-7 of themselves; bf16 roundings of both backward
+    passes add at most as much again."""
+    sky1 = cdl.sky1
+    blk = sky1.Sky1Config(batch=2, seqlen=256, hidden=256, heads=2, kv_heads=2, head_dim=128, ffn=512)
+    models = [sky1.Sky1LM(sky1.Sky1LMConfig(block=blk, layers=2, vocab=2048, keep_logits=k), seed=4) for k in (True, False)]
+    assert models[1].logits is None
+    gen = torch.Generator().manual_seed(7)
+    data = torch.randint(0, 2048, (2, 2, 257), generator=gen, dtype=torch.int32)
+    tokens, targets = (data[:, :, i:256 + i].reshape(2, -1).cuda() for i in (0, 1))
+    targets[0, ::7] = -1
+    for m in models:
+        m.loss.zero_()
+        for i in range(2):
+            m.forward_backward(tokens[i], targets[i], 1.0 / tokens.numel())
+    a, b = models
+    assert abs(a.loss.item() - b.loss.item()) <= 2.0 ** -6
+    for name, _, _ in a.layout:
+        p, q = a.view("grads", name).double(), b.view("grads", name).double()
+        assert (p - q).norm() <= 4 * 2.0 ** -7 * p.norm(), name
+    for m in models:
+        m.optimizer_step()
+    assert cdl._lib.device_status() == 0
 
 
 # ------------------------------------------------------------------------------------------ refusals (no GPU)
