@@ -1031,7 +1031,7 @@ constexpr long long TARGET_ENTRIES = -1;
 
 // Rows that are taken at a time: their logits (and the gradients of those) are what the scratch holds.
 static long long choose_chunk(long long T, long long V, size_t bytes_per_logit) {
-  const long long most = (512LL << 20) / static_cast<long long>(bytes_per_logit * V);
+  const long long most = (1LL << 30) / static_cast<long long>(bytes_per_logit * V);
   long long rows = most < 256 ? 256 : most;
   if (rows >= T) return T;
   const long long chunks = (T + rows - 1) / rows;

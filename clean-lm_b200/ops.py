@@ -342,21 +342,20 @@ def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
     if not want_x:
         dx = None
     elif dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     if not want_w:
         dw = None
-    elif dw is None:  # laid out as w is
-        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w.stride(0) >= w.stride(1) else \
-            torch.empty(w.shape[::-1], dtype=w.dtype, device=w.device).t()
-    tokens, distil = x.shape[0], len(entries) > 1
-    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=x.device).unbind()
+    elif dw is None:
+        dw = torch.empty_like(w)  # (in w's order of strides)
+    device, tokens, distil = x.device, x.shape[0], len(entries) > 1
+    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=device).unbind()
     desc = _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
     tx, tw, tdx, tdw = tensor_bytes(x), tensor_bytes(w), tensor_bytes(dx), tensor_bytes(dw)
     if scratch is None:
         n = ctypes.c_size_t(0)
         check(packed_lib.cdl_b200_linear_loss_scratch_bytes(desc, tx, tw, entries[0].shape[-1] if distil else 1, tdx, tdw,
                                                             ctypes.byref(n)))
-        scratch = torch.empty(max(n.value, 256), dtype=torch.uint8, device=x.device)
+        scratch = torch.empty(max(n.value, 256), dtype=torch.uint8, device=device)
     fn = packed_lib.cdl_b200_linear_distillation if distil else packed_lib.cdl_b200_linear_cross_entropy
     check(fn(desc, tx, tw, *map(tensor_bytes, entries), tensor_bytes(d_loss), _lib.rows_bytes(loss.data_ptr(), tokens),
              _lib.rows_bytes(lse.data_ptr(), tokens), tdx, tdw, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
@@ -420,7 +419,7 @@ def distillation(logits, teacher_ids, teacher_logits, opts: DistillationOpts | N
     if not opts.grad:
         d_logits = None
     elif d_logits is None:
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
     check(packed_lib.cdl_b200_distillation(
         _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 0, 0), tensor_bytes(logits), tensor_bytes(teacher_ids),
         tensor_bytes(teacher_logits), tensor_bytes(d_loss), _lib.rows_bytes(loss.data_ptr(), tokens),
