@@ -674,8 +674,13 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
 // from the L1, through which C is read), cost those 0.2 to 0.9 us (2048 x 5632 x
 // 256 12.3 instead of 11.9, with a bf16 C 18.8 instead of 18.0).
 // D in any form; D += by TMA; the SwiGLU forms whose operands TMA brings; a loss's exponentials; every K slice in a plane of
-// its own; a bf16 D by TMA.
-enum Store { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP, STORE_PLANES, STORE_BF16 };
+// its own; a bf16 D by TMA; f32 operands as three bf16 pieces each, in planes if there are K slices.
+enum Store { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP, STORE_PLANES, STORE_BF16, STORE_PIECES };
+// The products of pieces that count, smallest first: an f32 value is the sum of its pieces 0, 1, 2, the others are below 2^-24.
+// A K slice goes through its K blocks once for each.
+constexpr int PIECE_PRODUCTS = 6;
+__device__ __forceinline__ int piece_of_a(int i) { return 0x210100 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
+__device__ __forceinline__ int piece_of_b(int i) { return 0x012010 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
 
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -714,10 +719,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
-  // Unit of work: a tile, or (STORE_PLANES) one of its K slices, numbered slice by slice.
-  const int num_units = KIND == STORE_PLANES ? p.num_tiles * p.split_k : p.num_tiles;
+  // Unit of work: a tile, or one of its K slices, numbered slice by slice.
+  constexpr bool SLICES = KIND == STORE_PLANES || KIND == STORE_PIECES;
+  const int num_units = SLICES ? p.num_tiles * p.split_k : p.num_tiles;
   auto unit_range = [&](int unit, int& tile, int& slice, int& kb0, int& kb1) {
-    if constexpr (KIND == STORE_PLANES) {
+    if constexpr (SLICES) {
       slice = unit / p.num_tiles;
       tile = unit - slice * p.num_tiles;
       kb0 = static_cast<int>(static_cast<long long>(slice) * p.k_blocks / p.split_k);
@@ -743,7 +749,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         unit_range(unit, tile, slice, kb0, kb1);
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * BM, n0 = tn * BN;
+        for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait(&bars->empty[s], ph ^ 1, abort_word, 101)) {
@@ -757,16 +765,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (p.a_mn) {
 #pragma unroll
             for (int i = 0; i < BM / 64; ++i)
-              tma_load_3d(sa + i * 8192, &tmap_a, &bars->full[s], m0 + i * 64, k0, b);
+              tma_load_3d(sa + i * 8192, &tmap_a, &bars->full[s], m0 + i * 64, k0, ba);
           } else {
-            tma_load_3d(sa, &tmap_a, &bars->full[s], k0, m0, b);
+            tma_load_3d(sa, &tmap_a, &bars->full[s], k0, m0, ba);
           }
           if (p.b_mn) {
 #pragma unroll
             for (int i = 0; i < BN / 64; ++i)
-              tma_load_3d(sb + i * 8192, &tmap_b, &bars->full[s], n0 + i * 64, k0, b);
+              tma_load_3d(sb + i * 8192, &tmap_b, &bars->full[s], n0 + i * 64, k0, bb);
           } else {
-            tma_load_3d(sb, &tmap_b, &bars->full[s], k0, n0, b);
+            tma_load_3d(sb, &tmap_b, &bars->full[s], k0, n0, bb);
           }
         }
       }
@@ -788,7 +796,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 201)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int blocks = (kb1 - kb0) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1);
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait(&bars->full[s], ph, abort_word, 202)) {
@@ -802,7 +811,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
             const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
-            umma_ss(d_tmem, da, db, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+            umma_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
           }
           umma_commit(&bars->empty[s]);
         }
@@ -828,7 +837,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
       if constexpr (KIND == STORE_EXP) {
         store_tile_rows_exp<false>(p, nullptr, nullptr, t_row, row, col, lane, want);
-      } else if constexpr (KIND == STORE_PLANES) {
+      } else if constexpr (SLICES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
@@ -869,7 +878,7 @@ constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = 2 * A_BYTES;  // A 128 x 64 and half of B 128 x 64
 constexpr int PAIR_M = 2 * BM;
 constexpr int PAIR_BARRIER_BYTES = 512;
-constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_PLANES ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
+constexpr int pair_staging(int kind) { return kind == STORE || kind == STORE_PLANES || kind == STORE_PIECES ? 0 : EPI_WARPS * CHUNK_BYTES; }  // a buffer per epilogue warp
 constexpr size_t pair_smem_bytes(int kind) {
   return 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + pair_staging(kind) + PAIR_BARRIER_BYTES;
 }
@@ -1018,7 +1027,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * PAIR_M + static_cast<int>(rank) * BM;
         const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
+        for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % PAIR_STAGES;
           const uint32_t ph = (it / PAIR_STAGES) & 1;
           if (!mbar_wait(&bars->empty[s], ph ^ 1, abort_word, 111)) {
@@ -1034,16 +1045,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (p.a_mn) {
 #pragma unroll
             for (int i = 0; i < BM / 64; ++i)
-              tma_load_3d_pair(sa + i * 8192, &tmap_a, full_leader, m0 + i * 64, k0, b);
+              tma_load_3d_pair(sa + i * 8192, &tmap_a, full_leader, m0 + i * 64, k0, ba);
           } else {
-            tma_load_3d_pair(sa, &tmap_a, full_leader, k0, m0, b);
+            tma_load_3d_pair(sa, &tmap_a, full_leader, k0, m0, ba);
           }
           if (p.b_mn) {
 #pragma unroll
             for (int i = 0; i < BN / 128; ++i)
-              tma_load_3d_pair(sb + i * 8192, &tmap_b, full_leader, n0 + i * 64, k0, b);
+              tma_load_3d_pair(sb + i * 8192, &tmap_b, full_leader, n0 + i * 64, k0, bb);
           } else {
-            tma_load_3d_pair(sb, &tmap_b, full_leader, k0, n0, b);
+            tma_load_3d_pair(sb, &tmap_b, full_leader, k0, n0, bb);
           }
         }
       }
@@ -1070,7 +1081,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 211)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int blocks = (kb1 - kb0) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1);
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % PAIR_STAGES;
           const uint32_t ph = (it / PAIR_STAGES) & 1;
           if (!mbar_wait(&bars->full[s], ph, abort_word, 212)) {
@@ -1084,7 +1096,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
             const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
-            umma_ss_pair(d_tmem, da, db, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+            umma_ss_pair(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
           }
           const uint32_t e = smem_u32(&bars->empty[s]);
           umma_commit_pair(e);                  // own producer
@@ -1131,7 +1143,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         else store_tile_rows_swiglu<true>(p, feed, t_row, row, col, lane, abort_word);
       } else if constexpr (KIND == STORE_EXP) {
         store_tile_rows_exp<true>(p, &tmap_e0, buf, t_row, row, col, lane, want);
-      } else if constexpr (KIND == STORE_PLANES) {
+      } else if constexpr (KIND == STORE_PLANES || KIND == STORE_PIECES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else if constexpr (KIND == STORE_BF16) {
         store_tile_rows_tma(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
@@ -1346,6 +1358,7 @@ static int32_t prepare_kernels(int* clusters) {
     one(gemm_bf16_kernel<STORE>);
     one(gemm_bf16_kernel<STORE_EXP>);
     one(gemm_bf16_kernel<STORE_PLANES>);
+    one(gemm_bf16_kernel<STORE_PIECES>);
     auto pair = [&](auto kernel, int kind) {
       if (attr_err == cudaSuccess)
         attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1357,6 +1370,7 @@ static int32_t prepare_kernels(int* clusters) {
     pair(gemm_bf16_pair_kernel<STORE_EXP>, STORE_EXP);
     pair(gemm_bf16_pair_kernel<STORE_PLANES>, STORE_PLANES);
     pair(gemm_bf16_pair_kernel<STORE_BF16>, STORE_BF16);
+    pair(gemm_bf16_pair_kernel<STORE_PIECES>, STORE_PIECES);
     int n = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
@@ -1689,18 +1703,20 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
   return CDL_OK;
 }
 
-// The wide tiles' operands of a plain product of bf16 tensors on the 16-byte grid; one CTA per tile up to 128 rows, else CTA
-// pairs.
+// The wide tiles' operands of a plain product of bf16 tensors on the 16-byte grid (or, rank 3, of the pieces of f32 ones); one
+// CTA per tile up to 128 rows, else CTA pairs.
 static int32_t wide_operands(const cdl_tensor* a, const cdl_tensor* b, gemm::Params& p, CUtensorMap* tm_a, CUtensorMap* tm_b, bool pair) {
   using namespace gemm;
-  const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
+  const int r = a->rank;
+  const long long M = a->shape[r - 2], K = a->shape[r - 1], N = b->shape[r - 1];
   OperandLayout la, lb;
   CDL_CHECK(analyze_operand("a", a, true, &la));
   CDL_CHECK(analyze_operand("b", b, false, &lb));
-  const uint64_t da[3] = {static_cast<uint64_t>(la.mn_major ? M : K), static_cast<uint64_t>(la.mn_major ? K : M), 1};
-  const uint64_t db[3] = {static_cast<uint64_t>(lb.mn_major ? N : K), static_cast<uint64_t>(lb.mn_major ? K : N), 1};
-  const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(la.ld) * da[1] * 2};
-  const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(lb.ld) * db[1] * 2};
+  const uint64_t pieces = r == 3 ? static_cast<uint64_t>(a->shape[0]) : 1;
+  const uint64_t da[3] = {static_cast<uint64_t>(la.mn_major ? M : K), static_cast<uint64_t>(la.mn_major ? K : M), pieces};
+  const uint64_t db[3] = {static_cast<uint64_t>(lb.mn_major ? N : K), static_cast<uint64_t>(lb.mn_major ? K : N), pieces};
+  const uint64_t sa[3] = {0, static_cast<uint64_t>(la.ld) * 2, static_cast<uint64_t>(r == 3 ? la.batch : la.ld * da[1]) * 2};
+  const uint64_t sb[3] = {0, static_cast<uint64_t>(lb.ld) * 2, static_cast<uint64_t>(r == 3 ? lb.batch : lb.ld * db[1]) * 2};
   const uint32_t ba[3] = {64, static_cast<uint32_t>(la.mn_major ? 64 : BM), 1};
   const uint32_t bb[3] = {64, static_cast<uint32_t>(lb.mn_major ? 64 : pair ? BN / 2 : BN), 1};
   CDL_CHECK(encode_tmap(tm_a, a->ptr, CDL_BF16, 3, da, sa, ba, true));
@@ -1782,16 +1798,17 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
 // K slices of a product whose output is small and whose K is long (dx of a head: K is the vocabulary), each stored in f32 in
 // a plane of its own, to be summed in their order.  Estimated in microseconds as in choose_cluster_splits: 0.28 per K
 // block, 4 per unit's store and set-up, a plane's way out and back at 5 TB/s and 3 for the kernel that sums them.
-int matmul_plane_slices(long long M, long long N, long long K) {
+int matmul_plane_slices(long long M, long long N, long long K, bool pieces) {
   using namespace gemm;
   const bool pair = M > BM;
+  const int least_slices = pieces ? static_cast<int>((K + PIECES_K - 1) / PIECES_K) : 1;
   const long long tiles = (pair ? (M + PAIR_M - 1) / PAIR_M : 1) * ((N + BN - 1) / BN), k_blocks = (K + BK - 1) / BK;
   const long long slots = pair ? sm_count() / 2 : sm_count();
-  int best = 1;
+  int best = least_slices;
   double least = 1e30;
-  for (int s = 1; s <= MAX_PLANES && (s == 1 || s * 8 <= k_blocks); ++s) {
+  for (int s = least_slices; s == least_slices || (s <= MAX_PLANES && s * (pieces ? 2 : 8) <= k_blocks); ++s) {
     const double waves = static_cast<double>((tiles * s + slots - 1) / slots);
-    double t = waves * (0.28 * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
+    double t = waves * (0.28 * (pieces ? PIECE_PRODUCTS : 1) * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
     if (s > 1) t = 1.05 * (t + 3.0 + 8e-6 * static_cast<double>(s) * M * N / 5.0);
     if (t < least) {
       least = t;
@@ -1812,6 +1829,32 @@ int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* p
   p.out_f32 = p.d_vec = p.wide = 1;  // (rows of whole 32 bytes)
   p.split_k = slices;
   return pair ? pair_launch<gemm::STORE_PLANES>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_PLANES>(p, tm_a, tm_b, stream);
+}
+
+// A product of f32 operands that lie in three bf16 pieces each, [3][M][K] and [3][K][N], the six largest products of pieces
+// summed.  One slice: D = product (+ D) itself; more: planes.  An accumulator takes at most PIECES_K of K, and what truncation
+// takes from it is put back (see matmul_exp_execute): what is left is below the rounding of f32 sums of that length.
+int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d, long long ldd, int slices, int add, cudaStream_t stream) {
+  gemm::Params p;
+  CUtensorMap tm_a, tm_b;
+  const bool pair = a->shape[1] > gemm::BM;
+  CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, pair));
+  p.d = d;
+  p.ldd = ldd;
+  p.d_batch = ldd * p.M;
+  p.out_f32 = 1;
+  p.d_vec = (reinterpret_cast<uintptr_t>(d) & 15) == 0 && ldd % 4 == 0;
+  p.wide = (reinterpret_cast<uintptr_t>(d) & 31) == 0 && ldd % 8 == 0;
+  if (add) {
+    p.c = d;
+    p.ldc = ldd;
+    p.c_mode = 2;
+    p.c_vec = p.d_vec;
+    p.beta = 1.f;
+  }
+  p.alpha = static_cast<float>(1.0 + 1e-9 * p.K / slices);
+  p.split_k = slices;
+  return pair ? pair_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, stream);
 }
 
 // Whether a plain product is bound by the store of its bf16 D, which TMA makes the shorter: a short K and pairs with several

@@ -705,87 +705,117 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
   }
 }
 
-// dst[r, c] = src[r, c] for any strides of the source, or 0 where keep[r] says that row r does not count; the threads run
-// along dst's columns.
+// ------------------------------------------------------------------------------------------ operands and gradients off the grid
+// A block has SEGMENT columns of a row, its threads neighbouring ones: any strides and alignment, eight accesses of a thread under
+// way.  (381 MB of bf16 rows of odd length 480 -> 173 us against a loop over 256 columns with one.)
+constexpr int SEGMENT = 2048;
+
+struct Segment {
+  long long row;
+  int col;
+  __device__ __forceinline__ Segment(int cols) {
+    const int per_row = (cols + SEGMENT - 1) / SEGMENT;
+    row = blockIdx.x / per_row;
+    col = static_cast<int>(blockIdx.x - row * per_row) * SEGMENT + threadIdx.x;
+  }
+};
+
+// dst[r, c] = src[r, c].
+template <typename T>
+__global__ void __launch_bounds__(256) copy_kernel(const T* src, long long s_row, long long s_col, T* dst, long long ld, int cols) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const Segment at(cols);
+  const T* from = src + at.row * s_row;
+  T v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (at.col + 256 * j < cols) v[j] = from[(at.col + 256 * j) * s_col];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (at.col + 256 * j < cols) dst[at.row * ld + at.col + 256 * j] = v[j];
+}
+
+// The three bf16 pieces of f32 values, v = p0 + p1 + p2 to 24 bits: the first two cut off (no finite value becomes infinite),
+// the last rounded.  Zeros where keep (nullptr: all rows count) says that a row does not count.  dst: [3][rows][ld], planes
+// `plane` apart.
+__global__ void __launch_bounds__(256)
+    split_kernel(const float* src, long long s_row, long long s_col, __nv_bfloat16* dst, long long ld, long long plane, int cols,
+                 const float* keep) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const Segment at(cols);
+  const float* from = src + at.row * s_row;
+  const bool zero = keep != nullptr && keep[at.row] == 0.f;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (at.col + 256 * j < cols) v[j] = from[(at.col + 256 * j) * s_col];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (at.col + 256 * j >= cols) break;
+    const float x = zero ? 0.f : v[j];
+    const float p0 = __uint_as_float(__float_as_uint(x) & 0xffff0000u), r = x - p0;
+    const float p1 = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    __nv_bfloat16* o = dst + at.row * ld + at.col + 256 * j;
+    o[0] = __float2bfloat16_rn(p0);
+    o[plane] = __float2bfloat16_rn(p1);
+    o[2 * plane] = __float2bfloat16_rn(r - p1);
+  }
+}
+
+// out[r, c] = the sum of the planes at r, c in their order (+ out[r, c]).  One plane: the end of a gradient that scratch held.
+// No plane: zeros.
+template <typename S, typename T>
+__global__ void __launch_bounds__(256)
+    sum_planes_kernel(const S* planes, long long ld, long long plane, int slices, T* out, long long o_row, long long o_col, int cols, int add) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const Segment at(cols);
+  const S* from = planes + at.row * ld + at.col;
+  T* o = out + at.row * o_row + at.col * o_col;
+  float v[8] = {};
+  for (int s = 0; s < slices; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at.col + 256 * j < cols) v[j] += to_f32(from[s * plane + 256 * j]);
+  if (add) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at.col + 256 * j < cols) v[j] += to_f32(o[256 * j * o_col]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (at.col + 256 * j < cols) o[256 * j * o_col] = from_f32<T>(v[j]);
+}
+// The same by vectors of four, where the rows of out and of the planes allow them: a thread has one.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    copy_kernel(const T* src, long long s_row, long long s_col, T* dst, long long ld, long long rows, int cols,
-                const float* keep) {
-  const long long per_row = (cols + 255) / 256;
-  for (long long b = blockIdx.x; b < rows * per_row; b += gridDim.x) {
-    const long long r = b / per_row;
-    const int c = static_cast<int>(b - r * per_row) * 256 + threadIdx.x;
-    if (c >= cols) continue;
-    dst[r * ld + c] = keep != nullptr && keep[r] == 0.f ? from_f32<T>(0.f) : src[r * s_row + c * s_col];
-  }
-}
-
-// out[r, c] = sum[r, c] (+ out[r, c]): the end of a gradient that is summed in f32 scratch; sum = nullptr: zeros.  A thread
-// has eight columns of a row, by vectors where out's rows allow them (sum's always do).
-template <typename T, bool VECTORS>
-__global__ void __launch_bounds__(256)
-    finish_kernel(const float* sum, long long ld, T* out, long long o_row, long long o_col, long long rows, int cols, int add) {
+    sum_vectors_kernel(const float* planes, long long ld, long long plane, int slices, T* out, long long o_row, long long all, int cols, int add) {
   grid_dep_wait();
   grid_dep_launch();
-  const int per_row = (cols + 7) / 8;
-  const long long all = rows * per_row, step = static_cast<long long>(gridDim.x) * 256;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
-    const long long r = i / per_row;
-    const int c = static_cast<int>(i - r * per_row) * 8;
-    float v[8] = {};
-    if (sum != nullptr) {  // (its rows are padded to whole vectors)
-      const float4 lo = *reinterpret_cast<const float4*>(sum + r * ld + c), hi = *reinterpret_cast<const float4*>(sum + r * ld + c + 4);
-      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-    }
-    T* o = out + r * o_row + c * o_col;
-    if (VECTORS && c + 8 <= cols) {
-      if (add) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += to_f32(o[j]);
-      }
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-      } else {
-        *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < cols) o[j * o_col] = from_f32<T>(add ? v[j] + to_f32(o[j * o_col]) : v[j]);
-    }
-  }
-}
-
-// out[r, c] = the planes' sum at r, c, in their order.
-__global__ void __launch_bounds__(256)
-    sum_planes_kernel(const float* planes, long long ld, int slices, __nv_bfloat16* out, long long ld_out, int rows, int cols, int vectors) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int per_row = (cols + 3) / 4;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, r = i / per_row;
-  if (r >= rows) return;
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= all) return;
+  const int per_row = cols / 4;
+  const long long r = i / per_row;
   const int c = static_cast<int>(i - r * per_row) * 4;
   const float* from = planes + r * ld + c;
+  T* o = out + r * o_row + c;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int s = 0; s < slices; ++s) {
-    const float4 x = *reinterpret_cast<const float4*>(from + s * (rows * ld));
+    const float4 x = *reinterpret_cast<const float4*>(from + s * plane);
     v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
   }
-  __nv_bfloat16* o = out + r * ld_out + c;
-  if (vectors && c + 4 <= cols) {
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-  } else {
-    const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < cols) o[j] = __float2bfloat16_rn(f[j]);
-  }
+  if (add) v.x += to_f32(o[0]), v.y += to_f32(o[1]), v.z += to_f32(o[2]), v.w += to_f32(o[3]);
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  else *reinterpret_cast<float4*>(o) = v;
 }
 
 // 1 for a row that counts, 0 for one without a target or entries.
 __global__ void __launch_bounds__(256) keep_kernel(const Entries src, long long rows, int vocab, float* keep) {
+  grid_dep_wait();
+  grid_dep_launch();
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   bool any = false;
@@ -870,40 +900,62 @@ static int32_t prepare_entries(const Entries& e, long long rows, int vocab, floa
   return CDL_OK;
 }
 
-static unsigned copy_grid(long long rows, long long cols) {
-  const long long blocks = rows * ((cols + 255) / 256), most = 32LL * sm_count();
-  return static_cast<unsigned>(blocks < most ? blocks : most);
+static int32_t segments(long long rows, long long cols, dim3* grid) {
+  const long long blocks = rows * ((cols + SEGMENT - 1) / SEGMENT);
+  if (blocks > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "linear loss: operand too large to be copied");
+  *grid = dim3(static_cast<unsigned>(blocks));
+  return CDL_OK;
 }
 
 // dst [rows, cols] (ld) = src, of which the threads' direction is dimension 1.
-static int32_t copy(const cdl_tensor& src, void* dst, long long ld, const float* keep, cudaStream_t stream) {
-  const long long rows = src.shape[0], cols = src.shape[1];
-  if (src.dtype == CDL_BF16)
-    copy_kernel<__nv_bfloat16><<<copy_grid(rows, cols), 256, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(src.ptr), src.stride[0], src.stride[1], static_cast<__nv_bfloat16*>(dst), ld, rows,
-        static_cast<int>(cols), keep);
-  else
-    copy_kernel<float><<<copy_grid(rows, cols), 256, 0, stream>>>(static_cast<const float*>(src.ptr), src.stride[0], src.stride[1],
-                                                                static_cast<float*>(dst), ld, rows, static_cast<int>(cols), keep);
-  CDL_CUDA(cudaGetLastError());
+static int32_t copy(const cdl_tensor& src, void* dst, long long ld, cudaStream_t stream) {
+  using bf = __nv_bfloat16;
+  dim3 grid;
+  CDL_CHECK(segments(src.shape[0], src.shape[1], &grid));
+  ProfileScope ps(PROF_ELEMENTWISE, 4.0 * src.shape[0] * src.shape[1], stream);
+  CDL_CUDA(launch_pdl(copy_kernel<bf>, grid, dim3(256), 0, stream, static_cast<const bf*>(src.ptr), static_cast<long long>(src.stride[0]),
+                      static_cast<long long>(src.stride[1]), static_cast<bf*>(dst), ld, static_cast<int>(src.shape[1])));
   return CDL_OK;
 }
 
-template <typename T>
-static int32_t finish_as(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
-  const long long rows = out.shape[0], cols = out.shape[1], blocks = (rows * ((cols + 7) / 8) + 255) / 256, most = 16LL * sm_count();
-  const bool vectors = out.stride[1] == 1 && (reinterpret_cast<uintptr_t>(out.ptr) & 15) == 0 && (rows == 1 || out.stride[0] % 8 == 0);
-  auto run = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, stream, sum, ld,
-                      static_cast<T*>(out.ptr), static_cast<long long>(out.stride[0]), static_cast<long long>(out.stride[1]), rows,
-                      static_cast<int>(cols), add);
-  };
-  CDL_CUDA(vectors ? run(finish_kernel<T, true>) : run(finish_kernel<T, false>));
+static int32_t split(const cdl_tensor& src, void* dst, long long ld, long long plane, const float* keep, cudaStream_t stream) {
+  dim3 grid;
+  CDL_CHECK(segments(src.shape[0], src.shape[1], &grid));
+  ProfileScope ps(PROF_ELEMENTWISE, 10.0 * src.shape[0] * src.shape[1], stream);
+  CDL_CUDA(launch_pdl(split_kernel, grid, dim3(256), 0, stream, static_cast<const float*>(src.ptr), static_cast<long long>(src.stride[0]),
+                      static_cast<long long>(src.stride[1]), static_cast<__nv_bfloat16*>(dst), ld, plane, static_cast<int>(src.shape[1]), keep));
   return CDL_OK;
 }
-static int32_t finish(const float* sum, long long ld, const cdl_tensor& out, int add, cudaStream_t stream) {
-  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(out.shape[0]) * out.shape[1] * (4 + dtype_size(out.dtype)), stream);
-  return out.dtype == CDL_BF16 ? finish_as<__nv_bfloat16>(sum, ld, out, add, stream) : finish_as<float>(sum, ld, out, add, stream);
+
+// out (dimension 1 the threads' direction) = the sum of f32 planes, or of one bf16 one.
+template <typename S, typename T>
+static int32_t sum_planes_as(const void* planes, long long ld, long long plane, int slices, const cdl_tensor& out, int add, cudaStream_t stream) {
+  const long long rows = out.shape[0], cols = out.shape[1];
+  const bool vectors = sizeof(S) == 4 && slices > 0 && cols % 4 == 0 && out.stride[1] == 1 && ld % 4 == 0 && plane % 4 == 0 &&
+                       reinterpret_cast<uintptr_t>(out.ptr) % (4 * sizeof(T)) == 0 && (rows == 1 || out.stride[0] % 4 == 0);
+  if constexpr (sizeof(S) == 4) {
+    const long long all = rows * (cols / 4);
+    if (vectors && (all + 255) / 256 <= INT32_MAX) {
+      CDL_CUDA(launch_pdl(sum_vectors_kernel<T>, dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream,
+                          static_cast<const float*>(planes), ld, plane, slices, static_cast<T*>(out.ptr),
+                          static_cast<long long>(out.stride[0]), all, static_cast<int>(cols), add));
+      return CDL_OK;
+    }
+  }
+  dim3 grid;
+  CDL_CHECK(segments(rows, cols, &grid));
+  CDL_CUDA(launch_pdl(sum_planes_kernel<S, T>, grid, dim3(256), 0, stream, static_cast<const S*>(planes), ld, plane, slices,
+                      static_cast<T*>(out.ptr), static_cast<long long>(out.stride[0]), static_cast<long long>(out.stride[1]),
+                      static_cast<int>(cols), add));
+  return CDL_OK;
+}
+static int32_t sum_planes(const void* planes, int32_t type, long long ld, long long plane, int slices, const cdl_tensor& out, int add,
+                          cudaStream_t stream) {
+  using bf = __nv_bfloat16;
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(out.shape[0]) * out.shape[1] * (dtype_size(type) * slices + dtype_size(out.dtype)), stream);
+  if (type == CDL_BF16) return sum_planes_as<bf, bf>(planes, ld, plane, slices, out, add, stream);
+  return out.dtype == CDL_BF16 ? sum_planes_as<float, bf>(planes, ld, plane, slices, out, add, stream)
+                               : sum_planes_as<float, float>(planes, ld, plane, slices, out, add, stream);
 }
 
 // ------------------------------------------------------------------------------------------ checks
@@ -986,31 +1038,27 @@ static int32_t distillation_execute(const cdl_head_loss_desc* desc, const cdl_te
 
 // ------------------------------------------------------------------------------------------ from the hidden states
 
-// Where a product's operand is read: its own place, or scratch that it is copied to (bf16: rows on the 16-byte grid).
-static bool readable(const cdl_tensor& t) {
-  const long long r = t.shape[0], c = t.shape[1], sr = t.stride[0], sc = t.stride[1];
-  if (t.dtype == CDL_F32) return sc == 1 || c == 1 || sr == 1 || r == 1;
+// Whether products read and write a bf16 or f32 [rows, cols] view where it is: one dimension contiguous, the other on the
+// 16-byte grid.
+static bool on_grid(const cdl_tensor& t) {
+  const long long r = t.shape[0], c = t.shape[1], sr = t.stride[0], sc = t.stride[1], unit = t.dtype == CDL_BF16 ? 8 : 4;
   if (reinterpret_cast<uintptr_t>(t.ptr) & 15) return false;
-  return ((sc == 1 || c == 1) && (r == 1 || (sr % 8 == 0 && sr >= c))) || ((sr == 1 || r == 1) && (c == 1 || (sc % 8 == 0 && sc >= r)));
+  return ((sc == 1 || c == 1) && (r == 1 || (sr % unit == 0 && sr >= c))) || ((sr == 1 || r == 1) && (c == 1 || (sc % unit == 0 && sc >= r)));
 }
 static bool columns_first(const cdl_tensor& t) { return t.stride[0] < t.stride[1]; }  // dimension 0 is the nearer one in memory
 
 struct Linear {
   const char* op;
   cdl_tensor x, w, dx, dw;  // dx, dw: ptr = nullptr where not wanted
-  bool has_dx, has_dw;
+  bool has_dx, has_dw, f32;
   long long T, D, V;
-  // scratch
-  long long chunk;
-  bool copy_x, copy_w, sums;  // sums: dw is summed in f32 scratch and written at the end
-  long long ld_z, ld_g, ld_sum;
-  size_t at_x, at_w, at_z, at_g, at_clean, at_keep, at_sum, at_products, bytes;
-  size_t products_bytes;
-  // bf16: the product writes statistics and exponentials (at_g), not logits
-  int pieces, K;
-  size_t at_stats, at_ids, at_first, at_p, at_p_log_p, at_at;
-  int slices;  // of dx's product, in f32 planes
-  size_t at_planes;
+  int K;
+  // Scratch.  Rows are taken `chunk` at a time.
+  long long chunk, ld_x, ld_w, ld_g, ld_sum;
+  bool copy_x, copy_w;
+  enum { DIRECT, HELD, SUMMED } dw_way;  // the product stores dw; a bf16 dw off the grid, stored beside it first; an f32 sum over the chunks
+  int pieces, slices_z, slices_dx, slices_dw;  // pieces: of the vocabulary, 128 columns each
+  size_t at_x, at_w, at_clean, at_keep, at_z, at_g, at_stats, at_ids, at_first, at_p, at_p_log_p, at_at, at_planes, at_sum, bytes;
 };
 
 // A view of `rows` rows from `row`.
@@ -1029,79 +1077,74 @@ static cdl_tensor strided2(void* p, int32_t dt, long long r, long long c, long l
 
 constexpr long long TARGET_ENTRIES = -1;
 
-// Rows that are taken at a time: their logits (and the gradients of those) are what the scratch holds.
-static long long choose_chunk(long long T, long long V, size_t bytes_per_logit) {
-  const long long most = (1LL << 30) / static_cast<long long>(bytes_per_logit * V);
-  long long rows = most < 256 ? 256 : most;
+// Rows that are taken at a time: their exponentials (f32: logits and the pieces of their gradients) are what the scratch holds,
+// up to 1 GB.  16384 x 2048 x 32768 in one go 5.21 ms, in two 5.44: dw is summed in memory then, dx's last wave is emptier.
+static long long choose_chunk(long long T, long long V, long long bytes_per_logit) {
+  long long rows = (1LL << 30) / (bytes_per_logit * V);
+  if (rows < 256) rows = 256;
   if (rows >= T) return T;
   const long long chunks = (T + rows - 1) / rows;
   return up((T + chunks - 1) / chunks, 256);
 }
 
-static int32_t plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long entries) {
-  const bool grad = p.has_dx || p.has_dw;
-  const int32_t type = p.x.dtype;
-  const size_t es = dtype_size(type);
-  p.copy_x = !readable(p.x);
-  if (type == CDL_BF16)  // (a chunk of its rows starts on the grid too)
-    p.copy_x = (reinterpret_cast<uintptr_t>(p.x.ptr) & 15) != 0 || (p.D > 1 && p.x.stride[1] != 1) ||
-               (p.T > 1 && (p.x.stride[0] % 8 != 0 || p.x.stride[0] < p.D));
-  p.copy_w = !readable(p.w);
-  p.chunk = desc->chunk_rows > 0 ? (desc->chunk_rows < p.T ? desc->chunk_rows : p.T) : choose_chunk(p.T, p.V, es);
-  const bool whole = p.chunk >= p.T;
-  const bool dw_rows = p.has_dw && (p.dw.stride[1] == 1 || p.dw.stride[0] == 1);
-  p.sums = p.has_dw && (!dw_rows || (p.dw.dtype == CDL_BF16 && !whole));
-  p.ld_z = up(p.V, 64);
-  p.ld_g = up(p.V, 128);
-  p.pieces = static_cast<int>(up(p.V, 128) / 128);
+static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long entries) {
+  const bool grad = p.has_dx || p.has_dw, teacher = entries != TARGET_ENTRIES;
+  p.f32 = p.x.dtype == CDL_F32;
   p.K = static_cast<int>(entries);
-  p.ld_sum = p.has_dw ? up(columns_first(p.dw) ? p.D : p.V, 64) : 0;
+  p.pieces = static_cast<int>(up(p.V, 128) / 128);
+  p.copy_x = (reinterpret_cast<uintptr_t>(p.x.ptr) & 15) != 0 || (p.D > 1 && p.x.stride[1] != 1) ||  // (chunks of its rows are on the grid)
+             (p.T > 1 && (p.x.stride[0] % 8 != 0 || p.x.stride[0] < p.D));
+  p.copy_w = !on_grid(p.w);
+  p.chunk = desc->chunk_rows > 0 ? desc->chunk_rows : choose_chunk(p.T, p.V, p.f32 ? 10 : 2);
+  if (p.chunk > p.T) p.chunk = p.T;
+  const bool whole = p.chunk >= p.T, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
+  p.dw_way = Linear::DIRECT;
+  if (p.has_dw && !(on_grid(p.dw) && (p.dw.dtype == CDL_F32 || whole)))
+    p.dw_way = p.dw.dtype == CDL_BF16 && whole && !desc->accumulate_dw ? Linear::HELD : Linear::SUMMED;
+  const size_t n = static_cast<size_t>(p.chunk);
+  p.ld_x = up(p.D, 8);
+  p.ld_w = up(wc ? p.D : p.V, 8);
+  p.ld_g = up(p.V, 128);
+  p.ld_sum = p.has_dw ? up(dc ? p.D : p.V, 8) : 0;
+  p.slices_z = p.f32 ? matmul_plane_slices(p.chunk, p.V, p.D, true) : 1;
+  p.slices_dx = p.has_dx ? matmul_plane_slices(p.chunk, p.D, p.V, p.f32) : 1;
+  p.slices_dw = p.has_dw && p.f32 ? matmul_plane_slices(dc ? p.V : p.D, dc ? p.D : p.V, p.chunk, true) : 1;
   size_t at = 0;
   auto take = [&](bool want, size_t bytes) {
     const size_t here = at;
     if (want) at += (bytes + 255) / 256 * 256;
     return here;
   };
-  const long long x_ld = up(p.D, 8);
-  p.at_x = take(p.copy_x, static_cast<size_t>(p.T) * x_ld * es);
-  const bool wc = columns_first(p.w);
-  p.at_w = take(p.copy_w, static_cast<size_t>(wc ? p.V : p.D) * up(wc ? p.D : p.V, 8) * es);
-  const bool fused = type == CDL_BF16, teacher = entries != TARGET_ENTRIES;
-  const size_t n = static_cast<size_t>(p.chunk);
-  p.at_z = take(!fused, n * p.ld_z * 4);
-  p.at_g = take(fused && grad, n * p.ld_g * 2);
-  if (!fused) p.at_g = p.at_z, p.ld_g = p.ld_z;  // in place
-  p.at_stats = take(fused, n * p.pieces * sizeof(float2));
-  p.at_at = take(fused, n * (teacher ? p.K : 1) * 4);
-  p.at_ids = take(fused && teacher, n * p.K * 4);
-  p.at_p = take(fused && teacher, n * p.K * 4);
-  p.at_p_log_p = take(fused && teacher, n * 4);
-  p.at_first = take(fused && teacher, n * (p.pieces + 1) * 2);
-  p.slices = fused && p.has_dx ? matmul_plane_slices(p.chunk, p.D, p.V) : 1;
-  p.at_planes = take(p.slices > 1, static_cast<size_t>(p.slices) * n * x_ld * 4);
-  p.at_clean = take(p.has_dw, static_cast<size_t>(p.chunk) * x_ld * es);
-  p.at_keep = take(!fused && p.has_dw, static_cast<size_t>(p.chunk) * 4);
-  p.at_sum = take(p.sums, static_cast<size_t>(columns_first(p.dw) ? p.V : p.D) * p.ld_sum * 4);
-  p.products_bytes = 0;
-  if (type == CDL_F32) {  // (bf16 operands are on the grid by now)
-    auto need = [&](const cdl_tensor& a, const cdl_tensor& b, const cdl_tensor& d) {
-      const size_t n = matmul_general_scratch_bytes(&a, &b, &d);
-      if (n > p.products_bytes) p.products_bytes = n;
-    };
-    alignas(256) static float nowhere[64];
-    const cdl_tensor z = strided2(nowhere, CDL_F32, p.chunk, p.V, p.ld_z);
-    const cdl_tensor x = p.copy_x ? strided2(nowhere, type, p.chunk, p.D, x_ld) : rows_of(p.x, 0, p.chunk);
-    need(x, p.w, z);
-    if (p.has_dx) need(z, transposed(p.w), strided2(nowhere, type, p.chunk, p.D, p.D));
-    if (p.has_dw) {
-      const cdl_tensor clean = strided2(nowhere, type, p.chunk, p.D, x_ld);
-      if (columns_first(p.dw)) need(transposed(z), clean, strided2(nowhere, CDL_F32, p.V, p.D, up(p.D, 4)));
-      else need(transposed(clean), z, strided2(nowhere, CDL_F32, p.D, p.V, p.ld_z));
-    }
+  const size_t w_rows = wc ? p.V : p.D, dw_rows = dc ? p.V : p.D;
+  if (p.f32) {
+    p.at_x = take(true, 3 * n * p.ld_x * 2);
+    p.at_w = take(true, 3 * w_rows * p.ld_w * 2);
+    p.at_clean = take(p.has_dw, 3 * n * p.ld_x * 2);
+    p.at_keep = take(p.has_dw, n * 4);
+    p.at_z = take(true, n * p.ld_g * 4);
+    p.at_g = take(grad, 3 * n * p.ld_g * 2);
+  } else {
+    p.at_x = take(p.copy_x, static_cast<size_t>(p.T) * p.ld_x * 2);
+    p.at_w = take(p.copy_w, w_rows * p.ld_w * 2);
+    p.at_clean = take(p.has_dw, n * p.ld_x * 2);
+    p.at_g = take(grad, n * p.ld_g * 2);
+    p.at_stats = take(true, n * p.pieces * sizeof(float2));
+    p.at_at = take(true, n * (teacher ? p.K : 1) * 4);
+    p.at_ids = take(teacher, n * p.K * 4);
+    p.at_p = take(teacher, n * p.K * 4);
+    p.at_p_log_p = take(teacher, n * 4);
+    p.at_first = take(teacher, n * (p.pieces + 1) * 2);
   }
-  p.at_products = take(p.products_bytes != 0, p.products_bytes);
+  size_t planes = 0;
+  auto need = [&](int slices, size_t rows, size_t ld) {
+    if (slices > 1 && slices * rows * ld * 4 > planes) planes = slices * rows * ld * 4;
+  };
+  need(p.slices_z, n, p.ld_g);
+  need(p.slices_dx, n, p.ld_x);
+  need(p.slices_dw, dw_rows, p.ld_sum);
+  p.at_planes = take(planes != 0, planes);
+  p.at_sum = take(p.dw_way != Linear::DIRECT, dw_rows * p.ld_sum * (p.dw_way == Linear::SUMMED ? 4 : 2));
   p.bytes = at;
-  return CDL_OK;
 }
 
 static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
@@ -1139,7 +1182,8 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
   }
   if (p.V == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
   if (p.D == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: hidden is zero", op);
-  return plan_linear(p, desc, entries);
+  if (p.T > 0) plan_linear(p, desc, entries);
+  return CDL_OK;
 }
 
 // The statistics, losses and logits' gradients of a chunk of rows of bf16 operands on the 16-byte grid.
@@ -1176,94 +1220,123 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
   return CDL_OK;
 }
 
+// [3][rows][cols] pieces (ld), planes `plane` apart; transposed: [3][cols][rows] views of them.
+static cdl_tensor pieces3(void* ptr, long long rows, long long cols, long long ld, long long plane, bool transpose = false) {
+  cdl_tensor t{};
+  t.ptr = ptr;
+  t.dtype = CDL_BF16;
+  t.rank = 3;
+  t.shape[0] = 3;
+  t.stride[0] = plane;
+  t.shape[transpose ? 2 : 1] = rows;
+  t.stride[transpose ? 2 : 1] = ld;
+  t.shape[transpose ? 1 : 2] = cols;
+  t.stride[transpose ? 1 : 2] = 1;
+  return t;
+}
+
+// D (+)= A B of pieces, by way of planes if there are slices.
+static int32_t pieces_product(const Linear& p, const cdl_tensor& a, const cdl_tensor& b, const cdl_tensor& d, int slices, int add, char* base,
+                              cudaStream_t stream) {
+  const long long M = d.shape[0], N = d.shape[1], ld = up(N, 8), k_blocks = (a.shape[2] + 63) / 64;
+  if (slices > k_blocks) slices = static_cast<int>(k_blocks);  // (the last rows are fewer)
+  if (slices == 1 && (d.stride[1] == 1 || N == 1))
+    return matmul_pieces_execute(&a, &b, static_cast<float*>(d.ptr), M > 1 ? d.stride[0] : ld, 1, add, stream);
+  float* planes = reinterpret_cast<float*>(base + p.at_planes);
+  CDL_CHECK(matmul_pieces_execute(&a, &b, planes, ld, slices, 0, stream));
+  return sum_planes(planes, CDL_F32, ld, M * ld, slices, d, add, stream);
+}
+
 static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& entries, const RowTerms& terms, void* scratch,
                               size_t scratch_bytes, cudaStream_t stream) {
-  const bool grad = p.has_dx || p.has_dw;
+  const bool grad = p.has_dx || p.has_dw, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
+  const cdl_tensor dw_near = dc ? transposed(p.dw) : p.dw;  // dimension 1 the nearer one in memory
   if (p.T == 0) {  // no rows: no loss, and a gradient of zeros
-    if (p.has_dw && !desc->accumulate_dw && p.D > 0 && p.V > 0) CDL_CHECK(finish(nullptr, 0, p.dw, 0, stream));
+    if (p.has_dw && !desc->accumulate_dw && p.D > 0 && p.V > 0) CDL_CHECK(sum_planes(nullptr, CDL_F32, 0, 0, 0, dw_near, 0, stream));
     return CDL_OK;
   }
   if (p.bytes > 0 && (!scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(scratch) & 255)))
     return fail(CDL_ERR_INVALID, "%s: scratch must hold %zu bytes, 256-byte aligned", p.op, p.bytes);
   const FixedWorkInGraph fixed_work(stream);
   char* base = static_cast<char*>(scratch);
-  const int32_t type = p.x.dtype;
-  const long long x_ld = up(p.D, 8);
-  cdl_tensor x = p.x, w = p.w;
-  if (p.copy_x) {
-    CDL_CHECK(copy(p.x, base + p.at_x, x_ld, nullptr, stream));
-    x = strided2(base + p.at_x, type, p.T, p.D, x_ld);
-  }
-  if (p.copy_w) {
-    if (columns_first(p.w)) {
-      const long long ld = up(p.D, 8);
-      CDL_CHECK(copy(transposed(p.w), base + p.at_w, ld, nullptr, stream));
-      w = transposed(strided2(base + p.at_w, type, p.V, p.D, ld));
-    } else {
-      const long long ld = up(p.V, 8);
-      CDL_CHECK(copy(p.w, base + p.at_w, ld, nullptr, stream));
-      w = strided2(base + p.at_w, type, p.D, p.V, ld);
-    }
-  }
-  const cdl_tensor wt = transposed(w);
-  void* products = p.products_bytes ? base + p.at_products : nullptr;
-  // Sums over the rows in a fixed order: the same gradient every time.
-  cdl_matmul_options fixed = {CDL_GEMM_AUTO, 1};
-  const bool dw_columns = p.has_dw && columns_first(p.dw);
-  cdl_tensor sum = p.dw;
-  if (p.sums)
-    sum = dw_columns ? transposed(strided2(base + p.at_sum, CDL_F32, p.V, p.D, p.ld_sum))
-                     : strided2(base + p.at_sum, CDL_F32, p.D, p.V, p.ld_sum);
-  const bool fused = type == CDL_BF16;
-  for (long long row = 0; row < p.T; row += p.chunk) {
-    const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
-    const cdl_tensor xc = rows_of(x, row, n);
-    const Entries e = from_row(entries, row);
-    const RowTerms t = from_row(terms, row);
-    const cdl_tensor g = strided2(base + p.at_g, type, n, p.V, p.ld_g);
-    // A row that does not count adds nothing to dw whatever x holds there, infinities and NaN too, which a gradient of zeros
-    // alone would not do: the product takes a copy of x with zeros in such rows (made before dx is written, which may
-    // be x itself).
-    const cdl_tensor clean = strided2(base + p.at_clean, type, n, p.D, x_ld);
-    if (fused) {
-      CDL_CHECK(fused_rows(p, xc, w, e, t, clean, base, grad, stream));
-    } else {
-      const cdl_tensor z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_z);
-      CDL_CHECK(matmul_execute(&xc, &w, nullptr, &z, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
-      CDL_CHECK(launch_rows<float>(z.ptr, p.ld_z, grad ? g.ptr : nullptr, p.ld_g, n, static_cast<int>(p.V), e, t, stream));
-      if (p.has_dw) {
+  const int vocab = static_cast<int>(p.V);
+  // Where dw's product goes, as [D, V] or (dc) [V, D].
+  cdl_tensor dw = dw_near;
+  if (p.dw_way != Linear::DIRECT)
+    dw = strided2(base + p.at_sum, p.dw_way == Linear::SUMMED ? CDL_F32 : CDL_BF16, dc ? p.V : p.D, dc ? p.D : p.V, p.ld_sum);
+  if (p.f32) {
+    const cdl_tensor w_near = wc ? transposed(p.w) : p.w;
+    const long long w_plane = w_near.shape[0] * p.ld_w, x_plane = p.chunk * p.ld_x, g_plane = p.chunk * p.ld_g;
+    CDL_CHECK(split(w_near, base + p.at_w, p.ld_w, w_plane, nullptr, stream));
+    const cdl_tensor w3 = pieces3(base + p.at_w, w_near.shape[0], w_near.shape[1], p.ld_w, w_plane, wc);    // [3][D][V]
+    const cdl_tensor wt3 = pieces3(base + p.at_w, w_near.shape[0], w_near.shape[1], p.ld_w, w_plane, !wc);  // [3][V][D]
+    for (long long row = 0; row < p.T; row += p.chunk) {
+      const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
+      const cdl_tensor xc = rows_of(p.x, row, n), z = strided2(base + p.at_z, CDL_F32, n, p.V, p.ld_g);
+      const Entries e = from_row(entries, row);
+      CDL_CHECK(split(xc, base + p.at_x, p.ld_x, x_plane, nullptr, stream));
+      CDL_CHECK(pieces_product(p, pieces3(base + p.at_x, n, p.D, p.ld_x, x_plane), w3, z, p.slices_z, 0, base, stream));
+      CDL_CHECK(launch_rows<float>(z.ptr, p.ld_g, grad ? z.ptr : nullptr, p.ld_g, n, vocab, e, from_row(terms, row), stream));
+      if (!grad) continue;
+      if (p.has_dw) {  // (the copy with zeros in rows that do not count, see below)
         float* keep = reinterpret_cast<float*>(base + p.at_keep);
-        keep_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(e, n, static_cast<int>(p.V), keep);
-        CDL_CUDA(cudaGetLastError());
-        CDL_CHECK(copy(xc, clean.ptr, x_ld, keep, stream));
+        CDL_CUDA(launch_pdl(keep_kernel, dim3(static_cast<unsigned>((n + 7) / 8)), dim3(256), 0, stream, e, n, vocab, keep));
+        CDL_CHECK(split(xc, base + p.at_clean, p.ld_x, x_plane, keep, stream));
+      }
+      CDL_CHECK(split(z, base + p.at_g, p.ld_g, g_plane, nullptr, stream));
+      if (p.has_dx)
+        CDL_CHECK(pieces_product(p, pieces3(base + p.at_g, n, p.V, p.ld_g, g_plane), wt3, rows_of(p.dx, row, n), p.slices_dx, 0, base, stream));
+      if (p.has_dw) {
+        const bool add = row > 0 || (p.dw_way == Linear::DIRECT && desc->accumulate_dw);
+        const cdl_tensor g3 = pieces3(base + p.at_g, n, p.V, p.ld_g, g_plane, dc), x3 = pieces3(base + p.at_clean, n, p.D, p.ld_x, x_plane, !dc);
+        CDL_CHECK(pieces_product(p, dc ? g3 : x3, dc ? x3 : g3, dw, p.slices_dw, add, base, stream));
       }
     }
-    const cdl_tensor d = p.has_dx ? rows_of(p.dx, row, n) : cdl_tensor{};
-    float* planes = reinterpret_cast<float*>(base + p.at_planes);
-    if (p.slices > 1) {
-      CDL_CHECK(matmul_planes_execute(&g, &wt, planes, x_ld, p.slices, stream));
-      const bool vectors = (reinterpret_cast<uintptr_t>(d.ptr) & 7) == 0 && (n == 1 || d.stride[0] % 4 == 0);
-      ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(n) * p.D * (4 * p.slices + 2), stream);
-      CDL_CUDA(launch_pdl(sum_planes_kernel, dim3(static_cast<unsigned>((n * ((p.D + 3) / 4) + 255) / 256)), dim3(256), 0, stream, planes, x_ld,
-                          p.slices, static_cast<__nv_bfloat16*>(d.ptr), static_cast<long long>(d.stride[0]), static_cast<int>(n),
-                          static_cast<int>(p.D), vectors ? 1 : 0));
-    } else if (p.has_dx) {
-      CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream, nullptr, products, p.products_bytes));
+  } else {
+    cdl_tensor x = p.x, w = p.w;
+    if (p.copy_x) {
+      CDL_CHECK(copy(p.x, base + p.at_x, p.ld_x, stream));
+      x = strided2(base + p.at_x, CDL_BF16, p.T, p.D, p.ld_x);
     }
-    if (p.has_dw) {
-      const bool add = row > 0 || (!p.sums && desc->accumulate_dw);
-      const cdl_tensor gt = transposed(g), xt = transposed(clean), sum_t = transposed(sum);
-      const cdl_tensor *a = dw_columns ? &gt : &xt, *b = dw_columns ? &clean : &g, *d = dw_columns ? &sum_t : &sum;
-      // (beside dx's product, whose last wave leaves SMs idle: the two share what they read alone)
-      if (fused && !add && matmul_store_bound(a, b, d)) CDL_CHECK(matmul_store_execute(a, b, d, stream, p.has_dx ? 1 : 0));
-      else CDL_CHECK(matmul_execute(a, b, add ? d : nullptr, d, 1.f, add ? 1.f : 0.f, stream, &fixed, products, p.products_bytes,
-                               fused && p.has_dx ? 1 : 0));
+    if (p.copy_w) {
+      const cdl_tensor w_near = wc ? transposed(p.w) : p.w;
+      CDL_CHECK(copy(w_near, base + p.at_w, p.ld_w, stream));
+      w = strided2(base + p.at_w, CDL_BF16, w_near.shape[0], w_near.shape[1], p.ld_w);
+      if (wc) w = transposed(w);
+    }
+    const cdl_tensor wt = transposed(w);
+    // Sums over the rows in a fixed order: the same gradient every time.
+    cdl_matmul_options fixed = {CDL_GEMM_AUTO, 1};
+    for (long long row = 0; row < p.T; row += p.chunk) {
+      const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
+      const cdl_tensor g = strided2(base + p.at_g, CDL_BF16, n, p.V, p.ld_g);
+      // A row that does not count adds nothing to dw whatever x holds there, infinities and NaN too, which a gradient of zeros
+      // alone would not do: the product takes a copy of x with zeros in such rows (made before dx is written, which may
+      // be x itself).
+      const cdl_tensor clean = strided2(base + p.at_clean, CDL_BF16, n, p.D, p.ld_x);
+      CDL_CHECK(fused_rows(p, rows_of(x, row, n), w, from_row(entries, row), from_row(terms, row), clean, base, grad, stream));
+      if (p.has_dx) {
+        const cdl_tensor d = rows_of(p.dx, row, n);
+        if (p.slices_dx > 1) {
+          float* planes = reinterpret_cast<float*>(base + p.at_planes);
+          CDL_CHECK(matmul_planes_execute(&g, &wt, planes, p.ld_x, p.slices_dx, stream));
+          CDL_CHECK(sum_planes(planes, CDL_F32, p.ld_x, n * p.ld_x, p.slices_dx, d, 0, stream));
+        } else {
+          CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream));
+        }
+      }
+      if (p.has_dw) {
+        const bool add = row > 0 || (p.dw_way == Linear::DIRECT && desc->accumulate_dw);
+        const cdl_tensor a = dc ? transposed(g) : transposed(clean), &b = dc ? clean : g;
+        // (beside the kernel ahead, dx's, whose last wave leaves SMs idle: the two share what they read alone)
+        const int early = p.has_dx ? 1 : 0;
+        if (!add && matmul_store_bound(&a, &b, &dw)) CDL_CHECK(matmul_store_execute(&a, &b, &dw, stream, early));
+        else CDL_CHECK(matmul_execute(&a, &b, add ? &dw : nullptr, &dw, 1.f, add ? 1.f : 0.f, stream, &fixed, nullptr, 0, early));
+      }
     }
   }
-  if (p.sums) {
-    if (dw_columns) CDL_CHECK(finish(static_cast<float*>(sum.ptr), p.ld_sum, transposed(p.dw), desc->accumulate_dw, stream));
-    else CDL_CHECK(finish(static_cast<float*>(sum.ptr), p.ld_sum, p.dw, desc->accumulate_dw, stream));
-  }
+  if (p.has_dw && p.dw_way != Linear::DIRECT)
+    CDL_CHECK(sum_planes(dw.ptr, dw.dtype, p.ld_sum, 0, 1, dw_near, desc->accumulate_dw, stream));
   return CDL_OK;
 }
 

@@ -291,6 +291,24 @@ def test_linear_losses_in_chunks_of_rows(cdl, gpu_ok, k, chunk):
 
 
 @gpu
+@pytest.mark.parametrize("layout", ["rows", "tied", "columns"])
+@pytest.mark.parametrize("t,d,v,chunk", [(601, 64, 777, 600), (601, 130, 260, 100), (5, 64, 300, 1), (1200, 72, 520, 0), (260, 40, 12000, 0), (90, 700, 9000, 0)])
+def test_linear_losses_of_f32_operands(cdl, gpu_ok, layout, t, d, v, chunk):
+    """K slices of the products, rows in chunks (one row left for the last), gradients added to what is there."""
+    gen = torch.Generator(device="cuda").manual_seed(t + v)
+    x, w = _operands(gen, t, d, v, F32, layout)
+    for k in (0, 11):
+        entries = _entries(gen, t, v, k)
+        o = _check_linear(cdl, x, w, entries, cdl.ops.LinearLossOpts(chunk_rows=chunk))
+        before = torch.randn(d, v, generator=gen, device="cuda")
+        dw = before.clone()
+        fn = cdl.ops.linear_cross_entropy if k == 0 else cdl.ops.linear_distillation
+        added = fn(x, w, *entries, cdl.ops.LinearLossOpts(chunk_rows=chunk, accumulate=True), dw=dw)
+        # (f32 sums of other terms in another order: 2^-22 of the parts)
+        assert bool(((added.dw - before - o.dw).abs() <= 2.0 ** -20 * (before.abs() + o.dw.abs() + 1)).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("tied", [False, True])
 @pytest.mark.parametrize("chunk", [0, 128])
@@ -375,6 +393,8 @@ def test_rows_that_do_not_count_add_nothing(cdl, gpu_ok, dtype, k):
 
 @gpu
 def test_no_tokens(cdl, gpu_ok):
+    empty = torch.empty(0, 0, dtype=BF16, device="cuda")
+    assert cdl.ops.linear_cross_entropy(empty, empty, torch.empty(0, dtype=torch.int32, device="cuda")).loss.shape == (0,)
     x, w = torch.empty(0, 64, dtype=BF16, device="cuda"), torch.randn(64, 100, device="cuda").to(BF16)
     o = cdl.ops.linear_cross_entropy(x, w, torch.empty(0, dtype=torch.int32, device="cuda"))
     assert o.loss.shape == (0,) and o.dx.shape == (0, 64) and bool((o.dw == 0).all())
