@@ -595,15 +595,18 @@ __global__ void __launch_bounds__(PREPARE_WARPS * 32)
 constexpr int PIECES_PER_WARP = 64;  // at most: 8192 columns
 constexpr int ROWS_PER_CTA = 8;      // a warp's each
 
-// From the pieces' statistics the rows': loss, lse, and (GRAD) the gradient of the logits in bf16 in place of the
+// From the pieces' statistics the rows': loss, lse, and (with gradients) the gradient of the logits in bf16 in place of the
 // exponentials, which are only multiplied with 2^(M' - M) s tau / S; the rows of x for the weight gradient's product,
-// zeros where a row does not count.  Grid (rows / 8, pieces / per), a row and `per` pieces per warp; the warps have nothing
+// zeros where a row does not count.  GRAD_TWICE: what bf16 rounds away, in bf16 `rows` rows further on, and the rows of x again
+// there: see Linear::twice.  Grid (rows / 8, pieces / per), a row and `per` pieces per warp; the warps have nothing
 // to wait for in one another.
-template <bool GRAD>
+enum RowsMode { LOSS_ONLY, GRAD_ONCE, GRAD_TWICE };
+template <int MODE>
 __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     softmax_rows_kernel(const float2* stats, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
                         int K, const Prepared src, const RowTerms terms, const __nv_bfloat16* x, long long ld_x, __nv_bfloat16* clean,
                         long long ld_clean, int cols) {
+  constexpr bool GRAD = MODE != LOSS_ONLY;
   __shared__ float factor[ROWS_PER_CTA][PIECES_PER_WARP];
   grid_dep_wait();
   grid_dep_launch();
@@ -654,6 +657,7 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
   for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i].x - base) * over_s;
   __syncwarp();
   uint4* at = reinterpret_cast<uint4*>(e + row * ld_e + piece0 * 128);
+  uint4* rest = reinterpret_cast<uint4*>(e + (static_cast<long long>(rows) + row) * ld_e + piece0 * 128);
   const int vecs = (piece1 - piece0) * 16;  // of 8 columns
   constexpr int DEEP = 2;  // (4 and 8: the same to 2 % more)
   for (int v = lane; v < vecs; v += 32 * DEEP) {
@@ -665,13 +669,16 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     for (int d = 0; d < DEEP; ++d) {
       if (v + 32 * d >= vecs) break;
       const float f = factor[warp][(v + 32 * d) >> 4];
-      uint32_t* w = &q[d].x;
+      uint4 lo;
+      uint32_t *w = &q[d].x, *l = &lo.x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
         w[j] = pack_bf16x2(h.x * f, h.y * f);
+        if (MODE == GRAD_TWICE) l[j] = pack_bf16x2(h.x * f - bf16_lo(w[j]), h.y * f - bf16_hi(w[j]));
       }
       at[v + 32 * d] = counts ? q[d] : make_uint4(0, 0, 0, 0);  // (whatever the logits were)
+      if (MODE == GRAD_TWICE) rest[v + 32 * d] = counts ? lo : make_uint4(0, 0, 0, 0);
     }
   }
   if (clean != nullptr) {  // the splits share the row of x
@@ -681,9 +688,14 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
       const __nv_bfloat16* from = x + row * ld_x + i * 8;
       __nv_bfloat16* to = clean + row * ld_clean + i * 8;
       if (i * 8 + 8 <= cols) {
-        *reinterpret_cast<uint4*>(to) = counts ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+        const uint4 v = counts ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(to) = v;
+        if (MODE == GRAD_TWICE) *reinterpret_cast<uint4*>(to + rows * ld_clean) = v;
       } else {
-        for (int j = 0; i * 8 + j < cols; ++j) to[j] = counts ? from[j] : __float2bfloat16_rn(0.f);
+        for (int j = 0; i * 8 + j < cols; ++j) {
+          to[j] = counts ? from[j] : __float2bfloat16_rn(0.f);
+          if (MODE == GRAD_TWICE) to[rows * ld_clean + j] = to[j];
+        }
       }
     }
   }
@@ -701,7 +713,10 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     if (src.first == nullptr ? id / 128 < piece0 || id / 128 >= piece1 : k > k0 && ids[k - 1] == id) continue;
     float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
     for (int i = k + 1; i < k1 && ids[i] == id; ++i) p += src.p[static_cast<long long>(row) * K + i];
-    e[row * ld_e + id] = __float2bfloat16_rn(scale * (ex2(src.at[static_cast<long long>(row) * K + k] - base) / S - p));
+    const float g = scale * (ex2(src.at[static_cast<long long>(row) * K + k] - base) / S - p);
+    const __nv_bfloat16 hi = __float2bfloat16_rn(g);
+    e[row * ld_e + id] = hi;
+    if (MODE == GRAD_TWICE) e[(static_cast<long long>(rows) + row) * ld_e + id] = __float2bfloat16_rn(g - __bfloat162float(hi));
   }
 }
 
@@ -840,8 +855,9 @@ static RowTerms from_row(RowTerms t, long long row) {
   return t;
 }
 
-// Warps and slices by the row's size alone: 4, 8 or 16 warps up to 4 KB, 16 KB and 64 KB; longer rows in a cluster of up to 8 CTAs,
-// of 8 warps up to 256 KB (1500 x 50000 f32 168 us; with 16 195), else of 16: 512 KB, and 1 MB with 16 vectors a lane.
+// Warps and slices by the row's size alone: a warp per 4 KB (8 vectors a lane; 6471 x 5047 f32 58 us, with 16 warps 123), per
+// 2 KB up to 8 KB (8192 x 2000 bf16 38, 45); rows beyond 64 KB in a cluster of up to 8 CTAs, of 8 warps up to 256 KB
+// (1500 x 50000 f32 168; with 16 195), else of 16: 512 KB, and 1 MB with 16 vectors a lane.
 // More CTAs share those warps while SMs are without one.  warps = 0: longer rows, which are read twice.
 struct Share {
   int warps, slice, ctas, slots_log2;  // warps of a row, vectors of a warp, CTAs of a row, the entries' hash table
@@ -852,13 +868,15 @@ static Share choose_share(const void* z, long long ld, long long rows, int vocab
   const bool on_grid = (reinterpret_cast<uintptr_t>(z) & 15) == 0 && (rows == 1 || ld * size % 16 == 0);
   const long long vecs = (static_cast<long long>(vocab) + (on_grid ? 1 : 2) * (vec - 1)) / vec;  // (wherever the row starts in its first)
   Share s = {};
-  const int warps = vecs <= 256 ? 4 : vecs <= 1024 ? 8 : vecs <= 16 * 256 || vecs > 8 * 8 * 256 ? 16 : 8;  // of a CTA
+  const int slice = vecs <= 512 ? 128 : 256;
+  const int warps = vecs <= 16 * 256 ? static_cast<int>((vecs + slice - 1) / slice) : vecs <= 8 * 8 * 256 ? 8 : 16;  // of a CTA
   const long long ctas = (vecs + warps * 256 - 1) / (warps * 256);
   s.ctas = ctas <= 8 ? static_cast<int>(ctas) : 8;
   s.warps = warps * s.ctas;
   s.slice = static_cast<int>((vecs + s.warps - 1) / s.warps);
   if (s.slice > 512) return {};
-  while (2 * s.ctas <= 8 && rows * s.ctas < sm_count() && s.warps / s.ctas >= 2 && s.slice >= 64) s.ctas *= 2;
+  for (int c = s.ctas + 1; c <= 8 && rows * s.ctas < sm_count() && s.slice >= 64; ++c)
+    if (s.warps % c == 0) s.ctas = c;
   s.slots_log2 = 5;
   while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (with 2 K slots 64 random ids cost 8192 x 32768 290 us, not 228)
   s.smem = static_cast<size_t>(ENTRY_BYTES) * K + (4u << s.slots_log2);  // at most 44 KB
@@ -1056,6 +1074,10 @@ struct Linear {
   // Scratch.  Rows are taken `chunk` at a time.
   long long chunk, ld_x, ld_w, ld_g, ld_sum;
   bool copy_x, copy_w;
+  // Few rows of bf16 operands: the bytes of w and dw set the products' time, which take d z as two bf16 pieces then, one below
+  // the other: [2 rows, V], the rows of x twice.  With one piece dx and dw are 1.4 times as far off as their own rounding
+  // to bf16, give or take what the rounding of a single row's largest value happens to be.
+  bool twice;
   enum { DIRECT, HELD, SUMMED } dw_way;  // the product stores dw; a bf16 dw off the grid, stored beside it first; an f32 sum over the chunks
   int pieces, slices_z, slices_dx, slices_dw;  // pieces: of the vocabulary, 128 columns each
   size_t at_x, at_w, at_clean, at_keep, at_z, at_g, at_stats, at_ids, at_first, at_p, at_p_log_p, at_at, at_planes, at_sum, bytes;
@@ -1101,13 +1123,14 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
   p.dw_way = Linear::DIRECT;
   if (p.has_dw && !(on_grid(p.dw) && (p.dw.dtype == CDL_F32 || whole)))
     p.dw_way = p.dw.dtype == CDL_BF16 && whole && !desc->accumulate_dw ? Linear::HELD : Linear::SUMMED;
-  const size_t n = static_cast<size_t>(p.chunk);
+  p.twice = !p.f32 && grad && whole && p.T <= 64;
+  const size_t n = static_cast<size_t>(p.chunk), g_rows = p.twice ? 2 * n : n;
   p.ld_x = up(p.D, 8);
   p.ld_w = up(wc ? p.D : p.V, 8);
   p.ld_g = up(p.V, 128);
   p.ld_sum = p.has_dw ? up(dc ? p.D : p.V, 8) : 0;
   p.slices_z = p.f32 ? matmul_plane_slices(p.chunk, p.V, p.D, true) : 1;
-  p.slices_dx = p.has_dx ? matmul_plane_slices(p.chunk, p.D, p.V, p.f32) : 1;
+  p.slices_dx = p.has_dx ? matmul_plane_slices(static_cast<long long>(g_rows), p.D, p.V, p.f32) : 1;
   p.slices_dw = p.has_dw && p.f32 ? matmul_plane_slices(dc ? p.V : p.D, dc ? p.D : p.V, p.chunk, true) : 1;
   size_t at = 0;
   auto take = [&](bool want, size_t bytes) {
@@ -1126,8 +1149,8 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
   } else {
     p.at_x = take(p.copy_x, static_cast<size_t>(p.T) * p.ld_x * 2);
     p.at_w = take(p.copy_w, w_rows * p.ld_w * 2);
-    p.at_clean = take(p.has_dw, n * p.ld_x * 2);
-    p.at_g = take(grad, n * p.ld_g * 2);
+    p.at_clean = take(p.has_dw, g_rows * p.ld_x * 2);
+    p.at_g = take(grad, g_rows * p.ld_g * 2);
     p.at_stats = take(true, n * p.pieces * sizeof(float2));
     p.at_at = take(true, n * (teacher ? p.K : 1) * 4);
     p.at_ids = take(teacher, n * p.K * 4);
@@ -1140,7 +1163,7 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
     if (slices > 1 && slices * rows * ld * 4 > planes) planes = slices * rows * ld * 4;
   };
   need(p.slices_z, n, p.ld_g);
-  need(p.slices_dx, n, p.ld_x);
+  need(p.twice ? 2 * p.slices_dx : p.slices_dx, n, p.ld_x);
   need(p.slices_dw, dw_rows, p.ld_sum);
   p.at_planes = take(planes != 0, planes);
   p.at_sum = take(p.dw_way != Linear::DIRECT, dw_rows * p.ld_sum * (p.dw_way == Linear::SUMMED ? 4 : 2));
@@ -1211,12 +1234,13 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
                       static_cast<int>(p.D));
   };
   if (!grad) {
-    CDL_CUDA(run(softmax_rows_kernel<false>, 1, p.pieces));
+    CDL_CUDA(run(softmax_rows_kernel<LOSS_ONLY>, 1, p.pieces));
     return CDL_OK;
   }
   int per = PIECES_PER_WARP;  // fewer where that leaves SMs without a CTA
   while (per > 8 && row_ctas * ((p.pieces + per - 1) / per) < 2u * sm_count()) per /= 2;
-  CDL_CUDA(run(softmax_rows_kernel<true>, (p.pieces + per - 1) / per, per));
+  const unsigned splits = (p.pieces + per - 1) / per;
+  CDL_CUDA(p.twice ? run(softmax_rows_kernel<GRAD_TWICE>, splits, per) : run(softmax_rows_kernel<GRAD_ONCE>, splits, per));
   return CDL_OK;
 }
 
@@ -1309,18 +1333,20 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
     cdl_matmul_options fixed = {CDL_GEMM_AUTO, 1};
     for (long long row = 0; row < p.T; row += p.chunk) {
       const long long n = p.T - row < p.chunk ? p.T - row : p.chunk;
-      const cdl_tensor g = strided2(base + p.at_g, CDL_BF16, n, p.V, p.ld_g);
+      const long long g_rows = p.twice ? 2 * n : n;
+      const cdl_tensor g = strided2(base + p.at_g, CDL_BF16, g_rows, p.V, p.ld_g);
       // A row that does not count adds nothing to dw whatever x holds there, infinities and NaN too, which a gradient of zeros
       // alone would not do: the product takes a copy of x with zeros in such rows (made before dx is written, which may
       // be x itself).
-      const cdl_tensor clean = strided2(base + p.at_clean, CDL_BF16, n, p.D, p.ld_x);
+      const cdl_tensor clean = strided2(base + p.at_clean, CDL_BF16, g_rows, p.D, p.ld_x);
       CDL_CHECK(fused_rows(p, rows_of(x, row, n), w, from_row(entries, row), from_row(terms, row), clean, base, grad, stream));
       if (p.has_dx) {
         const cdl_tensor d = rows_of(p.dx, row, n);
-        if (p.slices_dx > 1) {
+        const int planes_per_slice = p.twice ? 2 : 1;
+        if (p.slices_dx * planes_per_slice > 1) {
           float* planes = reinterpret_cast<float*>(base + p.at_planes);
           CDL_CHECK(matmul_planes_execute(&g, &wt, planes, p.ld_x, p.slices_dx, stream));
-          CDL_CHECK(sum_planes(planes, CDL_F32, p.ld_x, n * p.ld_x, p.slices_dx, d, 0, stream));
+          CDL_CHECK(sum_planes(planes, CDL_F32, p.ld_x, n * p.ld_x, p.slices_dx * planes_per_slice, d, 0, stream));
         } else {
           CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream));
         }

@@ -531,7 +531,7 @@ int32_t cdl_b200_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* 
  *   dw  (nullable) f32 or x's type [hidden, vocab], any strides:  x^T . d z, added to with accumulate_dw.  Held in f32 over
  *       all tokens and rounded once.
  * For bf16 operands d z is rounded to bf16 before both products, as cdl_b200_cross_entropy rounds it: an f32 dw has that
- * accuracy then.  f32 operands keep it in f32.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that
+ * accuracy then.  (Up to 64 tokens, where it costs no time, it goes into them as two bf16 values.)  f32 operands keep 24 bits of it.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that
  * the call below gives for the same operands (entries: teacher_ids' second dimension, 1 for targets). */
 int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
                                       const cdl_tensor* targets, const cdl_tensor* d_loss, const cdl_tensor* loss,

@@ -97,7 +97,8 @@ def _hit(ids, vocab):
     (64, 8192, 33, 2.0, BF16, 16), (9, 32768, 64, 2.0, BF16, 0), (6, 32768, 300, 4.0, F32, 8), (4, 50001, 1024, 1.0, BF16, 0),
     (3, 150000, 20, 1.5, BF16, 0), (3, 150001, 20, 1.5, F32, 2), (17, 129, 129, 1.0, F32, 0), (300, 2048, 16, 1.0, BF16, 0),
     (700, 1003, 3, 1.0, BF16, 0), (200, 36861, 9, 1.0, BF16, 0), (2, 900001, 8, 1.0, BF16, 0), (2, 450001, 8, 2.0, F32, 0),
-    (2, 400000, 1024, 2.0, F32, 4), (160, 2, 2, 1.0, BF16, 0), (160, 9, 4, 1.0, F32, 1)])
+    (2, 400000, 1024, 2.0, F32, 4), (160, 2, 2, 1.0, BF16, 0), (160, 9, 4, 1.0, F32, 1), (3, 6000, 4, 1.0, F32, 0), (40, 10000, 4, 1.0, BF16, 0),
+    (40, 14000, 40, 1.0, BF16, 0), (200, 14001, 40, 1.0, BF16, 0), (30, 26000, 3, 1.0, BF16, 0), (10, 45000, 3, 1.0, F32, 0), (2, 70000, 3, 1.0, F32, 0)])
 def test_distillation(cdl, gpu_ok, rows, vocab, k, tau, dtype, pad):
     gen = torch.Generator(device="cuda").manual_seed(rows * 7 + vocab)
     _, logits = _logits(gen, rows, vocab, dtype, pad)
