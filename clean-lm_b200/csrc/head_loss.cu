@@ -4,9 +4,10 @@
 // Every loss here holds q = softmax(z / tau) of a row of logits against a distribution p that is zero but for a few
 // entries (one for a target, K for a teacher), so that the gradient of the logits is
 //     G_j = s tau (q_j - p_j),      s = grad_scale * d_loss[row]
-// (cross entropy: tau = 1, p = 1 at the target).  With t_j = z_j log2(e) / tau, M = max t, S = sum 2^(t_j - M):
-//     q_j = 2^(t_j - M) / S,   log q_j = ln 2 ((t_j - M) - log2 S),   lse = ln 2 (M + log2 S).
-// All statistics are f32.
+// (cross entropy: tau = 1, p = 1 at the target).  With c = log2(e) / tau, M = max z, S = sum 2^(c (z_j - M)):
+//     q_j = 2^(c (z_j - M)) / S,   log q_j = ln 2 (c (z_j - M) - log2 S),   lse = M / tau + ln 2 log2 S.
+// All statistics are f32.  From stored logits differences are taken before they are scaled: a row masked with the type's
+// lowest value, which times c overflows, is a uniform one.
 #include "host.h"
 #include "ops.h"
 #include "ptx.cuh"
@@ -83,7 +84,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 struct RowEntries {
   int* id;    // -1: does not count
   float* p;   // of the entry
-  float* at;  // t of the row at the id
+  float* at;  // the row's logit at the id
   __device__ __forceinline__ RowEntries(void* smem, int K) : id(static_cast<int*>(smem)), p(static_cast<float*>(smem) + K), at(p + K) {}
 };
 constexpr int ENTRY_BYTES = 12;
@@ -104,7 +105,7 @@ __device__ __forceinline__ float cta_reduce(float v, bool max, float* part) {
 }
 
 // A row's entries by one warp: ids and p = softmax(teacher / tau) over those that count (id in [0, vocab), logit above
-// -inf); sum p log p; whether there are any; and (x != nullptr) t at the ids.  Four entries of a lane are under way at a
+// -inf); sum p log p; whether there are any; and (x != nullptr) the row's logits at the ids.  Four entries of a lane are under way at a
 // time: their latency is what this costs.
 template <typename T>
 __device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh, const Entries& src, long long row, int vocab,
@@ -117,7 +118,7 @@ __device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh,
     if (lane == 0) {
       e.id[0] = counts ? id : -1;
       e.p[0] = counts ? 1.f : 0.f;
-      if (x != nullptr) e.at[0] = counts ? c * to_f32(x[id]) : 0.f;
+      if (x != nullptr) e.at[0] = counts ? to_f32(x[id]) : 0.f;
       sh.counts = counts;
       sh.p_log_p = 0.f;
     }
@@ -138,7 +139,6 @@ __device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh,
     for (int j = 0; j < 4; ++j) {
       if (id[j] >= vocab) id[j] = -1;
       if (id[j] < 0) y[j] = -INFINITY;  // (padding may hold anything)
-      y[j] *= c;
       if (y[j] == -INFINITY) id[j] = -1;
       at[j] = x != nullptr && id[j] >= 0 ? to_f32(x[id[j]]) : 0.f;
       m = fmaxf(m, y[j] != y[j] ? INFINITY : y[j]);  // a NaN makes the row NaN
@@ -149,14 +149,14 @@ __device__ __forceinline__ void load_entries(const RowEntries& e, RowShared& sh,
       if (k >= src.K) break;
       e.id[k] = id[j];
       e.p[k] = y[j];
-      if (x != nullptr) e.at[k] = c * at[j];
+      if (x != nullptr) e.at[k] = at[j];
     }
   }
   m = warp_max(m);
   const bool counts = m != -INFINITY;
   float s = 0.f, sy = 0.f;
   for (int k = lane; k < src.K; k += 32) {
-    const float y = e.p[k] - m, v = e.id[k] < 0 ? 0.f : ex2(y);
+    const float y = c * (e.p[k] - m), v = e.id[k] < 0 ? 0.f : ex2(y);
     e.p[k] = v;
     s += v;
     if (v != 0.f) sy += v * y;
@@ -208,34 +208,34 @@ __global__ void __launch_bounds__(ROW_THREADS)
   float m = -INFINITY, s = 0.f;
   bool bad = false;
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS) {
-    const float t = c * to_f32(x[j]);
-    bad = bad || t != t;
-    if (t > m) {
-      s = s * ex2(m - t) + 1.f;
-      m = t;
-    } else if (t != -INFINITY) {
-      s += ex2(t - m);
+    const float v = to_f32(x[j]);
+    bad = bad || v != v;
+    if (v > m) {
+      s = s * ex2(c * (m - v)) + 1.f;
+      m = v;
+    } else if (v != -INFINITY) {
+      s += ex2(c * (v - m));
     }
   }
   const float top = cta_reduce(m, true, sh.part);
   const float base = top == -INFINITY ? 0.f : top;
-  s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(m - base)), false, sh.part);
+  s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(c * (m - base))), false, sh.part);
   const float log2_s = log2f(s);
   float cross = 0.f;  // sum_k p_k log2 q_k
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
-    if (e.p[k] != 0.f) cross += e.p[k] * ((e.at[k] - base) - log2_s);
+    if (e.p[k] != 0.f) cross += e.p[k] * (c * (e.at[k] - base) - log2_s);
   cross = cta_reduce(cross, false, sh.part);
   const bool counts = sh.counts;
   if (threadIdx.x == 0) {
     terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
-    if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+    if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * log2_s;
   }
   if (g == nullptr) return;
   T* y = g + row * ld_g;
   const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
   const float over_s = scale / s;
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS)
-    y[j] = from_f32<T>(counts ? ex2(fmaf(to_f32(x[j]), c, -base)) * over_s : 0.f);
+    y[j] = from_f32<T>(counts ? ex2(c * (to_f32(x[j]) - base)) * over_s : 0.f);
   __syncthreads();
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) {
     const int id = e.id[k];
@@ -247,13 +247,13 @@ __global__ void __launch_bounds__(ROW_THREADS)
       again = again || i < k;
       p += e.p[i];
     }
-    if (!again) y[id] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - p));
+    if (!again) y[id] = from_f32<T>(scale * (ex2(c * (e.at[k] - base)) / s - p));
   }
 }
 
 // The same with a row read from and written to HBM once: a cluster of 1 to 8 CTAs per row, whose warps have a slice of it each, at
 // most 32 x VECS vectors of 16 bytes, which stay in registers: the maximum; the exponentials in place of the logits (bf16: as
-// f16 of up to 2^15, see store_tile_rows_exp in gemm.cu; their sum is of the f32 values); and, behind the one barrier at
+// f16, 2^15 at the maximum, see store_tile_rows_exp in gemm.cu; their sum is of the f32 values); and, behind the one barrier at
 // which the slices' parts of the statistics meet, the gradient.  The row's entries are a thread's each, and their softmax
 // meets at the same barrier: where one warp prepared them all, the others waited for it (8192 x 32768 with 64
 // entries 244 us, not 216).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
@@ -310,8 +310,10 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   constexpr bool HALF = sizeof(T) == 2;
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float2 s_part[WARPS];     // (M', S') of the CTA's slices
-  __shared__ float3 s_entries[WARPS];  // of the entries of a warp's threads: max y, sum 2^(y - max), sum 2^(y - max) (y - max)
+  constexpr float OFF = HALF ? 15.f : 0.f;  // the exponentials are 2^(c (z - M) + OFF)
+  __shared__ float2 s_part[WARPS];  // (M, S) of the CTA's slices
+  // Of 32 entries each: their largest teacher's logit y, w = sum 2^(c (y - largest)), the sum of those times c (y - largest).
+  __shared__ float3 s_entries[MAX_ENTRIES / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const long long row = blockIdx.x / ctas;
   const int rank = blockIdx.x - static_cast<int>(row) * ctas;
@@ -343,33 +345,29 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   int* table = reinterpret_cast<int*>(smem + static_cast<size_t>(ENTRY_BYTES) * src.K);
   for (int i = threadIdx.x; i < 1 << slots_log2; i += blockDim.x) table[i] = -1;
   __syncthreads();
-  float at_first = 0.f;  // t at the thread's first entry: its load may take until the exponentials are done
-  {
-    float m = -INFINITY, s = 0.f, sy = 0.f;
-    for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
-      int id = src.ids[row * src.ids_ld + k];
-      float y = src.kind == TARGETS ? 0.f : c * teacher_logit(src, row, k);
-      if (id < 0 || id >= vocab || y == -INFINITY) id = -1, y = -INFINITY;  // (padding may hold anything)
-      else mark_id(table, slots_log2, id);
+  // A warp has 32 entries at a time.
+  float at_first = 0.f;  // the logit at the thread's first one: its load may take until the exponentials are done
+  for (int group = warp; group * 32 < src.K; group += warps) {
+    const int k = group * 32 + lane;
+    int id = -1;
+    float y = -INFINITY;
+    if (k < src.K) {
+      id = src.ids[row * src.ids_ld + k];
+      y = src.kind == TARGETS ? 0.f : teacher_logit(src, row, k);
+    }
+    if (id < 0 || id >= vocab || y == -INFINITY) id = -1, y = -INFINITY;  // (padding may hold anything)
+    else mark_id(table, slots_log2, id);
+    const float at = id < 0 ? 0.f : to_f32(x[id]);
+    const float top = warp_max(y != y ? INFINITY : y);  // (a NaN makes the row NaN)
+    const float d = c * (y - top), v = id < 0 ? 0.f : ex2(d);
+    if (k < src.K) {
       e.id[k] = id;
-      e.p[k] = y;
-      m = fmaxf(m, y != y ? INFINITY : y);  // a NaN makes the row NaN
-      const float at = id < 0 ? 0.f : to_f32(x[id]);
-      if (k == threadIdx.x) at_first = at;
-      else e.at[k] = c * at;
+      e.p[k] = v;
+      if (group != warp) e.at[k] = at;
     }
-    if (warp * 32 < src.K) {
-      m = warp_max(m);
-      for (int k = threadIdx.x; k < src.K; k += blockDim.x) {
-        const float y = e.p[k] - m, v = e.id[k] < 0 ? 0.f : ex2(y);
-        e.p[k] = v;  // over the warp's maximum
-        s += v;
-        if (v != 0.f) sy += v * y;
-      }
-      s = warp_sum(s);
-      sy = warp_sum(sy);
-    }
-    if (lane == 0) s_entries[warp] = make_float3(m, s, sy);
+    if (group == warp) at_first = at;
+    const float w = warp_sum(v), wd = warp_sum(v == 0.f ? 0.f : v * d);
+    if (lane == 0) s_entries[group] = make_float3(top, w, wd);
   }
   if ((v0 == 0 && lead != 0) || first + vocab < n * VEC) {  // vectors of which the row has a part
 #pragma unroll
@@ -392,9 +390,9 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
     for (int i = 0; i < VECS; ++i)
       m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(q[i].x), __uint_as_float(q[i].y)), fmaxf(__uint_as_float(q[i].z), __uint_as_float(q[i].w))));
   }
-  m = c * warp_max(m);
-  const float own = (m == -INFINITY ? 0.f : m) - (HALF ? 15.f : 0.f);  // M'
-  const uint64_t c2 = pack_f2(c, c), from2 = pack_f2(-own, -own);
+  m = warp_max(m);
+  const float own = m == -INFINITY ? 0.f : m;
+  const uint64_t c2 = pack_f2(c, c), from2 = pack_f2(-own, -own), off2 = pack_f2(OFF, OFF);
   uint64_t sum2 = pack_f2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
@@ -405,7 +403,7 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
       float lo, hi;
       if constexpr (HALF) lo = bf16_lo(w[j]), hi = bf16_hi(w[j]);
       else lo = __uint_as_float(w[2 * j]), hi = __uint_as_float(w[2 * j + 1]);
-      unpack_f2(fma_f2(pack_f2(lo, hi), c2, from2), lo, hi);
+      unpack_f2(fma_f2(add_f2(pack_f2(lo, hi), from2), c2, off2), lo, hi);
       lo = ex2(lo);
       hi = ex2(hi);
       sum2 = add_f2(sum2, pack_f2(lo, hi));
@@ -416,8 +414,8 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   float s, s_hi;
   unpack_f2(sum2, s, s_hi);
   s = warp_sum(s + s_hi);
-  if (lane == 0) s_part[warp] = make_float2(m == -INFINITY ? -INFINITY : own, s);
-  if (threadIdx.x < src.K) e.at[threadIdx.x] = c * at_first;
+  if (lane == 0) s_part[warp] = make_float2(m, s);
+  if (threadIdx.x < src.K) e.at[threadIdx.x] = at_first;
   if (ctas > 1) cluster_sync_all();  // (the entries' logits have been read, too: they may be overwritten)
   else __syncthreads();
   auto part = [&](int w) {
@@ -435,43 +433,43 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   for (int i = lane + 32; i < all_warps; i += 32) base = fmaxf(base, part(i).x);
   base = warp_max(base);
   if (base == -INFINITY) base = 0.f;
-  s = mine.y * ex2(mine.x - base);
+  s = mine.y * ex2(c * (mine.x - base));
   for (int i = lane + 32; i < all_warps; i += 32) {
     const float2 v = part(i);
-    s += v.y * ex2(v.x - base);
+    s += v.y * ex2(c * (v.x - base));
   }
   s = warp_sum(s);
   if (ctas > 1) cluster_arrive_relaxed();  // this warp has read its peers' parts
-  // The teacher's softmax: p of an entry is its 2^(y - max of its warp's) times that warp's weight.
-  const int holders = min(warps, (src.K + 31) / 32);
+  // The teacher's softmax: p of an entry is what it has in its group of 32 times the group's weight.
+  const int groups = (src.K + 31) / 32;
   float ent_top = -INFINITY, ent_sum = 0.f;
-  for (int i = 0; i < holders; ++i) ent_top = fmaxf(ent_top, s_entries[i].x);
+  for (int i = 0; i < groups; ++i) ent_top = fmaxf(ent_top, s_entries[i].x);
   const bool counts = ent_top != -INFINITY;
-  for (int i = 0; i < holders; ++i) ent_sum += s_entries[i].y * ex2(s_entries[i].x - ent_top);  // (counts)
+  for (int i = 0; i < groups; ++i) ent_sum += s_entries[i].y * ex2(c * (s_entries[i].x - ent_top));  // (where the row counts)
   const float over = 1.f / ent_sum;
-  auto weight_of = [&](int k) { return ex2(s_entries[(k % blockDim.x) >> 5].x - ent_top) * over; };  // (uniform in a warp's 32 entries)
+  auto weight_of = [&](int k) { return ex2(c * (s_entries[k / 32].x - ent_top)) * over; };
   if (rank == 0 && warp == warps - 1) {
     const float log2_s = log2f(s);
-    // sum_k p_k (log2 p_k - log2 q_k); the first part: sum p (y - max) - log2 of the sum
+    // sum_k p_k (log2 p_k - log2 q_k); the first part: sum p c (y - largest) - log2 of the sum
     float sum = 0.f;
     for (int k = lane; k < src.K; k += 32) {
       const float v = e.p[k];
-      if (v != 0.f) sum -= v * weight_of(k) * ((e.at[k] - base) - log2_s);
+      if (v != 0.f) sum -= v * weight_of(k) * ((c * (e.at[k] - base) + OFF) - log2_s);
     }
-    if (lane < holders && s_entries[lane].y != 0.f) {
+    if (lane < groups && s_entries[lane].y != 0.f) {
       const float3 v = s_entries[lane];
-      sum += ex2(v.x - ent_top) * over * (v.z + v.y * (v.x - ent_top));
+      sum += weight_of(32 * lane) * (v.z + v.y * (c * (v.x - ent_top)));
     }
     sum = warp_sum(sum) - log2f(ent_sum);
     if (lane == 0) {
       terms.loss[row] = counts ? terms.tau * terms.tau * LN2 * sum : 0.f;
-      if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+      if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * (log2_s - OFF);
     }
   }
   if (g != nullptr) {
     T* y = g + row * ld_g;
     const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f;
-    const float factor = ex2(own - base) * (scale / s);
+    const float factor = ex2(c * (own - base)) * (scale / s);
     const bool in_step = static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
     const int at0 = lane * VEC - first;  // the row's element at the lane's first vector
     const uint64_t f2 = pack_f2(factor, factor);
@@ -522,7 +520,7 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
         }
         if (again) continue;
       }
-      y[id] = from_f32<T>(scale * (ex2(e.at[k] - base) / s - p));
+      y[id] = from_f32<T>(scale * (ex2(c * (e.at[k] - base) + OFF) / s - p));
     }
   }
   if (ctas > 1) cluster_wait();  // the peers have read this CTA's parts

@@ -9,6 +9,15 @@ from __future__ import annotations
 import torch
 
 
+def _top(y):
+    """[rows, 1]: what is subtracted before exponentials are taken.  (Logits may be masked with a type's lowest value, beside which
+    even 64 bits have no room for the sum's logarithm.)"""
+    if not y.shape[1]:
+        return torch.zeros(y.shape[0], 1, dtype=y.dtype, device=y.device)
+    top = y.amax(1, keepdim=True)
+    return torch.where(top == -torch.inf, 0.0, top)
+
+
 def entries(ids, teacher, vocab, tau):
     """(p, log p) [rows, K]: 0 where an entry does not count."""
     ids = ids.long()
@@ -16,8 +25,9 @@ def entries(ids, teacher, vocab, tau):
     counts = (ids >= 0) & (ids < vocab)
     y = torch.where(counts, y, -torch.inf)
     counts &= y != -torch.inf
-    total = torch.where(counts.any(1), torch.logsumexp(y, 1) if y.shape[1] else torch.zeros(y.shape[0], dtype=y.dtype, device=y.device), 0.0)
-    log_p = torch.where(counts, y - total[:, None], 0.0)
+    log_p = torch.where(counts, y - _top(y), 0.0)
+    total = torch.where(counts, log_p.exp(), 0.0).sum(1)
+    log_p = torch.where(counts, log_p - torch.where(counts.any(1), total, 1.0).log()[:, None], 0.0)
     return torch.where(counts, log_p.exp(), 0.0), log_p, counts
 
 
@@ -27,14 +37,17 @@ def distillation(z, ids, teacher, tau=1.0, scale=None):
     p, log_p, counts = entries(ids, teacher, vocab, tau)
     some = counts.any(1)
     u = z / tau
-    lse = torch.logsumexp(u, 1)
+    top = _top(u)
+    u = u - top
+    rest = u.exp().sum(1).log()
+    lse = top[:, 0] + rest
     at = u.gather(1, torch.where(counts, ids.long(), 0)) if ids.shape[1] else u[:, :0]
-    loss = tau * tau * torch.where(p > 0, p * (log_p - (at - lse[:, None])), 0.0).sum(1)
+    loss = tau * tau * torch.where(p > 0, p * (log_p - (at - rest[:, None])), 0.0).sum(1)
     loss = torch.where(some, loss, 0.0)
     want = torch.zeros_like(z)
     want.scatter_add_(1, torch.where(counts, ids.long(), 0), p)
     scale = torch.ones(rows, dtype=z.dtype, device=z.device) if scale is None else scale.double()
-    grad = torch.where(some[:, None], (tau * scale)[:, None] * ((u - lse[:, None]).exp() - want), 0.0)
+    grad = torch.where(some[:, None], (tau * scale)[:, None] * ((u - rest[:, None]).exp() - want), 0.0)
     return loss, lse, grad
 
 

@@ -156,6 +156,51 @@ def test_distillation_masked_logits_and_entries(cdl, gpu_ok, dtype, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [100, 5000, 40001, 900001])
+def test_distillation_rows_masked_with_the_lowest_value(cdl, gpu_ok, dtype, vocab):
+    """Masks of the type's lowest (or largest) value, which times log2(e) is no f32: a row of nothing else is a uniform one, and a
+    teacher of nothing else, too."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    _, logits = _logits(gen, 6, vocab, dtype)
+    logits[0] = low
+    logits[1, 50:] = low
+    logits[2] = high
+    logits[3], logits[3, 7] = low, high
+    ids = torch.arange(8, dtype=torch.int32, device="cuda").expand(6, 8).contiguous()
+    teacher = (torch.randn(6, 8, generator=gen, device="cuda") * 2).to(dtype)
+    teacher[4], teacher[5, 3:] = low, low
+    teacher[3], teacher[3, 7] = low, high  # (the student agrees: no loss)
+    o = cdl.ops.distillation(logits, ids, teacher, cdl.ops.DistillationOpts(temperature=0.8))
+    loss, lse, grad = ref.distillation(logits.double(), ids, teacher, 0.8)
+    assert bool((torch.isfinite(o.loss) | (o.loss.double() == loss)).all()) and not bool(torch.isnan(o.d_logits).any())
+    # the statistics as above; logits that large are rounded to 2^-24 of themselves in lse, and their differences are 0 or beyond 2^100
+    e = _stat(vocab) * (8 + torch.log(torch.tensor(float(vocab))))
+    rows = [0, 1, 2, 4, 5]
+    _close("loss", o.loss[rows], loss[rows], torch.full_like(loss[rows], float(e) + 2.0 ** -18))
+    assert abs(o.loss[3].item()) <= 1e-5
+    finite = torch.isfinite(lse.float())
+    _close("lse", o.lse[finite], lse[finite], e.cuda() + 2.0 ** -22 * lse[finite].abs())
+    half = HALF[dtype] + 2.0 ** -10
+    _close("d_logits", o.d_logits, grad, (half + 2 * float(e)) * grad.abs() + 2.0 ** -17 * _hit(ids, vocab) + 1e-9)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab,k", [(300, 5), (1000, 200), (9000, 64), (33000, 100), (50001, 300)])
+def test_distillation_row_by_row(cdl, gpu_ok, dtype, vocab, k):
+    """A row's bits do not depend on how many rows there are (and so on how many CTAs share one)."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    _, logits = _logits(gen, 600, vocab, dtype, pad=(-vocab) % 8)
+    ids, teacher = _teacher(gen, 600, vocab, k, dtype)
+    o = cdl.ops.distillation(logits, ids, teacher, cdl.ops.DistillationOpts(temperature=1.3))
+    for rows in (slice(0, 1), slice(2, 5), slice(100, 140)):
+        p = cdl.ops.distillation(logits[rows], ids[rows], teacher[rows], cdl.ops.DistillationOpts(temperature=1.3))
+        assert torch.equal(p.loss, o.loss[rows]) and torch.equal(p.lse, o.lse[rows]) and torch.equal(p.d_logits, o.d_logits[rows])
+
+
+@gpu
 def test_distillation_no_entries_no_rows(cdl, gpu_ok):
     logits = torch.randn(3, 100, device="cuda")
     none = torch.empty(3, 0, dtype=torch.int32, device="cuda")
