@@ -23,6 +23,7 @@ namespace head {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int MAX_ENTRIES = 1024;  // of a teacher, per row: they are kept in shared memory
+constexpr long long MAX_DIM = 1LL << 30;  // of vocabulary and hidden size: indices a few thousand further on are ints, too
 constexpr int ROW_THREADS = 512;
 
 static long long up(long long v, long long m) { return (v + m - 1) / m * m; }
@@ -257,13 +258,12 @@ __global__ void __launch_bounds__(ROW_THREADS)
 // which the slices' parts of the statistics meet, the gradient.  The row's entries are a thread's each, and their softmax
 // meets at the same barrier: where one warp prepared them all, the others waited for it (8192 x 32768 with 64
 // entries 244 us, not 216).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
-// whose share of the HBM's rate takes 5500.  The slices depend on the vocabulary alone, not on how many CTAs share a row, so
-// a row's results do not depend on the number of rows.
+// whose share of the HBM's rate takes 5500.  The slices depend on the vocabulary and on whether rows are on the 16-byte
+// grid, not on how many CTAs share a row, so a row's results do not depend on the number of rows.
 //
 // A vector that starts before the row or ends behind it is read whole where it holds an element of the row (the same 16
 // bytes of memory); what is not the row's counts as -inf and is never written.
 constexpr int WARPS = 16;              // of a CTA, at most
-constexpr int MAX_ROW_WARPS = 8 * WARPS;
 
 // Elements of a vector outside [lo, hi) become -inf.
 template <typename T>
@@ -979,7 +979,8 @@ static bool is_float(int32_t t) { return t == CDL_BF16 || t == CDL_F32; }
 
 static int32_t check_desc(const char* op, const cdl_head_loss_desc* d) {
   if (!d) return fail(CDL_ERR_INVALID, "%s: desc is required", op);
-  if (!(d->temperature > 0.f) || isinf(d->temperature)) return fail(CDL_ERR_INVALID, "%s: temperature must be positive and finite", op);
+  if (!(d->temperature >= 1e-6f && d->temperature <= 1e6f))  // (its square and log2(e) over it are factors)
+    return fail(CDL_ERR_INVALID, "%s: temperature must be positive, from 1e-6 to 1e6", op);
   if (d->chunk_rows < 0) return fail(CDL_ERR_INVALID, "%s: chunk_rows must not be negative", op);
   return CDL_OK;
 }
@@ -1032,7 +1033,7 @@ static int32_t distillation_execute(const cdl_head_loss_desc* desc, const cdl_te
     return fail(CDL_ERR_INVALID, "%s: logits must be bf16 or f32 [tokens, vocab]", op);
   const long long T = logits->shape[0], V = logits->shape[1];
   if (V > 1 && logits->stride[1] != 1) return fail(CDL_ERR_INVALID, "%s: logits must have contiguous rows", op);
-  if (T > INT32_MAX || V > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  if (T > INT32_MAX || V > MAX_DIM) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
   RowTerms terms;
   Entries e;
   CDL_CHECK(check_teacher(op, T, ids, teacher, &e));
@@ -1100,7 +1101,7 @@ constexpr long long TARGET_ENTRIES = -1;
 // Rows that are taken at a time: their exponentials (f32: logits and the pieces of their gradients) are what the scratch holds,
 // up to 1 GB.  16384 x 2048 x 32768 in one go 5.21 ms, in two 5.44: dw is summed in memory then, dx's last wave is emptier.
 static long long choose_chunk(long long T, long long V, long long bytes_per_logit) {
-  long long rows = (1LL << 30) / (bytes_per_logit * V);
+  long long rows = (1LL << 30) / (bytes_per_logit * up(V, 128));
   if (rows < 256) rows = 256;
   if (rows >= T) return T;
   const long long chunks = (T + rows - 1) / rows;
@@ -1185,7 +1186,7 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
   p.has_dw = dw != nullptr;
   if (w->shape[0] != p.D)
     return fail(CDL_ERR_INVALID, "%s: x is [tokens, %lld], w is [%lld, vocab]: the hidden sizes differ", op, p.D, (long long)w->shape[0]);
-  if (p.T > INT32_MAX || p.D > INT32_MAX || p.V > 65535LL * 8 * 128) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  if (p.T > INT32_MAX || p.D > MAX_DIM || p.V > 65535LL * 8 * 128) return fail(CDL_ERR_UNSUPPORTED, "%s: dimension too large", op);
   if (dx) {
     if (dx->rank != 2 || dx->dtype != x->dtype || dx->shape[0] != p.T || dx->shape[1] != p.D || (p.D > 1 && dx->stride[1] != 1) ||
         (p.T > 1 && dx->stride[0] < p.D))

@@ -511,9 +511,10 @@ int32_t cdl_b200_adamw(float* master, void* replica_bf16, float* grad, float* m,
  *
  * Operands: targets packed i32 [tokens]; teacher_ids i32 and teacher_logits bf16 or f32 [tokens, entries], contiguous
  * rows, at most 1024 entries; d_loss f32 [tokens] of any stride, 0 too (nullable: 1); loss and lse (nullable) packed f32
- * [tokens]. */
+ * [tokens].  vocab up to 2^30 (linear losses: 67107840).  Outputs overlap neither inputs nor one another, but where it says so
+ * below. */
 typedef struct {
-  float temperature; /* > 0; 1 for the cross entropy */
+  float temperature; /* 1e-6 to 1e6; 1 for the cross entropy */
   float grad_scale;  /* of every gradient, e.g. 1 / tokens of the step */
   int32_t accumulate_dw; /* != 0: dw is added to, else written */
   int64_t chunk_rows;    /* tokens whose rows the scratch holds at a time; 0 = the library's choice */
@@ -531,8 +532,9 @@ int32_t cdl_b200_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* 
  *   dw  (nullable) f32 or x's type [hidden, vocab], any strides:  x^T . d z, added to with accumulate_dw.  Held in f32 over
  *       all tokens and rounded once.
  * For bf16 operands d z is rounded to bf16 before both products, as cdl_b200_cross_entropy rounds it: an f32 dw has that
- * accuracy then.  (Up to 64 tokens, where it costs no time, it goes into them as two bf16 values.)  f32 operands keep 24 bits of it.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that
- * the call below gives for the same operands (entries: teacher_ids' second dimension, 1 for targets). */
+ * accuracy then.  (Up to 64 tokens, where it costs no time, it goes into them as two bf16 values.)  f32 operands keep 24
+ * bits of it.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that the call below gives for the same
+ * operands (entries: teacher_ids' second dimension, 1 for targets); calls that may run at the same time have one each. */
 int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
                                       const cdl_tensor* targets, const cdl_tensor* d_loss, const cdl_tensor* loss,
                                       const cdl_tensor* lse, const cdl_tensor* dx, const cdl_tensor* dw, void* scratch,

@@ -668,6 +668,8 @@ def test_linear_refusals(cdl):
             ({"teacher": _t(L, (8, 4), dtype=i32)}, "teacher_logits must be"), ({"teacher": _t(L, (9, 4))}, "teacher_logits must be"),
             ({"ids": _t(L, (8, 1025), dtype=i32), "teacher": _t(L, (8, 1025))}, "at most 1024"), ({}, "scratch must hold")]:
         assert _linear_status(L, distil=True, **other) < 0 and said in L.last_error(), (other, L.last_error())
+    for tau in (0.0, -1.0, 1e-7, 2e6, float("inf"), float("nan")):
+        assert _linear_status(L, distil=True, temperature=tau) < 0 and "temperature must be positive" in L.last_error()
     n = ctypes.c_size_t(0)
     x = _t(L, (8, 16))
     desc = L.CdlHeadLossDesc(1.0, 1.0, 0, 0)
@@ -685,7 +687,8 @@ def test_distillation_refusals(cdl):
             ({"logits": _t(L, (8, 40), (1, 8))}, "contiguous rows"), ({"logits": _t(L, (8, 0)), "d_logits": None}, "vocab is zero"),
             ({"d_logits": _t(L, (8, 40), dtype=L.CDL_F32)}, "d_logits must"), ({"d_logits": _t(L, (8, 40), (20, 1))}, "overlap"),
             ({"d_logits": _t(L, (8, 40), (48, 1))}, "themselves"), ({"ids": _t(L, (7, 4), dtype=L.CDL_I32)}, "teacher_ids must"),
-            ({"loss": None}, "loss is required"), ({"lse": _t(L, (8,))}, "lse must be")]:
+            ({"loss": None}, "loss is required"), ({"lse": _t(L, (8,))}, "lse must be"),
+            ({"logits": _t(L, (8, (1 << 30) + 1)), "d_logits": None}, "too large")]:
         a = {**base, **other}
         desc = L.CdlHeadLossDesc(1.0, 1.0, 0, 0)
         st = L.lib.cdl_b200_distillation(ctypes.byref(desc), *(None if a[n] is None else ctypes.byref(a[n]) for n in (
@@ -702,6 +705,8 @@ def test_front_ends_refuse_host_tensors_and_missing_gradients(cdl):
             call()
     assert cdl.ops.linear_loss_scratch_bytes(x, w) > 0
     wider = cdl.ops.linear_loss_scratch_bytes(torch.zeros(100000, 8), torch.zeros(8, 32768), cdl.ops.LinearLossOpts())
+    thin = cdl.ops.linear_loss_scratch_bytes(torch.zeros(1, 1).expand(1 << 26, 8), torch.zeros(8, 3))
+    assert thin < 1.2e9, "a small vocabulary is padded to 128"
     assert wider < 100000 * 32768, "the scratch does not grow with the tokens"
 
 
