@@ -803,11 +803,11 @@ __global__ void __launch_bounds__(256)
 }
 // The same by vectors of four, where the rows of out and of the planes allow them: a thread has one.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
     sum_vectors_kernel(const float* planes, long long ld, long long plane, int slices, T* out, long long o_row, long long all, int cols, int add) {
   grid_dep_wait();
   grid_dep_launch();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long i = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
   if (i >= all) return;
   const int per_row = cols / 4;
   const long long r = i / per_row;
@@ -815,7 +815,7 @@ __global__ void __launch_bounds__(256)
   const float* from = planes + r * ld + c;
   T* o = out + r * o_row + c;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 18
   for (int s = 0; s < slices; ++s) {
     const float4 x = *reinterpret_cast<const float4*>(from + s * plane);
     v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
@@ -951,8 +951,8 @@ static int32_t sum_planes_as(const void* planes, long long ld, long long plane, 
                        reinterpret_cast<uintptr_t>(out.ptr) % (4 * sizeof(T)) == 0 && (rows == 1 || out.stride[0] % 4 == 0);
   if constexpr (sizeof(S) == 4) {
     const long long all = rows * (cols / 4);
-    if (vectors && (all + 255) / 256 <= INT32_MAX) {
-      CDL_CUDA(launch_pdl(sum_vectors_kernel<T>, dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream,
+    if (vectors && (all + 127) / 128 <= INT32_MAX) {
+      CDL_CUDA(launch_pdl(sum_vectors_kernel<T>, dim3(static_cast<unsigned>((all + 127) / 128)), dim3(128), 0, stream,
                           static_cast<const float*>(planes), ld, plane, slices, static_cast<T*>(out.ptr),
                           static_cast<long long>(out.stride[0]), all, static_cast<int>(cols), add));
       return CDL_OK;
