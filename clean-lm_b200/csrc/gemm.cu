@@ -682,6 +682,53 @@ constexpr int PIECE_PRODUCTS = 6;
 __device__ __forceinline__ int piece_of_a(int i) { return 0x210100 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
 __device__ __forceinline__ int piece_of_b(int i) { return 0x012010 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
 
+// An accumulator takes PART K blocks of all products; the parts of a slice are added by the epilogue, in registers, rounded to
+// nearest. A tensor-core accumulator truncates, and a large term that comes early (a target's column in dx) loses a bit in every step
+// after it: with 1800 of K in one accumulator dx of 159 x 576 x 43584 was 1.3e-6 off.
+constexpr int PART = 4;
+template <int KIND>
+__device__ __forceinline__ int part_end(int from, int kb1) { return KIND == STORE_PIECES ? min(from + PART, kb1) : kb1; }
+template <int KIND>
+__device__ __forceinline__ int num_parts(int kb0, int kb1) { return KIND == STORE_PIECES ? (kb1 - kb0 + PART - 1) / PART : 1; }
+
+// 128 columns of a warp's rows, sum += accumulator.
+__device__ __forceinline__ void add_part(float (&sum)[8][16], uint32_t t_row) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t r[16];
+    tmem_ld16(t_row + 16 * c, r);
+    tmem_wait_ld(r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[c][j] += __uint_as_float(r[j]);
+  }
+}
+__device__ __forceinline__ void put_parts(const float (&sum)[8][16], uint32_t t_row) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t r[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(sum[c][j]);
+    tmem_st16(t_row + 16 * c, r);
+  }
+  tmem_wait_st();
+}
+
+// The sum of a slice's parts in place of the last one's accumulator, which is number `a`, counted on, then: `full` waits for an
+// accumulator, `give` hands it back.
+template <typename Full, typename Give>
+__device__ __forceinline__ bool sum_parts(int parts, int& a, uint32_t t_row, Full full, Give give) {
+  if (parts == 1) return full(a);
+  float sum[8][16] = {};
+  for (int part = 0;; ++part, ++a) {
+    if (!full(a)) return false;
+    add_part(sum, t_row + (a & 1) * BN);
+    if (part == parts - 1) break;
+    give(a);
+  }
+  put_parts(sum, t_row + (a & 1) * BN);
+  return true;
+}
+
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
@@ -749,8 +796,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         unit_range(unit, tile, slice, kb0, kb1);
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * BM, n0 = tn * BN;
+        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(from, kb1))
         for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int kb = from; kb < part_end<KIND>(from, kb1); ++kb, ++it) {
           const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
@@ -788,34 +836,40 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t it = 0;
       int t = 0;
       bool ok = true;
-      for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x, ++t) {
+      for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x) {
         int tile, slice, kb0, kb1;
         unit_range(unit, tile, slice, kb0, kb1);
-        const int acc = t & 1;
-        const uint32_t acc_ph = (t >> 1) & 1;
-        if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 201)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        const int blocks = (kb1 - kb0) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1);
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const int s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait(&bars->full[s], ph, abort_word, 202)) {
+        for (int part = 0; part < num_parts<KIND>(kb0, kb1) && ok; ++part, ++t) {
+          const int acc = t & 1;
+          const uint32_t acc_ph = (t >> 1) & 1;
+          if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 201)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
-          const uint32_t sb = sa + A_BYTES;
+          const uint32_t d_tmem = tmem_base + acc * BN;
+          const int from = kb0 + part * PART;
+          const int blocks = KIND == STORE_PIECES ? (part_end<KIND>(from, kb1) - from) * PIECE_PRODUCTS : kb1 - kb0;
+          for (int kb = 0; kb < blocks; ++kb, ++it) {
+            const int s = it % STAGES;
+            const uint32_t ph = (it / STAGES) & 1;
+            if (!mbar_wait(&bars->full[s], ph, abort_word, 202)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
+            const uint32_t sb = sa + A_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
-            const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
-            umma_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
+              const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
+              umma_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            }
+            umma_commit(&bars->empty[s]);
           }
-          umma_commit(&bars->empty[s]);
+          if (ok) umma_commit(&bars->acc_full[acc]);
         }
-        if (ok) umma_commit(&bars->acc_full[acc]);
       }
     }
   } else {
@@ -827,13 +881,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       int tile, slice, kb0, kb1, b, tm, tn;
       unit_range(unit, tile, slice, kb0, kb1);
       tile_coords(p, tile, b, tm, tn);
-      const int acc = t & 1;
-      const uint32_t acc_ph = (t >> 1) & 1;
       Wanted want;
       if (KIND == STORE_EXP) want.load(p, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
-      if (!mbar_wait(&bars->acc_full[acc], acc_ph, abort_word, 301)) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
+      const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
+      auto full = [&](int n) {
+        if (!mbar_wait(&bars->acc_full[n & 1], (n >> 1) & 1, abort_word, 301)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto give = [&](int n) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[n & 1]);
+      };
+      if (!(KIND == STORE_PIECES ? sum_parts(num_parts<KIND>(kb0, kb1), t, t_lane, full, give) : full(t))) break;
+      const uint32_t t_row = t_lane + (t & 1) * BN;
       const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
       if constexpr (KIND == STORE_EXP) {
         store_tile_rows_exp<false>(p, nullptr, nullptr, t_row, row, col, lane, want);
@@ -843,9 +905,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
         else store_tile_rows(p, t_row, b, row, col);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
+      give(t);
     }
   }
 
@@ -1027,8 +1087,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * PAIR_M + static_cast<int>(rank) * BM;
         const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
+        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(from, kb1))
         for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int kb = from; kb < part_end<KIND>(from, kb1); ++kb, ++it) {
           const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % PAIR_STAGES;
           const uint32_t ph = (it / PAIR_STAGES) & 1;
@@ -1066,7 +1127,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const uint32_t a_lbo = p.a_mn ? 8192u : 16u, b_lbo = p.b_mn ? 8192u : 16u;
       const uint32_t a_kstep = p.a_mn ? 2048u : 32u, b_kstep = p.b_mn ? 2048u : 32u;
       uint32_t it = 0;
-      int t = 0;
+      int t = 0, a = 0;  // units, accumulators
       bool ok = true;
       for (; ok; ++t) {
         const int slot = t % SCHED_SLOTS;
@@ -1076,36 +1137,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int unit = static_cast<int>(unit_u);
         int tile, slice, kb0, kb1;
         unit_range(unit, tile, slice, kb0, kb1);
-        const int acc = t & 1;
-        const uint32_t acc_ph = (t >> 1) & 1;
-        if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 211)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        const int blocks = (kb1 - kb0) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1);
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const int s = it % PAIR_STAGES;
-          const uint32_t ph = (it / PAIR_STAGES) & 1;
-          if (!mbar_wait(&bars->full[s], ph, abort_word, 212)) {
+        for (int part = 0; part < num_parts<KIND>(kb0, kb1) && ok; ++part, ++a) {
+          const int acc = a & 1;
+          const uint32_t acc_ph = (a >> 1) & 1;
+          if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 211)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * PAIR_STAGE_BYTES);
-          const uint32_t sb = sa + A_BYTES;
+          const uint32_t d_tmem = tmem_base + acc * BN;
+          const int from = kb0 + part * PART;
+          const int blocks = KIND == STORE_PIECES ? (part_end<KIND>(from, kb1) - from) * PIECE_PRODUCTS : kb1 - kb0;
+          for (int kb = 0; kb < blocks; ++kb, ++it) {
+            const int s = it % PAIR_STAGES;
+            const uint32_t ph = (it / PAIR_STAGES) & 1;
+            if (!mbar_wait(&bars->full[s], ph, abort_word, 212)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * PAIR_STAGE_BYTES);
+            const uint32_t sb = sa + A_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
-            const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
-            umma_ss_pair(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              const uint64_t da = smem_desc_sw128(sa + k * a_kstep, a_lbo, 1024);
+              const uint64_t db = smem_desc_sw128(sb + k * b_kstep, b_lbo, 1024);
+              umma_ss_pair(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            }
+            const uint32_t e = smem_u32(&bars->empty[s]);
+            umma_commit_pair(e);                  // own producer
+            umma_commit_pair(mapa_shared(e, 1));  // the peer's producer
           }
-          const uint32_t e = smem_u32(&bars->empty[s]);
-          umma_commit_pair(e);                  // own producer
-          umma_commit_pair(mapa_shared(e, 1));  // the peer's producer
-        }
-        if (ok) {
-          const uint32_t f = smem_u32(&bars->acc_full[acc]);
-          umma_commit_pair(f);
-          umma_commit_pair(mapa_shared(f, 1));
+          if (ok) {
+            const uint32_t f = smem_u32(&bars->acc_full[acc]);
+            umma_commit_pair(f);
+            umma_commit_pair(mapa_shared(f, 1));
+          }
         }
       }
     }
@@ -1116,8 +1183,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t* buf = staging + (warp - 2) * CHUNK_BYTES;
     SwigluFeed feed{&tmap_e0, &tmap_e1, buf, &bars->extra_full[warp - 2], p.epi_mode == 2, 0};
     if (p.early == 2) grid_dep_wait();
-    int t = 0;
-    for (;; ++t) {
+    int t = 0, a = 0;  // units, accumulators
+    for (;; ++t, ++a) {
       const int slot = t % SCHED_SLOTS;
       if (!mbar_wait(&bars->sched_full[slot], (t / SCHED_SLOTS) & 1, abort_word, 312)) break;
       const uint32_t unit_u = bars->unit_ring[slot];
@@ -1126,16 +1193,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int tile, slice, kb0, kb1, b, tm, tn;
       unit_range(unit, tile, slice, kb0, kb1);
       tile_coords(p, tile, b, tm, tn);
-      const int acc = t & 1;
-      const uint32_t acc_ph = (t >> 1) & 1;
       const int row = tm * PAIR_M + static_cast<int>(rank) * BM + quad * 32 + lane;
       const int col = tn * BN + half * (BN / 2);
       if (KIND == STORE_SWIGLU && row - lane < p.M && col < p.N) feed.load(lane, row - lane, col);  // under the products
       Wanted want;
       if (KIND == STORE_EXP) want.load(p, row, col);
-      if (!mbar_wait(&bars->acc_full[acc], acc_ph, abort_word, 311)) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
+      const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
+      auto full = [&](int n) {
+        if (!mbar_wait(&bars->acc_full[n & 1], (n >> 1) & 1, abort_word, 311)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto give = [&](int n) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[n & 1]), 0));
+      };
+      if (!(KIND == STORE_PIECES ? sum_parts(num_parts<KIND>(kb0, kb1), a, t_lane, full, give) : full(a))) break;
+      const uint32_t t_row = t_lane + (a & 1) * BN;
       if constexpr (KIND == STORE_ADD) {
         add_tile_rows(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
       } else if constexpr (KIND == STORE_SWIGLU) {
@@ -1151,9 +1226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
         else store_tile_rows(p, t_row, b, row, col);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[acc]), 0));
+      give(a);
     }
     if ((KIND == STORE_ADD || KIND == STORE_BF16 || KIND == STORE_EXP) && lane == 0) tma_store_wait<0>();
   }
@@ -1801,12 +1874,11 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
 int matmul_plane_slices(long long M, long long N, long long K, bool pieces) {
   using namespace gemm;
   const bool pair = M > BM;
-  const int least_slices = pieces ? static_cast<int>((K + PIECES_K - 1) / PIECES_K) : 1;
   const long long tiles = (pair ? (M + PAIR_M - 1) / PAIR_M : 1) * ((N + BN - 1) / BN), k_blocks = (K + BK - 1) / BK;
   const long long slots = pair ? sm_count() / 2 : sm_count();
-  int best = least_slices;
+  int best = 1;
   double least = 1e30;
-  for (int s = least_slices; s == least_slices || (s <= MAX_PLANES && s * (pieces ? 2 : 8) <= k_blocks); ++s) {
+  for (int s = 1; s == 1 || (s <= MAX_PLANES && s * (pieces ? 2 : 8) <= k_blocks); ++s) {
     const double waves = static_cast<double>((tiles * s + slots - 1) / slots);
     double t = waves * (0.28 * (pieces ? PIECE_PRODUCTS : 1) * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
     if (s > 1) t = 1.05 * (t + 3.0 + 8e-6 * static_cast<double>(s) * M * N / 5.0);
@@ -1832,8 +1904,8 @@ int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* p
 }
 
 // A product of f32 operands that lie in three bf16 pieces each, [3][M][K] and [3][K][N], the six largest products of pieces
-// summed.  One slice: D = product (+ D) itself; more: planes.  An accumulator takes at most PIECES_K of K, and what truncation
-// takes from it is put back (see matmul_exp_execute): what is left is below the rounding of f32 sums of that length.
+// summed.  One slice: D = product (+ D) itself; more: planes.  What truncation takes from a part's accumulator is put back (see
+// matmul_exp_execute and PART).
 int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d, long long ldd, int slices, int add, cudaStream_t stream) {
   gemm::Params p;
   CUtensorMap tm_a, tm_b;
@@ -1852,7 +1924,7 @@ int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d
     p.c_vec = p.d_vec;
     p.beta = 1.f;
   }
-  p.alpha = static_cast<float>(1.0 + 1e-9 * p.K / slices);
+  p.alpha = static_cast<float>(1.0 + 1e-9 * (p.k_blocks / slices < gemm::PART ? p.K / slices : gemm::PART * gemm::BK));
   p.split_k = slices;
   return pair ? pair_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, stream);
 }

@@ -58,9 +58,8 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
                            cudaStream_t stream);
 // A product of bf16 tensors on the 16-byte grid in K slices: slice s is stored at planes + s M ld (f32, 32-byte aligned, ld >= N a
 // multiple of 8).  matmul_plane_slices: how many pay; 1: none do.
-// pieces: of a product of f32 operands in three bf16 pieces each (rank 3, [3][M][K] and [3][K][N]), with at most PIECES_K of
-// K per slice; matmul_pieces_execute stores one slice at d (added to what is there with `add`), several in planes from d on.
-constexpr int MAX_PLANES = 24, PIECES_K = 4096;
+// pieces: of a product of f32 operands in three bf16 pieces each (rank 3, [3][M][K] and [3][K][N]); matmul_pieces_execute stores one slice at d (added to what is there with `add`), several in planes from d on.
+constexpr int MAX_PLANES = 24;
 int matmul_plane_slices(long long M, long long N, long long K, bool pieces = false);
 int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d, long long ldd, int slices, int add, cudaStream_t stream);
 int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream);

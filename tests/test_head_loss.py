@@ -355,6 +355,22 @@ def test_linear_losses_of_f32_operands(cdl, gpu_ok, layout, t, d, v, chunk):
 
 
 @gpu
+@pytest.mark.parametrize("t", [40, 159])
+def test_f32_gradient_whose_largest_term_comes_first(cdl, gpu_ok, t):
+    """d x is the target's column and what tens of thousands of small terms add to it. A tensor-core accumulator drops up to a bit of
+    the last place (2^-24) in each of its steps of 16; one takes 256 of K, so 16 steps lie behind the target's. The six products of pieces
+    leave out three below 2^-24 each; the sums of 171 parts are rounded to nearest, 2^-25 times their square root as they are independent: 7
+    of 2^-24. In all 26 2^-24 of the 2-norm."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(t, 576, generator=gen, device="cuda")
+    w = torch.randn(576, 43584, generator=gen, device="cuda") * 0.02
+    targets = torch.zeros(t, dtype=torch.int32, device="cuda")
+    o = cdl.ops.linear_cross_entropy(x, w, targets)
+    _, _, _, dx, _ = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
+    assert ((o.dx - dx).norm() / dx.norm()).item() <= 26 * 2.0 ** -24
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("tied", [False, True])
 @pytest.mark.parametrize("chunk", [0, 128])
