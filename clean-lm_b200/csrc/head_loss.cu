@@ -735,7 +735,8 @@ struct Segment {
 
 // dst[r, c] = src[r, c].
 template <typename T>
-__global__ void __launch_bounds__(256) copy_kernel(const T* src, long long s_row, long long s_col, T* dst, long long ld, int cols) {
+__global__ void __launch_bounds__(256) copy_kernel(const T* src, long long s_row, long long s_col, T* dst, long long d_row, long long d_col,
+                                                          int cols) {
   grid_dep_wait();
   grid_dep_launch();
   const Segment at(cols);
@@ -746,7 +747,56 @@ __global__ void __launch_bounds__(256) copy_kernel(const T* src, long long s_row
     if (at.col + 256 * j < cols) v[j] = from[(at.col + 256 * j) * s_col];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (at.col + 256 * j < cols) dst[at.row * ld + at.col + 256 * j] = v[j];
+    if (at.col + 256 * j < cols) dst[at.row * d_row + (at.col + 256 * j) * d_col] = v[j];
+}
+
+// The same for rows of neighbouring elements, from and to any alignment: a thread has 16 aligned bytes of dst at a time, out
+// of the two aligned 16 bytes of src that hold them (both hold an element of the row); what a row has of its first and last 16 bytes
+// goes one by one. 190 MB of bf16 rows of 85695 there and back: 130 us, element by element 330.
+constexpr int COPY_VECS = 4;  // of a thread, 256 apart
+__global__ void __launch_bounds__(256)
+    copy_rows_kernel(const __nv_bfloat16* src, long long s_row, __nv_bfloat16* dst, long long d_row, int cols, unsigned per_row, long long all) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const long long first = static_cast<long long>(blockIdx.x) * (256 * COPY_VECS) + threadIdx.x;
+  const long long row0 = first / per_row;  // the thread's next vectors lie a few rows further on at most
+  const unsigned in_row0 = static_cast<unsigned>(first - row0 * per_row);
+  uint4 lo[COPY_VECS], hi[COPY_VECS];
+  int at[COPY_VECS];  // the row's element that the vector begins with, INT_MIN: none
+  unsigned shift[COPY_VECS];
+#pragma unroll
+  for (int j = 0; j < COPY_VECS; ++j) {
+    at[j] = INT32_MIN;
+    if (first + 256 * j >= all) continue;
+    const unsigned on = (in_row0 + 256 * j) / per_row;
+    const __nv_bfloat16* to = dst + (row0 + on) * d_row;
+    at[j] = static_cast<int>(in_row0 + 256 * j - on * per_row) * 8 - static_cast<int>((reinterpret_cast<uintptr_t>(to) & 15) / 2);
+    if (at[j] < 0 || at[j] + 8 > cols) continue;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(src + (row0 + on) * s_row + at[j]);
+    shift[j] = from & 15;
+    lo[j] = *reinterpret_cast<const uint4*>(from - shift[j]);
+    if (shift[j] != 0) hi[j] = *reinterpret_cast<const uint4*>(from - shift[j] + 16);
+  }
+#pragma unroll
+  for (int j = 0; j < COPY_VECS; ++j) {
+    if (at[j] == INT32_MIN || at[j] >= cols) continue;
+    const long long row = row0 + (in_row0 + 256 * j) / per_row;
+    __nv_bfloat16* to = dst + row * d_row + at[j];
+    if (at[j] < 0 || at[j] + 8 > cols) {
+      const __nv_bfloat16* from = src + row * s_row + at[j];
+      for (int i = 0; i < 8; ++i)
+        if (at[j] + i >= 0 && at[j] + i < cols) to[i] = from[i];
+      continue;
+    }
+    uint32_t w[8] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w, hi[j].x, hi[j].y, hi[j].z, hi[j].w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = shift[j] & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = shift[j] & 4 ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = shift[j] & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // The three bf16 pieces of f32 values, v = p0 + p1 + p2 to 24 bits: the first two cut off (no finite value becomes infinite),
@@ -777,21 +827,21 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// out[r, c] = the sum of the planes at r, c in their order (+ out[r, c]).  One plane: the end of a gradient that scratch held.
+// out[r, c] = the sum of the f32 planes at r, c in their order (+ out[r, c]).  One plane: the end of a gradient that scratch held.
 // No plane: zeros.
-template <typename S, typename T>
+template <typename T>
 __global__ void __launch_bounds__(256)
-    sum_planes_kernel(const S* planes, long long ld, long long plane, int slices, T* out, long long o_row, long long o_col, int cols, int add) {
+    sum_planes_kernel(const float* planes, long long ld, long long plane, int slices, T* out, long long o_row, long long o_col, int cols, int add) {
   grid_dep_wait();
   grid_dep_launch();
   const Segment at(cols);
-  const S* from = planes + at.row * ld + at.col;
+  const float* from = planes + at.row * ld + at.col;
   T* o = out + at.row * o_row + at.col * o_col;
   float v[8] = {};
   for (int s = 0; s < slices; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (at.col + 256 * j < cols) v[j] += to_f32(from[s * plane + 256 * j]);
+      if (at.col + 256 * j < cols) v[j] += from[s * plane + 256 * j];
   if (add) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -923,14 +973,25 @@ static int32_t segments(long long rows, long long cols, dim3* grid) {
   return CDL_OK;
 }
 
-// dst [rows, cols] (ld) = src, of which the threads' direction is dimension 1.
-static int32_t copy(const cdl_tensor& src, void* dst, long long ld, cudaStream_t stream) {
+// dst = src, of which dimension 1 is the nearer one in memory; bf16.
+static int32_t copy(const cdl_tensor& src, const cdl_tensor& dst, cudaStream_t stream) {
   using bf = __nv_bfloat16;
+  const long long rows = src.shape[0], cols = src.shape[1];
+  ProfileScope ps(PROF_ELEMENTWISE, 4.0 * rows * cols, stream);
+  if ((src.stride[1] == 1 || cols == 1) && (dst.stride[1] == 1 || cols == 1)) {
+    const bool on_grid = (reinterpret_cast<uintptr_t>(dst.ptr) & 15) == 0 && (rows == 1 || dst.stride[0] % 8 == 0);
+    const long long per_row = (cols + (on_grid ? 7 : 14)) / 8, all = rows * per_row, blocks = (all + 256 * COPY_VECS - 1) / (256 * COPY_VECS);
+    if (blocks > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "linear loss: operand too large to be copied");
+    CDL_CUDA(launch_pdl(copy_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<const bf*>(src.ptr),
+                        static_cast<long long>(src.stride[0]), static_cast<bf*>(dst.ptr), static_cast<long long>(dst.stride[0]),
+                        static_cast<int>(cols), static_cast<unsigned>(per_row), all));
+    return CDL_OK;
+  }
   dim3 grid;
-  CDL_CHECK(segments(src.shape[0], src.shape[1], &grid));
-  ProfileScope ps(PROF_ELEMENTWISE, 4.0 * src.shape[0] * src.shape[1], stream);
+  CDL_CHECK(segments(rows, cols, &grid));
   CDL_CUDA(launch_pdl(copy_kernel<bf>, grid, dim3(256), 0, stream, static_cast<const bf*>(src.ptr), static_cast<long long>(src.stride[0]),
-                      static_cast<long long>(src.stride[1]), static_cast<bf*>(dst), ld, static_cast<int>(src.shape[1])));
+                      static_cast<long long>(src.stride[1]), static_cast<bf*>(dst.ptr), static_cast<long long>(dst.stride[0]),
+                      static_cast<long long>(dst.stride[1]), static_cast<int>(cols)));
   return CDL_OK;
 }
 
@@ -943,35 +1004,29 @@ static int32_t split(const cdl_tensor& src, void* dst, long long ld, long long p
   return CDL_OK;
 }
 
-// out (dimension 1 the threads' direction) = the sum of f32 planes, or of one bf16 one.
-template <typename S, typename T>
+// out (dimension 1 the threads' direction) = the sum of f32 planes.
+template <typename T>
 static int32_t sum_planes_as(const void* planes, long long ld, long long plane, int slices, const cdl_tensor& out, int add, cudaStream_t stream) {
-  const long long rows = out.shape[0], cols = out.shape[1];
-  const bool vectors = sizeof(S) == 4 && slices > 0 && cols % 4 == 0 && out.stride[1] == 1 && ld % 4 == 0 && plane % 4 == 0 &&
+  const long long rows = out.shape[0], cols = out.shape[1], all = rows * (cols / 4);
+  const bool vectors = slices > 0 && cols % 4 == 0 && out.stride[1] == 1 && ld % 4 == 0 && plane % 4 == 0 &&
                        reinterpret_cast<uintptr_t>(out.ptr) % (4 * sizeof(T)) == 0 && (rows == 1 || out.stride[0] % 4 == 0);
-  if constexpr (sizeof(S) == 4) {
-    const long long all = rows * (cols / 4);
-    if (vectors && (all + 127) / 128 <= INT32_MAX) {
-      CDL_CUDA(launch_pdl(sum_vectors_kernel<T>, dim3(static_cast<unsigned>((all + 127) / 128)), dim3(128), 0, stream,
-                          static_cast<const float*>(planes), ld, plane, slices, static_cast<T*>(out.ptr),
-                          static_cast<long long>(out.stride[0]), all, static_cast<int>(cols), add));
-      return CDL_OK;
-    }
+  if (vectors && (all + 127) / 128 <= INT32_MAX) {
+    CDL_CUDA(launch_pdl(sum_vectors_kernel<T>, dim3(static_cast<unsigned>((all + 127) / 128)), dim3(128), 0, stream,
+                        static_cast<const float*>(planes), ld, plane, slices, static_cast<T*>(out.ptr),
+                        static_cast<long long>(out.stride[0]), all, static_cast<int>(cols), add));
+    return CDL_OK;
   }
   dim3 grid;
   CDL_CHECK(segments(rows, cols, &grid));
-  CDL_CUDA(launch_pdl(sum_planes_kernel<S, T>, grid, dim3(256), 0, stream, static_cast<const S*>(planes), ld, plane, slices,
+  CDL_CUDA(launch_pdl(sum_planes_kernel<T>, grid, dim3(256), 0, stream, static_cast<const float*>(planes), ld, plane, slices,
                       static_cast<T*>(out.ptr), static_cast<long long>(out.stride[0]), static_cast<long long>(out.stride[1]),
                       static_cast<int>(cols), add));
   return CDL_OK;
 }
-static int32_t sum_planes(const void* planes, int32_t type, long long ld, long long plane, int slices, const cdl_tensor& out, int add,
-                          cudaStream_t stream) {
-  using bf = __nv_bfloat16;
-  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(out.shape[0]) * out.shape[1] * (dtype_size(type) * slices + dtype_size(out.dtype)), stream);
-  if (type == CDL_BF16) return sum_planes_as<bf, bf>(planes, ld, plane, slices, out, add, stream);
-  return out.dtype == CDL_BF16 ? sum_planes_as<float, bf>(planes, ld, plane, slices, out, add, stream)
-                               : sum_planes_as<float, float>(planes, ld, plane, slices, out, add, stream);
+static int32_t sum_planes(const void* planes, long long ld, long long plane, int slices, const cdl_tensor& out, int add, cudaStream_t stream) {
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(out.shape[0]) * out.shape[1] * (4 * slices + dtype_size(out.dtype)), stream);
+  return out.dtype == CDL_BF16 ? sum_planes_as<__nv_bfloat16>(planes, ld, plane, slices, out, add, stream)
+                               : sum_planes_as<float>(planes, ld, plane, slices, out, add, stream);
 }
 
 // ------------------------------------------------------------------------------------------ checks
@@ -1267,7 +1322,7 @@ static int32_t pieces_product(const Linear& p, const cdl_tensor& a, const cdl_te
     return matmul_pieces_execute(&a, &b, static_cast<float*>(d.ptr), M > 1 ? d.stride[0] : ld, 1, add, stream);
   float* planes = reinterpret_cast<float*>(base + p.at_planes);
   CDL_CHECK(matmul_pieces_execute(&a, &b, planes, ld, slices, 0, stream));
-  return sum_planes(planes, CDL_F32, ld, M * ld, slices, d, add, stream);
+  return sum_planes(planes, ld, M * ld, slices, d, add, stream);
 }
 
 static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& entries, const RowTerms& terms, void* scratch,
@@ -1275,7 +1330,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
   const bool grad = p.has_dx || p.has_dw, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
   const cdl_tensor dw_near = dc ? transposed(p.dw) : p.dw;  // dimension 1 the nearer one in memory
   if (p.T == 0) {  // no rows: no loss, and a gradient of zeros
-    if (p.has_dw && !desc->accumulate_dw && p.D > 0 && p.V > 0) CDL_CHECK(sum_planes(nullptr, CDL_F32, 0, 0, 0, dw_near, 0, stream));
+    if (p.has_dw && !desc->accumulate_dw && p.D > 0 && p.V > 0) CDL_CHECK(sum_planes(nullptr, 0, 0, 0, dw_near, 0, stream));
     return CDL_OK;
   }
   if (p.bytes > 0 && (!scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(scratch) & 255)))
@@ -1318,13 +1373,13 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
   } else {
     cdl_tensor x = p.x, w = p.w;
     if (p.copy_x) {
-      CDL_CHECK(copy(p.x, base + p.at_x, p.ld_x, stream));
       x = strided2(base + p.at_x, CDL_BF16, p.T, p.D, p.ld_x);
+      CDL_CHECK(copy(p.x, x, stream));
     }
     if (p.copy_w) {
       const cdl_tensor w_near = wc ? transposed(p.w) : p.w;
-      CDL_CHECK(copy(w_near, base + p.at_w, p.ld_w, stream));
       w = strided2(base + p.at_w, CDL_BF16, w_near.shape[0], w_near.shape[1], p.ld_w);
+      CDL_CHECK(copy(w_near, w, stream));
       if (wc) w = transposed(w);
     }
     const cdl_tensor wt = transposed(w);
@@ -1345,7 +1400,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
         if (p.slices_dx * planes_per_slice > 1) {
           float* planes = reinterpret_cast<float*>(base + p.at_planes);
           CDL_CHECK(matmul_planes_execute(&g, &wt, planes, p.ld_x, p.slices_dx, stream));
-          CDL_CHECK(sum_planes(planes, CDL_F32, p.ld_x, n * p.ld_x, p.slices_dx * planes_per_slice, d, 0, stream));
+          CDL_CHECK(sum_planes(planes, p.ld_x, n * p.ld_x, p.slices_dx * planes_per_slice, d, 0, stream));
         } else {
           CDL_CHECK(matmul_execute(&g, &wt, nullptr, &d, 1.f, 0.f, stream));
         }
@@ -1360,8 +1415,8 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       }
     }
   }
-  if (p.has_dw && p.dw_way != Linear::DIRECT)
-    CDL_CHECK(sum_planes(dw.ptr, dw.dtype, p.ld_sum, 0, 1, dw_near, desc->accumulate_dw, stream));
+  if (p.has_dw && p.dw_way == Linear::HELD) CDL_CHECK(copy(dw, dw_near, stream));
+  if (p.has_dw && p.dw_way == Linear::SUMMED) CDL_CHECK(sum_planes(dw.ptr, p.ld_sum, 0, 1, dw_near, desc->accumulate_dw, stream));
   return CDL_OK;
 }
 
