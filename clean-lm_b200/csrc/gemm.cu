@@ -546,6 +546,47 @@ __device__ __forceinline__ void store_tile_rows_tma(const Params& p, const CUten
   }
 }
 
+// The same for rows off the 16-byte grid: by way of the buffer, 64 bytes of a row per instruction. A tile's 512 of them per
+// warp and column half take half the time of its bytes' way to the L2; a product beside them and a copy of its rows cost 3 times the bytes.
+__device__ __forceinline__ void store_tile_rows_odd(const Params& p, uint8_t* buf, uint32_t t_row, int row0, int col_base, int lane) {
+  const int rows = min(32, p.M - row0);
+  if (rows <= 0) return;  // warp-uniform
+#pragma unroll 1
+  for (int ch = 0; ch < 2; ++ch) {
+    const int col0 = col_base + ch * 64;
+    if (col0 >= p.N) break;
+    uint32_t r[2][32];
+    tmem_ld32(t_row + ch * 64, r[0]);
+    tmem_ld32(t_row + ch * 64 + 32, r[1]);
+    tmem_wait_ld(r[0], r[1]);
+    __syncwarp();  // the chunk before has been read
+    const uint32_t base = smem_u32(buf), row = base + lane * 128, x = (lane & 7) << 4;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = pack_bf16x2(p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j]),
+                           p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j + 1]));
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((c << 4) ^ x)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+    __syncwarp();
+    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.d) + static_cast<long long>(row0) * p.ldd + col0 + lane;
+    const bool first = col0 + lane < p.N, second = col0 + lane + 32 < p.N;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i, to += p.ldd) {
+      if (i >= rows) break;
+      const uint32_t from = base + i * 128 + ((lane * 2) ^ ((i & 7) << 4));
+      unsigned short v0, v1;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v0) : "r"(from));
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v1) : "r"(from ^ 64));
+      if (first) reinterpret_cast<unsigned short*>(to)[0] = v0;
+      if (second) reinterpret_cast<unsigned short*>(to)[32] = v1;
+    }
+  }
+}
+
 // One of 32 registers, by a tree of selections.
 __device__ __forceinline__ uint32_t pick32(const uint32_t (&r)[32], int i) {
   uint32_t a[16];
@@ -1221,7 +1262,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       } else if constexpr (KIND == STORE_PLANES || KIND == STORE_PIECES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else if constexpr (KIND == STORE_BF16) {
-        store_tile_rows_tma(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
+        if (p.d_vec) store_tile_rows_tma(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
+        else store_tile_rows_odd(p, buf, t_row, row - lane, col, lane);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
         else store_tile_rows(p, t_row, b, row, col);
@@ -1929,23 +1971,28 @@ int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d
   return pair ? pair_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, tm_a, 0, stream) : one_launch<gemm::STORE_PIECES>(p, tm_a, tm_b, stream);
 }
 
-// Whether a plain product is bound by the store of its bf16 D, which TMA makes the shorter: a short K and pairs with several
-// tiles each.
-bool matmul_store_bound(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d) {
+// Plain products whose bf16 D is stored by way of shared memory: those that the store bounds (a short K and pairs with several
+// tiles each), by TMA; and all with that many tiles whose rows are off the 16-byte grid.
+bool matmul_store_bound(long long M, long long N, long long K, const cdl_tensor* d) {
   using namespace gemm;
-  const long long M = a->shape[0], K = a->shape[1], N = b->shape[1];
-  return d->dtype == CDL_BF16 && K <= 512 && M > BM && ((M + PAIR_M - 1) / PAIR_M) * ((N + BN - 1) / BN) >= sm_count() &&
-         (reinterpret_cast<uintptr_t>(d->ptr) & 15) == 0 && d->stride[1] == 1 && d->stride[0] % 8 == 0 && d->stride[0] >= N;
+  if (d->dtype != CDL_BF16 || M <= BM || ((M + PAIR_M - 1) / PAIR_M) * ((N + BN - 1) / BN) < sm_count() || d->stride[1] != 1) return false;
+  return K <= 512 || (reinterpret_cast<uintptr_t>(d->ptr) & 15) != 0 || d->stride[0] % 8 != 0;
 }
 
 int32_t matmul_store_execute(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d, cudaStream_t stream, int early) {
   gemm::Params p;
   CUtensorMap tm_a, tm_b, tm_d;
   CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, true));
-  const uint64_t ld = static_cast<uint64_t>(d->stride[0]) * 2;
-  const uint64_t dims[3] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M), 1}, strides[3] = {0, ld, ld * p.M};
-  const uint32_t box[3] = {64, 32, 1};
-  CDL_CHECK(encode_tmap(&tm_d, d->ptr, CDL_BF16, 3, dims, strides, box, true));
+  p.d = d->ptr;
+  p.ldd = d->stride[0];
+  p.d_vec = (reinterpret_cast<uintptr_t>(d->ptr) & 15) == 0 && d->stride[0] % 8 == 0;
+  tm_d = tm_a;  // (a valid map where none is used)
+  if (p.d_vec) {
+    const uint64_t ld = static_cast<uint64_t>(d->stride[0]) * 2;
+    const uint64_t dims[3] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M), 1}, strides[3] = {0, ld, ld * p.M};
+    const uint32_t box[3] = {64, 32, 1};
+    CDL_CHECK(encode_tmap(&tm_d, d->ptr, CDL_BF16, 3, dims, strides, box, true));
+  }
   return pair_launch<gemm::STORE_BF16>(p, tm_a, tm_b, tm_d, early, stream);
 }
 

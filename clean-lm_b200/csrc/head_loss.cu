@@ -1175,10 +1175,14 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
   if (p.chunk > p.T) p.chunk = p.T;
   const bool whole = p.chunk >= p.T, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
   p.dw_way = Linear::DIRECT;
-  if (p.has_dw && !(on_grid(p.dw) && (p.dw.dtype == CDL_F32 || whole)))
-    p.dw_way = p.dw.dtype == CDL_BF16 && whole && !desc->accumulate_dw ? Linear::HELD : Linear::SUMMED;
   p.twice = !p.f32 && grad && whole && p.T <= 64;
   const size_t n = static_cast<size_t>(p.chunk), g_rows = p.twice ? 2 * n : n;
+  if (p.has_dw && !(on_grid(p.dw) && (p.dw.dtype == CDL_F32 || whole))) {
+    const cdl_tensor near = dc ? transposed(p.dw) : p.dw;
+    p.dw_way = p.dw.dtype != CDL_BF16 || !whole || desc->accumulate_dw                                          ? Linear::SUMMED
+               : matmul_store_bound(near.shape[0], near.shape[1], static_cast<long long>(g_rows), &near) ? Linear::DIRECT
+                                                                                                                : Linear::HELD;
+  }
   p.ld_x = up(p.D, 8);
   p.ld_w = up(wc ? p.D : p.V, 8);
   p.ld_g = up(p.V, 128);
@@ -1410,7 +1414,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
         const cdl_tensor a = dc ? transposed(g) : transposed(clean), &b = dc ? clean : g;
         // (beside the kernel ahead, dx's, whose last wave leaves SMs idle: the two share what they read alone)
         const int early = p.has_dx ? 1 : 0;
-        if (!add && matmul_store_bound(&a, &b, &dw)) CDL_CHECK(matmul_store_execute(&a, &b, &dw, stream, early));
+        if (!add && matmul_store_bound(dw.shape[0], dw.shape[1], a.shape[1], &dw)) CDL_CHECK(matmul_store_execute(&a, &b, &dw, stream, early));
         else CDL_CHECK(matmul_execute(&a, &b, add ? &dw : nullptr, &dw, 1.f, add ? 1.f : 0.f, stream, &fixed, nullptr, 0, early));
       }
     }

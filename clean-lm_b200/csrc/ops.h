@@ -63,8 +63,8 @@ constexpr int MAX_PLANES = 24;
 int matmul_plane_slices(long long M, long long N, long long K, bool pieces = false);
 int32_t matmul_pieces_execute(const cdl_tensor* a, const cdl_tensor* b, float* d, long long ldd, int slices, int add, cudaStream_t stream);
 int32_t matmul_planes_execute(const cdl_tensor* a, const cdl_tensor* b, float* planes, long long ld, int slices, cudaStream_t stream);
-// D = A . B of such tensors with a bf16 D whose store sets the time (matmul_store_bound), stored by TMA.
-bool matmul_store_bound(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d);
+// D = A . B of such operands with a bf16 D of any rows of neighbouring elements, where matmul_store_bound says so of its M, N and K.
+bool matmul_store_bound(long long M, long long N, long long K, const cdl_tensor* d);
 int32_t matmul_store_execute(const cdl_tensor* a, const cdl_tensor* b, const cdl_tensor* d, cudaStream_t stream, int early);
 // norm_general.cu: any float types, strides and column counts (layer = 0 RmsNorm, 1 LayerNorm).
 int32_t norm_general_execute(int layer, const cdl_tensor* x, const cdl_tensor* scale,

@@ -412,6 +412,23 @@ def test_gradients_on_their_own_and_odd_outputs(cdl, gpu_ok):
 
 
 @gpu
+@pytest.mark.parametrize("t,d,v,tied", [(3, 1100, 9001, False), (90, 1101, 9000, True), (600, 390, 20003, False), (257, 1030, 9472, False),
+                                        (1, 9473, 1025, False)])
+@pytest.mark.parametrize("wider,off", [(0, 0), (5, 2), (8, 3)])
+def test_weight_gradient_of_rows_off_the_grid(cdl, gpu_ok, t, d, v, tied, wider, off):
+    """Outputs of many tiles whose rows begin anywhere; what lies between and around the rows stays as it was."""
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    x, w = _operands(gen, t, d, v, BF16, "tied" if tied else "rows")
+    rows, cols = (v, d) if tied else (d, v)
+    buffer = torch.full((rows + 2, cols + wider), 7.0, dtype=BF16, device="cuda")
+    view = buffer[1:-1, off:off + cols]
+    dw = view.t() if tied else view
+    _check_linear(cdl, x, w, _entries(gen, t, v, 0), cdl.ops.LinearLossOpts(), dw=dw)
+    view.fill_(7.0)
+    assert bool((buffer == 7.0).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("k", [0, 4])
 def test_rows_that_do_not_count_add_nothing(cdl, gpu_ok, dtype, k):
