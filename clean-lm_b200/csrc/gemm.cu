@@ -546,8 +546,8 @@ __device__ __forceinline__ void store_tile_rows_tma(const Params& p, const CUten
   }
 }
 
-// The same for rows off the 16-byte grid: by way of the buffer, 64 bytes of a row per instruction. A tile's 512 of them per
-// warp and column half take half the time of its bytes' way to the L2; a product beside them and a copy of its rows cost 3 times the bytes.
+// The same for rows off the 16-byte grid: by way of the buffer, 64 bytes of a row per instruction.  (95 x 2185 x 94464: the loss with its
+// gradients 502 us; with D stored on the grid and copied behind the product, which moves its bytes three times, 591.)
 __device__ __forceinline__ void store_tile_rows_odd(const Params& p, uint8_t* buf, uint32_t t_row, int row0, int col_base, int lane) {
   const int rows = min(32, p.M - row0);
   if (rows <= 0) return;  // warp-uniform

@@ -81,6 +81,32 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The three bf16 pieces of an f32 value, v = p0 + p1 + p2 to 24 bits: the first two cut off (no finite value becomes infinite),
+// the last rounded.
+__device__ __forceinline__ void pieces_of(float v, float (&p)[3]) {
+  p[0] = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  const float r = v - p[0];
+  p[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+  p[2] = r - p[1];
+}
+
+// Where a row's gradient goes: T [.., ld], or the pieces of f32 values, bf16 [3][.., ld], planes `plane` apart.
+struct GradRows {
+  void* ptr;  // nullptr: not wanted
+  long long ld, plane;
+};
+template <typename T, bool PIECES>
+__device__ __forceinline__ void put(const GradRows& g, long long row, long long j, float v) {
+  if constexpr (PIECES) {
+    float p[3];
+    pieces_of(v, p);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) static_cast<__nv_bfloat16*>(g.ptr)[i * g.plane + row * g.ld + j] = __float2bfloat16_rn(p[i]);
+  } else {
+    static_cast<T*>(g.ptr)[row * g.ld + j] = from_f32<T>(v);
+  }
+}
+
 // A row's entries in shared memory, and what a reduction over the CTA uses.
 struct RowEntries {
   int* id;    // -1: does not count
@@ -193,9 +219,9 @@ __device__ __forceinline__ bool is_marked(const int* table, int slots_log2, int 
 }
 
 // One CTA per row: the row is read twice (the second time from the L2), any alignment and length.
-template <typename T>
+template <typename T, bool PIECES>
 __global__ void __launch_bounds__(ROW_THREADS)
-    loss_row_kernel(const T* z, long long ld_z, T* g, long long ld_g, int vocab, const Entries src, const RowTerms terms) {
+    loss_row_kernel(const T* z, long long ld_z, const GradRows g, int vocab, const Entries src, const RowTerms terms) {
   __shared__ int entries[3 * MAX_ENTRIES];
   __shared__ RowShared sh;
   const RowEntries e(entries, src.K);
@@ -231,12 +257,11 @@ __global__ void __launch_bounds__(ROW_THREADS)
     terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
     if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * log2_s;
   }
-  if (g == nullptr) return;
-  T* y = g + row * ld_g;
+  if (g.ptr == nullptr) return;
   const float scale = counts ? terms.grad_scale * terms.tau * (terms.d_loss ? terms.d_loss[row * terms.d_loss_stride] : 1.f) : 0.f;
   const float over_s = scale / s;
   for (int j = threadIdx.x; j < vocab; j += ROW_THREADS)
-    y[j] = from_f32<T>(counts ? ex2(c * (to_f32(x[j]) - base)) * over_s : 0.f);
+    put<T, PIECES>(g, row, j, counts ? ex2(c * (to_f32(x[j]) - base)) * over_s : 0.f);
   __syncthreads();
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS) {
     const int id = e.id[k];
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(ROW_THREADS)
       again = again || i < k;
       p += e.p[i];
     }
-    if (!again) y[id] = from_f32<T>(scale * (ex2(c * (e.at[k] - base)) / s - p));
+    if (!again) put<T, PIECES>(g, row, id, scale * (ex2(c * (e.at[k] - base)) / s - p));
   }
 }
 
@@ -303,9 +328,9 @@ __device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
   return d;
 }
 
-template <typename T, int VECS>
+template <typename T, int VECS, bool PIECES>
 __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
-    loss_slices_kernel(const T* z, long long ld_z, T* g, long long ld_g, long long rows, long long ahead, int vocab, int slice, int ctas,
+    loss_slices_kernel(const T* z, long long ld_z, const GradRows g, long long rows, long long ahead, int vocab, int slice, int ctas,
                        int slots_log2, const Entries src, const RowTerms terms) {
   constexpr bool HALF = sizeof(T) == 2;
   constexpr int VEC = 16 / sizeof(T);
@@ -466,11 +491,11 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
       if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * (log2_s - OFF);
     }
   }
-  if (g != nullptr) {
-    T* y = g + row * ld_g;
+  if (g.ptr != nullptr) {
+    T* y = PIECES ? nullptr : static_cast<T*>(g.ptr) + row * g.ld;
     const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f;
     const float factor = ex2(c * (own - base)) * (scale / s);
-    const bool in_step = static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
+    const bool in_step = PIECES ? lead == 0 : static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
     const int at0 = lane * VEC - first;  // the row's element at the lane's first vector
     const uint64_t f2 = pack_f2(factor, factor);
 #pragma unroll
@@ -493,7 +518,23 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
       if (!counts) q[i] = make_uint4(0, 0, 0, 0);  // (whatever the logits were)
       if (lane + 32 * i >= n) continue;
       const int at = at0 + i * 32 * VEC;
-      if (in_step && at >= 0 && at + VEC <= vocab) {
+      if constexpr (PIECES) {
+        float v[4][3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pieces_of(__uint_as_float(w[j]), v[j]);
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(g.ptr) + row * g.ld + at;
+#pragma unroll
+        for (int k = 0; k < 3; ++k, to += g.plane) {
+          const uint2 pair = make_uint2(pack_bf16x2(v[0][k], v[1][k]), pack_bf16x2(v[2][k], v[3][k]));
+          if (in_step && at >= 0 && at + VEC <= vocab) {
+            *reinterpret_cast<uint2*>(to) = pair;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (at + j >= 0 && at + j < vocab) to[j] = __float2bfloat16_rn(v[j][k]);
+          }
+        }
+      } else if (in_step && at >= 0 && at + VEC <= vocab) {
         *reinterpret_cast<uint4*>(y + at) = q[i];
       } else {
 #pragma unroll
@@ -520,7 +561,7 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
         }
         if (again) continue;
       }
-      y[id] = from_f32<T>(scale * (ex2(c * (e.at[k] - base) + OFF) / s - p));
+      put<T, PIECES>(g, row, id, scale * (ex2(c * (e.at[k] - base) + OFF) / s - p));
     }
   }
   if (ctas > 1) cluster_wait();  // the peers have read this CTA's parts
@@ -799,8 +840,7 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// The three bf16 pieces of f32 values, v = p0 + p1 + p2 to 24 bits: the first two cut off (no finite value becomes infinite),
-// the last rounded.  Zeros where keep (nullptr: all rows count) says that a row does not count.  dst: [3][rows][ld], planes
+// The pieces of f32 values.  Zeros where keep (nullptr: all rows count) says that a row does not count.  dst: [3][rows][ld], planes
 // `plane` apart.
 __global__ void __launch_bounds__(256)
     split_kernel(const float* src, long long s_row, long long s_col, __nv_bfloat16* dst, long long ld, long long plane, int cols,
@@ -818,12 +858,12 @@ __global__ void __launch_bounds__(256)
   for (int j = 0; j < 8; ++j) {
     if (at.col + 256 * j >= cols) break;
     const float x = zero ? 0.f : v[j];
-    const float p0 = __uint_as_float(__float_as_uint(x) & 0xffff0000u), r = x - p0;
-    const float p1 = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    float p[3];
+    pieces_of(x, p);
     __nv_bfloat16* o = dst + at.row * ld + at.col + 256 * j;
-    o[0] = __float2bfloat16_rn(p0);
-    o[plane] = __float2bfloat16_rn(p1);
-    o[2 * plane] = __float2bfloat16_rn(r - p1);
+    o[0] = __float2bfloat16_rn(p[0]);
+    o[plane] = __float2bfloat16_rn(p[1]);
+    o[2 * plane] = __float2bfloat16_rn(p[2]);
   }
 }
 
@@ -931,22 +971,22 @@ static Share choose_share(const void* z, long long ld, long long rows, int vocab
   return s;
 }
 
-template <typename T>
-static int32_t launch_rows(const void* z, long long ld_z, void* g, long long ld_g, long long rows, int vocab, const Entries& e,
+template <typename T, bool PIECES>
+static int32_t launch_rows(const void* z, long long ld_z, const GradRows& g, long long rows, int vocab, const Entries& e,
                            const RowTerms& t, cudaStream_t stream) {
-  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * sizeof(T) * (g ? 2 : 1), stream);
+  ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (sizeof(T) + (g.ptr ? (PIECES ? 6 : sizeof(T)) : 0)), stream);
   const Share share = choose_share(z, ld_z, rows, vocab, sizeof(T), e.K);
   if (share.warps == 0 || rows * share.ctas > INT32_MAX) {
-    CDL_CUDA(launch_pdl(loss_row_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(z),
-                        ld_z, static_cast<T*>(g), ld_g, vocab, e, t));
+    CDL_CUDA(launch_pdl(loss_row_kernel<T, PIECES>, dim3(static_cast<unsigned>(rows)), dim3(ROW_THREADS), 0, stream,
+                        static_cast<const T*>(z), ld_z, g, vocab, e, t));
     return CDL_OK;
   }
-  auto kernel = share.slice <= 256 ? loss_slices_kernel<T, 8> : loss_slices_kernel<T, 16>;
+  auto kernel = share.slice <= 256 ? loss_slices_kernel<T, 8, PIECES> : loss_slices_kernel<T, 16, PIECES>;
   // Rows that run at once: two CTAs of 16 warps, or as many threads in more, per SM.
   const long long ahead = static_cast<long long>(sm_count()) * (share.slice <= 256 ? 1024 : 512) / (share.warps * 32);
   CDL_CUDA(launch_pdl_cluster(kernel, dim3(static_cast<unsigned>(rows * share.ctas)), dim3(share.warps / share.ctas * 32), share.smem,
-                              share.ctas, stream, static_cast<const T*>(z), ld_z, static_cast<T*>(g), ld_g, rows, ahead, vocab,
-                              share.slice, share.ctas, share.slots_log2, e, t));
+                              share.ctas, stream, static_cast<const T*>(z), ld_z, g, rows, ahead, vocab, share.slice, share.ctas,
+                              share.slots_log2, e, t));
   return CDL_OK;
 }
 
@@ -1103,9 +1143,9 @@ static int32_t distillation_execute(const cdl_head_loss_desc* desc, const cdl_te
   }
   if (T == 0) return CDL_OK;
   if (V == 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
-  auto rows = logits->dtype == CDL_BF16 ? launch_rows<__nv_bfloat16> : launch_rows<float>;
-  return rows(logits->ptr, logits->stride[0], d_logits ? d_logits->ptr : nullptr, d_logits ? d_logits->stride[0] : 0, T,
-              static_cast<int>(V), e, terms, stream);
+  auto rows = logits->dtype == CDL_BF16 ? launch_rows<__nv_bfloat16, false> : launch_rows<float, false>;
+  const GradRows g = {d_logits ? d_logits->ptr : nullptr, d_logits ? static_cast<long long>(d_logits->stride[0]) : 0, 0};
+  return rows(logits->ptr, logits->stride[0], g, T, static_cast<int>(V), e, terms, stream);
 }
 
 // ------------------------------------------------------------------------------------------ from the hidden states
@@ -1358,14 +1398,14 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
       const Entries e = from_row(entries, row);
       CDL_CHECK(split(xc, base + p.at_x, p.ld_x, x_plane, nullptr, stream));
       CDL_CHECK(pieces_product(p, pieces3(base + p.at_x, n, p.D, p.ld_x, x_plane), w3, z, p.slices_z, 0, base, stream));
-      CDL_CHECK(launch_rows<float>(z.ptr, p.ld_g, grad ? z.ptr : nullptr, p.ld_g, n, vocab, e, from_row(terms, row), stream));
+      const GradRows g = {grad ? base + p.at_g : nullptr, p.ld_g, g_plane};
+      CDL_CHECK((launch_rows<float, true>(z.ptr, p.ld_g, g, n, vocab, e, from_row(terms, row), stream)));
       if (!grad) continue;
       if (p.has_dw) {  // (the copy with zeros in rows that do not count, see below)
         float* keep = reinterpret_cast<float*>(base + p.at_keep);
         CDL_CUDA(launch_pdl(keep_kernel, dim3(static_cast<unsigned>((n + 7) / 8)), dim3(256), 0, stream, e, n, vocab, keep));
         CDL_CHECK(split(xc, base + p.at_clean, p.ld_x, x_plane, keep, stream));
       }
-      CDL_CHECK(split(z, base + p.at_g, p.ld_g, g_plane, nullptr, stream));
       if (p.has_dx)
         CDL_CHECK(pieces_product(p, pieces3(base + p.at_g, n, p.V, p.ld_g, g_plane), wt3, rows_of(p.dx, row, n), p.slices_dx, 0, base, stream));
       if (p.has_dw) {
