@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(256) copy_kernel(const T* src, long long s_row
 
 // The same for rows of neighbouring elements, from and to any alignment: a thread has 16 aligned bytes of dst at a time, out
 // of the two aligned 16 bytes of src that hold them (both hold an element of the row); what a row has of its first and last 16 bytes
-// goes one by one. 190 MB of bf16 rows of 85695 there and back: 130 us, element by element 330.
+// goes one by one. 190 MB of bf16 rows of 85695: 71 us, 5.4 TB/s; element by element 93.
 constexpr int COPY_VECS = 4;  // of a thread, 256 apart
 __global__ void __launch_bounds__(256)
     copy_rows_kernel(const __nv_bfloat16* src, long long s_row, __nv_bfloat16* dst, long long d_row, int cols, unsigned per_row, long long all) {
