@@ -931,6 +931,236 @@ __global__ void __launch_bounds__(256) keep_kernel(const Entries src, long long 
   if ((threadIdx.x & 31) == 0) keep[row] = any ? 1.f : 0.f;
 }
 
+// ------------------------------------------------------------------------------------------ few rows of f32 operands
+// Up to FEW_ROWS tokens an f32 product reads w once, as it is, and multiplies in f32, two tokens per instruction: 2 T operations per 4
+// bytes, at 16 tokens a third of what the SMs do while HBM brings the bytes.  (The pieces of w alone are 2.5 times its
+// bytes, written and read by three products: 4 x 2048 x 112256 1546 us, 492 so; 16 tokens 1538 and 820.)  TT tokens are a
+// thread's accumulators; those behind the last are zeros.  Any alignment: lanes have neighbouring elements.
+constexpr int FEW_ROWS = 16, FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
+constexpr int FEW_CHUNK = 512;      // of K in shared memory at a time
+constexpr int FEW_OUTER_COLS = 128, FEW_INNER_COLS = 4 * FEW_WARPS;  // of a block
+
+// [k][TT] in shared memory: all tokens of columns k0 .. k0 + n - 1 of a, zeros for tokens that do not exist or (keep: nullptr, or
+// a flag per token) do not count.
+template <int TT>
+__device__ __forceinline__ void few_columns(float* s, const float* a, long long lda, int T, long long k0, int n, const float* keep) {
+  for (int k = threadIdx.x; k < n; k += FEW_THREADS) {
+#pragma unroll
+    for (int q = 0; q < TT / 4; ++q) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = 4 * q + j;
+        v[j] = t < T && (keep == nullptr || keep[t] != 0.f) ? a[t * lda + k0 + k] : 0.f;
+      }
+      *reinterpret_cast<float4*>(s + k * TT + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// out[slice][t, n] = sum over the slice's k of a[t, k] b[k, n]: a block has 128 columns, a lane four of them, the warps every eighth k.
+template <int TT>
+__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
+    few_outer_kernel(const float* a, long long lda, const float* b, long long ldb, int T, int K, int N, int slices, float* out, long long ldo,
+                     long long plane) {
+  __shared__ __align__(16) float s_a[FEW_CHUNK * TT];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = blockIdx.y, first = blockIdx.x * FEW_OUTER_COLS, n0 = first + lane;
+  const bool whole = first + FEW_OUTER_COLS <= N;
+  const int k0 = static_cast<int>(static_cast<long long>(K) * slice / slices), k1 = static_cast<int>(static_cast<long long>(K) * (slice + 1) / slices);
+  constexpr int U = 4, STEP = FEW_WARPS * U;
+  uint64_t acc[4][TT / 2];  // of two tokens each
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int t = 0; t < TT / 2; ++t) acc[c][t] = 0;
+  for (int kc = k0; kc < k1; kc += FEW_CHUNK) {
+    const int n = min(FEW_CHUNK, k1 - kc);
+    __syncthreads();
+    few_columns<TT>(s_a, a, lda, T, kc, n, nullptr);
+    __syncthreads();
+    const float* from = b + static_cast<long long>(kc + warp) * ldb + n0;
+    for (int k = warp; k < n; k += STEP, from += STEP * ldb) {
+      float v[U][4];
+      if (whole && k + FEW_WARPS * (U - 1) < n) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[u][c] = from[u * FEW_WARPS * ldb + 32 * c];
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[u][c] = k + FEW_WARPS * u < n && n0 + 32 * c < N ? from[u * FEW_WARPS * ldb + 32 * c] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k + FEW_WARPS * u >= n) break;
+        uint64_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = pack_f2(v[u][c], v[u][c]);
+#pragma unroll
+        for (int q = 0; q < TT / 4; ++q) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(s_a + (k + FEW_WARPS * u) * TT + 4 * q);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            acc[c][2 * q] = fma_f2(x.x, w[c], acc[c][2 * q]);
+            acc[c][2 * q + 1] = fma_f2(x.y, w[c], acc[c][2 * q + 1]);
+          }
+        }
+      }
+    }
+  }
+  // The warps' sums in their order, half of the tokens at a time: [warps][TT / 4][128] pairs where the columns of a were.
+  constexpr int PAIRS = TT / 4;
+  uint64_t* s_sum = reinterpret_cast<uint64_t*>(s_a);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < PAIRS; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s_sum[(warp * PAIRS + t) * FEW_OUTER_COLS + lane + 32 * c] = acc[c][half * PAIRS + t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < PAIRS * FEW_OUTER_COLS; i += FEW_THREADS) {
+      const int t = 2 * (half * PAIRS + i / FEW_OUTER_COLS), col = first + i % FEW_OUTER_COLS;
+      uint64_t sum = s_sum[i];
+#pragma unroll
+      for (int w = 1; w < FEW_WARPS; ++w) sum = add_f2(sum, s_sum[w * PAIRS * FEW_OUTER_COLS + i]);
+      float lo, hi;
+      unpack_f2(sum, lo, hi);
+      if (t < T && col < N) out[slice * plane + t * ldo + col] = lo;
+      if (t + 1 < T && col < N) out[slice * plane + (t + 1) * ldo + col] = hi;
+    }
+  }
+}
+
+// out[slice][t, n] = sum over the slice's k of a[t, k] b[n, k]: a warp has four n, its lanes neighbouring k.
+template <int TT>
+__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
+    few_inner_kernel(const float* a, long long lda, const float* b, long long ldb, int T, int K, int N, int slices, float* out, long long ldo,
+                     long long plane) {
+  __shared__ __align__(16) float2 s_a[TT / 2][FEW_CHUNK];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = blockIdx.y, n0 = blockIdx.x * FEW_INNER_COLS + warp * 4;
+  const bool whole = n0 + 4 <= N;
+  const int k0 = static_cast<int>(static_cast<long long>(K) * slice / slices), k1 = static_cast<int>(static_cast<long long>(K) * (slice + 1) / slices);
+  constexpr int U = 4, STEP = 32 * U;
+  uint64_t acc[TT / 2][4];  // of two tokens each
+#pragma unroll
+  for (int t = 0; t < TT / 2; ++t)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[t][c] = 0;
+  for (int kc = k0; kc < k1; kc += FEW_CHUNK) {
+    const int n = min(FEW_CHUNK, k1 - kc);
+    __syncthreads();
+    for (int k = threadIdx.x; k < FEW_CHUNK; k += FEW_THREADS)
+#pragma unroll
+      for (int t = 0; t < TT; t += 2)
+        s_a[t / 2][k] = make_float2(t < T && k < n ? a[t * lda + kc + k] : 0.f, t + 1 < T && k < n ? a[(t + 1) * lda + kc + k] : 0.f);
+    __syncthreads();
+    const float* from = b + static_cast<long long>(n0) * ldb + kc + lane;
+    for (int k = 0; k < n; k += STEP, from += STEP) {
+      float v[U][4];
+      if (whole && k + STEP <= n) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[u][c] = from[c * ldb + 32 * u];
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[u][c] = k + lane + 32 * u < n && n0 + c < N ? from[c * ldb + 32 * u] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k + 32 * u >= n) break;
+        uint64_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = pack_f2(v[u][c], v[u][c]);
+#pragma unroll
+        for (int t = 0; t < TT / 2; ++t) {
+          const uint64_t x = *reinterpret_cast<const uint64_t*>(&s_a[t][k + lane + 32 * u]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[t][c] = fma_f2(x, w[c], acc[t][c]);
+        }
+      }
+    }
+  }
+  // Sums over the lanes: in each step a lane keeps one half of its pairs and gives the other away; then it has pair lane of TT * 2, or
+  // (TT = 4) four lanes the same one.
+  int left = TT * 2;
+  uint64_t* flat = &acc[0][0];
+  auto other = [](uint64_t v, int o) { return __shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(v), o); };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (left > 1) {
+      left /= 2;
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        if (i >= left) break;
+        const uint64_t give = lane & o ? flat[i] : flat[i + left], keep = lane & o ? flat[i + left] : flat[i];
+        flat[i] = add_f2(keep, other(give, o));
+      }
+    } else {
+      flat[0] = add_f2(flat[0], other(flat[0], o));
+    }
+  }
+  const int pair = lane * (TT * 2) / 32, t = pair / 4 * 2, col = n0 + pair % 4;
+  float lo, hi;
+  unpack_f2(flat[0], lo, hi);
+  if (t < T && col < N) out[slice * plane + t * ldo + col] = lo;
+  if (t + 1 < T && col < N) out[slice * plane + (t + 1) * ldo + col] = hi;
+}
+
+// out[m, n] (+)= sum over the tokens of a[t, m] b[t, n]; keep_a, keep_b as above.  A block has 128 columns, whose values of b stay in
+// registers, and every `groups`th FEW_OUT_ROWS rows.
+constexpr int FEW_OUT_ROWS = 256;
+template <int TT>
+__global__ void __launch_bounds__(FEW_THREADS, 2)
+    few_update_kernel(const float* a, long long lda, const float* keep_a, const float* b, long long ldb, const float* keep_b, int T, int M, int N,
+                      float* out, long long ldo, int groups, int add) {
+  __shared__ __align__(16) float s_a[FEW_OUT_ROWS * TT];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col_blocks = (N + FEW_OUTER_COLS - 1) / FEW_OUTER_COLS;
+  const int first = static_cast<int>(blockIdx.x % col_blocks) * FEW_OUTER_COLS, n0 = first + lane;
+  const bool whole = first + FEW_OUTER_COLS <= N;
+  uint64_t v[4][TT / 2];
+#pragma unroll
+  for (int t = 0; t < TT; t += 2)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      auto at = [&](int t) { return t < T && n0 + 32 * c < N && (keep_b == nullptr || keep_b[t] != 0.f) ? b[t * ldb + n0 + 32 * c] : 0.f; };
+      v[c][t / 2] = pack_f2(at(t), at(t + 1));
+    }
+  for (int m0 = static_cast<int>(blockIdx.x / col_blocks) * FEW_OUT_ROWS; m0 < M; m0 += groups * FEW_OUT_ROWS) {
+    const int rows = min(FEW_OUT_ROWS, M - m0);
+    __syncthreads();
+    few_columns<TT>(s_a, a, lda, T, m0, rows, keep_a);
+    __syncthreads();
+    float* to = out + static_cast<long long>(m0 + warp) * ldo + n0;
+    for (int m = warp; m < rows; m += FEW_WARPS, to += FEW_WARPS * ldo) {
+      uint64_t acc[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < TT / 4; ++q) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(s_a + m * TT + 4 * q);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = fma_f2(x.y, v[c][2 * q + 1], fma_f2(x.x, v[c][2 * q], acc[c]));
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float even, odd;
+        unpack_f2(acc[c], even, odd);
+        if (whole || n0 + 32 * c < N) to[32 * c] = add ? to[32 * c] + (even + odd) : even + odd;
+      }
+    }
+  }
+}
+
 static Entries from_row(Entries e, long long row) {
   e.ids += row * e.ids_ld;
   if (e.kind != TARGETS) e.teacher = static_cast<const char*>(e.teacher) + row * e.teacher_ld * (e.kind == TEACHER_F32 ? 4 : 2);
@@ -1172,6 +1402,7 @@ struct Linear {
   // the other: [2 rows, V], the rows of x twice.  With one piece dx and dw are 1.4 times as far off as their own rounding
   // to bf16, give or take what the rounding of a single row's largest value happens to be.
   bool twice;
+  bool few;  // few rows of f32 operands
   enum { DIRECT, HELD, SUMMED } dw_way;  // the product stores dw; a bf16 dw off the grid, stored beside it first; an f32 sum over the chunks
   int pieces, slices_z, slices_dx, slices_dw;  // pieces: of the vocabulary, 128 columns each
   size_t at_x, at_w, at_clean, at_keep, at_z, at_g, at_stats, at_ids, at_first, at_p, at_p_log_p, at_at, at_planes, at_sum, bytes;
@@ -1203,6 +1434,14 @@ static long long choose_chunk(long long T, long long V, long long bytes_per_logi
   return up((T + chunks - 1) / chunks, 256);
 }
 
+// K slices of a product of few rows: as many as give four blocks per SM, of 512 and more.
+static int few_slices(bool inner, long long K, long long N) {
+  const int cols = inner ? FEW_INNER_COLS : FEW_OUTER_COLS;
+  const long long blocks = (N + cols - 1) / cols, want = 4LL * sm_count() / blocks, most = K / FEW_CHUNK;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : s > MAX_PLANES ? MAX_PLANES : static_cast<int>(s);
+}
+
 static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long entries) {
   const bool grad = p.has_dx || p.has_dw, teacher = entries != TARGET_ENTRIES;
   p.f32 = p.x.dtype == CDL_F32;
@@ -1227,6 +1466,28 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
   p.ld_w = up(wc ? p.D : p.V, 8);
   p.ld_g = up(p.V, 128);
   p.ld_sum = p.has_dw ? up(dc ? p.D : p.V, 8) : 0;
+  auto near = [](const cdl_tensor& t) {  // a row's elements lie next to one another
+    const cdl_tensor n = columns_first(t) ? transposed(t) : t;
+    return n.stride[1] == 1 || n.shape[1] == 1;
+  };
+  p.few = p.f32 && whole && p.T <= FEW_ROWS && (p.x.stride[1] == 1 || p.D == 1) && near(p.w) && (!p.has_dw || near(p.dw));
+  if (p.few) {
+    p.dw_way = Linear::DIRECT;
+    p.slices_z = few_slices(wc, p.D, p.V);
+    p.slices_dx = p.has_dx ? few_slices(!wc, p.V, p.D) : 1;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += (bytes + 255) / 256 * 256;
+      return here;
+    };
+    p.at_z = take(n * p.ld_g * 4);
+    p.at_keep = take(n * 4);
+    const size_t z = p.slices_z > 1 ? p.slices_z * n * up(p.V, 4) : 0, dx = p.slices_dx > 1 ? p.slices_dx * n * up(p.D, 4) : 0;
+    p.at_planes = take(4 * (z > dx ? z : dx));
+    p.bytes = at;
+    return;
+  }
   p.slices_z = p.f32 ? matmul_plane_slices(p.chunk, p.V, p.D, true) : 1;
   p.slices_dx = p.has_dx ? matmul_plane_slices(static_cast<long long>(g_rows), p.D, p.V, p.f32) : 1;
   p.slices_dw = p.has_dw && p.f32 ? matmul_plane_slices(dc ? p.V : p.D, dc ? p.D : p.V, p.chunk, true) : 1;
@@ -1369,6 +1630,57 @@ static int32_t pieces_product(const Linear& p, const cdl_tensor& a, const cdl_te
   return sum_planes(planes, ld, M * ld, slices, d, add, stream);
 }
 
+// out [T, N] = a [T, K] times w, of which N (inner: K) is the nearer dimension in memory, by way of planes if there are slices.
+static int32_t few_product(const Linear& p, const float* a, long long lda, const cdl_tensor& w_near, bool inner, int slices, const cdl_tensor& out,
+                           char* base, cudaStream_t stream) {
+  const long long N = inner ? w_near.shape[0] : w_near.shape[1], K = inner ? w_near.shape[1] : w_near.shape[0];
+  const long long ldo = slices > 1 ? up(N, 4) : static_cast<long long>(out.stride[0]), plane = p.T * up(N, 4);
+  float* to = slices > 1 ? reinterpret_cast<float*>(base + p.at_planes) : static_cast<float*>(out.ptr);
+  auto run = [&](auto kernel) -> int32_t {
+    const int cols = inner ? FEW_INNER_COLS : FEW_OUTER_COLS;
+    const long long blocks = (N + cols - 1) / cols;
+    ProfileScope ps(PROF_GEMM, 2.0 * p.T * K * N, stream);
+    CDL_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(blocks), slices), dim3(FEW_THREADS), 0, stream, a, lda,
+                        static_cast<const float*>(w_near.ptr), static_cast<long long>(w_near.stride[0]), static_cast<int>(p.T),
+                        static_cast<int>(K), static_cast<int>(N), slices, to, ldo, plane));
+    return CDL_OK;
+  };
+  if (p.T <= 4) CDL_CHECK(inner ? run(few_inner_kernel<4>) : run(few_outer_kernel<4>));
+  else CDL_CHECK(inner ? run(few_inner_kernel<16>) : run(few_outer_kernel<16>));
+  return slices > 1 ? sum_planes(to, ldo, plane, slices, out, 0, stream) : CDL_OK;
+}
+
+static int32_t few_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& e, const RowTerms& terms, char* base, cudaStream_t stream) {
+  const bool wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
+  const int T = static_cast<int>(p.T), vocab = static_cast<int>(p.V);
+  const cdl_tensor w_near = wc ? transposed(p.w) : p.w, z = strided2(base + p.at_z, CDL_F32, p.T, p.V, p.ld_g);
+  const float *x = static_cast<const float*>(p.x.ptr), *g = static_cast<const float*>(z.ptr);
+  CDL_CHECK(few_product(p, x, p.x.stride[0], w_near, wc, p.slices_z, z, base, stream));
+  const GradRows grad = {p.has_dx || p.has_dw ? z.ptr : nullptr, p.ld_g, 0};
+  CDL_CHECK((launch_rows<float, false>(z.ptr, p.ld_g, grad, p.T, vocab, e, terms, stream)));
+  if (p.has_dw) {  // (ahead of dx, which may be x; rows that do not count add nothing whatever x holds there)
+    float* keep = reinterpret_cast<float*>(base + p.at_keep);
+    CDL_CUDA(launch_pdl(keep_kernel, dim3((T + 7) / 8), dim3(256), 0, stream, e, p.T, vocab, keep));
+    const cdl_tensor d = dc ? transposed(p.dw) : p.dw;
+    const int M = static_cast<int>(d.shape[0]), N = static_cast<int>(d.shape[1]);
+    auto run = [&](auto kernel) -> int32_t {
+      // Six blocks per SM, or as many as there are: a block's columns of b take as long to come as 128 rows to leave.
+      const int col_blocks = (N + FEW_OUTER_COLS - 1) / FEW_OUTER_COLS, most = (M + FEW_OUT_ROWS - 1) / FEW_OUT_ROWS;
+      const int want = (6 * sm_count() + col_blocks - 1) / col_blocks, groups = want < most ? want : most;
+      const long long blocks = static_cast<long long>(col_blocks) * groups;
+      ProfileScope ps(PROF_GEMM, 2.0 * p.T * M * N, stream);
+      CDL_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(FEW_THREADS), 0, stream, dc ? g : x,
+                          dc ? p.ld_g : static_cast<long long>(p.x.stride[0]), dc ? nullptr : keep, dc ? x : g,
+                          dc ? static_cast<long long>(p.x.stride[0]) : p.ld_g, dc ? keep : nullptr, T, M, N, static_cast<float*>(d.ptr),
+                          static_cast<long long>(d.stride[0]), groups, desc->accumulate_dw));
+      return CDL_OK;
+    };
+    CDL_CHECK(T <= 4 ? run(few_update_kernel<4>) : run(few_update_kernel<16>));
+  }
+  if (p.has_dx) CDL_CHECK(few_product(p, g, p.ld_g, w_near, !wc, p.slices_dx, p.dx, base, stream));
+  return CDL_OK;
+}
+
 static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const Entries& entries, const RowTerms& terms, void* scratch,
                               size_t scratch_bytes, cudaStream_t stream) {
   const bool grad = p.has_dx || p.has_dw, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
@@ -1382,6 +1694,7 @@ static int32_t linear_execute(Linear& p, const cdl_head_loss_desc* desc, const E
   const FixedWorkInGraph fixed_work(stream);
   char* base = static_cast<char*>(scratch);
   const int vocab = static_cast<int>(p.V);
+  if (p.few) return few_execute(p, desc, entries, terms, base, stream);
   // Where dw's product goes, as [D, V] or (dc) [V, D].
   cdl_tensor dw = dw_near;
   if (p.dw_way != Linear::DIRECT)

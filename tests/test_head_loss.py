@@ -299,7 +299,8 @@ SHAPES = [(1, 64, 1000, 0, BF16, "rows"), (1, 8, 1, 0, BF16, "rows"), (7, 65, 12
           (65, 515, 770, 0, F32, "rows"), (40, 64, 301, 0, F32, "tied"), (33, 48, 100, 0, F32, "strided"), (70, 64, 300, 0, BF16, "columns"),
           (1, 64, 1000, 5, BF16, "rows"), (257, 256, 4097, 64, BF16, "rows"), (300, 72, 1001, 7, BF16, "tied"), (12, 128, 640, 300, BF16, "rows"),
           (50, 65, 300, 16, F32, "rows"), (200, 64, 8200, 1, BF16, "tied"), (600, 64, 128, 128, BF16, "rows"), (5, 64, 2000, 1024, BF16, "rows"),
-          (100, 512, 3000, 0, BF16, "rows"), (128, 320, 40000, 0, BF16, "rows"), (128, 320, 40001, 9, BF16, "tied"), (700, 256, 30000, 33, BF16, "rows")]
+          (100, 512, 3000, 0, BF16, "rows"), (128, 320, 40000, 0, BF16, "rows"), (128, 320, 40001, 9, BF16, "tied"), (700, 256, 30000, 33, BF16, "rows"),
+          (3, 24, 270001, 6, F32, "rows"), (2, 16, 600001, 3, BF16, "rows"), (130, 16, 140000, 20, BF16, "tied")]
 
 
 @gpu
@@ -368,6 +369,28 @@ def test_f32_gradient_whose_largest_term_comes_first(cdl, gpu_ok, t):
     o = cdl.ops.linear_cross_entropy(x, w, targets)
     _, _, _, dx, _ = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
     assert ((o.dx - dx).norm() / dx.norm()).item() <= 26 * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 4, 5, 16, 17])
+@pytest.mark.parametrize("d,v,layout", [(1100, 9003, "rows"), (1101, 9002, "tied"), (515, 130, "rows"), (3, 700, "tied"), (1030, 2049, "strided")])
+def test_f32_losses_of_few_tokens(cdl, gpu_ok, t, d, v, layout):
+    """Rows anywhere, K slices and none, gradients that are written and added to, d x in place of x."""
+    gen = torch.Generator(device="cuda").manual_seed(t + v)
+    x, w = _operands(gen, t, d, v, F32, layout)
+    rows, cols = (v, d) if layout == "tied" else (d, v)
+    buffer = torch.randn(rows, cols + 3, generator=gen, device="cuda") * 0.01
+    kept = buffer.clone()
+    dw = buffer[:, 2:2 + cols].t() if layout == "tied" else buffer[:, 2:2 + cols]
+    before = dw.clone()
+    entries = _entries(gen, t, v, 0)
+    _check_linear(cdl, x, w, entries, cdl.ops.LinearLossOpts(accumulate=True), dw=dw, before=before)
+    assert torch.equal(buffer[:, :2], kept[:, :2]) and torch.equal(buffer[:, -1], kept[:, -1])
+    o = _check_linear(cdl, x, w, _entries(gen, t, v, min(v, 40)), cdl.ops.LinearLossOpts(temperature=1.4))
+    y = x.clone(memory_format=torch.contiguous_format)
+    p = cdl.ops.linear_cross_entropy(y, w, *entries)
+    q = cdl.ops.linear_cross_entropy(y, w, *entries, dx=y)
+    assert q.dx.data_ptr() == y.data_ptr() and torch.equal(p.dx, q.dx) and torch.equal(p.dw, q.dw) and o.dw is not None
 
 
 @gpu
