@@ -934,7 +934,7 @@ __global__ void __launch_bounds__(256) keep_kernel(const Entries src, long long 
 // ------------------------------------------------------------------------------------------ few rows of f32 operands
 // Up to FEW_ROWS tokens an f32 product reads w once, as it is, and multiplies in f32, two tokens per instruction: 2 T operations per 4
 // bytes, at 16 tokens a third of what the SMs do while HBM brings the bytes.  (The pieces of w alone are 2.5 times its
-// bytes, written and read by three products: 4 x 2048 x 112256 1546 us, 492 so; 16 tokens 1538 and 820.)  TT tokens are a
+// bytes, written and read by three products: 4 x 2048 x 112256 1546 us, 492 so; 8 tokens 1568 and 574, 16 tokens 1538 and 820.)  TT tokens are a
 // thread's accumulators; those behind the last are zeros.  Any alignment: lanes have neighbouring elements.
 constexpr int FEW_ROWS = 16, FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
 constexpr int FEW_CHUNK = 512;      // of K in shared memory at a time
@@ -960,7 +960,7 @@ __device__ __forceinline__ void few_columns(float* s, const float* a, long long 
 
 // out[slice][t, n] = sum over the slice's k of a[t, k] b[k, n]: a block has 128 columns, a lane four of them, the warps every eighth k.
 template <int TT>
-__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
+__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : TT == 8 ? 3 : 2)
     few_outer_kernel(const float* a, long long lda, const float* b, long long ldb, int T, int K, int N, int slices, float* out, long long ldo,
                      long long plane) {
   __shared__ __align__(16) float s_a[FEW_CHUNK * TT];
@@ -1038,7 +1038,7 @@ __global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
 
 // out[slice][t, n] = sum over the slice's k of a[t, k] b[n, k]: a warp has four n, its lanes neighbouring k.
 template <int TT>
-__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
+__global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : TT == 8 ? 3 : 2)
     few_inner_kernel(const float* a, long long lda, const float* b, long long ldb, int T, int K, int N, int slices, float* out, long long ldo,
                      long long plane) {
   __shared__ __align__(16) float2 s_a[TT / 2][FEW_CHUNK];
@@ -1091,7 +1091,7 @@ __global__ void __launch_bounds__(FEW_THREADS, TT == 4 ? 4 : 2)
     }
   }
   // Sums over the lanes: in each step a lane keeps one half of its pairs and gives the other away; then it has pair lane of TT * 2, or
-  // (TT = 4) four lanes the same one.
+  // (fewer tokens) two or four lanes the same one.
   int left = TT * 2;
   uint64_t* flat = &acc[0][0];
   auto other = [](uint64_t v, int o) { return __shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(v), o); };
@@ -1434,10 +1434,11 @@ static long long choose_chunk(long long T, long long V, long long bytes_per_logi
   return up((T + chunks - 1) / chunks, 256);
 }
 
-// K slices of a product of few rows: as many as give four blocks per SM, of 512 and more.
+// K slices of a product of few rows, of 512 and more: where there are fewer than four blocks per SM as many as give twelve (two to
+// four run at once, and the last ones alone: 5 x 3198 x 102440 with slices for four 912 us, for twelve 792).
 static int few_slices(bool inner, long long K, long long N) {
   const int cols = inner ? FEW_INNER_COLS : FEW_OUTER_COLS;
-  const long long blocks = (N + cols - 1) / cols, want = 4LL * sm_count() / blocks, most = K / FEW_CHUNK;
+  const long long blocks = (N + cols - 1) / cols, want = blocks < 4 * sm_count() ? 12LL * sm_count() / blocks : 1, most = K / FEW_CHUNK;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : s > MAX_PLANES ? MAX_PLANES : static_cast<int>(s);
 }
@@ -1646,6 +1647,7 @@ static int32_t few_product(const Linear& p, const float* a, long long lda, const
     return CDL_OK;
   };
   if (p.T <= 4) CDL_CHECK(inner ? run(few_inner_kernel<4>) : run(few_outer_kernel<4>));
+  else if (p.T <= 8) CDL_CHECK(inner ? run(few_inner_kernel<8>) : run(few_outer_kernel<8>));
   else CDL_CHECK(inner ? run(few_inner_kernel<16>) : run(few_outer_kernel<16>));
   return slices > 1 ? sum_planes(to, ldo, plane, slices, out, 0, stream) : CDL_OK;
 }
@@ -1675,7 +1677,7 @@ static int32_t few_execute(Linear& p, const cdl_head_loss_desc* desc, const Entr
                           static_cast<long long>(d.stride[0]), groups, desc->accumulate_dw));
       return CDL_OK;
     };
-    CDL_CHECK(T <= 4 ? run(few_update_kernel<4>) : run(few_update_kernel<16>));
+    CDL_CHECK(T <= 4 ? run(few_update_kernel<4>) : T <= 8 ? run(few_update_kernel<8>) : run(few_update_kernel<16>));
   }
   if (p.has_dx) CDL_CHECK(few_product(p, g, p.ld_g, w_near, !wc, p.slices_dx, p.dx, base, stream));
   return CDL_OK;

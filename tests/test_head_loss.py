@@ -372,7 +372,7 @@ def test_f32_gradient_whose_largest_term_comes_first(cdl, gpu_ok, t):
 
 
 @gpu
-@pytest.mark.parametrize("t", [1, 4, 5, 16, 17])
+@pytest.mark.parametrize("t", [1, 4, 5, 8, 9, 16, 17])
 @pytest.mark.parametrize("d,v,layout", [(1100, 9003, "rows"), (1101, 9002, "tied"), (515, 130, "rows"), (3, 700, "tied"), (1030, 2049, "strided")])
 def test_f32_losses_of_few_tokens(cdl, gpu_ok, t, d, v, layout):
     """Rows anywhere, K slices and none, gradients that are written and added to, d x in place of x."""
