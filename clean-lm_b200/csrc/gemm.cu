@@ -1923,6 +1923,7 @@ int matmul_plane_slices(long long M, long long N, long long K, bool pieces) {
   for (int s = 1; s == 1 || (s <= MAX_PLANES && s * (pieces ? 2 : 8) <= k_blocks); ++s) {
     const double waves = static_cast<double>((tiles * s + slots - 1) / slots);
     double t = waves * (0.28 * (pieces ? PIECE_PRODUCTS : 1) * static_cast<double>((k_blocks + s - 1) / s) + 4.0);
+    if (pieces && (k_blocks + s - 1) / s > PART) t += 2.0;  // the parts' sum, at its end
     if (s > 1) t = 1.05 * (t + 3.0 + 8e-6 * static_cast<double>(s) * M * N / 5.0);
     if (t < least) {
       least = t;
