@@ -348,7 +348,7 @@ def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
     elif dw is None:
         dw = torch.empty_like(w)  # (in w's order of strides)
     device, tokens, distil = x.device, x.shape[0], len(entries) > 1
-    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=device).unbind()
+    loss, lse = torch.empty(tokens, dtype=torch.float32, device=device), torch.empty(tokens, dtype=torch.float32, device=device)
     desc = _lib.head_loss_bytes(opts.temperature, opts.grad_scale, 1 if opts.accumulate else 0, int(opts.chunk_rows))
     tx, tw, tdx, tdw = tensor_bytes(x), tensor_bytes(w), tensor_bytes(dx), tensor_bytes(dw)
     if scratch is None:
@@ -414,8 +414,8 @@ def distillation(logits, teacher_ids, teacher_logits, opts: DistillationOpts | N
         raise _lib.CdlError(-1, "distillation: logits must be [tokens, vocab]")
     d_loss = opts.d_loss
     _require_current_device(logits, teacher_ids, teacher_logits, d_loss, d_logits)
-    tokens = logits.shape[0]
-    loss, lse = torch.empty(2, tokens, dtype=torch.float32, device=logits.device).unbind()
+    tokens, device = logits.shape[0], logits.device
+    loss, lse = torch.empty(tokens, dtype=torch.float32, device=device), torch.empty(tokens, dtype=torch.float32, device=device)
     if not opts.grad:
         d_logits = None
     elif d_logits is None:
