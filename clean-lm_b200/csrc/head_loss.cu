@@ -934,7 +934,7 @@ __global__ void __launch_bounds__(256) keep_kernel(const Entries src, long long 
 // ------------------------------------------------------------------------------------------ few rows of f32 operands
 // Up to FEW_ROWS tokens an f32 product reads w once, as it is, and multiplies in f32, two tokens per instruction: 2 T operations per 4
 // bytes, at 16 tokens a third of what the SMs do while HBM brings the bytes.  (The pieces of w alone are 2.5 times its
-// bytes, written and read by three products: 4 x 2048 x 112256 1546 us, 492 so; 8 tokens 1568 and 574, 16 tokens 1538 and 820.)  TT tokens are a
+// bytes, written and read by three products: 4 x 2048 x 112256 1546 us, 492 so; 8 tokens 1568 and 562, 16 tokens 1538 and 844.)  TT tokens are a
 // thread's accumulators; those behind the last are zeros.  Any alignment: lanes have neighbouring elements.
 constexpr int FEW_ROWS = 16, FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
 constexpr int FEW_CHUNK = 512;      // of K in shared memory at a time
