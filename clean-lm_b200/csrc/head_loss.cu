@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   if (g.ptr != nullptr) {
     T* y = PIECES ? nullptr : static_cast<T*>(g.ptr) + row * g.ld;
     const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f;
-    const float factor = ex2(c * (own - base)) * (scale / s);
+    // (a slice of nothing but -inf: 0 wherever the others lie; NaN where the row is)
+    const float factor = (m == -INFINITY ? 0.f : ex2(c * (own - base))) * (scale / s);
     const bool in_step = PIECES ? lead == 0 : static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) == lead * static_cast<int>(sizeof(T));
     const int at0 = lane * VEC - first;  // the row's element at the lane's first vector
     const uint64_t f2 = pack_f2(factor, factor);
