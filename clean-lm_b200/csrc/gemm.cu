@@ -617,11 +617,13 @@ struct Wanted {
   }
 };
 
-// The store of a loss's logits for the calling warp, 32 rows and a piece of 128 columns, t = alpha * product in the base-2
-// domain (alpha = log2(e) / temperature).  The logits stay here: what leaves is, per row, M' = max t - 15 and S' = sum 2^(t - M'),
-// t itself at the row's ids, and (with a gradient to come) the exponentials 2^(t - M') in f16.  Those are at most 2^15,
+// The store of a loss's logits z for the calling warp, 32 rows and a piece of 128 columns (alpha = log2(e) / temperature).
+// The logits stay here: what leaves is, per row, M = max z and S = sum 2^(alpha (z - M) + 15), z itself at the
+// row's ids, and (with a gradient to come) those exponentials in f16.  They are at most 2^15,
 // so they keep f16's 11 bits down to 2^-29 of the piece's largest: bf16's 8 would round the gradient a second time as
-// coarsely as its own rounding does.  128 accumulators at a time are a thread's registers: one read of the tensor memory.
+// coarsely as its own rounding does.  Differences are taken before they are scaled: from |alpha z| = 2^24 the product's last
+// place is 2 and more, which would carry exponentials beyond f16.  128 accumulators at a time are a thread's registers: one
+// read of the tensor memory.
 // Up to a K of about 1000 these warps, not the products, set the pace.  Packed arithmetic, and (TMA) the exponentials stored
 // as two boxes of 32 x 64 from the warp's 4 KiB buffer instead of 32 bytes of 32 rows per instruction: 8192 x 512
 // x 32768 271 -> 226 us.
@@ -649,7 +651,7 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
       if (!__any_sync(0xffffffffu, has)) break;
       const uint32_t v = pick32(r[c], want.id & 31);
       if (has) {
-        p.exp.at[row * p.exp.ids_ld + want.e] = p.alpha * __uint_as_float(v);
+        p.exp.at[row * p.exp.ids_ld + want.e] = __uint_as_float(v);
         if (++want.e < want.end) want.id = p.exp.ids[row * p.exp.ids_ld + want.e];
       }
     }
@@ -659,9 +661,8 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int j = 0; j < 32; j += 2) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1])));
-  const float m = p.alpha * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-  const float base = (m == -INFINITY ? 0.f : m) - 15.f;
-  const F32x2 scale(p.alpha, p.alpha), from(-base, -base);
+  const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), base = m == -INFINITY ? 0.f : m;
+  const F32x2 scale(p.alpha, p.alpha), from(-base, -base), off(15.f, 15.f);
   F32x2 s[2] = {F32x2(0.f, 0.f), F32x2(0.f, 0.f)};
   __half* dp = static_cast<__half*>(p.d) + static_cast<long long>(row) * p.ldd + col_base;
   const bool store = p.d != nullptr;
@@ -671,7 +672,7 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
     uint32_t w[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const F32x2 t = fma2(F32x2(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), scale, from);
+      const F32x2 t = fma2(add2(F32x2(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), from), scale, off);
       float e0, e1;
       t.get(e0, e1);
       asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
@@ -707,8 +708,7 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
   float a0, a1, b0, b1;
   s[0].get(a0, a1);
   s[1].get(b0, b1);
-  p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] =
-      make_float2(m == -INFINITY ? -INFINITY : base, (a0 + a1) + (b0 + b1));
+  p.exp.stats[static_cast<long long>(row) * p.exp.pieces + (col_base >> 7)] = make_float2(m, (a0 + a1) + (b0 + b1));
 }
 
 // One kernel per kind of store.  All of them in one, with the buffers that the plain ones do not need (they take room
@@ -1885,6 +1885,11 @@ static int32_t one_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtens
   return CDL_OK;
 }
 
+// A tensor-core accumulator truncates: the sum of n steps of 16 products lies about 1.6e-8 n below its value (measured in
+// gemm_general.cu).  Put back, the loss of a trained head is 1.7e-7 off at K = 2048 and 4.3e-7 at 4096 (2-norm, against
+// f64; f32 products 1.9e-7 and 4.1e-7), without it 7.5e-7 and 2.0e-6.
+float matmul_exp_scale(float scale, long long K) { return static_cast<float>(scale * (1.0 + 1e-9 * static_cast<double>(K))); }
+
 // The logits of a loss (see store_tile_rows_exp).  Up to 128 rows one CTA per 256 columns: a pair's second half would have no
 // rows but take as long over its products, which then, not the bytes of B, set the time (64 x 2048 x 32768 40 -> 32 us).
 int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
@@ -1895,10 +1900,7 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
   CDL_CHECK(wide_operands(a, b, p, &tm_a, &tm_b, pair));
   p.d = d;
   p.ldd = ldd;
-  // A tensor-core accumulator truncates: the sum of n steps of 16 products lies about 1.6e-8 n below its value (measured in
-  // gemm_general.cu).  Put back, the loss of a trained head is 1.7e-7 off at K = 2048 and 4.3e-7 at 4096 (2-norm, against
-  // f64; f32 products 1.9e-7 and 4.1e-7), without it 7.5e-7 and 2.0e-6.
-  p.alpha = static_cast<float>(scale * (1.0 + 1e-9 * p.K));
+  p.alpha = scale;
   p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
   CUtensorMap tm_d = tm_a;  // (a valid map where none is used)
   if (pair && d != nullptr) {

@@ -10,11 +10,11 @@ constexpr int RASTER_W = 8;  // N tiles per raster panel (upper bound; see Param
 
 // The store of the losses' logits (pair kernel): see store_tile_rows_exp in gemm.cu.  A piece is 128 columns.
 struct ExpStore {
-  float2* stats;  // [rows][pieces]: (M', S') of every row and piece
-  const int* ids;  // the columns whose t is wanted besides: [rows][ids_ld], ascending
+  float2* stats;  // [rows][pieces]: (M, S) of every row and piece
+  const int* ids;  // the columns whose logit is wanted besides: [rows][ids_ld], ascending
   long long ids_ld;
   const unsigned short* first;  // [rows][pieces + 1]: a row's first id at or behind a piece's columns; nullptr: one id, not sorted
-  float* at;                    // t at the ids, [rows][ids_ld]
+  float* at;                    // the logits at the ids, [rows][ids_ld]
   int pieces;
 };
 

@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
 }
 
 // ------------------------------------------------------------------------------------------ rows behind the fused product
-// (matmul_exp_execute in gemm.cu: per row and piece of 128 columns M' and S', the exponentials 2^(t - M') in f16, t at the
+// (matmul_exp_execute in gemm.cu: per row and piece of 128 columns M and S, the exponentials 2^(c (z - M) + 15) in f16, z at the
 // entries' ids.)
 
 // What the product and the row kernel read of a row's entries.
@@ -636,14 +636,14 @@ constexpr int PIECES_PER_WARP = 64;  // at most: 8192 columns
 constexpr int ROWS_PER_CTA = 8;      // a warp's each
 
 // From the pieces' statistics the rows': loss, lse, and (with gradients) the gradient of the logits in bf16 in place of the
-// exponentials, which are only multiplied with 2^(M' - M) s tau / S; the rows of x for the weight gradient's product,
+// exponentials, which are only multiplied with 2^(c (M - the row's)) s tau / S; the rows of x for the weight gradient's product,
 // zeros where a row does not count.  GRAD_TWICE: what bf16 rounds away, in bf16 `rows` rows further on, and the rows of x again
 // there: see Linear::twice.  Grid (rows / 8, pieces / per), a row and `per` pieces per warp; the warps have nothing
 // to wait for in one another.
 enum RowsMode { LOSS_ONLY, GRAD_ONCE, GRAD_TWICE };
 template <int MODE>
 __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
-    softmax_rows_kernel(const float2* stats, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
+    softmax_rows_kernel(const float2* stats, float c, __nv_bfloat16* e, long long ld_e, int rows, int vocab, int pieces, int per,
                         int K, const Prepared src, const RowTerms terms, const __nv_bfloat16* x, long long ld_x, __nv_bfloat16* clean,
                         long long ld_clean, int cols) {
   constexpr bool GRAD = MODE != LOSS_ONLY;
@@ -669,32 +669,32 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, v[j].x);
     const float from = top == -INFINITY ? 0.f : top;
-    S *= ex2(m - from);
+    S *= ex2(c * (m - from));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) S += v[j].y * ex2(v[j].x - from);
+    for (int j = 0; j < 8; ++j) S += v[j].y * ex2(c * (v[j].x - from));
     m = top;
   }
   const float top = warp_max(m);
   const float base = top == -INFINITY ? 0.f : top;
-  S = warp_sum(S * ex2(m - base));
-  const float log2_s = log2f(S);
+  S = warp_sum(S * ex2(c * (m - base)));  // (2^15 times the sum)
+  const float log2_s = log2f(S) - 15.f;
   const bool counts = entries > 0;
   if (blockIdx.y == 0) {
     float cross = 0.f;  // sum_k p_k log2 q_k
     for (int k = lane; k < entries; k += 32) {
       const float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
-      if (p != 0.f) cross += p * ((src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
+      if (p != 0.f) cross += p * (c * (src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
     }
     cross = warp_sum(cross);
     if (lane == 0) {
       const float entropy = src.p == nullptr ? 0.f : src.p_log_p[row];
       terms.loss[row] = counts ? terms.tau * terms.tau * (entropy - LN2 * cross) : 0.f;
-      if (terms.lse) terms.lse[row] = LN2 * (base + log2_s);
+      if (terms.lse) terms.lse[row] = LN2 * (c * base + log2_s);
     }
   }
   if (!GRAD) return;
   const float scale = counts ? terms.grad_scale * terms.tau * d_loss : 0.f, over_s = scale / S;
-  for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(stats[i].x - base) * over_s;
+  for (int i = piece0 + lane; i < piece1; i += 32) factor[warp][i - piece0] = ex2(c * (stats[i].x - base)) * over_s;
   __syncwarp();
   uint4* at = reinterpret_cast<uint4*>(e + row * ld_e + piece0 * 128);
   uint4* rest = reinterpret_cast<uint4*>(e + (static_cast<long long>(rows) + row) * ld_e + piece0 * 128);
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
     if (src.first == nullptr ? id / 128 < piece0 || id / 128 >= piece1 : k > k0 && ids[k - 1] == id) continue;
     float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
     for (int i = k + 1; i < k1 && ids[i] == id; ++i) p += src.p[static_cast<long long>(row) * K + i];
-    const float g = scale * (ex2(src.at[static_cast<long long>(row) * K + k] - base) / S - p);
+    const float g = scale * (ex2(c * (src.at[static_cast<long long>(row) * K + k] - base) + 15.f) / S - p);
     const __nv_bfloat16 hi = __float2bfloat16_rn(g);
     e[row * ld_e + id] = hi;
     if (MODE == GRAD_TWICE) e[(static_cast<long long>(rows) + row) * ld_e + id] = __float2bfloat16_rn(g - __bfloat162float(hi));
@@ -1584,12 +1584,13 @@ static int32_t fused_rows(const Linear& p, const cdl_tensor& x, const cdl_tensor
   if (teacher)
     CDL_CHECK(prepare_entries(e, rows, vocab, t.tau, p.pieces, ids, first, probs, p_log_p, stream));
   void* out = grad ? base + p.at_g : nullptr;
-  CDL_CHECK(matmul_exp_execute(&x, &w, LOG2E / t.tau, out, p.ld_g, {stats, src.ids, src.ids_ld, src.first, at}, stream));
+  const float c = matmul_exp_scale(LOG2E / t.tau, p.D);
+  CDL_CHECK(matmul_exp_execute(&x, &w, c, out, p.ld_g, {stats, src.ids, src.ids_ld, src.first, at}, stream));
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(rows) * vocab * (grad ? 4 : 0) + 8.0 * rows * p.pieces, stream);
   const dim3 block(ROWS_PER_CTA * 32);
   const unsigned row_ctas = (rows + ROWS_PER_CTA - 1) / ROWS_PER_CTA;
   auto run = [&](auto kernel, unsigned splits, int per) {
-    return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
+    return launch_pdl(kernel, dim3(row_ctas, splits), block, 0, stream, stats, c, static_cast<__nv_bfloat16*>(out), p.ld_g, rows,
                       vocab, p.pieces, per, e.K, src, t, static_cast<const __nv_bfloat16*>(x.ptr), static_cast<long long>(x.stride[0]),
                       p.has_dw ? static_cast<__nv_bfloat16*>(clean.ptr) : nullptr, static_cast<long long>(clean.stride[0]),
                       static_cast<int>(p.D));

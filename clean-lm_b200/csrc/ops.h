@@ -44,16 +44,18 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
                            cudaStream_t stream, const cdl_matmul_options* opts = nullptr,
                            const RopeEpilogue* rope = nullptr, void* scratch = nullptr, size_t scratch_bytes = 0,
                            int early = 0);
-// The logits of a loss, t = scale * (A . B), of which statistics, exponentials and single values are stored (bf16 operands
-// on the 16-byte grid; see store_tile_rows_exp in gemm.cu).
+// The logits of a loss, A . B, of which statistics, exponentials of scale * (logit - maximum) and single values are stored (bf16
+// operands on the 16-byte grid; see store_tile_rows_exp in gemm.cu).
 struct ExpOutputs {
   float2* stats;  // [rows][pieces of 128 columns]
-  const int* ids;  // columns whose t is stored besides, [rows][ids_ld]; nullptr: none
+  const int* ids;  // columns whose logit is stored besides, [rows][ids_ld]; nullptr: none
   long long ids_ld;
   const unsigned short* first;  // [rows][pieces + 1], nullptr: one id per row
   float* at;                    // [rows][ids_ld]
 };
 // d: f16 [rows, ldd], 32-byte aligned, ldd a multiple of 128 that holds all columns; nullptr: no exponentials.
+// matmul_exp_scale: the scale to pass for a sum of K products, and to use on what is stored.
+float matmul_exp_scale(float scale, long long K);
 int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale, void* d, long long ldd, const ExpOutputs& out,
                            cudaStream_t stream);
 // A product of bf16 tensors on the 16-byte grid in K slices: slice s is stored at planes + s M ld (f32, 32-byte aligned, ld >= N a

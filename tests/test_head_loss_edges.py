@@ -1,9 +1,10 @@
-"""Losses of the head where values are extreme: whole slices of a row masked.  The restatements in 64 bits are those of
-test_head_loss.py; tolerances are derived where they stand."""
+"""Losses of the head where values are extreme: whole slices of a row masked, differences of logits that a temperature makes
+large.  The restatements in 64 bits are those of test_head_loss.py; tolerances are derived where they stand."""
 import pytest
 import torch
 
-from test_head_loss import BF16, F32, _check_distillation
+from oracle import head_loss_ref as ref
+from test_head_loss import BF16, F32, HALF, _check_distillation, _close, _hit, _stat
 
 gpu = pytest.mark.gpu
 
@@ -35,3 +36,54 @@ def test_distillation_slices_without_a_logit(cdl, gpu_ok, dtype, vocab, pad, tau
     o = cdl.ops.distillation(logits, ids, teacher, cdl.ops.DistillationOpts(temperature=tau))
     assert bool(torch.isnan(o.d_logits[5:]).all()) and bool(torch.isnan(o.loss[5:]).all())
     assert bool(torch.isfinite(o.d_logits[:5]).all())
+
+
+@gpu
+@pytest.mark.parametrize("t,v,layout", [(40, 1000, "rows"), (100, 5000, "tied"), (300, 4099, "rows"), (513, 1000, "tied")])
+@pytest.mark.parametrize("tau,far", [(1e-6, 1.0), (1e-4, 1.0), (0.5, 2.0 ** 19), (1.0, 2.0 ** 20), (1e6, 2.0 ** 27)])
+def test_linear_losses_of_far_logits(cdl, gpu_ok, t, v, layout, tau, far):
+    """bf16 operands whose logits are sums of two values, b + k u with u near 4 tau, that 24 bits hold: exact in any order of
+    summation, so that all errors are the loss's own.  |z| log2(e) / tau reaches 2^25, where the last place is 4, and the
+    softmax is set by differences of a few u.
+
+    Differences are exact; times log2(e) / tau, a factor off by 2^-22, those that count (probabilities above 2^-40) are off by 40 2^-22 =
+    2^-17 at most in the exponent, so a probability by 2^-17 of itself, and from its sum by what _stat has.  d z is rounded to f16 and
+    bf16 (2 * 2^-8)."""
+    gen = torch.Generator(device="cuda").manual_seed(t + v)
+    u = 2.0 ** round(torch.log2(torch.tensor(4 * tau)).item())
+    coarse = torch.tensor([0.0, 12.0, -12.0, 24.0, -24.0, 30.0, -30.0, 28.0]) * far
+    d = 64
+    w = torch.randint(-64, 65, (d, v), generator=gen, device="cuda") * u
+    w[:8] = coarse.cuda()[:, None]
+    x = torch.zeros(t, d, device="cuda")
+    rows = torch.arange(t, device="cuda")
+    x[rows, rows % 8] = 1.0
+    x[rows, torch.randint(8, d, (t,), generator=gen, device="cuda")] = 1.0
+    x, w = x.to(BF16), w.to(BF16)
+    assert torch.equal((x.double() @ w.double()).float().double(), x.double() @ w.double())
+    if layout == "tied":
+        w = w.t().contiguous().t()
+    k = 20
+    ids = torch.randint(0, v, (t, k), generator=gen, device="cuda", dtype=torch.int32)
+    teacher = torch.randn(t, k, generator=gen, device="cuda") * 2 * tau
+    ids[3:5, 1] = ids[3:5, 0]
+    ids[5] = -1
+    best = (x.double() @ w.double()).argmax(1).to(torch.int32)
+    ids[6::5, 2] = best[6::5]
+    forms = [((ids, teacher), cdl.ops.linear_distillation, lambda z: ref.distillation(z, ids, teacher, tau))]
+    if tau == 1.0:
+        targets = torch.where(rows % 3 == 0, best, ids[:, 3])
+        forms.append(((targets,), cdl.ops.linear_cross_entropy, lambda z: ref.cross_entropy(z, targets)))
+    for entries, fn, loss_of in forms:
+        loss, lse, g, dx, dw = ref.linear(x, w, loss_of)
+        o = fn(x, w, *entries, cdl.ops.LinearLossOpts(temperature=tau))
+        _close("lse", o.lse, lse, 3 * _stat(v) + 2.0 ** -21 * lse.abs())
+        # log q at an entry is a difference of up to 2 * 64 u = 512 tau or so: 2^-21 of it
+        _close("loss", o.loss, loss, tau * tau * (6 * _stat(v) + 2.0 ** -21 * 1200 + 0 * loss))
+        hit = _hit(entries[0] if len(entries) > 1 else entries[0][:, None], v)
+        keep = (g != 0).any(1)[:, None]
+        p_err = 2 * (_stat(v) + 2.0 ** -17)
+        g_err = torch.where(keep, 2 * HALF[BF16] * g.abs() + p_err * (g.abs() + tau * hit) + 2.0 ** -30 * tau, 0.0)
+        sums = 2.0 ** -23 * 40
+        _close("dx", o.dx, dx, (g_err + sums * g.abs()) @ w.double().abs().t() + HALF[BF16] * dx.abs() + 1e-30)
+        _close("dw", o.dw, dw, x.double().abs().t() @ (g_err + sums * g.abs()) + (HALF[BF16] + 2.0 ** -22) * dw.abs() + 1e-30)
