@@ -723,14 +723,26 @@ constexpr int PIECE_PRODUCTS = 6;
 __device__ __forceinline__ int piece_of_a(int i) { return 0x210100 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
 __device__ __forceinline__ int piece_of_b(int i) { return 0x012010 >> (4 * (PIECE_PRODUCTS - 1 - i)) & 3; }
 
-// An accumulator takes PART K blocks of all products; the parts of a slice are added by the epilogue, in registers, rounded to
+// An accumulator takes PART K blocks of all products of pieces; the parts of a slice are added by the epilogue, in registers, rounded to
 // nearest. A tensor-core accumulator truncates, and a large term that comes early (a target's column in dx) loses a bit in every step
 // after it: with 1800 of K in one accumulator dx of 159 x 576 x 43584 was 1.3e-6 off.
 constexpr int PART = 4;
+// A loss's logits: an accumulator takes up to LOGIT_PART K blocks (Params::part, all parts alike).  A sum of positive terms loses 1e-5 of
+// itself over 4096 of K, but 6.8e-3 over 2^20 in one accumulator.
+constexpr int LOGIT_PART = 64;
 template <int KIND>
-__device__ __forceinline__ int part_end(int from, int kb1) { return KIND == STORE_PIECES ? min(from + PART, kb1) : kb1; }
+constexpr bool in_parts = KIND == STORE_PIECES || KIND == STORE_EXP;
 template <int KIND>
-__device__ __forceinline__ int num_parts(int kb0, int kb1) { return KIND == STORE_PIECES ? (kb1 - kb0 + PART - 1) / PART : 1; }
+__device__ __forceinline__ int part_blocks(const Params& p) { return KIND == STORE_PIECES ? PART : p.part; }
+template <int KIND>
+__device__ __forceinline__ int part_end(const Params& p, int from, int kb1) {
+  return in_parts<KIND> ? min(from + part_blocks<KIND>(p), kb1) : kb1;
+}
+template <int KIND>
+__device__ __forceinline__ int num_parts(const Params& p, int kb0, int kb1) {
+  if constexpr (!in_parts<KIND>) return 1;
+  return (kb1 - kb0 + part_blocks<KIND>(p) - 1) / part_blocks<KIND>(p);
+}
 
 // 128 columns of a warp's rows, sum += accumulator.
 __device__ __forceinline__ void add_part(float (&sum)[8][16], uint32_t t_row) {
@@ -837,9 +849,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         unit_range(unit, tile, slice, kb0, kb1);
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * BM, n0 = tn * BN;
-        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(from, kb1))
+        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(p, from, kb1))
         for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
-        for (int kb = from; kb < part_end<KIND>(from, kb1); ++kb, ++it) {
+        for (int kb = from; kb < part_end<KIND>(p, from, kb1); ++kb, ++it) {
           const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
@@ -880,7 +892,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x) {
         int tile, slice, kb0, kb1;
         unit_range(unit, tile, slice, kb0, kb1);
-        for (int part = 0; part < num_parts<KIND>(kb0, kb1) && ok; ++part, ++t) {
+        for (int part = 0; part < num_parts<KIND>(p, kb0, kb1) && ok; ++part, ++t) {
           const int acc = t & 1;
           const uint32_t acc_ph = (t >> 1) & 1;
           if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 201)) {
@@ -889,8 +901,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * BN;
-          const int from = kb0 + part * PART;
-          const int blocks = KIND == STORE_PIECES ? (part_end<KIND>(from, kb1) - from) * PIECE_PRODUCTS : kb1 - kb0;
+          const int from = kb0 + part * part_blocks<KIND>(p);
+          const int blocks = in_parts<KIND> ? (part_end<KIND>(p, from, kb1) - from) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) : kb1 - kb0;
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int s = it % STAGES;
             const uint32_t ph = (it / STAGES) & 1;
@@ -935,7 +947,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->acc_empty[n & 1]);
       };
-      if (!(KIND == STORE_PIECES ? sum_parts(num_parts<KIND>(kb0, kb1), t, t_lane, full, give) : full(t))) break;
+      if (!(in_parts<KIND> ? sum_parts(num_parts<KIND>(p, kb0, kb1), t, t_lane, full, give) : full(t))) break;
       const uint32_t t_row = t_lane + (t & 1) * BN;
       const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
       if constexpr (KIND == STORE_EXP) {
@@ -1128,9 +1140,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tile_coords(p, tile, b, tm, tn);
         const int m0 = tm * PAIR_M + static_cast<int>(rank) * BM;
         const int n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
-        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(from, kb1))
+        for (int from = kb0; from < kb1 && ok; from = part_end<KIND>(p, from, kb1))
         for (int product = 0; product < (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) && ok; ++product)
-        for (int kb = from; kb < part_end<KIND>(from, kb1); ++kb, ++it) {
+        for (int kb = from; kb < part_end<KIND>(p, from, kb1); ++kb, ++it) {
           const int ba = KIND == STORE_PIECES ? piece_of_a(product) : b, bb = KIND == STORE_PIECES ? piece_of_b(product) : b;
           const int s = it % PAIR_STAGES;
           const uint32_t ph = (it / PAIR_STAGES) & 1;
@@ -1178,7 +1190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int unit = static_cast<int>(unit_u);
         int tile, slice, kb0, kb1;
         unit_range(unit, tile, slice, kb0, kb1);
-        for (int part = 0; part < num_parts<KIND>(kb0, kb1) && ok; ++part, ++a) {
+        for (int part = 0; part < num_parts<KIND>(p, kb0, kb1) && ok; ++part, ++a) {
           const int acc = a & 1;
           const uint32_t acc_ph = (a >> 1) & 1;
           if (!mbar_wait(&bars->acc_empty[acc], acc_ph ^ 1, abort_word, 211)) {
@@ -1187,8 +1199,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * BN;
-          const int from = kb0 + part * PART;
-          const int blocks = KIND == STORE_PIECES ? (part_end<KIND>(from, kb1) - from) * PIECE_PRODUCTS : kb1 - kb0;
+          const int from = kb0 + part * part_blocks<KIND>(p);
+          const int blocks = in_parts<KIND> ? (part_end<KIND>(p, from, kb1) - from) * (KIND == STORE_PIECES ? PIECE_PRODUCTS : 1) : kb1 - kb0;
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int s = it % PAIR_STAGES;
             const uint32_t ph = (it / PAIR_STAGES) & 1;
@@ -1250,7 +1262,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[n & 1]), 0));
       };
-      if (!(KIND == STORE_PIECES ? sum_parts(num_parts<KIND>(kb0, kb1), a, t_lane, full, give) : full(a))) break;
+      if (!(in_parts<KIND> ? sum_parts(num_parts<KIND>(p, kb0, kb1), a, t_lane, full, give) : full(a))) break;
       const uint32_t t_row = t_lane + (a & 1) * BN;
       if constexpr (KIND == STORE_ADD) {
         add_tile_rows(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
@@ -1886,9 +1898,16 @@ static int32_t one_launch(gemm::Params& p, const CUtensorMap& tm_a, const CUtens
 }
 
 // A tensor-core accumulator truncates: the sum of n steps of 16 products lies about 1.6e-8 n below its value (measured in
-// gemm_general.cu).  Put back, the loss of a trained head is 1.7e-7 off at K = 2048 and 4.3e-7 at 4096 (2-norm, against
+// gemm_general.cu), up to the 256 steps of LOGIT_PART.  Put back, the loss of a trained head is 1.7e-7 off at K = 2048 and 4.3e-7 at 4096 (2-norm, against
 // f64; f32 products 1.9e-7 and 4.1e-7), without it 7.5e-7 and 2.0e-6.
-float matmul_exp_scale(float scale, long long K) { return static_cast<float>(scale * (1.0 + 1e-9 * static_cast<double>(K))); }
+static int logit_part(long long K) {  // K blocks of an accumulator
+  const long long blocks = (K + gemm::BK - 1) / gemm::BK, parts = (blocks + gemm::LOGIT_PART - 1) / gemm::LOGIT_PART;
+  return static_cast<int>((blocks + parts - 1) / parts);
+}
+float matmul_exp_scale(float scale, long long K) {
+  const long long part = static_cast<long long>(logit_part(K)) * gemm::BK;
+  return static_cast<float>(scale * (1.0 + 1e-9 * static_cast<double>(K < part ? K : part)));
+}
 
 // The logits of a loss (see store_tile_rows_exp).  Up to 128 rows one CTA per 256 columns: a pair's second half would have no
 // rows but take as long over its products, which then, not the bytes of B, set the time (64 x 2048 x 32768 40 -> 32 us).
@@ -1901,6 +1920,7 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
   p.d = d;
   p.ldd = ldd;
   p.alpha = scale;
+  p.part = logit_part(p.K);
   p.exp = {out.stats, out.ids, out.ids_ld, out.first, out.at, (p.N + 127) / 128};
   CUtensorMap tm_d = tm_a;  // (a valid map where none is used)
   if (pair && d != nullptr) {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import head_loss_ref as ref
-from test_head_loss import BF16, F32, HALF, _check_distillation, _close, _hit, _stat
+from test_head_loss import (BF16, F32, HALF, _check_distillation, _check_linear, _close, _entries, _hit, _operands, _stat)
 
 gpu = pytest.mark.gpu
 
@@ -87,3 +87,38 @@ def test_linear_losses_of_far_logits(cdl, gpu_ok, t, v, layout, tau, far):
         sums = 2.0 ** -23 * 40
         _close("dx", o.dx, dx, (g_err + sums * g.abs()) @ w.double().abs().t() + HALF[BF16] * dx.abs() + 1e-30)
         _close("dw", o.dw, dw, x.double().abs().t() @ (g_err + sums * g.abs()) + (HALF[BF16] + 2.0 ** -22) * dw.abs() + 1e-30)
+
+
+@gpu
+@pytest.mark.parametrize("t", [3, 130])
+@pytest.mark.parametrize("d", [4096, 4097, 1 << 18])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_of_long_sums(cdl, gpu_ok, t, d, sign):
+    """Positive terms, which lose the most in an accumulator that truncates: 2^-23 of the sum in each of 256 steps of 16 and 8 more, which
+    is all that one takes, then one rounding to nearest per 4096 terms.  What is put back is less.  (One accumulator for 2^18 terms was
+    1.4e-3 off.)"""
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.rand(t, d, generator=gen, device="cuda").to(BF16)
+    w = (torch.rand(d, 1, generator=gen, device="cuda") * sign / d * 64).to(BF16)
+    w = torch.cat([w, -w], 1)
+    z = x.double() @ w.double()
+    targets = torch.arange(t, device="cuda", dtype=torch.int32) % 2
+    o = cdl.ops.linear_cross_entropy(x, w, targets, cdl.ops.LinearLossOpts(grad=False))
+    off = (264 * 2.0 ** -23 + (d // 4096 + 2) * 2.0 ** -24) * z.abs().amax(1)
+    loss, lse, _ = ref.cross_entropy(z, targets)
+    _close("lse", o.lse, lse, off + 2.0 ** -20)
+    _close("loss", o.loss, loss, 2 * off + 2.0 ** -20 * (1 + loss))
+
+
+@gpu
+@pytest.mark.parametrize("t,d,v,k", [(5, 4097, 300, 0), (130, 8200, 700, 3), (700, 8264, 3001, 0), (1300, 12352, 2000, 9), (100, 20000, 520, 0)])
+def test_linear_losses_of_wide_hidden_states(cdl, gpu_ok, t, d, v, k):
+    """Logits that several accumulators make up, tile after tile."""
+    gen = torch.Generator(device="cuda").manual_seed(t + d)
+    x, w = _operands(gen, t, d, v, BF16, "rows")
+    entries = _entries(gen, t, v, k)
+    opts = cdl.ops.LinearLossOpts(temperature=1.0 if k == 0 else 1.7)
+    o = _check_linear(cdl, x, w, entries, opts)
+    fn = cdl.ops.linear_cross_entropy if k == 0 else cdl.ops.linear_distillation
+    again = fn(x, w, *entries, opts)
+    assert torch.equal(o.loss, again.loss) and torch.equal(o.dx, again.dx) and torch.equal(o.dw, again.dw)
