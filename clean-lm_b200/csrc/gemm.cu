@@ -510,56 +510,27 @@ __device__ __forceinline__ void add_tile_rows(const Params& p, const CUtensorMap
   }
 }
 
-// The epilogue of a bf16 D = alpha * accumulator for the calling warp: rows row0 .. row0 + 31, 128 columns, as two TMA stores
-// of 32 x 64 from its 4 KiB buffer (128-byte swizzle).  A thread's own stores cover 32 bytes of 32 rows per instruction; a
-// product of a short K is bound by them: 2048 x 32768 with K = 64 45 -> 31 us (134 MB).
-__device__ __forceinline__ void store_tile_rows_tma(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row,
-                                                    int b, int row0, int col_base, int lane) {
-  if (row0 >= p.M) return;  // warp-uniform; rows past M inside the box are clipped
+// The epilogue of a bf16 D = alpha * accumulator for the calling warp: rows row0 .. row0 + 31, 128 columns, 64 at a time by way of
+// its 4 KiB buffer (128-byte swizzle).  A thread's own stores cover 32 bytes of 32 rows per instruction; a product of a short K is
+// bound by them.  On the 16-byte grid TMA stores the 32 x 64: 2048 x 32768 with K = 64 45 -> 31 us (134 MB).  Off it the warp does, 64
+// bytes of a row per instruction.  (95 x 2185 x 94464: the loss with its gradients 502 us; with D stored on the grid and copied behind
+// the product, which moves its bytes three times, 591.)  TMA clips a row at 16 bytes, not at N: columns that end inside are the warp's,
+// too.
+__device__ __forceinline__ void store_tile_rows_bf16(const Params& p, const CUtensorMap* tm_d, uint8_t* buf, uint32_t t_row, int b, int row0,
+                                                     int col_base, int lane) {
+  const int rows = min(32, p.M - row0);
+  if (rows <= 0) return;  // warp-uniform; rows past M inside the box are clipped
 #pragma unroll 1
   for (int ch = 0; ch < 2; ++ch) {
     const int col0 = col_base + ch * 64;
     if (col0 >= p.N) break;
+    const bool by_tma = p.d_vec && (col0 + 64 <= p.N || p.N % 8 == 0);
     uint32_t r[2][32];
     tmem_ld32(t_row + ch * 64, r[0]);
     tmem_ld32(t_row + ch * 64 + 32, r[1]);
     tmem_wait_ld(r[0], r[1]);
     if (lane == 0) tma_store_wait_read<0>();  // the buffer's last store has read it
     __syncwarp();
-    const uint32_t row = smem_u32(buf) + lane * 128, x = (lane & 7) << 4;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = pack_bf16x2(p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j]),
-                           p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j + 1]));
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((c << 4) ^ x)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                   : "memory");
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_3d(tm_d, buf, col0, row0, b);
-      tma_store_commit();
-    }
-  }
-}
-
-// The same for rows off the 16-byte grid: by way of the buffer, 64 bytes of a row per instruction.  (95 x 2185 x 94464: the loss with its
-// gradients 502 us; with D stored on the grid and copied behind the product, which moves its bytes three times, 591.)
-__device__ __forceinline__ void store_tile_rows_odd(const Params& p, uint8_t* buf, uint32_t t_row, int row0, int col_base, int lane) {
-  const int rows = min(32, p.M - row0);
-  if (rows <= 0) return;  // warp-uniform
-#pragma unroll 1
-  for (int ch = 0; ch < 2; ++ch) {
-    const int col0 = col_base + ch * 64;
-    if (col0 >= p.N) break;
-    uint32_t r[2][32];
-    tmem_ld32(t_row + ch * 64, r[0]);
-    tmem_ld32(t_row + ch * 64 + 32, r[1]);
-    tmem_wait_ld(r[0], r[1]);
-    __syncwarp();  // the chunk before has been read
     const uint32_t base = smem_u32(buf), row = base + lane * 128, x = (lane & 7) << 4;
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
@@ -570,6 +541,15 @@ __device__ __forceinline__ void store_tile_rows_odd(const Params& p, uint8_t* bu
                            p.alpha * __uint_as_float(r[c >> 2][(c & 3) * 8 + 2 * j + 1]));
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((c << 4) ^ x)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                    : "memory");
+    }
+    if (by_tma) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(tm_d, buf, col0, row0, b);
+        tma_store_commit();
+      }
+      continue;
     }
     __syncwarp();
     __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.d) + static_cast<long long>(row0) * p.ldd + col0 + lane;
@@ -1274,8 +1254,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       } else if constexpr (KIND == STORE_PLANES || KIND == STORE_PIECES) {
         store_tile_rows(p, t_row, slice, row, col);
       } else if constexpr (KIND == STORE_BF16) {
-        if (p.d_vec) store_tile_rows_tma(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
-        else store_tile_rows_odd(p, buf, t_row, row - lane, col, lane);
+        store_tile_rows_bf16(p, &tmap_e0, buf, t_row, b, row - lane, col, lane);
       } else {
         if (p.epi_mode == 3) store_tile_rows_rope(p, t_row, row, col);
         else store_tile_rows(p, t_row, b, row, col);

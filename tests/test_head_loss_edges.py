@@ -122,3 +122,18 @@ def test_linear_losses_of_wide_hidden_states(cdl, gpu_ok, t, d, v, k):
     fn = cdl.ops.linear_cross_entropy if k == 0 else cdl.ops.linear_distillation
     again = fn(x, w, *entries, opts)
     assert torch.equal(o.loss, again.loss) and torch.equal(o.dx, again.dx) and torch.equal(o.dw, again.dw)
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 3, 7, 9, 100, 127, 129, 200, 1101])
+@pytest.mark.parametrize("t", [20, 300])
+def test_weight_gradient_leaves_what_lies_behind_its_rows(cdl, gpu_ok, n, t):
+    """Rows on the 16-byte grid that end inside 16 bytes: the columns behind them belong to something else."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    vocab = 40000
+    x, w = _operands(gen, t, n, vocab, BF16, "tied")
+    buffer = torch.full((vocab, (n + 7) // 8 * 8 + 8), 7.0, dtype=BF16, device="cuda")
+    view = buffer[:, :n]
+    _check_linear(cdl, x, w, _entries(gen, t, vocab, 0), cdl.ops.LinearLossOpts(), dw=view.t())
+    view.fill_(7.0)
+    assert bool((buffer == 7.0).all())
