@@ -695,8 +695,10 @@ __device__ __forceinline__ void store_tile_rows_exp(const Params& p, const CUten
 // from the L1, through which C is read), cost those 0.2 to 0.9 us (2048 x 5632 x
 // 256 12.3 instead of 11.9, with a bf16 C 18.8 instead of 18.0).
 // D in any form; D += by TMA; the SwiGLU forms whose operands TMA brings; a loss's exponentials; every K slice in a plane of
-// its own; a bf16 D by TMA; f32 operands as three bf16 pieces each, in planes if there are K slices.
-enum Store { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP, STORE_PLANES, STORE_BF16, STORE_PIECES };
+// its own; a bf16 D by TMA; f32 operands as three bf16 pieces each, in planes if there are K slices; exponentials of logits that several
+// accumulators add up to.
+enum Store { STORE, STORE_ADD, STORE_SWIGLU, STORE_EXP, STORE_PLANES, STORE_BF16, STORE_PIECES, STORE_EXP_PARTS };
+constexpr bool stores_exp(int kind) { return kind == STORE_EXP || kind == STORE_EXP_PARTS; }
 // The products of pieces that count, smallest first: an f32 value is the sum of its pieces 0, 1, 2, the others are below 2^-24.
 // A K slice goes through its K blocks once for each.
 constexpr int PIECE_PRODUCTS = 6;
@@ -708,10 +710,11 @@ __device__ __forceinline__ int piece_of_b(int i) { return 0x012010 >> (4 * (PIEC
 // after it: with 1800 of K in one accumulator dx of 159 x 576 x 43584 was 1.3e-6 off.
 constexpr int PART = 4;
 // A loss's logits: an accumulator takes up to LOGIT_PART K blocks (Params::part, all parts alike).  A sum of positive terms loses 1e-5 of
-// itself over 4096 of K, but 6.8e-3 over 2^20 in one accumulator.
+// itself over 4096 of K, but 6.8e-3 over 2^20 in one accumulator.  (A kernel of its own: 64 x 2048 x 32768 104 us; with parts in the kernel
+// for shorter sums, too, 105.)
 constexpr int LOGIT_PART = 64;
 template <int KIND>
-constexpr bool in_parts = KIND == STORE_PIECES || KIND == STORE_EXP;
+constexpr bool in_parts = KIND == STORE_PIECES || KIND == STORE_EXP_PARTS;
 template <int KIND>
 __device__ __forceinline__ int part_blocks(const Params& p) { return KIND == STORE_PIECES ? PART : p.part; }
 template <int KIND>
@@ -915,7 +918,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       unit_range(unit, tile, slice, kb0, kb1);
       tile_coords(p, tile, b, tm, tn);
       Wanted want;
-      if (KIND == STORE_EXP) want.load(p, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
+      if (stores_exp(KIND)) want.load(p, tm * BM + quad * 32 + lane, tn * BN + half * (BN / 2));
       const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
       auto full = [&](int n) {
         if (!mbar_wait(&bars->acc_full[n & 1], (n >> 1) & 1, abort_word, 301)) return false;
@@ -930,7 +933,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!(in_parts<KIND> ? sum_parts(num_parts<KIND>(p, kb0, kb1), t, t_lane, full, give) : full(t))) break;
       const uint32_t t_row = t_lane + (t & 1) * BN;
       const int row = tm * BM + quad * 32 + lane, col = tn * BN + half * (BN / 2);
-      if constexpr (KIND == STORE_EXP) {
+      if constexpr (stores_exp(KIND)) {
         store_tile_rows_exp<false>(p, nullptr, nullptr, t_row, row, col, lane, want);
       } else if constexpr (SLICES) {
         store_tile_rows(p, t_row, slice, row, col);
@@ -1230,7 +1233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int col = tn * BN + half * (BN / 2);
       if (KIND == STORE_SWIGLU && row - lane < p.M && col < p.N) feed.load(lane, row - lane, col);  // under the products
       Wanted want;
-      if (KIND == STORE_EXP) want.load(p, row, col);
+      if (stores_exp(KIND)) want.load(p, row, col);
       const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * (BN / 2);
       auto full = [&](int n) {
         if (!mbar_wait(&bars->acc_full[n & 1], (n >> 1) & 1, abort_word, 311)) return false;
@@ -1249,7 +1252,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       } else if constexpr (KIND == STORE_SWIGLU) {
         if (p.epi_mode == 1) store_tile_rows_swiglu<false>(p, feed, t_row, row, col, lane, abort_word);
         else store_tile_rows_swiglu<true>(p, feed, t_row, row, col, lane, abort_word);
-      } else if constexpr (KIND == STORE_EXP) {
+      } else if constexpr (stores_exp(KIND)) {
         store_tile_rows_exp<true>(p, &tmap_e0, buf, t_row, row, col, lane, want);
       } else if constexpr (KIND == STORE_PLANES || KIND == STORE_PIECES) {
         store_tile_rows(p, t_row, slice, row, col);
@@ -1261,7 +1264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
       give(a);
     }
-    if ((KIND == STORE_ADD || KIND == STORE_BF16 || KIND == STORE_EXP) && lane == 0) tma_store_wait<0>();
+    if ((KIND == STORE_ADD || KIND == STORE_BF16 || stores_exp(KIND)) && lane == 0) tma_store_wait<0>();
   }
 
   // ------------------------------------------------------------ tear-down
@@ -1463,6 +1466,7 @@ static int32_t prepare_kernels(int* clusters) {
     };
     one(gemm_bf16_kernel<STORE>);
     one(gemm_bf16_kernel<STORE_EXP>);
+    one(gemm_bf16_kernel<STORE_EXP_PARTS>);
     one(gemm_bf16_kernel<STORE_PLANES>);
     one(gemm_bf16_kernel<STORE_PIECES>);
     auto pair = [&](auto kernel, int kind) {
@@ -1474,6 +1478,7 @@ static int32_t prepare_kernels(int* clusters) {
     pair(gemm_bf16_pair_kernel<STORE_ADD>, STORE_ADD);
     pair(gemm_bf16_pair_kernel<STORE_SWIGLU>, STORE_SWIGLU);
     pair(gemm_bf16_pair_kernel<STORE_EXP>, STORE_EXP);
+    pair(gemm_bf16_pair_kernel<STORE_EXP_PARTS>, STORE_EXP_PARTS);
     pair(gemm_bf16_pair_kernel<STORE_PLANES>, STORE_PLANES);
     pair(gemm_bf16_pair_kernel<STORE_BF16>, STORE_BF16);
     pair(gemm_bf16_pair_kernel<STORE_PIECES>, STORE_PIECES);
@@ -1908,6 +1913,9 @@ int32_t matmul_exp_execute(const cdl_tensor* a, const cdl_tensor* b, float scale
     const uint32_t box[3] = {64, 32, 1};
     CDL_CHECK(encode_tmap(&tm_d, d, CDL_BF16, 3, dims, strides, box, true));  // (16 bits each, moved as they are)
   }
+  if (p.part < p.k_blocks)
+    return pair ? pair_launch<gemm::STORE_EXP_PARTS>(p, tm_a, tm_b, tm_d, 0, stream)
+                : one_launch<gemm::STORE_EXP_PARTS>(p, tm_a, tm_b, stream);
   return pair ? pair_launch<gemm::STORE_EXP>(p, tm_a, tm_b, tm_d, 0, stream) : one_launch<gemm::STORE_EXP>(p, tm_a, tm_b, stream);
 }
 

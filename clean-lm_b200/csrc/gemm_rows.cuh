@@ -59,7 +59,7 @@ struct Params {
   // epilogue reads comes from that kernel: the epilogue waits for it.
   int early;
   ExpStore exp;
-  int part;  // (of ExpStore's kernel) K blocks of an accumulator; what the parts of a tile add up to is stored
+  int part;  // (of STORE_EXP_PARTS) K blocks of an accumulator; what the parts of a tile add up to is stored
 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& b, int& m, int& n) {
