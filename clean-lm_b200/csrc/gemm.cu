@@ -506,7 +506,8 @@ __device__ __forceinline__ void add_tile_rows(const Params& p, const CUtensorMap
     tmem_wait_ld(r);
     if (lane == 0) tma_store_wait_read<0>();  // the buffer's last reduction has read it
     __syncwarp();
-    add_chunk(tm_d, buf, r, p.alpha, lane, col0, row0, b);
+    add_chunk(tm_d, buf, r, p.alpha, lane, col0, row0, b,
+              static_cast<float*>(p.d) + b * p.d_batch + static_cast<long long>(row0 + lane) * p.ldd + col0, p.N - col0, row0 + lane < p.M);
   }
 }
 

@@ -707,7 +707,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           uint8_t* buf = staging + (warp - 2) * gemm::CHUNK_BYTES;
           if (lane == 0) tma_store_wait_read<0>();  // the buffer's last reduction has read it
           __syncwarp();
-          gemm::add_chunk(&tmap_d, buf, r, p.alpha, lane, col0, row - lane, 0);
+          gemm::add_chunk(&tmap_d, buf, r, p.alpha, lane, col0, row - lane, 0,
+                          static_cast<float*>(p.d) + static_cast<long long>(row) * p.ldd + col0, p.N - col0, row < p.M);
         } else if (p.out_mx == 0) {
           if (row < p.M && col0 < p.N) store32(p, r, row, col0);
         } else if (col0 < p.N) {

@@ -99,9 +99,18 @@ int32_t gemm_cluster_launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b, co
 // stores meet no bank twice).  A thread owns a row of the accumulator, so its own accesses to D take 32 lines
 // per instruction and, where C is read first, a round trip to HBM per 32 columns; the reduction is one
 // instruction, nothing waits for it, and the L2 adds whole lines.  Every element is added to once per K slice.
+// TMA clips a row at 16 bytes, not at N, and would add to what lies behind a row that ends inside them (zeros, but NaN where A is
+// not finite): there the threads add to the columns that exist.  d: the lane's row at col0, cols: columns from there on.
 constexpr int CHUNK_BYTES = 32 * 32 * 4;
 __device__ __forceinline__ void add_chunk(const CUtensorMap* tm_d, uint8_t* buf, const uint32_t (&r)[32], float alpha,
-                                          int lane, int col0, int row0, int b) {
+                                          int lane, int col0, int row0, int b, float* d, int cols, bool row_ok) {
+  if (cols < 32 && cols % 4 != 0) {  // warp-uniform
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (row_ok && j < cols)
+        asm volatile("red.global.add.f32 [%0], %1;" ::"l"(d + j), "f"(alpha * __uint_as_float(r[j])) : "memory");
+    return;
+  }
   const uint32_t row = smem_u32(buf) + lane * 128, x = (lane & 7) << 4;
 #pragma unroll
   for (int c = 0; c < 8; ++c)
