@@ -1390,6 +1390,13 @@ static bool on_grid(const cdl_tensor& t) {
 }
 static bool columns_first(const cdl_tensor& t) { return t.stride[0] < t.stride[1]; }  // dimension 0 is the nearer one in memory
 
+// The stride of a dimension of extent 1, which may be any, becomes the one that columns_first and on_grid read alike: a view on
+// the grid then has neighbouring elements along its nearer dimension.
+static void settle_strides(cdl_tensor& t) {
+  if (t.shape[1] == 1) t.stride[1] = t.shape[0] > 1 && t.stride[0] == 1 ? t.shape[0] : 1;
+  if (t.shape[0] == 1) t.stride[0] = t.stride[1] == 1 ? t.shape[1] : 1;
+}
+
 struct Linear {
   const char* op;
   cdl_tensor x, w, dx, dw;  // dx, dw: ptr = nullptr where not wanted
@@ -1541,6 +1548,7 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
   p.op = op;
   p.x = *x;
   p.w = *w;
+  settle_strides(p.w);
   p.T = x->shape[0];
   p.D = x->shape[1];
   p.V = w->shape[1];
@@ -1563,6 +1571,7 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
                                         : a < b ? (p.V <= 1 || b >= (p.D - 1) * a + 1) : (p.D <= 1 || a >= (p.V - 1) * b + 1);
     if (!apart) return fail(CDL_ERR_INVALID, "%s: elements of dw overlap", op);
     p.dw = *dw;
+    settle_strides(p.dw);
   }
   if (p.V == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: vocab is zero", op);
   if (p.D == 0 && p.T > 0) return fail(CDL_ERR_INVALID, "%s: hidden is zero", op);
@@ -1626,7 +1635,7 @@ static int32_t pieces_product(const Linear& p, const cdl_tensor& a, const cdl_te
                               cudaStream_t stream) {
   const long long M = d.shape[0], N = d.shape[1], ld = up(N, 8), k_blocks = (a.shape[2] + 63) / 64;
   if (slices > k_blocks) slices = static_cast<int>(k_blocks);  // (the last rows are fewer)
-  if (slices == 1 && (d.stride[1] == 1 || N == 1))
+  if (slices == 1)  // (D's rows are neighbouring elements, here and in its planes)
     return matmul_pieces_execute(&a, &b, static_cast<float*>(d.ptr), M > 1 ? d.stride[0] : ld, 1, add, stream);
   float* planes = reinterpret_cast<float*>(base + p.at_planes);
   CDL_CHECK(matmul_pieces_execute(&a, &b, planes, ld, slices, 0, stream));

@@ -137,3 +137,50 @@ def test_weight_gradient_leaves_what_lies_behind_its_rows(cdl, gpu_ok, n, t):
     _check_linear(cdl, x, w, _entries(gen, t, vocab, 0), cdl.ops.LinearLossOpts(), dw=view.t())
     view.fill_(7.0)
     assert bool((buffer == 7.0).all())
+
+
+def _strided(extents, strides, dtype, device="cpu"):
+    """A view of these strides in a buffer of its own, filled with 7, and the buffer."""
+    buffer = torch.full((sum((n - 1) * s for n, s in zip(extents, strides)) + 1,), 7.0, dtype=dtype, device=device)
+    return buffer.as_strided(extents, strides), buffer
+
+
+ONE_WIDE = [((1, 3000), (12000, 4)), ((1, 3000), (24000, 8)), ((1, 3000), (3, 3)), ((1, 100000), (800000, 8)), ((1, 3000), (1, 1)),
+            ((900, 1), (4, 1000)), ((900, 1), (8, 7200)), ((900, 1), (1, 5)), ((900, 1), (3, 1)), ((1, 1), (5, 9))]
+
+
+@pytest.mark.parametrize("extents,strides", ONE_WIDE)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_stride_of_an_extent_of_one_does_not_matter(cdl, extents, strides, dtype):
+    """The same memory described in several ways is one plan: one size of the scratch."""
+    sizes = set()
+    for other in (1, 4, 8, 1000, 800000):
+        view = tuple(other if n == 1 else s for n, s in zip(extents, strides))
+        w, _ = _strided(extents, view, dtype)
+        x = torch.zeros(20, extents[0], dtype=dtype)
+        sizes.add((cdl.ops.linear_loss_scratch_bytes(x, w, dx=x, dw=w), cdl.ops.linear_loss_scratch_bytes(x, w.contiguous(), dx=x, dw=w)))
+    assert len(sizes) == 1
+
+
+@gpu
+@pytest.mark.parametrize("extents,strides", ONE_WIDE)
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("t", [5, 20, 300])
+def test_one_hidden_or_one_token_id_in_any_strides(cdl, gpu_ok, extents, strides, dtype, out, t):
+    """Heads of one hidden value or one token id; nothing is written beyond the scratch that is asked for, nor between the
+    elements of dw."""
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    d, v = extents
+    x = torch.randn(t, d, generator=gen, device="cuda").to(dtype)
+    w, _ = _strided(extents, strides, dtype, "cuda")
+    w.copy_(torch.randn(d, v, generator=gen, device="cuda"))
+    entries = _entries(gen, t, v, 0)
+    for accumulate in (False, True):
+        dw, buffer = _strided(extents, strides, out, "cuda")
+        before = dw.clone() if accumulate else None
+        n = cdl.ops.linear_loss_scratch_bytes(x, w, cdl.ops.LinearLossOpts(accumulate=accumulate), dx=x, dw=dw)
+        scratch = torch.full((n + (1 << 20),), 90, dtype=torch.uint8, device="cuda")
+        _check_linear(cdl, x, w, entries, cdl.ops.LinearLossOpts(accumulate=accumulate), dw=dw, before=before, scratch=scratch[:n])
+        assert bool((scratch[n:] == 90).all())
+        dw.fill_(7.0)
+        assert bool((buffer == 7.0).all())
