@@ -1561,6 +1561,9 @@ static int32_t check_linear(const char* op, const cdl_head_loss_desc* desc, cons
     if (dx->rank != 2 || dx->dtype != x->dtype || dx->shape[0] != p.T || dx->shape[1] != p.D || (p.D > 1 && dx->stride[1] != 1) ||
         (p.T > 1 && dx->stride[0] < p.D))
       return fail(CDL_ERR_INVALID, "%s: dx must have x's type and shape and contiguous rows that do not overlap", op);
+    // (a chunk's rows of dx are written before the next chunk's rows of x are read)
+    if (p.T > 0 && dx->ptr == x->ptr && ((p.T > 1 && dx->stride[0] != x->stride[0]) || (p.D > 1 && dx->stride[1] != x->stride[1])))
+      return fail(CDL_ERR_INVALID, "%s: dx must be x itself or lie elsewhere", op);
     p.dx = *dx;
   }
   if (dw) {

@@ -184,3 +184,17 @@ def test_one_hidden_or_one_token_id_in_any_strides(cdl, gpu_ok, extents, strides
         assert bool((scratch[n:] == 90).all())
         dw.fill_(7.0)
         assert bool((buffer == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_dx_in_place_of_x_has_its_strides(cdl, dtype):
+    """Another stride from the same address: rows of x that a later chunk of rows reads would be overwritten."""
+    buffer, w = torch.zeros(20, 48, dtype=dtype), torch.zeros(16, 40, dtype=dtype)
+    size = cdl.ops.linear_loss_scratch_bytes
+    x = buffer[:, :16]
+    dense = buffer.flatten()[:320].view(20, 16)
+    assert size(x, w, dx=x) > 0 and size(dense, w, dx=dense) > 0 and size(x[:1], w, dx=dense[:1]) > 0
+    assert size(x, w, dx=torch.zeros(20, 16, dtype=dtype)) > 0 and size(x.t()[:0, :16], w, dx=x[:0]) == 0
+    for a, b in ((x, dense), (dense, x), (buffer.flatten()[:320].view(16, 20).t(), dense)):
+        with pytest.raises(cdl._lib.CdlError, match="dx must be x itself or lie elsewhere"):
+            size(a, w, dx=b)
