@@ -1432,10 +1432,10 @@ static cdl_tensor strided2(void* p, int32_t dt, long long r, long long c, long l
 
 constexpr long long TARGET_ENTRIES = -1;
 
-// Rows that are taken at a time: their exponentials (f32: logits and the pieces of their gradients) are what the scratch holds,
-// up to 1 GB.  16384 x 2048 x 32768 in one go 5.21 ms, in two 5.44: dw is summed in memory then, dx's last wave is emptier.
-static long long choose_chunk(long long T, long long V, long long bytes_per_logit) {
-  long long rows = (1LL << 30) / (bytes_per_logit * up(V, 128));
+// Rows that are taken at a time: up to 1 GB of what grows with them and the vocabulary, but 256 rows at least (w is read once per
+// chunk).  16384 x 2048 x 32768 in one go 5.21 ms, in two 5.44: dw is summed in memory then, dx's last wave is emptier.
+static long long choose_chunk(long long T, long long bytes_per_row) {
+  long long rows = (1LL << 30) / bytes_per_row;
   if (rows < 256) rows = 256;
   if (rows >= T) return T;
   const long long chunks = (T + rows - 1) / rows;
@@ -1459,7 +1459,11 @@ static void plan_linear(Linear& p, const cdl_head_loss_desc* desc, long long ent
   p.copy_x = (reinterpret_cast<uintptr_t>(p.x.ptr) & 15) != 0 || (p.D > 1 && p.x.stride[1] != 1) ||  // (chunks of its rows are on the grid)
              (p.T > 1 && (p.x.stride[0] % 8 != 0 || p.x.stride[0] < p.D));
   p.copy_w = !on_grid(p.w);
-  p.chunk = desc->chunk_rows > 0 ? desc->chunk_rows : choose_chunk(p.T, p.V, p.f32 ? 10 : 2);
+  // f32: logits and the pieces of their gradients, or of x; bf16: exponentials, for the loss alone statistics and entries (a target
+  // as one entry: the scratch's size is asked for without saying which it is).
+  const long long ld = up(p.V, 128), row_bytes = p.f32 ? (grad ? 10 * ld : 4 * ld + 6 * up(p.D, 8))
+                                                 : grad ? 2 * ld : 10LL * p.pieces + 12LL * (p.K > 1 ? p.K : 1) + 6;
+  p.chunk = desc->chunk_rows > 0 ? desc->chunk_rows : choose_chunk(p.T, row_bytes);
   if (p.chunk > p.T) p.chunk = p.T;
   const bool whole = p.chunk >= p.T, wc = columns_first(p.w), dc = p.has_dw && columns_first(p.dw);
   p.dw_way = Linear::DIRECT;

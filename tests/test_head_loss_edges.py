@@ -198,3 +198,35 @@ def test_dx_in_place_of_x_has_its_strides(cdl, dtype):
     for a, b in ((x, dense), (dense, x), (buffer.flatten()[:320].view(16, 20).t(), dense)):
         with pytest.raises(cdl._lib.CdlError, match="dx must be x itself or lie elsewhere"):
             size(a, w, dx=b)
+
+
+def test_loss_alone_is_not_taken_apart_for_gradients_that_are_not_wanted(cdl):
+    """Without gradients the scratch holds statistics, not exponentials: many more rows fit into the same bytes."""
+    def size(t, d, v, dtype, entries, chunk):
+        x, w = torch.zeros(1, 1, dtype=dtype).expand(t, d), torch.zeros(1, 1, dtype=dtype).expand(d, v)
+        return cdl.ops.linear_loss_scratch_bytes(x, w, cdl.ops.LinearLossOpts(chunk_rows=chunk), entries=entries)
+
+    for t, d, v, dtype, entries in ((65536, 256, 32768, BF16, 1), (200000, 64, 32768, BF16, 1), (65536, 256, 32768, BF16, 64),
+                                    (2000, 128, 100000, F32, 1)):
+        assert size(t, d, v, dtype, entries, 0) == size(t, d, v, dtype, entries, t)
+    # still bounded, whatever else a row holds
+    operands = lambda t, d, v: 2 * (t * ((d + 7) // 8 * 8) + d * (v + 7))  # noqa: E731  (laid out anew)
+    for t, d, v, entries in ((1 << 20, 64, 128, 1024), (1 << 24, 8, 1000, 3), (1 << 22, 8, 150000, 256)):
+        assert size(t, d, v, BF16, entries, 0) <= (1 << 30) * 1.01 + operands(t, d, v)
+
+
+@gpu
+@pytest.mark.parametrize("t,d,v,k,dtype", [(500000, 16, 32768, 0, BF16), (300000, 16, 32768, 5, BF16), (3000, 16, 100001, 0, F32)])
+def test_loss_alone_of_many_tokens(cdl, gpu_ok, t, d, v, k, dtype):
+    """More than one chunk of rows, and as many as the caller asks for: the same statistics."""
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    x, w = _operands(gen, t, d, v, dtype, "rows")
+    entries = _entries(gen, t, v, k)
+    fn = cdl.ops.linear_cross_entropy if k == 0 else cdl.ops.linear_distillation
+    o = fn(x, w, *entries, cdl.ops.LinearLossOpts(grad=False))
+    p = fn(x, w, *entries, cdl.ops.LinearLossOpts(grad=False, chunk_rows=1024 if dtype == F32 else 1 << 16))
+    assert torch.equal(o.loss, p.loss) and torch.equal(o.lse, p.lse)
+    rows = torch.cat([torch.arange(64), torch.arange(t - 64, t)]).cuda()
+    _check_linear(cdl, x[rows], w, [e[rows] for e in entries], cdl.ops.LinearLossOpts(grad=False))
+    want = fn(x[rows], w, *[e[rows] for e in entries], cdl.ops.LinearLossOpts(grad=False))
+    _close("loss", o.loss[rows], want.loss, 2.0 ** -18 * (1 + want.loss.abs()))
