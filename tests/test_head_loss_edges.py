@@ -230,3 +230,58 @@ def test_loss_alone_of_many_tokens(cdl, gpu_ok, t, d, v, k, dtype):
     _check_linear(cdl, x[rows], w, [e[rows] for e in entries], cdl.ops.LinearLossOpts(grad=False))
     want = fn(x[rows], w, *[e[rows] for e in entries], cdl.ops.LinearLossOpts(grad=False))
     _close("loss", o.loss[rows], want.loss, 2.0 ** -18 * (1 + want.loss.abs()))
+
+
+# ------------------------------------------------------------------------------------------ what f32 operands keep
+def _leading(v, bits):
+    """f32 values cut off behind their first 8, 16 or 24 bits: one, two or three bf16 pieces."""
+    return (v.view(torch.int32) & -(1 << (24 - bits))).view(torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("t", [20, 200])
+@pytest.mark.parametrize("of_x,of_w", [(8, 24), (24, 8), (16, 16), (16, 8), (8, 16)])
+def test_each_product_of_pieces_counts(cdl, gpu_ok, t, of_x, of_w):
+    """The logsumexp of one token id is its logit.  With x and w of one to three pieces, positive, and every lower piece large, each of
+    the products (0, 2), (2, 0), (1, 1), (1, 0), (0, 1) is 2^-17 of the logit and more, and those that are left out, (1, 2), (2, 1), (2, 2), are
+    none.  Six steps of an accumulator cut 2^-23 each, putting back and rounding adds as much as two more."""
+    gen = torch.Generator(device="cuda").manual_seed(t)
+
+    def values(*shape, bits):  # 1.x with the first bits of every piece set
+        v = torch.randint(0, 1 << 23, shape, generator=gen, device="cuda", dtype=torch.int32) | 0x3f80c0c0
+        return _leading(v.view(torch.float32), bits)
+
+    x, w = values(t, 16, bits=of_x), values(16, 1, bits=of_w)
+    o = cdl.ops.linear_cross_entropy(x, w, torch.zeros(t, dtype=torch.int32, device="cuda"))
+    z = (x.double() @ w.double())[:, 0]
+    lower = [(a.double() - _leading(a, 8)) for a in (x, w)]
+    assert ((lower[0] @ w.double())[:, 0].min() > 0) == (of_x > 8) and ((x.double() @ lower[1])[:, 0].min() > 0) == (of_w > 8)
+    _close("lse", o.lse, z, 8 * 2.0 ** -23 * z)
+
+
+@gpu
+@pytest.mark.parametrize("t,d,v,layout", [(300, 200, 1500, "rows"), (100, 333, 2001, "tied"), (40, 600, 900, "rows"), (700, 515, 8190, "tied")])
+def test_f32_gradients_in_the_2_norm(cdl, gpu_ok, t, d, v, layout):
+    """Logits below 4: their rounding, the exponential's and the sum's leave d z 2^-20 off, the products of pieces and their sums 2^-22, the
+    result's rounding less.  2^-19 in all; without any one of the six products of pieces it would be 8e-6 (four times as much)."""
+    gen = torch.Generator(device="cuda").manual_seed(t + d)
+    x, w = _operands(gen, t, d, v, F32, layout)
+    targets = _entries(gen, t, v, 0)[0]
+    o = cdl.ops.linear_cross_entropy(x, w, targets)
+    _, _, _, dx, dw = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
+    assert (o.dx - dx).norm() <= 2.0 ** -19 * dx.norm() and (o.dw - dw).norm() <= 2.0 ** -19 * dw.norm()
+
+
+@gpu
+@pytest.mark.parametrize("t", [40, 159])
+def test_f32_gradient_with_a_large_first_term_is_as_good_as_f32_products(cdl, gpu_ok, t):
+    """dx is the target's column and what 43583 small terms add.  In the accumulator of the first 256 of K some 16 steps behind the target's
+    cut half a unit each on average, 0.7 2^-23 of the value on average over a binade: 11.5 2^-24; 4.3 2^-24 is put back.  171 parts rounded
+    to nearest, independently: 3 2^-24.  8 2^-24 in the 2-norm, where one accumulator for all of K loses 22 (and f32 products 10)."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(t, 576, generator=gen, device="cuda")
+    w = torch.randn(576, 43584, generator=gen, device="cuda") * 0.02
+    targets = torch.zeros(t, dtype=torch.int32, device="cuda")
+    o = cdl.ops.linear_cross_entropy(x, w, targets)
+    _, _, _, dx, _ = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
+    assert ((o.dx - dx).norm() / dx.norm()).item() <= 10 * 2.0 ** -24
