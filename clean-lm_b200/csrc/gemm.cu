@@ -586,7 +586,7 @@ struct Wanted {
   __device__ __forceinline__ void load(const Params& p, int row, int col_base) {
     e = end = 0;
     id = -1;
-    if (row >= p.M || col_base >= p.N || p.exp.ids == nullptr) return;
+    if (row >= p.M || col_base >= p.N) return;
     if (p.exp.first == nullptr) {
       end = 1;
     } else {

@@ -48,7 +48,7 @@ int32_t matmul_execute_epi(const cdl_tensor* a, const cdl_tensor* b, const cdl_t
 // operands on the 16-byte grid; see store_tile_rows_exp in gemm.cu).
 struct ExpOutputs {
   float2* stats;  // [rows][pieces of 128 columns]
-  const int* ids;  // columns whose logit is stored besides, [rows][ids_ld]; nullptr: none
+  const int* ids;  // columns whose logit is stored besides, [rows][ids_ld]
   long long ids_ld;
   const unsigned short* first;  // [rows][pieces + 1], nullptr: one id per row
   float* at;                    // [rows][ids_ld]
