@@ -311,7 +311,7 @@ class Sky1LM:
         self.hf = torch.empty(t, b.hidden, **bf)
         self.r_inv = torch.empty(t, **f32)
         self.logits = torch.empty(t, cfg.vocab, **bf) if cfg.keep_logits else None
-        self.loss_tok = torch.empty(t, **f32)
+        self.loss_tok = torch.empty(t, **f32) if cfg.keep_logits else None  # (else the loss's own output)
         self.loss = torch.zeros(1, **f32)
         self.sumsq = torch.zeros(1, **f32)
         self.dx = [torch.empty(t, b.hidden, **bf) for _ in range(2)]

@@ -285,3 +285,15 @@ def test_f32_gradient_with_a_large_first_term_is_as_good_as_f32_products(cdl, gp
     o = cdl.ops.linear_cross_entropy(x, w, targets)
     _, _, _, dx, _ = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
     assert ((o.dx - dx).norm() / dx.norm()).item() <= 10 * 2.0 ** -24
+
+
+@gpu
+def test_language_model_without_stored_logits_keeps_no_buffer_for_them(cdl, gpu_ok):
+    sky1 = cdl.sky1
+    blk = sky1.Sky1Config(batch=1, seqlen=128, hidden=128, heads=1, kv_heads=1, head_dim=128, ffn=256)
+    m = sky1.Sky1LM(sky1.Sky1LMConfig(block=blk, layers=1, vocab=512, keep_logits=False), seed=4)
+    assert m.logits is None and m.loss_tok is None
+    tokens = torch.arange(128, dtype=torch.int32, device="cuda") % 512
+    m.loss.zero_()
+    m.forward_backward(tokens, (tokens + 1) % 512, 1.0 / 128)
+    assert abs(m.loss.item() - torch.log(torch.tensor(512.0)).item()) < 0.5  # (weights of N(0, 0.02^2): logits near 0)
