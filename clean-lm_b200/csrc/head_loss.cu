@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(ROW_THREADS)
 // most 32 x VECS vectors of 16 bytes, which stay in registers: the maximum; the exponentials in place of the logits (bf16: as
 // f16, 2^15 at the maximum, see store_tile_rows_exp in gemm.cu; their sum is of the f32 values); and, behind the one barrier at
 // which the slices' parts of the statistics meet, the gradient.  The row's entries are a thread's each, and their softmax
-// meets at the same barrier: where one warp prepared them all, the others waited for it (8192 x 32768 with 64
-// entries 244 us, not 216).  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
+// meets at the same barrier (8192 x 32768 with 64 entries 215 us, with one 183): where one warp prepared them all, the others waited
+// for it, an eighth more time.  One exponential per element: a second one would put 4096 clk of special functions per 64 KB on an SM,
 // whose share of the HBM's rate takes 5500.  The slices depend on the vocabulary and on whether rows are on the 16-byte
 // grid, not on how many CTAs share a row, so a row's results do not depend on the number of rows.
 //
@@ -1206,7 +1206,7 @@ static Share choose_share(const void* z, long long ld, long long rows, int vocab
   for (int c = s.ctas + 1; c <= 8 && rows * s.ctas < sm_count() && s.slice >= 64; ++c)
     if (s.warps % c == 0) s.ctas = c;
   s.slots_log2 = 5;
-  while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (with 2 K slots 64 random ids cost 8192 x 32768 290 us, not 228)
+  while ((1 << s.slots_log2) < 8 * K) ++s.slots_log2;  // (8192 x 32768 with 64 random ids: 2 K slots 257 us, 4 K 223, 8 K 215)
   s.smem = static_cast<size_t>(ENTRY_BYTES) * K + (4u << s.slots_log2);  // at most 44 KB
   return s;
 }
@@ -1442,7 +1442,7 @@ static cdl_tensor strided2(void* p, int32_t dt, long long r, long long c, long l
 constexpr long long TARGET_ENTRIES = -1;
 
 // Rows that are taken at a time: up to 1 GB of what grows with them and the vocabulary, but 256 rows at least (w is read once per
-// chunk).  16384 x 2048 x 32768 in one go 5.21 ms, in two 5.44: dw is summed in memory then, dx's last wave is emptier.
+// chunk).  16384 x 2048 x 32768 in one go 4.83 ms, in two 5.01: dw is summed in memory then, dx's last wave is emptier.
 static long long choose_chunk(long long T, long long bytes_per_row) {
   long long rows = (1LL << 30) / bytes_per_row;
   if (rows < 256) rows = 256;

@@ -228,8 +228,9 @@ class Sky1LMConfig:
     adam_eps: float = 1e-8
     weight_decay: float = 0.1
     max_grad_norm: float = 0.0  # 0 = no clipping
-    # False: the loss and the head's gradients straight from the hidden states (ops.linear_cross_entropy), without the
-    # bf16 [tokens, vocab] buffer; its logits are not rounded to bf16 either.
+    # False: the loss and the head's gradients straight from the hidden states (ops.linear_cross_entropy), whose logits are not
+    # rounded to bf16.  In place of the bf16 [tokens, vocab] buffer it has a scratch that stops growing at about 1 GB, which is
+    # what 16384 tokens of vocabulary 32768 take either way.
     keep_logits: bool = True
 
     def param_count(self) -> int:

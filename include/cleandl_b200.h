@@ -527,12 +527,14 @@ int32_t cdl_b200_distillation(const cdl_head_loss_desc* desc, const cdl_tensor* 
                               const cdl_tensor* lse, const cdl_tensor* d_logits, cdl_stream stream);
 /* The losses of z = x . w, x [tokens, hidden] and w [hidden, vocab] both bf16 or both f32, of any strides (w may be the
  * transposed view of a [vocab, hidden] embedding table; operands whose rows are off the 16-byte grid are copied first).
- * The logits are not kept: the scratch holds chunk_rows tokens' worth at a time, however many tokens there are.
- *   dx  (nullable) x's type [tokens, hidden], contiguous rows:  d z . w^T; may be x itself
+ * The logits are not kept: the scratch holds chunk_rows tokens' worth at a time, however many tokens there are (by the library's
+ * choice up to 1 GB of exponentials, but 256 tokens at least; f32 operands: logits and their gradients' pieces, and 6 bytes per
+ * element of w beside them).
+ *   dx  (nullable) x's type [tokens, hidden], contiguous rows:  d z . w^T; may be x itself, with x's strides
  *   dw  (nullable) f32 or x's type [hidden, vocab], any strides:  x^T . d z, added to with accumulate_dw.  Held in f32 over
  *       all tokens and rounded once.
  * For bf16 operands d z is rounded to bf16 before both products, as cdl_b200_cross_entropy rounds it: an f32 dw has that
- * accuracy then.  (Up to 64 tokens, where it costs no time, it goes into them as two bf16 values.)  f32 operands keep 24
+ * accuracy then.  (Up to 64 tokens in one chunk, where it costs no time, it goes into them as two bf16 values.)  f32 operands keep 24
  * bits of it.  Without tokens dw is zero.  Scratch: 256-byte aligned, of the size that the call below gives for the same
  * operands (entries: teacher_ids' second dimension, 1 for targets); calls that may run at the same time have one each. */
 int32_t cdl_b200_linear_cross_entropy(const cdl_head_loss_desc* desc, const cdl_tensor* x, const cdl_tensor* w,
