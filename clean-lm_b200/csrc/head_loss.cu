@@ -6,8 +6,9 @@
 //     G_j = s tau (q_j - p_j),      s = grad_scale * d_loss[row]
 // (cross entropy: tau = 1, p = 1 at the target).  With c = log2(e) / tau, M = max z, S = sum 2^(c (z_j - M)):
 //     q_j = 2^(c (z_j - M)) / S,   log q_j = ln 2 (c (z_j - M) - log2 S),   lse = M / tau + ln 2 log2 S.
-// All statistics are f32.  From stored logits differences are taken before they are scaled: a row masked with the type's
-// lowest value, which times c overflows, is a uniform one.
+// All statistics are f32.  Differences are taken before they are scaled: a row masked with the type's lowest value, which times c
+// overflows, is a uniform one; and what p holds of z - M is summed as it is: loss = tau^2 (sum p log p + ln S) - tau sum p (z - M),
+// finite for an entry that is masked that way.
 #include "host.h"
 #include "ops.h"
 #include "ptx.cuh"
@@ -248,13 +249,13 @@ __global__ void __launch_bounds__(ROW_THREADS)
   const float base = top == -INFINITY ? 0.f : top;
   s = cta_reduce((bad ? NAN : s) * (m == -INFINITY ? (bad ? NAN : 0.f) : ex2(c * (m - base))), false, sh.part);
   const float log2_s = log2f(s);
-  float cross = 0.f;  // sum_k p_k log2 q_k
+  float cross = 0.f;  // tau sum_k p_k (z_k - M)
   for (int k = threadIdx.x; k < src.K; k += ROW_THREADS)
-    if (e.p[k] != 0.f) cross += e.p[k] * (c * (e.at[k] - base) - log2_s);
+    if (e.p[k] != 0.f) cross += e.p[k] * terms.tau * (e.at[k] - base);
   cross = cta_reduce(cross, false, sh.part);
   const bool counts = sh.counts;
   if (threadIdx.x == 0) {
-    terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p - LN2 * cross) : 0.f;
+    terms.loss[row] = counts ? terms.tau * terms.tau * (sh.p_log_p + LN2 * log2_s) - cross : 0.f;
     if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * log2_s;
   }
   if (g.ptr == nullptr) return;
@@ -475,19 +476,21 @@ __global__ void __launch_bounds__(WARPS * 32, VECS <= 8 ? 2 : 1)
   auto weight_of = [&](int k) { return ex2(c * (s_entries[k / 32].x - ent_top)) * over; };
   if (rank == 0 && warp == warps - 1) {
     const float log2_s = log2f(s);
-    // sum_k p_k (log2 p_k - log2 q_k); the first part: sum p c (y - largest) - log2 of the sum
+    // (sum p log2 p = sum p c (y - largest) - log2 of the sum)
+    const float tau2 = terms.tau * terms.tau * LN2;
+    const float rest = tau2 * ((log2_s - OFF) - log2f(ent_sum));
     float sum = 0.f;
     for (int k = lane; k < src.K; k += 32) {
       const float v = e.p[k];
-      if (v != 0.f) sum -= v * weight_of(k) * ((c * (e.at[k] - base) + OFF) - log2_s);
+      if (v != 0.f) sum -= v * weight_of(k) * terms.tau * (e.at[k] - base);
     }
     if (lane < groups && s_entries[lane].y != 0.f) {
       const float3 v = s_entries[lane];
-      sum += weight_of(32 * lane) * (v.z + v.y * (c * (v.x - ent_top)));
+      sum += tau2 * weight_of(32 * lane) * (v.z + v.y * (c * (v.x - ent_top)));
     }
-    sum = warp_sum(sum) - log2f(ent_sum);
+    sum = warp_sum(sum) + rest;
     if (lane == 0) {
-      terms.loss[row] = counts ? terms.tau * terms.tau * LN2 * sum : 0.f;
+      terms.loss[row] = counts ? sum : 0.f;
       if (terms.lse) terms.lse[row] = base / terms.tau + LN2 * (log2_s - OFF);
     }
   }
@@ -680,15 +683,16 @@ __global__ void __launch_bounds__(ROWS_PER_CTA * 32)
   const float log2_s = log2f(S) - 15.f;
   const bool counts = entries > 0;
   if (blockIdx.y == 0) {
-    float cross = 0.f;  // sum_k p_k log2 q_k
+    const float tau = LN2 * c * (terms.tau * terms.tau);  // (c has what the products put back)
+    float cross = 0.f;  // tau sum_k p_k (z_k - M)
     for (int k = lane; k < entries; k += 32) {
       const float p = src.p == nullptr ? 1.f : src.p[static_cast<long long>(row) * K + k];
-      if (p != 0.f) cross += p * (c * (src.at[static_cast<long long>(row) * K + k] - base) - log2_s);
+      if (p != 0.f) cross += p * tau * (src.at[static_cast<long long>(row) * K + k] - base);
     }
     cross = warp_sum(cross);
     if (lane == 0) {
       const float entropy = src.p == nullptr ? 0.f : src.p_log_p[row];
-      terms.loss[row] = counts ? terms.tau * terms.tau * (entropy - LN2 * cross) : 0.f;
+      terms.loss[row] = counts ? terms.tau * terms.tau * (entropy + LN2 * log2_s) - cross : 0.f;
       if (terms.lse) terms.lse[row] = LN2 * (c * base + log2_s);
     }
   }

@@ -297,3 +297,43 @@ def test_language_model_without_stored_logits_keeps_no_buffer_for_them(cdl, gpu_
     m.loss.zero_()
     m.forward_backward(tokens, (tokens + 1) % 512, 1.0 / 128)
     assert abs(m.loss.item() - torch.log(torch.tensor(512.0)).item()) < 0.5  # (weights of N(0, 0.02^2): logits near 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [100, 5000, 40001, 900001])
+@pytest.mark.parametrize("tau", [0.25, 1.0])
+def test_teacher_wants_what_the_lowest_value_masks(cdl, gpu_ok, dtype, vocab, tau):
+    """The loss of an entry whose logit is the type's lowest value is finite: temperature p 3.4e38.  Rounded: p and three operations,
+    2^-20; gradients are as they would be with any other mask."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    low = torch.finfo(dtype).min
+    logits = (torch.randn(5, vocab, generator=gen, device="cuda") * tau).to(dtype)
+    logits[:, 10:40] = low
+    ids = torch.tensor([[12, -1, -1], [12, 3, 50], [1, 2, 60], [13, 13, 5], [11, 12, 13]], dtype=torch.int32, device="cuda")
+    teacher = torch.randn(5, 3, generator=gen, device="cuda") * tau
+    o = cdl.ops.distillation(logits, ids, teacher, cdl.ops.DistillationOpts(temperature=tau))
+    loss, lse, grad = ref.distillation(logits.double(), ids, teacher, tau)
+    fits = loss < torch.finfo(F32).max
+    assert bool(fits[1:4].all()) and bool(torch.isfinite(o.loss[fits]).all())
+    _close("loss", o.loss[fits], loss[fits], 2.0 ** -20 * loss[fits] + 2.0 ** -16)
+    _close("d_logits", o.d_logits, grad, (HALF[dtype] + 2.0 ** -10 + _stat(vocab)) * grad.abs() + 2.0 ** -17 * _hit(ids, vocab) + 1e-9)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t", [6, 40, 200])
+def test_target_that_the_lowest_value_masks(cdl, gpu_ok, dtype, t):
+    """The same from hidden states that pick one row of w each (the logits are w's values): x is one-hot."""
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    low = torch.finfo(BF16).min / 2
+    x = torch.zeros(t, 64, device="cuda")
+    x[torch.arange(t), torch.arange(t) % 64] = 1.0
+    w = torch.randn(64, 3000, generator=gen, device="cuda").to(BF16)
+    w[:, 10:40] = low
+    targets = torch.where(torch.arange(t, device="cuda") % 3 == 0, 12, 50).to(torch.int32)
+    o = cdl.ops.linear_cross_entropy(x.to(dtype), w.to(dtype), targets)
+    loss, lse, g, dx, _ = ref.linear(x, w, lambda z: ref.cross_entropy(z, targets.long()))
+    # w has 8 bits: one piece, a sum of one term
+    _close("lse", o.lse, lse, _stat(3000) * (2 + lse.abs()) + 2.0 ** -20 * (1 + 0 * lse))
+    _close("loss", o.loss, loss, 2.0 ** -20 * loss + 2.0 ** -17)
