@@ -337,3 +337,52 @@ def test_target_that_the_lowest_value_masks(cdl, gpu_ok, dtype, t):
     # w has 8 bits: one piece, a sum of one term
     _close("lse", o.lse, lse, _stat(3000) * (2 + lse.abs()) + 2.0 ** -20 * (1 + 0 * lse))
     _close("loss", o.loss, loss, 2.0 ** -20 * loss + 2.0 ** -17)
+
+
+@gpu
+@pytest.mark.parametrize("t,v,k,dtype", [(70000, 32776, 0, BF16), (70000, 32776, 7, BF16), (24000, 100003, 0, F32)])
+def test_gradients_beyond_32_bit_offsets(cdl, gpu_ok, t, v, k, dtype):
+    """More than 2^31 logits in one chunk of rows, against the same call in chunks of the library's choice: statistics have the same bits,
+    gradients are sums of the same d z over other K slices and chunks (how many depends on the rows of a chunk).  bf16: a sum of V or t terms in
+    steps of 16 that cut 2^-23 each, 4375 at most, twice: 2^-10 of a value, and dx rounded to half a step on either side.  f32: parts of
+    256, rounded to nearest, 400 of them, and 16 steps within: 2 * 416 * 2^-24 < 2^-14."""
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    assert t * v > 2 ** 31
+    x, w = _operands(gen, t, 64, v, dtype, "rows")
+    entries = _entries(gen, t, v, k)
+    fn = cdl.ops.linear_cross_entropy if k == 0 else cdl.ops.linear_distillation
+    o, p = (fn(x, w, *entries, cdl.ops.LinearLossOpts(chunk_rows=c), dw=torch.empty(64, v, device="cuda")) for c in (t, 0))
+    assert torch.equal(o.loss, p.loss) and torch.equal(o.lse, p.lse)
+    sums = 2.0 ** -10 if dtype == BF16 else 2.0 ** -14
+    assert (o.dx.double() - p.dx.double()).norm() <= (2 * HALF[dtype] + sums) * p.dx.double().norm()
+    assert (o.dw - p.dw).norm() <= sums * p.dw.norm()
+    rows = slice(t - 100, t)
+    _check_linear(cdl, x[rows], w, [e[rows] for e in entries], cdl.ops.LinearLossOpts())
+    tail = fn(x[rows], w, *[e[rows] for e in entries])
+    assert (o.dx[rows].double() - tail.dx.double()).norm() <= (2 * HALF[dtype] + sums) * tail.dx.double().norm()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,t", [(F32, 12), (F32, 300), (BF16, 50), (BF16, 3)])
+def test_captured_calls_of_every_form_replay_with_new_inputs(cdl, gpu_ok, dtype, t):
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    x, w = _operands(gen, t, 96, 3001, dtype, "tied")
+    targets = _entries(gen, t, 3001, 0)[0]
+    dw = torch.zeros(3001, 96, device="cuda").t()
+    opts = cdl.ops.LinearLossOpts(accumulate=True)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        cdl.ops.linear_cross_entropy(x, w, targets, opts, dw=dw)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        o = cdl.ops.linear_cross_entropy(x, w, targets, opts, dw=dw)
+    for _ in range(2):
+        x.normal_(generator=gen)
+        targets.random_(0, 3001, generator=gen)
+        want = torch.zeros(3001, 96, device="cuda").t()
+        p = cdl.ops.linear_cross_entropy(x, w, targets, opts, dw=want)
+        dw.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o.loss, p.loss) and torch.equal(o.dx, p.dx) and torch.equal(dw, want)
