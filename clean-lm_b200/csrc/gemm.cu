@@ -1347,8 +1347,7 @@ static int32_t analyze_operand(const char* name, const cdl_tensor* t, bool contr
 // slices), 256 x 2048 x 2048 15.4 -> 9.2 (4), 512 x 5632 x 2048 31.8 -> 16.9 (2); the other way at 2048 x 2048 x 2048, 17.2 against
 // 19.1, and for narrow outputs, where a wide tile's loads and store shrink with N: 128 x 32 x 64 3.4
 // against 5.0, 59 x (1024 x 32 x 128) 8.4 against 12.0, D += A^T B 200 x 32 x 4096 7.0 against 10.6; D += A^T B
-// 512 x 5632 x 5632, whose 176 tiles of 128 x 128 leave most SMs waiting for two, 30.6 against 42.6, and 2048 x 3072 x 5616, 384 tiles
-// to walk in turns of 148, 56 against 91.
+// 512 x 5632 x 5632, whose 176 tiles of 128 x 128 leave most SMs waiting for two, 30.6 against 42.6.
 static int choose_cluster_splits(long long batch, long long M, long long N, long long K, bool adds_f32,
                                  bool adds_bf16, bool may_slice, bool reduces, bool tma_adds) {
   auto up = [](long long a, long long b) { return (a + b - 1) / b; };
