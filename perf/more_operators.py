@@ -314,7 +314,7 @@ def _plain_plan(s):
     need = torch.where(fits, (c + a + page - 1) // page - old, 0)
     upto = need.cumsum(0)
     served = fits & ((need == 0) | (upto <= free))
-    left = free - torch.where(served, upto, 0).amax()
+    left = free - torch.where(served & (need > 0), upto, 0).amax()
     # the new entries of the block tables
     i = torch.arange(width, device="cuda")
     j = i[None, :] - old[:, None]
