@@ -106,6 +106,15 @@ class CdlHeadLossDesc(ctypes.Structure):
                 ("accumulate_dw", ctypes.c_int32), ("chunk_rows", ctypes.c_int64)]
 
 
+class CdlAttnDecodeDesc(ctypes.Structure):
+    _fields_ = [("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int32)]
+
+
+class CdlSampleDesc(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
+
+
 _BLOCK_PARAMS = ("norm1", "wqkv", "wo", "norm2", "wup", "wgate", "wdown")
 
 
@@ -128,8 +137,9 @@ if not LIB_PATH.exists():
     )
 
 lib = ctypes.CDLL(str(LIB_PATH))
-# The same library for callers that pass every `const cdl_tensor*` as the bytes of tensor_bytes() and every
-# `const cdl_head_loss_desc*` as those of head_loss_bytes(): nothing else is taken there.
+# The same library for callers that pass every `const cdl_tensor*` as the bytes of tensor_bytes(), and the descriptors of the
+# losses, of the decoding attention and of sampling as those of head_loss_bytes(), attn_decode_bytes() and sample_bytes():
+# nothing else is taken there.
 packed_lib = ctypes.CDLL(str(LIB_PATH))
 
 _T = ctypes.POINTER(CdlTensor)
@@ -137,6 +147,8 @@ _MX = ctypes.POINTER(CdlMxTensor)
 _MO = ctypes.POINTER(CdlMatmulOptions)
 _NO = ctypes.POINTER(CdlNormOptions)
 _HL = ctypes.POINTER(CdlHeadLossDesc)
+_AD = ctypes.POINTER(CdlAttnDecodeDesc)
+_SD = ctypes.POINTER(CdlSampleDesc)
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 
@@ -197,6 +209,11 @@ SIGNATURES = {
                                       ctypes.c_int32),
     "cdl_b200_attn_bwd_packed_scratch_bytes": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                 ctypes.POINTER(_sz)], ctypes.c_int32),
+    "cdl_b200_attn_decode": ([_AD, _T, _T, _T, _T, _T, _T, _T, _vp, _sz, _vp], ctypes.c_int32),
+    "cdl_b200_attn_decode_scratch_bytes": ([_T, _T, ctypes.POINTER(_sz)], ctypes.c_int32),
+    "cdl_b200_cache_plan": ([ctypes.c_int32, ctypes.c_int32, _T, _T, _T, _T, _T, _T, _T, _T, _T, _T, _vp], ctypes.c_int32),
+    "cdl_b200_cache_write": ([_T, _T, _T, _T, _T, _T, _T, _T, _T, _T, _vp], ctypes.c_int32),
+    "cdl_b200_sample": ([_SD, _T, _T, _T, _T, _T, _T, _T, _T, _vp], ctypes.c_int32),
     "cdl_b200_rope": ([_T, _T, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp], ctypes.c_int32),
     "cdl_b200_rope_ragged": ([_T, _T, ctypes.c_int32, _T, ctypes.c_int32, _vp], ctypes.c_int32),
     "cdl_b200_swiglu_fwd": ([_T, _T, _T, _vp], ctypes.c_int32),
@@ -238,9 +255,9 @@ SIGNATURES = {
 }
 
 for _name, (_args, _res) in SIGNATURES.items():
-    for _of, _tensor, _desc in ((lib, _T, _HL), (packed_lib, ctypes.c_char_p, ctypes.c_char_p)):
+    for _of in (lib, packed_lib):
         _fn = getattr(_of, _name)
-        _fn.argtypes = [_tensor if a is _T else _desc if a is _HL else a for a in _args]
+        _fn.argtypes = [ctypes.c_char_p if _of is packed_lib and a in (_T, _HL, _AD, _SD) else a for a in _args]
         _fn.restype = _res
 
 
@@ -287,6 +304,14 @@ def rows_bytes(ptr: int, n: int) -> bytes:
 _HEAD_LOSS_BYTES = struct.Struct("ffiq")  # the layout of cdl_head_loss_desc
 assert _HEAD_LOSS_BYTES.size == ctypes.sizeof(CdlHeadLossDesc)
 head_loss_bytes = _HEAD_LOSS_BYTES.pack  # (temperature, grad_scale, accumulate_dw, chunk_rows)
+
+_ATTN_DECODE_BYTES = struct.Struct("ffi")  # the layout of cdl_attn_decode_desc
+assert _ATTN_DECODE_BYTES.size == ctypes.sizeof(CdlAttnDecodeDesc)
+attn_decode_bytes = _ATTN_DECODE_BYTES.pack  # (softmax_scale, softcap, window)
+
+_SAMPLE_BYTES = struct.Struct("fiff")  # the layout of cdl_sample_desc
+assert _SAMPLE_BYTES.size == ctypes.sizeof(CdlSampleDesc)
+sample_bytes = _SAMPLE_BYTES.pack  # (temperature, top_k, top_p, min_p)
 
 
 def tensor_arg(t):

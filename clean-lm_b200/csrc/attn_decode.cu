@@ -1,0 +1,580 @@
+// Attention of one new token per request over a paged key-value cache.
+//
+//   s_j = f(scale q . k_j),  f(x) = cap tanh(x / cap) or x;   out = sum_j softmax(s)_j v_j over the keys a request sees,
+//   lse = log sum_j exp(s_j)
+//
+// Bound by reading the keys and values once (2 multiply-adds per 2-byte element and query head of a group; the tensor cores
+// see 8 or 16 query columns).  The 16-key tiles of all requests and kv heads form one line that the warps of the grid share
+// evenly, whatever the lengths are; a warp's running maximum, sum and output stay in registers.  Where a warp's share cuts the
+// keys of a (request, kv head), its partial result goes to the scratch and a second kernel joins them.
+//
+// Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
+// of mma.m16n8k16 (as rows they would leave at least half of it empty) and both K and V rows go from global memory straight
+// into the fragments, 16 bytes at a time: for the scores the order of d within a product is free, for the output the order of
+// its rows is.  (No shared memory, no barrier: a tile of the 5th-generation tensor cores has 64 or 128 rows of queries, of
+// which one token per request fills 1 to 16.)  Probabilities are rounded to bf16 for the second product, as in the prompt's
+// attention; their sum is of the unrounded ones, in f32.
+#include "ops.h"
+#include "ptx.cuh"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace cdl {
+namespace decode {
+
+constexpr int WARPS = 4;          // per CTA; each works alone
+constexpr int MAX_BATCH = 16384;  // the prefix of the lengths is kept in shared memory
+
+struct Params {
+  const __nv_bfloat16* q;
+  long long q_sb, q_sh;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  long long k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // page, slot, head
+  const int* table;
+  long long table_sb;
+  const int* lens;
+  int batch, heads, kv_heads, group, chunks;  // group: query heads of a kv head; chunks: of COLS of them
+  int pages, page_size, width, window;
+  float scale, cap;  // of the scores, in natural units; cap 0: none
+  __nv_bfloat16* out;
+  long long out_sb, out_sh;
+  float* lse;
+  int max_workers;
+  int* prefix;      // [batch + 1] tiles of the requests ahead
+  float* part_o;    // [2 max_workers][COLS][D]
+  float2* part_ml;  // [2 max_workers][COLS]
+};
+
+// Keys a request sees: [first, end).
+__device__ __forceinline__ void visible(const Params& p, int b, int& first, int& end) {
+  const long long most = static_cast<long long>(p.width) * p.page_size;
+  const int len = p.lens[b];
+  end = static_cast<int>(min(static_cast<long long>(max(len, 0)), most));
+  first = p.window > 0 ? max(0, end - p.window) : 0;
+}
+
+// How many warps share `units` tiles: all of them, but at least MIN_TILES for each (a cut costs its partial result's way
+// through memory, as much as the keys of two tiles for 8 query columns).
+constexpr int MIN_TILES = 4;
+__host__ __device__ __forceinline__ long long workers_of(long long units, int max_workers) {
+  const long long w = (units + MIN_TILES - 1) / MIN_TILES;
+  return w < 1 ? 1 : (w > max_workers ? max_workers : w);
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Keys and values are read once: they need not stay in the L1.
+__device__ __forceinline__ uint4 load_row(const __nv_bfloat16* p, bool live) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (live)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4& q, int i) { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
+__device__ __forceinline__ long long shfl64(long long x, int lane) { return __shfl_sync(0xffffffffu, x, lane); }
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Keys of a tile: 16 of D = 128, 32 of D = 64, 8 KB of keys and values either way.
+template <int D>
+constexpr int tile_keys() { return D == 128 ? 16 : 32; }
+
+// D: head dimension; NT: tiles of 8 query heads of one kv head.
+template <int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kernel(const Params p) {
+  constexpr int COLS = 8 * NT;
+  constexpr int KEYS = tile_keys<D>();
+  constexpr int SUB = KEYS / 16;   // 16-key products of a tile
+  constexpr int KCH = D / 32;      // 16-byte pieces of a key row per thread
+  constexpr int VCH = D / 64;      // 16-byte pieces of a value row per thread
+  constexpr int MT = D / 16;       // 16-row tiles of the transposed output
+  extern __shared__ int prefix[];  // [batch + 1]
+  __shared__ int warp_sum[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  // ---- the tiles ahead of each request
+  int run = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += WARPS * 32) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < p.batch) {
+      int first, end;
+      visible(p, b, first, end);
+      n = (end - first + KEYS - 1) / KEYS;
+    }
+    int x = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int before = run, all = run;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < p.batch) prefix[b] = before + x - n;
+    run = all;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[p.batch] = run;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= p.batch; b += WARPS * 32) p.prefix[b] = prefix[b];
+
+  const int rows = p.kv_heads * p.chunks;  // lines of tiles of a request
+  const long long units = static_cast<long long>(run) * rows;
+  if (units == 0) return;
+  const long long workers = workers_of(units, p.max_workers);
+  // neighbouring shares on different SMs, so that few of them are spread over the whole card
+  const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+  if (me >= workers) return;
+  long long u = units * me / workers;
+  const long long u_end = units * (me + 1) / workers;
+  const float sm2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
+  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
+
+  while (u < u_end) {
+    int b = 0;
+    {
+      const int at = static_cast<int>(u / rows);
+      int hi = p.batch;  // largest b with prefix[b] <= at
+      while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (prefix[mid] <= at) b = mid;
+        else hi = mid;
+      }
+    }
+    const int n = prefix[b + 1] - prefix[b];
+    const long long rest = u - static_cast<long long>(prefix[b]) * rows;
+    const int row = static_cast<int>(rest / n), t0 = static_cast<int>(rest - static_cast<long long>(row) * n);
+    const int t1 = static_cast<int>(min(static_cast<long long>(n), t0 + (u_end - u)));
+    const int kvh = row / p.chunks, col0 = (row - kvh * p.chunks) * COLS;
+    const int cols = min(COLS, p.group - col0);
+    const int head0 = kvh * p.group + col0;
+    int first, end;
+    visible(p, b, first, end);
+
+    // ---- q: thread (g, t) has the pieces t, t + 4, .. of column g
+    uint4 qf[NT][KCH];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < KCH; ++i)
+        qf[j][i] = load_row(p.q + b * p.q_sb + (head0 + j * 8 + g) * p.q_sh + (t + 4 * i) * 8, j * 8 + g < cols);
+
+    const int* table = p.table + b * p.table_sb;
+    const __nv_bfloat16* kb = p.k + kvh * p.k_sh + t * 8;
+    const __nv_bfloat16* vb = p.v + kvh * p.v_sh + g * 8;
+    // Lane l looks the page of the tile's key l up, one tile ahead of the loads that go there.
+    auto look_up = [&](int tile) {
+      const int key = first + tile * KEYS + (lane & (KEYS - 1));
+      return tile < t1 && key < end ? table[static_cast<unsigned>(key) / static_cast<unsigned>(p.page_size)] : -1;
+    };
+    long long at_k = -1, at_v = -1;  // where the row of key l lies; -1: not read
+    auto place = [&](int tile, int page) {
+      const int key = first + tile * KEYS + (lane & (KEYS - 1));
+      const int slot = static_cast<int>(static_cast<unsigned>(key) % static_cast<unsigned>(p.page_size));
+      const bool live = page >= 0 && page < p.pages;
+      at_k = live ? page * p.k_sp + slot * p.k_ss : -1;
+      at_v = live ? page * p.v_sp + slot * p.v_ss : -1;
+    };
+    uint4 kf[SUB][2][KCH], vf[SUB][4][VCH];
+    auto load_k = [&](bool (&live)[SUB][2]) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const long long at = shfl64(at_k, s * 16 + r * 8 + g);
+          live[s][r] = at >= 0;
+#pragma unroll
+          for (int i = 0; i < KCH; ++i) kf[s][r][i] = load_row(kb + at + i * 32, at >= 0);
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const long long at = shfl64(at_v, s * 16 + 2 * t + (r & 1) + (r >> 1) * 8);
+#pragma unroll
+          for (int i = 0; i < VCH; ++i) vf[s][r][i] = load_row(vb + at + i * 64, at >= 0);
+        }
+    };
+
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      m[j][0] = m[j][1] = -INFINITY;
+      l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+    }
+    bool live[SUB][2];
+    int page = look_up(t0);
+    place(t0, page);
+    page = look_up(t0 + 1);
+    load_k(live);
+    load_v();
+    for (int tile = t0; tile < t1; ++tile) {
+      // ---- scores^T: rows are keys, columns query heads
+      float s[SUB][NT][4];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          s[x][j][0] = s[x][j][1] = s[x][j][2] = s[x][j][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < KCH; ++i) {
+            mma_bf16(s[x][j], kf[x][0][i].x, kf[x][1][i].x, kf[x][0][i].y, kf[x][1][i].y, qf[j][i].x, qf[j][i].y);
+            mma_bf16(s[x][j], kf[x][0][i].z, kf[x][1][i].z, kf[x][0][i].w, kf[x][1][i].w, qf[j][i].z, qf[j][i].w);
+          }
+        }
+      bool had[SUB][2];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x) had[x][0] = live[x][0], had[x][1] = live[x][1];
+      // the next tile's keys, while this one's values are still on their way
+      if (tile + 1 < t1) {
+        place(tile + 1, page);
+        page = look_up(tile + 2);
+        load_k(live);
+      }
+      // ---- running softmax, in powers of 2
+      uint32_t pf[SUB][NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < SUB; ++x)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float y = s[x][j][c];
+            y = p.cap > 0.f ? cap2 * tanhf(y * to_cap) : y * sm2;
+            y = had[x][c >> 1] ? y : -INFINITY;
+            s[x][j][c] = y;
+            top[c & 1] = fmaxf(top[c & 1], y);
+          }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[j][0] || top[1] > m[j][1])) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float now = fmaxf(m[j][c], top[c]);
+            const float f = m[j][c] == -INFINITY ? 0.f : ex2(m[j][c] - now);
+            m[j][c] = now;
+            l[j][c] *= f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[j][i][c] *= f, o[j][i][c + 2] *= f;
+          }
+        }
+        const float m0 = m[j][0] == -INFINITY ? 0.f : m[j][0], m1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
+#pragma unroll
+        for (int x = 0; x < SUB; ++x) {
+          const float p0 = ex2(s[x][j][0] - m0), p1 = ex2(s[x][j][1] - m1);
+          const float p2 = ex2(s[x][j][2] - m0), p3 = ex2(s[x][j][3] - m1);
+          l[j][0] += p0 + p2;
+          l[j][1] += p1 + p3;
+          pf[x][j][0] = transpose_8x8(pack_bf16x2(p0, p1));
+          pf[x][j][1] = transpose_8x8(pack_bf16x2(p2, p3));
+        }
+      }
+      // ---- out^T += V^T p^T: row i of a 16-row tile is an element of piece g (and g + 8) of the value rows
+#pragma unroll
+      for (int x = 0; x < SUB; ++x)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          constexpr int H = D == 128 ? 0 : 2;  // D = 64: the upper 8 rows are the piece's upper half
+          const int w0 = i >> 1, w1 = (i >> 1) + H, c1 = VCH - 1;
+          const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
+          const uint32_t a0 = __byte_perm(word(vf[x][0][0], w0), word(vf[x][1][0], w0), sel);
+          const uint32_t a1 = __byte_perm(word(vf[x][0][c1], w1), word(vf[x][1][c1], w1), sel);
+          const uint32_t a2 = __byte_perm(word(vf[x][2][0], w0), word(vf[x][3][0], w0), sel);
+          const uint32_t a3 = __byte_perm(word(vf[x][2][c1], w1), word(vf[x][3][c1], w1), sel);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_bf16(o[j][i], a0, a1, a2, a3, pf[x][j][0], pf[x][j][1]);
+        }
+      if (tile + 1 < t1) load_v();
+    }
+
+    // ---- the sums over the keys; out, or the partial result
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
+    const bool whole = t0 == 0 && t1 == n;
+    const long long slot = (2 * me + (t0 == 0)) * COLS;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = j * 8 + 2 * t + c;
+        if (col >= cols) continue;
+        // element e of this thread's 8 (D = 128: in each half of the row)
+        float lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (D == 128) lo[e] = o[j][e % MT][c], hi[e] = o[j][e % MT][c + 2];
+          else lo[e] = e < 4 ? o[j][e & 3][c] : o[j][e & 3][c + 2];
+        }
+        if (whole) {
+          const float inv = l[j][c] == 0.f ? 0.f : 1.f / l[j][c];
+          __nv_bfloat16* to = p.out + b * p.out_sb + (head0 + col) * p.out_sh + g * 8;
+          uint4 w;
+          w.x = pack_bf16x2(lo[0] * inv, lo[1] * inv), w.y = pack_bf16x2(lo[2] * inv, lo[3] * inv);
+          w.z = pack_bf16x2(lo[4] * inv, lo[5] * inv), w.w = pack_bf16x2(lo[6] * inv, lo[7] * inv);
+          *reinterpret_cast<uint4*>(to) = w;
+          if (D == 128) {
+            w.x = pack_bf16x2(hi[0] * inv, hi[1] * inv), w.y = pack_bf16x2(hi[2] * inv, hi[3] * inv);
+            w.z = pack_bf16x2(hi[4] * inv, hi[5] * inv), w.w = pack_bf16x2(hi[6] * inv, hi[7] * inv);
+            *reinterpret_cast<uint4*>(to + 64) = w;
+          }
+          if (p.lse != nullptr && g == 0)
+            p.lse[static_cast<long long>(b) * p.heads + head0 + col] =
+                l[j][c] == 0.f ? -INFINITY : (m[j][c] + log2f(l[j][c])) * LN2;
+        } else {
+          float* to = p.part_o + (slot + col) * D + g * 8;
+          *reinterpret_cast<float4*>(to) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<float4*>(to + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
+          if (D == 128) {
+            *reinterpret_cast<float4*>(to + 64) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<float4*>(to + 68) = make_float4(hi[4], hi[5], hi[6], hi[7]);
+          }
+          if (g == 0) p.part_ml[slot + col] = make_float2(m[j][c], l[j][c]);
+        }
+      }
+    u += t1 - t0;
+  }
+}
+
+// Joins the partial results of a (request, head): one warp each, in the order of the keys.  Requests that see no key get
+// zeros and -inf here.
+template <int D, int COLS>
+__global__ void __launch_bounds__(WARPS * 32) attn_decode_join_kernel(const Params p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  if (item >= static_cast<long long>(p.batch) * p.heads) return;
+  const int b = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(b) * p.heads);
+  const int kvh = head / p.group, in = head - kvh * p.group, row = kvh * p.chunks + in / COLS, col = in % COLS;
+  const int ahead = p.prefix[b], n = p.prefix[b + 1] - ahead;
+  const int rows = p.kv_heads * p.chunks;
+  const long long units = static_cast<long long>(p.prefix[p.batch]) * rows;
+  constexpr int E = D / 32;  // elements of a lane
+  float sum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = 0.f;
+  float top = -INFINITY, l = 0.f;
+  if (n > 0) {
+    const long long workers = workers_of(units, p.max_workers);
+    const long long u0 = static_cast<long long>(ahead) * rows + static_cast<long long>(row) * n;
+    const long long w0 = ((u0 + 1) * workers - 1) / units, w1 = ((u0 + n) * workers - 1) / units;
+    if (w0 == w1) return;  // one warp had all of it
+    for (long long w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, p.part_ml[(2 * w + (w == w0)) * COLS + col].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (long long w = w0; w <= w1; ++w) {
+      const long long slot = (2 * w + (w == w0)) * COLS + col;
+      const float2 ml = p.part_ml[slot];
+      // (a maximum that is NaN does not occur; sums and outputs that are NaN stay so)
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+      const float* from = p.part_o + slot * D + lane * E;
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;
+      l += ml.y * (ml.x == -INFINITY ? 1.f : f);
+      if (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from);
+        sum[0] += f * x.x, sum[1] += f * x.y, sum[E - 2] += f * x.z, sum[E - 1] += f * x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(from);
+        sum[0] += f * x.x, sum[1] += f * x.y;
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* to = p.out + b * p.out_sb + head * p.out_sh + lane * E;
+  if (E == 4)
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[E - 2] * inv, sum[E - 1] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+  if (p.lse != nullptr && lane == 0) p.lse[item] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+}
+}  // namespace decode
+
+// Bytes of the scratch: tiles ahead of each request, then the partial results of 2 per warp.
+static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+static int tiles_of_columns(long long group) { return group <= 8 ? 1 : 2; }
+static int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
+static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tensor* k_cache) {
+  if (!q || !k_cache) return fail(CDL_ERR_INVALID, "%s: q and k_cache are required", op);
+  if (q->rank != 3 || q->dtype != CDL_BF16) return fail(CDL_ERR_INVALID, "%s: q must be bf16 [batch, heads, head_dim]", op);
+  if (k_cache->rank != 4 || k_cache->dtype != CDL_BF16)
+    return fail(CDL_ERR_INVALID, "%s: the caches must be bf16 [pages, page_size, kv_heads, head_dim]", op);
+  const long long d = q->shape[2];
+  if (d != 64 && d != 128) return fail(CDL_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128 (got %lld)", op, d);
+  if (k_cache->shape[3] != d) return fail(CDL_ERR_INVALID, "%s: head_dim of q and of the cache differ", op);
+  if (q->shape[0] < 0 || q->shape[0] > decode::MAX_BATCH)
+    return fail(CDL_ERR_UNSUPPORTED, "%s: at most %d requests (got %lld)", op, decode::MAX_BATCH, (long long)q->shape[0]);
+  if (k_cache->shape[2] <= 0 || q->shape[1] % k_cache->shape[2] != 0)
+    return fail(CDL_ERR_INVALID, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", op, (long long)q->shape[1],
+                (long long)k_cache->shape[2]);
+  if (q->shape[1] > 65536) return fail(CDL_ERR_UNSUPPORTED, "%s: at most 65536 heads", op);
+  return CDL_OK;
+}
+
+static size_t decode_scratch_bytes(long long batch, int nt, long long d) {
+  const size_t slots = 2ull * sm_count() * ctas_per_sm(nt) * decode::WARPS * 8 * nt;
+  return align256((batch + 1) * 4) + align256(slots * 8) + slots * d * 4;
+}
+
+// Rows of `d` elements from a 16-byte boundary on, whatever the strides of the outer dimensions.
+static int32_t check_rows(const char* op, const char* name, const cdl_tensor* t) {
+  const int last = t->rank - 1;
+  bool ok = (reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && (t->shape[last] <= 1 || t->stride[last] == 1);
+  for (int i = 0; i < last; ++i) ok = ok && (t->shape[i] <= 1 || (t->stride[i] % 8 == 0 && t->stride[i] >= 0));
+  return ok ? CDL_OK
+            : fail(CDL_ERR_INVALID, "%s: %s must have a contiguous last dimension, 16-byte aligned, and other strides that are multiples of 8",
+                   op, name);
+}
+
+int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* q, const cdl_tensor* k_cache,
+                            const cdl_tensor* v_cache, const cdl_tensor* block_table, const cdl_tensor* seq_lens,
+                            const cdl_tensor* out, const cdl_tensor* lse, void* scratch, size_t scratch_bytes,
+                            cudaStream_t stream) {
+  const char* op = "attn_decode";
+  if (!desc || !v_cache || !block_table || !seq_lens || !out)
+    return fail(CDL_ERR_INVALID, "%s: desc, v_cache, block_table, seq_lens and out are required", op);
+  CDL_CHECK(decode_shapes(op, q, k_cache));
+  const long long B = q->shape[0], H = q->shape[1], D = q->shape[2], Hkv = k_cache->shape[2];
+  const long long pages = k_cache->shape[0], page_size = k_cache->shape[1];
+  if (v_cache->rank != 4 || v_cache->dtype != CDL_BF16) return fail(CDL_ERR_INVALID, "%s: v_cache must have k_cache's type and shape", op);
+  for (int i = 0; i < 4; ++i)
+    if (v_cache->shape[i] != k_cache->shape[i]) return fail(CDL_ERR_INVALID, "%s: v_cache must have k_cache's type and shape", op);
+  if (page_size <= 0 || pages < 0 || pages > INT32_MAX || page_size > INT32_MAX)
+    return fail(CDL_ERR_INVALID, "%s: pages must be 0 to 2^31 - 1 and hold a key at least", op);
+  if (block_table->rank != 2 || block_table->dtype != CDL_I32 || block_table->shape[0] != B || block_table->shape[1] < 0 ||
+      (block_table->shape[1] > 1 && block_table->stride[1] != 1))
+    return fail(CDL_ERR_INVALID, "%s: block_table must be i32 [batch, pages of a request] with contiguous rows", op);
+  if (seq_lens->rank != 1 || seq_lens->dtype != CDL_I32 || seq_lens->shape[0] != B || (B > 1 && seq_lens->stride[0] != 1))
+    return fail(CDL_ERR_INVALID, "%s: seq_lens must be a packed i32 [batch]", op);
+  if (out->rank != 3 || out->dtype != CDL_BF16 || out->shape[0] != B || out->shape[1] != H || out->shape[2] != D)
+    return fail(CDL_ERR_INVALID, "%s: out must have q's type and shape", op);
+  if (lse && (lse->rank != 2 || lse->dtype != CDL_F32 || lse->shape[0] != B || lse->shape[1] != H ||
+              (H > 1 && lse->stride[1] != 1) || (B > 1 && lse->stride[0] != H)))
+    return fail(CDL_ERR_INVALID, "%s: lse must be a packed f32 [batch, heads]", op);
+  CDL_CHECK(check_rows(op, "q", q));
+  CDL_CHECK(check_rows(op, "k_cache", k_cache));
+  CDL_CHECK(check_rows(op, "v_cache", v_cache));
+  CDL_CHECK(check_rows(op, "out", out));
+  if (!(desc->softcap >= 0.f) || isinf(desc->softcap)) return fail(CDL_ERR_INVALID, "%s: softcap must be 0 (none) or positive", op);
+  if (isnan(desc->softmax_scale) || isinf(desc->softmax_scale)) return fail(CDL_ERR_INVALID, "%s: softmax_scale must be finite", op);
+  if (desc->window < 0) return fail(CDL_ERR_INVALID, "%s: window must be 0 (all keys) or positive", op);
+  if (B == 0 || H == 0) return CDL_OK;
+  const void* given[] = {q->ptr, seq_lens->ptr, out->ptr};
+  for (const void* x : given)
+    if (!x) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
+  const long long width = pages == 0 ? 0 : block_table->shape[1];
+  if (width > 0 && (!block_table->ptr || !k_cache->ptr || !v_cache->ptr)) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
+  if (!view_apart_from_itself(*out)) return fail(CDL_ERR_INVALID, "%s: elements of out overlap", op);
+  const cdl_tensor* ins[] = {q, k_cache, v_cache, block_table, seq_lens};
+  for (const cdl_tensor* i : ins)
+    if (!views_apart(*out, *i) || (lse && !views_apart(*lse, *i))) return fail(CDL_ERR_INVALID, "%s: an output overlaps an input", op);
+  if (lse && !views_apart(*out, *lse)) return fail(CDL_ERR_INVALID, "%s: out and lse overlap", op);
+  const long long group = H / Hkv;
+  const int nt = tiles_of_columns(group), cols = 8 * nt;
+  const long long chunks = (group + cols - 1) / cols, rows = Hkv * chunks;
+  const long long tile = D == 128 ? decode::tile_keys<128>() : decode::tile_keys<64>();
+  long long most = width > INT32_MAX / page_size ? INT32_MAX : width * page_size;  // keys of a request
+  if (desc->window > 0) most = std::min<long long>(most, desc->window);
+  const long long tiles = B * ((most + tile - 1) / tile);
+  if (tiles > INT32_MAX) return fail(CDL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles of keys in the block table", op);
+  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255) || scratch_bytes < decode_scratch_bytes(B, nt, D))
+    return fail(CDL_ERR_INVALID, "%s: scratch must be 256-byte aligned and hold %zu bytes", op, decode_scratch_bytes(B, nt, D));
+
+  const int full = sm_count() * ctas_per_sm(nt);
+  const int grid = static_cast<int>(std::min<long long>(full, decode::workers_of(tiles * rows, full)));
+  decode::Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q->ptr), p.q_sb = q->stride[0], p.q_sh = q->stride[1];
+  p.k = static_cast<const __nv_bfloat16*>(k_cache->ptr), p.v = static_cast<const __nv_bfloat16*>(v_cache->ptr);
+  p.k_sp = k_cache->stride[0], p.k_ss = k_cache->stride[1], p.k_sh = k_cache->stride[2];
+  p.v_sp = v_cache->stride[0], p.v_ss = v_cache->stride[1], p.v_sh = v_cache->stride[2];
+  p.table = static_cast<const int*>(block_table->ptr), p.table_sb = block_table->stride[0];
+  p.lens = static_cast<const int*>(seq_lens->ptr);
+  p.batch = static_cast<int>(B), p.heads = static_cast<int>(H), p.kv_heads = static_cast<int>(Hkv);
+  p.group = static_cast<int>(group), p.chunks = static_cast<int>(chunks);
+  p.pages = static_cast<int>(pages), p.page_size = static_cast<int>(page_size);
+  p.width = static_cast<int>(std::min<long long>(width, INT32_MAX)), p.window = desc->window;
+  p.scale = desc->softmax_scale > 0.f ? desc->softmax_scale : 1.f / sqrtf(static_cast<float>(D));
+  p.cap = desc->softcap;
+  p.out = static_cast<__nv_bfloat16*>(out->ptr), p.out_sb = out->stride[0], p.out_sh = out->stride[1];
+  p.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
+  p.max_workers = grid * decode::WARPS;
+  char* at = static_cast<char*>(scratch);
+  const size_t slots = 2ull * p.max_workers * cols;
+  p.prefix = reinterpret_cast<int*>(at), at += align256((B + 1) * 4);
+  p.part_ml = reinterpret_cast<float2*>(at), at += align256(slots * 8);
+  p.part_o = reinterpret_cast<float*>(at);
+
+  ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
+  void (*kernel)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1> : decode::attn_decode_kernel<128, 2>)
+                                            : (nt == 1 ? decode::attn_decode_kernel<64, 1> : decode::attn_decode_kernel<64, 2>);
+  void (*join)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
+                                          : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
+  const size_t smem = (B + 1) * sizeof(int);
+  if (smem > 40 * 1024)
+    CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
+  const long long joins = (B * H + decode::WARPS - 1) / decode::WARPS;
+  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(joins)), dim3(decode::WARPS * 32), 0, stream, p));
+  return CDL_OK;
+}
+
+}  // namespace cdl
+
+extern "C" {
+
+int32_t cdl_b200_attn_decode(const cdl_attn_decode_desc* desc, const cdl_tensor* q, const cdl_tensor* k_cache,
+                             const cdl_tensor* v_cache, const cdl_tensor* block_table, const cdl_tensor* seq_lens,
+                             const cdl_tensor* out, const cdl_tensor* lse, void* scratch, size_t scratch_bytes,
+                             cdl_stream stream) {
+  return cdl::attn_decode_execute(desc, q, k_cache, v_cache, block_table, seq_lens, out, lse, scratch, scratch_bytes,
+                                  static_cast<cudaStream_t>(stream));
+}
+int32_t cdl_b200_attn_decode_scratch_bytes(const cdl_tensor* q, const cdl_tensor* k_cache, size_t* bytes_out) {
+  if (!bytes_out) return cdl::fail(CDL_ERR_INVALID, "attn_decode: bytes_out is required");
+  CDL_CHECK(cdl::decode_shapes("attn_decode", q, k_cache));
+  *bytes_out = cdl::decode_scratch_bytes(q->shape[0], cdl::tiles_of_columns(q->shape[1] / k_cache->shape[2]), q->shape[2]);
+  return CDL_OK;
+}
+
+}  // extern "C"

@@ -124,6 +124,10 @@ int32_t swiglu_fwd_execute(const cdl_tensor* gate, const cdl_tensor* up, const c
 int32_t swiglu_bwd_execute(const cdl_tensor* d_act, const cdl_tensor* gate, const cdl_tensor* up,
                            const cdl_tensor* d_gate, const cdl_tensor* d_up, cudaStream_t stream);
 
+// cache.cu: whether two views provably share no element; whether no two indices of a view name the same one.
+bool views_apart(const cdl_tensor& a, const cdl_tensor& b);
+bool view_apart_from_itself(const cdl_tensor& t);
+
 // Block-scaled (MXFP8) tensors.
 int32_t mx_layout(int32_t format, int32_t dim, long long rows, long long cols, size_t* values_bytes,
                   size_t* scale_bytes);

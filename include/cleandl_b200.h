@@ -432,6 +432,91 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
                                       const cdl_tensor* dk, const cdl_tensor* dv, void* scratch,
                                       size_t scratch_bytes, cdl_stream stream);
 
+/* ---- Serving: a paged key-value cache, attention of new tokens over it, sampling -------------------
+ * k_cache and v_cache are bf16 [pages, page_size, kv_heads, head_dim] of any page size, the last dimension contiguous, base
+ * and other strides 16-byte aligned (a permuted view of [pages, kv_heads, page_size, head_dim] is fine).  Key j of request b
+ * lies in slot j % page_size of page block_table[b][j / page_size]; the slot number of a key is page * page_size + slot.
+ * One step of a batch is cdl_b200_cache_plan, once; and per layer cdl_b200_cache_write and cdl_b200_attn_decode (for a prompt:
+ * cdl_b200_attn_fwd_packed over the new rows); then cdl_b200_sample.  Nothing of it reads a length on the host, so a step can be
+ * captured once and replayed. */
+
+/* Attention of one new token per request (the reference's attention with KvLayout::Paged and split-KV,
+ * crates/cleandl/src/execgraph/ops/attention/mod.rs:83-91, 129-130):
+ *   s_j = f(scale q . k_j), f(x) = softcap tanh(x / softcap) or x;  out = sum_j softmax(s)_j v_j;  lse = log sum_j exp(s_j)
+ * over the keys j in [max(0, n - window), n), n = seq_lens[b] (the new token's key among them), at most block_table's width
+ * times page_size.  q and out bf16 [batch, heads, head_dim], last dimension contiguous, other strides and base 16-byte
+ * aligned, head_dim 64 or 128, heads a multiple of kv_heads; block_table i32 [batch, width], contiguous rows; seq_lens packed
+ * i32 [batch]; lse (nullable) packed f32 [batch, heads].  out overlaps no input.
+ * Keys of a page outside [0, pages) are not read and do not count, nor does a key whose score is -inf.  A request in which no
+ * key counts (an empty one among them) has zeros in out and lse -inf; a NaN or +inf among its scores makes its results NaN.
+ * What the cache holds behind a request's last key may be anything.  Statistics and sums are f32; probabilities are rounded to
+ * bf16 for their product with the values, as in cdl_b200_attn_fwd.  Results do not depend on timing.
+ * Scratch: 256-byte aligned, of the size that the call below gives; calls that may run at the same time have one each. */
+typedef struct {
+  float softmax_scale; /* <= 0 selects 1/sqrt(head_dim) */
+  float softcap;       /* 0: none */
+  int32_t window;      /* keys that a token sees, its own among them; 0: all */
+} cdl_attn_decode_desc;
+int32_t cdl_b200_attn_decode(const cdl_attn_decode_desc* desc, const cdl_tensor* q, const cdl_tensor* k_cache,
+                             const cdl_tensor* v_cache, const cdl_tensor* block_table, const cdl_tensor* seq_lens,
+                             const cdl_tensor* out, const cdl_tensor* lse, void* scratch, size_t scratch_bytes,
+                             cdl_stream stream);
+int32_t cdl_b200_attn_decode_scratch_bytes(const cdl_tensor* q, const cdl_tensor* k_cache, size_t* bytes_out);
+
+/* What a step's new tokens get, from request lengths on the device: pages off a stack of free ones, block tables, positions and
+ * slots.  With c = cached[b] tokens in the cache, a = added[b] new ones (negative: 0) and E_b the sum of a up to b:
+ *   need_b = ceil((c + a) / page_size) - ceil(c / page_size) pages, C_b the sum of them up to b
+ * in the order of the requests, which take free_pages[free_count - 1], free_pages[free_count - 2], ..  A request is not served
+ * if its pages would go past block_table's width or its rows past `rows`, or if it needs pages and C_b > free_count: its
+ * tokens get no slot, seq_lens[b] stays c and no page is taken for it (after one that the stack does not suffice for, only
+ * requests that need none are served).
+ *   block_table i32 [requests, width], contiguous rows: entries of pages in use are read, new ones written
+ *   seq_lens [requests]: c + a, c if not served;  cu_seqlens [requests + 1]: 0 and E_b, at most rows
+ *   positions, slots [rows]: rows cu_seqlens[b] .. cu_seqlens[b + 1] are request b's new tokens, at positions c, c + 1, ..;
+ *     slot -1 where a request is not served or a page lies outside [0, pages); both -1 behind the last request's rows
+ *   free_left [1]: free_count less the pages taken
+ * All are packed i32; free_count [1] is at most the stack's size.  No output overlaps an input or another one.  page_size *
+ * pages < 2^31. */
+int32_t cdl_b200_cache_plan(int32_t page_size, int32_t pages, const cdl_tensor* cached, const cdl_tensor* added,
+                            const cdl_tensor* block_table, const cdl_tensor* free_pages, const cdl_tensor* free_count,
+                            const cdl_tensor* seq_lens, const cdl_tensor* cu_seqlens, const cdl_tensor* positions,
+                            const cdl_tensor* slots, const cdl_tensor* free_left, cdl_stream stream);
+
+/* New keys and values into their slots, after the rotary embedding of q and k (as cdl_b200_rope does it, crates/sky-1/src/
+ * training/model/decoder.rs:363-378): q_out = RoPE(q), k_out = RoPE(k), k_cache[slots[i]] = RoPE(k[i]), v_cache[slots[i]] = v[i].
+ * q, q_out bf16 [tokens, heads, head_dim], k, v, k_out [tokens, kv_heads, head_dim] (views of one fused tensor, say): last
+ * dimension contiguous, other strides and base 16-byte aligned, head_dim a multiple of 16.  q_out may be q itself, k_out k;
+ * otherwise outputs overlap neither inputs nor one another.  q with q_out, k_out, and cos_sin with positions are nullable (no
+ * rotation then, and neither q nor k_out).  cos_sin packed f32 [table rows, head_dim] as for cdl_b200_rope; positions, slots packed
+ * i32 [tokens].  A token whose position is outside the table is not rotated; one whose slot is outside the cache is not
+ * stored.  A slot may occur once among a call's tokens. */
+int32_t cdl_b200_cache_write(const cdl_tensor* q, const cdl_tensor* k, const cdl_tensor* v, const cdl_tensor* cos_sin,
+                             const cdl_tensor* positions, const cdl_tensor* slots, const cdl_tensor* q_out,
+                             const cdl_tensor* k_out, const cdl_tensor* k_cache, const cdl_tensor* v_cache, cdl_stream stream);
+
+/* A token per row of logits (bf16 or f32 [rows, vocab], contiguous rows, vocab at most 2^30), drawn by uniform[row] in [0, 1).
+ * With w_i = exp((z_i - max z) / temperature) and the entries in the order of falling logits, the lowest index first among
+ * equals:
+ *   kept: the first min(top_k, m_p, m_m) entries, at least one; m_p = the least number of entries whose w sum to top_p of the
+ *         sum over the first top_k, m_m = the number of w_i >= min_p
+ *   token = the first kept i, by index, such that the w of the kept entries up to i sum to more than uniform times the sum
+ *         over all of them;  logprob = log(w_token / that sum)
+ * top_k <= 0, top_p >= 1 and min_p <= 0 (or NaN) keep all entries; min_p above 1 counts as 1.  temperature <= 0 (or NaN): the
+ * largest logit, the lowest index among equals, with logprob 0.  uniform below 0 or NaN counts as 0, from 1 on as the last number
+ * below it.  -inf: never drawn (masked vocabulary).  A row that holds a NaN or +inf, or -inf alone, has token -1 and logprob NaN.
+ * temperature, top_p, min_p (f32) and top_k (i32) are packed [rows], nullable: the values of desc for all rows.  token packed
+ * i32 [rows], logprob (nullable) packed f32 [rows]; neither overlaps an input.  Weights are f64, added in 64-bit fixed point:
+ * results do not depend on timing, nor on the number of rows. */
+typedef struct {
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} cdl_sample_desc;
+int32_t cdl_b200_sample(const cdl_sample_desc* desc, const cdl_tensor* logits, const cdl_tensor* uniform,
+                        const cdl_tensor* temperature, const cdl_tensor* top_k, const cdl_tensor* top_p, const cdl_tensor* min_p,
+                        const cdl_tensor* token, const cdl_tensor* logprob, cdl_stream stream);
+
 /* ---- Elementwise glue of the sky-1 block -----------------------------------------------
  * The reference's kernels for these lived in its legacy `cleandl::operators` module, which is
  * absent from its tree; the call sites are crates/sky-1/src/training/model/decoder.rs:363-378
