@@ -6,8 +6,8 @@
 //
 // The result is a whole number, so sums must not depend on the order in which threads add up, and a draw next to a border must
 // fall as it does in exact arithmetic: weights are f64 exponentials, rounded to multiples of 2^-S and added as 64-bit integers
-// (S = 62 - log2 of the vocabulary, so that no sum overflows; 2^-47 of the largest weight for 32768 entries, against 2^-24 in
-// f32, where one draw in a few hundred of a flat row would fall on another token).
+// (S = 62 - log2 of the vocabulary, 50 at most, so that no sum overflows; 2^-47 of the largest weight for 32768 entries, against
+// 2^-24 in f32, where one draw in a few hundred of a flat row would fall on another token).
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -27,12 +27,13 @@ constexpr int CAP = 2048;    // entries that are sorted at most
 constexpr int BINS = 2048;   // of the logits below the largest, in units of T ln 2 / BIN_PER
 constexpr int BIN_PER = 64;
 constexpr int TILES = 1024;  // of a row, whose sums are kept
+constexpr int SMALL = THREADS;  // entries of a list that are not sorted
 constexpr int LIST_K = 384;  // top_k up to which a bound from the threads' largest logits finds the candidates
 
 struct Params {
   const void* z;
   long long ld;
-  long long vocab;
+  int vocab;
   const float* u;
   const float *temperature, *top_p, *min_p;  // per row, nullable: the values below
   const int* top_k;
@@ -52,44 +53,86 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // of -inf
 // An entry as a number: larger logits first, then lower indices.
-__device__ __forceinline__ u64 packed(uint32_t key, long long i) {
+__device__ __forceinline__ u64 packed(uint32_t key, int i) {
   return (static_cast<u64>(key) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // of two bf16 each
+  uint32_t c;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+  return c;
+}
+
+// ---- A row of logits, as the 16-byte vectors that it touches.  What a kernel runs once it fetches once: code that is not fetched
+// bounds the smallest calls, so there is one copy of each pass and loops are unrolled where loads have to overlap only.
 template <typename T>
 struct Row {
-  static constexpr int N = 16 / sizeof(T);  // logits of a 16-byte vector
+  static constexpr int N = 16 / sizeof(T);  // logits of a vector
   const T* z;
-  long long vocab, vectors;
+  int vocab, vectors;
   int lead;  // logits between the 16-byte boundary and the row's first
-  __device__ __forceinline__ Row(const void* p, long long V) : z(static_cast<const T*>(p)), vocab(V) {
-    lead = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-    vectors = (V + lead + N - 1) / N;
+
+  // A vector at the row's ends: -inf in front of it and behind it; nothing outside the row is read.
+  __device__ __noinline__ static uint4 load_end(const T* z, int vocab, int i) {
+    uint4 q;
+    T* t = reinterpret_cast<T*>(&q);
+    for (int e = 0; e < N; ++e) t[e] = i + e >= 0 && i + e < vocab ? z[i + e] : static_cast<T>(-INFINITY);
+    return q;
   }
-  __device__ __forceinline__ long long first(long long v) const { return v * N - lead; }
-  // Vector v of the row, -inf in front of it and behind it; nothing outside the row is read.
-  __device__ __forceinline__ uint4 load(long long v) const {
-    const long long i = first(v);
-    if (i >= 0 && i + N <= vocab) return ld_nc_v4(z + i);
-    union {
-      T t[N];
-      uint4 q;
-    } r;
-#pragma unroll
-    for (int e = 0; e < N; ++e) r.t[e] = i + e >= 0 && i + e < vocab ? z[i + e] : static_cast<T>(-INFINITY);
-    return r.q;
+  __device__ __forceinline__ int first(int v) const { return v * N - lead; }
+  __device__ __forceinline__ uint4 load(int v) const {
+    const int i = first(v);
+    return i >= 0 && i <= vocab - N ? ld_nc_v4(z + i) : load_end(z, vocab, i);
   }
-  static __device__ __forceinline__ void values(const uint4& q, float (&x)[N]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (N == 8) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
-      else x[i] = __uint_as_float(w[i]);
-    }
-  }
-  __device__ __forceinline__ float at(long long i) const {
+  __device__ __forceinline__ float at(int i) const {
     if constexpr (N == 8) return __bfloat162float(z[i]);
     else return z[i];
+  }
+  // The largest value, NaN where there is one.
+  static __device__ __forceinline__ float top(const uint4& q) {
+    if constexpr (N == 8) {
+      const uint32_t a = max2(max2(q.x, q.y), max2(q.z, q.w));
+      return max_nan(bf16_lo(a), bf16_hi(a));
+    } else {
+      return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+    }
+  }
+  // f(vector, index of its first value) for the vectors v0, v0 + step, .. below v1, with D loads ahead.
+  template <int D, typename F>
+  __device__ __forceinline__ void each(int v0, int v1, int step, F f) const {
+    uint4 q[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+      if (v0 + i * step < v1) q[i] = load(v0 + i * step);
+#pragma unroll 1
+    for (int v = v0; v < v1; v += step) {
+      const uint4 now = q[0];
+#pragma unroll
+      for (int i = 0; i + 1 < D; ++i) q[i] = q[i + 1];
+      if (v + D * step < v1) q[D - 1] = load(v + D * step);
+      f(now, first(v));
+    }
+  }
+  // f(4 values, index of the first) of a vector.
+  template <typename F>
+  static __device__ __forceinline__ void fours(const uint4& q, int i, F f) {
+    if constexpr (N == 8) {
+      uint32_t a = q.x, b = q.y;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const float x[4] = {bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b)};
+        f(x, i + 4 * h);
+        a = q.z, b = q.w;
+      }
+    } else {
+      const float x[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+      f(x, i);
+    }
   }
 };
 
@@ -122,6 +165,43 @@ __device__ __forceinline__ u64 least_of(float top_p, u64 mass) {
   return q < 1 ? 1 : q;
 }
 
+// 2^(j/32), rounded to f64.
+__device__ const double POW2[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
+// w = exp((z - top) / T) in units of 2^-S: 2^((k + r) / 32) with (z - top) 32 log2(e) / T = k + r, |r| <= 1/2, from a table of
+// 2^(j/32) and the Taylor series up to r^6, whose rest is 4e-18 (the table-driven method of P. T. P. Tang, 1989).  S <= 50: the
+// addition of 2^52 rounds to whole units.
+struct Weight {
+  double top, per_t;  // 32 log2(e) / T
+  float least;        // 80 T ln 2 below the top, where w is less than half a unit (what is computed there has no meaning)
+  const double* pow2;
+  int bits;
+  __device__ __forceinline__ u64 operator()(float z) const {
+    constexpr double L = 0.6931471805599453094 / 32, MAGIC = 6755399441055744.0;  // 1.5 2^52
+    const double d = static_cast<double>(z) - top;
+    const double k = fma(d, per_t, MAGIC);
+    const int n = __double2loint(k);
+    const double r = fma(d, per_t, MAGIC - k);
+    double y = fma(r, L * L * L * L * L * L / 720, L * L * L * L * L / 120);
+    y = fma(r, y, L * L * L * L / 24);
+    y = fma(r, y, L * L * L / 6);
+    y = fma(r, y, L * L / 2);
+    y = fma(r, y, L) * r;
+    const double tab = pow2[n & 31];
+    y = fma(tab, y, tab);
+    y = __hiloint2double(__double2hiint(y) + (((n >> 5) + bits) << 20), __double2loint(y)) + 4503599627370496.0;
+    return z > least ? static_cast<u64>(__double_as_longlong(y)) & 0xFFFFFFFFFFFFFull : 0;
+  }
+};
+
 struct Shared {
   u64 list[CAP];
   union {
@@ -130,44 +210,21 @@ struct Shared {
     u64 wide_hist[256];
   };
   u64 tile[TILES];  // a CTA's tiles at their number in the row
-  double pow2[256];
+  double pow2[32];
   u64 sums[WARPS];
-  float fsums[WARPS];
+  float tops[WARPS];
   uint32_t rank_of[256];
-  float top_of[WARPS];
-  int at_of[WARPS];
+  Weight weight;
   // what the cluster's other CTAs read
   float top;
-  int at, bad;
+  int at;
   uint32_t count;
   u64 above, all;
   int mode, lo, hi;
   uint32_t before;
+  // what a CTA's threads tell one another
   u64 word;
-  long long index;
-};
-
-// w = exp((z - top) / T) in units of 2^-S: 2^x with x = (z - top) log2(e) / T, split into n + j / 256 + r with |r| <= 1/512, a table
-// of 2^(j/256) and the Taylor series of 2^r up to r^4, whose rest is 4e-17 (the table-driven method of P. T. P. Tang, 1989).
-struct Weight {
-  double top, per_t;  // log2(e) / T
-  const double* pow2;
-  int bits;
-  __device__ __forceinline__ u64 operator()(float z) const {
-    constexpr double L = 0.6931471805599453094, MAGIC = 6755399441055744.0;  // 1.5 2^52
-    const double x = (static_cast<double>(z) - top) * per_t;
-    if (!(x >= -70.0)) return 0;
-    const double k = fma(x, 256.0, MAGIC);
-    const int n = __double2loint(k);
-    const double r = fma(k - MAGIC, -1.0 / 256.0, x);
-    const double tab = pow2[n & 255];
-    const double poly = fma(fma(fma(r, L * L * L * L / 24, L * L * L / 6), r, L * L / 2), r, L) * r;
-    const long long v = __double_as_longlong(fma(tab, poly, tab));
-    const u64 m = (static_cast<u64>(v) & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull;
-    const int sh = 52 + 1023 - static_cast<int>(v >> 52) - (n >> 8) - bits;
-    if (sh <= 0) return m << -sh;
-    return sh < 64 ? (m + (1ull << (sh - 1))) >> sh : 0;
-  }
+  int index;
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 x) {
@@ -175,54 +232,61 @@ __device__ __forceinline__ u64 warp_sum(u64 x) {
   for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
   return x;
 }
+struct Sums {
+  u64 before, all;
+};
 // Sum over the threads ahead of this one, and over all of them.  Ends in a barrier.
-__device__ __forceinline__ u64 block_scan(u64 x, u64* sums, u64& all) {
+__device__ __noinline__ Sums block_scan(u64 x, u64* sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 y = x;
-#pragma unroll
+#pragma unroll 1
   for (int d = 1; d < 32; d <<= 1) {
     const u64 o = __shfl_up_sync(0xffffffffu, y, d);
     if (lane >= d) y += o;
   }
   if (lane == 31) sums[warp] = y;
   __syncthreads();
-  u64 before = y - x;
-  all = 0;
-#pragma unroll
+  Sums r{y - x, 0};
+#pragma unroll 2
   for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += sums[w];
-    all += sums[w];
+    const u64 v = sums[w];
+    if (w < warp) r.before += v;
+    r.all += v;
   }
   __syncthreads();
-  return before;
+  return r;
 }
 
 // a[0, n) in falling order, n <= CAP, all different; returns where it is, a or b.  Ends in a barrier.
-__device__ u64* sort_down(Shared& sh, u64* a, u64* b, int n) {
+__device__ __noinline__ u64* sort_down(uint32_t* rank_of, u64* a, u64* b, int n) {
   const int tid = threadIdx.x;
   if (n <= 256) {  // every entry counts those above it
     int p = 32;
     while (p < n) p <<= 1;
-    if (tid < 256) sh.rank_of[tid] = 0;
+    if (tid < 256) rank_of[tid] = 0;
     __syncthreads();
     const int i = tid & (p - 1), part = tid / p, parts = THREADS / p;
     if (i < n) {
       const u64 x = a[i];
       uint32_t r = 0;
+#pragma unroll 2
       for (int j = part; j < n; j += parts) r += a[j] > x;
-      atomicAdd(&sh.rank_of[i], r);
+      atomicAdd(&rank_of[i], r);
     }
     __syncthreads();
-    if (tid < n) b[sh.rank_of[tid]] = a[tid];
+    if (tid < n) b[rank_of[tid]] = a[tid];
     __syncthreads();
     return b;
   }
   int p = 512;
   while (p < n) p <<= 1;
   for (int i = n + tid; i < p; i += THREADS) a[i] = 0;
+#pragma unroll 1
   for (int k = 2; k <= p; k <<= 1)
+#pragma unroll 1
     for (int j = k >> 1; j > 0; j >>= 1) {
       __syncthreads();
+#pragma unroll 1
       for (int t = tid; t < p / 2; t += THREADS) {
         const int i = 2 * t - (t & (j - 1));  // the pairs i, i + j
         const u64 x = a[i], y = a[i + j];
@@ -233,253 +297,208 @@ __device__ u64* sort_down(Shared& sh, u64* a, u64* b, int n) {
   return a;
 }
 
-enum Mode { ALL = 0, WINDOW_P = 1, WINDOW_K = 2, LIST = 3, SLOW = 4 };
+__device__ __forceinline__ uint32_t key_in(u64 entry) { return static_cast<uint32_t>(entry >> 32); }
+__device__ __forceinline__ int index_in(u64 entry) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(entry)); }
 
-template <typename T>
-struct Work {
-  const Params& p;
-  Shared& sh;
-  Row<T> row;
-  long long r;
-  Weight weight;
+// The settings of a row.
+struct Settings {
+  int k;  // 0: all
+  float top_p, u;
+  uint32_t key_min;  // of min_p; entries below it are not kept
   double t;
-  float top, bin_scale;
-  uint32_t key_min;           // of min_p; entries below it are not kept
-  long long per_tile, tiles;  // vectors of a tile
-  static constexpr int N = Row<T>::N;
+};
+// How many units of `mass` lie in front of the draw.
+__device__ __forceinline__ u64 drawn(float u, u64 mass) {
+  bool rest;
+  return u > 0.f ? (u < 1.f ? share_of(u, mass, rest) : mass - 1) : 0;
+}
+__device__ __noinline__ void write_out(const Params& p, const Shared& sh, long long r, double t, int i, float x, u64 mass) {
+  p.token[r] = i;
+  if (p.logprob)
+    p.logprob[r] = static_cast<float>((static_cast<double>(x) - sh.weight.top) / t - log(ldexp(static_cast<double>(mass), -p.scale_bits)));
+}
 
-  __device__ __forceinline__ int bin(float x) const { return min(BINS - 1, static_cast<int>((top - x) * bin_scale)); }
+// The draw from a list of more than SMALL entries that holds all that may be kept.
+__device__ __noinline__ void draw_sorted(const Params& p, Shared& sh, const Settings& set, long long r, int n) {
+  const int tid = threadIdx.x;
+  const u64* order = sort_down(sh.rank_of, sh.list, sh.other, n);
+  u64* spare = order == sh.list ? sh.other : sh.list;
+  const int per = (n + THREADS - 1) / THREADS;  // neighbouring entries of a thread
+  const int first = min(n, tid * per), last = min(n, first + per);
+  u64 sum = 0;
+  for (int i = first; i < last; ++i) sum += sh.weight(of_key(key_in(order[i])));
+  u64 upto = block_scan(sum, sh.sums).before;
+  for (int i = first; i < last; ++i) {
+    upto += sh.weight(of_key(key_in(order[i])));
+    spare[i] = upto;
+  }
+  __syncthreads();
+  const int n_k = set.k > 0 && set.k < n ? set.k : n;
+  const u64 want_p = set.top_p < 1.f ? least_of(set.top_p, spare[n_k - 1]) : ~0ull;
+  u64 keeps = 0;
+  for (int i = first; i < min(n_k, last); ++i) keeps += (i == 0 || spare[i - 1] < want_p) && key_in(order[i]) >= set.key_min;
+  const int kept = max(1, static_cast<int>(block_scan(keeps, sh.sums).all));
+  const u64 mass = spare[kept - 1], want = drawn(set.u, mass);
+  __syncthreads();
+  // by index
+  for (int i = tid; i < kept; i += THREADS) spare[i] = (order[i] << 32) | (order[i] >> 32);
+  __syncthreads();
+  const u64* line = sort_down(sh.rank_of, spare, const_cast<u64*>(order), kept);
+  sum = 0;
+  for (int i = first; i < min(kept, last); ++i) sum += sh.weight(of_key(static_cast<uint32_t>(line[i])));
+  u64 ahead = block_scan(sum, sh.sums).before;
+  for (int i = first; i < min(kept, last); ++i) {
+    const float x = of_key(static_cast<uint32_t>(line[i]));
+    const u64 w = sh.weight(x);
+    if (ahead <= want && want < ahead + w) write_out(p, sh, r, set.t, index_in(line[i] >> 32), x, mass);
+    ahead += w;
+  }
+}
 
-  __device__ __forceinline__ void write(long long i, float x, u64 mass) {
-    p.token[r] = static_cast<int>(i);
-    if (p.logprob)
-      p.logprob[r] = static_cast<float>((static_cast<double>(x) - static_cast<double>(top)) / t -
-                                        log(ldexp(static_cast<double>(mass), -p.scale_bits)));
+// The draw from up to SMALL entries: each is held against all others, by 32 threads at most, once for what is ahead of it in
+// falling order and once for what is ahead of it by index.
+__device__ __noinline__ void draw_small(const Params& p, Shared& sh, const Settings& set, long long r, int n) {
+  const int tid = threadIdx.x;
+  int parts = 32;
+  while (parts * n > THREADS) parts >>= 1;
+  const int i = tid / parts, part = tid & (parts - 1);
+  for (int j = tid; j < n; j += THREADS) sh.other[j] = sh.weight(of_key(key_in(sh.list[j])));
+  __syncthreads();
+  const u64 me = i < n ? sh.list[i] : 0, w = i < n ? sh.other[i] : 0;
+  u64 ahead = 0;
+  uint32_t rank = 0;
+  if (i < n)
+#pragma unroll 2
+    for (int j = part; j < n; j += parts)
+      if (sh.list[j] > me) ahead += sh.other[j], ++rank;
+  for (int d = 1; d < parts; d <<= 1) {
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+    rank += __shfl_xor_sync(0xffffffffu, rank, d);
   }
-  // How many units of `mass` lie in front of the draw.
-  __device__ __forceinline__ u64 drawn(u64 mass) const {
-    const float u = p.u[r];
-    bool rest;
-    return u > 0.f ? (u < 1.f ? share_of(u, mass, rest) : mass - 1) : 0;
+  bool kept = i < n && (set.k == 0 || rank < static_cast<uint32_t>(set.k));
+  if (set.top_p < 1.f) {
+    const u64 mass = block_scan(kept && part == 0 ? w : 0, sh.sums).all;
+    kept = kept && (rank == 0 || ahead < least_of(set.top_p, mass));
   }
+  kept = kept && (key_in(me) >= set.key_min || rank == 0);
+  if (part == 0 && i < n && !kept) sh.other[i] = 0;
+  const u64 mass = block_scan(kept && part == 0 ? w : 0, sh.sums).all;
+  const u64 want = drawn(set.u, mass);
+  ahead = 0;
+  if (i < n)
+#pragma unroll 2
+    for (int j = part; j < n; j += parts)
+      if (static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(me)) ahead += sh.other[j];
+  for (int d = 1; d < parts; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+  if (kept && part == 0 && ahead <= want && want < ahead + w) write_out(p, sh, r, set.t, index_in(me), of_key(key_in(me)), mass);
+}
 
-  // f(vector's values, index of its first) over [v0, v1), four loads under way.
-  template <typename F>
-  __device__ __forceinline__ void each(long long v0, long long v1, int from, int step, F f) const {
-    for (long long v = v0 + from; v < v1; v += 4 * step) {
-      uint4 q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (v + i * step < v1) q[i] = row.load(v + i * step);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (v + i * step < v1) {
-          float x[N];
-          Row<T>::values(q[i], x);
-          f(x, row.first(v + i * step));
-        }
-    }
-  }
-  __device__ __forceinline__ void append(uint32_t key, long long i) {
-    const uint32_t at = atomicAdd(&sh.count, 1u);
-    if (at < CAP) sh.list[at] = packed(key, i);
-  }
-
-  // Sums of the tiles [t0, t1): of the entries that are kept, which are those from `cut` on, without those below key_min.
-  __device__ void sum_tiles(long long t0, long long t1, u64 cut) {
-    const int lane = threadIdx.x & 31;
-    const uint32_t least = max(key_min, KEY_NONE + 1);
-    for (long long tile = t0 + (threadIdx.x >> 5); tile < t1; tile += WARPS) {
-      u64 sum = 0;
-      each(tile * per_tile, min(row.vectors, (tile + 1) * per_tile), lane, 32, [&](const float (&x)[N], long long i) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const uint32_t key = key_of(x[e]);
-          if (key >= least && packed(key, i + e) >= cut) sum += weight(x[e]);
-        }
-      });
-      sum = warp_sum(sum);
-      if (lane == 0) sh.tile[tile] = sum;
-    }
-  }
-  // The draw from the tiles' sums, which all of the block see.
-  __device__ void draw_tiles(u64 cut) {
-    const int tid = threadIdx.x;
-    const u64 a = 2 * tid < tiles ? sh.tile[2 * tid] : 0, b = 2 * tid + 1 < tiles ? sh.tile[2 * tid + 1] : 0;
-    u64 mass;
-    const u64 before = block_scan(a + b, sh.sums, mass);
-    const u64 want = drawn(mass);
-    if (before <= want && want < before + a + b) {
-      const bool second = want >= before + a;
-      sh.index = 2 * tid + second;
-      sh.word = second ? before + a : before;
+// The entry at which the sum over the entries from `cut` on, in falling order, reaches `want`: of their weights, or their number.
+// 8 bits of the logit at a time, then by index.  For windows that hold more than CAP entries: equal logits by the thousand,
+// logits far from any scale that the bins have.
+template <typename T>
+__device__ __noinline__ u64 select(const Row<T>& row, Shared& sh, bool weights, u64 want, u64 cut) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Weight weight = sh.weight;
+  uint32_t prefix = 0;
+  u64 above = 0;
+#pragma unroll 1
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) sh.wide_hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < row.vocab; i += THREADS) {
+      const float x = row.at(i);
+      const uint32_t key = key_of(x);
+      if (key > KEY_NONE && packed(key, i) >= cut && (shift == 24 || (key >> (shift + 8)) == prefix))
+        atomicAdd(&sh.wide_hist[(key >> shift) & 255], weights ? weight(x) : 1);
     }
     __syncthreads();
-    u64 ahead = sh.word;
-    const uint32_t least = max(key_min, KEY_NONE + 1);
-    const long long i0 = max(0LL, row.first(sh.index * per_tile));
-    const long long i1 = min(row.vocab, row.first((sh.index + 1) * per_tile));
-    for (long long base = i0; base < i1 && ahead <= want; base += THREADS) {
-      const long long i = base + tid;
-      float x = -INFINITY;
-      u64 w = 0;
-      if (i < i1) {
-        x = row.at(i);
-        const uint32_t key = key_of(x);
-        if (key >= least && packed(key, i) >= cut) w = weight(x);
+    if (tid == 0) {
+      u64 sum = above;
+      int bin = 255;
+      while (bin > 0 && sum + sh.wide_hist[bin] < want) sum += sh.wide_hist[bin--];
+      sh.index = static_cast<int>((prefix << 8) | static_cast<uint32_t>(bin));
+      sh.word = sum;
+    }
+    __syncthreads();
+    prefix = static_cast<uint32_t>(sh.index);
+    above = sh.word;
+    __syncthreads();
+  }
+  // how many of the entries equal to it, the lowest indices first
+  const u64 one = weights ? weight(of_key(prefix)) : 1;
+  const u64 ties = one == 0 ? 1 : (want - above + one - 1) / one;
+  const int seg = static_cast<int>((static_cast<long long>(row.vocab) + THREADS * WARPS - 1) / (THREADS * WARPS) * THREADS);
+  const int i0 = static_cast<int>(min(static_cast<long long>(row.vocab), static_cast<long long>(warp) * seg));
+  const int i1 = static_cast<int>(min(static_cast<long long>(row.vocab), static_cast<long long>(i0) + seg));
+  auto is = [&](int i) {
+    const uint32_t key = key_of(row.at(i));
+    return key == prefix && packed(key, i) >= cut;
+  };
+  u64 n = 0;
+  for (int i = i0 + lane; i < i1; i += 32) n += is(i);
+  u64 before = __shfl_sync(0xffffffffu, block_scan(n, sh.sums).before, 0);
+  n = warp_sum(n);
+  if (tid == 0) sh.word = packed(prefix, -1);  // all of them
+  __syncthreads();
+  if (before < ties && before + n >= ties) {
+    for (int i = i0; i < i1; i += 32) {
+      const bool hit = i + lane < i1 && is(i + lane);
+      const unsigned mask = __ballot_sync(0xffffffffu, hit);
+      if (before + __popc(mask) >= ties) {
+        if (hit && before + __popc(mask & ((2u << lane) - 1)) == ties) sh.word = packed(prefix, i + lane);
+        break;
       }
-      u64 all;
-      const u64 upto = ahead + block_scan(w, sh.sums, all);
-      if (upto <= want && want < upto + w) write(i, x, mass);
-      ahead += all;
+      before += __popc(mask);
     }
   }
+  __syncthreads();
+  const u64 at = sh.word;
+  __syncthreads();
+  return at;
+}
+// Sums of all tiles, of the entries from `cut` on without those below key_min.
+template <typename T>
+__device__ __noinline__ void sum_tiles(const Row<T>& row, Shared& sh, int per_tile, int tiles, u64 cut, uint32_t key_min) {
+  const int lane = threadIdx.x & 31;
+  const Weight weight = sh.weight;
+  const uint32_t least = max(key_min, KEY_NONE + 1);
+  for (int tile = threadIdx.x >> 5; tile < tiles; tile += WARPS) {
+    const int i0 = max(0, row.first(tile * per_tile)), i1 = min(row.vocab, row.first(min(row.vectors, (tile + 1) * per_tile)));
+    u64 sum = 0;
+    for (int i = i0 + lane; i < i1; i += 32) {
+      const float x = row.at(i);
+      const uint32_t key = key_of(x);
+      if (key >= least && packed(key, i) >= cut) sum += weight(x);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) sh.tile[tile] = sum;
+  }
+  __syncthreads();
+}
+// The cut of a row and its tiles' sums by one CTA alone, whatever the row is like.
+template <typename T>
+__device__ __noinline__ u64 slow_cut(const Row<T>& row, Shared& sh, const Settings& set, int per_tile, int tiles) {
+  u64 cut = 0;
+  __syncthreads();
+  if (set.k > 0) cut = select(row, sh, false, static_cast<u64>(set.k), 0);
+  if (set.top_p < 1.f) {
+    sum_tiles(row, sh, per_tile, tiles, cut, 0);
+    u64 sum = 0;
+    for (int i = threadIdx.x; i < tiles; i += THREADS) sum += sh.tile[i];
+    cut = select(row, sh, true, least_of(set.top_p, block_scan(sum, sh.sums).all), cut);
+  }
+  sum_tiles(row, sh, per_tile, tiles, cut, set.key_min);
+  return cut;
+}
 
-  // The draw where everything that may be kept is on the list.
-  __device__ void draw_list(int n, long long k_in, float top_p) {
-    const int tid = threadIdx.x;
-    u64* order = sort_down(sh, sh.list, sh.other, n);
-    u64* spare = order == sh.list ? sh.other : sh.list;
-    const int per = (n + THREADS - 1) / THREADS;  // neighbouring entries of a thread, 4 at most
-    u64 w[4], sum = 0, all;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      w[j] = j < per && i < n ? weight(of_key(static_cast<uint32_t>(order[i] >> 32))) : 0;
-      sum += w[j];
-    }
-    u64 upto = block_scan(sum, sh.sums, all);
-    const int n_k = k_in > 0 && k_in < n ? static_cast<int>(k_in) : n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      upto += w[j];
-      if (j < per && i < n) {
-        spare[i] = upto;
-      }
-    }
-    __syncthreads();
-    int kept = n_k;
-    const u64 want_p = top_p < 1.f ? least_of(top_p, spare[n_k - 1]) : ~0ull;
-    u64 less = 0;  // entries that are kept: below the sum, from the least key on
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      if (j < per && i < n_k) {
-        const u64 ahead = i == 0 ? 0 : spare[i - 1];
-        less += (i == 0 || ahead < want_p) && static_cast<uint32_t>(order[i] >> 32) >= key_min;
-      }
-    }
-    u64 count;
-    block_scan(less, sh.sums, count);
-    kept = max(1, static_cast<int>(count));
-    const u64 mass = spare[kept - 1];
-    const u64 want = drawn(mass);
-    __syncthreads();
-    // by index
-    for (int i = tid; i < kept; i += THREADS) spare[i] = (order[i] << 32) | (order[i] >> 32);
-    __syncthreads();
-    const u64* line = sort_down(sh, spare, order, kept);
-    sum = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      w[j] = j < per && i < kept ? weight(of_key(static_cast<uint32_t>(line[i]))) : 0;
-      sum += w[j];
-    }
-    u64 ahead = block_scan(sum, sh.sums, all);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      if (ahead <= want && want < ahead + w[j])
-        write(0xFFFFFFFFu - static_cast<uint32_t>(line[i] >> 32), of_key(static_cast<uint32_t>(line[i])), mass);
-      ahead += w[j];
-    }
-  }
-
-  // The entry at which the sum of f over the entries from `cut` on, in falling order, reaches `want`: 8 bits of the logit at a
-  // time, then by index.  For windows that hold more than CAP entries: equal logits by the thousand, logits far from any scale
-  // that the bins have.
-  template <typename F>
-  __device__ u64 select(F f, u64 want, u64 cut) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t prefix = 0;
-    u64 above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) sh.wide_hist[tid] = 0;
-      __syncthreads();
-      each(0, row.vectors, tid, THREADS, [&](const float (&x)[N], long long i) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const uint32_t key = key_of(x[e]);
-          if (key > KEY_NONE && packed(key, i + e) >= cut && (shift == 24 || (key >> (shift + 8)) == prefix))
-            atomicAdd(&sh.wide_hist[(key >> shift) & 255], f(x[e]));
-        }
-      });
-      __syncthreads();
-      if (tid == 0) {
-        u64 sum = above;
-        int bin = 255;
-        while (bin > 0 && sum + sh.wide_hist[bin] < want) sum += sh.wide_hist[bin--];
-        sh.index = (prefix << 8) | static_cast<uint32_t>(bin);
-        sh.word = sum;
-      }
-      __syncthreads();
-      prefix = static_cast<uint32_t>(sh.index);
-      above = sh.word;
-      __syncthreads();
-    }
-    // how many of the entries equal to it, the lowest indices first
-    const u64 one = f(of_key(prefix));
-    const u64 ties = one == 0 ? 1 : (want - above + one - 1) / one;
-    const long long seg = (row.vocab + THREADS * WARPS - 1) / (THREADS * WARPS) * THREADS;
-    const long long i0 = min(row.vocab, warp * seg), i1 = min(row.vocab, i0 + seg);
-    auto is = [&](long long i) {
-      const uint32_t key = key_of(row.at(i));
-      return key == prefix && packed(key, i) >= cut;
-    };
-    u64 n = 0, all;
-    for (long long i = i0 + lane; i < i1; i += 32) n += is(i);
-    u64 before = block_scan(n, sh.sums, all);
-    before = __shfl_sync(0xffffffffu, before, 0);
-    n = warp_sum(n);
-    if (tid == 0) sh.word = packed(prefix, 0xFFFFFFFFLL);  // all of them
-    __syncthreads();
-    if (before < ties && before + n >= ties) {
-      for (long long i = i0; i < i1; i += 32) {
-        const bool hit = i + lane < i1 && is(i + lane);
-        const unsigned mask = __ballot_sync(0xffffffffu, hit);
-        if (before + __popc(mask) >= ties) {
-          if (hit && before + __popc(mask & ((2u << lane) - 1)) == ties) sh.word = packed(prefix, i + lane);
-          break;
-        }
-        before += __popc(mask);
-      }
-    }
-    __syncthreads();
-    const u64 at = sh.word;
-    __syncthreads();
-    return at;
-  }
-  // One CTA alone, whatever the row is like.
-  __device__ void slow(long long k_in, float top_p) {
-    u64 cut = 0;
-    if (k_in > 0 && k_in < row.vocab) cut = select([](float) { return u64{1}; }, static_cast<u64>(k_in), 0);
-    if (top_p < 1.f) {
-      const uint32_t least = key_min;
-      key_min = 0;
-      sum_tiles(0, tiles, cut);
-      key_min = least;
-      __syncthreads();
-      u64 sum = 0, mass;
-      for (long long i = threadIdx.x; i < tiles; i += THREADS) sum += sh.tile[i];
-      block_scan(sum, sh.sums, mass);
-      cut = select(weight, least_of(top_p, mass), cut);
-    }
-    sum_tiles(0, tiles, cut);
-    __syncthreads();
-    draw_tiles(cut);
-  }
+// What the pass over the row's weights has to find.
+enum Mode {
+  ALL,       // everything (but what min_p leaves out) is kept
+  WINDOW_P,  // the cut of top_p lies in a window of bins
+  WINDOW_K,  // that of top_k
+  LIST,      // what may be kept fits on the list
+  SLOW       // one CTA alone searches
 };
 
 template <typename T>
@@ -494,320 +513,336 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     else __syncthreads();
   };
   auto of = [&](int other) -> Shared& { return C > 1 ? *cluster.map_shared_rank(&sh, other) : sh; };
-  if (tid < 256) sh.pow2[tid] = exp2(tid / 256.0);
-  if (tid == 0) sh.count = 0, sh.above = 0, sh.all = 0;
+  if (tid < 32) sh.pow2[tid] = POW2[tid];
+  if (tid == 0) sh.count = 0;
+  const long long r = blockIdx.x / C;
+  Row<T> row;
+  row.z = static_cast<const T*>(p.z) + r * p.ld;
+  row.vocab = p.vocab;
+  constexpr int N = Row<T>::N;
+  row.lead = static_cast<int>((reinterpret_cast<uintptr_t>(row.z) & 15) / sizeof(T));
+  row.vectors = (p.vocab + row.lead + N - 1) / N;
+  // vectors of a tile: 512 logits, or as many times that as leave at most TILES of them
+  constexpr int BASE = 512 / N;
+  const int per_tile = (row.vectors + BASE * TILES - 1) / (BASE * TILES) * BASE;
+  const int tiles = (row.vectors + per_tile - 1) / per_tile;
+  const int share = (tiles + C - 1) / C;  // tiles of a CTA
+  const int t0 = min(tiles, rank * share), t1 = min(tiles, t0 + share);
+  const int v0 = min(row.vectors, t0 * per_tile), v1 = min(row.vectors, t1 * per_tile);
   grid_dep_wait();
   grid_dep_launch();
-  const long long r = blockIdx.x / C;
-  Work<T> w{p, sh, Row<T>(static_cast<const T*>(p.z) + r * p.ld, p.vocab), r};
-  constexpr int N = Row<T>::N;
-  const long long vectors = w.row.vectors;
-  constexpr int BASE = 512 / N;  // vectors of a tile: 512 logits, or as many more as leave at most TILES of them
-  w.per_tile = (vectors + static_cast<long long>(BASE) * TILES - 1) / (static_cast<long long>(BASE) * TILES) * BASE;
-  w.tiles = (vectors + w.per_tile - 1) / w.per_tile;
-  const long long share = (w.tiles + C - 1) / C;  // tiles of a CTA
-  const long long t0 = min(w.tiles, rank * share), t1 = min(w.tiles, t0 + share);
-  const long long v0 = min(vectors, t0 * w.per_tile), v1 = min(vectors, t1 * w.per_tile);
-  const float temperature = p.temperature ? p.temperature[r] : p.all_temperature;
-  const long long k_in = p.top_k ? p.top_k[r] : p.all_top_k;
-  const float top_p = p.top_p ? p.top_p[r] : p.all_top_p;
-  const float min_p = p.min_p ? p.min_p[r] : p.all_min_p;
 
-  // ---- the largest logit and its first place; NaN and +inf
+  // ---- the largest logit; NaN and +inf
   float mine = -INFINITY;
-  int at = 0;
-  bool bad = false;
-  w.each(v0, v1, tid, THREADS, [&](const float (&x)[N], long long i) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      bad |= !(x[e] < INFINITY);
-      if (x[e] > mine) mine = x[e], at = static_cast<int>(i) + e;
-    }
-  });
+  row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int) { mine = max_nan(mine, Row<T>::top(q)); });
+  const float temperature = p.temperature ? p.temperature[r] : p.all_temperature;
+  const float min_p = p.min_p ? p.min_p[r] : p.all_min_p;
+  Settings set;
+  set.k = p.top_k ? p.top_k[r] : p.all_top_k;
+  set.top_p = p.top_p ? p.top_p[r] : p.all_top_p;
+  set.u = p.u[r];
+  if (set.k < 0 || set.k >= p.vocab) set.k = 0;
+  const bool p_on = set.top_p < 1.f;
   float top = mine;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const float x = __shfl_xor_sync(0xffffffffu, top, d);
-    const int y = __shfl_xor_sync(0xffffffffu, at, d);
-    if (x > top || (x == top && y < at)) top = x, at = y;
+  for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) sh.tops[warp] = top;
+  __syncthreads();
+  top = sh.tops[lane & (WARPS - 1)];
+#pragma unroll
+  for (int d = WARPS / 2; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (C > 1) {
+    if (tid == 0) sh.top = top;
+    cluster.sync();
+    for (int c = 0; c < C; ++c) top = max_nan(top, of(c).top);
   }
-  if (lane == 0) sh.top_of[warp] = top, sh.at_of[warp] = at;
-  bad = __syncthreads_or(bad);
-  if (tid == 0) {
-    for (int i = 1; i < WARPS; ++i)
-      if (sh.top_of[i] > top || (sh.top_of[i] == top && sh.at_of[i] < at)) top = sh.top_of[i], at = sh.at_of[i];
-    sh.top = top, sh.at = at, sh.bad = bad;
-  }
-  meet();
-  top = -INFINITY, at = 0, bad = false;
-  for (int c = 0; c < C; ++c) {
-    const Shared& o = of(c);
-    if (o.top > top) top = o.top, at = o.at;
-    bad |= o.bad != 0;
-  }
-  if (bad || top == -INFINITY || !(temperature > 0.f)) {
+  if (!(top < INFINITY) || top == -INFINITY || !(temperature > 0.f)) {
+    const bool bad = !(top < INFINITY) || top == -INFINITY;
+    if (tid == 0) sh.at = INT32_MAX;
+    __syncthreads();
+    if (!bad)  // the first place of the largest
+      row.template each<2>(v0 + tid, v1, THREADS, [&](const uint4& q, int i) {
+        if (Row<T>::top(q) != top) return;
+        Row<T>::fours(q, i, [&](const float (&x)[4], int j) {
+          const int e = x[0] == top ? 0 : x[1] == top ? 1 : x[2] == top ? 2 : x[3] == top ? 3 : 4;
+          if (e < 4) atomicMin(&sh.at, j + e);
+        });
+      });
+    meet();
     if (rank == 0 && tid == 0) {
-      const bool none = bad || top == -INFINITY;
-      p.token[r] = none ? -1 : at;
-      if (p.logprob) p.logprob[r] = none ? __uint_as_float(0x7FC00000u) : 0.f;
+      int at = sh.at;
+      for (int c = 1; c < C; ++c) at = min(at, of(c).at);
+      p.token[r] = bad ? -1 : at;
+      if (p.logprob) p.logprob[r] = bad ? __uint_as_float(0x7FC00000u) : 0.f;
     }
     if (C > 1) cluster.sync();
     return;
   }
-  w.top = top;
-  w.t = static_cast<double>(temperature);
-  w.weight = Weight{static_cast<double>(top), 1.4426950408889634074 / w.t, sh.pow2, p.scale_bits};
-  w.bin_scale = static_cast<float>(w.weight.per_t) * BIN_PER;
+  set.t = static_cast<double>(temperature);
+  const double per_t = 32 * 1.4426950408889634074 / set.t;
+  if (tid == 0)
+    sh.weight = Weight{static_cast<double>(top), per_t,
+                       fminf(__double2float_rd(static_cast<double>(top) - 80 * 0.6931471805599453 * set.t), of_key(key_of(top) - 1)),
+                       sh.pow2, p.scale_bits};
   // w >= min_p: a bound on the logit, rounded up to the next one in f32
-  w.key_min = min_p > 0.f ? key_of(__double2float_ru(static_cast<double>(top) + w.t * log(static_cast<double>(fminf(min_p, 1.f))))) : 0;
-  w.key_min = min(w.key_min, key_of(top));
-  const bool k_on = k_in > 0 && k_in < p.vocab, p_on = top_p < 1.f;
+  set.key_min = 0;
+  if (min_p > 0.f)
+    set.key_min = min(key_of(top), key_of(__double2float_ru(static_cast<double>(top) + set.t * log(static_cast<double>(fminf(min_p, 1.f))))));
 
-  const long long have = min(static_cast<long long>(THREADS), vectors / C);  // threads with a vector, in a CTA
-  if ((k_on && k_in <= min(static_cast<long long>(LIST_K), have * 3 / 4)) || ((k_on || p_on) && p.vocab <= CAP)) {
-    // ---- Few entries, all of them on a list.  The k-th of the threads' largest logits is a bound that at least k logits of this
-    // CTA reach, and few more than k: its part of the row's k largest are among those.
-    uint32_t bound = 0;
-    if (k_on && p.vocab > CAP) {
-      const uint32_t key = key_of(mine);
-      constexpr int LOW = N == 8 ? 16 : 0;  // bits that tell no two bf16 apart
-      for (int bit = 31; bit >= LOW; --bit) {
-        const uint32_t tried = bound | (1u << bit);
-        if (__syncthreads_count(key >= tried) >= k_in) bound = tried;
-      }
+  auto append = [&](uint32_t key, int i) {
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < CAP) sh.list[at] = packed(key, i);
+  };
+  Mode mode = ALL;
+  int lo = BINS, hi = 0;  // bins of the window
+  const float bin_scale = fminf(static_cast<float>(per_t) * (BIN_PER / 32), 1e30f);
+  // How far a logit lies below the largest; rounded by the addition of 1.5 2^23, infinite distances in the last bin.
+  auto bin = [&](float x) { return min(BINS - 1, __float_as_int(fmaf(top - x, bin_scale, 12582912.f)) - 0x4B400000); };
+  uint32_t bound = 0;  // of the list's keys
+  const int have = min(THREADS, row.vectors / C);  // threads with a vector, in a CTA
+  if ((set.k > 0 || p_on) && p.vocab <= CAP) {
+    mode = LIST;
+  } else if (set.k > 0 && set.k <= min(LIST_K, have * 3 / 4)) {
+    // The k-th of the threads' largest logits is a bound that at least k logits of this CTA reach, and few more than k: its part of
+    // the row's k largest are among those.
+    mode = LIST;
+    const uint32_t key = key_of(mine);
+    constexpr int LOW = N == 8 ? 16 : 0;  // bits that tell no two bf16 apart
+#pragma unroll 1
+    for (int bit = 31; bit >= LOW; --bit) {
+      const uint32_t tried = bound | (1u << bit);
+      const int n = __syncthreads_count(key >= tried);
+      if (n >= set.k) bound = tried;
+      if (n == set.k) break;
     }
-    if (!p_on) bound = max(bound, w.key_min);
-    bound = max(bound, KEY_NONE + 1);
-    w.each(v0, v1, tid, THREADS, [&](const float (&x)[N], long long i) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t key = key_of(x[e]);
-        if (key >= bound) w.append(key, i + e);
-      }
-    });
-    meet();
-    uint32_t n = sh.count;
-    if (rank == 0) {
-      bool fits = n <= CAP;
-      for (int c = 1; c < C; ++c) {
-        const Shared& o = of(c);
-        const uint32_t m = o.count;
-        fits = fits && n + m <= CAP;
-        if (fits)
-          for (uint32_t i = tid; i < m; i += THREADS) sh.list[n + i] = o.list[i];
-        n += m;
-      }
-      if (!fits) n = CAP + 1;
-    }
-    meet();
-    if (rank != 0) return;
-    if (n <= CAP) w.draw_list(static_cast<int>(n), k_in, top_p);
-    else w.slow(k_in, top_p);
-    return;
-  }
-
-  int mode = ALL, lo = 0, hi = 0;
-  if (k_on || p_on) {
+  } else if (set.k > 0 || p_on) {
     // ---- How many logits lie how far below the largest: which bin the cut falls to, almost surely
     for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
     __syncthreads();
     uint32_t far = 0;
-    w.each(v0, v1, tid, THREADS, [&](const float (&x)[N], long long) {
+    row.template each<3>(v0 + tid, v1, THREADS, [&](const uint4& q, int i0) {
+      Row<T>::fours(q, i0, [&](const float (&x)[4], int) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (!(x[e] > -INFINITY)) continue;
-        const int b = w.bin(x[e]);
-        if (b < BINS - 1) atomicAdd(&sh.hist[b], 1u);
-        else ++far;
-      }
+        for (int e = 0; e < 4; ++e) {
+          const int b = bin(x[e]);
+          if (b < BINS - 1) atomicAdd(&sh.hist[b], 1u);
+          else far += x[e] > -INFINITY;
+        }
+      });
     });
-    far = static_cast<uint32_t>(warp_sum(far));
+    far = __reduce_add_sync(0xffffffffu, far);
     if (lane == 0 && far) atomicAdd(&sh.hist[BINS - 1], far);
     meet();
     if (rank == 0) {
       constexpr int PER = BINS / THREADS;
-      uint32_t n[PER];
-      u64 sum = 0;
-      float mass = 0.f, m[PER];
-#pragma unroll
+      // (the sums fit: at most 2^30 entries, and estimated masses in units of 2^-32)
+      u64 sum = 0, mass = 0;
+      auto estimate = [&](int b, uint32_t n) {
+        return static_cast<u64>(n * exp2f((b + 0.5f) * (-1.f / BIN_PER)) * 4294967296.f);
+      };
+#pragma unroll 1
       for (int j = 0; j < PER; ++j) {
         const int b = tid * PER + j;
-        n[j] = sh.hist[b];
-        for (int c = 1; c < C; ++c) n[j] += of(c).hist[b];
-        m[j] = n[j] * exp2f((b + 0.5f) * (-1.f / BIN_PER));
-        sum += n[j], mass += m[j];
+        uint32_t n = sh.hist[b];
+        for (int c = 1; c < C; ++c) n += of(c).hist[b];
+        sh.hist[b] = n;
+        sum += n, mass += estimate(b, n);
       }
-      u64 all;
-      u64 upto = block_scan(sum, sh.sums, all);
-      float fupto = mass;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const float o = __shfl_up_sync(0xffffffffu, fupto, d);
-        if (lane >= d) fupto += o;
-      }
-      if (lane == 31) sh.fsums[warp] = fupto;
-      if (tid == 0) sh.lo = sh.hi = BINS - 1, sh.before = 0;
+      Sums s = block_scan(set.k > 0 ? sum : mass, sh.sums);
+      if (tid == 0) sh.lo = BINS - 1, sh.before = 0;
       __syncthreads();
-      fupto -= mass;
-      float ftotal = 0.f;
-      for (int i = 0; i < WARPS; ++i) {
-        if (i < warp) fupto += sh.fsums[i];
-        ftotal += sh.fsums[i];
-      }
-      const float target = fmaxf(top_p * ftotal, 1e-30f);
-#pragma unroll
+      const u64 want = set.k > 0 ? static_cast<u64>(set.k) : max(u64{1}, static_cast<u64>(set.top_p * static_cast<float>(s.all)));
+#pragma unroll 1
       for (int j = 0; j < PER; ++j) {
         const int b = tid * PER + j;
-        if (k_on) {
-          if (upto < static_cast<u64>(k_in) && upto + n[j] >= static_cast<u64>(k_in)) sh.lo = sh.hi = b, sh.before = static_cast<uint32_t>(upto);
-        } else if (fupto < target && fupto + m[j] >= target) {
-          sh.lo = sh.hi = b;
-        }
-        upto += n[j], fupto += m[j];
-        sh.hist[b] = n[j];
+        const u64 y = set.k > 0 ? sh.hist[b] : estimate(b, sh.hist[b]);
+        if (s.before < want && s.before + y >= want) sh.lo = b, sh.before = static_cast<uint32_t>(s.before);
+        s.before += y;
       }
       __syncthreads();
-      if (tid < 32) {
+      if (warp == 0) {
         const int b = sh.lo;
-        const u64 through = sh.before + sh.hist[b];  // entries up to the bin of the k-th
-        int m_now = SLOW, from = b, to = b;
-        if (k_on) {
-          if (k_in >= static_cast<long long>(all)) m_now = p_on ? SLOW : ALL;  // (the rest is -inf)
-          else if (through <= CAP) m_now = LIST;
-          else if (!p_on && sh.hist[b] <= CAP) m_now = WINDOW_K;
-        } else {
-          // A window around the bin, as wide as its sums may be wrong: by the logits' places within the bins, 2^-8 of all at
+        const uint32_t n = sh.hist[b];
+        int from = b, to = b;
+        mode = SLOW;
+        if (set.k > 0) {
+          if (static_cast<u64>(set.k) >= s.all) mode = p_on ? SLOW : ALL;  // (the rest is -inf)
+          else if (sh.before + n <= CAP) mode = LIST;
+          else if (!p_on && n <= CAP) mode = WINDOW_K;
+        } else if (n <= CAP) {
+          // A window around the bin, as wide as the estimates may be wrong: by the logits' places within the bins, 2^-8 of all at
           // most.  (Whether it holds the cut is checked by exact sums.)
-          const float each_bin = exp2f((b + 0.5f) * (-1.f / BIN_PER));
           const int d = lane + 1;
-          uint32_t both = (b - d >= 0 ? sh.hist[b - d] : 0) + (b + d < BINS ? sh.hist[b + d] : 0);
-          const float half = min(b - d >= 0 ? sh.hist[b - d] : 0x7FFFFFFFu, b + d < BINS ? sh.hist[b + d] : 0x7FFFFFFFu) * each_bin;
-          float reach = half;
-#pragma unroll
-          for (int s = 1; s < 32; s <<= 1) {
-            const uint32_t o = __shfl_up_sync(0xffffffffu, both, s);
-            const float f = __shfl_up_sync(0xffffffffu, reach, s);
-            if (lane >= s) both += o, reach += f;
+          const uint32_t below = b - d >= 0 ? sh.hist[b - d] : 0, behind = b + d < BINS ? sh.hist[b + d] : 0;
+          uint32_t both = below + behind;
+          u64 reach = estimate(b, min(b - d >= 0 ? below : 1u << 30, b + d < BINS ? behind : 1u << 30));
+#pragma unroll 1
+          for (int i = 1; i < 32; i <<= 1) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, both, i);
+            const u64 f = __shfl_up_sync(0xffffffffu, reach, i);
+            if (lane >= i) both += o, reach += f;
           }
-          const unsigned fits = __ballot_sync(0xffffffffu, sh.hist[b] + both <= CAP);
-          const unsigned wide = __ballot_sync(0xffffffffu, reach >= ftotal * (1.f / 256));
-          int width = wide ? __ffs(wide) : 32;         // bins on either side that suffice
-          width = min(width, __popc(fits));            // and that the list holds (fits is a run of ones from bit 0)
-          if (sh.hist[b] <= CAP) m_now = WINDOW_P, from = max(0, b - width), to = min(BINS - 1, b + width);
+          const unsigned fits = __ballot_sync(0xffffffffu, n + both <= CAP);       // a run of ones from bit 0
+          const unsigned wide = __ballot_sync(0xffffffffu, reach >= (s.all >> 8));
+          const int width = min(wide ? __ffs(wide) : 32, __popc(fits));
+          mode = WINDOW_P, from = max(0, b - width), to = min(BINS - 1, b + width);
         }
         __syncwarp();
-        if (lane == 0) sh.mode = m_now, sh.lo = from, sh.hi = to;
+        if (lane == 0) {
+          sh.mode = mode, sh.hi = to;
+          sh.lo = mode == LIST ? 0 : mode == ALL ? BINS : from;
+        }
       }
     }
     meet();
     const Shared& o = of(0);
-    mode = o.mode, lo = o.lo, hi = o.hi;
+    mode = static_cast<Mode>(o.mode), lo = o.lo, hi = o.hi;
+    if (mode == LIST) {  // the least logit of the bins up to hi: those behind it have larger numbers
+      uint32_t below = KEY_NONE, from = key_of(top);
+      while (from - below > 1) {
+        const uint32_t mid = below + (from - below) / 2;
+        if (bin(of_key(mid)) <= hi) from = mid;
+        else below = mid;
+      }
+      bound = from;
+    }
   }
+  __syncthreads();
 
+  u64 cut = 0;
   if (mode == LIST) {
-    w.each(v0, v1, tid, THREADS, [&](const float (&x)[N], long long i) {
+    if (!p_on) bound = max(bound, set.key_min);
+    const float low = of_key(max(bound, KEY_NONE + 1));
+    row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int i) {
+      if (!(Row<T>::top(q) >= low)) return;
+      Row<T>::fours(q, i, [&](const float (&x)[4], int j) {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (x[e] > -INFINITY && w.bin(x[e]) <= hi) w.append(key_of(x[e]), i + e);
+        for (int e = 0; e < 4; ++e)
+          if (x[e] >= low) append(key_of(x[e]), j + e);
+      });
     });
-  } else if (mode == ALL) {
-    w.sum_tiles(t0, t1, 0);
   } else if (mode != SLOW) {
     // ---- sums of the tiles above the window, of all above it and of all; the window's entries on the list
+    const Weight weight = sh.weight;
+    const float min_kept = of_key(max(set.key_min, KEY_NONE + 1));
     u64 above = 0, all = 0;
-    for (long long tile = t0 + warp; tile < t1; tile += WARPS) {
+#pragma unroll 1
+    for (int tile = t0 + warp; tile < t1; tile += WARPS) {
       u64 sum = 0;
-      w.each(tile * w.per_tile, min(vectors, (tile + 1) * w.per_tile), lane, 32, [&](const float (&x)[N], long long i) {
+      row.template each<2>(tile * per_tile + lane, min(row.vectors, (tile + 1) * per_tile), 32, [&](const uint4& q, int i0) {
+        const float most = Row<T>::top(q);
+        if (mode == ALL ? most < min_kept : mode == WINDOW_K && bin(most) > hi) return;
+        Row<T>::fours(q, i0, [&](const float (&x)[4], int i) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int b = w.bin(x[e]);
-          if (b > hi && mode == WINDOW_K) continue;
-          const uint32_t key = key_of(x[e]);
-          if (key <= KEY_NONE) continue;
-          const u64 y = w.weight(x[e]);
-          all += y;
-          if (b < lo) {
-            above += y;
-            if (key >= w.key_min) sum += y;
-          } else if (b <= hi) {
-            w.append(key, i + e);
+          for (int e = 0; e < 4; ++e) {
+            const u64 y = weight(x[e]);
+            const int b = bin(x[e]);
+            all += y;
+            if (b < lo) {
+              above += y;
+              if (x[e] >= min_kept) sum += y;
+            } else if (b <= hi && x[e] > -INFINITY) {
+              append(key_of(x[e]), i + e);
+            }
           }
-        }
+        });
       });
       sum = warp_sum(sum);
       if (lane == 0) sh.tile[tile] = sum;
     }
-    u64 total;
-    block_scan(above, sh.sums, total);
-    if (tid == 0) sh.above = total;
-    block_scan(all, sh.sums, total);
-    if (tid == 0) sh.all = total;
-  }
-  meet();
-  uint32_t n = sh.count;
-  u64 above = sh.above, all = sh.all;
-  if (rank == 0 && mode != SLOW) {
-    for (int c = 1; c < C; ++c) {
-      const Shared& o = of(c);
-      const uint32_t m = o.count;
-      if (n + m <= CAP)  // (by the bins' counts it is)
-        for (uint32_t i = tid; i < m; i += THREADS) sh.list[n + i] = o.list[i];
-      n += m;
-      above += o.above, all += o.all;
-      if (mode != LIST)
-        for (long long i = c * share + tid; i < min(w.tiles, (c + 1) * share); i += THREADS) sh.tile[i] = o.tile[i];
-    }
-  }
-  meet();
-  if (rank != 0) return;
-  if (mode == SLOW || n > CAP) {
-    w.slow(k_in, top_p);
-  } else if (mode == LIST) {
-    w.draw_list(static_cast<int>(n), k_in, top_p);
-  } else if (mode == ALL) {
-    w.draw_tiles(0);
-  } else {
-    // ---- the cut within the window, exactly
-    const u64* order = sort_down(sh, sh.list, sh.other, static_cast<int>(n));
-    int keep;
-    const int per = (static_cast<int>(n) + THREADS - 1) / THREADS;
-    u64 y[4], sum = 0, inside;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      y[j] = j < per && i < static_cast<int>(n) ? w.weight(of_key(static_cast<uint32_t>(order[i] >> 32))) : 0;
-      sum += y[j];
-    }
-    u64 ahead = above + block_scan(sum, sh.sums, inside);
     if (mode == WINDOW_P) {
-      const u64 want = least_of(top_p, all);
-      if (!(above < want && want <= above + inside)) {
-        w.slow(k_in, top_p);
-        return;
+      above = block_scan(above, sh.sums).all;
+      all = block_scan(all, sh.sums).all;
+      if (tid == 0) sh.above = above, sh.all = all;
+    }
+  }
+  meet();
+  int n = static_cast<int>(min(sh.count, static_cast<uint32_t>(CAP + 1)));
+  u64 above = sh.above, all = sh.all;
+  if (C > 1) {
+    if (rank == 0)
+      for (int c = 1; c < C; ++c) {
+        const Shared& o = of(c);
+        const int m = static_cast<int>(min(o.count, static_cast<uint32_t>(CAP + 1)));
+        if (n + m <= CAP)
+          for (int i = tid; i < m; i += THREADS) sh.list[n + i] = o.list[i];
+        n = min(n + m, CAP + 1);
+        above += o.above, all += o.all;
+        if (mode == ALL || mode == WINDOW_P || mode == WINDOW_K)
+          for (int i = c * share + tid; i < min(tiles, (c + 1) * share); i += THREADS) sh.tile[i] = o.tile[i];
       }
-      u64 less = 0, count;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = tid * per + j;
-        ahead += y[j];
-        less += j < per && i < static_cast<int>(n) && ahead < want;
+    cluster.sync();
+    if (rank != 0) return;
+  }
+  if (mode == LIST && n <= CAP) {
+    if (n <= SMALL) draw_small(p, sh, set, r, n);
+    else draw_sorted(p, sh, set, r, n);
+    return;
+  }
+  if (mode == WINDOW_P || mode == WINDOW_K) {
+    // ---- the cut within the window, exactly
+    const u64* order = sort_down(sh.rank_of, sh.list, sh.other, n);
+    const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
+    u64 sum = 0;
+#pragma unroll 1
+    for (int i = first; i < last; ++i) sum += sh.weight(of_key(key_in(order[i])));
+    Sums s = block_scan(sum, sh.sums);
+    s.before += above;
+    int keep = 0;
+    if (mode == WINDOW_P) {
+      const u64 want = least_of(set.top_p, all);
+      if (above < want && want <= above + s.all) {
+        u64 less = 0;
+#pragma unroll 1
+        for (int i = first; i < last; ++i) {
+          s.before += sh.weight(of_key(key_in(order[i])));
+          less += s.before < want;
+        }
+        keep = static_cast<int>(block_scan(less, sh.sums).all) + 1;
+      } else {
+        mode = SLOW;
       }
-      block_scan(less, sh.sums, count);
-      keep = static_cast<int>(count) + 1;
     } else {
-      keep = static_cast<int>(k_in - sh.before);
+      keep = set.k - static_cast<int>(sh.before);
     }
-    const u64 cut = order[keep - 1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * per + j;
-      if (j < per && i < keep && static_cast<uint32_t>(order[i] >> 32) >= w.key_min) {
-        const long long at_i = 0xFFFFFFFFu - static_cast<uint32_t>(order[i]);
-        atomicAdd(&sh.tile[(at_i + w.row.lead) / N / w.per_tile], y[j]);
-      }
+    if (mode != SLOW) {
+      cut = order[keep - 1];
+#pragma unroll 1
+      for (int i = tid; i < keep; i += THREADS)
+        if (key_in(order[i]) >= set.key_min)
+          atomicAdd(&sh.tile[(index_in(order[i]) + row.lead) / N / per_tile], sh.weight(of_key(key_in(order[i]))));
+      __syncthreads();
     }
-    __syncthreads();
-    w.draw_tiles(cut);
+  }
+  if (mode == SLOW || mode == LIST) cut = slow_cut(row, sh, set, per_tile, tiles);
+
+  // ---- the draw: which tile, and which entry of it
+  const u64 a = 2 * tid < tiles ? sh.tile[2 * tid] : 0, b = 2 * tid + 1 < tiles ? sh.tile[2 * tid + 1] : 0;
+  const Sums s = block_scan(a + b, sh.sums);
+  const u64 want = drawn(set.u, s.all);
+  if (s.before <= want && want < s.before + a + b) {
+    const bool second = want >= s.before + a;
+    sh.index = 2 * tid + second;
+    sh.word = second ? s.before + a : s.before;
+  }
+  __syncthreads();
+  u64 ahead = sh.word;
+  const uint32_t least = max(set.key_min, KEY_NONE + 1);
+  const int i0 = max(0, row.first(sh.index * per_tile)), i1 = min(row.vocab, row.first(min(row.vectors, (sh.index + 1) * per_tile)));
+#pragma unroll 1
+  for (int base = i0; base < i1 && ahead <= want; base += THREADS) {
+    const int i = base + tid;
+    float x = -INFINITY;
+    u64 w = 0;
+    if (i < i1) {
+      x = row.at(i);
+      const uint32_t key = key_of(x);
+      if (key >= least && packed(key, i) >= cut) w = sh.weight(x);
+    }
+    const Sums in = block_scan(w, sh.sums);
+    const u64 upto = ahead + in.before;
+    if (upto <= want && want < upto + w) write_out(p, sh, r, set.t, i, x, s.all);
+    ahead += in.all;
   }
 }
 }  // namespace sample
@@ -844,7 +879,7 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
       return fail(CDL_ERR_INVALID, "%s: an output overlaps an input", op);
   if (logprob && !views_apart(*token, *logprob)) return fail(CDL_ERR_INVALID, "%s: token and logprob overlap", op);
   sample::Params p{};
-  p.z = logits->ptr, p.ld = logits->stride[0], p.vocab = V;
+  p.z = logits->ptr, p.ld = logits->stride[0], p.vocab = static_cast<int>(V);
   p.u = static_cast<const float*>(uniform->ptr);
   p.temperature = temperature ? static_cast<const float*>(temperature->ptr) : nullptr;
   p.top_k = top_k ? static_cast<const int*>(top_k->ptr) : nullptr;
@@ -855,10 +890,10 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   p.logprob = logprob ? static_cast<float*>(logprob->ptr) : nullptr;
   int bits = 0;
   while ((1LL << bits) < V) ++bits;
-  p.scale_bits = 62 - bits;
+  p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
-  // CTAs of a row: as many as leave every SM one, with 8192 logits each or more
-  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({8, sm_count() / R, V / 8192})));
+  // CTAs of a row: as many as leave every SM one, with 16384 logits each or more
+  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({8, sm_count() / R, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));
   CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
