@@ -177,36 +177,43 @@ __device__ const double POW2[32] = {
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
 // w = exp((z - top) / T) in units of 2^-S: 2^((k + r) / 32) with (z - top) 32 log2(e) / T = k + r, |r| <= 1/2, from a table of
-// 2^(j/32) and the Taylor series up to r^6, whose rest is 4e-18 (the table-driven method of P. T. P. Tang, 1989).  S <= 50: the
-// addition of 2^52 rounds to whole units.
+// 2^(S + j/32) and the Taylor series up to r^5, whose rest is 2e-15 (the table-driven method of P. T. P. Tang, 1989).  S <= 50: the
+// addition of 2^52 rounds to whole units.  The last two coefficients have 20 bits, which is what they matter with (1e-15), so that
+// they fit into an instruction; the others are members so that they stay in registers.
 struct Weight {
   double top, per_t;  // 32 log2(e) / T
-  float least;        // 80 T ln 2 below the top, where w is less than half a unit (what is computed there has no meaning)
-  const double* pow2;
-  int bits;
-  __device__ __forceinline__ u64 operator()(float z) const {
-    constexpr double L = 0.6931471805599453094 / 32, MAGIC = 6755399441055744.0;  // 1.5 2^52
+  double c1, c2, c3;  // (ln 2 / 32)^i / i!
+  float least;        // 80 T ln 2 below the top, where w is less than half a unit
+  uint32_t pow2;      // the table in shared memory
+  // (without meaning for z <= least)
+  __device__ __forceinline__ u64 above_least(float z) const {
+    constexpr double C4 = 0x1.3b2ab00000000p-27, C5 = 0x1.5d88000000000p-35, MAGIC = 6755399441055744.0;  // 1.5 2^52
     const double d = static_cast<double>(z) - top;
     const double k = fma(d, per_t, MAGIC);
     const int n = __double2loint(k);
     const double r = fma(d, per_t, MAGIC - k);
-    double y = fma(r, L * L * L * L * L * L / 720, L * L * L * L * L / 120);
-    y = fma(r, y, L * L * L * L / 24);
-    y = fma(r, y, L * L * L / 6);
-    y = fma(r, y, L * L / 2);
-    y = fma(r, y, L) * r;
-    const double tab = pow2[n & 31];
+    double y = fma(r, C5, C4);
+    y = fma(r, y, c3);
+    y = fma(r, y, c2);
+    y = fma(r, y, c1) * r;
+    double tab;
+    asm("ld.shared.f64 %0, [%1];" : "=d"(tab) : "r"(pow2 + (n & 31) * 8));
     y = fma(tab, y, tab);
-    y = __hiloint2double(__double2hiint(y) + (((n >> 5) + bits) << 20), __double2loint(y)) + 4503599627370496.0;
-    return z > least ? static_cast<u64>(__double_as_longlong(y)) & 0xFFFFFFFFFFFFFull : 0;
+    y = __hiloint2double(__double2hiint(y) + ((n << 15) & static_cast<int>(0xFFF00000u)), __double2loint(y)) + 4503599627370496.0;
+    return static_cast<u64>(__double_as_longlong(y)) & 0xFFFFFFFFFFFFFull;
+  }
+  __device__ __forceinline__ u64 operator()(float z) const {
+    const u64 w = above_least(z);
+    return z > least ? w : 0;
   }
 };
 
 struct Shared {
-  u64 list[CAP];
+  u64 list[CAP], weight_of[CAP];
   union {
     u64 other[CAP];
     uint32_t hist[BINS];
+    uint32_t fine[3][THREADS];
     u64 wide_hist[256];
   };
   u64 tile[TILES];  // a CTA's tiles at their number in the row
@@ -355,42 +362,47 @@ __device__ __noinline__ void draw_sorted(const Params& p, Shared& sh, const Sett
   }
 }
 
-// The draw from up to SMALL entries: each is held against all others, by 32 threads at most, once for what is ahead of it in
-// falling order and once for what is ahead of it by index.
-__device__ __noinline__ void draw_small(const Params& p, Shared& sh, const Settings& set, long long r, int n) {
+// The draw from up to SMALL entries: each is held against all others, by 32 threads at most, for its place in falling order and
+// then, of those that are kept, for what is ahead of it by index.
+__device__ __forceinline__ void draw_small(const Params& p, Shared& sh, const Settings& set, long long r, int n) {
   const int tid = threadIdx.x;
   int parts = 32;
   while (parts * n > THREADS) parts >>= 1;
-  const int i = tid / parts, part = tid & (parts - 1);
-  for (int j = tid; j < n; j += THREADS) sh.other[j] = sh.weight(of_key(key_in(sh.list[j])));
+  int i = tid / parts;
+  const int part = tid & (parts - 1);
+  {
+    const u64 me = i < n ? sh.list[i] : 0;
+    uint32_t rank = 0;
+    if (i < n)
+#pragma unroll 4
+      for (int j = part; j < n; j += parts) rank += sh.list[j] > me;
+    for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+    if (i < n && part == 0) sh.other[rank] = me;
+  }
   __syncthreads();
-  const u64 me = i < n ? sh.list[i] : 0, w = i < n ? sh.other[i] : 0;
+  if (set.k > 0 && set.k < n) n = set.k;
+  const u64 entry = tid < n ? sh.other[tid] : 0;
+  u64 w = tid < n ? sh.weight(of_key(key_in(entry))) : 0;
+  const Sums s = block_scan(w, sh.sums);
+  const bool kept = tid < n && (tid == 0 || (key_in(entry) >= set.key_min && (!(set.top_p < 1.f) || s.before < least_of(set.top_p, s.all))));
+  if (kept) sh.list[tid] = w;
+  n = __syncthreads_count(kept);
+  if (tid == n - 1) sh.word = s.before + w;
+  __syncthreads();
+  const u64 mass = sh.word, want = drawn(set.u, mass);
+  parts = 32;
+  while (parts * n > THREADS) parts >>= 1;
+  i = tid / parts;
   u64 ahead = 0;
-  uint32_t rank = 0;
+  const int at = tid & (parts - 1);
+  const u64 me = i < n ? sh.other[i] : 0;
   if (i < n)
 #pragma unroll 2
-    for (int j = part; j < n; j += parts)
-      if (sh.list[j] > me) ahead += sh.other[j], ++rank;
-  for (int d = 1; d < parts; d <<= 1) {
-    ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
-    rank += __shfl_xor_sync(0xffffffffu, rank, d);
-  }
-  bool kept = i < n && (set.k == 0 || rank < static_cast<uint32_t>(set.k));
-  if (set.top_p < 1.f) {
-    const u64 mass = block_scan(kept && part == 0 ? w : 0, sh.sums).all;
-    kept = kept && (rank == 0 || ahead < least_of(set.top_p, mass));
-  }
-  kept = kept && (key_in(me) >= set.key_min || rank == 0);
-  if (part == 0 && i < n && !kept) sh.other[i] = 0;
-  const u64 mass = block_scan(kept && part == 0 ? w : 0, sh.sums).all;
-  const u64 want = drawn(set.u, mass);
-  ahead = 0;
-  if (i < n)
-#pragma unroll 2
-    for (int j = part; j < n; j += parts)
-      if (static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(me)) ahead += sh.other[j];
+    for (int j = at; j < n; j += parts)
+      if (static_cast<uint32_t>(sh.other[j]) > static_cast<uint32_t>(me)) ahead += sh.list[j];
   for (int d = 1; d < parts; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
-  if (kept && part == 0 && ahead <= want && want < ahead + w) write_out(p, sh, r, set.t, index_in(me), of_key(key_in(me)), mass);
+  if (i < n && at == 0 && ahead <= want && want < ahead + sh.list[i])
+    write_out(p, sh, r, set.t, index_in(me), of_key(key_in(me)), mass);
 }
 
 // The entry at which the sum over the entries from `cut` on, in falling order, reaches `want`: of their weights, or their number.
@@ -513,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     else __syncthreads();
   };
   auto of = [&](int other) -> Shared& { return C > 1 ? *cluster.map_shared_rank(&sh, other) : sh; };
-  if (tid < 32) sh.pow2[tid] = POW2[tid];
+  if (tid < 32) sh.pow2[tid] = __hiloint2double(__double2hiint(POW2[tid]) + (p.scale_bits << 20), __double2loint(POW2[tid]));
   if (tid == 0) sh.count = 0;
   const long long r = blockIdx.x / C;
   Row<T> row;
@@ -534,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
 
   // ---- the largest logit; NaN and +inf
   float mine = -INFINITY;
-  row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int) { mine = max_nan(mine, Row<T>::top(q)); });
+  row.template each<6>(v0 + tid, v1, THREADS, [&](const uint4& q, int) { mine = max_nan(mine, Row<T>::top(q)); });
   const float temperature = p.temperature ? p.temperature[r] : p.all_temperature;
   const float min_p = p.min_p ? p.min_p[r] : p.all_min_p;
   Settings set;
@@ -579,11 +591,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     return;
   }
   set.t = static_cast<double>(temperature);
+  constexpr double L = 0.6931471805599453094 / 32;
   const double per_t = 32 * 1.4426950408889634074 / set.t;
   if (tid == 0)
-    sh.weight = Weight{static_cast<double>(top), per_t,
+    sh.weight = Weight{static_cast<double>(top), per_t, L, L * L / 2, L * L * L / 6,
                        fminf(__double2float_rd(static_cast<double>(top) - 80 * 0.6931471805599453 * set.t), of_key(key_of(top) - 1)),
-                       sh.pow2, p.scale_bits};
+                       smem_u32(sh.pow2)};
   // w >= min_p: a bound on the logit, rounded up to the next one in f32
   set.key_min = 0;
   if (min_p > 0.f)
@@ -594,11 +607,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     if (at < CAP) sh.list[at] = packed(key, i);
   };
   Mode mode = ALL;
-  int lo = BINS, hi = 0;  // bins of the window
   const float bin_scale = fminf(static_cast<float>(per_t) * (BIN_PER / 32), 1e30f);
   // How far a logit lies below the largest; rounded by the addition of 1.5 2^23, infinite distances in the last bin.
   auto bin = [&](float x) { return min(BINS - 1, __float_as_int(fmaf(top - x, bin_scale, 12582912.f)) - 0x4B400000); };
-  uint32_t bound = 0;  // of the list's keys
+  uint32_t bound = 0;                      // of the list's keys
+  float over = 0.f, low = 0.f;             // logits of the window: [low, over)
   const int have = min(THREADS, row.vectors / C);  // threads with a vector, in a CTA
   if ((set.k > 0 || p_on) && p.vocab <= CAP) {
     mode = LIST;
@@ -640,13 +653,18 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       auto estimate = [&](int b, uint32_t n) {
         return static_cast<u64>(n * exp2f((b + 0.5f) * (-1.f / BIN_PER)) * 4294967296.f);
       };
-#pragma unroll 1
+      static_assert(PER == 4, "");
+      uint4 bins = reinterpret_cast<const uint4*>(sh.hist)[tid];
+#pragma unroll 4
+      for (int c = 1; c < C; ++c) {
+        const uint4 o = reinterpret_cast<const uint4*>(of(c).hist)[tid];
+        bins.x += o.x, bins.y += o.y, bins.z += o.z, bins.w += o.w;
+      }
+      if (C > 1) reinterpret_cast<uint4*>(sh.hist)[tid] = bins;
+#pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int b = tid * PER + j;
-        uint32_t n = sh.hist[b];
-        for (int c = 1; c < C; ++c) n += of(c).hist[b];
-        sh.hist[b] = n;
-        sum += n, mass += estimate(b, n);
+        const uint32_t n = j == 0 ? bins.x : j == 1 ? bins.y : j == 2 ? bins.z : bins.w;
+        sum += n, mass += estimate(tid * PER + j, n);
       }
       Sums s = block_scan(set.k > 0 ? sum : mass, sh.sums);
       if (tid == 0) sh.lo = BINS - 1, sh.before = 0;
@@ -670,8 +688,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
           else if (sh.before + n <= CAP) mode = LIST;
           else if (!p_on && n <= CAP) mode = WINDOW_K;
         } else if (n <= CAP) {
-          // A window around the bin, as wide as the estimates may be wrong: by the logits' places within the bins, 2^-8 of all at
-          // most.  (Whether it holds the cut is checked by exact sums.)
+          // A window around the bin, as wide as the estimates may be wrong: a logit's place in its bin is worth 2^-8 of its weight at
+          // most, which averages out over the bins; where all of a bin are equal (bf16) about 2^-12 of the whole sum is left.  2^-10
+          // are taken.  (Whether the window holds the cut is checked by exact sums.)
           const int d = lane + 1;
           const uint32_t below = b - d >= 0 ? sh.hist[b - d] : 0, behind = b + d < BINS ? sh.hist[b + d] : 0;
           uint32_t both = below + behind;
@@ -683,28 +702,33 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             if (lane >= i) both += o, reach += f;
           }
           const unsigned fits = __ballot_sync(0xffffffffu, n + both <= CAP);       // a run of ones from bit 0
-          const unsigned wide = __ballot_sync(0xffffffffu, reach >= (s.all >> 8));
+          const unsigned wide = __ballot_sync(0xffffffffu, reach >= (s.all >> 10));
           const int width = min(wide ? __ffs(wide) : 32, __popc(fits));
           mode = WINDOW_P, from = max(0, b - width), to = min(BINS - 1, b + width);
         }
         __syncwarp();
         if (lane == 0) {
           sh.mode = mode, sh.hi = to;
-          sh.lo = mode == LIST ? 0 : mode == ALL ? BINS : from;
+          sh.lo = from;
         }
       }
     }
     meet();
     const Shared& o = of(0);
-    mode = static_cast<Mode>(o.mode), lo = o.lo, hi = o.hi;
-    if (mode == LIST) {  // the least logit of the bins up to hi: those behind it have larger numbers
-      uint32_t below = KEY_NONE, from = key_of(top);
+    mode = static_cast<Mode>(o.mode);
+    if (mode == WINDOW_P || mode == WINDOW_K || mode == LIST) {
+      // the least logits of the bins up to lo - 1 and up to hi: the logits below have larger bins
+      const int last = lane == 0 ? o.lo - 1 : o.hi;
+      uint32_t below = KEY_NONE, from = last < 0 ? KEY_NONE + 1 : key_of(top);
+#pragma unroll 1
       while (from - below > 1) {
         const uint32_t mid = below + (from - below) / 2;
-        if (bin(of_key(mid)) <= hi) from = mid;
+        if (bin(of_key(mid)) <= last) from = mid;
         else below = mid;
       }
-      bound = from;
+      over = last < 0 ? INFINITY : of_key(from);
+      bound = __shfl_sync(0xffffffffu, from, 1);
+      over = __shfl_sync(0xffffffffu, over, 0), low = of_key(bound);
     }
   }
   __syncthreads();
@@ -712,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   u64 cut = 0;
   if (mode == LIST) {
     if (!p_on) bound = max(bound, set.key_min);
-    const float low = of_key(max(bound, KEY_NONE + 1));
+    low = of_key(max(bound, KEY_NONE + 1));
     row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int i) {
       if (!(Row<T>::top(q) >= low)) return;
       Row<T>::fours(q, i, [&](const float (&x)[4], int j) {
@@ -722,38 +746,58 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       });
     });
   } else if (mode != SLOW) {
-    // ---- sums of the tiles above the window, of all above it and of all; the window's entries on the list
-    const Weight weight = sh.weight;
+    // ---- sums of the tiles above the window and of the whole row; the window's entries on the list.  Where min_p's bound lies
+    // above the window, what is above it is summed instead, and nothing of the window is kept.
     const float min_kept = of_key(max(set.key_min, KEY_NONE + 1));
-    u64 above = 0, all = 0;
+    if (mode == ALL || min_kept >= over) over = min_kept, low = INFINITY;
+    const Weight weight = sh.weight;
+    const float from = fmaxf(over, of_key(key_of(weight.least) + 1));
+    u64 rest = 0, above = 0;
+    // f(4 values, index of the first) of each vector that has one from `least` on, tile by tile
+    auto tiles_of = [&](float least, auto f) {
 #pragma unroll 1
-    for (int tile = t0 + warp; tile < t1; tile += WARPS) {
-      u64 sum = 0;
-      row.template each<2>(tile * per_tile + lane, min(row.vectors, (tile + 1) * per_tile), 32, [&](const uint4& q, int i0) {
-        const float most = Row<T>::top(q);
-        if (mode == ALL ? most < min_kept : mode == WINDOW_K && bin(most) > hi) return;
-        Row<T>::fours(q, i0, [&](const float (&x)[4], int i) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u64 y = weight(x[e]);
-            const int b = bin(x[e]);
-            all += y;
-            if (b < lo) {
-              above += y;
-              if (x[e] >= min_kept) sum += y;
-            } else if (b <= hi && x[e] > -INFINITY) {
-              append(key_of(x[e]), i + e);
-            }
-          }
+      for (int tile = t0 + warp; tile < t1; tile += WARPS) {
+        u64 sum = 0;
+        row.template each<2>(tile * per_tile + lane, min(row.vectors, (tile + 1) * per_tile), 32, [&](const uint4& q, int i0) {
+          if (Row<T>::top(q) < least) return;
+          Row<T>::fours(q, i0, [&](const float (&x)[4], int i) { f(x, i, sum); });
         });
-      });
-      sum = warp_sum(sum);
-      if (lane == 0) sh.tile[tile] = sum;
-    }
+        sum = warp_sum(sum);
+        if (lane == 0) sh.tile[tile] = sum;
+        above += sum;  // (the same in all lanes)
+      }
+    };
+    auto window = [&](const float (&x)[4], int i) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) any |= x[e] >= low && !(x[e] >= over);
+      if (any)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x[e] >= low && !(x[e] >= over)) append(key_of(x[e]), i + e);
+    };
     if (mode == WINDOW_P) {
-      above = block_scan(above, sh.sums).all;
-      all = block_scan(all, sh.sums).all;
-      if (tid == 0) sh.above = above, sh.all = all;
+      tiles_of(weight.least, [&](const float (&x)[4], int i, u64& sum) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 y = weight.above_least(x[e]);
+          sum += x[e] >= from ? y : 0;
+          rest += x[e] > weight.least && !(x[e] >= from) ? y : 0;
+        }
+        window(x, i);
+      });
+      rest = block_scan(rest, sh.sums).all;
+      above = block_scan(lane == 0 ? above : 0, sh.sums).all;
+      if (tid == 0) sh.above = above, sh.all = above + rest;
+    } else {
+      tiles_of(fminf(over, low), [&](const float (&x)[4], int i, u64& sum) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 y = weight.above_least(x[e]);
+          sum += x[e] >= from ? y : 0;
+        }
+        window(x, i);
+      });
     }
   }
   meet();
@@ -780,38 +824,77 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     return;
   }
   if (mode == WINDOW_P || mode == WINDOW_K) {
-    // ---- the cut within the window, exactly
-    const u64* order = sort_down(sh.rank_of, sh.list, sh.other, n);
-    const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
-    u64 sum = 0;
-#pragma unroll 1
-    for (int i = first; i < last; ++i) sum += sh.weight(of_key(key_in(order[i])));
-    Sums s = block_scan(sum, sh.sums);
-    s.before += above;
-    int keep = 0;
+    // ---- the cut within the window, exactly.  Its entries' weights in 512 parts of the window (as three numbers of 17 bits, whose
+    // sums stay below 32 bits), the part in which the sum reaches what is wanted, and that part's entries each against all others.
+    constexpr int PER = CAP / THREADS;
+    const float edge = fminf(over, top), fine_scale = fminf((THREADS - 1) / (edge - low), 1e30f);
+    auto part_of = [&](u64 x) { return min(THREADS - 1, static_cast<int>((edge - of_key(key_in(x))) * fine_scale)); };
+    u64 want = static_cast<u64>(set.k) - sh.before;
     if (mode == WINDOW_P) {
-      const u64 want = least_of(set.top_p, all);
-      if (above < want && want <= above + s.all) {
-        u64 less = 0;
-#pragma unroll 1
-        for (int i = first; i < last; ++i) {
-          s.before += sh.weight(of_key(key_in(order[i])));
-          less += s.before < want;
-        }
-        keep = static_cast<int>(block_scan(less, sh.sums).all) + 1;
-      } else {
-        mode = SLOW;
-      }
-    } else {
-      keep = set.k - static_cast<int>(sh.before);
+      want = least_of(set.top_p, all);
+      if (want <= above) mode = SLOW;
+      want -= above;
     }
-    if (mode != SLOW) {
-      cut = order[keep - 1];
-#pragma unroll 1
-      for (int i = tid; i < keep; i += THREADS)
-        if (key_in(order[i]) >= set.key_min)
-          atomicAdd(&sh.tile[(index_in(order[i]) + row.lead) / N / per_tile], sh.weight(of_key(key_in(order[i]))));
+    if (low == INFINITY) {  // min_p's bound is above the window
+      if (mode != SLOW) mode = ALL;
+    } else {
+      for (int i = tid; i < 3 * THREADS; i += THREADS) (&sh.fine[0][0])[i] = 0;
       __syncthreads();
+#pragma unroll 1
+      for (int j = 0; j < PER; ++j) {
+        const int i = tid + j * THREADS;
+        if (i >= n) break;
+        const u64 x = sh.list[i];
+        const int part = part_of(x);
+        const u64 w = mode == WINDOW_K ? 1 : sh.weight(of_key(key_in(x)));
+        sh.weight_of[i] = w;
+        atomicAdd(&sh.fine[0][part], static_cast<uint32_t>(w) & 0x1FFFFu);
+        if (w >> 17) atomicAdd(&sh.fine[1][part], static_cast<uint32_t>(w >> 17) & 0x1FFFFu);
+        if (w >> 34) atomicAdd(&sh.fine[2][part], static_cast<uint32_t>(w >> 34));
+      }
+      __syncthreads();
+      const u64 mine_in = sh.fine[0][tid] + (static_cast<u64>(sh.fine[1][tid]) << 17) + (static_cast<u64>(sh.fine[2][tid]) << 34);
+      if (tid == 0) sh.index = 0;
+      const Sums s = block_scan(mine_in, sh.sums);
+      if (want > s.all) mode = SLOW;
+      if (mode != SLOW) {
+        if (s.before < want && want <= s.before + mine_in) sh.lo = tid, sh.word = s.before;
+        __syncthreads();
+        const int part = sh.lo;
+        want -= sh.word;
+#pragma unroll 1
+        for (int j = 0; j < PER; ++j) {
+          const int i = tid + j * THREADS;
+          if (i >= n) break;
+          const u64 x = sh.list[i];
+          if (part_of(x) == part) sh.other[atomicAdd(&sh.index, 1)] = static_cast<u64>(i);
+        }
+        __syncthreads();
+        const int m = sh.index;
+#pragma unroll 1
+        for (int i = tid; i < m; i += THREADS) {
+          const u64 me = sh.list[sh.other[i]];
+          u64 ahead = 0;
+#pragma unroll 4
+          for (int j = 0; j < m; ++j) {
+            const u64 at = sh.other[j];
+            if (sh.list[at] > me) ahead += sh.weight_of[at];
+          }
+          if (ahead < want && want <= ahead + sh.weight_of[sh.other[i]]) sh.word = me;
+        }
+        __syncthreads();
+        cut = sh.word;
+#pragma unroll 1
+        for (int j = 0; j < PER; ++j) {
+          const int i = tid + j * THREADS;
+          if (i >= n) break;
+          const u64 x = sh.list[i];
+          if (x >= cut && key_in(x) >= set.key_min)
+            atomicAdd(&sh.tile[(index_in(x) + row.lead) / N / per_tile],
+                      mode == WINDOW_K ? sh.weight(of_key(key_in(x))) : sh.weight_of[i]);
+        }
+        __syncthreads();
+      }
     }
   }
   if (mode == SLOW || mode == LIST) cut = slow_cut(row, sh, set, per_tile, tiles);
@@ -892,8 +975,8 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   while ((1LL << bits) < V) ++bits;
   p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
-  // CTAs of a row: as many as leave every SM one, with 16384 logits each or more
-  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({8, sm_count() / R, V / 16384})));
+  // CTAs of a row: as many as leave an SM one or two, with 16384 logits each or more
+  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, 3 * sm_count() / 2 / R, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));
   CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
