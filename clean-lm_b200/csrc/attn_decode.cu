@@ -4,16 +4,19 @@
 //   lse = log sum_j exp(s_j)
 //
 // Bound by reading the keys and values once (2 multiply-adds per 2-byte element and query head of a group; the tensor cores
-// see 8 or 16 query columns).  The 16-key tiles of all requests and kv heads form one line that the warps of the grid share
-// evenly, whatever the lengths are; a warp's running maximum, sum and output stay in registers.  Where a warp's share cuts the
-// keys of a (request, kv head), its partial result goes to the scratch and a second kernel joins them.
+// see 8 or 16 query columns).  The tiles of 16 or 32 keys of all requests and kv heads form one line that the SMs share evenly,
+// whatever the lengths are, and the warps of an SM its part.  Every warp works alone on a ring of its own in shared memory, which
+// asynchronous 16-byte copies fill STAGES tiles ahead and across the borders of requests, 8 lanes a row, wherever its page lies.
+// (Measured on 1.14 GB, 174 us at 6.5 TB/s: loaded straight into the fragments, the next keys on their way behind the scores,
+// 12 warps of an SM had too little under way, 270 us; a bulk copy per row, which a warp issues one lane after the other, 262 us.)
+// A warp's running maximum, sum and output stay in registers.  Where a warp's part cuts the keys of a (request, kv head), the
+// warps of the SM join what they have of it; what the SM's part cuts goes to the scratch, and a second kernel joins that.
 //
 // Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
-// of mma.m16n8k16 (as rows they would leave at least half of it empty) and both K and V rows go from global memory straight
-// into the fragments, 16 bytes at a time: for the scores the order of d within a product is free, for the output the order of
-// its rows is.  (No shared memory, no barrier: a tile of the 5th-generation tensor cores has 64 or 128 rows of queries, of
-// which one token per request fills 1 to 16.)  Probabilities are rounded to bf16 for the second product, as in the prompt's
-// attention; their sum is of the unrounded ones, in f32.
+// of mma.m16n8k16 (as rows they would leave at least half of it empty) and the pieces of K and V rows that a thread reads are its
+// fragments: for the scores the order of d within a product is free, for the output the order of its rows is.  (A tile of the
+// 5th-generation tensor cores has 64 or 128 rows of queries, of which one token per request fills 1 to 16.)  Probabilities are
+// rounded to bf16 for the second product, as in the prompt's attention; their sum is of the unrounded ones, in f32.
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -24,8 +27,10 @@
 namespace cdl {
 namespace decode {
 
-constexpr int WARPS = 4;          // per CTA; each works alone
-constexpr int MAX_BATCH = 16384;  // the prefix of the lengths is kept in shared memory
+constexpr int WARPS = 8;         // of a CTA, one CTA per SM
+constexpr int STAGES = 3;        // tiles of a warp's ring
+constexpr int JOIN_WARPS = 4;    // of a CTA of the second kernel
+constexpr int MAX_BATCH = 4096;  // the prefix of the lengths is kept in shared memory beside the rings
 
 struct Params {
   const __nv_bfloat16* q;
@@ -42,10 +47,11 @@ struct Params {
   __nv_bfloat16* out;
   long long out_sb, out_sh;
   float* lse;
-  int max_workers;
+  int ctas;
   int* prefix;      // [batch + 1] tiles of the requests ahead
-  float* part_o;    // [2 max_workers][COLS][D]
-  float2* part_ml;  // [2 max_workers][COLS]
+  float2* part_ml;  // [2 ctas][COLS]
+  float* part_o;    // [2 ctas][COLS][D]
+  float* warp_o;    // [2 ctas WARPS][COLS][D]
 };
 
 // Keys a request sees: [first, end).
@@ -56,12 +62,11 @@ __device__ __forceinline__ void visible(const Params& p, int b, int& first, int&
   first = p.window > 0 ? max(0, end - p.window) : 0;
 }
 
-// How many warps share `units` tiles: all of them, but at least MIN_TILES for each (a cut costs its partial result's way
-// through memory, as much as the keys of two tiles for 8 query columns).
+// A warp has at least so many tiles while there are warps left over: a cut costs as much as the keys of two tiles.
 constexpr int MIN_TILES = 4;
-__host__ __device__ __forceinline__ long long workers_of(long long units, int max_workers) {
-  const long long w = (units + MIN_TILES - 1) / MIN_TILES;
-  return w < 1 ? 1 : (w > max_workers ? max_workers : w);
+// CTAs that share `units` tiles: every one has some, so that all partial results between a line's first and last are there.
+__device__ __forceinline__ int ctas_of(long long units, int ctas) {
+  return static_cast<int>(min(units, static_cast<long long>(ctas)));
 }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -80,17 +85,7 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Keys and values are read once: they need not stay in the L1.
-__device__ __forceinline__ uint4 load_row(const __nv_bfloat16* p, bool live) {
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (live)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
-  return r;
-}
 __device__ __forceinline__ uint32_t word(const uint4& q, int i) { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
-__device__ __forceinline__ long long shfl64(long long x, int lane) { return __shfl_sync(0xffffffffu, x, lane); }
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -98,19 +93,50 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 template <int D>
 constexpr int tile_keys() { return D == 128 ? 16 : 32; }
 
+// A row in shared memory is 16 bytes longer than in the cache: of the 8 lanes that read 16 bytes each at a time, no two meet in a
+// bank then (the pieces 2 t, 2 t + 1, .. of a key row for the scores; piece g of the rows 2 t, 2 t + 1, .. for the output).
+template <int D>
+constexpr int row_bytes() { return 2 * D + 16; }
+template <int D>
+constexpr int stage_bytes() { return 2 * tile_keys<D>() * row_bytes<D>(); }
+
+// The partial results of a CTA's warps, two each: of the line (request, kv head) that its part starts within and of the one that
+// it ends within.  Their outputs are in the scratch.
+template <int COLS>
+struct Cuts {
+  long long line[2 * WARPS];  // -1: none
+  int starts[2 * WARPS], ends[2 * WARPS];
+  float2 ml[2 * WARPS][COLS];
+};
+
+// 16 bytes to shared memory, `bytes` of them from `from` and zeros behind.
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the last N groups of this thread's copies are there.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // D: head dimension; NT: tiles of 8 query heads of one kv head.
 template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kernel(const Params p) {
+__global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params p) {
   constexpr int COLS = 8 * NT;
   constexpr int KEYS = tile_keys<D>();
   constexpr int SUB = KEYS / 16;   // 16-key products of a tile
   constexpr int KCH = D / 32;      // 16-byte pieces of a key row per thread
   constexpr int VCH = D / 64;      // 16-byte pieces of a value row per thread
   constexpr int MT = D / 16;       // 16-row tiles of the transposed output
-  extern __shared__ int prefix[];  // [batch + 1]
+  constexpr int RS = row_bytes<D>(), STAGE = stage_bytes<D>();
+  extern __shared__ __align__(128) char smem[];
+  int* prefix = reinterpret_cast<int*>(smem + WARPS * STAGES * STAGE);  // [batch + 1]
   __shared__ int warp_sum[WARPS];
+  __shared__ Cuts<COLS> cuts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  if (tid < 2 * WARPS) cuts.line[tid] = -1;
   grid_dep_wait();
   grid_dep_launch();
 
@@ -149,83 +175,114 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
 
   const int rows = p.kv_heads * p.chunks;  // lines of tiles of a request
   const long long units = static_cast<long long>(run) * rows;
-  if (units == 0) return;
-  const long long workers = workers_of(units, p.max_workers);
-  // neighbouring shares on different SMs, so that few of them are spread over the whole card
-  const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-  if (me >= workers) return;
-  long long u = units * me / workers;
-  const long long u_end = units * (me + 1) / workers;
+  // this CTA's part, and this warp's of it
+  const int ctas = ctas_of(units, p.ctas);
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
+  const long long c0 = units * blockIdx.x / ctas, c1 = units * (blockIdx.x + 1) / ctas;
+  const long long busy = min(static_cast<long long>(WARPS), (c1 - c0 + MIN_TILES - 1) / MIN_TILES);  // warps with a part
+  long long u = 0, u_end = 0;
+  if (warp < busy) u = c0 + (c1 - c0) * warp / busy, u_end = c0 + (c1 - c0) * (warp + 1) / busy;
+
+  // Line and tile of unit x: the largest b with prefix[b] <= x / rows has it.
+  struct Place {
+    int b, row, tile, n;
+  };
+  auto place_of = [&](long long x) {
+    Place at;
+    const int ahead = static_cast<int>(x / rows);
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= ahead) lo = mid;
+      else hi = mid;
+    }
+    at.b = lo;
+    at.n = prefix[lo + 1] - prefix[lo];
+    const long long rest = x - static_cast<long long>(prefix[lo]) * rows;
+    at.row = static_cast<int>(rest / at.n);
+    at.tile = static_cast<int>(rest - static_cast<long long>(at.row) * at.n);
+    return at;
+  };
+
+  // ---- the fetching side: which tile comes next, and where this lane's rows of it lie
+  const uint32_t ring = smem_u32(smem + warp * STAGES * STAGE);
+  long long next = u;  // unit
+  int left = 0;        // tiles of its line from it on
+  int key = 0, end = 0, page = -1;
+  const int* table = nullptr;
+  const __nv_bfloat16 *from_k = nullptr, *from_v = nullptr;
+  auto look_up = [&]() {  // the page of this lane's key, a tile ahead of the copies
+    page = next < u_end && key < end ? table[static_cast<unsigned>(key) / static_cast<unsigned>(p.page_size)] : -1;
+  };
+  auto enter = [&]() {  // the line of `next`
+    const Place at = place_of(next);
+    const int kvh = at.row / p.chunks;
+    int first;
+    visible(p, at.b, first, end);
+    key = first + at.tile * KEYS + (lane & (KEYS - 1));
+    left = at.n - at.tile;
+    table = p.table + at.b * p.table_sb;
+    from_k = p.k + kvh * p.k_sh;
+    from_v = p.v + kvh * p.v_sh;
+  };
+  // Fetches tile `next` into a stage, zeros where a key is not there, and goes on to the one behind it; returns which of its keys
+  // there are.
+  auto fetch = [&](int stage) -> uint32_t {
+    uint32_t mask = 0;
+    if (next < u_end) {
+      const int slot = static_cast<int>(static_cast<unsigned>(key) % static_cast<unsigned>(p.page_size));
+      const bool live = page >= 0 && page < p.pages;
+      mask = __ballot_sync(0xffffffffu, live);
+      // Where this lane's row lies; D = 128: lanes 16 to 31 have the same keys again and hold the places of their values.
+      const bool value = D == 128 && lane >= 16;
+      const long long at = value ? page * p.v_sp + slot * p.v_ss : page * p.k_sp + slot * p.k_ss;
+      const char* mine = live ? reinterpret_cast<const char*>((value ? from_v : from_k) + at) : nullptr;
+      const char* mine_v = live ? reinterpret_cast<const char*>(from_v + page * p.v_sp + slot * p.v_ss) : nullptr;  // (D = 64)
+      const uint32_t to = ring + stage * STAGE + (lane >> 3) * RS + (lane & 7) * 16;
+#pragma unroll
+      for (int j = 0; j < 2 * KEYS / 4; ++j) {
+        const char* of = D == 128 || j < KEYS / 4 ? mine : mine_v;
+        const char* row = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<long long>(of), (4 * j + (lane >> 3)) & 31));
+        const char* from = row != nullptr ? row + (lane & 7) * 16 : reinterpret_cast<const char*>(p.q);
+        const int bytes = row != nullptr ? 16 : 0;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) copy_16(to + 4 * j * RS + h * 128, from + (row != nullptr ? h * 128 : 0), bytes);
+      }
+      ++next, --left, key += KEYS;
+      if (left == 0 && next < u_end) enter();
+      look_up();
+    }
+    copies_commit();
+    return mask;
+  };
+  uint32_t live_of[STAGES];
+  if (u < u_end) {
+    enter();
+    look_up();
+  }
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) live_of[s] = fetch(s);
+
   const float sm2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
   const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
-
+  int stage = 0;
   while (u < u_end) {
-    int b = 0;
-    {
-      const int at = static_cast<int>(u / rows);
-      int hi = p.batch;  // largest b with prefix[b] <= at
-      while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (prefix[mid] <= at) b = mid;
-        else hi = mid;
-      }
-    }
-    const int n = prefix[b + 1] - prefix[b];
-    const long long rest = u - static_cast<long long>(prefix[b]) * rows;
-    const int row = static_cast<int>(rest / n), t0 = static_cast<int>(rest - static_cast<long long>(row) * n);
-    const int t1 = static_cast<int>(min(static_cast<long long>(n), t0 + (u_end - u)));
-    const int kvh = row / p.chunks, col0 = (row - kvh * p.chunks) * COLS;
+    const Place at = place_of(u);
+    const int t0 = at.tile, t1 = static_cast<int>(min(static_cast<long long>(at.n), t0 + (u_end - u)));
+    const int kvh = at.row / p.chunks, col0 = (at.row - kvh * p.chunks) * COLS;
     const int cols = min(COLS, p.group - col0);
     const int head0 = kvh * p.group + col0;
-    int first, end;
-    visible(p, b, first, end);
 
-    // ---- q: thread (g, t) has the pieces t, t + 4, .. of column g
+    // ---- q: thread (g, t) has the pieces 2 t, 2 t + 1 (and those 8 further on) of column g
     uint4 qf[NT][KCH];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < KCH; ++i)
-        qf[j][i] = load_row(p.q + b * p.q_sb + (head0 + j * 8 + g) * p.q_sh + (t + 4 * i) * 8, j * 8 + g < cols);
-
-    const int* table = p.table + b * p.table_sb;
-    const __nv_bfloat16* kb = p.k + kvh * p.k_sh + t * 8;
-    const __nv_bfloat16* vb = p.v + kvh * p.v_sh + g * 8;
-    // Lane l looks the page of the tile's key l up, one tile ahead of the loads that go there.
-    auto look_up = [&](int tile) {
-      const int key = first + tile * KEYS + (lane & (KEYS - 1));
-      return tile < t1 && key < end ? table[static_cast<unsigned>(key) / static_cast<unsigned>(p.page_size)] : -1;
-    };
-    long long at_k = -1, at_v = -1;  // where the row of key l lies; -1: not read
-    auto place = [&](int tile, int page) {
-      const int key = first + tile * KEYS + (lane & (KEYS - 1));
-      const int slot = static_cast<int>(static_cast<unsigned>(key) % static_cast<unsigned>(p.page_size));
-      const bool live = page >= 0 && page < p.pages;
-      at_k = live ? page * p.k_sp + slot * p.k_ss : -1;
-      at_v = live ? page * p.v_sp + slot * p.v_ss : -1;
-    };
-    uint4 kf[SUB][2][KCH], vf[SUB][4][VCH];
-    auto load_k = [&](bool (&live)[SUB][2]) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const long long at = shfl64(at_k, s * 16 + r * 8 + g);
-          live[s][r] = at >= 0;
-#pragma unroll
-          for (int i = 0; i < KCH; ++i) kf[s][r][i] = load_row(kb + at + i * 32, at >= 0);
-        }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const long long at = shfl64(at_v, s * 16 + 2 * t + (r & 1) + (r >> 1) * 8);
-#pragma unroll
-          for (int i = 0; i < VCH; ++i) vf[s][r][i] = load_row(vb + at + i * 64, at >= 0);
-        }
-    };
+      for (int i = 0; i < KCH; ++i) {
+        qf[j][i] = make_uint4(0, 0, 0, 0);
+        if (j * 8 + g < cols)
+          qf[j][i] = ld_nc_v4(p.q + at.b * p.q_sb + (head0 + j * 8 + g) * p.q_sh + (2 * t + (i & 1) + 8 * (i >> 1)) * 8);
+      }
 
     float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -235,35 +292,49 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     }
-    bool live[SUB][2];
-    int page = look_up(t0);
-    place(t0, page);
-    page = look_up(t0 + 1);
-    load_k(live);
-    load_v();
+#pragma unroll 1
     for (int tile = t0; tile < t1; ++tile) {
+      copies_wait<STAGES - 1>();
+      __syncwarp();
+      const uint32_t live = live_of[0];
+      const char* keys = smem + (warp * STAGES + stage) * STAGE;
+      const char* values = keys + KEYS * RS;
       // ---- scores^T: rows are keys, columns query heads
       float s[SUB][NT][4];
 #pragma unroll
-      for (int x = 0; x < SUB; ++x)
+      for (int x = 0; x < SUB; ++x) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          s[x][j][0] = s[x][j][1] = s[x][j][2] = s[x][j][3] = 0.f;
+        for (int j = 0; j < NT; ++j) s[x][j][0] = s[x][j][1] = s[x][j][2] = s[x][j][3] = 0.f;
 #pragma unroll
-          for (int i = 0; i < KCH; ++i) {
-            mma_bf16(s[x][j], kf[x][0][i].x, kf[x][1][i].x, kf[x][0][i].y, kf[x][1][i].y, qf[j][i].x, qf[j][i].y);
-            mma_bf16(s[x][j], kf[x][0][i].z, kf[x][1][i].z, kf[x][0][i].w, kf[x][1][i].w, qf[j][i].z, qf[j][i].w);
+        for (int i = 0; i < KCH; ++i) {
+          const char* piece = keys + (x * 16 + g) * RS + (2 * t + (i & 1) + 8 * (i >> 1)) * 16;
+          const uint4 a = ld_shared_v4(piece), b = ld_shared_v4(piece + 8 * RS);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_bf16(s[x][j], a.x, b.x, a.y, b.y, qf[j][i].x, qf[j][i].y);
+            mma_bf16(s[x][j], a.z, b.z, a.w, b.w, qf[j][i].z, qf[j][i].w);
           }
         }
-      bool had[SUB][2];
-#pragma unroll
-      for (int x = 0; x < SUB; ++x) had[x][0] = live[x][0], had[x][1] = live[x][1];
-      // the next tile's keys, while this one's values are still on their way
-      if (tile + 1 < t1) {
-        place(tile + 1, page);
-        page = look_up(tile + 2);
-        load_k(live);
       }
+      // ---- this thread's values
+      uint4 vf[SUB][4][VCH];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = x * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
+#pragma unroll
+          for (int i = 0; i < VCH; ++i) vf[x][r][i] = ld_shared_v4(values + row * RS + (g + 8 * i) * 16);
+        }
+      constexpr uint32_t ALL = KEYS == 32 ? 0xFFFFFFFFu : (1u << (KEYS & 31)) - 1;
+      const bool every = (live & ALL) == ALL;
+      // ---- the stage is free for the tile STAGES further on
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i + 1 < STAGES; ++i) live_of[i] = live_of[i + 1];
+      live_of[STAGES - 1] = fetch(stage);
+      if (++stage == STAGES) stage = 0;
+
       // ---- running softmax, in powers of 2
       uint32_t pf[SUB][NT][2];
 #pragma unroll
@@ -275,7 +346,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
           for (int c = 0; c < 4; ++c) {
             float y = s[x][j][c];
             y = p.cap > 0.f ? cap2 * tanhf(y * to_cap) : y * sm2;
-            y = had[x][c >> 1] ? y : -INFINITY;
+            if (!every) y = (live >> (x * 16 + g + (c >> 1) * 8)) & 1 ? y : -INFINITY;
             s[x][j][c] = y;
             top[c & 1] = fmaxf(top[c & 1], y);
           }
@@ -321,7 +392,6 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
 #pragma unroll
           for (int j = 0; j < NT; ++j) mma_bf16(o[j][i], a0, a1, a2, a3, pf[x][j][0], pf[x][j][1]);
         }
-      if (tile + 1 < t1) load_v();
     }
 
     // ---- the sums over the keys; out, or the partial result
@@ -331,8 +401,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
-    const bool whole = t0 == 0 && t1 == n;
-    const long long slot = (2 * me + (t0 == 0)) * COLS;
+    const bool whole = t0 == 0 && t1 == at.n;
+    const int entry = 2 * warp + (t0 == 0);
+    if (!whole && lane == 0) {
+      cuts.line[entry] = static_cast<long long>(at.b) * rows + at.row;
+      cuts.starts[entry] = t0 == 0, cuts.ends[entry] = t1 == at.n;
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -348,7 +422,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
         }
         if (whole) {
           const float inv = l[j][c] == 0.f ? 0.f : 1.f / l[j][c];
-          __nv_bfloat16* to = p.out + b * p.out_sb + (head0 + col) * p.out_sh + g * 8;
+          __nv_bfloat16* to = p.out + at.b * p.out_sb + (head0 + col) * p.out_sh + g * 8;
           uint4 w;
           w.x = pack_bf16x2(lo[0] * inv, lo[1] * inv), w.y = pack_bf16x2(lo[2] * inv, lo[3] * inv);
           w.z = pack_bf16x2(lo[4] * inv, lo[5] * inv), w.w = pack_bf16x2(lo[6] * inv, lo[7] * inv);
@@ -359,31 +433,76 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_decode_kerne
             *reinterpret_cast<uint4*>(to + 64) = w;
           }
           if (p.lse != nullptr && g == 0)
-            p.lse[static_cast<long long>(b) * p.heads + head0 + col] =
+            p.lse[static_cast<long long>(at.b) * p.heads + head0 + col] =
                 l[j][c] == 0.f ? -INFINITY : (m[j][c] + log2f(l[j][c])) * LN2;
         } else {
-          float* to = p.part_o + (slot + col) * D + g * 8;
+          float* to = p.warp_o + ((static_cast<long long>(blockIdx.x) * 2 * WARPS + entry) * COLS + col) * D + g * 8;
           *reinterpret_cast<float4*>(to) = make_float4(lo[0], lo[1], lo[2], lo[3]);
           *reinterpret_cast<float4*>(to + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
           if (D == 128) {
             *reinterpret_cast<float4*>(to + 64) = make_float4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<float4*>(to + 68) = make_float4(hi[4], hi[5], hi[6], hi[7]);
           }
-          if (g == 0) p.part_ml[slot + col] = make_float2(m[j][c], l[j][c]);
+          if (g == 0) cuts.ml[entry][col] = make_float2(m[j][c], l[j][c]);
         }
       }
     u += t1 - t0;
+  }
+  __syncthreads();
+
+  // ---- joins what the warps have of the same line, in the order of the keys
+  for (int e0 = 0, e1; e0 < 2 * WARPS; e0 = e1) {
+    e1 = e0 + 1;
+    const long long line = cuts.line[e0];
+    if (line < 0) continue;
+    int last = e0;
+    while (e1 < 2 * WARPS && (cuts.line[e1] < 0 || cuts.line[e1] == line)) {
+      if (cuts.line[e1] == line) last = e1;
+      ++e1;
+    }
+    const int b = static_cast<int>(line / rows), row = static_cast<int>(line - static_cast<long long>(b) * rows);
+    const int kvh = row / p.chunks, col0 = (row - kvh * p.chunks) * COLS;
+    const int cols = min(COLS, p.group - col0), head0 = kvh * p.group + col0;
+    const bool whole = cuts.starts[e0] && cuts.ends[last];
+    for (int i = tid; i < cols * (D / 4); i += WARPS * 32) {
+      const int col = i / (D / 4), d = i % (D / 4) * 4;
+      float top = -INFINITY, l = 0.f;
+      for (int e = e0; e <= last; ++e)
+        if (cuts.line[e] == line) top = fmaxf(top, cuts.ml[e][col].x);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int e = e0; e <= last; ++e) {
+        if (cuts.line[e] != line) continue;
+        const float2 ml = cuts.ml[e][col];
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(
+            p.warp_o + ((static_cast<long long>(blockIdx.x) * 2 * WARPS + e) * COLS + col) * D + d));
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);  // (1: NaN, which stays)
+        l += f * ml.y;
+        sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
+      }
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(p.out + b * p.out_sb + (head0 + col) * p.out_sh + d) =
+            make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+        if (p.lse != nullptr && d == 0)
+          p.lse[static_cast<long long>(b) * p.heads + head0 + col] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+      } else {
+        const long long slot = (2LL * blockIdx.x + (cuts.starts[e0] != 0)) * COLS + col;
+        *reinterpret_cast<float4*>(p.part_o + slot * D + d) = sum;
+        if (d == 0) p.part_ml[slot] = make_float2(top, l);
+      }
+    }
   }
 }
 
 // Joins the partial results of a (request, head): one warp each, in the order of the keys.  Requests that see no key get
 // zeros and -inf here.
 template <int D, int COLS>
-__global__ void __launch_bounds__(WARPS * 32) attn_decode_join_kernel(const Params p) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_decode_join_kernel(const Params p) {
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  const long long item = static_cast<long long>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
   if (item >= static_cast<long long>(p.batch) * p.heads) return;
   const int b = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(b) * p.heads);
   const int kvh = head / p.group, in = head - kvh * p.group, row = kvh * p.chunks + in / COLS, col = in % COLS;
@@ -396,21 +515,20 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_join_kernel(const Para
   for (int e = 0; e < E; ++e) sum[e] = 0.f;
   float top = -INFINITY, l = 0.f;
   if (n > 0) {
-    const long long workers = workers_of(units, p.max_workers);
     const long long u0 = static_cast<long long>(ahead) * rows + static_cast<long long>(row) * n;
-    const long long w0 = ((u0 + 1) * workers - 1) / units, w1 = ((u0 + n) * workers - 1) / units;
-    if (w0 == w1) return;  // one warp had all of it
-    for (long long w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, p.part_ml[(2 * w + (w == w0)) * COLS + col].x);
+    const int ctas = ctas_of(units, p.ctas);
+    const int c0 = static_cast<int>(((u0 + 1) * ctas - 1) / units), c1 = static_cast<int>(((u0 + n) * ctas - 1) / units);
+    if (c0 == c1) return;  // one CTA had all of it
+    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(2LL * c + (c == c0)) * COLS + col].x);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    for (long long w = w0; w <= w1; ++w) {
-      const long long slot = (2 * w + (w == w0)) * COLS + col;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const long long slot = (2LL * c + (c == c0)) * COLS + col;
       const float2 ml = p.part_ml[slot];
-      // (a maximum that is NaN does not occur; sums and outputs that are NaN stay so)
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);  // (1: NaN, which stays)
       const float* from = p.part_o + slot * D + lane * E;
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;
-      l += ml.y * (ml.x == -INFINITY ? 1.f : f);
+      l += f * ml.y;
       if (E == 4) {
         const float4 x = *reinterpret_cast<const float4*>(from);
         sum[0] += f * x.x, sum[1] += f * x.y, sum[E - 2] += f * x.z, sum[E - 1] += f * x.w;
@@ -433,8 +551,6 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_join_kernel(const Para
 // Bytes of the scratch: tiles ahead of each request, then the partial results of 2 per warp.
 static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 static int tiles_of_columns(long long group) { return group <= 8 ? 1 : 2; }
-static int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-
 static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tensor* k_cache) {
   if (!q || !k_cache) return fail(CDL_ERR_INVALID, "%s: q and k_cache are required", op);
   if (q->rank != 3 || q->dtype != CDL_BF16) return fail(CDL_ERR_INVALID, "%s: q must be bf16 [batch, heads, head_dim]", op);
@@ -453,8 +569,8 @@ static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tens
 }
 
 static size_t decode_scratch_bytes(long long batch, int nt, long long d) {
-  const size_t slots = 2ull * sm_count() * ctas_per_sm(nt) * decode::WARPS * 8 * nt;
-  return align256((batch + 1) * 4) + align256(slots * 8) + slots * d * 4;
+  const size_t slots = 2ull * sm_count() * 8 * nt;
+  return align256((batch + 1) * 4) + align256(slots * 8) + slots * d * 4 * (1 + decode::WARPS);
 }
 
 // Rows of `d` elements from a 16-byte boundary on, whatever the strides of the outer dimensions.
@@ -521,8 +637,7 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255) || scratch_bytes < decode_scratch_bytes(B, nt, D))
     return fail(CDL_ERR_INVALID, "%s: scratch must be 256-byte aligned and hold %zu bytes", op, decode_scratch_bytes(B, nt, D));
 
-  const int full = sm_count() * ctas_per_sm(nt);
-  const int grid = static_cast<int>(std::min<long long>(full, decode::workers_of(tiles * rows, full)));
+  const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(sm_count(), tiles * rows)));
   decode::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q->ptr), p.q_sb = q->stride[0], p.q_sh = q->stride[1];
   p.k = static_cast<const __nv_bfloat16*>(k_cache->ptr), p.v = static_cast<const __nv_bfloat16*>(v_cache->ptr);
@@ -538,24 +653,25 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   p.cap = desc->softcap;
   p.out = static_cast<__nv_bfloat16*>(out->ptr), p.out_sb = out->stride[0], p.out_sh = out->stride[1];
   p.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  p.max_workers = grid * decode::WARPS;
+  p.ctas = grid;
   char* at = static_cast<char*>(scratch);
-  const size_t slots = 2ull * p.max_workers * cols;
+  const size_t slots = 2ull * sm_count() * cols;
   p.prefix = reinterpret_cast<int*>(at), at += align256((B + 1) * 4);
   p.part_ml = reinterpret_cast<float2*>(at), at += align256(slots * 8);
-  p.part_o = reinterpret_cast<float*>(at);
+  p.part_o = reinterpret_cast<float*>(at), at += slots * D * 4;
+  p.warp_o = reinterpret_cast<float*>(at);
 
   ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
   void (*kernel)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1> : decode::attn_decode_kernel<128, 2>)
                                             : (nt == 1 ? decode::attn_decode_kernel<64, 1> : decode::attn_decode_kernel<64, 2>);
   void (*join)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
-  const size_t smem = (B + 1) * sizeof(int);
-  if (smem > 40 * 1024)
-    CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  const size_t smem = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>()) +
+                      (B + 1) * sizeof(int);
+  CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
-  const long long joins = (B * H + decode::WARPS - 1) / decode::WARPS;
-  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(joins)), dim3(decode::WARPS * 32), 0, stream, p));
+  const long long joins = (B * H + decode::JOIN_WARPS - 1) / decode::JOIN_WARPS;
+  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(joins)), dim3(decode::JOIN_WARPS * 32), 0, stream, p));
   return CDL_OK;
 }
 
