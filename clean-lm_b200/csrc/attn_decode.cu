@@ -4,13 +4,15 @@
 //   lse = log sum_j exp(s_j)
 //
 // Bound by reading the keys and values once (2 multiply-adds per 2-byte element and query head of a group; the tensor cores
-// see 8 or 16 query columns).  The tiles of 16 or 32 keys of all requests and kv heads form one line that the SMs share evenly,
-// whatever the lengths are, and the warps of an SM its part.  Every warp works alone on a ring of its own in shared memory, which
-// asynchronous 16-byte copies fill STAGES tiles ahead and across the borders of requests, 8 lanes a row, wherever its page lies.
-// (Measured on 1.14 GB, 174 us at 6.5 TB/s: loaded straight into the fragments, the next keys on their way behind the scores,
-// 12 warps of an SM had too little under way, 270 us; a bulk copy per row, which a warp issues one lane after the other, 262 us.)
-// A warp's running maximum, sum and output stay in registers.  Where a warp's part cuts the keys of a (request, kv head), the
-// warps of the SM join what they have of it; what the SM's part cuts goes to the scratch, and a second kernel joins that.
+// see 8 or 16 query columns).  The tiles of 16 or 32 keys of all requests and kv heads form one line, whatever the lengths are,
+// that the CTAs share, and the warps of a CTA its part.  SMs do not read at the same rate (equal parts ended after 147 to 204 us,
+// the same SMs late each time), so the first CTAs, all of which run at once, take two thirds, and three more sets of smaller parts
+// follow as SMs become free.  Every warp works alone on a ring of its own in shared memory, which asynchronous 16-byte copies fill
+// STAGES tiles ahead and across the borders of requests, 8 lanes a row, wherever its page lies.  (Loaded straight into the
+// fragments, the next keys on their way behind the scores, 12 warps of an SM had too little under way, 270 us for 1.14 GB, which
+// are 174 us at 6.5 TB/s; a bulk copy per row, which a warp issues one lane after the other, took 262 us.)  A warp's running
+// maximum, sum and output stay in registers.  Where a warp's part cuts the keys of a (request, kv head), the warps of the CTA join
+// what they have of it; what the CTA's part cuts goes to the scratch, and a second kernel joins that.
 //
 // Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
 // of mma.m16n8k16 (as rows they would leave at least half of it empty) and the pieces of K and V rows that a thread reads are its
@@ -27,9 +29,11 @@
 namespace cdl {
 namespace decode {
 
-constexpr int WARPS = 8;         // of a CTA, one CTA per SM
-constexpr int STAGES = 3;        // tiles of a warp's ring
-constexpr int JOIN_WARPS = 4;    // of a CTA of the second kernel
+constexpr int WARPS = 4;         // of a CTA
+constexpr int STAGES = 2;        // tiles of a warp's ring
+// CTAs of an SM: as many as registers (168 of 12 warps, 255 of 8) and rings (70 KB each) allow; nt: tiles of 8 query columns
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int JOIN_WARPS = 8;    // of a CTA of the second kernel
 constexpr int MAX_BATCH = 4096;  // the prefix of the lengths is kept in shared memory beside the rings
 
 struct Params {
@@ -47,11 +51,11 @@ struct Params {
   __nv_bfloat16* out;
   long long out_sb, out_sh;
   float* lse;
-  int ctas;
+  int set;          // CTAs that run at once
   int* prefix;      // [batch + 1] tiles of the requests ahead
-  float2* part_ml;  // [2 ctas][COLS]
-  float* part_o;    // [2 ctas][COLS][D]
-  float* warp_o;    // [2 ctas WARPS][COLS][D]
+  float2* part_ml;  // [2 CTAs][COLS]
+  float* part_o;    // [2 CTAs][COLS][D]
+  float* warp_o;    // [CTAs][WARPS][COLS][D]
 };
 
 // Keys a request sees: [first, end).
@@ -64,10 +68,31 @@ __device__ __forceinline__ void visible(const Params& p, int b, int& first, int&
 
 // A warp has at least so many tiles while there are warps left over: a cut costs as much as the keys of two tiles.
 constexpr int MIN_TILES = 4;
-// CTAs that share `units` tiles: every one has some, so that all partial results between a line's first and last are there.
-__device__ __forceinline__ int ctas_of(long long units, int ctas) {
-  return static_cast<int>(min(units, static_cast<long long>(ctas)));
-}
+// How the CTAs share `units` tiles: few of them evenly, one or more each (so that all partial results between a line's first and
+// last are there); many in SETS sets of `set` CTAs, evenly within a set.
+constexpr int SETS = 4, PARTS = 128;  // of PARTS parts of the whole the sets have 84, 28, 11 and 5
+struct Shares {
+  long long units;
+  int set, ctas;
+  __host__ __device__ __forceinline__ Shares(long long units, int set) : units(units), set(set) {
+    ctas = units >= 32LL * WARPS * set ? SETS * set : static_cast<int>(units < set ? units : set);
+  }
+  static __host__ __device__ __forceinline__ int ahead(int i) { return i == 0 ? 0 : i == 1 ? 84 : i == 2 ? 112 : i == 3 ? 123 : 128; }
+  __device__ __forceinline__ long long begin(int c) const {
+    if (ctas <= set) return units * c / ctas;
+    const int i = c / set;  // (SETS for the end)
+    return units * (static_cast<long long>(ahead(i)) * set + static_cast<long long>(ahead(min(i + 1, SETS)) - ahead(i)) * (c - i * set)) /
+           (static_cast<long long>(PARTS) * set);
+  }
+  // The CTA that has unit u: the last one that begins at it or ahead of it.
+  __device__ __forceinline__ int of(long long u) const {
+    if (ctas <= set) return static_cast<int>(((u + 1) * ctas - 1) / units);
+    int i = SETS - 1;
+    while (begin(i * set) > u) --i;
+    const long long part = ahead(i + 1) - ahead(i);
+    return i * set + static_cast<int>(((u + 1) * PARTS * set - units * ahead(i) * set - 1) / (units * part));
+  }
+};
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -101,11 +126,11 @@ template <int D>
 constexpr int stage_bytes() { return 2 * tile_keys<D>() * row_bytes<D>(); }
 
 // The partial results of a CTA's warps, two each: of the line (request, kv head) that its part starts within and of the one that
-// it ends within.  Their outputs are in the scratch.
+// it ends within.  The output of a warp's last line takes the place of its ring, that of one ahead is in the scratch.
 template <int COLS>
 struct Cuts {
   long long line[2 * WARPS];  // -1: none
-  int starts[2 * WARPS], ends[2 * WARPS];
+  int starts[2 * WARPS], ends[2 * WARPS], in_ring[2 * WARPS];
   float2 ml[2 * WARPS][COLS];
 };
 
@@ -122,7 +147,7 @@ __device__ __forceinline__ void copies_wait() {
 
 // D: head dimension; NT: tiles of 8 query heads of one kv head.
 template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params p) {
+__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kernel(const Params p) {
   constexpr int COLS = 8 * NT;
   constexpr int KEYS = tile_keys<D>();
   constexpr int SUB = KEYS / 16;   // 16-key products of a tile
@@ -130,6 +155,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
   constexpr int VCH = D / 64;      // 16-byte pieces of a value row per thread
   constexpr int MT = D / 16;       // 16-row tiles of the transposed output
   constexpr int RS = row_bytes<D>(), STAGE = stage_bytes<D>();
+  static_assert(COLS * D * 4 <= STAGES * STAGE, "an output takes the place of a ring");
   extern __shared__ __align__(128) char smem[];
   int* prefix = reinterpret_cast<int*>(smem + WARPS * STAGES * STAGE);  // [batch + 1]
   __shared__ int warp_sum[WARPS];
@@ -176,9 +202,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
   const int rows = p.kv_heads * p.chunks;  // lines of tiles of a request
   const long long units = static_cast<long long>(run) * rows;
   // this CTA's part, and this warp's of it
-  const int ctas = ctas_of(units, p.ctas);
-  if (static_cast<int>(blockIdx.x) >= ctas) return;
-  const long long c0 = units * blockIdx.x / ctas, c1 = units * (blockIdx.x + 1) / ctas;
+  if (units == 0) return;
+  const Shares shares(units, p.set);
+  if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
+  const long long c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
   const long long busy = min(static_cast<long long>(WARPS), (c1 - c0 + MIN_TILES - 1) / MIN_TILES);  // warps with a part
   long long u = 0, u_end = 0;
   if (warp < busy) u = c0 + (c1 - c0) * warp / busy, u_end = c0 + (c1 - c0) * (warp + 1) / busy;
@@ -401,11 +428,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
-    const bool whole = t0 == 0 && t1 == at.n;
+    const bool whole = t0 == 0 && t1 == at.n, last = u + (t1 - t0) == u_end;
     const int entry = 2 * warp + (t0 == 0);
+    if (!whole && last) {  // the ring is empty (copies of nothing but zeros may be under way)
+      copies_wait<0>();
+      __syncwarp();
+    }
     if (!whole && lane == 0) {
       cuts.line[entry] = static_cast<long long>(at.b) * rows + at.row;
-      cuts.starts[entry] = t0 == 0, cuts.ends[entry] = t1 == at.n;
+      cuts.starts[entry] = t0 == 0, cuts.ends[entry] = t1 == at.n, cuts.in_ring[entry] = last;
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -436,7 +467,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
             p.lse[static_cast<long long>(at.b) * p.heads + head0 + col] =
                 l[j][c] == 0.f ? -INFINITY : (m[j][c] + log2f(l[j][c])) * LN2;
         } else {
-          float* to = p.warp_o + ((static_cast<long long>(blockIdx.x) * 2 * WARPS + entry) * COLS + col) * D + g * 8;
+          float* to = (last ? reinterpret_cast<float*>(smem + warp * STAGES * STAGE)
+                            : p.warp_o + (static_cast<long long>(blockIdx.x) * WARPS + warp) * COLS * D) + col * D + g * 8;
           *reinterpret_cast<float4*>(to) = make_float4(lo[0], lo[1], lo[2], lo[3]);
           *reinterpret_cast<float4*>(to + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
           if (D == 128) {
@@ -474,8 +506,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
       for (int e = e0; e <= last; ++e) {
         if (cuts.line[e] != line) continue;
         const float2 ml = cuts.ml[e][col];
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(
-            p.warp_o + ((static_cast<long long>(blockIdx.x) * 2 * WARPS + e) * COLS + col) * D + d));
+        const float4 x = cuts.in_ring[e]
+                             ? *reinterpret_cast<const float4*>(smem + (e >> 1) * STAGES * STAGE + (col * D + d) * 4)
+                             : __ldcg(reinterpret_cast<const float4*>(
+                                   p.warp_o + (static_cast<long long>(blockIdx.x) * WARPS + (e >> 1)) * COLS * D + col * D + d));
         const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);  // (1: NaN, which stays)
         l += f * ml.y;
         sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
@@ -495,56 +529,63 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attn_decode_kernel(const Params
   }
 }
 
-// Joins the partial results of a (request, head): one warp each, in the order of the keys.  Requests that see no key get
-// zeros and -inf here.
+// Joins the partial results of a (request, head), a CTA each: its warps take them in turn, and their sums meet in the order of the
+// warps.  Requests that see no key get zeros and -inf here.
 template <int D, int COLS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_decode_join_kernel(const Params p) {
+  __shared__ float4 sums[JOIN_WARPS][D / 4];
+  __shared__ float ls[JOIN_WARPS];
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
-  if (item >= static_cast<long long>(p.batch) * p.heads) return;
-  const int b = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(b) * p.heads);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / p.heads, head = blockIdx.x - b * p.heads;
   const int kvh = head / p.group, in = head - kvh * p.group, row = kvh * p.chunks + in / COLS, col = in % COLS;
   const int ahead = p.prefix[b], n = p.prefix[b + 1] - ahead;
   const int rows = p.kv_heads * p.chunks;
   const long long units = static_cast<long long>(p.prefix[p.batch]) * rows;
-  constexpr int E = D / 32;  // elements of a lane
-  float sum[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = 0.f;
+  constexpr int LANES = D / 4;  // of a partial result; D = 64: a warp takes two at a time
+  constexpr int PER = 32 / LANES;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float top = -INFINITY, l = 0.f;
   if (n > 0) {
     const long long u0 = static_cast<long long>(ahead) * rows + static_cast<long long>(row) * n;
-    const int ctas = ctas_of(units, p.ctas);
-    const int c0 = static_cast<int>(((u0 + 1) * ctas - 1) / units), c1 = static_cast<int>(((u0 + n) * ctas - 1) / units);
+    const Shares shares(units, p.set);
+    const int c0 = shares.of(u0), c1 = shares.of(u0 + n - 1);
     if (c0 == c1) return;  // one CTA had all of it
     for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(2LL * c + (c == c0)) * COLS + col].x);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
+#pragma unroll 8
+    for (int c = c0 + warp * PER + lane / LANES; c <= c1; c += JOIN_WARPS * PER) {
       const long long slot = (2LL * c + (c == c0)) * COLS + col;
       const float2 ml = p.part_ml[slot];
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane % LANES * 4);
       const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);  // (1: NaN, which stays)
-      const float* from = p.part_o + slot * D + lane * E;
       l += f * ml.y;
-      if (E == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(from);
-        sum[0] += f * x.x, sum[1] += f * x.y, sum[E - 2] += f * x.z, sum[E - 1] += f * x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(from);
-        sum[0] += f * x.x, sum[1] += f * x.y;
-      }
+      sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
+    }
+    if (PER == 2) {
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16), sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
+      sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16), sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
     }
   }
+  if (lane < LANES) sums[warp][lane] = sum;
+  if (lane == 0) ls[warp] = l;
+  __syncthreads();
+  if (tid >= LANES) return;
+  l = 0.f;
+  sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < JOIN_WARPS; ++w) {
+    const float4 x = sums[w][tid];
+    l += ls[w];
+    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* to = p.out + b * p.out_sb + head * p.out_sh + lane * E;
-  if (E == 4)
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[E - 2] * inv, sum[E - 1] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(sum[0] * inv, sum[1] * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[item] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+  *reinterpret_cast<uint2*>(p.out + b * p.out_sb + head * p.out_sh + tid * 4) =
+      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+  if (p.lse != nullptr && tid == 0) p.lse[blockIdx.x] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 }  // namespace decode
 
@@ -569,8 +610,8 @@ static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tens
 }
 
 static size_t decode_scratch_bytes(long long batch, int nt, long long d) {
-  const size_t slots = 2ull * sm_count() * 8 * nt;
-  return align256((batch + 1) * 4) + align256(slots * 8) + slots * d * 4 * (1 + decode::WARPS);
+  const size_t ctas = static_cast<size_t>(decode::SETS) * sm_count() * decode::ctas_per_sm(nt), cols = 8 * nt;
+  return align256((batch + 1) * 4) + align256(2 * ctas * cols * 8) + (2 + decode::WARPS) * ctas * cols * d * 4;
 }
 
 // Rows of `d` elements from a 16-byte boundary on, whatever the strides of the outer dimensions.
@@ -637,7 +678,9 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255) || scratch_bytes < decode_scratch_bytes(B, nt, D))
     return fail(CDL_ERR_INVALID, "%s: scratch must be 256-byte aligned and hold %zu bytes", op, decode_scratch_bytes(B, nt, D));
 
-  const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(sm_count(), tiles * rows)));
+  if (tiles * rows > (1LL << 40)) return fail(CDL_ERR_UNSUPPORTED, "%s: more than 2^40 tiles of keys", op);
+  const int set = sm_count() * decode::ctas_per_sm(nt);
+  const int grid = std::max(1, decode::Shares(tiles * rows, set).ctas);  // (the lengths may leave some without a part)
   decode::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q->ptr), p.q_sb = q->stride[0], p.q_sh = q->stride[1];
   p.k = static_cast<const __nv_bfloat16*>(k_cache->ptr), p.v = static_cast<const __nv_bfloat16*>(v_cache->ptr);
@@ -653,12 +696,12 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   p.cap = desc->softcap;
   p.out = static_cast<__nv_bfloat16*>(out->ptr), p.out_sb = out->stride[0], p.out_sh = out->stride[1];
   p.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  p.ctas = grid;
+  p.set = set;
   char* at = static_cast<char*>(scratch);
-  const size_t slots = 2ull * sm_count() * cols;
+  const size_t ctas = static_cast<size_t>(decode::SETS) * set;
   p.prefix = reinterpret_cast<int*>(at), at += align256((B + 1) * 4);
-  p.part_ml = reinterpret_cast<float2*>(at), at += align256(slots * 8);
-  p.part_o = reinterpret_cast<float*>(at), at += slots * D * 4;
+  p.part_ml = reinterpret_cast<float2*>(at), at += align256(2 * ctas * cols * 8);
+  p.part_o = reinterpret_cast<float*>(at), at += 2 * ctas * cols * D * 4;
   p.warp_o = reinterpret_cast<float*>(at);
 
   ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
@@ -670,8 +713,7 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
                       (B + 1) * sizeof(int);
   CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
-  const long long joins = (B * H + decode::JOIN_WARPS - 1) / decode::JOIN_WARPS;
-  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(joins)), dim3(decode::JOIN_WARPS * 32), 0, stream, p));
+  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(B * H)), dim3(decode::JOIN_WARPS * 32), 0, stream, p));
   return CDL_OK;
 }
 
