@@ -71,6 +71,8 @@ constexpr int MIN_TILES = 4;
 // How the CTAs share `units` tiles: few of them evenly, one or more each (so that all partial results between a line's first and
 // last are there); many in SETS sets of `set` CTAs, evenly within a set.
 constexpr int SETS = 4, PARTS = 128;  // of PARTS parts of the whole the sets have 84, 28, 11 and 5
+// (Quotients are taken in f64, a tenth of the time of a 64-bit division: exact where units * ctas < 2^53, and in any case the same
+// everywhere and never falling.)
 struct Shares {
   long long units;
   int set, ctas;
@@ -78,19 +80,26 @@ struct Shares {
     ctas = units >= 32LL * WARPS * set ? SETS * set : static_cast<int>(units < set ? units : set);
   }
   static __host__ __device__ __forceinline__ int ahead(int i) { return i == 0 ? 0 : i == 1 ? 84 : i == 2 ? 112 : i == 3 ? 123 : 128; }
-  __device__ __forceinline__ long long begin(int c) const {
-    if (ctas <= set) return units * c / ctas;
-    const int i = c / set;  // (SETS for the end)
-    return units * (static_cast<long long>(ahead(i)) * set + static_cast<long long>(ahead(min(i + 1, SETS)) - ahead(i)) * (c - i * set)) /
-           (static_cast<long long>(PARTS) * set);
+  __host__ __device__ __forceinline__ long long begin(int c) const {
+    const double n = static_cast<double>(units);
+    if (ctas <= set) return static_cast<long long>(n * c / ctas);
+    const int i = c >= 3 * set ? 3 : c >= 2 * set ? 2 : c >= set ? 1 : 0;
+    return static_cast<long long>(n * (ahead(i) * set + (ahead(i + 1) - ahead(i)) * (c - i * set)) / (PARTS * set));
   }
   // The CTA that has unit u: the last one that begins at it or ahead of it.
-  __device__ __forceinline__ int of(long long u) const {
-    if (ctas <= set) return static_cast<int>(((u + 1) * ctas - 1) / units);
-    int i = SETS - 1;
-    while (begin(i * set) > u) --i;
-    const long long part = ahead(i + 1) - ahead(i);
-    return i * set + static_cast<int>(((u + 1) * PARTS * set - units * ahead(i) * set - 1) / (units * part));
+  __host__ __device__ __forceinline__ int of(long long u) const {
+    int c;
+    if (ctas <= set) {
+      c = static_cast<int>(static_cast<double>(u) * ctas / static_cast<double>(units));
+    } else {
+      const double x = static_cast<double>(u) * PARTS / static_cast<double>(units);
+      const int i = x >= ahead(3) ? 3 : x >= ahead(2) ? 2 : x >= ahead(1) ? 1 : 0;
+      c = i * set + static_cast<int>((x - ahead(i)) * set / (ahead(i + 1) - ahead(i)));
+    }
+    if (c >= ctas) c = ctas - 1;
+    while (c > 0 && begin(c) > u) --c;
+    while (c + 1 < ctas && begin(c + 1) <= u) ++c;
+    return c;
   }
 };
 
@@ -136,7 +145,7 @@ struct Cuts {
 
 // 16 bytes to shared memory, `bytes` of them from `from` and zeros behind.
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the last N groups of this thread's copies are there.
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   };
   auto place_of = [&](long long x) {
     Place at;
-    const int ahead = static_cast<int>(x / rows);
+    const int ahead = static_cast<int>(static_cast<double>(x) / rows);  // (exact: x < 2^40, rows < 2^17)
     int lo = 0, hi = p.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -226,7 +235,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
     at.b = lo;
     at.n = prefix[lo + 1] - prefix[lo];
     const long long rest = x - static_cast<long long>(prefix[lo]) * rows;
-    at.row = static_cast<int>(rest / at.n);
+    at.row = static_cast<int>(static_cast<double>(rest) / at.n);
     at.tile = static_cast<int>(rest - static_cast<long long>(at.row) * at.n);
     return at;
   };
@@ -529,63 +538,114 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   }
 }
 
-// Joins the partial results of a (request, head), a CTA each: its warps take them in turn, and their sums meet in the order of the
-// warps.  Requests that see no key get zeros and -inf here.
+// Joins the partial results of each (request, head), `items` of them per CTA: a warp takes one that has a few; those that have more
+// all warps share, and their sums meet in the order of the warps.  Requests that see no key get zeros and -inf here.
+constexpr int FEW = 16;
 template <int D, int COLS>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_decode_join_kernel(const Params p) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_decode_join_kernel(const Params p, int items) {
   __shared__ float4 sums[JOIN_WARPS][D / 4];
-  __shared__ float ls[JOIN_WARPS];
+  __shared__ float2 mls[JOIN_WARPS];
+  __shared__ int firsts[JOIN_WARPS], lasts[JOIN_WARPS];
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / p.heads, head = blockIdx.x - b * p.heads;
-  const int kvh = head / p.group, in = head - kvh * p.group, row = kvh * p.chunks + in / COLS, col = in % COLS;
-  const int ahead = p.prefix[b], n = p.prefix[b + 1] - ahead;
-  const int rows = p.kv_heads * p.chunks;
-  const long long units = static_cast<long long>(p.prefix[p.batch]) * rows;
   constexpr int LANES = D / 4;  // of a partial result; D = 64: a warp takes two at a time
   constexpr int PER = 32 / LANES;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, l = 0.f;
-  if (n > 0) {
-    const long long u0 = static_cast<long long>(ahead) * rows + static_cast<long long>(row) * n;
-    const Shares shares(units, p.set);
-    const int c0 = shares.of(u0), c1 = shares.of(u0 + n - 1);
-    if (c0 == c1) return;  // one CTA had all of it
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(2LL * c + (c == c0)) * COLS + col].x);
+  const long long item0 = static_cast<long long>(blockIdx.x) * items, all = static_cast<long long>(p.batch) * p.heads;
+  auto column = [&](int head) { return (head % p.group) % COLS; };
+  float4 sum;
+  float top, l;
+  // Partial results c = from, from + step, .. <= last of a line whose first is `first`, into top, l and sum.
+  auto take = [&](int first, int last, int from, int step, int col) {
+    top = -INFINITY, l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = from + lane / LANES; c - lane / LANES <= last; c += 4 * step) {
+      float2 ml[4];
+      float4 x[4];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-#pragma unroll 8
-    for (int c = c0 + warp * PER + lane / LANES; c <= c1; c += JOIN_WARPS * PER) {
-      const long long slot = (2LL * c + (c == c0)) * COLS + col;
-      const float2 ml = p.part_ml[slot];
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane % LANES * 4);
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);  // (1: NaN, which stays)
-      l += f * ml.y;
-      sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
+      for (int k = 0; k < 4; ++k) {
+        const int at = c + k * step;
+        const long long slot = (2LL * at + (at == first)) * COLS + col;
+        ml[k] = at <= last ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+        x[k] = at <= last ? *reinterpret_cast<const float4*>(p.part_o + slot * D + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top);
+      const float old = top == -INFINITY ? 1.f : ex2(top - now);  // (1: zeros so far, or NaN, which stays)
+      top = now;
+      l *= old, sum.x *= old, sum.y *= old, sum.z *= old, sum.w *= old;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : ex2(ml[k].x - now);
+        l += f * ml[k].y;
+        sum.x += f * x[k].x, sum.y += f * x[k].y, sum.z += f * x[k].z, sum.w += f * x[k].w;
+      }
     }
-    if (PER == 2) {
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16), sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
-      sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16), sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
+    if (PER == 2) {  // the halves' sums
+      const float other = __shfl_xor_sync(0xffffffffu, top, 16), now = fmaxf(top, other);
+      const float f = top == -INFINITY ? 1.f : ex2(top - now), g = other == -INFINITY ? 1.f : ex2(other - now);
+      const bool low = lane < 16;  // (in the same order in both)
+      auto both = [&](float v) {
+        const float o = __shfl_xor_sync(0xffffffffu, v, 16);
+        return low ? f * v + g * o : g * o + f * v;
+      };
+      l = both(l), sum.x = both(sum.x), sum.y = both(sum.y), sum.z = both(sum.z), sum.w = both(sum.w);
+      top = now;
     }
+  };
+  auto write = [&](int b, int head) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (lane < LANES)
+      *reinterpret_cast<uint2*>(p.out + b * p.out_sb + head * p.out_sh + lane * 4) =
+          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    if (p.lse != nullptr && lane == 0)
+      p.lse[static_cast<long long>(b) * p.heads + head] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+  };
+  if (warp < items) {
+    const long long item = item0 + warp;
+    int first = 0, last = 0;
+    if (item < all) {
+      const int b = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(b) * p.heads);
+      const int ahead = p.prefix[b], n = p.prefix[b + 1] - ahead;
+      if (n > 0) {
+        const int rows = p.kv_heads * p.chunks, row = head / p.group * p.chunks + head % p.group / COLS;
+        const Shares shares(static_cast<long long>(p.prefix[p.batch]) * rows, p.set);
+        const long long u0 = static_cast<long long>(ahead) * rows + static_cast<long long>(row) * n;
+        first = shares.of(u0);
+        last = first + 1 >= shares.ctas || shares.begin(first + 1) >= u0 + n ? first : shares.of(u0 + n - 1);
+        if (first < last && last - first < FEW) {  // (first == last: one CTA had all of it)
+          take(first, last, first, PER, column(head));
+          write(b, head);
+          last = first;
+        }
+      } else {
+        top = -INFINITY, l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        write(b, head);
+      }
+    }
+    if (lane == 0) firsts[warp] = first, lasts[warp] = last;
   }
-  if (lane < LANES) sums[warp][lane] = sum;
-  if (lane == 0) ls[warp] = l;
   __syncthreads();
-  if (tid >= LANES) return;
-  l = 0.f;
-  sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < JOIN_WARPS; ++w) {
-    const float4 x = sums[w][tid];
-    l += ls[w];
-    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  for (int i = 0; i < items; ++i) {
+    const int first = firsts[i], last = lasts[i];
+    if (first == last) continue;
+    const int b = static_cast<int>((item0 + i) / p.heads), head = static_cast<int>(item0 + i - static_cast<long long>(b) * p.heads);
+    take(first, last, first + warp * PER, JOIN_WARPS * PER, column(head));
+    if (lane < LANES) sums[warp][lane] = sum;
+    if (lane == 0) mls[warp] = make_float2(top, l);
+    __syncthreads();
+    if (warp == 0) {
+      top = -INFINITY;
+      for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, mls[w].x);
+      l = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        const float f = mls[w].x == -INFINITY ? 1.f : ex2(mls[w].x - top);
+        const float4 x = sums[w][lane % LANES];
+        l += f * mls[w].y;
+        sum.x += f * x.x, sum.y += f * x.y, sum.z += f * x.z, sum.w += f * x.w;
+      }
+      write(b, head);
+    }
+    __syncthreads();
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + b * p.out_sb + head * p.out_sh + tid * 4) =
-      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
-  if (p.lse != nullptr && tid == 0) p.lse[blockIdx.x] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 }  // namespace decode
 
@@ -707,13 +767,15 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
   void (*kernel)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1> : decode::attn_decode_kernel<128, 2>)
                                             : (nt == 1 ? decode::attn_decode_kernel<64, 1> : decode::attn_decode_kernel<64, 2>);
-  void (*join)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
+  void (*join)(decode::Params, int) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
   const size_t smem = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>()) +
                       (B + 1) * sizeof(int);
   CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
-  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>(B * H)), dim3(decode::JOIN_WARPS * 32), 0, stream, p));
+  // items of a CTA: one while there are few, up to one per warp
+  const int items = static_cast<int>(std::max<long long>(1, std::min<long long>(decode::JOIN_WARPS, B * H / (2 * sm_count()))));
+  CDL_CUDA(launch_pdl(join, dim3(static_cast<unsigned>((B * H + items - 1) / items)), dim3(decode::JOIN_WARPS * 32), 0, stream, p, items));
   return CDL_OK;
 }
 
