@@ -2,7 +2,6 @@
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 import struct
 from pathlib import Path
@@ -283,7 +282,7 @@ def tensor_bytes(t):
     1.2 as a ctypes structure with a byref() (field by field 2.7)."""
     if t is None:
         return None
-    dt = _dtype_codes().get(t.dtype)
+    dt = (_codes or _dtype_codes()).get(t.dtype)
     if dt is None:
         raise CdlError(-1, f"unsupported element type {t.dtype}: f32 or bf16 expected")
     shape = t.shape
@@ -292,6 +291,8 @@ def tensor_bytes(t):
         return _pack_tensor(t.data_ptr(), dt, 2, *shape, 0, 0, *t.stride(), 0, 0)
     if rank > 4:
         raise CdlError(-1, f"rank {rank} exceeds 4")
+    if rank == 1:
+        return _pack_tensor(t.data_ptr(), dt, 1, shape[0], 0, 0, 0, t.stride(0), 0, 0, 0)
     rest = _UNUSED[rank]
     return _pack_tensor(t.data_ptr(), dt, rank, *shape, *rest, *t.stride(), *rest)
 
@@ -299,6 +300,16 @@ def tensor_bytes(t):
 def rows_bytes(ptr: int, n: int) -> bytes:
     """The bytes of a cdl_tensor for n packed f32 values."""
     return _pack_tensor(ptr, CDL_F32, 1, n, 0, 0, 0, 1, 0, 0, 0)
+
+
+def vector_bytes(ptr: int, dtype: int, n: int) -> bytes:
+    """The bytes of a cdl_tensor for n packed values of a CDL_* type."""
+    return _pack_tensor(ptr, dtype, 1, n, 0, 0, 0, 1, 0, 0, 0)
+
+
+def matrix_bytes(ptr: int, dtype: int, rows: int, cols: int) -> bytes:
+    """The same for packed rows."""
+    return _pack_tensor(ptr, dtype, 2, rows, cols, 0, 0, cols, 1, 0, 0)
 
 
 _HEAD_LOSS_BYTES = struct.Struct("ffiq")  # the layout of cdl_head_loss_desc
@@ -319,11 +330,14 @@ def tensor_arg(t):
     return None if t is None else CdlTensor.from_buffer_copy(tensor_bytes(t))
 
 
-@functools.cache
+_codes = {}
+
+
 def _dtype_codes():
     import torch
 
-    return {torch.bfloat16: CDL_BF16, torch.float32: CDL_F32, torch.int32: CDL_I32}
+    _codes.update({torch.bfloat16: CDL_BF16, torch.float32: CDL_F32, torch.int32: CDL_I32})
+    return _codes
 
 
 def ref(ct):

@@ -771,7 +771,7 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
   const size_t smem = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>()) +
                       (B + 1) * sizeof(int);
-  CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
   // items of a CTA: one while there are few, up to one per warp
   const int items = static_cast<int>(std::max<long long>(1, std::min<long long>(decode::JOIN_WARPS, B * H / (2 * sm_count()))));

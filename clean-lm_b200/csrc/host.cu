@@ -56,6 +56,26 @@ int sm_count() {
   return counts[dev];
 }
 
+cudaError_t allow_shared_memory(const void* kernel, int bytes) {
+  // (the attribute is per kernel and device, and the call takes 0.5 us)
+  constexpr int SLOTS = 64;
+  static std::mutex mu;
+  static struct {
+    const void* kernel;
+    int dev, bytes;
+  } known[SLOTS];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  int i = 0;
+  while (i < SLOTS && known[i].kernel != nullptr && (known[i].kernel != kernel || known[i].dev != dev)) ++i;
+  if (i < SLOTS && known[i].kernel != nullptr && known[i].bytes >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && i < SLOTS) known[i].kernel = kernel, known[i].dev = dev, known[i].bytes = bytes;
+  return e;
+}
+
 // Work counters of the kernels that hand out their work at run time (the CTA-pair GEMM's units,
 // kind 0; the persistent attention forward's items, kind 1; the persistent attention backward
 // kernels' items, kinds 2 and 3; GEMMs that start early, kinds 4 to 7): one per kind, device and stream, zero

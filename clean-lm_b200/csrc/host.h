@@ -95,6 +95,9 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device (asked of the runtime where it is more than before).
+cudaError_t allow_shared_memory(const void* kernel, int bytes);
+
 // Device counter for a kernel that hands out its work at run time (see host.cu); nullptr: none.
 unsigned int* sched_counter_for(int kind, int dev, cudaStream_t stream);
 // While it lives, the calling thread's launches get no counter if `stream` is being captured: graphs captured on one stream may

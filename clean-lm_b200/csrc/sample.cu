@@ -979,7 +979,7 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, 3 * sm_count() / 2 / R, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));
-  CDL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), smem));
   const dim3 grid(static_cast<unsigned>(R * p.cluster));
   CDL_CUDA(p.cluster == 1 ? launch_pdl(kernel, grid, dim3(sample::THREADS), smem, stream, p)
                           : launch_pdl_cluster(kernel, grid, dim3(sample::THREADS), smem, p.cluster, stream, p));

@@ -25,7 +25,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from ._lib import check, current_stream, packed_lib, tensor_bytes
+from ._lib import CDL_F32, CDL_I32, check, current_stream, matrix_bytes, packed_lib, tensor_bytes, vector_bytes
 from .ops import _require_current_device
 
 
@@ -53,18 +53,23 @@ def cache_plan(cached, added, block_table, free_pages, free_count, opts: CachePl
     [requests, pages of a request], written in place).  A request that does not get its pages, or whose table row or rows of
     the batch do not suffice, is not served: its tokens have slot -1 and its seq_lens stays at `cached`."""
     _require_current_device(cached, added, block_table, free_pages, free_count)
-    if opts.rows < 0:
+    rows = opts.rows
+    if rows < 0:
         raise _lib.CdlError(-1, "cache_plan: rows must not be negative")
-    requests = cached.shape[0] if cached.dim() == 1 else -1
-    if requests < 0:
+    if cached.dim() != 1:
         raise _lib.CdlError(-1, "cache_plan: cached must be a vector")
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=cached.device)
-    plan = CachePlan(new(requests), new(requests + 1), new(opts.rows), new(opts.rows), new(1))
+    n = cached.shape[0]
+    # one allocation, of which each output is a part: five take 3 us more
+    sizes = (n, n + 1, rows, rows, 1)
+    block = torch.empty(2 * n + 2 * rows + 2, dtype=torch.int32, device=cached.device)
+    at, outputs = block.data_ptr(), []
+    for size in sizes:
+        outputs.append(vector_bytes(at, CDL_I32, size))
+        at += 4 * size
     check(packed_lib.cdl_b200_cache_plan(
-        opts.page_size, opts.pages, *map(tensor_bytes, (cached, added, block_table, free_pages, free_count, plan.seq_lens,
-                                                        plan.cu_seqlens, plan.positions, plan.slots, plan.free_left)),
-        current_stream()))
-    return plan
+        opts.page_size, opts.pages, tensor_bytes(cached), tensor_bytes(added), tensor_bytes(block_table),
+        tensor_bytes(free_pages), tensor_bytes(free_count), *outputs, current_stream()))
+    return CachePlan(*block.split(sizes))
 
 
 # --------------------------------------------------------------------------- the way into the cache
@@ -101,6 +106,7 @@ class AttentionDecodeOutputs:
 
 
 def attention_decode_scratch_bytes(q, k_cache) -> int:
+    """The scratch that the call below needs for these operands."""
     n = ctypes.c_size_t(0)
     check(packed_lib.cdl_b200_attn_decode_scratch_bytes(tensor_bytes(q), tensor_bytes(k_cache), ctypes.byref(n)))
     return n.value
@@ -118,10 +124,14 @@ def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: Attention
         scratch = torch.empty(n.value, dtype=torch.uint8, device=q.device)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse_t = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if lse else None
+    lse_t = tl = None
+    if lse:
+        batch, heads = q.shape[0], q.shape[1]
+        lse_t = torch.empty(batch, heads, dtype=torch.float32, device=q.device)
+        tl = matrix_bytes(lse_t.data_ptr(), CDL_F32, batch, heads)
     check(packed_lib.cdl_b200_attn_decode(
         _lib.attn_decode_bytes(opts.softmax_scale or 0.0, opts.softcap, opts.window), tq, tk, tensor_bytes(v_cache),
-        tensor_bytes(block_table), tensor_bytes(seq_lens), tensor_bytes(out), tensor_bytes(lse_t), scratch.data_ptr(),
+        tensor_bytes(block_table), tensor_bytes(seq_lens), tensor_bytes(out), tl, scratch.data_ptr(),
         scratch.numel() * scratch.element_size(), current_stream()))
     return AttentionDecodeOutputs(out, lse_t)
 
@@ -148,13 +158,19 @@ def sample(logits, uniform, opts: SampleOpts | None = None, logprob: bool = True
     opts = opts or SampleOpts()
     if logits.dim() != 2:
         raise _lib.CdlError(-1, "sample: logits must be [rows, vocab]")
-    given = [opts.temperature, opts.top_k, opts.top_p, opts.min_p]
-    per_row = [x if isinstance(x, torch.Tensor) else None for x in given]
-    _require_current_device(logits, uniform, *per_row)
+    all_rows, per_row = [0.0, 0, 1.0, 0.0], [None] * 4
+    _require_current_device(logits, uniform)
+    for i, x in enumerate((opts.temperature, opts.top_k, opts.top_p, opts.min_p)):
+        if isinstance(x, torch.Tensor):
+            _require_current_device(x)
+            per_row[i] = tensor_bytes(x)
+        else:
+            all_rows[i] = x
     rows, device = logits.shape[0], logits.device
-    token = torch.empty(rows, dtype=torch.int32, device=device)
-    lp = torch.empty(rows, dtype=torch.float32, device=device) if logprob else None
-    check(packed_lib.cdl_b200_sample(
-        _lib.sample_bytes(*(0 if t is not None else x for t, x in zip(per_row, given))),
-        *map(tensor_bytes, (logits, uniform, *per_row, token, lp)), current_stream()))
+    token, lp, tl = torch.empty(rows, dtype=torch.int32, device=device), None, None
+    if logprob:
+        lp = torch.empty(rows, dtype=torch.float32, device=device)
+        tl = vector_bytes(lp.data_ptr(), CDL_F32, rows)
+    check(packed_lib.cdl_b200_sample(_lib.sample_bytes(*all_rows), tensor_bytes(logits), tensor_bytes(uniform), *per_row,
+                                     vector_bytes(token.data_ptr(), CDL_I32, rows), tl, current_stream()))
     return SampleOutputs(token, lp)
