@@ -485,7 +485,7 @@ int32_t cdl_b200_cache_plan(int32_t page_size, int32_t pages, const cdl_tensor* 
 /* New keys and values into their slots, after the rotary embedding of q and k (as cdl_b200_rope does it, crates/sky-1/src/
  * training/model/decoder.rs:363-378): q_out = RoPE(q), k_out = RoPE(k), k_cache[slots[i]] = RoPE(k[i]), v_cache[slots[i]] = v[i].
  * q, q_out bf16 [tokens, heads, head_dim], k, v, k_out [tokens, kv_heads, head_dim] (views of one fused tensor, say): last
- * dimension contiguous, other strides and base 16-byte aligned, head_dim a multiple of 16.  q_out may be q itself, k_out k;
+ * dimension contiguous, other strides and base 16-byte aligned, head_dim a multiple of 16 up to 2048.  q_out may be q itself, k_out k;
  * otherwise outputs overlap neither inputs nor one another.  q with q_out, k_out, and cos_sin with positions are nullable (no
  * rotation then, and neither q nor k_out).  cos_sin packed f32 [table rows, head_dim] as for cdl_b200_rope; positions, slots packed
  * i32 [tokens].  A token whose position is outside the table is not rotated; one whose slot is outside the cache is not
