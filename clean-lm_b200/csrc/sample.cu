@@ -102,19 +102,31 @@ struct Row {
       return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
     }
   }
-  // f(vector, index of its first value) for the vectors v0, v0 + step, .. below v1, with D loads ahead.
+  // f(vector, index of its first value) for the vectors v0, v0 + step, .. below v1: for little work, D loads and then D times f.
   template <int D, typename F>
   __device__ __forceinline__ void each(int v0, int v1, int step, F f) const {
-    uint4 q[D];
+#pragma unroll 1
+    for (int v = v0; v < v1; v += D * step) {
+      uint4 q[D];
 #pragma unroll
-    for (int i = 0; i < D; ++i)
-      if (v0 + i * step < v1) q[i] = load(v0 + i * step);
+      for (int i = 0; i < D; ++i)
+        if (i == 0 || v + i * step < v1) q[i] = load(v + i * step);
+#pragma unroll
+      for (int i = 0; i < D; ++i)
+        if (i == 0 || v + i * step < v1) f(q[i], first(v + i * step));
+    }
+  }
+  // The same for more work, with the next two loads under way.
+  template <typename F>
+  __device__ __forceinline__ void one_by_one(int v0, int v1, int step, F f) const {
+    if (v0 >= v1) return;
+    uint4 next = load(v0), after = next;
+    if (v0 + step < v1) after = load(v0 + step);
 #pragma unroll 1
     for (int v = v0; v < v1; v += step) {
-      const uint4 now = q[0];
-#pragma unroll
-      for (int i = 0; i + 1 < D; ++i) q[i] = q[i + 1];
-      if (v + D * step < v1) q[D - 1] = load(v + D * step);
+      const uint4 now = next;
+      next = after;
+      if (v + 2 * step < v1) after = load(v + 2 * step);
       f(now, first(v));
     }
   }
@@ -165,48 +177,106 @@ __device__ __forceinline__ u64 least_of(float top_p, u64 mass) {
   return q < 1 ? 1 : q;
 }
 
-// 2^(j/32), rounded to f64.
-__device__ const double POW2[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
-    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
-    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
-    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
-    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+// 2^(j/256), rounded to f64.
+__device__ const double POW2[256] = {
+    0x1.0000000000000p+0, 0x1.00b1afa5abcbfp+0, 0x1.0163da9fb3335p+0, 0x1.02168143b0281p+0,
+    0x1.02c9a3e778061p+0, 0x1.037d42e11bbccp+0, 0x1.04315e86e7f85p+0, 0x1.04e5f72f654b1p+0,
+    0x1.059b0d3158574p+0, 0x1.0650a0e3c1f89p+0, 0x1.0706b29ddf6dep+0, 0x1.07bd42b72a836p+0,
+    0x1.0874518759bc8p+0, 0x1.092bdf66607e0p+0, 0x1.09e3ecac6f383p+0, 0x1.0a9c79b1f3919p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0c0f145e46c85p+0, 0x1.0cc922b7247f7p+0, 0x1.0d83b23395decp+0,
+    0x1.0e3ec32d3d1a2p+0, 0x1.0efa55fdfa9c5p+0, 0x1.0fb66affed31bp+0, 0x1.1073028d7233ep+0,
+    0x1.11301d0125b51p+0, 0x1.11edbab5e2ab6p+0, 0x1.12abdc06c31ccp+0, 0x1.136a814f204abp+0,
+    0x1.1429aaea92de0p+0, 0x1.14e95934f312ep+0, 0x1.15a98c8a58e51p+0, 0x1.166a45471c3c2p+0,
+    0x1.172b83c7d517bp+0, 0x1.17ed48695bbc0p+0, 0x1.18af9388c8deap+0, 0x1.1972658375d2fp+0,
+    0x1.1a35beb6fcb75p+0, 0x1.1af99f8138a1cp+0, 0x1.1bbe084045cd4p+0, 0x1.1c82f95281c6bp+0,
+    0x1.1d4873168b9aap+0, 0x1.1e0e75eb44027p+0, 0x1.1ed5022fcd91dp+0, 0x1.1f9c18438ce4dp+0,
+    0x1.2063b88628cd6p+0, 0x1.212be3578a819p+0, 0x1.21f49917ddc96p+0, 0x1.22bdda27912d1p+0,
+    0x1.2387a6e756238p+0, 0x1.2451ffb82140ap+0, 0x1.251ce4fb2a63fp+0, 0x1.25e85711ece75p+0,
+    0x1.26b4565e27cddp+0, 0x1.2780e341ddf29p+0, 0x1.284dfe1f56381p+0, 0x1.291ba7591bb70p+0,
+    0x1.29e9df51fdee1p+0, 0x1.2ab8a66d10f13p+0, 0x1.2b87fd0dad990p+0, 0x1.2c57e39771b2fp+0,
+    0x1.2d285a6e4030bp+0, 0x1.2df961f641589p+0, 0x1.2ecafa93e2f56p+0, 0x1.2f9d24abd886bp+0,
+    0x1.306fe0a31b715p+0, 0x1.31432edeeb2fdp+0, 0x1.32170fc4cd831p+0, 0x1.32eb83ba8ea32p+0,
+    0x1.33c08b26416ffp+0, 0x1.3496266e3fa2dp+0, 0x1.356c55f929ff1p+0, 0x1.36431a2de883bp+0,
+    0x1.371a7373aa9cbp+0, 0x1.37f26231e754ap+0, 0x1.38cae6d05d866p+0, 0x1.39a401b7140efp+0,
+    0x1.3a7db34e59ff7p+0, 0x1.3b57fbfec6cf4p+0, 0x1.3c32dc313a8e5p+0, 0x1.3d0e544ede173p+0,
+    0x1.3dea64c123422p+0, 0x1.3ec70df1c5175p+0, 0x1.3fa4504ac801cp+0, 0x1.40822c367a024p+0,
+    0x1.4160a21f72e2ap+0, 0x1.423fb2709468ap+0, 0x1.431f5d950a897p+0, 0x1.43ffa3f84b9d4p+0,
+    0x1.44e086061892dp+0, 0x1.45c2042a7d232p+0, 0x1.46a41ed1d0057p+0, 0x1.4786d668b3237p+0,
+    0x1.486a2b5c13cd0p+0, 0x1.494e1e192aed2p+0, 0x1.4a32af0d7d3dep+0, 0x1.4b17dea6db7d7p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4ce41b817c114p+0, 0x1.4dcb299fddd0dp+0, 0x1.4eb2d81d8abffp+0,
+    0x1.4f9b2769d2ca7p+0, 0x1.508417f4531eep+0, 0x1.516daa2cf6642p+0, 0x1.5257de83f4eefp+0,
+    0x1.5342b569d4f82p+0, 0x1.542e2f4f6ad27p+0, 0x1.551a4ca5d920fp+0, 0x1.56070dde910d2p+0,
+    0x1.56f4736b527dap+0, 0x1.57e27dbe2c4cfp+0, 0x1.58d12d497c7fdp+0, 0x1.59c0827ff07ccp+0,
+    0x1.5ab07dd485429p+0, 0x1.5ba11fba87a03p+0, 0x1.5c9268a5946b7p+0, 0x1.5d84590998b93p+0,
+    0x1.5e76f15ad2148p+0, 0x1.5f6a320dceb71p+0, 0x1.605e1b976dc09p+0, 0x1.6152ae6cdf6f4p+0,
+    0x1.6247eb03a5585p+0, 0x1.633dd1d1929fdp+0, 0x1.6434634ccc320p+0, 0x1.652b9febc8fb7p+0,
+    0x1.6623882552225p+0, 0x1.671c1c70833f6p+0, 0x1.68155d44ca973p+0, 0x1.690f4b19e9538p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6b052fa75173ep+0, 0x1.6c012750bdabfp+0, 0x1.6cfdcddd47645p+0,
+    0x1.6dfb23c651a2fp+0, 0x1.6ef9298593ae5p+0, 0x1.6ff7df9519484p+0, 0x1.70f7466f42e87p+0,
+    0x1.71f75e8ec5f74p+0, 0x1.72f8286ead08ap+0, 0x1.73f9a48a58174p+0, 0x1.74fbd35d7cbfdp+0,
+    0x1.75feb564267c9p+0, 0x1.77024b1ab6e09p+0, 0x1.780694fde5d3fp+0, 0x1.790b938ac1cf6p+0,
+    0x1.7a11473eb0187p+0, 0x1.7b17b0976cfdbp+0, 0x1.7c1ed0130c132p+0, 0x1.7d26a62ff86f0p+0,
+    0x1.7e2f336cf4e62p+0, 0x1.7f3878491c491p+0, 0x1.80427543e1a12p+0, 0x1.814d2add106d9p+0,
+    0x1.82589994cce13p+0, 0x1.8364c1eb941f7p+0, 0x1.8471a4623c7adp+0, 0x1.857f4179f5b21p+0,
+    0x1.868d99b4492edp+0, 0x1.879cad931a436p+0, 0x1.88ac7d98a6699p+0, 0x1.89bd0a478580fp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8be05bad61778p+0, 0x1.8cf3216b5448cp+0, 0x1.8e06a5e0866d9p+0,
+    0x1.8f1ae99157736p+0, 0x1.902fed0282c8ap+0, 0x1.9145b0b91ffc6p+0, 0x1.925c353aa2fe2p+0,
+    0x1.93737b0cdc5e5p+0, 0x1.948b82b5f98e5p+0, 0x1.95a44cbc8520fp+0, 0x1.96bdd9a7670b3p+0,
+    0x1.97d829fde4e50p+0, 0x1.98f33e47a22a2p+0, 0x1.9a0f170ca07bap+0, 0x1.9b2bb4d53fe0dp+0,
+    0x1.9c49182a3f090p+0, 0x1.9d674194bb8d5p+0, 0x1.9e86319e32323p+0, 0x1.9fa5e8d07f29ep+0,
+    0x1.a0c667b5de565p+0, 0x1.a1e7aed8eb8bbp+0, 0x1.a309bec4a2d33p+0, 0x1.a42c980460ad8p+0,
+    0x1.a5503b23e255dp+0, 0x1.a674a8af46052p+0, 0x1.a799e1330b358p+0, 0x1.a8bfe53c12e59p+0,
+    0x1.a9e6b5579fdbfp+0, 0x1.ab0e521356ebap+0, 0x1.ac36bbfd3f37ap+0, 0x1.ad5ff3a3c2774p+0,
+    0x1.ae89f995ad3adp+0, 0x1.afb4ce622f2ffp+0, 0x1.b0e07298db666p+0, 0x1.b20ce6c9a8952p+0,
+    0x1.b33a2b84f15fbp+0, 0x1.b468415b749b1p+0, 0x1.b59728de5593ap+0, 0x1.b6c6e29f1c52ap+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.b928cf22749e4p+0, 0x1.ba5b030a1064ap+0, 0x1.bb8e0b79a6f1fp+0,
+    0x1.bcc1e904bc1d2p+0, 0x1.bdf69c3f3a207p+0, 0x1.bf2c25bd71e09p+0, 0x1.c06286141b33dp+0,
+    0x1.c199bdd85529cp+0, 0x1.c2d1cd9fa652cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c544778fafb22p+0,
+    0x1.c67f12e57d14bp+0, 0x1.c7ba88988c933p+0, 0x1.c8f6d9406e7b5p+0, 0x1.ca3405751c4dbp+0,
+    0x1.cb720dcef9069p+0, 0x1.ccb0f2e6d1675p+0, 0x1.cdf0b555dc3fap+0, 0x1.cf3155b5bab74p+0,
+    0x1.d072d4a07897cp+0, 0x1.d1b532b08c968p+0, 0x1.d2f87080d89f2p+0, 0x1.d43c8eacaa1d6p+0,
+    0x1.d5818dcfba487p+0, 0x1.d6c76e862e6d3p+0, 0x1.d80e316c98398p+0, 0x1.d955d71ff6075p+0,
+    0x1.da9e603db3285p+0, 0x1.dbe7cd63a8315p+0, 0x1.dd321f301b460p+0, 0x1.de7d5641c0658p+0,
+    0x1.dfc97337b9b5fp+0, 0x1.e11676b197d17p+0, 0x1.e264614f5a129p+0, 0x1.e3b333b16ee12p+0,
+    0x1.e502ee78b3ff6p+0, 0x1.e653924676d76p+0, 0x1.e7a51fbc74c83p+0, 0x1.e8f7977cdb740p+0,
+    0x1.ea4afa2a490dap+0, 0x1.eb9f4867cca6ep+0, 0x1.ecf482d8e67f1p+0, 0x1.ee4aaa2188510p+0,
+    0x1.efa1bee615a27p+0, 0x1.f0f9c1cb6412ap+0, 0x1.f252b376bba97p+0, 0x1.f3ac948dd7274p+0,
+    0x1.f50765b6e4540p+0, 0x1.f6632798844f8p+0, 0x1.f7bfdad9cbe14p+0, 0x1.f91d802243c89p+0,
+    0x1.fa7c1819e90d8p+0, 0x1.fbdba3692d514p+0, 0x1.fd3c22b8f71f1p+0, 0x1.fe9d96b2a23d9p+0};
 
-// w = exp((z - top) / T) in units of 2^-S: 2^((k + r) / 32) with (z - top) 32 log2(e) / T = k + r, |r| <= 1/2, from a table of
-// 2^(S + j/32) and the Taylor series up to r^5, whose rest is 2e-15 (the table-driven method of P. T. P. Tang, 1989).  S <= 50: the
-// addition of 2^52 rounds to whole units.  The last two coefficients have 20 bits, which is what they matter with (1e-15), so that
-// they fit into an instruction; the others are members so that they stay in registers.
+// w = exp((z - top) / T) in units of 2^-S: 2^((k + r) / 256) with (z - top) 256 log2(e) / T = k + r, |r| <= 1/2, from a table of
+// 2^(S + j/256) and the Taylor series up to r^4, whose rest is 4e-17 (the table-driven method of P. T. P. Tang, 1989).  S <= 50: the
+// addition of 1.5 2^52 rounds to whole units.  Constants are members so that they stay in registers: as literals they took two
+// moves each, and the pass over a row is bound by the number of its instructions.
 struct Weight {
-  double top, per_t;  // 32 log2(e) / T
-  double c1, c2, c3;  // (ln 2 / 32)^i / i!
-  float least;        // 80 T ln 2 below the top, where w is less than half a unit
-  uint32_t pow2;      // the table in shared memory
+  double top, per_t;          // 256 log2(e) / T
+  double c1, c2, c3, c4;      // (ln 2 / 256)^i / i!
+  double magic;               // 1.5 2^52
+  float least;                // 80 T ln 2 below the top, where w is less than half a unit
+  uint32_t pow2;              // the table in shared memory
   // (without meaning for z <= least)
   __device__ __forceinline__ u64 above_least(float z) const {
-    constexpr double C4 = 0x1.3b2ab00000000p-27, C5 = 0x1.5d88000000000p-35, MAGIC = 6755399441055744.0;  // 1.5 2^52
     const double d = static_cast<double>(z) - top;
-    const double k = fma(d, per_t, MAGIC);
+    const double k = fma(d, per_t, magic);
     const int n = __double2loint(k);
-    const double r = fma(d, per_t, MAGIC - k);
-    double y = fma(r, C5, C4);
-    y = fma(r, y, c3);
+    const double r = fma(d, per_t, magic - k);
+    double y = fma(r, c4, c3);
     y = fma(r, y, c2);
     y = fma(r, y, c1) * r;
     double tab;
-    asm("ld.shared.f64 %0, [%1];" : "=d"(tab) : "r"(pow2 + (n & 31) * 8));
+    asm("ld.shared.f64 %0, [%1];" : "=d"(tab) : "r"(pow2 + (n & 255) * 8));
     y = fma(tab, y, tab);
-    y = __hiloint2double(__double2hiint(y) + ((n << 15) & static_cast<int>(0xFFF00000u)), __double2loint(y)) + 4503599627370496.0;
-    return static_cast<u64>(__double_as_longlong(y)) & 0xFFFFFFFFFFFFFull;
+    y = __hiloint2double(__double2hiint(y) + ((n << 12) & static_cast<int>(0xFFF00000u)), __double2loint(y)) + magic;
+    return static_cast<u64>(__double_as_longlong(y)) & 0x7FFFFFFFFFFFFull;
   }
   __device__ __forceinline__ u64 operator()(float z) const {
     const u64 w = above_least(z);
     return z > least ? w : 0;
   }
 };
+__device__ __forceinline__ void add_if_from(u64& sum, u64 y, float x, float from) {  // sum += y where x >= from
+  asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %2, %3;\n\t@p add.u64 %0, %0, %1;\n\t}" : "+l"(sum) : "l"(y), "f"(x), "f"(from));
+}
 
 struct Shared {
   u64 list[CAP], weight_of[CAP];
@@ -217,7 +287,7 @@ struct Shared {
     u64 wide_hist[256];
   };
   u64 tile[TILES];  // a CTA's tiles at their number in the row
-  double pow2[32];
+  double pow2[256];
   u64 sums[WARPS];
   float tops[WARPS];
   uint32_t rank_of[256];
@@ -246,20 +316,21 @@ struct Sums {
 __device__ __noinline__ Sums block_scan(u64 x, u64* sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 y = x;
-#pragma unroll 1
+#pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const u64 o = __shfl_up_sync(0xffffffffu, y, d);
     if (lane >= d) y += o;
   }
   if (lane == 31) sums[warp] = y;
   __syncthreads();
-  Sums r{y - x, 0};
-#pragma unroll 2
-  for (int w = 0; w < WARPS; ++w) {
-    const u64 v = sums[w];
-    if (w < warp) r.before += v;
-    r.all += v;
+  u64 z = sums[lane & (WARPS - 1)];
+#pragma unroll
+  for (int d = 1; d < WARPS; d <<= 1) {
+    const u64 o = __shfl_up_sync(0xffffffffu, z, d);
+    if ((lane & (WARPS - 1)) >= d) z += o;
   }
+  const u64 ahead = __shfl_sync(0xffffffffu, z, warp > 0 ? warp - 1 : 0);
+  Sums r{y - x + (warp > 0 ? ahead : 0), __shfl_sync(0xffffffffu, z, WARPS - 1)};
   __syncthreads();
   return r;
 }
@@ -525,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     else __syncthreads();
   };
   auto of = [&](int other) -> Shared& { return C > 1 ? *cluster.map_shared_rank(&sh, other) : sh; };
-  if (tid < 32) sh.pow2[tid] = __hiloint2double(__double2hiint(POW2[tid]) + (p.scale_bits << 20), __double2loint(POW2[tid]));
+  if (tid < 256) sh.pow2[tid] = __hiloint2double(__double2hiint(POW2[tid]) + (p.scale_bits << 20), __double2loint(POW2[tid]));
   if (tid == 0) sh.count = 0;
   const long long r = blockIdx.x / C;
   Row<T> row;
@@ -546,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
 
   // ---- the largest logit; NaN and +inf
   float mine = -INFINITY;
-  row.template each<6>(v0 + tid, v1, THREADS, [&](const uint4& q, int) { mine = max_nan(mine, Row<T>::top(q)); });
+  row.template each<8>(v0 + tid, v1, THREADS, [&](const uint4& q, int) { mine = max_nan(mine, Row<T>::top(q)); });
   const float temperature = p.temperature ? p.temperature[r] : p.all_temperature;
   const float min_p = p.min_p ? p.min_p[r] : p.all_min_p;
   Settings set;
@@ -591,10 +662,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     return;
   }
   set.t = static_cast<double>(temperature);
-  constexpr double L = 0.6931471805599453094 / 32;
-  const double per_t = 32 * 1.4426950408889634074 / set.t;
+  constexpr double L = 0.6931471805599453094 / 256;
+  const double per_t = 256 * 1.4426950408889634074 / set.t;
   if (tid == 0)
-    sh.weight = Weight{static_cast<double>(top), per_t, L, L * L / 2, L * L * L / 6,
+    sh.weight = Weight{static_cast<double>(top), per_t, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, 6755399441055744.0,
                        fminf(__double2float_rd(static_cast<double>(top) - 80 * 0.6931471805599453 * set.t), of_key(key_of(top) - 1)),
                        smem_u32(sh.pow2)};
   // w >= min_p: a bound on the logit, rounded up to the next one in f32
@@ -607,7 +678,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     if (at < CAP) sh.list[at] = packed(key, i);
   };
   Mode mode = ALL;
-  const float bin_scale = fminf(static_cast<float>(per_t) * (BIN_PER / 32), 1e30f);
+  const float bin_scale = fminf(static_cast<float>(per_t) * (BIN_PER / 256.f), 1e30f);
   // How far a logit lies below the largest; rounded by the addition of 1.5 2^23, infinite distances in the last bin.
   auto bin = [&](float x) { return min(BINS - 1, __float_as_int(fmaf(top - x, bin_scale, 12582912.f)) - 0x4B400000); };
   uint32_t bound = 0;                      // of the list's keys
@@ -633,7 +704,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
     __syncthreads();
     uint32_t far = 0;
-    row.template each<3>(v0 + tid, v1, THREADS, [&](const uint4& q, int i0) {
+    row.one_by_one(v0 + tid, v1, THREADS, [&](const uint4& q, int i0) {
       Row<T>::fours(q, i0, [&](const float (&x)[4], int) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -753,51 +824,63 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const Weight weight = sh.weight;
     const float from = fmaxf(over, of_key(key_of(weight.least) + 1));
     u64 rest = 0, above = 0;
-    // f(4 values, index of the first) of each vector that has one from `least` on, tile by tile
+    // f(4 values, index of the first) of each vector that has one from `least` on, tile by tile; the next load is under way
     auto tiles_of = [&](float least, auto f) {
+      const int per_lane = per_tile / 32;
+      int tile = t0 + warp, in = 0;
+      u64 sum = 0;
+      auto load = [&](int t, int k) {
+        const int v = t * per_tile + k * 32 + lane;
+        constexpr uint32_t NONE = N == 8 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+        return t < t1 && v < row.vectors ? row.load(v) : make_uint4(NONE, NONE, NONE, NONE);
+      };
+      uint4 next = load(tile, 0);
 #pragma unroll 1
-      for (int tile = t0 + warp; tile < t1; tile += WARPS) {
-        u64 sum = 0;
-        row.template each<2>(tile * per_tile + lane, min(row.vectors, (tile + 1) * per_tile), 32, [&](const uint4& q, int i0) {
-          if (Row<T>::top(q) < least) return;
-          Row<T>::fours(q, i0, [&](const float (&x)[4], int i) { f(x, i, sum); });
-        });
-        sum = warp_sum(sum);
-        if (lane == 0) sh.tile[tile] = sum;
-        above += sum;  // (the same in all lanes)
+      while (tile < t1) {
+        const uint4 now = next;
+        const int v = tile * per_tile + in * 32 + lane;
+        const bool ends = ++in == per_lane;
+        next = ends ? load(tile + WARPS, 0) : load(tile, in);
+        if (__any_sync(0xffffffffu, Row<T>::top(now) >= least))  // (by whole warps: lanes that part here would go on apart)
+          Row<T>::fours(now, row.first(v), [&](const float (&x)[4], int i) { f(x, i, sum); });
+        if (ends) {
+          sum = warp_sum(sum);
+          if (lane == 0) sh.tile[tile] = sum;
+          above += sum;  // (the same in all lanes)
+          sum = 0, in = 0, tile += WARPS;
+        }
       }
     };
     auto window = [&](const float (&x)[4], int i) {
       bool any = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) any |= x[e] >= low && !(x[e] >= over);
-      if (any)
+      for (int e = 0; e < 4; ++e) any |= (x[e] >= low) & !(x[e] >= over);
+      if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (x[e] >= low && !(x[e] >= over)) append(key_of(x[e]), i + e);
+          if ((x[e] >= low) & !(x[e] >= over)) append(key_of(x[e]), i + e);
+        __syncwarp();
+      }
     };
-    if (mode == WINDOW_P) {
-      tiles_of(weight.least, [&](const float (&x)[4], int i, u64& sum) {
+    if (mode == ALL) {
+      tiles_of(from, [&](const float (&x)[4], int, u64& sum) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const u64 y = weight.above_least(x[e]);
-          sum += x[e] >= from ? y : 0;
-          rest += x[e] > weight.least && !(x[e] >= from) ? y : 0;
-        }
-        window(x, i);
+        for (int e = 0; e < 4; ++e) add_if_from(sum, weight.above_least(x[e]), x[e], from);
       });
-      rest = block_scan(rest, sh.sums).all;
-      above = block_scan(lane == 0 ? above : 0, sh.sums).all;
-      if (tid == 0) sh.above = above, sh.all = above + rest;
     } else {
-      tiles_of(fminf(over, low), [&](const float (&x)[4], int i, u64& sum) {
+      const float any = of_key(key_of(weight.least) + 1), least = mode == WINDOW_P ? any : fminf(over, low);
+      tiles_of(least, [&](const float (&x)[4], int i, u64& sum) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const u64 y = weight.above_least(x[e]);
-          sum += x[e] >= from ? y : 0;
+          add_if_from(rest, y, x[e], any);
+          add_if_from(sum, y, x[e], from);
         }
         window(x, i);
       });
+      rest = block_scan(rest, sh.sums).all;  // (of the whole row, where mode is WINDOW_P)
+      above = block_scan(lane == 0 ? above : 0, sh.sums).all;
+      if (tid == 0) sh.above = above, sh.all = rest;
     }
   }
   meet();
