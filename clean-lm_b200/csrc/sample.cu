@@ -284,7 +284,6 @@ struct Shared {
     u64 other[CAP];
     uint32_t hist[BINS];
     uint32_t fine[3][THREADS];
-    u64 wide_hist[256];
   };
   u64 tile[TILES];  // a CTA's tiles at their number in the row
   double pow2[256];
@@ -295,7 +294,7 @@ struct Shared {
   // what the cluster's other CTAs read
   float top;
   int at;
-  uint32_t count;
+  uint32_t count, bound;
   u64 above, all;
   int mode, lo, hi;
   uint32_t before;
@@ -477,37 +476,42 @@ __device__ __forceinline__ void draw_small(const Params& p, Shared& sh, const Se
 }
 
 // The entry at which the sum over the entries from `cut` on, in falling order, reaches `want`: of their weights, or their number.
-// 8 bits of the logit at a time, then by index.  For windows that hold more than CAP entries: equal logits by the thousand,
-// logits far from any scale that the bins have.
+// A quarter of the range of logits at a time, then by index.  For windows that hold more than CAP entries: equal logits by the
+// thousand, logits far from any scale that the bins have, top_p of a top_k of thousands.
 template <typename T>
-__device__ __noinline__ u64 select(const Row<T>& row, Shared& sh, bool weights, u64 want, u64 cut) {
+__device__ __noinline__ u64 select(const Row<T>& row_in, Shared& sh, bool weights, u64 want, u64 cut) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Row<T> row = row_in;
   const Weight weight = sh.weight;
-  uint32_t prefix = 0;
-  u64 above = 0;
+  uint32_t lo = KEY_NONE + 1, hi = key_of(static_cast<float>(weight.top));  // the entry's key is among these
+  u64 above = 0;                                                            // sum of the keys above hi
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) sh.wide_hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < row.vocab; i += THREADS) {
-      const float x = row.at(i);
-      const uint32_t key = key_of(x);
-      if (key > KEY_NONE && packed(key, i) >= cut && (shift == 24 || (key >> (shift + 8)) == prefix))
-        atomicAdd(&sh.wide_hist[(key >> shift) & 255], weights ? weight(x) : 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      u64 sum = above;
-      int bin = 255;
-      while (bin > 0 && sum + sh.wide_hist[bin] < want) sum += sh.wide_hist[bin--];
-      sh.index = static_cast<int>((prefix << 8) | static_cast<uint32_t>(bin));
-      sh.word = sum;
-    }
-    __syncthreads();
-    prefix = static_cast<uint32_t>(sh.index);
-    above = sh.word;
-    __syncthreads();
+  while (lo < hi) {
+    const uint32_t part = (hi - lo) / 4 + 1;
+    const uint32_t p1 = lo + part, p2 = min(hi, p1 + part), p3 = min(hi, p2 + part);
+    u64 s1 = 0, s2 = 0, s3 = 0;  // from p1, p2, p3 on
+    row.template each<2>(tid, row.vectors, THREADS, [&](const uint4& q, int i0) {
+      Row<T>::fours(q, i0, [&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t key = key_of(x[e]);
+          if (key < p1 || key > hi || packed(key, i + e) < cut) continue;
+          const u64 y = weights ? weight(x[e]) : 1;
+          s1 += y;
+          if (key >= p2) s2 += y;
+          if (key >= p3) s3 += y;
+        }
+      });
+    });
+    s1 = above + block_scan(s1, sh.sums).all;
+    s2 = above + block_scan(s2, sh.sums).all;
+    s3 = above + block_scan(s3, sh.sums).all;
+    if (s3 >= want) lo = p3;
+    else if (s2 >= want) lo = p2, hi = p3 - 1, above = s3;
+    else if (s1 >= want) lo = p1, hi = p2 - 1, above = s2;
+    else hi = p1 - 1, above = s1;
   }
+  const uint32_t prefix = lo;
   // how many of the entries equal to it, the lowest indices first
   const u64 one = weights ? weight(of_key(prefix)) : 1;
   const u64 ties = one == 0 ? 1 : (want - above + one - 1) / one;
@@ -699,6 +703,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       if (n >= set.k) bound = tried;
       if (n == set.k) break;
     }
+    if (C > 1) {  // the row's k-th is not below any CTA's
+      if (tid == 0) sh.bound = bound;
+      cluster.sync();
+      for (int c = 0; c < C; ++c) bound = max(bound, of(c).bound);
+    }
   } else if (set.k > 0 || p_on) {
     // ---- How many logits lie how far below the largest: which bin the cut falls to, almost surely
     for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
@@ -851,17 +860,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         }
       }
     };
-    auto window = [&](const float (&x)[4], int i) {
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) any |= (x[e] >= low) & !(x[e] >= over);
-      if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((x[e] >= low) & !(x[e] >= over)) append(key_of(x[e]), i + e);
-        __syncwarp();
-      }
-    };
     if (mode == ALL) {
       tiles_of(from, [&](const float (&x)[4], int, u64& sum) {
 #pragma unroll
@@ -870,13 +868,21 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     } else {
       const float any = of_key(key_of(weight.least) + 1), least = mode == WINDOW_P ? any : fminf(over, low);
       tiles_of(least, [&](const float (&x)[4], int i, u64& sum) {
+        uint32_t inside = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const u64 y = weight.above_least(x[e]);
           add_if_from(rest, y, x[e], any);
           add_if_from(sum, y, x[e], from);
+          asm("{\n\t.reg .pred p, q;\n\tsetp.lt.f32 p, %1, %3;\n\tsetp.ge.and.f32 q, %1, %2, p;\n\t@q or.b32 %0, %0, %4;\n\t}"
+              : "+r"(inside) : "f"(x[e]), "f"(low), "f"(over), "r"(1 << e));
         }
-        window(x, i);
+        if (__any_sync(0xffffffffu, inside != 0)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (inside >> e & 1) append(key_of(x[e]), i + e);
+          __syncwarp();
+        }
       });
       rest = block_scan(rest, sh.sums).all;  // (of the whole row, where mode is WINDOW_P)
       above = block_scan(lane == 0 ? above : 0, sh.sums).all;
