@@ -559,3 +559,184 @@ def test_sample_strides_and_repeats(cdl, gpu_ok, dtype):
     assert torch.equal(res.token, cdl.serve.sample(z.flip(0).contiguous(), u, opts).token)
     assert cdl.serve.sample(z, u, opts, logprob=False).logprob is None
     assert cdl.serve.sample(z[:0], u[:0], opts).token.shape == (0,)
+
+
+# --------------------------------------------------------------------------- far offsets
+@gpu
+def test_cache_of_more_than_2_31_elements(cdl, gpu_ok):
+    """Pages whose elements lie beyond 2^31 from the cache's start: written and attended to."""
+    pages, page_size, heads = 140000, 16, 8
+    k = torch.empty(pages, page_size, heads, 128, dtype=BF16, device="cuda")  # 2.3 10^9 elements
+    assert k.numel() > 2 ** 31
+    v = torch.empty_like(k)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    new = torch.randn(2, 40, heads, 128, generator=gen, device="cuda").to(BF16)
+    at = [pages - 1, 3, pages - 2]
+    slots = [at[j // page_size] * page_size + j % page_size for j in range(40)]
+    cdl.serve.cache_write(new[0], new[1], ints(slots), k, v)
+    q = torch.randn(1, heads, 128, generator=gen, device="cuda").to(BF16)
+    got = cdl.serve.attention_decode(q, k, v, ints([at]).reshape(1, 3), ints([40]), lse=True)
+    small_k, small_v = (torch.zeros(3, page_size, heads, 128, dtype=BF16, device="cuda") for _ in range(2))
+    small_k.view(48, heads, 128)[:40], small_v.view(48, heads, 128)[:40] = new[0], new[1]
+    want = check_decode(cdl, q, small_k, small_v, ints([[0, 1, 2]]), ints([40]))
+    assert torch.equal(got.out, want.out) and torch.equal(got.lse, want.lse)
+
+
+@gpu
+def test_logits_of_more_than_2_31_elements(cdl, gpu_ok):
+    vocab = 150001
+    rows = 2 ** 31 // vocab + 2
+    z = torch.zeros(rows, vocab, dtype=BF16, device="cuda")
+    z[-1, 77], z[-1, 99] = 30.0, 30.0
+    z[-2, 5] = 40.0
+    u = torch.full((rows,), 0.75, device="cuda")
+    got = cdl.serve.sample(z, u, cdl.serve.SampleOpts(top_k=2)).token
+    assert got[-1] == 99 and got[-2] == 5 and got[0] == 1
+    assert cdl.serve.sample(z, u, cdl.serve.SampleOpts(temperature=0.0)).token[-2:].tolist() == [5, 77]
+
+
+# --------------------------------------------------------------------------- refusals (no GPU: operands are checked first)
+def status(cdl, name, *args):
+    L = cdl._lib
+    given = [L.tensor_bytes(a) if isinstance(a, torch.Tensor) else a for a in args]
+    return getattr(L.packed_lib, name)(*given, None), L.last_error()
+
+
+def swap(args, i, x):
+    return [x if j == i else a for j, a in enumerate(args)]
+
+
+def bf(*shape):
+    return torch.zeros(*shape, dtype=BF16)
+
+
+def i32(*shape):
+    return torch.zeros(*shape, dtype=I32)
+
+
+def test_plan_refusals(cdl):
+    # page_size, pages, cached, added, block_table, free_pages, free_count | seq_lens, cu_seqlens, positions, slots, free_left
+    good = [16, 9, i32(4), i32(4), i32(4, 3), i32(9), i32(1), i32(4), i32(5), i32(7), i32(7), i32(1)]
+    call = lambda args: status(cdl, "cdl_b200_cache_plan", *args)
+    for i, bad, message in [
+        (0, 0, "page_size"), (0, -3, "page_size"), (1, -1, "page_size"), (1, 2 ** 30, "2^31"), (2, i32(3), "must be"),
+        (3, i32(5), "added"), (3, torch.zeros(4), "added"), (3, i32(8)[::2], "added"), (4, i32(3, 3), "block_table"),
+        (4, i32(4, 6)[:, ::2], "block_table"), (4, i32(1, 3).expand(4, 3), "overlap"), (4, torch.zeros(4, 3), "block_table"),
+        (5, i32(3, 3), "free_pages"), (6, i32(2), "free_count"), (7, i32(5), "seq_lens"), (8, i32(4), "cu_seqlens"),
+        (9, i32(6), "positions"), (10, i32(2, 7), "vectors"), (11, i32(0), "free_left"), (2, None, "required"), (6, None, "free_count"),
+    ]:
+        st, text = call(swap(good, i, bad))
+        assert st == -1 and message in text, (i, message, st, text)
+    for i, j in ((7, 2), (7, 3), (11, 6), (9, 10), (8, 7), (4, 2), (10, 5)):  # an output that is an input, or another output
+        shared = i32(64)
+        size = lambda a: shared[:a.numel()].view(a.shape)
+        st, text = call(swap(swap(good, i, size(good[i])), j, size(good[j])))
+        assert st == -1 and "overlap" in text, (i, j, text)
+
+
+def test_write_refusals(cdl):
+    # q, k, v, cos_sin, positions, slots, q_out, k_out, k_cache, v_cache
+    good = [bf(5, 4, 32), bf(5, 2, 32), bf(5, 2, 32), torch.zeros(8, 32), i32(5), i32(5), bf(5, 4, 32), None, bf(3, 4, 2, 32), bf(3, 4, 2, 32)]
+    call = lambda args: status(cdl, "cdl_b200_cache_write", *args)
+    flat = bf(5 * 8 * 32 + 8)
+    for i, bad, message in [
+        (0, None, "together"), (6, None, "together"), (3, None, "together"), (4, None, "together"), (1, None, "required"),
+        (0, bf(4, 4, 32), "q must be"), (0, torch.zeros(5, 4, 32), "q must be"), (1, bf(5, 64), "k must be"), (2, bf(5, 3, 32), "v must be"),
+        (1, flat[1:1 + 320].view(5, 2, 32), "16-byte"), (1, flat[:5 * 68].view(5, 68)[:, :64].view(5, 2, 32), "16-byte"),
+        (2, bf(5, 32, 2).transpose(1, 2), "contiguous"), (3, torch.zeros(8, 64), "cos_sin"), (3, torch.zeros(8, 64)[:, ::2], "cos_sin"),
+        (4, i32(4), "positions"), (5, i32(6), "slots"), (5, torch.zeros(5), "slots"), (6, bf(5, 4, 64), "q_out"),
+        (6, bf(1, 4, 32).expand(5, 4, 32), "overlap"), (8, bf(3, 4, 3, 32), "caches"), (8, bf(3, 4, 2, 64), "caches"),
+        (9, bf(4, 4, 2, 32), "caches"), (9, torch.zeros(3, 4, 2, 32), "caches"), (8, bf(1, 4, 2, 32).expand(3, 4, 2, 32), "overlap"),
+        (9, good[8], "overlap"), (6, good[1].expand(2, 5, 2, 32)[0].reshape(5, 2, 32), "q_out"), (7, good[2], "overlap"), (6, good[0][:, :, :], None),
+    ]:
+        if message is None:
+            continue
+        st, text = call(swap(good, i, bad))
+        assert st == -1 and message in text, (i, message, st, text)
+    # q_out and k_out without a table, head_dim off 16 or too long, q_out one row behind q
+    st, text = call(swap(swap(good, 3, None), 4, None))
+    assert st == -1 and "table" in text
+    for d in (24, 4096):
+        st, text = call([None, bf(5, 2, d), bf(5, 2, d), None, None, i32(5), None, None, bf(3, 4, 2, d), bf(3, 4, 2, d)])
+        assert st == -1 and "head_dim" in text
+    rows = bf(6, 4, 32)
+    st, text = call(swap(swap(good, 0, rows[:5]), 6, rows[1:]))
+    assert st == -1 and "overlaps an input" in text
+
+
+def test_views_of_one_fused_tensor_are_told_apart(cdl):
+    """q_out = q inside qkv beside k and v, k_cache and v_cache inside one tensor: not refused as overlapping (no tokens: nothing
+    runs); a head further on is."""
+    qkv = bf(0, 8, 32)
+    both = bf(3, 4, 2, 2, 32)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    args = [q, k, v, torch.zeros(8, 32), i32(0), i32(0), q, k, both[:, :, 0], both[:, :, 1]]
+    assert status(cdl, "cdl_b200_cache_write", *args)[0] == 0
+    pages = bf(3, 2, 4, 2, 32)
+    assert status(cdl, "cdl_b200_cache_write", *args[:8], pages[:, 0], pages[:, 1])[0] == 0
+    st, text = status(cdl, "cdl_b200_cache_write", *args[:8], both[:, :, 0], both[:, :, 0])
+    assert st == -1 and "overlap" in text
+    qkv = bf(2, 8, 32)
+    st, text = status(cdl, "cdl_b200_cache_write", qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], torch.zeros(8, 32), i32(2), i32(2), qkv[:, 1:5], None,
+                      both[:, :, 0], both[:, :, 1])
+    assert st == -1 and "overlaps an input" in text
+
+
+def test_decode_refusals(cdl):
+    L = cdl._lib
+    desc = lambda scale=0.0, cap=0.0, window=0: L.attn_decode_bytes(scale, cap, window)
+    buf = torch.zeros(1 << 20, dtype=torch.uint8)
+    at = (buf.data_ptr() + 255) // 256 * 256
+    # desc, q, k_cache, v_cache, block_table, seq_lens, out, lse, scratch, bytes
+    good = [desc(), bf(3, 4, 64), bf(5, 16, 2, 64), bf(5, 16, 2, 64), i32(3, 2), i32(3), bf(3, 4, 64), torch.zeros(3, 4), at, 1 << 40]
+    call = lambda args: status(cdl, "cdl_b200_attn_decode", *args)
+    nan, inf = float("nan"), float("inf")
+    for i, bad, message in [
+        (0, None, "required"), (0, desc(cap=-1.0), "softcap"), (0, desc(cap=nan), "softcap"), (0, desc(cap=inf), "softcap"),
+        (0, desc(scale=nan), "softmax_scale"), (0, desc(scale=inf), "softmax_scale"), (0, desc(window=-1), "window"),
+        (1, torch.zeros(3, 4, 64), "q must be"), (1, bf(3, 256), "q must be"), (1, bf(3, 3, 64), "multiple"), (1, bf(3, 4, 128), "differ"),
+        (2, bf(5, 16, 64), "caches"), (2, torch.zeros(5, 16, 2, 64), "caches"), (3, bf(4, 16, 2, 64), "v_cache"), (3, None, "required"),
+        (4, i32(4, 2), "block_table"), (4, torch.zeros(3, 2), "block_table"), (4, i32(3, 4)[:, ::2], "block_table"),
+        (5, i32(4), "seq_lens"), (5, torch.zeros(3), "seq_lens"), (6, bf(3, 4, 128), "out"), (6, bf(1, 4, 64).expand(3, 4, 64), "overlap"),
+        (6, good[1], "overlaps an input"), (7, torch.zeros(4, 3), "lse"), (7, bf(3, 4), "lse"), (8, None, "scratch"), (8, at + 16, "scratch"),
+        (9, 1000, "scratch"), (2, bf(5, 16, 2, 72)[:, :, :, :64].transpose(2, 3), "caches"), (1, bf(3, 4, 65)[:, :, 1:], "q must have"),
+        (2, bf(5, 16, 2, 65)[:, :, :, :64], "k_cache must have"),
+    ]:
+        st, text = call(swap(good, i, bad))
+        assert st in (-1, -2) and (message in text or message == "caches" and "differ" in text), (i, message, st, text)
+    st, text = call(swap(swap(swap(swap(good, 1, bf(3, 4, 96)), 2, bf(5, 16, 2, 96)), 3, bf(5, 16, 2, 96)), 6, bf(3, 4, 96)))
+    assert st == -2 and "64 or 128" in text
+    n = ctypes.c_size_t(0)
+    assert L.packed_lib.cdl_b200_attn_decode_scratch_bytes(L.tensor_bytes(bf(5000, 1, 64)), L.tensor_bytes(bf(5, 16, 1, 64)), ctypes.byref(n)) == -2
+    assert L.packed_lib.cdl_b200_attn_decode_scratch_bytes(L.tensor_bytes(bf(3, 4, 64)), L.tensor_bytes(bf(5, 16, 2, 64)), None) == -1
+
+
+def test_sample_refusals(cdl):
+    L = cdl._lib
+    # desc, logits, uniform, temperature, top_k, top_p, min_p, token, logprob
+    f = torch.zeros
+    good = [L.sample_bytes(1.0, 0, 1.0, 0.0), f(4, 50), f(4), f(4), i32(4), f(4), f(4), i32(4), f(4)]
+    call = lambda args: status(cdl, "cdl_b200_sample", *args)
+    for i, bad, message in [
+        (0, None, "required"), (1, f(200), "logits"), (1, i32(4, 50), "logits"), (1, f(4, 100)[:, ::2], "contiguous"), (1, f(4, 0), "empty"),
+        (2, f(3), "uniform"), (2, i32(4), "uniform"), (2, f(8)[::2], "uniform"), (3, i32(4), "temperature"), (4, f(4), "top_k"),
+        (5, f(5), "top_p"), (6, f(4, 1), "min_p"), (7, f(4), "token"), (7, None, "required"), (8, i32(4), "logprob"), (8, good[2], "overlaps"),
+    ]:
+        st, text = call(swap(good, i, bad))
+        assert st == -1 and message in text, (i, message, st, text)
+    shared = i32(4)
+    st, text = call(swap(swap(good, 4, shared), 7, shared))
+    assert st == -1 and "overlaps an input" in text
+
+
+def test_python_refusals(cdl):
+    """What the Python layer refuses by itself: operands that are not in device memory, shapes that it reads."""
+    S = cdl.serve
+    with pytest.raises(cdl._lib.CdlError, match="device memory"):
+        S.cache_plan(i32(4), i32(4), i32(4, 3), i32(9), i32(1), S.CachePlanOpts(16, 9, 7))
+    with pytest.raises(cdl._lib.CdlError, match="device memory"):
+        S.attention_decode(bf(3, 4, 64), bf(5, 16, 2, 64), bf(5, 16, 2, 64), i32(3, 2), i32(3))
+    with pytest.raises(cdl._lib.CdlError, match="device memory"):
+        S.cache_write(bf(5, 2, 32), bf(5, 2, 32), i32(5), bf(3, 4, 2, 32), bf(3, 4, 2, 32))
+    with pytest.raises(cdl._lib.CdlError, match="rows, vocab"):
+        S.sample(torch.zeros(50), torch.zeros(1))
