@@ -298,6 +298,8 @@ struct Shared {
   u64 above, all;
   int mode, lo, hi;
   uint32_t before;
+  int edge[6];
+  uint32_t ahead_of[6];
   // what a CTA's threads tell one another
   u64 word;
   int index;
@@ -730,6 +732,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       constexpr int PER = BINS / THREADS;
       // (the sums fit: at most 2^30 entries, and estimated masses in units of 2^-32)
       u64 sum = 0, mass = 0;
+      float squares = 0.f;
       auto estimate = [&](int b, uint32_t n) {
         return static_cast<u64>(n * exp2f((b + 0.5f) * (-1.f / BIN_PER)) * 4294967296.f);
       };
@@ -740,57 +743,64 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         const uint4 o = reinterpret_cast<const uint4*>(of(c).hist)[tid];
         bins.x += o.x, bins.y += o.y, bins.z += o.z, bins.w += o.w;
       }
-      if (C > 1) reinterpret_cast<uint4*>(sh.hist)[tid] = bins;
+      const uint32_t count[PER] = {bins.x, bins.y, bins.z, bins.w};
+      u64 about[PER];
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const uint32_t n = j == 0 ? bins.x : j == 1 ? bins.y : j == 2 ? bins.z : bins.w;
-        sum += n, mass += estimate(tid * PER + j, n);
+        about[j] = estimate(tid * PER + j, count[j]);
+        sum += count[j], mass += about[j];
+        squares += static_cast<float>(about[j]) * static_cast<float>(about[j]);
       }
-      Sums s = block_scan(set.k > 0 ? sum : mass, sh.sums);
-      if (tid == 0) sh.lo = BINS - 1, sh.before = 0;
-      __syncthreads();
-      const u64 want = set.k > 0 ? static_cast<u64>(set.k) : max(u64{1}, static_cast<u64>(set.top_p * static_cast<float>(s.all)));
-#pragma unroll 1
-      for (int j = 0; j < PER; ++j) {
-        const int b = tid * PER + j;
-        const u64 y = set.k > 0 ? sh.hist[b] : estimate(b, sh.hist[b]);
-        if (s.before < want && s.before + y >= want) sh.lo = b, sh.before = static_cast<uint32_t>(s.before);
-        s.before += y;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        const int b = sh.lo;
-        const uint32_t n = sh.hist[b];
-        int from = b, to = b;
-        mode = SLOW;
-        if (set.k > 0) {
-          if (static_cast<u64>(set.k) >= s.all) mode = p_on ? SLOW : ALL;  // (the rest is -inf)
-          else if (sh.before + n <= CAP) mode = LIST;
-          else if (!p_on && n <= CAP) mode = WINDOW_K;
-        } else if (n <= CAP) {
-          // A window around the bin, as wide as the estimates may be wrong: a logit's place in its bin is worth 2^-8 of its weight at
-          // most, which averages out over the bins; where all of a bin are equal (bf16) about 2^-12 of the whole sum is left.  2^-10
-          // are taken.  (Whether the window holds the cut is checked by exact sums.)
-          const int d = lane + 1;
-          const uint32_t below = b - d >= 0 ? sh.hist[b - d] : 0, behind = b + d < BINS ? sh.hist[b + d] : 0;
-          uint32_t both = below + behind;
-          u64 reach = estimate(b, min(b - d >= 0 ? below : 1u << 30, b + d < BINS ? behind : 1u << 30));
-#pragma unroll 1
-          for (int i = 1; i < 32; i <<= 1) {
-            const uint32_t o = __shfl_up_sync(0xffffffffu, both, i);
-            const u64 f = __shfl_up_sync(0xffffffffu, reach, i);
-            if (lane >= i) both += o, reach += f;
+      Sums n = block_scan(sum, sh.sums), m{0, 0};
+      if (tid == 0) sh.before = 0, sh.mode = SLOW;
+      if (tid < 6) sh.edge[tid] = BINS - 1, sh.ahead_of[tid] = tid & 1 ? static_cast<uint32_t>(n.all) : 0;
+      if (set.k > 0) {
+        __syncthreads();
+        const u64 want = static_cast<u64>(set.k);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          if (n.before < want && n.before + count[j] >= want) {  // the bin of the k-th
+            const u64 through = n.before + count[j];
+            sh.before = static_cast<uint32_t>(n.before);
+            sh.lo = sh.hi = tid * PER + j;
+            if (want >= n.all) sh.mode = p_on ? SLOW : ALL;  // (the rest is -inf)
+            else if (through <= CAP) sh.mode = LIST;
+            else if (!p_on && count[j] <= CAP) sh.mode = WINDOW_K;
           }
-          const unsigned fits = __ballot_sync(0xffffffffu, n + both <= CAP);       // a run of ones from bit 0
-          const unsigned wide = __ballot_sync(0xffffffffu, reach >= (s.all >> 10));
-          const int width = min(wide ? __ffs(wide) : 32, __popc(fits));
-          mode = WINDOW_P, from = max(0, b - width), to = min(BINS - 1, b + width);
+          n.before += count[j];
         }
-        __syncwarp();
-        if (lane == 0) {
-          sh.mode = mode, sh.hi = to;
-          sh.lo = from;
+        if (tid == 0 && want > n.all && !p_on) sh.mode = ALL;
+      } else {
+        m = block_scan(mass, sh.sums);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+        if (lane == 0) sh.tops[warp] = squares;
+        __syncthreads();
+        squares = 0.f;
+        for (int i = 0; i < WARPS; ++i) squares += sh.tops[i];
+        // A window around the cut, as wide as the estimates may be wrong.  A logit's place in its bin is worth ln 2 / 128 of its weight
+        // at most; the share of what is above an edge is off by half of that, at most 2^-8 of all, and by four standard deviations of
+        // errors that are spread evenly and the same for all of a bin (bf16).  Or a quarter of it, or the bin alone, where the list does
+        // not hold more.  (Whether the window holds the cut is checked by exact sums.)
+        const float all = static_cast<float>(m.all), target = set.top_p * all;
+        const float margin = fminf(all * (1.f / 256), 4 * 0.0031f * sqrtf(squares));
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+#pragma unroll
+          for (int t = 0; t < 6; ++t) {
+            const float reach = t < 2 ? margin : t < 4 ? margin * 0.25f : 0.f;
+            const u64 want = max(u64{1}, static_cast<u64>(fmaxf(0.f, fminf(all, t & 1 ? target + reach : target - reach))));
+            if (m.before < want && m.before + about[j] >= want) {
+              sh.edge[t] = tid * PER + j;
+              sh.ahead_of[t] = static_cast<uint32_t>(n.before + (t & 1 ? count[j] : 0));
+            }
+          }
+          m.before += about[j], n.before += count[j];
         }
+        __syncthreads();
+        if (tid == 0)
+          for (int t = 4; t >= 0; t -= 2)
+            if (sh.ahead_of[t + 1] - sh.ahead_of[t] <= CAP) sh.mode = WINDOW_P, sh.lo = sh.edge[t], sh.hi = sh.edge[t + 1];
       }
     }
     meet();
