@@ -28,7 +28,7 @@ constexpr int BINS = 2048;   // of the logits below the largest, in units of T l
 constexpr int BIN_PER = 64;
 constexpr int TILES = 1024;  // of a row, whose sums are kept
 constexpr int SMALL = THREADS;  // entries of a list that are not sorted
-constexpr int LIST_K = 384;  // top_k up to which a bound from the threads' largest logits finds the candidates
+constexpr int LIST_K = 384;  // a CTA's part of top_k up to which a bound from the threads' largest logits finds the candidates
 
 struct Params {
   const void* z;
@@ -690,11 +690,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   uint32_t bound = 0;                      // of the list's keys
   float over = 0.f, low = 0.f;             // logits of the window: [low, over)
   const int have = min(THREADS, row.vectors / C);  // threads with a vector, in a CTA
+  const int each_k = (set.k + C - 1) / C;
   if ((set.k > 0 || p_on) && p.vocab <= CAP) {
     mode = LIST;
-  } else if (set.k > 0 && set.k <= min(LIST_K, have * 3 / 4)) {
-    // The k-th of the threads' largest logits is a bound that at least k logits of this CTA reach, and few more than k: its part of
-    // the row's k largest are among those.
+  } else if (set.k > 0 && each_k <= min(LIST_K, have * 3 / 4)) {
+    // A CTA's part of top_k: that many of its threads' largest logits reach its bound, so the least of the CTAs' bounds is one that
+    // at least top_k logits of the row reach, and not many more.
     mode = LIST;
     const uint32_t key = key_of(mine);
     constexpr int LOW = N == 8 ? 16 : 0;  // bits that tell no two bf16 apart
@@ -702,13 +703,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     for (int bit = 31; bit >= LOW; --bit) {
       const uint32_t tried = bound | (1u << bit);
       const int n = __syncthreads_count(key >= tried);
-      if (n >= set.k) bound = tried;
-      if (n == set.k) break;
+      if (n >= each_k) bound = tried;
+      if (n == each_k) break;
     }
-    if (C > 1) {  // the row's k-th is not below any CTA's
+    if (C > 1) {
       if (tid == 0) sh.bound = bound;
       cluster.sync();
-      for (int c = 0; c < C; ++c) bound = max(bound, of(c).bound);
+      for (int c = 0; c < C; ++c) bound = min(bound, of(c).bound);
     }
   } else if (set.k > 0 || p_on) {
     // ---- How many logits lie how far below the largest: which bin the cut falls to, almost surely
