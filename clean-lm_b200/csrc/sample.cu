@@ -299,7 +299,7 @@ struct Shared {
   int mode, lo, hi;
   uint32_t before;
   int edge[6];
-  uint32_t ahead_of[6];
+  uint32_t ahead_of[6], least_of[2];
   // what a CTA's threads tell one another
   u64 word;
   int index;
@@ -807,9 +807,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     meet();
     const Shared& o = of(0);
     mode = static_cast<Mode>(o.mode);
-    if (mode == WINDOW_P || mode == WINDOW_K || mode == LIST) {
+    const bool window = mode == WINDOW_P || mode == WINDOW_K || mode == LIST;
+    if (window && tid < 2) {  // (two threads: all of them doing it took 4900 cycles)
       // the least logits of the bins up to lo - 1 and up to hi: the logits below have larger bins
-      const int last = lane == 0 ? o.lo - 1 : o.hi;
+      const int last = tid == 0 ? o.lo - 1 : o.hi;
       uint32_t below = KEY_NONE, from = last < 0 ? KEY_NONE + 1 : key_of(top);
 #pragma unroll 1
       while (from - below > 1) {
@@ -817,10 +818,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         if (bin(of_key(mid)) <= last) from = mid;
         else below = mid;
       }
-      over = last < 0 ? INFINITY : of_key(from);
-      bound = __shfl_sync(0xffffffffu, from, 1);
-      over = __shfl_sync(0xffffffffu, over, 0), low = of_key(bound);
+      sh.least_of[tid] = last < 0 ? key_of(INFINITY) : from;
     }
+    __syncthreads();
+    if (window) over = of_key(sh.least_of[0]), bound = sh.least_of[1], low = of_key(bound);
   }
   __syncthreads();
 
