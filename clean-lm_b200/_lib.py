@@ -312,6 +312,13 @@ def matrix_bytes(ptr: int, dtype: int, rows: int, cols: int) -> bytes:
     return _pack_tensor(ptr, dtype, 2, rows, cols, 0, 0, cols, 1, 0, 0)
 
 
+def shape_bytes(dtype: int, shape) -> bytes:
+    """The bytes of a cdl_tensor of which a call reads type and shape alone."""
+    if len(shape) > 4:
+        raise CdlError(-1, f"rank {len(shape)} exceeds 4")
+    return _pack_tensor(0, dtype, len(shape), *shape, *_UNUSED[len(shape)], 0, 0, 0, 0)
+
+
 _HEAD_LOSS_BYTES = struct.Struct("ffiq")  # the layout of cdl_head_loss_desc
 assert _HEAD_LOSS_BYTES.size == ctypes.sizeof(CdlHeadLossDesc)
 head_loss_bytes = _HEAD_LOSS_BYTES.pack  # (temperature, grad_scale, accumulate_dw, chunk_rows)

@@ -19,6 +19,7 @@ As in `ops`, this layer allocates outputs and scratch and calls the C ABI on the
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional, Union
 
@@ -112,6 +113,15 @@ def attention_decode_scratch_bytes(q, k_cache) -> int:
     return n.value
 
 
+@functools.lru_cache(maxsize=4096)
+def _scratch_of(q_shape, cache_shape, device: int) -> int:
+    """The same from the shapes, which is all that it depends on; the attention's call checks the rest."""
+    n = ctypes.c_size_t(0)
+    check(packed_lib.cdl_b200_attn_decode_scratch_bytes(*(_lib.shape_bytes(_lib.CDL_BF16, s) for s in (q_shape, cache_shape)),
+                                                        ctypes.byref(n)))
+    return n.value
+
+
 def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: AttentionDecodeOpts | None = None, lse: bool = False,
                      out=None, scratch=None) -> AttentionDecodeOutputs:
     """Attention of one new token per request (q [batch, heads, head_dim]) over its seq_lens keys in the paged cache."""
@@ -119,9 +129,7 @@ def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: Attention
     _require_current_device(q, k_cache, v_cache, block_table, seq_lens, out, scratch)
     tq, tk = tensor_bytes(q), tensor_bytes(k_cache)
     if scratch is None:
-        n = ctypes.c_size_t(0)
-        check(packed_lib.cdl_b200_attn_decode_scratch_bytes(tq, tk, ctypes.byref(n)))
-        scratch = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        scratch = torch.empty(_scratch_of(q.shape, k_cache.shape, q.get_device()), dtype=torch.uint8, device=q.device)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse_t = tl = None
