@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
     if (b < p.batch) {
       int first, end;
       visible(p, b, first, end);
-      n = (end - first + KEYS - 1) / KEYS;
+      n = static_cast<int>((static_cast<unsigned>(end - first) + (KEYS - 1)) / KEYS);
     }
     int x = n;
 #pragma unroll
@@ -243,18 +243,20 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   const uint32_t ring = smem_u32(smem + warp * STAGES * STAGE);
   long long next = u;  // unit
   int left = 0;        // tiles of its line from it on
-  int key = 0, end = 0, page = -1;
+  unsigned key = 0, end = 0;  // (up to 31 behind the last key of a request, which may be 2^31 - 1)
+  int page = -1;
   const int* table = nullptr;
   const __nv_bfloat16 *from_k = nullptr, *from_v = nullptr;
   auto look_up = [&]() {  // the page of this lane's key, a tile ahead of the copies
-    page = next < u_end && key < end ? table[static_cast<unsigned>(key) / static_cast<unsigned>(p.page_size)] : -1;
+    page = next < u_end && key < end ? table[key / static_cast<unsigned>(p.page_size)] : -1;
   };
   auto enter = [&]() {  // the line of `next`
     const Place at = place_of(next);
     const int kvh = at.row / p.chunks;
-    int first;
-    visible(p, at.b, first, end);
-    key = first + at.tile * KEYS + (lane & (KEYS - 1));
+    int first, last;
+    visible(p, at.b, first, last);
+    end = static_cast<unsigned>(last);
+    key = static_cast<unsigned>(first) + static_cast<unsigned>(at.tile) * KEYS + (lane & (KEYS - 1));
     left = at.n - at.tile;
     table = p.table + at.b * p.table_sb;
     from_k = p.k + kvh * p.k_sh;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   auto fetch = [&](int stage) -> uint32_t {
     uint32_t mask = 0;
     if (next < u_end) {
-      const int slot = static_cast<int>(static_cast<unsigned>(key) % static_cast<unsigned>(p.page_size));
+      const int slot = static_cast<int>(key % static_cast<unsigned>(p.page_size));
       const bool live = page >= 0 && page < p.pages;
       mask = __ballot_sync(0xffffffffu, live);
       // Where this lane's row lies; D = 128: lanes 16 to 31 have the same keys again and hold the places of their values.

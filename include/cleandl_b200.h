@@ -447,9 +447,9 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
  * times page_size.  q and out bf16 [batch, heads, head_dim], last dimension contiguous, other strides and base 16-byte
  * aligned, head_dim 64 or 128, heads a multiple of kv_heads; block_table i32 [batch, width], contiguous rows; seq_lens packed
  * i32 [batch]; lse (nullable) packed f32 [batch, heads].  out overlaps no input.
- * Keys of a page outside [0, pages) are not read and do not count, nor does a key whose score is -inf.  A request in which no
- * key counts (an empty one among them) has zeros in out and lse -inf; a NaN or +inf among its scores makes its results NaN.
- * What the cache holds behind a request's last key may be anything.  Statistics and sums are f32; probabilities are rounded to
+ * Keys of a page outside [0, pages) are not read and do not count.  A key whose score is -inf has weight 0, which its values are
+ * multiplied by.  A request in which no key has weight (an empty one among them) has zeros in out and lse -inf; a NaN or +inf
+ * among its scores makes its results NaN.  What the cache holds behind a request's last key or ahead of its window may be anything.  Statistics and sums are f32; probabilities are rounded to
  * bf16 for their product with the values, as in cdl_b200_attn_fwd.  Results do not depend on timing.
  * Scratch: 256-byte aligned, of the size that the call below gives; calls that may run at the same time have one each. */
 typedef struct {

@@ -740,3 +740,24 @@ def test_python_refusals(cdl):
         S.cache_write(bf(5, 2, 32), bf(5, 2, 32), i32(5), bf(3, 4, 2, 32), bf(3, 4, 2, 32))
     with pytest.raises(cdl._lib.CdlError, match="rows, vocab"):
         S.sample(torch.zeros(50), torch.zeros(1))
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_of_2_31_keys(cdl, gpu_ok, dim):
+    """The longest request there is: one large page again and again, whose keys all score the same; its last tile ends behind
+    2^31 - 1.  And the window at its end."""
+    page_size = 1 << 20
+    k = torch.ones(1, page_size, 1, dim, dtype=BF16, device="cuda")
+    v = torch.full_like(k, 3.0)
+    q = torch.ones(1, 1, dim, dtype=BF16, device="cuda")
+    table = torch.zeros(1, 2048, dtype=I32, device="cuda")
+    n = 2 ** 31 - 1
+    got = cdl.serve.attention_decode(q, k, v, table, ints([n]), lse=True)
+    # equal weights: the mean is exact; the logarithm of a sum of 2^31 ones in f32, in parts of at most 2^24 of them each
+    assert (got.out == 3.0).all()
+    want = dim ** 0.5 + np.log(float(n))
+    assert abs(got.lse.item() - want) <= 2.0 ** -20 * want
+    v[0, page_size - 40:] = 5.0
+    got = cdl.serve.attention_decode(q, k, v, table, ints([n]), cdl.serve.AttentionDecodeOpts(window=39))
+    assert (got.out == 5.0).all()
