@@ -6,8 +6,7 @@
 // Bound by reading the keys and values once (2 multiply-adds per 2-byte element and query head of a group; the tensor cores
 // see 8 or 16 query columns).  The tiles of 16 or 32 keys of all requests and kv heads form one line, whatever the lengths are,
 // that the CTAs share, and the warps of a CTA its part.  SMs do not read at the same rate (equal parts ended after 147 to 204 us,
-// the same SMs late each time), so the first CTAs, all of which run at once, take two thirds, and three more sets of smaller parts
-// follow as SMs become free.  Every warp works alone on a ring of its own in shared memory, which asynchronous 16-byte copies fill
+// the same SMs late each time), so a set of smaller parts follows the first where there is much to read.  Every warp works alone on a ring of its own in shared memory, which asynchronous 16-byte copies fill
 // STAGES tiles ahead and across the borders of requests, 8 lanes a row, wherever its page lies.  (Loaded straight into the
 // fragments, the next keys on their way behind the scores, 12 warps of an SM had too little under way, 270 us for 1.14 GB, which
 // are 174 us at 6.5 TB/s; a bulk copy per row, which a warp issues one lane after the other, took 262 us.)  A warp's running
@@ -66,23 +65,23 @@ __device__ __forceinline__ void visible(const Params& p, int b, int& first, int&
   first = p.window > 0 ? max(0, end - p.window) : 0;
 }
 
-// How the CTAs share `units` tiles: few of them evenly, one or more each (so that all partial results between a line's first and
-// last are there); many in SETS sets of `set` CTAs, evenly within a set.
-constexpr int SETS = 4, PARTS = 128;  // of PARTS parts of the whole the sets have 84, 28, 11 and 5
-// (Quotients are taken in f64, a tenth of the time of a 64-bit division: exact where units * ctas < 2^53, and in any case the same
-// everywhere and never falling.)
+// How the CTAs share `units` tiles: evenly, one or more each (so that all partial results between a line's first and last are
+// there); from 192 tiles each on, the CTAs that run at once share 7/8 evenly and a second set of as many the rest, as SMs become
+// free.  (Evenly / in two sets, us: 82 tiles each 60.7 / 64.6, 160 106.0 / 105.8, 315 195 / 185, 630 371 / 347.  Four sets of 84,
+// 28, 11 and 5 of 128 parts: 70, 109, 186, 343; a CTA's start is not hidden by the others of its SM.)
+// Quotients are taken in f64, a tenth of the time of a 64-bit division: exact where units * ctas < 2^53, and in any case the same
+// everywhere and never falling.
+constexpr int SETS = 2, PARTS = 8, FIRST = 7;
 struct Shares {
   long long units;
   int set, ctas;
   __host__ __device__ __forceinline__ Shares(long long units, int set) : units(units), set(set) {
-    ctas = units >= 32LL * WARPS * set ? SETS * set : static_cast<int>(units < set ? units : set);
+    ctas = units >= 192LL * set ? SETS * set : static_cast<int>(units < set ? units : set);
   }
-  static __host__ __device__ __forceinline__ int ahead(int i) { return i == 0 ? 0 : i == 1 ? 84 : i == 2 ? 112 : i == 3 ? 123 : 128; }
   __host__ __device__ __forceinline__ long long begin(int c) const {
     const double n = static_cast<double>(units);
     if (ctas <= set) return static_cast<long long>(n * c / ctas);
-    const int i = c >= 3 * set ? 3 : c >= 2 * set ? 2 : c >= set ? 1 : 0;
-    return static_cast<long long>(n * (ahead(i) * set + (ahead(i + 1) - ahead(i)) * (c - i * set)) / (PARTS * set));
+    return static_cast<long long>(n * (c < set ? FIRST * c : FIRST * set + (PARTS - FIRST) * (c - set)) / (PARTS * set));
   }
   // The CTA that has unit u: the last one that begins at it or ahead of it.
   __host__ __device__ __forceinline__ int of(long long u) const {
@@ -90,9 +89,8 @@ struct Shares {
     if (ctas <= set) {
       c = static_cast<int>(static_cast<double>(u) * ctas / static_cast<double>(units));
     } else {
-      const double x = static_cast<double>(u) * PARTS / static_cast<double>(units);
-      const int i = x >= ahead(3) ? 3 : x >= ahead(2) ? 2 : x >= ahead(1) ? 1 : 0;
-      c = i * set + static_cast<int>((x - ahead(i)) * set / (ahead(i + 1) - ahead(i)));
+      const double x = static_cast<double>(u) * PARTS / static_cast<double>(units) * set;
+      c = static_cast<int>(x < FIRST * set ? x / FIRST : set + (x - FIRST * set) / (PARTS - FIRST));
     }
     if (c >= ctas) c = ctas - 1;
     while (c > 0 && begin(c) > u) --c;
