@@ -8,6 +8,13 @@
 // fall as it does in exact arithmetic: weights are f64 exponentials, rounded to multiples of 2^-S and added as 64-bit integers
 // (S = 62 - log2 of the vocabulary, 50 at most, so that no sum overflows; 2^-47 of the largest weight for 32768 entries, against
 // 2^-24 in f32, where one draw in a few hundred of a flat row would fall on another token).
+//
+// A row is one to four CTAs' work.  They read it two or three times, from L2 but for the first: for the largest logit; where top_k
+// is large or top_p is on, for a histogram, which gives a bound that the kept entries reach or a window that the cut lies in; and
+// for the candidates, the sums of whole tiles and, around the cut, the entries on a list in shared memory.  The rest is that list
+// and one tile.  What bounds it is instructions and barriers, not memory: 148 rows of 32768 bf16 logits (1.5 us at 6.56 TB/s) take
+// 5.4 us for the largest, 12.3 for top_k of 50, 15.2 for an unrestricted draw (all weights, in f64) and 31.7 for top_p of 0.9 (a
+// histogram and all weights); one row in two CTAs 4.5, 11.0, 11.1 and 25.
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -23,12 +30,14 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int CAP = 2048;    // entries that are sorted at most
+constexpr int CAP = 2048;    // entries of a list
 constexpr int BINS = 2048;   // of the logits below the largest, in units of T ln 2 / BIN_PER
 constexpr int BIN_PER = 64;
 constexpr int TILES = 1024;  // of a row, whose sums are kept
-constexpr int SMALL = THREADS;  // entries of a list that are not sorted
-constexpr int LIST_K = 384;  // a CTA's part of top_k up to which a bound from the threads' largest logits finds the candidates
+constexpr int SMALL = THREADS;  // entries of a list that are each held against all others (100 to 256, the rest sorted: no faster)
+// A CTA's part of top_k up to which a bound from its threads' largest logits finds the candidates.  (Bound / histogram, us, 148
+// rows of 32768: top_k of 50 12.3 / 17.6, 100 14.2 / 19.0, 300 30 / 31; of 150001: 50 26 / 81, 300 59 / 94.)
+constexpr int LIST_K = 384;
 
 struct Params {
   const void* z;
@@ -676,15 +685,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
                        smem_u32(sh.pow2)};
   // w >= min_p: a bound on the logit, rounded up to the next one in f32
   set.key_min = 0;
-  if (min_p > 0.f)
-    set.key_min = min(key_of(top), key_of(__double2float_ru(static_cast<double>(top) + set.t * log(static_cast<double>(fminf(min_p, 1.f))))));
+  if (min_p > 0.f) {
+    const double far = set.t * log(static_cast<double>(fminf(min_p, 1.f)));  // (NaN: of an infinite temperature, where all w are 1)
+    set.key_min = isnan(far) ? 0 : min(key_of(top), key_of(__double2float_ru(static_cast<double>(top) + far)));
+  }
 
   auto append = [&](uint32_t key, int i) {
     const uint32_t at = atomicAdd(&sh.count, 1u);
     if (at < CAP) sh.list[at] = packed(key, i);
   };
   Mode mode = ALL;
-  const float bin_scale = fminf(static_cast<float>(per_t) * (BIN_PER / 256.f), 1e30f);
+  const float bin_scale = fmaxf(1e-36f, fminf(static_cast<float>(per_t) * (BIN_PER / 256.f), 1e30f));
   // How far a logit lies below the largest; rounded by the addition of 1.5 2^23, infinite distances in the last bin.
   auto bin = [&](float x) { return min(BINS - 1, __float_as_int(fmaf(top - x, bin_scale, 12582912.f)) - 0x4B400000); };
   uint32_t bound = 0;                      // of the list's keys
@@ -1076,8 +1087,11 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   while ((1LL << bits) < V) ++bits;
   p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
-  // CTAs of a row: as many as leave an SM one or two, with 16384 logits each or more
-  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, 3 * sm_count() / 2 / R, V / 16384})));
+  // CTAs of a row: as many as find an SM each, pairs on all SMs, larger clusters on 7/8 of them, with 16384 logits each or more.
+  // (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us: 16 rows of 150001 logits 93, 60, 48, 42, in 6 43; 37 rows 94, 61, 50, 60; 48 rows 94,
+  // 62, 71, 60; 100 rows 96, 91, 106, 109; 32768 logits, 16 rows 30, 25, 25, 23, 100 rows 31, 36, 51, 53; 16384 logits 21, 21.)
+  const long long sms = sm_count(), fit = 2 * R > sms ? 1 : std::max<long long>(2, sms * 7 / 8 / R);
+  p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, fit, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));
   CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), smem));

@@ -91,7 +91,8 @@ def sample(z, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not temperature > 0:
         return int(z.argmax()), 0.0
     order = np.argsort(-z, kind="stable")
-    d = (z - z.max()) / float(np.float32(temperature))
+    d = np.full(len(z), -np.inf)
+    d[z > -np.inf] = (z[z > -np.inf] - z.max()) / float(np.float32(temperature))
     # Weights as whole multiples of 2^-46 (2^-44 for more than 2^18 entries), so that sums are exact: with sums that round, equal
     # weights on both sides of a border decide by the order of additions.
     exact = 46 if len(z) <= 1 << 17 else 44

@@ -518,6 +518,26 @@ def test_sample_extreme_settings(cdl, gpu_ok):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [700, 5003, 40000])
+def test_sample_of_an_infinite_temperature(cdl, gpu_ok, vocab):
+    """Every entry that is not masked has the same weight."""
+    z, u = logits_of(6, vocab, F32, seed=7)
+    z[:, ::3] = -torch.inf
+    for opts in ({}, {"min_p": 1.0}, {"min_p": 0.5}, {"top_p": 0.4}, {"top_k": 37}, {"top_k": 1500, "top_p": 0.7}):
+        check_sample(cdl, z, u, temperature=torch.inf, **opts)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 40, 70, 80])
+def test_sample_rows_shared_by_several_ctas(cdl, gpu_ok, rows):
+    z, u = logits_of(rows, 66001, BF16, seed=rows)
+    check_sample(cdl, z, u)
+    check_sample(cdl, z, u, top_p=0.9)
+    check_sample(cdl, z, u, top_k=50)
+    check_sample(cdl, z, u, top_k=5000, min_p=0.01)
+
+
+@gpu
 def test_sample_draws_next_to_a_border(cdl, gpu_ok):
     """Random numbers as near to the borders between two tokens as f32 has them, on flat and on falling rows."""
     vocab = 30000
