@@ -6,12 +6,16 @@
 // Bound by reading the keys and values once (2 multiply-adds per 2-byte element and query head of a group; the tensor cores
 // see 8 or 16 query columns).  The tiles of 16 or 32 keys of all requests and kv heads form one line, whatever the lengths are,
 // that the CTAs share, and the warps of a CTA its part.  SMs do not read at the same rate (equal parts ended after 147 to 204 us,
-// the same SMs late each time), so a set of smaller parts follows the first where there is much to read.  Every warp works alone on a ring of its own in shared memory, which asynchronous 16-byte copies fill
-// STAGES tiles ahead and across the borders of requests, 8 lanes a row, wherever its page lies.  (Loaded straight into the
-// fragments, the next keys on their way behind the scores, 12 warps of an SM had too little under way, 270 us for 1.14 GB, which
-// are 174 us at 6.5 TB/s; a bulk copy per row, which a warp issues one lane after the other, took 262 us.)  A warp's running
-// maximum, sum and output stay in registers.  Where a warp's part cuts the keys of a (request, kv head), the warps of the CTA join
-// what they have of it; what the CTA's part cuts goes to the scratch, and a second kernel joins that.
+// the same SMs late each time), so a set of smaller parts follows the first where there is much to read.  Every warp works alone
+// on a ring of its own in shared memory, which asynchronous 16-byte copies fill STAGES tiles ahead and across the borders of
+// requests, 8 lanes a row, wherever its page lies.  (Loaded straight into the fragments, the next keys on their way behind the
+// scores, 12 warps of an SM had too little under way, 270 us for 1.14 GB, which are 174 us at 6.56 TB/s and take 183.7 now; a bulk
+// copy per row, which a warp issues one lane after the other, took 262.)  A warp's running maximum, sum and output stay in
+// registers.  Where a warp's part cuts the keys of a (request, kv head), the warps of the CTA join what they have of it; what the
+// CTA's part cuts goes to the scratch, and a second kernel joins that.
+//
+// Short work is bound by latency instead: one request of some hundred keys and 16 heads takes 10.9 us, two launches and some dozen trips to memory
+// one after the other (lengths, page, keys, values, the partial results and back).
 //
 // Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
 // of mma.m16n8k16 (as rows they would leave at least half of it empty) and the pieces of K and V rows that a thread reads are its
@@ -211,8 +215,8 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   const Shares shares(units, p.set);
   if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
   const long long c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
-  const long long busy = min(static_cast<long long>(WARPS), c1 - c0);  // warps with a part (tiles each: one too, 12.6 -> 10.9 us where
-                                                                       // 4 or more left warps without one in a short context)
+  // Warps with a part, of one tile or more.  (Of 4 tiles or more, so that some had none, a short context took 12.6 us, not 10.9.)
+  const long long busy = min(static_cast<long long>(WARPS), c1 - c0);
   long long u = 0, u_end = 0;
   if (warp < busy) u = c0 + (c1 - c0) * warp / busy, u_end = c0 + (c1 - c0) * (warp + 1) / busy;
 
@@ -277,7 +281,8 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
 #pragma unroll
       for (int j = 0; j < 2 * KEYS / 4; ++j) {
         const char* of = D == 128 || j < KEYS / 4 ? mine : mine_v;
-        const char* row = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<long long>(of), (4 * j + (lane >> 3)) & 31));
+        const char* row =
+            reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<long long>(of), (4 * j + (lane >> 3)) & 31));
         const char* from = row != nullptr ? row + (lane & 7) * 16 : reinterpret_cast<const char*>(p.q);
         const int bytes = row != nullptr ? 16 : 0;
 #pragma unroll
@@ -648,7 +653,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_decode_join_kernel(const
 }
 }  // namespace decode
 
-// Bytes of the scratch: tiles ahead of each request, then the partial results of 2 per warp.
+// Bytes of the scratch: tiles ahead of each request, then the partial results, two of a CTA and one of each of its warps.
 static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 static int tiles_of_columns(long long group) { return group <= 8 ? 1 : 2; }
 static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tensor* k_cache) {

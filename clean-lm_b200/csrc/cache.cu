@@ -14,7 +14,8 @@ namespace cache {
 // Served requests with need take stack[free - C_b ..], in the order of the requests: the served ones with need are the first
 // ones with it, as C only grows.
 // Bound by latency: one kernel, in which every CTA sums the lengths up itself (1024 requests at a time) and then takes its
-// share of the rows and pages, each found by a binary search in shared memory.
+// share of the rows and pages, each found by a binary search in shared memory.  (5.2 us for 64 requests of a token each, 9.9 for
+// 1999 of 1 to 64, two rounds of sums.)
 constexpr int THREADS = 256, PER = 4, CHUNK = THREADS * PER;
 
 struct PlanParams {
