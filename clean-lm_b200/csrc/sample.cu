@@ -1087,10 +1087,13 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   while ((1LL << bits) < V) ++bits;
   p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
-  // CTAs of a row: as many as find an SM each, pairs on all SMs, larger clusters on 7/8 of them, with 16384 logits each or more.
-  // (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us: 16 rows of 150001 logits 93, 60, 48, 42, in 6 43; 37 rows 94, 61, 50, 60; 48 rows 94,
-  // 62, 71, 60; 100 rows 96, 91, 106, 109; 32768 logits, 16 rows 30, 25, 25, 23, 100 rows 31, 36, 51, 53; 16384 logits 21, 21.)
-  const long long sms = sm_count(), fit = 2 * R > sms ? 1 : std::max<long long>(2, sms * 7 / 8 / R);
+  // CTAs of a row, of 16384 logits each or more: 4 or 3 where larger clusters find an SM for each (7/8 of them), 4 to two SMs where
+  // rows are long, pairs where each finds an SM.  (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us, from HBM: 150001 f32 logits, 16 rows 94,
+  // 58, 46, 39, in 6 and 8 slower; 37 rows 96, 59, 48, 58; 48 rows 98, 61, 69, 59, with what L2 holds of them 73 in 2, 61 in 4; 74
+  // rows 110, 68, 72, 88; 100 rows 120, 98, 111, 94.  65536: 48 rows 48, 35, 42, 37; 100 rows 53, 51, 66, 68.  32768 bf16: 16
+  // rows 30, 26, 25, 23, 100 rows 32, 36, 52, 54.)
+  const long long sms = sm_count(), own_sm = sms * 7 / 8 / R;
+  const long long fit = own_sm >= 3 ? own_sm : V >= 131072 && 4 * R <= sms * 7 / 4 ? 4 : 2 * R <= sms ? 2 : 1;
   p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, fit, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));
