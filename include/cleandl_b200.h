@@ -449,8 +449,9 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
  * i32 [batch]; lse (nullable) packed f32 [batch, heads].  out overlaps no input.
  * Keys of a page outside [0, pages) are not read and do not count.  A key whose score is -inf has weight 0, which its values are
  * multiplied by.  A request in which no key has weight (an empty one among them) has zeros in out and lse -inf; a NaN or +inf
- * among its scores makes its results NaN.  What the cache holds behind a request's last key or ahead of its window may be anything.  Statistics and sums are f32; probabilities are rounded to
- * bf16 for their product with the values, as in cdl_b200_attn_fwd.  Results do not depend on timing.
+ * among its scores makes its results NaN.  What the cache holds behind a request's last key or ahead of its window may be
+ * anything.  Statistics and sums are f32; probabilities are rounded to bf16 for their product with the values, as in
+ * cdl_b200_attn_fwd.  Results do not depend on timing.  At most 4096 requests.
  * Scratch: 256-byte aligned, of the size that the call below gives; calls that may run at the same time have one each. */
 typedef struct {
   float softmax_scale; /* <= 0 selects 1/sqrt(head_dim) */

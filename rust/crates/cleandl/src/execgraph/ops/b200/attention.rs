@@ -3,7 +3,8 @@
 //! exec.rs:358-416), which forwards to flash-attention-rs.  The library implements the dense and
 //! the packed layouts, masks None and Causal, bf16, head_dim 128 (GQA included); `AttentionOpts`
 //! with paged KV, seqused, softcap, sliding windows, fp8 or other head dimensions keep the
-//! existing executor (`supported` below is what `build` asks).
+//! existing executor (`supported` below is what `build` asks).  One query token per sequence over
+//! paged KV, with seqused, softcap or a left window, is `ffi::cdl_b200_attn_decode`.
 use super::{check, ffi, plain, plain_mut, raw_stream, tensor_ro, tensor_rw};
 use crate::{
     context::Context,

@@ -34,6 +34,25 @@ pub struct CdlAttnDesc {
     pub variant: i32,       // cdl_attn_variant: 0 auto, 1 one short-lived CTA per block, 2 one CTA per SM (forward and backward)
 }
 
+/// `cdl_attn_decode_desc`.
+#[repr(C)]
+#[derive(Copy, Clone, Debug)]
+pub struct CdlAttnDecodeDesc {
+    pub softmax_scale: f32, // <= 0: 1 / sqrt(head_dim)
+    pub softcap: f32,       // 0: none
+    pub window: i32,        // keys that a token sees, its own among them; 0: all
+}
+
+/// `cdl_sample_desc`.
+#[repr(C)]
+#[derive(Copy, Clone, Debug)]
+pub struct CdlSampleDesc {
+    pub temperature: f32, // <= 0: the largest logit
+    pub top_k: i32,       // <= 0: all
+    pub top_p: f32,       // >= 1: all
+    pub min_p: f32,       // <= 0: all
+}
+
 /// `cdl_matmul_options`: what a tuner candidate of the matmul executor carries.
 #[repr(C)]
 #[derive(Copy, Clone, Debug, PartialEq, Eq, serde::Serialize, serde::Deserialize)]
@@ -172,6 +191,36 @@ extern "C" {
         cu_seqlens_q: *const CdlTensor, cu_seqlens_k: *const CdlTensor, max_seqlen_q: i64,
         max_seqlen_k: i64, cos_sin: *const CdlTensor, dq: *const CdlTensor, dk: *const CdlTensor,
         dv: *const CdlTensor, scratch: *mut c_void, scratch_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+
+    // ---- serving: a paged cache (KvLayout::Paged, crates/cleandl/src/execgraph/ops/attention/mod.rs:83-91), attention of one
+    // new token per request over it, sampling
+    pub fn cdl_b200_attn_decode(
+        desc: *const CdlAttnDecodeDesc, q: *const CdlTensor, k_cache: *const CdlTensor,
+        v_cache: *const CdlTensor, block_table: *const CdlTensor, seq_lens: *const CdlTensor,
+        out: *const CdlTensor, lse: *const CdlTensor, scratch: *mut c_void, scratch_bytes: usize,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn cdl_b200_attn_decode_scratch_bytes(
+        q: *const CdlTensor, k_cache: *const CdlTensor, bytes_out: *mut usize,
+    ) -> i32;
+    pub fn cdl_b200_cache_plan(
+        page_size: i32, pages: i32, cached: *const CdlTensor, added: *const CdlTensor,
+        block_table: *const CdlTensor, free_pages: *const CdlTensor, free_count: *const CdlTensor,
+        seq_lens: *const CdlTensor, cu_seqlens: *const CdlTensor, positions: *const CdlTensor,
+        slots: *const CdlTensor, free_left: *const CdlTensor, stream: *mut c_void,
+    ) -> i32;
+    pub fn cdl_b200_cache_write(
+        q: *const CdlTensor, k: *const CdlTensor, v: *const CdlTensor, cos_sin: *const CdlTensor,
+        positions: *const CdlTensor, slots: *const CdlTensor, q_out: *const CdlTensor,
+        k_out: *const CdlTensor, k_cache: *const CdlTensor, v_cache: *const CdlTensor,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn cdl_b200_sample(
+        desc: *const CdlSampleDesc, logits: *const CdlTensor, uniform: *const CdlTensor,
+        temperature: *const CdlTensor, top_k: *const CdlTensor, top_p: *const CdlTensor,
+        min_p: *const CdlTensor, token: *const CdlTensor, logprob: *const CdlTensor,
+        stream: *mut c_void,
     ) -> i32;
 
     // ---- block-scaled tensors (MxTensor, crates/cleandl/src/mx_tensor.rs:11-30)
