@@ -70,7 +70,7 @@ def cache_plan(cached, added, block_table, free_pages, free_count, opts: CachePl
     check(packed_lib.cdl_b200_cache_plan(
         opts.page_size, opts.pages, tensor_bytes(cached), tensor_bytes(added), tensor_bytes(block_table),
         tensor_bytes(free_pages), tensor_bytes(free_count), *outputs, current_stream()))
-    return CachePlan(*block.split(sizes))
+    return CachePlan(*block.split_with_sizes(sizes))
 
 
 # --------------------------------------------------------------------------- the way into the cache
@@ -166,14 +166,14 @@ def sample(logits, uniform, opts: SampleOpts | None = None, logprob: bool = True
     opts = opts or SampleOpts()
     if logits.dim() != 2:
         raise _lib.CdlError(-1, "sample: logits must be [rows, vocab]")
-    all_rows, per_row = [0.0, 0, 1.0, 0.0], [None] * 4
-    _require_current_device(logits, uniform)
+    all_rows, per_row, given = [0.0, 0, 1.0, 0.0], [None] * 4, [logits, uniform]
     for i, x in enumerate((opts.temperature, opts.top_k, opts.top_p, opts.min_p)):
         if isinstance(x, torch.Tensor):
-            _require_current_device(x)
+            given.append(x)
             per_row[i] = tensor_bytes(x)
         else:
             all_rows[i] = x
+    _require_current_device(*given)
     rows, device = logits.shape[0], logits.device
     token, lp, tl = torch.empty(rows, dtype=torch.int32, device=device), None, None
     if logprob:
