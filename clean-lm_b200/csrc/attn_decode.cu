@@ -14,8 +14,9 @@
 // registers.  Where a warp's part cuts the keys of a (request, kv head), the warps of the CTA join what they have of it; what the
 // CTA's part cuts goes to the scratch, and a second kernel joins that.
 //
-// Short work is bound by latency instead: one request of some hundred keys and 16 heads takes 10.9 us, two launches and some dozen trips to memory
-// one after the other (lengths, page, keys, values, the partial results and back).
+// Short work is bound by latency instead, trips to memory one after the other (lengths, page, keys, values, results).  There each
+// (request, kv head) has a cluster of CTAs of its own, which join their results by way of shared memory: one request of some
+// hundred keys and 16 heads takes 7.6 us, 10.9 on the common line with its second kernel.
 //
 // Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
 // of mma.m16n8k16 (as rows they would leave at least half of it empty) and the pieces of K and V rows that a thread reads are its
@@ -25,6 +26,7 @@
 #include "ops.h"
 #include "ptx.cuh"
 
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -32,11 +34,20 @@
 namespace cdl {
 namespace decode {
 
+namespace cg = cooperative_groups;
+
 constexpr int WARPS = 4;         // of a CTA
 constexpr int STAGES = 2;        // tiles of a warp's ring
 // CTAs of an SM: as many as registers (168 of 12 warps, 255 of 8) and rings (70 KB each) allow; nt: tiles of 8 query columns
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int JOIN_WARPS = 8;    // of a CTA of the second kernel
+// Where no request sees more keys than this (by the width of its table, by the window), each line has CTAs of its own, as one long line
+// among short ones cannot take much longer than the rest.  (Own CTAs / shared ones, us, 16 heads of 128, requests of 1 to L keys:
+// L = 512: 1 request 7.2 / 10.8, 37 25 / 30, 256 106 / 126; 2048: 1 10.5 / 14.3, 16 40 / 38, 64 102 / 109; 4096: 1 14.6 / 15.9, 16
+// 75 / 61, 37 128 / 120.  24 heads on 2 of 64, L = 2048: 1 9.8 / 10.9, 256 49 / 53; 8192: 1 16.5 / 14.5.  Slower: 4096 lines of 1 to
+// 100 keys, 56 / 51.)
+constexpr int OWN_KEYS = 2048;
+constexpr int MAX_SPLIT = 8;     // CTAs of a line that has its own
 constexpr int MAX_BATCH = 4096;  // the prefix of the lengths is kept in shared memory beside the rings
 
 struct Params {
@@ -55,6 +66,7 @@ struct Params {
   long long out_sb, out_sh;
   float* lse;
   int set;          // CTAs that run at once
+  int split;        // CTAs of a line, where each has its own (a cluster)
   int* prefix;      // [batch + 1] tiles of the requests ahead
   float2* part_ml;  // [2 CTAs][COLS]
   float* part_o;    // [2 CTAs][COLS][D]
@@ -154,8 +166,9 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// D: head dimension; NT: tiles of 8 query heads of one kv head.
-template <int D, int NT>
+// D: head dimension; NT: tiles of 8 query heads of one kv head; OWN: a cluster of p.split CTAs has one line and joins what they have
+// of it by way of their shared memory (no second kernel, and nobody looks for its part).
+template <int D, int NT, bool OWN>
 __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kernel(const Params p) {
   constexpr int COLS = 8 * NT;
   constexpr int KEYS = tile_keys<D>();
@@ -169,52 +182,80 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
   int* prefix = reinterpret_cast<int*>(smem + WARPS * STAGES * STAGE);  // [batch + 1]
   __shared__ int warp_sum[WARPS];
   __shared__ Cuts<COLS> cuts;
+  __shared__ __align__(16) float own_o[OWN ? COLS * D : 4];  // what this CTA has of its line
+  __shared__ float2 own_ml[OWN ? COLS : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   if (tid < 2 * WARPS) cuts.line[tid] = -1;
   grid_dep_wait();
   grid_dep_launch();
 
-  // ---- the tiles ahead of each request
-  int run = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += WARPS * 32) {
-    const int b = b0 + tid;
-    int n = 0;
-    if (b < p.batch) {
-      int first, end;
-      visible(p, b, first, end);
-      n = static_cast<int>((static_cast<unsigned>(end - first) + (KEYS - 1)) / KEYS);
-    }
-    int x = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    if (lane == 31) warp_sum[warp] = x;
-    __syncthreads();
-    int before = run, all = run;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (b < p.batch) prefix[b] = before + x - n;
-    run = all;
-    __syncthreads();
-  }
-  if (tid == 0) prefix[p.batch] = run;
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= p.batch; b += WARPS * 32) p.prefix[b] = prefix[b];
-
   const int rows = p.kv_heads * p.chunks;  // lines of tiles of a request
-  const long long units = static_cast<long long>(run) * rows;
-  // this CTA's part, and this warp's of it
-  if (units == 0) return;
-  const Shares shares(units, p.set);
-  if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
-  const long long c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
+  // ---- this CTA's part of the line
+  long long c0 = 0, c1 = 0;
+  int own_b = 0, own_row = 0, own_n = 0;
+  const int own_rank = OWN ? static_cast<int>(blockIdx.x % p.split) : 0;
+  bool alone = true;  // one CTA has all of it
+  if constexpr (OWN) {
+    const int line = static_cast<int>(blockIdx.x / p.split);
+    own_b = line / rows, own_row = line - own_b * rows;
+    int first, end;
+    visible(p, own_b, first, end);
+    own_n = static_cast<int>((static_cast<unsigned>(end - first) + (KEYS - 1)) / KEYS);
+    c0 = static_cast<long long>(own_n) * own_rank / p.split, c1 = static_cast<long long>(own_n) * (own_rank + 1) / p.split;
+    alone = p.split == 1 || own_n <= 1;
+    if (own_n == 0) {
+      const int kvh = own_row / p.chunks, col0 = (own_row - kvh * p.chunks) * COLS, head0 = kvh * p.group + col0;
+      if (own_rank == 0)
+        for (int i = tid; i < min(COLS, p.group - col0) * (D / 8); i += WARPS * 32) {
+          const int head = head0 + i / (D / 8);
+          *reinterpret_cast<uint4*>(p.out + own_b * p.out_sb + head * p.out_sh + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+          if (p.lse != nullptr && i % (D / 8) == 0) p.lse[static_cast<long long>(own_b) * p.heads + head] = -INFINITY;
+        }
+      return;
+    }
+    if (tid < COLS) own_ml[tid] = make_float2(-INFINITY, 0.f);
+    __syncthreads();
+  } else {
+    // the tiles ahead of each request
+    int run = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += WARPS * 32) {
+      const int b = b0 + tid;
+      int n = 0;
+      if (b < p.batch) {
+        int first, end;
+        visible(p, b, first, end);
+        n = static_cast<int>((static_cast<unsigned>(end - first) + (KEYS - 1)) / KEYS);
+      }
+      int x = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (lane == 31) warp_sum[warp] = x;
+      __syncthreads();
+      int before = run, all = run;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += warp_sum[w];
+        all += warp_sum[w];
+      }
+      if (b < p.batch) prefix[b] = before + x - n;
+      run = all;
+      __syncthreads();
+    }
+    if (tid == 0) prefix[p.batch] = run;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = tid; b <= p.batch; b += WARPS * 32) p.prefix[b] = prefix[b];
+
+    const long long units = static_cast<long long>(run) * rows;
+    if (units == 0) return;
+    const Shares shares(units, p.set);
+    if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
+    c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
+  }
   // Warps with a part, of one tile or more.  (Of 4 tiles or more, so that some had none, a short context took 12.6 us, not 10.9.)
   const long long busy = min(static_cast<long long>(WARPS), c1 - c0);
   long long u = 0, u_end = 0;
@@ -225,6 +266,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
     int b, row, tile, n;
   };
   auto place_of = [&](long long x) {
+    if constexpr (OWN) return Place{own_b, own_row, static_cast<int>(x), own_n};
     Place at;
     const int ahead = static_cast<int>(static_cast<double>(x) / rows);  // (exact: x < 2^40, rows < 2^17)
     int lo = 0, hi = p.batch;
@@ -533,12 +575,50 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attn_decode_kerne
             make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
         if (p.lse != nullptr && d == 0)
           p.lse[static_cast<long long>(b) * p.heads + head0 + col] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+      } else if constexpr (OWN) {
+        *reinterpret_cast<float4*>(own_o + col * D + d) = sum;
+        if (d == 0) own_ml[col] = make_float2(top, l);
       } else {
         const long long slot = (2LL * blockIdx.x + (cuts.starts[e0] != 0)) * COLS + col;
         *reinterpret_cast<float4*>(p.part_o + slot * D + d) = sum;
         if (d == 0) p.part_ml[slot] = make_float2(top, l);
       }
     }
+  }
+  if constexpr (OWN) {
+    if (alone) return;
+    // ---- and what the CTAs have of it
+    const cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int kvh = own_row / p.chunks, col0 = (own_row - kvh * p.chunks) * COLS, head0 = kvh * p.group + col0;
+    const int cols = min(COLS, p.group - col0);
+    for (int i = own_rank * WARPS * 32 + tid; i < cols * (D / 4); i += p.split * WARPS * 32) {
+      const int col = i / (D / 4), d = i % (D / 4) * 4;
+      float2 ml[MAX_SPLIT];
+      float4 x[MAX_SPLIT];
+      float top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c) {
+        ml[c] = c < p.split ? *cluster.map_shared_rank(&own_ml[col], c) : make_float2(-INFINITY, 0.f);
+        // (a CTA without a tile has no output there)
+        x[c] = ml[c].x == -INFINITY && ml[c].y == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                      : *reinterpret_cast<const float4*>(cluster.map_shared_rank(own_o + col * D + d, c));
+        top = fmaxf(top, ml[c].x);
+      }
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c) {
+        const float f = ml[c].x == -INFINITY ? (ml[c].y == 0.f ? 0.f : 1.f) : ex2(ml[c].x - top);  // (1: NaN, which stays)
+        l += f * ml[c].y;
+        sum.x += f * x[c].x, sum.y += f * x[c].y, sum.z += f * x[c].z, sum.w += f * x[c].w;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(p.out + own_b * p.out_sb + (head0 + col) * p.out_sh + d) =
+          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+      if (p.lse != nullptr && d == 0)
+        p.lse[static_cast<long long>(own_b) * p.heads + head0 + col] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+    }
+    cluster.sync();  // (nobody's shared memory goes while it is read)
   }
 }
 
@@ -769,12 +849,29 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   p.warp_o = reinterpret_cast<float*>(at);
 
   ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
-  void (*kernel)(decode::Params) = D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1> : decode::attn_decode_kernel<128, 2>)
-                                            : (nt == 1 ? decode::attn_decode_kernel<64, 1> : decode::attn_decode_kernel<64, 2>);
+  const size_t rings = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>());
+  const long long lines = B * rows;
+  if (most <= decode::OWN_KEYS) {
+    void (*own)(decode::Params) =
+        D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1, true> : decode::attn_decode_kernel<128, 2, true>)
+                 : (nt == 1 ? decode::attn_decode_kernel<64, 1, true> : decode::attn_decode_kernel<64, 2, true>);
+    // CTAs of a line: a tile or more for each warp, and 7/8 of the places, which clusters do not fill (74 lines of 512 keys in 3 CTAs
+    // each 10.2 us; in 4, one for each of 296 places, 14.5)
+    const long long line_tiles = (most + tile - 1) / tile;
+    p.split = static_cast<int>(std::max<long long>(
+        1, std::min<long long>({decode::MAX_SPLIT, set * 7LL / 8 / lines, (line_tiles + decode::WARPS - 1) / decode::WARPS})));
+    CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(own), static_cast<int>(rings)));
+    const dim3 of_lines(static_cast<unsigned>(lines * p.split)), block(decode::WARPS * 32);
+    CDL_CUDA(p.split == 1 ? launch_pdl(own, of_lines, block, rings, stream, p)
+                          : launch_pdl_cluster(own, of_lines, block, rings, p.split, stream, p));
+    return CDL_OK;
+  }
+  void (*kernel)(decode::Params) =
+      D == 128 ? (nt == 1 ? decode::attn_decode_kernel<128, 1, false> : decode::attn_decode_kernel<128, 2, false>)
+               : (nt == 1 ? decode::attn_decode_kernel<64, 1, false> : decode::attn_decode_kernel<64, 2, false>);
   void (*join)(decode::Params, int) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
-  const size_t smem = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>()) +
-                      (B + 1) * sizeof(int);
+  const size_t smem = rings + (B + 1) * sizeof(int);
   CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
   // items of a CTA: one while there are few, up to one per warp

@@ -239,12 +239,23 @@ def decode_inputs(lens, heads, kv_heads, dim, page_size, layout="packed", seed=0
 def check_decode(cdl, q, k, v, table, lens, scale=None, softcap=0.0, window=0, **more):
     opts = cdl.serve.AttentionDecodeOpts(softmax_scale=scale, softcap=softcap, window=window)
     got = cdl.serve.attention_decode(q, k, v, table, lens, opts, lse=True, **more)
+    others = []
+    if 0 < table.shape[1] * k.shape[1] <= 2048 and not more:  # the form for longer ones too: entries that no request reaches
+        wide = torch.full((len(lens), 2048 // k.shape[1] + 2), -1, dtype=I32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        others.append(cdl.serve.attention_decode(q, k, v, wide, lens, opts, lse=True))
     out, lse, spread, reach = serve_ref.attention_decode(f64(q), f64(k), f64(v), table.cpu().numpy(), lens.cpu().numpy(), scale,
                                                          softcap, window)
     n, dim = int(lens.max().clamp(min=1)), q.shape[2]
     # a score's roundings: of the sum of dim products, of the scale and the cap; the exponential's
     off = (dim + 8) * 2.0 ** -24 * reach + 2.0 ** -20
     bound = 2.0 ** -8 * (np.abs(out) + spread) + 2 * off[..., None] * spread + n * 2.0 ** -24 * spread
+    for x in [got] + others:
+        _check_decoded(x, out, lse, bound, off, n)
+    return got
+
+
+def _check_decoded(got, out, lse, bound, off, n):
     have, have_lse = f64(got.out), f64(got.lse)
     assert np.array_equal(np.isnan(have_lse), np.isnan(lse)) and np.array_equal(np.isneginf(have_lse), np.isneginf(lse))
     dead = np.isnan(lse)
@@ -254,7 +265,6 @@ def check_decode(cdl, q, k, v, table, lens, scale=None, softcap=0.0, window=0, *
     assert worst.size == 0 or worst.max() <= 1, worst.max()
     lse_bound = off + n * 2.0 ** -24 + 2.0 ** -22 * np.abs(np.where(fine, lse, 0))
     assert (np.abs(have_lse - lse)[fine] <= lse_bound[fine]).all()
-    return got
 
 
 @gpu
@@ -299,6 +309,47 @@ def test_decode_window_and_cap(cdl, gpu_ok, window, softcap):
     inputs = decode_inputs([1, 33, 500, 0, 1300], 6, 2, 128, 16, seed=window, lean=2.0)
     check_decode(cdl, *inputs, window=window, softcap=softcap)
     check_decode(cdl, *inputs, window=window, softcap=softcap, scale=0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,heads,kv_heads", [(1, 1, 1), (1, 20, 2), (7, 4, 4), (16, 12, 3), (20, 16, 4), (33, 4, 4), (99, 2, 2), (205, 2, 2)])
+def test_decode_short_lines(cdl, gpu_ok, dim, batch, heads, kv_heads):
+    """Requests of at most 2048 keys, whose lines have 1 to 8 CTAs each; some with fewer keys than those have warps, some with none."""
+    lens = [(2047, 0, 1, 15, 17, 33, 129, 500, 0, 64)[b % 10] + b // 10 for b in range(batch)]
+    check_decode(cdl, *decode_inputs(lens, heads, kv_heads, dim, 16, seed=batch))
+
+
+@gpu
+@pytest.mark.parametrize("window", [2047, 2048, 2049, 3001])
+def test_decode_long_windows(cdl, gpu_ok, window):
+    check_decode(cdl, *decode_inputs([5000, 100, 2600, 0, 2049, 2048], 6, 2, 128, 16, seed=window, lean=2.0), window=window, softcap=30.0)
+
+
+@gpu
+def test_decode_short_lines_captured(cdl, gpu_ok):
+    """Graphs of calls of two widths on one stream, replayed beside one another on two, on new lengths."""
+    made, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    inputs = [decode_inputs([900, 17, 2000, 300], 8, 2, 128, 16, seed=30 + i) for i in range(2)]
+    inputs[1] = (*inputs[1][:3], torch.cat([inputs[1][3], inputs[1][3] * 0 - 1], 1), inputs[1][4])
+    torch.cuda.synchronize()
+    for x in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            made.append((graph, cdl.serve.attention_decode(*x, lse=True)))
+    for lens in ([900, 17, 2000, 300], [0, 2000, 1, 44]):
+        for x in inputs:
+            x[4].copy_(ints(lens))
+        want = [cdl.serve.attention_decode(*x, lse=True) for x in inputs]
+        torch.cuda.synchronize()
+        for st, (graph, _) in zip(streams, made):
+            with torch.cuda.stream(st):
+                for _ in range(5):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for w, (_, got) in zip(want, made):
+            # (bits: keys behind a request's first length are NaN, which the second one's reaches)
+            assert torch.equal(got.out.view(torch.int16), w.out.view(torch.int16)) and torch.equal(got.lse.view(I32), w.lse.view(I32))
 
 
 @gpu
