@@ -155,6 +155,22 @@ struct Row {
       f(x, i);
     }
   }
+  // The same, all of it at once.
+  template <typename F>
+  static __device__ __forceinline__ void fours_at_once(const uint4& q, int i, F f) {
+    if constexpr (N == 8) {
+      uint32_t a = q.x, b = q.y;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x[4] = {bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b)};
+        f(x, i + 4 * h);
+        a = q.z, b = q.w;
+      }
+    } else {
+      const float x[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+      f(x, i);
+    }
+  }
 };
 
 // floor(f n) for f of [0, 1), and whether something is left over: with f = m 2^-s and a product of 128 bits, so that the half of
@@ -796,12 +812,19 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         // not hold more.  (Whether the window holds the cut is checked by exact sums.)
         const float all = static_cast<float>(m.all), target = set.top_p * all;
         const float margin = fminf(all * (1.f / 256), 4 * 0.0031f * sqrtf(squares));
+        u64 wanted[6];
+#pragma unroll
+        for (int t = 0; t < 6; ++t) {
+          const float reach = t < 2 ? margin : t < 4 ? margin * 0.25f : 0.f;
+          wanted[t] = max(u64{1}, static_cast<u64>(fmaxf(0.f, fminf(all, t & 1 ? target + reach : target - reach))));
+        }
+        const bool has_edge = m.before < wanted[1] && m.before + mass >= wanted[0];  // (all of them lie among these two)
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
+          if (!has_edge) break;
 #pragma unroll
           for (int t = 0; t < 6; ++t) {
-            const float reach = t < 2 ? margin : t < 4 ? margin * 0.25f : 0.f;
-            const u64 want = max(u64{1}, static_cast<u64>(fmaxf(0.f, fminf(all, t & 1 ? target + reach : target - reach))));
+            const u64 want = wanted[t];
             if (m.before < want && m.before + about[j] >= want) {
               sh.edge[t] = tid * PER + j;
               sh.ahead_of[t] = static_cast<uint32_t>(n.before + (t & 1 ? count[j] : 0));
@@ -819,17 +842,19 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const Shared& o = of(0);
     mode = static_cast<Mode>(o.mode);
     const bool window = mode == WINDOW_P || mode == WINDOW_K || mode == LIST;
-    if (window && tid < 2) {  // (two threads: all of them doing it took 4900 cycles)
+    if (window && warp < 2) {  // (a warp each, 32 keys at a time: by halves, in one thread, 3900 cycles)
       // the least logits of the bins up to lo - 1 and up to hi: the logits below have larger bins
-      const int last = tid == 0 ? o.lo - 1 : o.hi;
+      const int last = warp == 0 ? o.lo - 1 : o.hi;
       uint32_t below = KEY_NONE, from = last < 0 ? KEY_NONE + 1 : key_of(top);
 #pragma unroll 1
       while (from - below > 1) {
-        const uint32_t mid = below + (from - below) / 2;
-        if (bin(of_key(mid)) <= last) from = mid;
-        else below = mid;
+        const uint32_t part = (from - below) / 32 + 1, mid = below + min(part * (lane + 1), from - below);
+        const uint32_t low_bins = __ballot_sync(0xffffffffu, bin(of_key(mid)) <= last);  // (from itself among them: its bin is)
+        const int first_of = __ffs(low_bins) - 1;  // of the lanes
+        from = __shfl_sync(0xffffffffu, mid, first_of);
+        if (first_of > 0) below = __shfl_sync(0xffffffffu, mid, first_of - 1);
       }
-      sh.least_of[tid] = last < 0 ? key_of(INFINITY) : from;
+      if (lane == 0) sh.least_of[warp] = last < 0 ? key_of(INFINITY) : from;
     }
     __syncthreads();
     if (window) over = of_key(sh.least_of[0]), bound = sh.least_of[1], low = of_key(bound);
@@ -874,7 +899,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         const bool ends = ++in == per_lane;
         next = ends ? load(tile + WARPS, 0) : load(tile, in);
         if (__any_sync(0xffffffffu, Row<T>::top(now) >= least))  // (by whole warps: lanes that part here would go on apart)
-          Row<T>::fours(now, row.first(v), [&](const float (&x)[4], int i) { f(x, i, sum); });
+          Row<T>::fours_at_once(now, row.first(v), [&](const float (&x)[4], int i) { f(x, i, sum); });
         if (ends) {
           sum = warp_sum(sum);
           if (lane == 0) sh.tile[tile] = sum;
