@@ -13,8 +13,8 @@
 // is large or top_p is on, for a histogram, which gives a bound that the kept entries reach or a window that the cut lies in; and
 // for the candidates, the sums of whole tiles and, around the cut, the entries on a list in shared memory.  The rest is that list
 // and one tile.  What bounds it is instructions and barriers, not memory: 148 rows of 32768 bf16 logits (1.5 us at 6.56 TB/s) take
-// 5.4 us for the largest, 12.3 for top_k of 50, 15.2 for an unrestricted draw (all weights, in f64) and 31.7 for top_p of 0.9 (a
-// histogram and all weights); one row in two CTAs 4.5, 11.0, 11.1 and 25.
+// 5.3 us for the largest, 11.5 for top_k of 50, 14.0 for an unrestricted draw (all weights, in f64) and 29.2 for top_p of 0.9 (a
+// histogram and all weights); one row in two CTAs 4.6, 10.8, 10.2 and 23.
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -36,7 +36,7 @@ constexpr int BIN_PER = 64;
 constexpr int TILES = 1024;  // of a row, whose sums are kept
 constexpr int SMALL = THREADS;  // entries of a list that are each held against all others (100 to 256, the rest sorted: no faster)
 // A CTA's part of top_k up to which a bound from its threads' largest logits finds the candidates.  (Bound / histogram, us, 148
-// rows of 32768: top_k of 50 12.3 / 17.6, 100 14.2 / 19.0, 300 30 / 31; of 150001: 50 26 / 81, 300 59 / 94.)
+// rows of 32768: top_k of 50 11.9 / 17.0, 100 13.5 / 18.2, 300 29.4 / 30.6; of 150001: 50 29 / 51, 300 51 / 68.)
 constexpr int LIST_K = 384;
 
 struct Params {
@@ -1112,13 +1112,14 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   while ((1LL << bits) < V) ++bits;
   p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
-  // CTAs of a row, of 16384 logits each or more: 4 or 3 where larger clusters find an SM for each (7/8 of them), 4 to two SMs where
-  // rows are long, pairs where each finds an SM.  (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us, from HBM: 150001 f32 logits, 16 rows 94,
-  // 58, 46, 39, in 6 and 8 slower; 37 rows 96, 59, 48, 58; 48 rows 98, 61, 69, 59, with what L2 holds of them 73 in 2, 61 in 4; 74
-  // rows 110, 68, 72, 88; 100 rows 120, 98, 111, 94.  65536: 48 rows 48, 35, 42, 37; 100 rows 53, 51, 66, 68.  32768 bf16: 16
-  // rows 30, 26, 25, 23, 100 rows 32, 36, 52, 54.)
+  // CTAs of a row, of 16384 logits each or more: 4 or 3 where such clusters find an SM for each (7/8 of them), pairs where those do;
+  // two to an SM where rows are long.  (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us, from HBM: 150001 f32 logits, 16 rows 93, 57, 45,
+  // 38, in 6 and 8 slower; 37 rows 94, 58, 47, 56; 48 rows 97, 60, 67, 57, with what L2 holds of them 120, 73, 70, 59; 74 rows 108,
+  // 66, 70, 86; 148 rows 125, 105, 136, 134.  65536: 48 rows 47, 34, 40, 35; 148 rows 57, 52, 75, 83, with top_k of 50 21, 21.
+  // 32768 bf16: 16 rows 28, 24, 23, 22; 100 rows 29, 33, 49, 49.)
   const long long sms = sm_count(), own_sm = sms * 7 / 8 / R;
-  const long long fit = own_sm >= 3 ? own_sm : V >= 131072 && 4 * R <= sms * 7 / 4 ? 4 : 2 * R <= sms ? 2 : 1;
+  const bool long_rows = V >= 131072;
+  const long long fit = own_sm >= 3 ? own_sm : long_rows && 4 * R <= sms * 7 / 4 ? 4 : 2 * R <= (long_rows ? 2 * sms : sms) ? 2 : 1;
   p.cluster = static_cast<int>(std::max<long long>(1, std::min<long long>({4, fit, V / 16384})));
   void (*kernel)(sample::Params) = logits->dtype == CDL_BF16 ? sample::sample_kernel<__nv_bfloat16> : sample::sample_kernel<float>;
   const int smem = static_cast<int>(sizeof(sample::Shared));

@@ -579,9 +579,9 @@ def test_sample_of_an_infinite_temperature(cdl, gpu_ok, vocab):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [3, 40, 70, 80])
-def test_sample_rows_shared_by_several_ctas(cdl, gpu_ok, rows):
-    z, u = logits_of(rows, 66001, BF16, seed=rows)
+@pytest.mark.parametrize("rows,vocab", [(3, 66001), (40, 66001), (70, 66001), (80, 66001), (50, 140001), (90, 140001)])
+def test_sample_rows_shared_by_several_ctas(cdl, gpu_ok, rows, vocab):
+    z, u = logits_of(rows, vocab, BF16, seed=rows)
     check_sample(cdl, z, u)
     check_sample(cdl, z, u, top_p=0.9)
     check_sample(cdl, z, u, top_k=50)
