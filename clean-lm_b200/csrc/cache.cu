@@ -9,8 +9,8 @@ namespace cache {
 
 // ---------------------------------------------------------------- plan
 // Per request b, with c = cached, a = added (negative: 0) and P = page_size:
-//   E_b = sum of a up to b;  need_b = pages(c + a) - pages(c), 0 where the request does not fit (its table row is too short or
-//   E_b > rows);  C_b = sum of need up to b;  served_b = fits and (need_b == 0 or C_b <= free)
+//   E_b = sum of a up to b;  need_b = pages(c + a) - pages(c), 0 where the request does not fit (its table row is too short,
+//   E_b > rows or c + a > 2^31 - 1);  C_b = sum of need up to b;  served_b = fits and (need_b == 0 or C_b <= free)
 // Served requests with need take stack[free - C_b ..], in the order of the requests: the served ones with need are the first
 // ones with it, as C only grows.
 // Bound by latency: one kernel, in which every CTA sums the lengths up itself (1024 requests at a time) and then takes its
@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   grid_dep_launch();
   const long long P = p.page_size;
   const long long free = min(max(*p.free_count, 0), p.stack);
+  const long long longest = min(p.width * P, static_cast<long long>(INT32_MAX));  // (a table may name a page twice: more keys than slots)
   const int share = blockIdx.x * THREADS + tid, step = gridDim.x * THREADS;
   long long rows_before = 0, pages_before = 0, left = free;
   // sums of x and y over the threads ahead of this one (exclusive), and over all
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     for (int i = 0; i < PER; ++i) {
       e += a[i];
       end[i] = e;
-      fits[i] = c[i] + a[i] <= p.width * P && e <= p.rows;
+      fits[i] = c[i] + a[i] <= longest && e <= p.rows;
       need[i] = fits[i] ? (c[i] + a[i] + P - 1) / P - (c[i] + P - 1) / P : 0;
       pages += need[i];
     }

@@ -51,8 +51,8 @@ def cache_plan(cached, added, block_table, free_pages, free_count, opts: CachePl
     """Pages, positions and slots of `added` (i32 [requests]) new tokens for requests with `cached` ones.
 
     Pages come off the end of the stack free_pages[:free_count], in the order of the requests, into `block_table` (i32
-    [requests, pages of a request], written in place).  A request that does not get its pages, or whose table row or rows of
-    the batch do not suffice, is not served: its tokens have slot -1 and its seq_lens stays at `cached`."""
+    [requests, pages of a request], written in place).  A request that does not get its pages, whose table row or rows of the
+    batch do not suffice, or that would be longer than 2^31 - 1, is not served: its tokens have slot -1 and its seq_lens stays at `cached`."""
     _require_current_device(cached, added, block_table, free_pages, free_count)
     rows = opts.rows
     if rows < 0:

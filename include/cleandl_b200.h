@@ -468,9 +468,9 @@ int32_t cdl_b200_attn_decode_scratch_bytes(const cdl_tensor* q, const cdl_tensor
  * slots.  With c = cached[b] tokens in the cache, a = added[b] new ones (negative: 0) and E_b the sum of a up to b:
  *   need_b = ceil((c + a) / page_size) - ceil(c / page_size) pages, C_b the sum of them up to b
  * in the order of the requests, which take free_pages[free_count - 1], free_pages[free_count - 2], ..  A request is not served
- * if its pages would go past block_table's width or its rows past `rows`, or if it needs pages and C_b > free_count: its
- * tokens get no slot, seq_lens[b] stays c and no page is taken for it (after one that the stack does not suffice for, only
- * requests that need none are served).
+ * if its pages would go past block_table's width, its rows past `rows` or c + a past 2^31 - 1, or if it needs pages and
+ * C_b > free_count: its tokens get no slot, seq_lens[b] stays c and no page is taken for it (after one that the stack does not
+ * suffice for, only requests that need none are served).  Positions past 2^31 - 1 are given as that number.
  *   block_table i32 [requests, width], contiguous rows: entries of pages in use are read, new ones written
  *   seq_lens [requests]: c + a, c if not served;  cu_seqlens [requests + 1]: 0 and E_b, at most rows
  *   positions, slots [rows]: rows cu_seqlens[b] .. cu_seqlens[b + 1] are request b's new tokens, at positions c, c + 1, ..;

@@ -16,7 +16,7 @@ def cache_plan(cached, added, table, stack, free, page_size, pages, rows):
     for b, (c, a) in enumerate(zip(cached, added)):
         c, a = max(c, 0), max(a, 0)
         end += a
-        fits = c + a <= len(table[b]) * page_size and end <= rows
+        fits = c + a <= min(len(table[b]) * page_size, 2 ** 31 - 1) and end <= rows
         need = count(c + a) - count(c) if fits else 0
         asked += need
         served = fits and (need == 0 or asked <= free)

@@ -1,0 +1,30 @@
+"""Calls of the serving operators (cdl.serve) at the ends of what they take, against their definitions in 64 bits (oracle/serve_ref.py),
+and what they refuse there."""
+import pytest
+import torch
+
+from oracle import serve_ref
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+gpu = pytest.mark.gpu
+
+
+def ints(x):
+    return torch.tensor(x, dtype=I32, device="cuda")
+
+
+# --------------------------------------------------------------------------- lengths
+@gpu
+def test_plan_of_lengths_around_2_31(cdl, gpu_ok):
+    """A table that names pages again and again has room for more keys than 32 bits count: a request that would pass 2^31 - 1 is not
+    served, whether it needs a page for that or not, and the one behind it is."""
+    page_size, width, pages, big = 1 << 20, 2049, 1500, 2 ** 31 - 1
+    table, stack = [[5] * 2048 + [-1]] * 6, [1, 2, 3]
+    cached, added = [big - 1, big - 1, big, big - 3, big, 3], [1, 2, 3, 3, 0, 1]
+    t = ints(table)
+    got = cdl.serve.cache_plan(ints(cached), ints(added), t, ints(stack), ints([3]), cdl.serve.CachePlanOpts(page_size, pages, 12))
+    want = serve_ref.cache_plan(cached, added, table, stack, 3, page_size, pages, 12)
+    assert want[0] == [big, big - 1, big, big, big, 4]
+    have = (got.seq_lens, got.cu_seqlens, got.positions, got.slots, got.free_left, t)
+    for name, g, w in zip(("seq_lens", "cu_seqlens", "positions", "slots", "free_left", "block_table"), have, want):
+        assert g.tolist() == ([w] if name == "free_left" else w), name
