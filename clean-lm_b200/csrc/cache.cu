@@ -402,6 +402,7 @@ int32_t cache_write_execute(const cdl_tensor* q, const cdl_tensor* k, const cdl_
         cos_sin->shape[0] > INT32_MAX || cos_sin->stride[1] != 1 || (cos_sin->shape[0] > 1 && cos_sin->stride[0] != D) ||
         (reinterpret_cast<uintptr_t>(cos_sin->ptr) & 15))
       return fail(CDL_ERR_INVALID, "%s: cos_sin must be packed f32 [positions, head_dim], 16-byte aligned", op);
+    if (T > 0 && cos_sin->shape[0] > 0 && !cos_sin->ptr) return fail(CDL_ERR_INVALID, "%s: null pointer (cos_sin)", op);
   }
   const cdl_tensor* caches[] = {k_cache, v_cache};
   for (const cdl_tensor* c : caches) {
@@ -411,6 +412,7 @@ int32_t cache_write_execute(const cdl_tensor* q, const cdl_tensor* k, const cdl_
     if (!ok)
       return fail(CDL_ERR_INVALID, "%s: the caches must be bf16 [pages, page_size, kv_heads %lld, head_dim %lld] of one shape with a "
                   "contiguous last dimension and 16-byte aligned strides", op, Hkv, D);
+    if (T > 0 && c->shape[0] > 0 && Hkv > 0 && !c->ptr) return fail(CDL_ERR_INVALID, "%s: null pointer (a cache)", op);
     if (!view_apart_from_itself(*c)) return fail(CDL_ERR_INVALID, "%s: elements of a cache overlap", op);
   }
   if (k_cache->shape[1] > INT32_MAX || k_cache->shape[0] > INT32_MAX / k_cache->shape[1])

@@ -28,3 +28,40 @@ def test_plan_of_lengths_around_2_31(cdl, gpu_ok):
     have = (got.seq_lens, got.cu_seqlens, got.positions, got.slots, got.free_left, t)
     for name, g, w in zip(("seq_lens", "cu_seqlens", "positions", "slots", "free_left", "block_table"), have, want):
         assert g.tolist() == ([w] if name == "free_left" else w), name
+
+
+# --------------------------------------------------------------------------- refusals (no GPU: operands are checked first)
+def status(cdl, name, *args):
+    L = cdl._lib
+    given = [L.tensor_bytes(a) if isinstance(a, torch.Tensor) else a for a in args]
+    return getattr(L.packed_lib, name)(*given, None), L.last_error()
+
+
+def swap(args, i, x):
+    return [x if j == i else a for j, a in enumerate(args)]
+
+
+def bf(*shape):
+    return torch.zeros(*shape, dtype=BF16)
+
+
+def i32(*shape):
+    return torch.zeros(*shape, dtype=I32)
+
+
+def null(cdl, t):
+    """A tensor's shape and strides without memory, as a C caller may give them."""
+    return bytes(8) + cdl._lib.tensor_bytes(t)[8:]
+
+
+def test_write_refuses_null_pointers(cdl):
+    # q, k, v, cos_sin, positions, slots, q_out, k_out, k_cache, v_cache
+    good = [bf(5, 4, 32), bf(5, 2, 32), bf(5, 2, 32), torch.zeros(8, 32), i32(5), i32(5), bf(5, 4, 32), bf(5, 2, 32), bf(3, 4, 2, 32),
+            bf(3, 4, 2, 32)]
+    for i, t in enumerate(good):
+        st, text = status(cdl, "cdl_b200_cache_write", *swap(good, i, null(cdl, t)))
+        assert st == -1 and ("null pointer" in text or "must" in text), (i, st, text)
+    # nothing to store to, nothing to rotate: no memory is needed
+    none = [t[:0] if i < 8 and i != 3 else t for i, t in enumerate(good)]
+    for i in (3, 8, 9):
+        assert status(cdl, "cdl_b200_cache_write", *swap(none, i, null(cdl, good[i])))[0] == 0
