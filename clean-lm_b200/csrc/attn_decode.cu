@@ -805,7 +805,7 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   for (const void* x : given)
     if (!x) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
   const long long width = pages == 0 ? 0 : block_table->shape[1];
-  if (width > 0 && (!block_table->ptr || !k_cache->ptr || !v_cache->ptr)) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
+  if ((lse && !lse->ptr) || (width > 0 && (!block_table->ptr || !k_cache->ptr || !v_cache->ptr))) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
   if (!view_apart_from_itself(*out)) return fail(CDL_ERR_INVALID, "%s: elements of out overlap", op);
   const cdl_tensor* ins[] = {q, k_cache, v_cache, block_table, seq_lens};
   for (const cdl_tensor* i : ins)

@@ -65,3 +65,18 @@ def test_write_refuses_null_pointers(cdl):
     none = [t[:0] if i < 8 and i != 3 else t for i, t in enumerate(good)]
     for i in (3, 8, 9):
         assert status(cdl, "cdl_b200_cache_write", *swap(none, i, null(cdl, good[i])))[0] == 0
+
+
+def decode_call(cdl):
+    """desc, q, k_cache, v_cache, block_table, seq_lens, out, lse, scratch, bytes of a call that is in order."""
+    buf = torch.zeros(1024, dtype=torch.uint8)
+    at = (buf.data_ptr() + 255) // 256 * 256  # (its contents are never reached)
+    return [cdl._lib.attn_decode_bytes(0.0, 0.0, 0), bf(3, 4, 64), bf(5, 16, 2, 64), bf(5, 16, 2, 64), i32(3, 2), i32(3), bf(3, 4, 64),
+            torch.zeros(3, 4), at, 1 << 40]
+
+
+def test_decode_refuses_null_pointers(cdl):
+    good = decode_call(cdl)
+    for i in range(1, 8):
+        st, text = status(cdl, "cdl_b200_attn_decode", *swap(good, i, null(cdl, good[i])))
+        assert st == -1 and "null pointer" in text, (i, st, text)
