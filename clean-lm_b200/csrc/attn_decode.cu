@@ -746,7 +746,7 @@ static int32_t decode_shapes(const char* op, const cdl_tensor* q, const cdl_tens
   if (k_cache->shape[3] != d) return fail(CDL_ERR_INVALID, "%s: head_dim of q and of the cache differ", op);
   if (q->shape[0] < 0 || q->shape[0] > decode::MAX_BATCH)
     return fail(CDL_ERR_UNSUPPORTED, "%s: at most %d requests (got %lld)", op, decode::MAX_BATCH, (long long)q->shape[0]);
-  if (k_cache->shape[2] <= 0 || q->shape[1] % k_cache->shape[2] != 0)
+  if (q->shape[1] < 0 || k_cache->shape[2] <= 0 || q->shape[1] % k_cache->shape[2] != 0)
     return fail(CDL_ERR_INVALID, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", op, (long long)q->shape[1],
                 (long long)k_cache->shape[2]);
   if (q->shape[1] > 65536) return fail(CDL_ERR_UNSUPPORTED, "%s: at most 65536 heads", op);

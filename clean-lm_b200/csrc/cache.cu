@@ -306,7 +306,7 @@ static bool same_view(const cdl_tensor& a, const cdl_tensor& b) {
 }
 
 static int32_t check_ints(const char* op, const char* name, const cdl_tensor* t, long long n) {
-  if (!t || t->rank != 1 || t->dtype != CDL_I32 || t->shape[0] != n || (n > 1 && t->stride[0] != 1) || (n > 0 && !t->ptr))
+  if (!t || t->rank != 1 || t->dtype != CDL_I32 || n < 0 || t->shape[0] != n || (n > 1 && t->stride[0] != 1) || (n > 0 && !t->ptr))
     return fail(CDL_ERR_INVALID, "%s: %s must be a packed i32 vector of %lld", op, name, n);
   return CDL_OK;
 }

@@ -80,3 +80,35 @@ def test_decode_refuses_null_pointers(cdl):
     for i in range(1, 8):
         st, text = status(cdl, "cdl_b200_attn_decode", *swap(good, i, null(cdl, good[i])))
         assert st == -1 and "null pointer" in text, (i, st, text)
+
+
+def sized(cdl, t, *shape):
+    """A tensor's memory and strides with sizes that a C caller may give."""
+    x = cdl._lib.CdlTensor.from_buffer_copy(cdl._lib.tensor_bytes(t))
+    x.shape[:len(shape)] = shape
+    return bytes(x)
+
+
+def test_negative_sizes_are_refused(cdl):
+    """(A negative number of heads came to a division by zero on the host.)"""
+    L, good = cdl._lib, decode_call(cdl)
+    heads = swap(swap(swap(good, 1, sized(cdl, good[1], 3, -2, 64)), 6, sized(cdl, good[6], 3, -2, 64)), 7, None)
+    st, text = status(cdl, "cdl_b200_attn_decode", *heads)
+    assert st == -1 and "multiple" in text
+    n = L.ctypes.c_size_t(0)
+    assert L.packed_lib.cdl_b200_attn_decode_scratch_bytes(heads[1], L.tensor_bytes(good[2]), L.ctypes.byref(n)) == -1
+    plan = [16, 9, i32(4), i32(4), i32(4, 3), i32(9), i32(1), i32(4), i32(5), i32(7), i32(7), i32(1)]
+    for i in range(2, 12):
+        st, text = status(cdl, "cdl_b200_cache_plan", *swap(plan, i, sized(cdl, plan[i], -3)))
+        assert st == -1 and "must be" in text, (i, st, text)
+    write = [bf(5, 4, 32), bf(5, 2, 32), bf(5, 2, 32), torch.zeros(8, 32), i32(5), i32(5), bf(5, 4, 32), bf(5, 2, 32), bf(3, 4, 2, 32),
+             bf(3, 4, 2, 32)]
+    sample = [L.sample_bytes(1.0, 0, 1.0, 0.0), torch.zeros(4, 50), torch.zeros(4), torch.zeros(4), i32(4), torch.zeros(4), torch.zeros(4),
+              i32(4), torch.zeros(4)]
+    for name, args in (("cdl_b200_attn_decode", good), ("cdl_b200_cache_write", write), ("cdl_b200_sample", sample)):
+        for i, t in enumerate(args):
+            for d in range(t.dim() if isinstance(t, torch.Tensor) else 0):
+                shape = list(t.shape)
+                shape[d] = -shape[d]
+                st, text = status(cdl, name, *swap(args, i, sized(cdl, t, *shape)))
+                assert st in (-1, -2), (name, i, d, st, text)
