@@ -28,6 +28,14 @@ def _require_cuda(*tensors):
             raise _lib.CdlError(-1, "operands must live in device memory (there is no CPU path)")
 
 
+def _scratch_args(scratch):
+    """Address and bytes of a scratch; of a strided or expanded view the library would use memory that the view does not name."""
+    _require_cuda(scratch)
+    if not scratch.is_contiguous():
+        raise _lib.CdlError(-1, "scratch must be contiguous")
+    return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+
+
 # --------------------------------------------------------------------------- matmul
 @dataclass
 class MatmulOpts:
@@ -166,11 +174,9 @@ def norm_bwd(x, dy, scale, r_inv, dscale, residual_dy=None, scratch=None, dx=Non
     if variant != _lib.NORM_AUTO:
         no = _lib.CdlNormOptions(int(variant))
         check(packed_lib.cdl_b200_rmsnorm_bwd_opt(*(ref(a) for a in args), ctypes.byref(no),
-                                           ctypes.c_void_p(scratch.data_ptr()),
-                                           scratch.numel() * scratch.element_size(), current_stream()))
+                                           *_scratch_args(scratch), current_stream()))
         return dx
-    check(packed_lib.cdl_b200_rmsnorm_bwd(*(ref(a) for a in args), ctypes.c_void_p(scratch.data_ptr()),
-                                   scratch.numel() * scratch.element_size(), current_stream()))
+    check(packed_lib.cdl_b200_rmsnorm_bwd(*(ref(a) for a in args), *_scratch_args(scratch), current_stream()))
     return dx
 
 
@@ -282,8 +288,7 @@ def attention_bwd(q, k, v, out, d_out, lse, opts: AttentionOpts | None = None, s
             b.insert(0, tensor_bytes(rope_table))
         fn = packed_lib.cdl_b200_attn_bwd_packed if rope_table is None else packed_lib.cdl_b200_attn_bwd_packed_rope
         check(fn(ctypes.byref(desc), *(ref(x) for x in a), max_q, int(opts.max_seqlen_k or 0),
-                 *(ref(x) for x in b), ctypes.c_void_p(scratch.data_ptr()),
-                 scratch.numel() * scratch.element_size(), current_stream()))
+                 *(ref(x) for x in b), *_scratch_args(scratch), current_stream()))
         return dq, dk, dv
     need = attention_bwd_scratch_bytes(q, k)
     if scratch is None:
@@ -292,8 +297,7 @@ def attention_bwd(q, k, v, out, d_out, lse, opts: AttentionOpts | None = None, s
     tensors = (q, k, v, out, d_out, lse) + (() if rope_table is None else (rope_table,)) + (dq, dk, dv)
     args = [tensor_bytes(t) for t in tensors]
     fn = packed_lib.cdl_b200_attn_bwd if rope_table is None else packed_lib.cdl_b200_attn_bwd_rope
-    check(fn(ctypes.byref(desc), *(ref(a) for a in args), ctypes.c_void_p(scratch.data_ptr()),
-             scratch.numel() * scratch.element_size(), current_stream()))
+    check(fn(ctypes.byref(desc), *(ref(a) for a in args), *_scratch_args(scratch), current_stream()))
     return dq, dk, dv
 
 
@@ -356,10 +360,12 @@ def _linear_loss(name, x, w, entries, opts, dx, dw, scratch):
         check(packed_lib.cdl_b200_linear_loss_scratch_bytes(desc, tx, tw, entries[0].shape[-1] if distil else 1, tdx, tdw,
                                                             ctypes.byref(n)))
         scratch = torch.empty(max(n.value, 256), dtype=torch.uint8, device=device)
+        space = scratch.data_ptr(), scratch.numel()
+    else:
+        space = _scratch_args(scratch)
     fn = packed_lib.cdl_b200_linear_distillation if distil else packed_lib.cdl_b200_linear_cross_entropy
     check(fn(desc, tx, tw, *map(tensor_bytes, entries), tensor_bytes(d_loss), _lib.rows_bytes(loss.data_ptr(), tokens),
-             _lib.rows_bytes(lse.data_ptr(), tokens), tdx, tdw, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
-             current_stream()))
+             _lib.rows_bytes(lse.data_ptr(), tokens), tdx, tdw, *space, current_stream()))
     return LinearLossOutputs(loss, lse, dx, dw)
 
 

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import CDL_F32, CDL_I32, check, current_stream, matrix_bytes, packed_lib, tensor_bytes, vector_bytes
-from .ops import _require_current_device
+from .ops import _require_current_device, _scratch_args
 
 
 # --------------------------------------------------------------------------- the cache's plan
@@ -129,7 +129,11 @@ def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: Attention
     _require_current_device(q, k_cache, v_cache, block_table, seq_lens, out, scratch)
     tq, tk = tensor_bytes(q), tensor_bytes(k_cache)
     if scratch is None:
-        scratch = torch.empty(_scratch_of(q.shape, k_cache.shape, q.get_device()), dtype=torch.uint8, device=q.device)
+        bytes_of = _scratch_of(q.shape, k_cache.shape, q.get_device())
+        scratch = torch.empty(bytes_of, dtype=torch.uint8, device=q.device)
+        space = scratch.data_ptr(), bytes_of
+    else:
+        space = _scratch_args(scratch)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse_t = tl = None
@@ -139,8 +143,7 @@ def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: Attention
         tl = matrix_bytes(lse_t.data_ptr(), CDL_F32, batch, heads)
     check(packed_lib.cdl_b200_attn_decode(
         _lib.attn_decode_bytes(opts.softmax_scale or 0.0, opts.softcap, opts.window), tq, tk, tensor_bytes(v_cache),
-        tensor_bytes(block_table), tensor_bytes(seq_lens), tensor_bytes(out), tl, scratch.data_ptr(),
-        scratch.numel() * scratch.element_size(), current_stream()))
+        tensor_bytes(block_table), tensor_bytes(seq_lens), tensor_bytes(out), tl, *space, current_stream()))
     return AttentionDecodeOutputs(out, lse_t)
 
 

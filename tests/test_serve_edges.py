@@ -112,3 +112,44 @@ def test_negative_sizes_are_refused(cdl):
                 shape[d] = -shape[d]
                 st, text = status(cdl, name, *swap(args, i, sized(cdl, t, *shape)))
                 assert st in (-1, -2), (name, i, d, st, text)
+
+
+def bad_scratch(device):
+    block = torch.zeros(1 << 20, dtype=torch.uint8, device=device)
+    return [block[:1].expand(1 << 20), block[::2], block.view(1024, 1024).t()]
+
+
+def test_views_are_no_scratch(cdl, monkeypatch):
+    """One byte expanded to a million is one byte of memory: what a kernel stored there went past its end."""
+    from cleanlm_b200 import ops
+
+    with pytest.raises(cdl._lib.CdlError, match="device memory"):
+        ops._scratch_args(torch.zeros(16, dtype=torch.uint8))
+    monkeypatch.setattr(ops, "_require_cuda", lambda *tensors: None)
+    whole = torch.zeros(16, 4, dtype=torch.float32)
+    assert ops._scratch_args(whole[4:]) == (whole[4:].data_ptr(), 192)
+    for x in bad_scratch("cpu"):
+        with pytest.raises(cdl._lib.CdlError, match="scratch must be contiguous"):
+            ops._scratch_args(x)
+
+
+@gpu
+def test_calls_refuse_views_as_scratch(cdl, gpu_ok):
+    ops, S = cdl.ops, cdl.serve
+    rnd = lambda *s: torch.randn(*s, device="cuda").to(BF16)
+    q, cache = rnd(2, 4, 64), rnd(5, 16, 2, 64)
+    x, dy, scale = rnd(16, 256), rnd(16, 256), rnd(256)
+    r_inv, dscale = torch.ones(16, device="cuda"), torch.zeros(256, device="cuda")
+    a = [rnd(1, 128, 2, 128) for _ in range(5)] + [torch.zeros(1, 2, 128, device="cuda")]
+    packed = [t[0] for t in a[:5]] + [torch.zeros(2, 128, device="cuda")]
+    cu = ops.AttentionOpts(cu_seqlens_q=ints([0, 128]), cu_seqlens_k=ints([0, 128]))
+    for scratch in bad_scratch("cuda") + [torch.zeros(1 << 20, dtype=torch.uint8)]:
+        for call in (lambda: S.attention_decode(q, cache, cache, ints([[0, 1], [2, 3]]), ints([20, 9]), scratch=scratch),
+                     lambda: ops.norm_bwd(x, dy, scale, r_inv, dscale, scratch=scratch),
+                     lambda: ops.norm_bwd(x, dy, scale, r_inv, dscale, scratch=scratch, variant=1),
+                     lambda: ops.attention_bwd(*a, scratch=scratch),
+                     lambda: ops.attention_bwd(*packed, cu, scratch=scratch),
+                     lambda: ops.linear_cross_entropy(x, rnd(256, 512), ints([3] * 16), scratch=scratch)):
+            with pytest.raises(cdl._lib.CdlError, match="scratch must be contiguous|device memory|current device"):
+                call()
+    torch.cuda.synchronize()
