@@ -27,6 +27,7 @@
 #include "ptx.cuh"
 
 #include <cooperative_groups.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -799,6 +800,11 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   CDL_CHECK(check_rows(op, "out", out));
   if (!(desc->softcap >= 0.f) || isinf(desc->softcap)) return fail(CDL_ERR_INVALID, "%s: softcap must be 0 (none) or positive", op);
   if (isnan(desc->softmax_scale) || isinf(desc->softmax_scale)) return fail(CDL_ERR_INVALID, "%s: softmax_scale must be finite", op);
+  const float scale = desc->softmax_scale > 0.f ? desc->softmax_scale : 1.f / sqrtf(static_cast<float>(D));
+  // (the kernel's scale / cap, scale log2 e and cap log2 e are finite then, and the first is not denormal)
+  if (scale > 0x1p126f || desc->softcap > 0x1p126f ||
+      (desc->softcap > 0.f && (scale / desc->softcap < FLT_MIN || scale / desc->softcap > FLT_MAX)))
+    return fail(CDL_ERR_INVALID, "%s: softmax_scale and softcap must be at most 2^126 and their quotient a normal f32 number", op);
   if (desc->window < 0) return fail(CDL_ERR_INVALID, "%s: window must be 0 (all keys) or positive", op);
   if (B == 0 || H == 0) return CDL_OK;
   const void* given[] = {q->ptr, seq_lens->ptr, out->ptr};
@@ -836,8 +842,7 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   p.group = static_cast<int>(group), p.chunks = static_cast<int>(chunks);
   p.pages = static_cast<int>(pages), p.page_size = static_cast<int>(page_size);
   p.width = static_cast<int>(std::min<long long>(width, INT32_MAX)), p.window = desc->window;
-  p.scale = desc->softmax_scale > 0.f ? desc->softmax_scale : 1.f / sqrtf(static_cast<float>(D));
-  p.cap = desc->softcap;
+  p.scale = scale, p.cap = desc->softcap;
   p.out = static_cast<__nv_bfloat16*>(out->ptr), p.out_sb = out->stride[0], p.out_sh = out->stride[1];
   p.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
   p.set = set;

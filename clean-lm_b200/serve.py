@@ -95,7 +95,7 @@ def cache_write(k, v, slots, k_cache, v_cache, q=None, table=None, positions=Non
 # --------------------------------------------------------------------------- attention over the cache
 @dataclass
 class AttentionDecodeOpts:
-    softmax_scale: Optional[float] = None  # None is 1 / sqrt(head_dim)
+    softmax_scale: Optional[float] = None  # None (and numbers that are not positive): 1 / sqrt(head_dim)
     softcap: float = 0.0  # scores x become softcap tanh(x / softcap); 0: as they are
     window: int = 0  # keys that a token sees, its own among them; 0: all
 

@@ -455,7 +455,7 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
  * Scratch: 256-byte aligned, of the size that the call below gives; calls that may run at the same time have one each. */
 typedef struct {
   float softmax_scale; /* <= 0 selects 1/sqrt(head_dim) */
-  float softcap;       /* 0: none */
+  float softcap;       /* 0: none; scale and cap at most 2^126, scale / cap a normal f32 number */
   int32_t window;      /* keys that a token sees, its own among them; 0: all */
 } cdl_attn_decode_desc;
 int32_t cdl_b200_attn_decode(const cdl_attn_decode_desc* desc, const cdl_tensor* q, const cdl_tensor* k_cache,

@@ -153,3 +153,36 @@ def test_calls_refuse_views_as_scratch(cdl, gpu_ok):
             with pytest.raises(cdl._lib.CdlError, match="scratch must be contiguous|device memory|current device"):
                 call()
     torch.cuda.synchronize()
+
+
+def test_decode_refuses_scales_and_caps_that_f32_cannot_divide(cdl):
+    """cap tanh(scale x / cap) with a quotient of infinity made NaN of a score of 0, and a cap whose product with log2 e is
+    infinite of every score."""
+    good = decode_call(cdl)
+    desc = cdl._lib.attn_decode_bytes
+    for scale, cap in ((0.0, 1e-45), (0.0, 1e-40), (0.0, 3e38), (0.0, 2e37), (1e-10, 1e30), (1e20, 1e-30), (3e38, 0.0), (1e38, 1.0)):
+        st, text = status(cdl, "cdl_b200_attn_decode", *swap(good, 0, desc(scale, cap, 0)))
+        assert st == -1 and "quotient" in text, (scale, cap, st, text)
+
+
+@gpu
+def test_decode_at_the_ends_of_scales_and_caps(cdl, gpu_ok):
+    """The largest and smallest caps and scales that are taken: scores of 0 among others, nothing turns NaN; where the cap is far
+    above the scores it is as if there were none, where it is far below all scores are alike."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(*s, generator=gen, device="cuda").to(BF16) for s in ((2, 4, 64), (9, 16, 4, 64), (9, 16, 4, 64)))
+    q[:, 1] = 0
+    table, lens = ints([[0, 1, 2, 3], [4, 5, 6, 7]]), ints([60, 33])
+
+    def call(scale, cap):
+        return cdl.serve.attention_decode(q, k, v, table, lens, cdl.serve.AttentionDecodeOpts(softmax_scale=scale, softcap=cap), lse=True)
+
+    plain, flat = call(None, 0.0), call(1e-30, 0.0)
+    for scale, cap, like in ((None, 1e37, plain), (None, 1e20, plain), (None, 1e-37, flat), (2.0 ** 126, 2.0 ** 126 / 2 ** 70, None),
+                             (1e-37, 1.0, flat), (1e-20, 1e10, flat), (2.0 ** 126, 0.0, None)):
+        got = call(scale, cap)
+        assert not got.out[:, 1].isnan().any() and not got.lse[:, 1].isnan().any(), (scale, cap)
+        if like is not None:
+            # weights that differ by a few roundings of scores below 2^5: 2^-20, and bf16's rounding of p and of the result
+            assert ((got.out.float() - like.out.float()).abs() <= 2.0 ** -6 * v.float().abs().max()).all(), (scale, cap)
+            assert ((got.lse - like.lse).abs() <= 2.0 ** -18).all(), (scale, cap)
