@@ -271,31 +271,35 @@ bool view_apart_from_itself(const cdl_tensor& t) {
   }
   return true;
 }
-// Whether two views of the same element type provably share no element: their extents are apart, or they step in the same
-// way along their first dimensions (the heads of one fused tensor) and what is left lies in different parts of a step.
+// Whether two views provably share no element: their extents are apart, or some stride of theirs divides the memory into steps in
+// which they lie in different places (q, k and v in the heads of a fused tensor, keys and values in halves of a page, of a head or
+// of a row).  Dimensions whose strides are multiples of the step go from one step to another and do not matter.
 bool views_apart(const cdl_tensor& a, const cdl_tensor& b) {
-  const long long size = static_cast<long long>(dtype_size(a.dtype));
-  auto reach = [](const cdl_tensor& t, int from) {
-    long long n = 1;
-    for (int i = from; i < t.rank; ++i) {
+  // Bytes from a view's first to behind its last, without the dimensions that are multiples of `step` bytes (0: none is); 0: empty.
+  auto reach = [](const cdl_tensor& t, long long step) {
+    const long long size = static_cast<long long>(dtype_size(t.dtype));
+    long long n = size;
+    for (int i = 0; i < t.rank; ++i) {
       if (t.shape[i] == 0) return 0LL;
-      n += (t.shape[i] - 1) * t.stride[i];
+      if (step == 0 || t.stride[i] * size % step != 0) n += (t.shape[i] - 1) * t.stride[i] * size;
     }
     return n;
   };
-  if (reach(a, 0) == 0 || reach(b, 0) == 0) return true;
+  const long long all_a = reach(a, 0), all_b = reach(b, 0);
+  if (all_a == 0 || all_b == 0) return true;
+  const cdl_tensor* views[] = {&a, &b};
+  for (const cdl_tensor* t : views)
+    for (int i = 0; i < t->rank; ++i)
+      if (t->shape[i] > 1 && t->stride[i] < 0) return false;
   const long long pa = reinterpret_cast<intptr_t>(a.ptr), pb = reinterpret_cast<intptr_t>(b.ptr);
-  if (pa + reach(a, 0) * size <= pb || pb + reach(b, 0) * static_cast<long long>(dtype_size(b.dtype)) <= pa) return true;
-  if (a.dtype != b.dtype || a.rank != b.rank || (pb - pa) % size != 0) return false;
-  for (int d = 0; d + 1 < a.rank; ++d) {
-    const long long step = a.stride[d];
-    if (step <= 0) return false;
-    for (int i = 0; i <= d; ++i)
-      if (a.stride[i] != b.stride[i] || a.stride[i] % step != 0) return false;
-    long long off = ((pb - pa) / size) % step;
-    if (off < 0) off += step;
-    if (reach(a, d + 1) <= off && off + reach(b, d + 1) <= step) return true;
-  }
+  if (pa + all_a <= pb || pb + all_b <= pa) return true;
+  for (const cdl_tensor* t : views)
+    for (int i = 0; i < t->rank; ++i) {
+      const long long step = t->stride[i] * static_cast<long long>(dtype_size(t->dtype));
+      if (step <= 0) continue;
+      const long long off = ((pb - pa) % step + step) % step;
+      if (reach(a, step) <= off && off + reach(b, step) <= step) return true;
+    }
   return false;
 }
 static bool same_view(const cdl_tensor& a, const cdl_tensor& b) {

@@ -186,3 +186,47 @@ def test_decode_at_the_ends_of_scales_and_caps(cdl, gpu_ok):
             # weights that differ by a few roundings of scores below 2^5: 2^-20, and bf16's rounding of p and of the result
             assert ((got.out.float() - like.out.float()).abs() <= 2.0 ** -6 * v.float().abs().max()).all(), (scale, cap)
             assert ((got.lse - like.lse).abs() <= 2.0 ** -18).all(), (scale, cap)
+
+
+def write_status(cdl, k_cache, v_cache, tokens=0):
+    """Of a call without tokens, which checks its operands and launches nothing."""
+    heads, dim = k_cache.shape[2:]
+    new = bf(tokens, heads, dim)
+    return status(cdl, "cdl_b200_cache_write", None, new, new, None, None, i32(tokens), None, None, k_cache, v_cache)
+
+
+def test_caches_that_share_a_tensor_are_told_apart(cdl):
+    """Keys and values side by side in every order of pages, slots, heads and halves, also with one head, one page or one slot."""
+    import itertools
+
+    for sizes in ((3, 4, 2), (1, 4, 2), (3, 1, 2), (3, 4, 1), (1, 1, 1)):
+        extent = dict(zip("psh", sizes), t=2)
+        for order in itertools.permutations("psht"):
+            whole = bf(*(extent[c] for c in order), 16).permute(*(order.index(c) for c in "tpsh"), 4)
+            st, text = write_status(cdl, whole[0], whole[1])
+            assert st == 0, (sizes, order, text)
+            st, text = write_status(cdl, whole[0], whole[0])
+            assert st == -1 and "overlap" in text, (sizes, order)
+
+
+def test_no_views_that_share_elements_are_let_through(cdl):
+    """Random views of one buffer: whatever is not refused has no element twice."""
+    import random
+
+    rng, buffer = random.Random(3), torch.zeros(1 << 14, dtype=BF16)
+    taken = apart = 0
+    for _ in range(20000):
+        shape = [rng.choice([1, 2, 3]) for _ in range(3)] + [16]
+        views, cells = [], []
+        for _ in range(2):
+            stride = [8 * rng.choice([0, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 96]) for _ in range(3)] + [1]
+            start = 8 * rng.randrange(64)
+            views.append(buffer.as_strided(shape, stride, start))
+            cells.append([start + i * stride[0] + j * stride[1] + k * stride[2] + d for i in range(shape[0]) for j in range(shape[1])
+                          for k in range(shape[2]) for d in range(16)])
+        none_twice = len(set(cells[0] + cells[1])) == 2 * len(cells[0])
+        apart += none_twice
+        if write_status(cdl, *views)[0] == 0:
+            taken += 1
+            assert none_twice, [(v.shape, v.stride(), v.storage_offset()) for v in views]
+    assert taken > 1000 and apart > taken
