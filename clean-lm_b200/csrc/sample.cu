@@ -654,7 +654,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   Settings set;
   set.k = p.top_k ? p.top_k[r] : p.all_top_k;
   set.top_p = p.top_p ? p.top_p[r] : p.all_top_p;
-  set.u = p.u[r];
   if (set.k < 0 || set.k >= p.vocab) set.k = 0;
   const bool p_on = set.top_p < 1.f;
   float top = mine;
@@ -782,7 +781,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       Sums n = block_scan(sum, sh.sums), m{0, 0};
       if (tid == 0) sh.before = 0, sh.mode = SLOW;
       if (tid < 6) sh.edge[tid] = BINS - 1, sh.ahead_of[tid] = tid & 1 ? static_cast<uint32_t>(n.all) : 0;
-      if (set.k > 0) {
+      if (set.k > 0 && static_cast<u64>(set.k) < n.all) {  // (a top_k of all finite logits or more cuts nothing: as without it)
         __syncthreads();
         const u64 want = static_cast<u64>(set.k);
 #pragma unroll
@@ -791,13 +790,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             const u64 through = n.before + count[j];
             sh.before = static_cast<uint32_t>(n.before);
             sh.lo = sh.hi = tid * PER + j;
-            if (want >= n.all) sh.mode = p_on ? SLOW : ALL;  // (the rest is -inf)
-            else if (through <= CAP) sh.mode = LIST;
+            if (through <= CAP) sh.mode = LIST;
             else if (!p_on && count[j] <= CAP) sh.mode = WINDOW_K;
           }
           n.before += count[j];
         }
-        if (tid == 0 && want > n.all && !p_on) sh.mode = ALL;
+      } else if (!p_on) {
+        if (tid == 0) sh.mode = ALL;
       } else {
         m = block_scan(mass, sh.sums);
 #pragma unroll
@@ -938,6 +937,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     }
   }
   meet();
+  set.u = p.u[r];  // (read here: a register less in the passes over the row, 1 us of 43 for 256 rows of 32768)
   int n = static_cast<int>(min(sh.count, static_cast<uint32_t>(CAP + 1)));
   u64 above = sh.above, all = sh.all;
   if (C > 1) {

@@ -230,3 +230,68 @@ def test_no_views_that_share_elements_are_let_through(cdl):
             taken += 1
             assert none_twice, [(v.shape, v.stride(), v.storage_offset()) for v in views]
     assert taken > 1000 and apart > taken
+
+
+# --------------------------------------------------------------------------- sampling
+def check_sample(cdl, z, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    got = cdl.serve.sample(z, u, cdl.serve.SampleOpts(temperature, top_k, top_p, min_p))
+    zs, us = z.double().cpu().numpy(), u.tolist()
+    for r in range(z.shape[0]):
+        token, logprob = serve_ref.sample(zs[r], us[r], temperature, top_k, top_p, min_p)
+        assert got.token[r].item() == token, r
+        # rounded once to f32; the sum behind it is 2^-30 off at most
+        assert abs(got.logprob[r].item() - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -30
+    return got
+
+
+def allowed_only(rows, vocab, allowed, dtype, seed):
+    """Logits of `allowed` tokens of a vocabulary, the others masked."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    z = torch.full((rows, vocab), -torch.inf, device="cuda")
+    for r in range(rows):
+        at = torch.randperm(vocab, generator=gen, device="cuda")[:allowed]
+        z[r, at] = torch.randn(allowed, generator=gen, device="cuda") * 2.5
+    return z.to(dtype), torch.rand(rows, generator=gen, device="cuda")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(3, 5003), (5, 40000), (3, 66001)])
+def test_sample_more_than_there_are(cdl, gpu_ok, rows, vocab, dtype):
+    """top_k of as many entries as are not masked, one less, one more and far more: what it does not cut is as without it."""
+    for allowed in (1, 600, 2048, 3000):
+        z, u = allowed_only(rows, vocab, allowed, dtype, vocab + allowed)
+        for more in ({}, {"top_p": 0.9}, {"top_p": 0.9, "min_p": 0.2}, {"min_p": 0.01}, {"top_p": 0.5, "temperature": 1e4}):
+            base = cdl.serve.sample(z, u, cdl.serve.SampleOpts(**more))
+            for k in (allowed - 1, allowed, allowed + 1, vocab - 1):
+                got = check_sample(cdl, z, u, top_k=k, **more)
+                if k >= allowed:
+                    assert torch.equal(got.token, base.token) and torch.equal(got.logprob, base.logprob), (allowed, more, k)
+
+
+@gpu
+@pytest.mark.parametrize("allowed", [100, 20000])
+def test_a_top_k_that_cuts_nothing_costs_no_search(cdl, gpu_ok, allowed):
+    """A masked row with a larger top_k takes about as long as without it; one CTA searching alone took 30 times that."""
+    z, u = allowed_only(4, 150001, allowed, F32, allowed)
+
+    def us(**opts):
+        opts = cdl.serve.SampleOpts(top_p=0.9, **opts)
+        cdl.serve.sample(z, u, opts)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(5):
+                cdl.serve.sample(z, u, opts)
+        times = []
+        for _ in range(10):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 200)
+        return min(times)
+
+    alone = us()
+    assert us(top_k=max(allowed, 2000)) <= 4 * alone and us(top_k=150000) <= 4 * alone
