@@ -295,3 +295,104 @@ def test_a_top_k_that_cuts_nothing_costs_no_search(cdl, gpu_ok, allowed):
 
     alone = us()
     assert us(top_k=max(allowed, 2000)) <= 4 * alone and us(top_k=150000) <= 4 * alone
+
+
+# --------------------------------------------------------------------------- attention: how the work is shared
+def decode_batch(batch, longest, heads, kv_heads, dim, page_size, seed):
+    """Requests of 1 to `longest` keys in pages in random order; a table wider than 2048 keys."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda", dtype=F32)
+    lens = 1 + torch.randperm(longest, generator=gen, device="cuda")[torch.arange(batch, device="cuda") % longest]
+    count = (lens + page_size - 1) // page_size
+    pages = int(count.sum())
+    order, at = torch.randperm(pages, generator=gen, device="cuda"), 0
+    table = torch.full((batch, max(longest, 2064) // page_size + 1), -1, dtype=I32, device="cuda")
+    for b, n in enumerate(count.tolist()):
+        table[b, :n] = order[at:at + n]
+        at += n
+    k, v = (torch.empty(pages, page_size, kv_heads, dim, dtype=BF16, device="cuda") for _ in range(2))
+    for c in (k, v):
+        for i in range(0, pages, 4096):
+            c[i:i + 4096] = rnd(*c[i:i + 4096].shape).to(BF16)
+    return (2 * rnd(batch, heads, dim)).to(BF16), k, v, table, lens.to(I32)
+
+
+def check_batch(cdl, q, k, v, table, lens):
+    """Against the definition in 64 bits, request by request on the GPU; the bounds are those of the roundings of a score's sum of
+    dim products and its scale, of p and of the result to bf16, and of the sum over n keys."""
+    got = cdl.serve.attention_decode(q, k, v, table, lens, lse=True)
+    group, dim, page_size = q.shape[1] // k.shape[2], q.shape[2], k.shape[1]
+    assert table.shape[1] * page_size > 2048
+    out, spread = torch.empty(q.shape, dtype=torch.float64, device="cuda"), torch.empty(q.shape, dtype=torch.float64, device="cuda")
+    lse, reach = (torch.empty(q.shape[:2], dtype=torch.float64, device="cuda") for _ in range(2))
+    for b, n in enumerate(lens.tolist()):
+        at = table[b, :-(-n // page_size)].long()
+        kb, vb = (c[at].flatten(0, 1)[:n].double().transpose(0, 1) for c in (k, v))  # [kv_heads, n, dim]
+        qb = q[b].double().view(-1, group, dim) * dim ** -0.5
+        s = qb @ kb.transpose(1, 2)
+        reach[b] = (qb.abs() @ kb.abs().transpose(1, 2)).amax(2).flatten()
+        lse[b] = s.logsumexp(2).flatten()
+        p = s.softmax(2)
+        out[b], spread[b] = (p @ vb).view(-1, dim), (p @ vb.abs()).view(-1, dim)
+    n = lens.double()[:, None]
+    off = (dim + 8) * 2.0 ** -24 * reach + 2.0 ** -20
+    bound = 2.0 ** -8 * (out.abs() + spread) + (2 * off + n * 2.0 ** -24)[..., None] * spread
+    assert ((got.out.double() - out).abs() <= bound).all()
+    assert ((got.lse.double() - lse).abs() <= off + n * 2.0 ** -24 + 2.0 ** -22 * lse.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("batch,longest,heads,kv_heads,dim,page_size", [
+    (64, 4096, 16, 16, 128, 16),   # 131000 tiles, 444 CTAs at once: more than 192 each, so there is a second set of parts
+    (64, 4096, 192, 16, 64, 16),   # 65000 tiles, 12 heads per kv head: 296 at once
+    (24, 9001, 32, 8, 128, 7),     # lines that several CTAs share, in both sets
+    (575, 700, 4, 2, 64, 16), (576, 700, 4, 2, 64, 16),    # as many requests as leave an SM room for three CTAs, and one more
+    (1700, 300, 2, 2, 128, 16), (4096, 130, 2, 1, 64, 8),  # two CTAs an SM
+    (4096, 500, 8, 2, 64, 16),     # in two sets of parts
+])
+def test_decode_batches(cdl, gpu_ok, batch, longest, heads, kv_heads, dim, page_size):
+    check_batch(cdl, *decode_batch(batch, longest, heads, kv_heads, dim, page_size, seed=batch + dim))
+
+
+def test_shares_cover_all_tiles_once(tmp_path):
+    """The kernel's own arithmetic of who has which tile, compiled for the host: parts follow one another from 0 to the last tile, none
+    is empty, and the CTA that a tile is looked up for is the one whose part it is in."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    source = (Path(__file__).resolve().parent.parent / "clean-lm_b200" / "csrc" / "attn_decode.cu").read_text()
+    start = source.index("constexpr int SETS")
+    shares = source[start:source.index("\n};\n", start) + 4]
+    (tmp_path / "shares.cpp").write_text("""
+#include <cstdio>
+#include <initializer_list>
+#define __host__
+#define __device__
+#define __forceinline__ inline
+""" + shares + """
+int main() {
+  for (int set : {1, 2, 3, 148, 296, 444}) {
+    const long long edge = 192LL * set;
+    for (long long n : {1LL, 2LL, set - 1LL, (long long)set, set + 1LL, 7LL * set, edge - 1, edge, edge + 1, edge + 12345, 3 * edge + 7,
+                        (1LL << 31) + 5, 1LL << 40}) {
+      if (n < 1) continue;
+      const Shares s(n, set);
+      if (s.ctas < 1 || s.ctas > SETS * set || s.begin(0) != 0 || s.begin(s.ctas) != n) return printf("ends %d %lld\\n", set, n), 1;
+      if ((s.ctas > set) != (n >= edge)) return printf("sets %d %lld\\n", set, n), 1;
+      for (int c = 0; c < s.ctas; ++c) {
+        const long long a = s.begin(c), b = s.begin(c + 1);
+        if (b <= a) return printf("empty %d %lld %d\\n", set, n, c), 1;
+        for (long long u : {a, a + 1, (a + b) / 2, b - 1})
+          if (u < b && s.of(u) != c) return printf("of %d %lld %lld\\n", set, n, u), 1;
+      }
+    }
+  }
+  return 0;
+}
+""")
+    compiler = shutil.which("g++")
+    assert compiler, "a host compiler is part of the toolkit's requirements"
+    subprocess.run([compiler, "-O2", "-std=c++17", "-o", str(tmp_path / "shares"), str(tmp_path / "shares.cpp")], check=True)
+    run = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout
