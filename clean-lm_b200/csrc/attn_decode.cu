@@ -156,6 +156,15 @@ struct Cuts {
   float2 ml[2 * WARPS][COLS];
 };
 
+// CTAs of an SM for which it has shared memory: 228 KB, of which the system takes 1 KB per CTA.  (From 576 requests of head_dim 64, 1600
+// of 128, the prefix of their lengths leaves room for two.  Parts for CTAs that run at once / for three per SM regardless, the last third
+// of them behind the rest, us: 8 heads on 2 of 64, 600 requests of up to 1200 keys 61 / 68, 1024 92 / 108, 2048 of up to 500 97 / 113; of
+// 128, 2048 137 / 157.)
+inline int ctas_by_memory(int nt, size_t dynamic) {
+  const size_t fixed = (nt == 1 ? sizeof(Cuts<8>) : sizeof(Cuts<16>)) + 64;  // and the kernel's few single words
+  return static_cast<int>((228 << 10) / ((dynamic + 127) / 128 * 128 + (fixed + 127) / 128 * 128 + 1024));
+}
+
 // 16 bytes to shared memory, `bytes` of them from `from` and zeros behind.
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -829,7 +838,10 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
     return fail(CDL_ERR_INVALID, "%s: scratch must be 256-byte aligned and hold %zu bytes", op, decode_scratch_bytes(B, nt, D));
 
   if (tiles * rows > (1LL << 40)) return fail(CDL_ERR_UNSUPPORTED, "%s: more than 2^40 tiles of keys", op);
-  const int set = sm_count() * decode::ctas_per_sm(nt);
+  const size_t rings = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>());
+  const size_t smem = rings + (B + 1) * sizeof(int);
+  // CTAs that run at once
+  const int set = sm_count() * std::min(decode::ctas_per_sm(nt), decode::ctas_by_memory(nt, smem));
   const int grid = std::max(1, decode::Shares(tiles * rows, set).ctas);  // (the lengths may leave some without a part)
   decode::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q->ptr), p.q_sb = q->stride[0], p.q_sh = q->stride[1];
@@ -854,7 +866,6 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   p.warp_o = reinterpret_cast<float*>(at);
 
   ProfileScope ps(PROF_ATTN_FWD, 4.0 * B * H * D * most, stream);
-  const size_t rings = decode::WARPS * decode::STAGES * (D == 128 ? decode::stage_bytes<128>() : decode::stage_bytes<64>());
   const long long lines = B * rows;
   if (most <= decode::OWN_KEYS) {
     void (*own)(decode::Params) =
@@ -876,7 +887,6 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
                : (nt == 1 ? decode::attn_decode_kernel<64, 1, false> : decode::attn_decode_kernel<64, 2, false>);
   void (*join)(decode::Params, int) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
-  const size_t smem = rings + (B + 1) * sizeof(int);
   CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
   // items of a CTA: one while there are few, up to one per warp
