@@ -887,7 +887,8 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
                : (nt == 1 ? decode::attn_decode_kernel<64, 1, false> : decode::attn_decode_kernel<64, 2, false>);
   void (*join)(decode::Params, int) = D == 128 ? (nt == 1 ? decode::attn_decode_join_kernel<128, 8> : decode::attn_decode_join_kernel<128, 16>)
                                           : (nt == 1 ? decode::attn_decode_join_kernel<64, 8> : decode::attn_decode_join_kernel<64, 16>);
-  CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)));
+  // (the most that any call needs: two threads' calls of different batches never take it from one another)
+  CDL_CUDA(allow_shared_memory(reinterpret_cast<const void*>(kernel), static_cast<int>(rings + (decode::MAX_BATCH + 1) * sizeof(int))));
   CDL_CUDA(launch_pdl(kernel, dim3(grid), dim3(decode::WARPS * 32), smem, stream, p));
   // items of a CTA: one while there are few, up to one per warp
   const int items = static_cast<int>(std::max<long long>(1, std::min<long long>(decode::JOIN_WARPS, B * H / (2 * sm_count()))));
