@@ -1,5 +1,6 @@
 """Calls of the serving operators (cdl.serve) at the ends of what they take, against their definitions in 64 bits (oracle/serve_ref.py),
 and what they refuse there."""
+import numpy as np
 import pytest
 import torch
 
@@ -320,7 +321,9 @@ def decode_batch(batch, longest, heads, kv_heads, dim, page_size, seed):
 def check_batch(cdl, q, k, v, table, lens):
     """Against the definition in 64 bits, request by request on the GPU; the bounds are those of the roundings of a score's sum of
     dim products and its scale, of p and of the result to bf16, and of the sum over n keys."""
-    got = cdl.serve.attention_decode(q, k, v, table, lens, lse=True)
+    made = [cdl.serve.attention_decode(q, k, v, table, lens, lse=True)]
+    if int(lens.max()) <= 2048:  # the form for tables of so few keys too
+        made.append(cdl.serve.attention_decode(q, k, v, table[:, :2048 // k.shape[1]], lens, lse=True))
     group, dim, page_size = q.shape[1] // k.shape[2], q.shape[2], k.shape[1]
     assert table.shape[1] * page_size > 2048
     out, spread = torch.empty(q.shape, dtype=torch.float64, device="cuda"), torch.empty(q.shape, dtype=torch.float64, device="cuda")
@@ -337,8 +340,9 @@ def check_batch(cdl, q, k, v, table, lens):
     n = lens.double()[:, None]
     off = (dim + 8) * 2.0 ** -24 * reach + 2.0 ** -20
     bound = 2.0 ** -8 * (out.abs() + spread) + (2 * off + n * 2.0 ** -24)[..., None] * spread
-    assert ((got.out.double() - out).abs() <= bound).all()
-    assert ((got.lse.double() - lse).abs() <= off + n * 2.0 ** -24 + 2.0 ** -22 * lse.abs()).all()
+    for got in made:
+        assert ((got.out.double() - out).abs() <= bound).all()
+        assert ((got.lse.double() - lse).abs() <= off + n * 2.0 ** -24 + 2.0 ** -22 * lse.abs()).all()
 
 
 @gpu
@@ -349,6 +353,7 @@ def check_batch(cdl, q, k, v, table, lens):
     (575, 700, 4, 2, 64, 16), (576, 700, 4, 2, 64, 16),    # as many requests as leave an SM room for three CTAs, and one more
     (1700, 300, 2, 2, 128, 16), (4096, 130, 2, 1, 64, 8),  # two CTAs an SM
     (4096, 500, 8, 2, 64, 16),     # in two sets of parts
+    (2, 700, 2048, 1, 64, 16), (3, 400, 1000, 8, 128, 5),  # groups of 2048 and 125
 ])
 def test_decode_batches(cdl, gpu_ok, batch, longest, heads, kv_heads, dim, page_size):
     check_batch(cdl, *decode_batch(batch, longest, heads, kv_heads, dim, page_size, seed=batch + dim))
@@ -396,3 +401,78 @@ int main() {
     subprocess.run([compiler, "-O2", "-std=c++17", "-o", str(tmp_path / "shares"), str(tmp_path / "shares.cpp")], check=True)
     run = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True)
     assert run.returncode == 0, run.stdout
+
+
+# --------------------------------------------------------------------------- sizes
+@gpu
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(1, 1, 1, 2048), (7, 3, 2, 1040), (5, 300, 1, 16), (9, 2, 70, 48), (40, 16, 4, 128), (3, 0, 2, 64)])
+def test_write_element_by_element(cdl, gpu_ok, tokens, heads, kv_heads, dim):
+    """Head sizes up to the largest and any number of heads; each element within its own roundings."""
+    gen = torch.Generator(device="cuda").manual_seed(dim + tokens)
+    qkv = torch.randn(tokens, heads + 2 * kv_heads, dim, generator=gen, device="cuda").to(BF16)
+    q, k, v = qkv.split([heads, kv_heads, kv_heads], 1)
+    caches = [torch.full((4, 11, kv_heads, dim), 7.0, dtype=BF16, device="cuda") for _ in range(2)]
+    slots = torch.randperm(44, generator=gen, device="cuda")[:tokens]
+    positions = torch.randint(0, 900, (tokens,), generator=gen, device="cuda")
+    table = cdl.sky1.rope_table(900, dim)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    got = cdl.serve.cache_write(k, v, slots.to(I32), *caches, q=q, table=table, positions=positions.to(I32), k_out=k_out)
+    cos, sin = (x[:, None] for x in table[positions].double().split(dim // 2, 1))
+
+    def near(have, x):
+        lo, hi = x.double().split(dim // 2, 2)
+        want = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], 2)
+        size = torch.cat([(lo * cos).abs() + (hi * sin).abs(), (hi * cos).abs() + (lo * sin).abs()], 2)
+        # half a step of bf16, and f32's of two products and their sum
+        assert ((have.double() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * 2.0 ** -24 * size).all()
+
+    near(got.q, q)
+    near(got.k, k)
+    k_flat, v_flat = (c.flatten(0, 1) for c in caches)
+    assert torch.equal(k_flat[slots], got.k) and torch.equal(v_flat[slots], v)
+    rest = torch.ones(44, dtype=torch.bool, device="cuda")
+    rest[slots] = False
+    assert (k_flat[rest] == 7).all() and (v_flat[rest] == 7).all()
+
+
+@gpu
+def test_plan_of_160000_requests(cdl, gpu_ok):
+    """More rounds of 1024 requests than there are CTAs, with a table that is a part of a wider one."""
+    rng, requests, page_size, pages = np.random.default_rng(1), 160001, 4, 400000
+    cached, added = rng.integers(0, 6, requests), rng.integers(0, 3, requests)
+    used = -(-cached // page_size)
+    order = rng.permutation(pages)
+    table = np.full((requests, 2), -1)
+    mine = np.arange(2)[None] < used[:, None]
+    table[mine] = order[:mine.sum()]
+    stack = order[mine.sum():][:60000]
+    rows = int(added.sum()) - 5
+    want = serve_ref.cache_plan(cached.tolist(), added.tolist(), table.tolist(), stack.tolist(), len(stack), page_size, pages, rows)
+    wide = torch.full((requests, 5), 9, dtype=I32, device="cuda")
+    wide[:, :2] = ints(table)
+    got = cdl.serve.cache_plan(ints(cached), ints(added), wide[:, :2], ints(stack), ints([len(stack)]),
+                               cdl.serve.CachePlanOpts(page_size, pages, rows))
+    have = (got.seq_lens, got.cu_seqlens, got.positions, got.slots, got.free_left, wide[:, :2])
+    for name, g, w in zip(("seq_lens", "cu_seqlens", "positions", "slots", "free_left", "block_table"), have, want):
+        assert torch.equal(g.cpu(), torch.tensor([w] if name == "free_left" else w, dtype=I32)), name
+    assert (wide[:, 2:] == 9).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_sample_of_three_million(cdl, gpu_ok, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    z = (torch.randn(2, 3000017, generator=gen, device="cuda") * 3).to(dtype)
+    u = torch.tensor([0.3, 0.9999], device="cuda")
+    for opts in ({}, {"top_p": 0.8}, {"top_k": 50}, {"top_k": 3000}, {"min_p": 1e-3}, {"temperature": 0.0}):
+        check_sample(cdl, z, u, **opts)
+
+
+@gpu
+def test_sample_of_odd_random_numbers(cdl, gpu_ok):
+    """Numbers outside [0, 1) beside ones inside, each row against the definition."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    z = torch.randn(10, 700, generator=gen, device="cuda")
+    u = torch.tensor([-1.0, float("nan"), 1.0, 2.0, torch.inf, -torch.inf, 0.0, 0.5, 1 - 2.0 ** -24, 2.0 ** -140], device="cuda")
+    check_sample(cdl, z, u)
+    check_sample(cdl, z, u, top_k=30, top_p=0.8)
