@@ -476,3 +476,58 @@ def test_sample_of_odd_random_numbers(cdl, gpu_ok):
     u = torch.tensor([-1.0, float("nan"), 1.0, 2.0, torch.inf, -torch.inf, 0.0, 0.5, 1 - 2.0 ** -24, 2.0 ** -140], device="cuda")
     check_sample(cdl, z, u)
     check_sample(cdl, z, u, top_k=30, top_p=0.8)
+
+
+# --------------------------------------------------------------------------- threads
+@gpu
+def test_steps_of_several_threads(cdl, gpu_ok):
+    """A step's four calls from four threads at once, each on its stream with a batch of its own size: the bits of the same calls one
+    thread after the other."""
+    import threading
+
+    S, sizes = cdl.serve, (1, 60, 700, 2500)
+
+    def inputs(batch):
+        gen = torch.Generator(device="cuda").manual_seed(batch)
+        rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+        q, k, v, table, lens = decode_batch(batch, 250, 4, 2, 64, 16, seed=batch)
+        pages = k.shape[0] + batch
+        k, v = (torch.cat([c, torch.zeros(batch, 16, 2, 64, dtype=BF16, device="cuda")]) for c in (k, v))
+        stack = torch.arange(k.shape[0] - batch, k.shape[0], device="cuda").to(I32)
+        return (rnd(batch, 8, 64).to(BF16), k, v, table, lens, torch.ones(batch, dtype=I32, device="cuda"), stack, ints([batch]), pages,
+                rnd(batch, 5000), torch.rand(batch, generator=gen, device="cuda"), cdl.sky1.rope_table(260, 64))
+
+    def step(qkv, k, v, table, lens, one, stack, count, pages, z, u, rope):
+        table, k, v = table.clone(), k.clone(), v.clone()
+        p = S.cache_plan(lens, one, table, stack, count, S.CachePlanOpts(16, pages, len(lens)))
+        w = S.cache_write(qkv[:, 4:6], qkv[:, 6:], p.slots, k, v, q=qkv[:, :4], table=rope, positions=p.positions)
+        a = S.attention_decode(w.q, k, v, table, p.seq_lens, lse=True)
+        short = S.attention_decode(w.q, k, v, table[:, :20], p.seq_lens)
+        t = S.sample(z, u, S.SampleOpts(top_p=0.9))
+        return p.slots, p.free_left, k, v, a.out, a.lse, short.out, t.token, t.logprob
+
+    data = [inputs(n) for n in sizes]
+    want = [step(*x) for x in data]
+    torch.cuda.synchronize()
+    got, errors, start = [None] * len(sizes), [], threading.Barrier(len(sizes))
+
+    def worker(i):
+        try:
+            torch.cuda.set_device(0)
+            stream = torch.cuda.Stream()
+            start.wait()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got[i] = step(*data[i])
+            stream.synchronize()
+        except Exception as e:  # raised below
+            errors.append(e)
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for w, g in zip(want, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, g))
