@@ -38,6 +38,9 @@ constexpr int SMALL = THREADS;  // entries of a list that are each held against 
 // A CTA's part of top_k up to which a bound from its threads' largest logits finds the candidates.  (Bound / histogram, us, 148
 // rows of 32768: top_k of 50 11.9 / 17.0, 100 13.5 / 18.2, 300 29.4 / 30.6; of 150001: 50 29 / 51, 300 51 / 68.)
 constexpr int LIST_K = 384;
+// And top_k itself: the bounds of three or four CTAs at more of their threads' largest leave more than CAP entries.  (top_k of 1100 of one
+// row of 150001 55 us by the bound, 59 by the histogram; of 1300 three passes more, for the list has to be made again.)
+constexpr int BOUND_K = CAP / 2;
 
 struct Params {
   const void* z;
@@ -94,6 +97,11 @@ struct Row {
     return q;
   }
   __device__ __forceinline__ int first(int v) const { return v * N - lead; }
+  // Vectors of a tile: 512 logits, or as many times that as leave at most TILES of them.
+  __device__ __forceinline__ int per_tile() const {
+    constexpr int BASE = 512 / N;
+    return (vectors + BASE * TILES - 1) / (BASE * TILES) * BASE;
+  }
   __device__ __forceinline__ uint4 load(int v) const {
     const int i = first(v);
     return i >= 0 && i <= vocab - N ? ld_nc_v4(z + i) : load_end(z, vocab, i);
@@ -172,6 +180,16 @@ struct Row {
     }
   }
 };
+
+template <typename T>
+__device__ __forceinline__ Row<T> row_of(const Params& p, long long r) {
+  Row<T> row;
+  row.z = static_cast<const T*>(p.z) + r * p.ld;
+  row.vocab = p.vocab;
+  row.lead = static_cast<int>((reinterpret_cast<uintptr_t>(row.z) & 15) / sizeof(T));
+  row.vectors = (p.vocab + row.lead + Row<T>::N - 1) / Row<T>::N;
+  return row;
+}
 
 // floor(f n) for f of [0, 1), and whether something is left over: with f = m 2^-s and a product of 128 bits, so that the half of
 // an even sum is that.
@@ -320,6 +338,8 @@ struct Shared {
   float top;
   int at;
   uint32_t count, bound;
+  int again;  // (written by the first)
+  uint32_t key_min;
   u64 above, all;
   int mode, lo, hi;
   uint32_t before;
@@ -606,6 +626,106 @@ __device__ __noinline__ u64 slow_cut(const Row<T>& row, Shared& sh, const Settin
   return cut;
 }
 
+// The draw where a bound of the threads' largest logits left more than CAP entries: a part of the row lies far below the others
+// (masked, or the row is in order), so that its CTA's bound does.  All CTAs of the row find the k-th entry from counts of 11 bits at a
+// time, of its key and, where more than CAP are alike, of its index; the list is made again of the entries from there on.  (Half of
+// 150001 logits masked, top_k of 50, one row: 43 us, 16 with nothing masked;
+// one CTA searching alone 534.)  It takes all that it needs from the parameters,
+// so that the kernel has to keep nothing for it.
+template <typename T>
+__device__ __noinline__ void draw_again(const Params& p, Shared& sh) {
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, C = p.cluster, rank = static_cast<int>(blockIdx.x % C);
+  const long long r = blockIdx.x / C;
+  const Row<T> row = row_of<T>(p, r);
+  const int per_tile = row.per_tile(), tiles = (row.vectors + per_tile - 1) / per_tile, share = (tiles + C - 1) / C;
+  const int v0 = min(row.vectors, min(tiles, rank * share) * per_tile), v1 = min(row.vectors, min(tiles, (rank + 1) * share) * per_tile);
+  auto meet = [&]() {
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+  };
+  auto of = [&](int other) -> Shared& { return C > 1 ? *cluster.map_shared_rank(&sh, other) : sh; };
+  Settings set;
+  set.k = p.top_k ? p.top_k[r] : p.all_top_k;
+  set.top_p = p.top_p ? p.top_p[r] : p.all_top_p;
+  set.u = p.u[r];
+  set.key_min = sh.key_min;
+  set.t = static_cast<double>(p.temperature ? p.temperature[r] : p.all_temperature);
+  const uint32_t k = static_cast<uint32_t>(set.k);
+  u64 bound = 0;       // the bits found so far
+  uint32_t above = 0;  // the entries above those that have them
+  __syncthreads();     // (the list's length was read by all)
+#pragma unroll 1
+  for (int level = 0; level < 6; ++level) {
+    const int low_bit = level < 3 ? 32 : 0, width = level % 3 < 2 ? 11 : 10, shift = low_bit + (level % 3 == 0 ? 21 : level % 3 == 1 ? 10 : 0);
+    const uint32_t mask = (1u << width) - 1;
+    for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
+    if (tid == 0) sh.lo = -1, sh.count = 0;
+    __syncthreads();
+    row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int i) {
+      Row<T>::fours(q, i, [&](const float (&x)[4], int j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t key = key_of(x[e]);
+          const u64 entry = packed(key, j + e);
+          if (key > KEY_NONE && (level == 0 || (entry ^ bound) >> (shift + width) == 0))
+            atomicAdd(&sh.hist[mask - (static_cast<uint32_t>(entry >> shift) & mask)], 1u);
+        }
+      });
+    });
+    meet();
+    constexpr int PER = BINS / THREADS;
+    static_assert(PER == 4, "");
+    uint4 bins = make_uint4(0, 0, 0, 0);  // the largest entries first
+    for (int c = 0; c < C; ++c) {
+      const uint4 o = reinterpret_cast<const uint4*>(of(c).hist)[tid];
+      bins.x += o.x, bins.y += o.y, bins.z += o.z, bins.w += o.w;
+    }
+    const uint32_t count[PER] = {bins.x, bins.y, bins.z, bins.w};
+    uint32_t upto = above + static_cast<uint32_t>(block_scan(static_cast<u64>(bins.x) + bins.y + bins.z + bins.w, sh.sums).before);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (upto < k && upto + count[j] >= k) sh.lo = tid * PER + j, sh.ahead_of[0] = upto, sh.ahead_of[1] = upto + count[j];
+      upto += count[j];
+    }
+    meet();
+    const int at = sh.lo;
+    above = sh.ahead_of[0];
+    const uint32_t through = sh.ahead_of[1];
+    __syncthreads();  // (read by all before it is written again)
+    if (at < 0) break;  // fewer than k entries are not masked: all of them
+    bound |= static_cast<u64>(mask - at) << shift;
+    if (through <= CAP) break;
+  }
+  row.template each<4>(v0 + tid, v1, THREADS, [&](const uint4& q, int i) {
+    Row<T>::fours(q, i, [&](const float (&x)[4], int j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t key = key_of(x[e]);
+        const u64 entry = packed(key, j + e);
+        if (key > KEY_NONE && entry >= bound) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < CAP) sh.list[at] = entry;
+        }
+      }
+    });
+  });
+  meet();
+  int n = static_cast<int>(sh.count);  // (up to CAP in all)
+  if (C > 1) {
+    for (int c = 1; rank == 0 && c < C; ++c) {
+      const Shared& o = of(c);
+      const int m = static_cast<int>(o.count);
+      for (int i = tid; i < m && n + i < CAP; i += THREADS) sh.list[n + i] = o.list[i];
+      n += m;
+    }
+    cluster.sync();  // (nobody's shared memory goes while it is read)
+    if (rank != 0) return;
+  }
+  __syncthreads();
+  draw_sorted(p, sh, set, r, min(n, CAP));
+}
+
 // What the pass over the row's weights has to find.
 enum Mode {
   ALL,       // everything (but what min_p leaves out) is kept
@@ -616,7 +736,7 @@ enum Mode {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -628,17 +748,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   };
   auto of = [&](int other) -> Shared& { return C > 1 ? *cluster.map_shared_rank(&sh, other) : sh; };
   if (tid < 256) sh.pow2[tid] = __hiloint2double(__double2hiint(POW2[tid]) + (p.scale_bits << 20), __double2loint(POW2[tid]));
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.count = 0, sh.again = 0;
   const long long r = blockIdx.x / C;
-  Row<T> row;
-  row.z = static_cast<const T*>(p.z) + r * p.ld;
-  row.vocab = p.vocab;
+  const Row<T> row = row_of<T>(p, r);
   constexpr int N = Row<T>::N;
-  row.lead = static_cast<int>((reinterpret_cast<uintptr_t>(row.z) & 15) / sizeof(T));
-  row.vectors = (p.vocab + row.lead + N - 1) / N;
-  // vectors of a tile: 512 logits, or as many times that as leave at most TILES of them
-  constexpr int BASE = 512 / N;
-  const int per_tile = (row.vectors + BASE * TILES - 1) / (BASE * TILES) * BASE;
+  const int per_tile = row.per_tile();
   const int tiles = (row.vectors + per_tile - 1) / per_tile;
   const int share = (tiles + C - 1) / C;  // tiles of a CTA
   const int t0 = min(tiles, rank * share), t1 = min(tiles, t0 + share);
@@ -704,6 +818,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const double far = set.t * log(static_cast<double>(fminf(min_p, 1.f)));  // (NaN: of an infinite temperature, where all w are 1)
     set.key_min = isnan(far) ? 0 : min(key_of(top), key_of(__double2float_ru(static_cast<double>(top) + far)));
   }
+  if (tid == 0) sh.key_min = set.key_min;
 
   auto append = [&](uint32_t key, int i) {
     const uint32_t at = atomicAdd(&sh.count, 1u);
@@ -719,9 +834,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   const int each_k = (set.k + C - 1) / C;
   if ((set.k > 0 || p_on) && p.vocab <= CAP) {
     mode = LIST;
-  } else if (set.k > 0 && each_k <= min(LIST_K, have * 3 / 4)) {
+  } else if (set.k > 0 && set.k <= BOUND_K && each_k <= min(LIST_K, have * 3 / 4)) {
     // A CTA's part of top_k: that many of its threads' largest logits reach its bound, so the least of the CTAs' bounds is one that
-    // at least top_k logits of the row reach, and not many more.
+    // at least top_k logits of the row reach, and not many more where the CTAs' parts of the row are alike.
     mode = LIST;
     const uint32_t key = key_of(mine);
     constexpr int LOW = N == 8 ? 16 : 0;  // bits that tell no two bf16 apart
@@ -941,7 +1056,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
   int n = static_cast<int>(min(sh.count, static_cast<uint32_t>(CAP + 1)));
   u64 above = sh.above, all = sh.all;
   if (C > 1) {
-    if (rank == 0)
+    if (rank == 0) {
       for (int c = 1; c < C; ++c) {
         const Shared& o = of(c);
         const int m = static_cast<int>(min(o.count, static_cast<uint32_t>(CAP + 1)));
@@ -952,10 +1067,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         if (mode == ALL || mode == WINDOW_P || mode == WINDOW_K)
           for (int i = c * share + tid; i < min(tiles, (c + 1) * share); i += THREADS) sh.tile[i] = o.tile[i];
       }
+      if (mode == LIST && n > CAP && tid > 0 && tid < C) of(tid).again = 1;
+    }
     cluster.sync();
-    if (rank != 0) return;
+    if (rank != 0 && !sh.again) return;
   }
-  if (mode == LIST && n <= CAP) {
+  if (mode == LIST && (rank != 0 || n > CAP)) {
+    draw_again<T>(p, sh);
+    return;
+  }
+  if (mode == LIST) {
     if (n <= SMALL) draw_small(p, sh, set, r, n);
     else draw_sorted(p, sh, set, r, n);
     return;
@@ -1034,7 +1155,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
       }
     }
   }
-  if (mode == SLOW || mode == LIST) cut = slow_cut(row, sh, set, per_tile, tiles);
+  if (mode == SLOW) cut = slow_cut(row, sh, set, per_tile, tiles);
 
   // ---- the draw: which tile, and which entry of it
   const u64 a = 2 * tid < tiles ? sh.tile[2 * tid] : 0, b = 2 * tid + 1 < tiles ? sh.tile[2 * tid + 1] : 0;

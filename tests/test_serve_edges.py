@@ -531,3 +531,64 @@ def test_steps_of_several_threads(cdl, gpu_ok):
     assert not errors, errors
     for w, g in zip(want, got):
         assert all(torch.equal(a, b) for a, b in zip(w, g))
+
+
+def uneven(z, kind):
+    """Logits whose parts a row's CTAs and threads find unlike: a masked or low range of the vocabulary, logits in order, equal ones."""
+    z, vocab = z.clone(), z.shape[1]
+    if kind == "half":
+        z[:, vocab // 2:] = -torch.inf
+    elif kind == "front":
+        z[:, :vocab // 3] = -torch.inf
+    elif kind == "low":
+        z[:, vocab // 4:vocab // 2] -= 20
+    elif kind == "order":
+        z = z.float().sort(1, descending=True)[0].to(z.dtype)
+    elif kind == "alike":  # the k-th has thousands of equals, in a few parts
+        z[:, :vocab // 4], z[:, vocab // 4:] = 4.0, -5.0
+    return z
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(3, 9001), (2, 40001), (3, 150001), (50, 66001), (100, 33000)])
+def test_sample_top_k_of_uneven_rows(cdl, gpu_ok, rows, vocab, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    z, u = (torch.randn(rows, vocab, generator=gen, device="cuda") * 2.5).to(dtype), torch.rand(rows, generator=gen, device="cuda")
+    pick = torch.tensor([0, rows - 1], device="cuda")
+    for kind in ("half", "front", "low", "order", "alike"):
+        x = uneven(z, kind)
+        for opts in ({"top_k": 1}, {"top_k": 50}, {"top_k": 300, "top_p": 0.8}, {"top_k": 384, "min_p": 0.2}, {"top_k": 1100}, {"top_k": 1024, "top_p": 0.9}):
+            whole = cdl.serve.sample(x, u, cdl.serve.SampleOpts(**opts))
+            some = check_sample(cdl, x[pick], u[pick], **opts)
+            assert torch.equal(whole.token[pick], some.token) and torch.equal(whole.logprob[pick], some.logprob), (kind, opts)
+
+
+@gpu
+def test_top_k_of_a_masked_vocabulary_costs_no_search(cdl, gpu_ok):
+    """Half the vocabulary masked, or a top_k of which three or four CTAs' bounds leave too many entries: a few passes more, where one
+    CTA searching alone took 10 to 60 times as long."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    z, u = torch.randn(4, 150001, generator=gen, device="cuda") * 2.5, torch.rand(4, generator=gen, device="cuda")
+
+    def us(x, **opts):
+        opts = cdl.serve.SampleOpts(**opts)
+        cdl.serve.sample(x, u, opts)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(5):
+                cdl.serve.sample(x, u, opts)
+        times = []
+        for _ in range(10):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 200)
+        return min(times)
+
+    base = us(z, top_k=50)
+    assert us(uneven(z, "half"), top_k=50) <= 6 * base and us(uneven(z, "half"), top_k=50, top_p=0.9) <= 6 * base
+    assert us(z, top_k=1300) <= 3 * us(z, top_k=1600)
