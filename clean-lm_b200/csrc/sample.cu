@@ -768,6 +768,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   Settings set;
   set.k = p.top_k ? p.top_k[r] : p.all_top_k;
   set.top_p = p.top_p ? p.top_p[r] : p.all_top_p;
+  set.u = p.u[r];
   if (set.k < 0 || set.k >= p.vocab) set.k = 0;
   const bool p_on = set.top_p < 1.f;
   float top = mine;
@@ -1052,7 +1053,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
   }
   meet();
-  set.u = p.u[r];  // (read here: a register less in the passes over the row, 1 us of 43 for 256 rows of 32768)
   int n = static_cast<int>(min(sh.count, static_cast<uint32_t>(CAP + 1)));
   u64 above = sh.above, all = sh.all;
   if (C > 1) {
