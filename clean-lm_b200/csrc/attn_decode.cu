@@ -16,7 +16,8 @@
 //
 // Short work is bound by latency instead, trips to memory one after the other (lengths, page, keys, values, results).  There each
 // (request, kv head) has a cluster of CTAs of its own, which join their results by way of shared memory: one request of some
-// hundred keys and 16 heads takes 7.6 us, 10.9 on the common line with its second kernel.
+// hundred keys and 16 heads (777 of 128) takes 7.8 us, 10.7 on the common line with its second kernel.  The host knows no lengths, so it
+// is the table's width and the window that choose: one of 129 pages of 16 takes the common line whatever its requests hold.
 //
 // Products are taken transposed, scores^T = K q^T and out^T = V^T p^T, so that the query heads of a group are the 8 columns
 // of mma.m16n8k16 (as rows they would leave at least half of it empty) and the pieces of K and V rows that a thread reads are its
@@ -45,8 +46,8 @@ constexpr int JOIN_WARPS = 8;    // of a CTA of the second kernel
 // Where no request sees more keys than this (by the width of its table, by the window), each line has CTAs of its own, as one long line
 // among short ones cannot take much longer than the rest.  (Own CTAs / shared ones, us, 16 heads of 128, requests of 1 to L keys:
 // L = 512: 1 request 7.2 / 10.8, 37 25 / 30, 256 106 / 126; 2048: 1 10.5 / 14.3, 16 40 / 38, 64 102 / 109; 4096: 1 14.6 / 15.9, 16
-// 75 / 61, 37 128 / 120.  24 heads on 2 of 64, L = 2048: 1 9.8 / 10.9, 256 49 / 53; 8192: 1 16.5 / 14.5.  Slower: 4096 lines of 1 to
-// 100 keys, 56 / 51.)
+// 75 / 61, 37 128 / 120.  24 heads on 2 of 64, L = 2048: 1 9.8 / 10.9, 256 49 / 53; 8192: 1 16.5 / 14.5.  What the rule gives away:
+// 4096 lines of 1 to 100 keys, 56 / 51.)
 constexpr int OWN_KEYS = 2048;
 constexpr int MAX_SPLIT = 8;     // CTAs of a line that has its own
 constexpr int MAX_BATCH = 4096;  // the prefix of the lengths is kept in shared memory beside the rings
@@ -820,7 +821,8 @@ int32_t attn_decode_execute(const cdl_attn_decode_desc* desc, const cdl_tensor* 
   for (const void* x : given)
     if (!x) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
   const long long width = pages == 0 ? 0 : block_table->shape[1];
-  if ((lse && !lse->ptr) || (width > 0 && (!block_table->ptr || !k_cache->ptr || !v_cache->ptr))) return fail(CDL_ERR_INVALID, "%s: null pointer", op);
+  if ((lse && !lse->ptr) || (width > 0 && (!block_table->ptr || !k_cache->ptr || !v_cache->ptr)))
+    return fail(CDL_ERR_INVALID, "%s: null pointer", op);
   if (!view_apart_from_itself(*out)) return fail(CDL_ERR_INVALID, "%s: elements of out overlap", op);
   const cdl_tensor* ins[] = {q, k_cache, v_cache, block_table, seq_lens};
   for (const cdl_tensor* i : ins)

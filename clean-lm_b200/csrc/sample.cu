@@ -13,8 +13,13 @@
 // is large or top_p is on, for a histogram, which gives a bound that the kept entries reach or a window that the cut lies in; and
 // for the candidates, the sums of whole tiles and, around the cut, the entries on a list in shared memory.  The rest is that list
 // and one tile.  What bounds it is instructions and barriers, not memory: 148 rows of 32768 bf16 logits (1.5 us at 6.56 TB/s) take
-// 5.3 us for the largest, 11.5 for top_k of 50, 14.0 for an unrestricted draw (all weights, in f64) and 29.2 for top_p of 0.9 (a
+// 4.4 us for the largest, 10.9 for top_k of 50, 13.1 for an unrestricted draw (all weights, in f64) and 28.0 for top_p of 0.9 (a
 // histogram and all weights); one row in two CTAs 4.6, 10.8, 10.2 and 23.
+//
+// What one CTA has to search for alone is far slower (one row of 150001 f32 logits, where an ordinary top_p takes 37 us): top_p of rows
+// so flat that the cut's bin, T ln 2 / 64 wide, holds more than 2048 entries (logits that spread less than about 0.17 T, 0.9 ms; of
+// 262144 entries 0.4 T, 1.6 ms); a cut among thousands of equal logits (1.2 ms); top_p of a top_k that cuts something, where the bins through
+// the k-th hold more than 2048 entries (top_k from about 2040 on; 1.2 ms).
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -629,9 +634,8 @@ __device__ __noinline__ u64 slow_cut(const Row<T>& row, Shared& sh, const Settin
 // The draw where a bound of the threads' largest logits left more than CAP entries: a part of the row lies far below the others
 // (masked, or the row is in order), so that its CTA's bound does.  All CTAs of the row find the k-th entry from counts of 11 bits at a
 // time, of its key and, where more than CAP are alike, of its index; the list is made again of the entries from there on.  (Half of
-// 150001 logits masked, top_k of 50, one row: 43 us, 16 with nothing masked;
-// one CTA searching alone 534.)  It takes all that it needs from the parameters,
-// so that the kernel has to keep nothing for it.
+// 150001 logits masked, top_k of 50, one row: 43 us, 16 with nothing masked; one CTA searching alone 534.)  It takes all that it needs
+// from the parameters, so that the kernel has to keep nothing for it.
 template <typename T>
 __device__ __noinline__ void draw_again(const Params& p, Shared& sh) {
   const cg::cluster_group cluster = cg::this_cluster();
@@ -1234,10 +1238,11 @@ int32_t sample_execute(const cdl_sample_desc* desc, const cdl_tensor* logits, co
   p.scale_bits = std::min(50, 62 - bits);
   ProfileScope ps(PROF_ELEMENTWISE, static_cast<double>(R) * V * dtype_size(logits->dtype), stream);
   // CTAs of a row, of 16384 logits each or more: 4 or 3 where such clusters find an SM for each (7/8 of them), pairs where those do;
-  // two to an SM where rows are long.  (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us, from HBM: 150001 f32 logits, 16 rows 93, 57, 45,
-  // 38, in 6 and 8 slower; 37 rows 94, 58, 47, 56; 48 rows 97, 60, 67, 57, with what L2 holds of them 120, 73, 70, 59; 74 rows 108,
-  // 66, 70, 86; 148 rows 125, 105, 136, 134.  65536: 48 rows 47, 34, 40, 35; 148 rows 57, 52, 75, 83, with top_k of 50 21, 21.
-  // 32768 bf16: 16 rows 28, 24, 23, 22; 100 rows 29, 33, 49, 49.)
+  // two to an SM where rows are long.  (top_p of 0.9 in 1, 2, 3 and 4 CTAs, us, from HBM: 150001 f32 logits, 16 rows 99, 59, 48,
+  // 40, in 6 and 8 slower; 37 rows 101, 62, 49, 56; 48 rows 104, 66, 68, 57; 64 rows 111, 70, 70, 59; 74 rows 115, 71, 70, 87; 148 rows
+  // 146, 106, 134, 135.  131072: 48 rows 91, 57, 61, 51; 64 rows 92, 58, 63, 52; of bf16 75, 50, 59, 50 and 76, 50, 60, 51.  65536: 48
+  // rows 50, 35, 39, 34; 74 rows 51, 36, 41, 53; 148 rows 55, 52, 75, 83, of which the rule takes the first, 4 us above the second.
+  // 32768 bf16: 16 rows 27, 23, 23, 22; 100 rows 28, 32, 45, 46.)
   const long long sms = sm_count(), own_sm = sms * 7 / 8 / R;
   const bool long_rows = V >= 131072;
   const long long fit = own_sm >= 3 ? own_sm : long_rows && 4 * R <= sms * 7 / 4 ? 4 : 2 * R <= (long_rows ? 2 * sms : sms) ? 2 : 1;

@@ -11,8 +11,16 @@ block_table[b, j // page_size].  One step of a batch:
     s = serve.sample(logits, uniform, serve.SampleOpts(temperature=0.8, top_p=0.95))
 
 Lengths stay on the device: the host only bounds the rows and the pages of a request, so a step can be captured into a graph once
-and replayed.  (A prompt attends to itself by `ops.attention_fwd` on the packed layout, with `plan.cu_seqlens`.)  The reference's
-attention takes the same cache as KvLayout::Paged (crates/cleandl/src/execgraph/ops/attention/mod.rs:83-91).
+and replayed.  The reference's attention takes the same cache as KvLayout::Paged (crates/cleandl/src/execgraph/ops/attention/
+mod.rs:83-91).
+
+What attends to what, which no call can check as lengths are on the device:
+* `attention_decode` takes row b of q for request b.  The rows of a plan are packed, so they are those rows only where every request
+  adds one token; where some add none, index q by `plan.cu_seqlens[:-1]` first (and leave out what the idle ones get).
+* A prompt that is new as a whole (`cached` 0) attends to itself by `ops.attention_fwd` on the packed layout, with `plan.cu_seqlens`:
+  head_dim 128, neither window nor softcap, of whichever a model has one its prompts cannot be read in here.
+* Several new tokens behind a cached prefix (a prompt in pieces, drafted tokens) get positions and slots, but no operator attends
+  for them: `attention_fwd` would see the new rows alone, and give no error.
 
 As in `ops`, this layer allocates outputs and scratch and calls the C ABI on the current CUDA stream.
 """
@@ -124,7 +132,8 @@ def _scratch_of(q_shape, cache_shape, device: int) -> int:
 
 def attention_decode(q, k_cache, v_cache, block_table, seq_lens, opts: AttentionDecodeOpts | None = None, lse: bool = False,
                      out=None, scratch=None) -> AttentionDecodeOutputs:
-    """Attention of one new token per request (q [batch, heads, head_dim]) over its seq_lens keys in the paged cache."""
+    """Attention of one new token per request (q [batch, heads, head_dim], row b of request b) over its seq_lens keys in the paged
+    cache.  `scratch` (contiguous, of attention_decode_scratch_bytes) must overlap no other operand."""
     opts = opts or AttentionDecodeOpts()
     _require_current_device(q, k_cache, v_cache, block_table, seq_lens, out, scratch)
     tq, tk = tensor_bytes(q), tensor_bytes(k_cache)

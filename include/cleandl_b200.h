@@ -436,9 +436,12 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
  * k_cache and v_cache are bf16 [pages, page_size, kv_heads, head_dim] of any page size, the last dimension contiguous, base
  * and other strides 16-byte aligned (a permuted view of [pages, kv_heads, page_size, head_dim] is fine).  Key j of request b
  * lies in slot j % page_size of page block_table[b][j / page_size]; the slot number of a key is page * page_size + slot.
- * One step of a batch is cdl_b200_cache_plan, once; and per layer cdl_b200_cache_write and cdl_b200_attn_decode (for a prompt:
- * cdl_b200_attn_fwd_packed over the new rows); then cdl_b200_sample.  Nothing of it reads a length on the host, so a step can be
- * captured once and replayed. */
+ * One step of a batch is cdl_b200_cache_plan, once; and per layer cdl_b200_cache_write and cdl_b200_attn_decode; then
+ * cdl_b200_sample.  Nothing of it reads a length on the host, so a step can be captured once and replayed.
+ * cdl_b200_attn_decode takes row b of q for request b, so a step of it adds one token to every request.  A prompt that is new as a
+ * whole attends to itself by cdl_b200_attn_fwd_packed over the plan's rows (head_dim 128, no window, no softcap).  Several new tokens
+ * behind a cached prefix get positions and slots, but no call attends for them: cdl_b200_attn_fwd_packed would see the new rows
+ * alone. */
 
 /* Attention of one new token per request (the reference's attention with KvLayout::Paged and split-KV,
  * crates/cleandl/src/execgraph/ops/attention/mod.rs:83-91, 129-130):
@@ -452,7 +455,8 @@ int32_t cdl_b200_attn_bwd_packed_rope(const cdl_attn_desc* desc, const cdl_tenso
  * among its scores makes its results NaN.  What the cache holds behind a request's last key or ahead of its window may be
  * anything.  Statistics and sums are f32; probabilities are rounded to bf16 for their product with the values, as in
  * cdl_b200_attn_fwd.  Results do not depend on timing.  At most 4096 requests.
- * Scratch: 256-byte aligned, of the size that the call below gives; calls that may run at the same time have one each. */
+ * Scratch: 256-byte aligned, of the size that the call below gives, apart from all operands; calls that may run at the same time
+ * have one each. */
 typedef struct {
   float softmax_scale; /* <= 0 selects 1/sqrt(head_dim) */
   float softcap;       /* 0: none; scale and cap at most 2^126, scale / cap a normal f32 number */
