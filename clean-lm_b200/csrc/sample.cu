@@ -660,8 +660,9 @@ __device__ __noinline__ void draw_again(const Params& p, Shared& sh) {
   uint32_t above = 0;  // the entries above those that have them
   __syncthreads();     // (the list's length was read by all)
 #pragma unroll 1
-  for (int level = 0; level < 6; ++level) {
-    const int low_bit = level < 3 ? 32 : 0, width = level % 3 < 2 ? 11 : 10, shift = low_bit + (level % 3 == 0 ? 21 : level % 3 == 1 ? 10 : 0);
+  for (int level = 0; level < 5; ++level) {  // (not an index's last 10 bits: 1024 entries and fewer than BOUND_K above them fit the list)
+    static_assert(BOUND_K + 1024 <= CAP, "");
+    const int width = level == 2 ? 10 : 11, shift = level == 0 ? 53 : level == 1 ? 42 : level == 2 ? 32 : level == 3 ? 21 : 10;
     const uint32_t mask = (1u << width) - 1;
     for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
     if (tid == 0) sh.lo = -1, sh.count = 0;
